@@ -1,0 +1,571 @@
+// seqcache8.cu -- a cache of keys and values in 8 bits and attention over it (calm_b200_seq_cache8_store, calm_b200_seq_attend8 in include/calm_b200_seq.h).
+
+#include "seqops.cuh"
+#include "tc05.cuh"
+
+#include <limits.h>
+
+#include <algorithm>
+
+namespace seqops {
+namespace {
+
+typedef __nv_bfloat16 bf16;
+
+// what the kernels know of the cache and the batch
+struct C8 {
+	uint8_t *k, *v;
+	float *ks, *vs;
+	const int* table;
+	int pages, heads, page, dim, slots, table_pages;
+	const int *start, *count, *slot, *pos0;
+};
+constexpr int C8_LEAST = -64; // exponent of the smallest scale
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); } // -126 <= e <= 127
+__device__ __forceinline__ int pow2_of(float scale) { return max((int)(__float_as_uint(scale) >> 23 & 255) - 127, C8_LEAST); }
+// the least e >= C8_LEAST with amax <= 448 * 2^e: amax = m 2^x with 1/2 <= m < 1, 448 = 0.875 * 2^9
+__device__ __forceinline__ int scale_exponent(float amax) {
+	const uint32_t u = __float_as_uint(amax);
+	const int x = (int)(u >> 23) - 126;
+	return max(x - ((u & 0x7fffff) <= 0x600000 ? 9 : 8), C8_LEAST);
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+	const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+	return lo | hi << 16;
+}
+// two codes (the lower byte first) as fp16
+__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t codes) {
+	uint32_t r;
+	asm("{\n\t.reg .b16 h, x;\n\tmov.b32 {h, x}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes));
+	return r;
+}
+
+// ---------------------------------------------------------------- storing
+// A warp takes one page of a sequence's new rows, one head, keys or values: the largest finite value, the scale, the codes of earlier rows where the scale grew, the codes
+// of the new rows.  Pages are independent, so a prompt's run side by side.  Bound: memory for prompts (rows read once from DRAM, once more from L1),
+// latency for single tokens.
+constexpr int ST_WARPS = 4;
+struct StoreRows {
+	const void* p;
+	long long row, head;
+	int rows, vec; // vec: four elements at a time
+};
+template <typename T>
+__device__ __forceinline__ float4 store_load(const T* p, bool vec) {
+	if constexpr (sizeof(T) == 4) {
+		if (vec) return *reinterpret_cast<const float4*>(p);
+	} else {
+		if (vec) {
+			const uint2 w = *reinterpret_cast<const uint2*>(p);
+			const T* h = reinterpret_cast<const T*>(&w);
+			return make_float4(as_f32(h[0]), as_f32(h[1]), as_f32(h[2]), as_f32(h[3]));
+		}
+	}
+	return make_float4(as_f32(p[0]), as_f32(p[1]), as_f32(p[2]), as_f32(p[3]));
+}
+template <typename T>
+__global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const StoreRows rk, const StoreRows rv) {
+	const int b = blockIdx.z, unit = blockIdx.y * ST_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+	if (unit >= 2 * c.heads) return;
+	const bool isv = unit >= c.heads;
+	const int h = isv ? unit - c.heads : unit, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b];
+	const StoreRows& r = isv ? rv : rk;
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || (unsigned)slot >= (unsigned)c.slots || start < 0 || n > r.rows - start) return;
+	const int block = p0 / c.page + blockIdx.x;
+	const long long page0 = (long long)block * c.page;
+	if (block >= c.table_pages || page0 >= (long long)p0 + n) return;
+	const int id = c.table[(size_t)slot * c.table_pages + block];
+	if ((unsigned)id >= (unsigned)c.pages) return;
+	const int lo = (int)max((long long)p0 - page0, 0LL), hi = (int)min((long long)p0 + n - page0, (long long)c.page); // rows of the page
+	const T* src = (const T*)r.p + (start + (page0 + lo - p0)) * r.row + h * r.head;
+	uint8_t* const codes = (isv ? c.v : c.k) + ((size_t)id * c.heads + h) * c.page * c.dim;
+	float* const scale = (isv ? c.vs : c.ks) + (size_t)id * c.heads + h;
+	const int old = pow2_of(*scale);
+	auto mag = [](float x) { const float a = fabsf(x); return a < INFINITY ? a : 0.f; };
+	float amax = 0.f;
+	for (int d = 4 * lane; d < c.dim; d += 128)
+#pragma unroll 4
+		for (int i = 0; i < hi - lo; ++i) {
+			const float4 x = store_load(src + i * r.row + d, r.vec);
+			amax = fmaxf(amax, fmaxf(fmaxf(mag(x.x), mag(x.y)), fmaxf(mag(x.z), mag(x.w))));
+		}
+	int e = scale_exponent(warp_max(amax));
+	if (lo > 0) {
+		e = max(e, old);
+		if (e > old) { // the earlier rows' codes under the raised scale: exact but for what becomes subnormal
+			const float f = pow2f(max(old - e, -126));
+			for (int d = 4 * lane; d < c.dim; d += 128)
+				for (int i = 0; i < lo; ++i) {
+					uint32_t* const w = reinterpret_cast<uint32_t*>(codes + (size_t)i * c.dim + d);
+					const uint32_t x = *w, p = e4m3x2_to_f16(x), q = e4m3x2_to_f16(x >> 16);
+					const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&p)), v = __half22float2(*reinterpret_cast<const __half2*>(&q));
+					*w = e4m3x4(u.x * f, u.y * f, v.x * f, v.y * f);
+				}
+		}
+	}
+	const float inv = pow2f(-e);
+	auto put = [&](float x) { return x == x ? x * inv : 0.f; };
+	for (int d = 4 * lane; d < c.dim; d += 128)
+#pragma unroll 4
+		for (int i = 0; i < hi - lo; ++i) {
+			const float4 x = store_load(src + i * r.row + d, r.vec);
+			*reinterpret_cast<uint32_t*>(codes + (size_t)(lo + i) * c.dim + d) = e4m3x4(put(x.x), put(x.y), put(x.z), put(x.w));
+		}
+	__syncwarp();
+	if (lane == 0) *scale = pow2f(e);
+}
+
+// ---------------------------------------------------------------- attention
+// The rows of a CTA are 16 pairs (token, query head) of one sequence that read one key head, so a key is read once for all of them: row i of a sequence's tile is token
+// i / group, head i % group of the group.  Each warp walks its own chunks of 32 keys with a running maximum and sum of its own (no barrier between warps until the end),
+// fed by a ring of asynchronous copies; codes become fp16 in registers on their way into m16n8k16 products.  An e4m3 code is exact in fp16; scales do not enter the
+// products: a key's scale multiplies its scores, a value's scale s joins the exponent, w_j = exp2(z_j), z_j = log2(e) score_j + log2 s_j, whose running maximum bounds
+// the weights that are rounded to fp16; the denominator sums w_j / s_j.
+constexpr int AT_WARPS = 4, AT_KEYS = 32;
+constexpr float AT_LOG2E = 1.4426950408889634f;
+constexpr int AT_LIFT = 15; // the largest query of a row and the largest weight stand at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of them
+
+struct Attend {
+	const void* q;
+	long long q_row, q_head;
+	void* out;
+	long long o_row, o_head;
+	int rows, heads, group;
+	float scale, softcap;
+	int window, keep_first, chunk;
+	const float *sinks, *slopes, *gate;
+	long long gate_row, gate_head, gate_dim;
+	int shares;
+	float* part; // [rows][heads][shares][dim + 2]: sum, running maximum, denominator
+};
+
+template <int D>
+struct AtStage { // a warp's chunk
+	uint8_t k[AT_KEYS * D], v[AT_KEYS * D];
+	float ks[AT_KEYS], vs[AT_KEYS];
+	uint32_t seen; // keys that are there
+	uint32_t pad[3];
+};
+template <int D>
+__host__ __device__ constexpr int at_stages() { return D == 64 ? 4 : D == 128 ? 3 : 2; }
+template <int D, bool SPLIT>
+constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 16 * D * 2 + (size_t)AT_WARPS * at_stages<D>() * sizeof(AtStage<D>); }
+
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool there) { // zeros where there is nothing to read
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(void* dst, const void* src, bool there) {
+	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+	             : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
+	const __half2 h = __floats2half2_rn(x, y);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) { // what rounding to `hi` left
+	const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+	return pack_f16(x - h.x, y - h.y);
+}
+// 16-byte piece of a row of codes that is stored at place `piece` of row r: rows read together meet different banks
+template <int D>
+__device__ __forceinline__ int at_place(int r, int piece) { return piece ^ (D == 64 ? (r >> 1) & 3 : r & 7); }
+
+struct AtSpan { // the positions that a tile of rows sees, in order: [0, kept), then [lo, last]
+	int lo, kept, total;
+};
+__device__ __forceinline__ int at_low(const Attend& a, int pos) {
+	int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+	return a.chunk > 0 ? max(lo, pos / a.chunk * a.chunk) : lo;
+}
+
+template <int D, typename QT, typename OT>
+__global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const Attend a) {
+	constexpr bool SPLIT = sizeof(QT) == 4;
+	constexpr int ST = at_stages<D>(), KS = D / 16, NT = D / 8, PIECES = D / 16;
+	extern __shared__ __align__(128) unsigned char at_sm[];
+	uint4* const qf = reinterpret_cast<uint4*>(at_sm); // A fragments [KS][32], then the remainders'
+	AtStage<D>* const ring = reinterpret_cast<AtStage<D>*>(at_sm + (size_t)(SPLIT ? 2 : 1) * 16 * D * 2);
+	__shared__ float qscale[16], fold_m[AT_WARPS][16], fold_l[AT_WARPS][16];
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+	const int b = blockIdx.z, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = blockIdx.x;
+	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * 16 >= (long long)n * a.group) return;
+	const bool known = (unsigned)slot < (unsigned)c.slots;
+	const int row0 = tile * 16, rows = (int)min(16LL, (long long)n * a.group - row0);
+	const int first = p0 + row0 / a.group, last = p0 + (row0 + rows - 1) / a.group; // positions of the tile
+	const int lo = at_low(a, first), kept = min(a.keep_first, lo), total = known ? kept + last - lo + 1 : 0;
+	const int chunks = (total + AT_KEYS - 1) / AT_KEYS, each = (chunks + a.shares - 1) / a.shares;
+	const int begin = min(chunks, share * each), end = min(chunks, begin + each);
+	const int H = c.heads, dim = c.dim;
+
+	auto position = [&](int j) { return j < kept ? j : lo + (j - kept); };
+	auto page_of = [&](int chunk) { // the page of this lane's key, -1: none
+		const int j = chunk * AT_KEYS + lane;
+		if (chunk >= end || j >= total) return -1;
+		const int at = position(j) / c.page;
+		if (at >= c.table_pages) return -1;
+		const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
+		return (unsigned)id < (unsigned)c.pages ? id : -1;
+	};
+	AtStage<D>* const mine = ring + warp * ST;
+	int next = begin + warp, next_page = page_of(next), stage_in = 0; // the chunk to request, its page
+	auto request = [&]() {
+		if (next < end) {
+			AtStage<D>& s = mine[stage_in];
+			const int at = position(min(next * AT_KEYS + lane, total - 1)) % c.page, id = next_page;
+			const uint32_t seen = __ballot_sync(0xffffffffu, id >= 0);
+			const long long unit = (long long)max(id, 0) * H + kvh, off = (unit * c.page + at) * dim;
+			if (lane == 0) s.seen = seen;
+			cp4(s.ks + lane, c.ks + unit, id >= 0), cp4(s.vs + lane, c.vs + unit, id >= 0);
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
+				const int r = (i * 32 + lane) / PIECES, piece = (i * 32 + lane) % PIECES;
+				const long long o = __shfl_sync(0xffffffffu, off, r) + piece * 16;
+				const bool there = (seen >> r & 1) && piece * 16 < dim;
+				const int place = (r * PIECES + at_place<D>(r, piece)) * 16;
+				cp16(s.k + place, c.k + (there ? o : 0), there), cp16(s.v + place, c.v + (there ? o : 0), there);
+			}
+			stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
+			next += AT_WARPS, next_page = page_of(next);
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	};
+#pragma unroll
+	for (int i = 0; i < ST - 1; ++i) request();
+
+	// queries as A fragments: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a thread's codes of a key lie side by side)
+	for (int r = warp; r < 16; r += AT_WARPS) {
+		const QT* src = (const QT*)a.q + (long long)(start + (row0 + min(r, rows - 1)) / a.group) * a.q_row + (long long)(kvh * a.group + (row0 + min(r, rows - 1)) % a.group) * a.q_head;
+		float x[D / 32], top = 0.f;
+#pragma unroll
+		for (int i = 0; i < D / 32; ++i) {
+			const int d = i * 32 + lane;
+			x[i] = r < rows && d < dim ? as_f32(src[d]) : 0.f;
+			top = fmaxf(top, fabsf(x[i]));
+		}
+		top = warp_max(top);
+		const int e = (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT; // the row's largest comes to 2^AT_LIFT
+		const float down = pow2f(-e);
+#pragma unroll
+		for (int i = 0; i < D / 32; ++i) {
+			const int d = i * 32 + lane, dt = d / (D / 4), ds = d % (D / 4) / 4, de = d & 3;
+			const int at = ((ds * 32 + (r & 7) * 4 + dt) * 4 + (de >> 1) * 2 + (r >> 3)) * 2 + (de & 1);
+			const float y = x[i] * down;
+			const __half hi = __float2half_rn(y);
+			reinterpret_cast<__half*>(qf)[at] = hi;
+			if (SPLIT) reinterpret_cast<__half*>(qf + KS * 32)[at] = __float2half_rn(y - __half2float(hi));
+		}
+		if (lane == 0) qscale[r] = a.scale * pow2f(e);
+	}
+	__syncthreads();
+
+	float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // rows g and g + 8
+#pragma unroll
+	for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+	int rpos[2], rlo[2];
+	float rs[2], slope[2];
+#pragma unroll
+	for (int i = 0; i < 2; ++i) {
+		const int r = g + 8 * i;
+		rpos[i] = r < rows ? p0 + (row0 + r) / a.group : -1, rlo[i] = r < rows ? at_low(a, rpos[i]) : 0, rs[i] = qscale[r];
+		slope[i] = a.slopes && r < rows ? a.slopes[kvh * a.group + (row0 + r) % a.group] : 0.f;
+	}
+	const int wide = at_low(a, last); // from here on, and before `first`, every row sees every key
+
+	int stage = 0;
+	for (int chunk = begin + warp; chunk < end; chunk += AT_WARPS) {
+		asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+		__syncwarp();
+		request(); // into the stage that was used up last
+		const AtStage<D>& s = mine[stage];
+		stage = stage + 1 == ST ? 0 : stage + 1;
+		float z[4][4];
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.f;
+			const int r = 8 * j + g;
+			uint32_t w[KS];
+#pragma unroll
+			for (int i = 0; i < (KS + 3) / 4; ++i) {
+				const uint4 x = *reinterpret_cast<const uint4*>(s.k + (r * PIECES + at_place<D>(r, t * (PIECES / 4) + i)) * 16);
+				w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+			}
+#pragma unroll
+			for (int i = 0; i < KS; ++i) {
+				const uint32_t b0 = e4m3x2_to_f16(w[i]), b1 = e4m3x2_to_f16(w[i] >> 16);
+				mma_f16(z[j], qf[i * 32 + lane], b0, b1);
+				if (SPLIT) mma_f16(z[j], qf[(KS + i) * 32 + lane], b0, b1);
+			}
+		}
+		// scores with the value's scale in the exponent
+		const uint32_t seen = s.seen;
+		const int j0 = chunk * AT_KEYS;
+		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= first;
+		float over[8]; // 1 / value scale
+		float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			const float2 ks = *reinterpret_cast<const float2*>(s.ks + 8 * j + 2 * t), vs = *reinterpret_cast<const float2*>(s.vs + 8 * j + 2 * t);
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				const int i = e >> 1, key = 8 * j + 2 * t + (e & 1);
+				const float vscale = e & 1 ? vs.y : vs.x;
+				const int ve = (int)(__float_as_uint(vscale) >> 23) - 127;
+				if (i == 0) over[2 * j + (e & 1)] = pow2f(-max(ve, -126));
+				float x = z[j][e] * (rs[i] * (e & 1 ? ks.y : ks.x));
+				if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+				const int kp = position(j0 + key);
+				if (a.slopes) x -= slope[i] * (float)(rpos[i] - kp);
+				x = fmaf(x, AT_LOG2E, (float)ve);
+				if (!all && !((seen >> key & 1) && kp <= rpos[i] && (kp >= rlo[i] || kp < a.keep_first))) x = -INFINITY;
+				z[j][e] = x;
+				top[i] = fmaxf(top[i], x);
+			}
+		}
+		float f[2];
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+			top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+			const float mn = fmaxf(m[i], top[i] - AT_LIFT);
+			f[i] = m[i] == -INFINITY ? 0.f : exp2f(m[i] - mn);
+			m[i] = mn, l[i] *= f[i];
+		}
+		const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+		for (int j = 0; j < 4; ++j)
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				const float w = exp2f(z[j][e] - base[e >> 1]);
+				z[j][e] = w, l[e >> 1] = fmaf(w, over[2 * j + (e & 1)], l[e >> 1]);
+			}
+#pragma unroll
+		for (int i = 0; i < NT; ++i) acc[i][0] *= f[0], acc[i][1] *= f[0], acc[i][2] *= f[1], acc[i][3] *= f[1];
+		// values: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step kk is key 16 kk + 2t + {0, 1}, + 8; column g of product i is channel g * D / 8 + i
+#pragma unroll
+		for (int kk = 0; kk < 2; ++kk) {
+			uint4 ph, pl;
+			ph.x = pack_f16(z[2 * kk][0], z[2 * kk][1]), ph.y = pack_f16(z[2 * kk][2], z[2 * kk][3]);
+			ph.z = pack_f16(z[2 * kk + 1][0], z[2 * kk + 1][1]), ph.w = pack_f16(z[2 * kk + 1][2], z[2 * kk + 1][3]);
+			if (SPLIT) {
+				pl.x = pack_rest(z[2 * kk][0], z[2 * kk][1], ph.x), pl.y = pack_rest(z[2 * kk][2], z[2 * kk][3], ph.y);
+				pl.z = pack_rest(z[2 * kk + 1][0], z[2 * kk + 1][1], ph.z), pl.w = pack_rest(z[2 * kk + 1][2], z[2 * kk + 1][3], ph.w);
+			}
+			uint32_t x[4][D / 32]; // this thread's channels of its four keys
+#pragma unroll
+			for (int u = 0; u < 4; ++u) {
+				const int r = 16 * kk + 2 * t + (u & 1) + (u >> 1) * 8;
+				if constexpr (D == 64) {
+					const uint2 w = *reinterpret_cast<const uint2*>(s.v + (r * PIECES + at_place<D>(r, g >> 1)) * 16 + (g & 1) * 8);
+					x[u][0] = w.x, x[u][1] = w.y;
+				} else {
+#pragma unroll
+					for (int i = 0; i < D / 128; ++i) {
+						const uint4 w = *reinterpret_cast<const uint4*>(s.v + (r * PIECES + at_place<D>(r, g * (D / 128) + i)) * 16);
+						x[u][4 * i] = w.x, x[u][4 * i + 1] = w.y, x[u][4 * i + 2] = w.z, x[u][4 * i + 3] = w.w;
+					}
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+				for (int e = 0; e < 2; ++e) { // bytes 2e, 2e + 1 of the words
+					const uint32_t p = __byte_perm(x[0][i], x[1][i], e ? 0x7362 : 0x5140), q = __byte_perm(x[2][i], x[3][i], e ? 0x7362 : 0x5140);
+					const uint32_t b0 = e4m3x2_to_f16(p), b1 = e4m3x2_to_f16(q), b2 = e4m3x2_to_f16(p >> 16), b3 = e4m3x2_to_f16(q >> 16);
+					mma_f16(acc[4 * i + 2 * e], ph, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], ph, b2, b3);
+					if (SPLIT) mma_f16(acc[4 * i + 2 * e], pl, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], pl, b2, b3);
+				}
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < 2; ++i) l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1), l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+
+	// the warps' sums as one
+	asm volatile("cp.async.wait_group 0;" ::: "memory");
+	__syncthreads();
+	float* const sums = reinterpret_cast<float*>(ring); // [warps][16][D]
+#pragma unroll
+	for (int i = 0; i < NT; ++i)
+#pragma unroll
+		for (int e = 0; e < 4; ++e) sums[((warp * 16) + g + (e >> 1) * 8) * D + (2 * t + (e & 1)) * (D / 8) + i] = acc[i][e];
+	if (t == 0) fold_m[warp][g] = m[0], fold_m[warp][g + 8] = m[1], fold_l[warp][g] = l[0], fold_l[warp][g + 8] = l[1];
+	__syncthreads();
+	for (int r = warp; r < rows; r += AT_WARPS) {
+		float mx = fold_m[0][r], den = 0.f, wt[AT_WARPS];
+#pragma unroll
+		for (int w = 1; w < AT_WARPS; ++w) mx = fmaxf(mx, fold_m[w][r]);
+#pragma unroll
+		for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : exp2f(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
+		const int token = start + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
+		float* const part = a.shares > 1 ? a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2) : nullptr;
+		float norm = 0.f;
+		if (a.shares == 1) {
+			if (a.sinks) { // one more term of the denominator
+				const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : exp2f(mx - mn);
+				den = den * down + exp2f(sk - mn), norm = down;
+			} else norm = 1.f;
+			norm = den > 0.f ? norm / den : den == 0.f ? 0.f : den; // (a NaN stays one)
+		} else if (lane == 0) part[dim] = mx, part[dim + 1] = den;
+		for (int d = lane; d < dim; d += 32) {
+			float v = 0.f;
+#pragma unroll
+			for (int w = 0; w < AT_WARPS; ++w) v = fmaf(wt[w], sums[(w * 16 + r) * D + d], v);
+			if (a.shares > 1) part[d] = v;
+			else {
+				v *= norm;
+				if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
+				((OT*)a.out)[token * a.o_row + head * a.o_head + d] = from_f32<OT>(v);
+			}
+		}
+	}
+}
+
+// folds the shares of one (token, head), in share order
+template <typename OT>
+__global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
+	pdl_wait_prev();
+	const int b = blockIdx.z, head = blockIdx.y, n = c.count[b], start = c.start[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	if (n < 1 || c.pos0[b] < 0 || c.pos0[b] > INT_MAX - n || start < 0 || n > a.rows - start) return;
+	for (int i = blockIdx.x * 4 + warp; i < n; i += gridDim.x * 4) {
+		const int token = start + i;
+		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * (c.dim + 2);
+		float mx = -INFINITY, den = 0.f;
+		for (int s = 0; s < a.shares; ++s) mx = fmaxf(mx, p[(size_t)s * (c.dim + 2) + c.dim]);
+		const float sk = a.sinks ? a.sinks[head] * AT_LOG2E : -INFINITY, mn = fmaxf(mx, sk);
+		for (int s = 0; s < a.shares; ++s) {
+			const float* q = p + (size_t)s * (c.dim + 2) + c.dim;
+			den = fmaf(q[0] == -INFINITY ? 0.f : exp2f(q[0] - mn), q[1], den);
+		}
+		if (a.sinks) den += exp2f(sk - mn);
+		const float norm = den > 0.f ? 1.f / den : den;
+		for (int d = lane; d < c.dim; d += 32) {
+			float v = 0.f;
+			for (int s = 0; s < a.shares; ++s) {
+				const float* q = p + (size_t)s * (c.dim + 2);
+				v = fmaf(q[c.dim] == -INFINITY ? 0.f : exp2f(q[c.dim] - mn), q[d], v);
+			}
+			v *= norm;
+			if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
+			((OT*)a.out)[token * a.o_row + head * a.o_head + d] = from_f32<OT>(v);
+		}
+	}
+}
+
+int check_cache(const char* what, const SeqCache8* q, const SeqPortions* p) {
+	if (!q || !p) return refuse("%s: no cache or no batch", what);
+	if (q->pages < 0 || q->heads < 1 || q->page < 1 || q->slots < 0 || q->table_pages < 0) return refuse("%s: a cache of %d pages, %d heads, %d tokens a page", what, q->pages, q->heads, q->page);
+	if (q->heads > 4096 || q->page > 65536) return refuse("%s: at most 4096 heads and 65536 tokens a page", what);
+	if (q->dim < 16 || q->dim > 256 || q->dim % 16) return refuse("%s: rows of %d channels: a multiple of 16 up to 256 is served", what, q->dim);
+	if (p->n < 0 || p->longest < 0 || p->n > 65535) return refuse("%s: %d sequences (at most 65535), longest %d", what, p->n, p->longest);
+	if (p->n && (!p->start || !p->count || !p->slot || !p->pos0)) return refuse("%s: the batch's description is missing", what);
+	if (q->pages && (!q->k || !q->v || !q->k_scale || !q->v_scale)) return refuse("%s: the cache has no memory", what);
+	if (q->slots > 0 && q->table_pages > 0 && !q->table) return refuse("%s: the page table is missing", what);
+	if (((uintptr_t)q->k | (uintptr_t)q->v) % 16) return refuse("%s: codes are not aligned to 16 bytes", what);
+	if (((uintptr_t)q->k_scale | (uintptr_t)q->v_scale) % 4) return refuse("%s: scales are not aligned to 4 bytes", what);
+	return 0;
+}
+int check_rows(const char* what, const char* name, const SeqRows& r) {
+	if (!type_ok(r.type)) return refuse("%s: %s has type %d", what, name, r.type);
+	if (r.rows < 0 || (r.rows && !r.p)) return refuse("%s: %s is missing", what, name);
+	if ((uintptr_t)r.p % type_size(r.type)) return refuse("%s: %s is not aligned to its type", what, name);
+	return 0;
+}
+C8 describe(const SeqCache8& q, const SeqPortions& p) {
+	return C8{(uint8_t*)q.k, (uint8_t*)q.v, q.k_scale, q.v_scale, q.table, q.pages, q.heads, q.page, q.dim, q.slots, q.table_pages, p.start, p.count, p.slot, p.pos0};
+}
+StoreRows store_rows(const SeqRows& r) {
+	const int bytes = 4 * type_size(r.type);
+	return StoreRows{r.p, r.row_stride, r.head_stride, r.rows, (uintptr_t)r.p % bytes == 0 && r.row_stride % 4 == 0 && r.head_stride % 4 == 0};
+}
+
+// CTAs that share the keys of a tile of rows: as many as the GPU has room for, four chunks for each at least
+int attend_shares(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
+	const int group = a.heads / c.heads;
+	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, 16) * c.heads, room = 148 * 2;
+	int keys = std::max(a.most_keys, 1);
+	if (a.window > 0) keys = (int)std::min<long long>(keys, (long long)a.window + a.keep_first + (p.longest > 1 ? 16 / group : 0));
+	if (a.chunk > 0) keys = (int)std::min<long long>(keys, (long long)a.chunk + a.keep_first);
+	return ctas >= room || ctas < 1 ? 1 : (int)std::max(1LL, std::min({room / ctas, (long long)cdiv(cdiv(keys, AT_KEYS), AT_WARPS), 64LL}));
+}
+size_t attend_bytes(const SeqCache8& c, const SeqAttend8& a, int shares) { return shares > 1 ? (size_t)a.q.rows * a.heads * shares * (c.dim + 2) * sizeof(float) : 0; }
+
+int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) {
+	if (const int rc = check_cache("attend8", c, p)) return rc;
+	if (!a) return refuse("attend8: no arguments");
+	if (const int rc = check_rows("attend8", "q", a->q)) return rc;
+	if (const int rc = check_rows("attend8", "out", a->out)) return rc;
+	if (a->heads < 1 || a->heads % c->heads) return refuse("attend8: %d query heads over %d key heads", a->heads, c->heads);
+	if (a->heads > 65535) return refuse("attend8: at most 65535 query heads");
+	if (a->out.type != a->q.type && !(a->q.type == SEQ_F32 && a->out.type == SEQ_BF16)) return refuse("attend8: out has type %d, q %d", a->out.type, a->q.type);
+	if (a->out.rows < a->q.rows) return refuse("attend8: out has %d rows, q %d", a->out.rows, a->q.rows);
+	if (!(a->scale == a->scale) || a->window < 0 || a->keep_first < 0 || a->chunk < 0 || !(a->softcap >= 0.f)) return refuse("attend8: scale, window, keep_first, chunk or softcap out of range");
+	return 0;
+}
+
+template <int D, typename QT, typename OT>
+cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
+	const size_t smem = at_smem<D, sizeof(QT) == 4>();
+	cudaError_t e = cudaFuncSetAttribute(k_c8_attend<D, QT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_attend<D, QT, OT>, grid, dim3(32 * AT_WARPS), smem, c, a);
+	return e;
+}
+template <typename QT, typename OT>
+cudaError_t attend_typed(const C8& c, const Attend& a, dim3 grid, dim3 fold, cudaStream_t st) {
+	cudaError_t e = c.dim <= 64 ? attend_launch<64, QT, OT>(c, a, grid, st) : c.dim <= 128 ? attend_launch<128, QT, OT>(c, a, grid, st) : attend_launch<256, QT, OT>(c, a, grid, st);
+	if (e == cudaSuccess && a.shares > 1) e = launch(st, true, 1, k_c8_fold<OT>, fold, dim3(128), 0, c, a);
+	return e;
+}
+} // namespace
+} // namespace seqops
+
+extern "C" int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqRows* k, const struct SeqRows* v, void* stream) {
+	using namespace seqops;
+	if (const int rc = check_cache("store8", cache, batch)) return rc;
+	if (!k || !v) return refuse("store8: no rows");
+	if (const int rc = check_rows("store8", "k", *k)) return rc;
+	if (const int rc = check_rows("store8", "v", *v)) return rc;
+	if (k->type != v->type) return refuse("store8: keys have type %d, values %d", k->type, v->type);
+	if (batch->n == 0 || batch->longest == 0) return 0;
+	const C8 c = describe(*cache, *batch);
+	const dim3 grid(cdiv((long long)batch->longest + cache->page - 1, cache->page), cdiv(2 * cache->heads, ST_WARPS), batch->n);
+	const StoreRows rk = store_rows(*k), rv = store_rows(*v);
+	auto kernel = k->type == SEQ_F32 ? k_c8_store<float> : k->type == SEQ_BF16 ? k_c8_store<bf16> : k_c8_store<__half>;
+	const cudaError_t e = launch((cudaStream_t)stream, false, 1, kernel, grid, dim3(32 * ST_WARPS), 0, c, rk, rv);
+	return e == cudaSuccess ? 0 : failed("store8", e);
+}
+
+extern "C" size_t calm_b200_seq_attend8_workspace(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args) {
+	using namespace seqops;
+	if (check_attend(cache, batch, args)) return 0;
+	return attend_bytes(*cache, *args, attend_shares(*cache, *batch, *args));
+}
+
+extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* q, void* stream) {
+	using namespace seqops;
+	if (const int rc = check_attend(cache, batch, q)) return rc;
+	if (batch->n == 0 || batch->longest == 0) return 0;
+	const int shares = attend_shares(*cache, *batch, *q);
+	const size_t need = attend_bytes(*cache, *q, shares);
+	if (need && (!q->workspace || (uintptr_t)q->workspace % 16 || q->workspace_bytes < need)) return refuse("attend8: the workspace has %zu bytes (16-byte aligned), %zu are needed", q->workspace ? q->workspace_bytes : (size_t)0, need);
+	const C8 c = describe(*cache, *batch);
+	Attend a;
+	a.q = q->q.p, a.q_row = q->q.row_stride, a.q_head = q->q.head_stride, a.out = q->out.p, a.o_row = q->out.row_stride, a.o_head = q->out.head_stride;
+	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap;
+	a.window = q->window, a.keep_first = q->keep_first, a.chunk = q->chunk, a.sinks = q->sinks, a.slopes = q->slopes;
+	a.gate = q->gate, a.gate_row = q->gate_row, a.gate_head = q->gate_head, a.gate_dim = q->gate_dim;
+	a.shares = shares, a.part = (float*)q->workspace;
+	const dim3 grid(cdiv((long long)batch->longest * a.group, 16), cache->heads * shares, batch->n), fold(std::min(cdiv(batch->longest, 4), 65535), q->heads, batch->n);
+	if (grid.y > 65535) return refuse("attend8: too many key heads");
+	const cudaStream_t st = (cudaStream_t)stream;
+	cudaError_t e;
+	if (q->q.type == SEQ_BF16) e = attend_typed<bf16, bf16>(c, a, grid, fold, st);
+	else if (q->q.type == SEQ_F16) e = attend_typed<__half, __half>(c, a, grid, fold, st);
+	else if (q->out.type == SEQ_BF16) e = attend_typed<float, bf16>(c, a, grid, fold, st);
+	else e = attend_typed<float, float>(c, a, grid, fold, st);
+	return e == cudaSuccess ? 0 : failed("attend8", e);
+}

@@ -16,6 +16,7 @@
 
 #include "seqkernels.cuh"
 #include "seqgemm_tc.cuh"
+#include "seqops.cuh"
 
 namespace {
 
@@ -1531,7 +1532,7 @@ extern "C" void* calm_b200_seq_upload(const void* host, size_t size) {
 	return p;
 }
 extern "C" void calm_b200_seq_free(void* p) { cudaFree(p); }
-extern "C" uint64_t calm_b200_seq_launch_count(void) { return g_seq_launches; }
+extern "C" uint64_t calm_b200_seq_launch_count(void) { return g_seq_launches + seqops::launches(); }
 extern "C" uint64_t calm_b200_seq_route_count(int route) { return route >= SEQ_ROUTE_PAIRS ? (route < SEQ_ROUTE_PAIRS + TG_EPILOGUES ? g_tg.pair_launches[route - SEQ_ROUTE_PAIRS] : 0) : route >= 0 ? g_seq_routes[route] : 0; }
 extern "C" int calm_b200_seq_skinny_warps(int m, int k, int groups, int rows, int sms) { return skinny_warps(m, k, groups, rows, sms); }
 extern "C" int calm_b200_seq_delta_blocks_pay(int longest, int few, int heads, int vdim, int sms) { return delta_blocks_pay(longest, few, heads, vdim, sms); }

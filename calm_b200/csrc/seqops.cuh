@@ -1,0 +1,64 @@
+// seqops.cuh -- what the operators on callers' device memory (seqbeam.cu, seqcopy.cu, seqcache8.cu; entry points in include/calm_b200_seq.h) share:
+// refusals that leave a message instead of ending the process, launches that report their error, element types.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/calm_b200_seq.h"
+#include "common.cuh"
+
+namespace seqops {
+
+// -3 with a message for calm_b200_seq_error() / -4 for a CUDA error; both leave the process and the context as they were
+int refuse(const char* fmt, ...);
+int failed(const char* what, cudaError_t e);
+
+int sm_count(); // of the current device
+void count_launch();
+uint64_t launches(); // since the library was loaded
+
+inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// `after`: programmatic dependent launch behind the previous kernel of the stream, which the kernel waits for with pdl_wait_prev()
+template <typename... KArgs, typename... Args>
+cudaError_t launch(cudaStream_t st, bool after, int cluster_x, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+	cudaLaunchAttribute at[2];
+	int n = 0;
+	if (after) at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[n++].val.programmaticStreamSerializationAllowed = 1;
+	if (cluster_x > 1) {
+		at[n].id = cudaLaunchAttributeClusterDimension;
+		at[n].val.clusterDim.x = cluster_x, at[n].val.clusterDim.y = 1, at[n++].val.clusterDim.z = 1;
+	}
+	cfg.attrs = at, cfg.numAttrs = n;
+	count_launch();
+	return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+inline int type_size(int t) { return t == SEQ_F32 ? 4 : 2; }
+inline bool type_ok(int t) { return t == SEQ_F32 || t == SEQ_BF16 || t == SEQ_F16; }
+
+__device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+// the elements of 16 bytes as floats
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& w, float (&v)[16 / sizeof(T)]) {
+	const T* p = reinterpret_cast<const T*>(&w);
+#pragma unroll
+	for (int i = 0; i < (int)(16 / sizeof(T)); ++i) v[i] = as_f32(p[i]);
+}
+
+} // namespace seqops

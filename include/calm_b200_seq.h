@@ -320,6 +320,103 @@ float calm_b200_seq_timer_stop(void* handle);
 void calm_b200_seq_set_perf(void* handle, int on);
 int calm_b200_seq_perf_stats(void* handle, int kind, char* name, int name_cap, double* ms_total, double* bytes_total, double* flops_total, long* launches);
 
+/* ---- operators on the caller's device memory -----------------------------------------------------------------------------------
+ * What continuing one text in several sequences needs, for callers with buffers of their own; the runtime above runs on the same kernels.
+ * Every call launches on `stream` (a cudaStream_t of the current device, NULL: the default one), returns before the work is done, allocates nothing and can
+ * be captured into a CUDA graph.  Returns 0; -3 when an argument is refused, -4 when CUDA reports an error (nothing has been launched then that the call's
+ * own kernels have not finished with): calm_b200_seq_error() says why, per host thread.  Calls from several host threads do not disturb each other as long as
+ * their outputs and workspaces are their own. */
+const char* calm_b200_seq_error(void);
+
+enum SeqType { SEQ_F32 = 0, SEQ_BF16 = 1, SEQ_F16 = 2 };
+
+/* The n best continuations of each of `groups` groups of `beams` beams: candidate (b, t) of group g scores scores[g][b] + x_t - log sum_u exp x_u, x being
+ * row (g, b) of the logits; the highest n over all beams and tokens, in order, ties to the lower beam, then to the lower token.  Tokens of one beam are compared by
+ * their logits, beams in 64 bits (a row's log-sum comes from fp32 exponentials: candidates of different beams that are nearer than about 1e-7 may come in either order).  A beam whose score is -inf (or NaN) is not there: its logits are not read.  A NaN logit counts as -inf; -inf is never chosen; where a
+ * row holds +inf, those tokens share its probability.  Places for which no candidate is left get token -1, parent -1, score -inf. */
+struct SeqBeam {
+	const void* logits;  /* [groups][beams][vocab], the tokens of a row side by side; any alignment that the type allows */
+	int type;            /* enum SeqType */
+	long long group_stride, row_stride; /* in elements */
+	const float* scores; /* [groups][beams] */
+	int groups, beams, vocab, n; /* 1 <= beams <= 64, 1 <= n <= 64, beams * vocab < 2^31 */
+	int* tokens;         /* [groups][n] */
+	int* parents;        /* [groups][n]: beam of the group */
+	float* best;         /* [groups][n] */
+	void* workspace;     /* calm_b200_seq_beam_workspace bytes, 16-byte aligned; undefined between calls, not to be shared by calls that may overlap */
+	size_t workspace_bytes;
+};
+size_t calm_b200_seq_beam_workspace(int groups, int beams, int vocab, int n);
+int calm_b200_seq_beam_select(const struct SeqBeam* args, void* stream);
+
+/* Copies of whole or partly filled units inside (or between) pools, any number of pools in one go: pages of position-indexed caches, slots of recurrent
+ * state.  Lists are host memory, read before the call returns.  A destination is named once and is no source of the same pool: what order copies run in
+ * never shows.  Pools of one kind share the lists of that kind. */
+struct SeqUnits {
+	const void* src;
+	void* dst;                        /* may be src */
+	long long unit_bytes;             /* bytes from one unit to the next */
+	long long row_bytes;              /* kind 0: a page's rows, page_rows[i] of which are copied; 0: always the whole unit */
+	int src_units, dst_units;         /* units in each pool: what is named beyond is refused */
+	int kind;                         /* 0: page lists, 1: slot lists */
+};
+int calm_b200_seq_copy_units(int n_pools, const struct SeqUnits* pools, int n_pages, const int* page_from, const int* page_to, const int* page_rows /* or NULL: whole pages */,
+                             int n_slots, const int* slot_from, const int* slot_to, void* stream);
+
+/* A cache of keys and values in 8 bits.  Codes are e4m3 (no infinities), [pages][heads][page][dim]; a scale, a power of two, serves the `page` tokens of a page and
+ * head, [pages][heads]; value = code * scale.  Sequence slot s finds its position p in page table[s][p / page], row p % page.
+ * Powers of two: an e4m3 code has its own exponent, so a finer scale buys nothing, and a scale that has to grow when later tokens join a page moves the codes
+ * of the earlier ones without rounding them again (but for what falls under the codes' smallest steps, 2^-15 of the page's largest value). */
+struct SeqCache8 {
+	void* k;
+	float* k_scale;
+	void* v;
+	float* v_scale;
+	int pages, heads, page, dim; /* dim a multiple of 16, at most 256; codes 16-byte aligned */
+	const int* table;            /* device [slots][table_pages] */
+	int slots, table_pages;
+};
+/* A packed batch: sequence b brings count[b] tokens, rows start[b] .. of the arrays, at positions pos0[b] .. of slot slot[b] (device arrays, so that a captured call
+ * follows them).  longest: at least the largest count.  Rows that belong to no sequence are left alone; so is what a slot, position or page number
+ * outside the cache names: it is neither read nor written, and attention does not see it. */
+struct SeqPortions {
+	int n;
+	const int *start, *count, *slot, *pos0;
+	int longest;
+};
+struct SeqRows { /* [rows][heads][dim], dim side by side */
+	void* p;
+	int type;
+	long long row_stride, head_stride; /* in elements */
+	int rows;
+};
+/* New rows of keys and values into the cache.  A page's scale becomes the least 2^e, e >= -64, with max|x| <= 448 * 2^e over the rows stored, or stays where it
+ * was higher; then the codes of the page's earlier rows are rounded to the raised scale.  A page whose row 0 is stored starts anew.  Rounding to nearest, ties to even; an
+ * infinity is stored as 448 * scale (and does not count for the scale), a NaN as zero.  Two sequences of a call must not store into one page. */
+int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqRows* k, const struct SeqRows* v, void* stream);
+
+/* Attention of the batch's tokens over the cache, which holds them already: token at position p of its sequence sees positions lo .. p and the first keep_first
+ * ones, lo = max(p - window + 1 with window > 0, floor(p / chunk) * chunk with chunk > 0, 0); query head h reads key head h / group.
+ *   s_j = softcap(scale q . k_j) - slopes[h] (p - j);  out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h])), times sigmoid(gate) where given.
+ * Scores, softmax and sums are fp32; queries and softmax weights enter the tensor cores as fp16 (queries scaled by a power of two a row), as a pair of fp16 value and
+ * remainder where the queries are fp32; codes enter exactly.  A token that sees nothing gets zeros. */
+struct SeqAttend8 {
+	struct SeqRows q, out;   /* out.type: as q's, or SEQ_BF16 where the queries are fp32 */
+	int heads;               /* query heads, a multiple of cache.heads */
+	float scale;
+	int window, keep_first, chunk;
+	float softcap;           /* > 0: s = softcap tanh(s / softcap) after the scale */
+	const float* sinks;      /* [heads] or NULL */
+	const float* slopes;     /* [heads] or NULL */
+	const float* gate;       /* or NULL: gate[row * gate_row + h * gate_head + d * gate_dim] */
+	long long gate_row, gate_head, gate_dim;
+	int most_keys;           /* at least the keys that any token sees (what the split of the work is planned for; more are still seen) */
+	void* workspace;         /* calm_b200_seq_attend8_workspace bytes, 16-byte aligned */
+	size_t workspace_bytes;
+};
+size_t calm_b200_seq_attend8_workspace(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args);
+int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,154 @@
+"""What the operators on callers' memory refuse, and how they plan their workspaces: no GPU needed, nothing is launched."""
+import ctypes as C
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import seqops_plain as plain  # noqa: E402
+
+from calm_b200 import seqops  # noqa: E402
+
+L = None
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    global L
+    L = seqops._load()
+
+
+def says(rc, *words):
+    text = L.calm_b200_seq_error().decode()
+    assert rc == -3 and all(w in text for w in words), (rc, text)
+
+
+def beam(**over):
+    f = dict(logits=4096, type=0, group_stride=40, row_stride=10, scores=4096, groups=2, beams=4, vocab=10, n=3, tokens=4096, parents=4096, best=4096, workspace=4096, workspace_bytes=1 << 20)
+    f.update(over)
+    return L.calm_b200_seq_beam_select(C.byref(seqops._Beam(*[f[n] for n, _ in seqops._Beam._fields_])), None)
+
+
+def test_beam_refusals():
+    says(L.calm_b200_seq_beam_select(None, None), "no arguments")
+    for over, word in ((dict(beams=0), "beams"), (dict(beams=65), "64"), (dict(groups=-1), "groups"), (dict(vocab=0), "tokens"), (dict(vocab=1 << 30), "2^31"), (dict(n=0), "n = 0"),
+                       (dict(n=65), "n = 65"), (dict(groups=20000), "65535"), (dict(type=3), "type"), (dict(logits=None), "pointer"), (dict(scores=None), "pointer"), (dict(tokens=None), "pointer"),
+                       (dict(parents=None), "pointer"), (dict(best=None), "pointer"), (dict(workspace=None), "pointer"), (dict(logits=4098), "aligned"), (dict(workspace=4104), "aligned"),
+                       (dict(workspace_bytes=8), "are needed"), (dict(type=1, logits=4097), "aligned")):
+        says(beam(**over), "beam", word)
+    assert beam(groups=0) == 0
+    assert L.calm_b200_seq_beam_workspace(2, 65, 10, 3) == 0
+    for G, K, V, n in ((1, 1, 1, 1), (32, 8, 128256, 16), (1, 64, 1 << 20, 64), (65535, 1, 3, 1)):
+        assert 0 < L.calm_b200_seq_beam_workspace(G, K, V, n) < 1 << 28
+
+
+def copy(pools, pages=((), ()), rows=None, slots=((), ())):
+    u = (seqops._Units * max(1, len(pools)))(*[seqops._Units(*p) for p in pools])
+    a = [np.ascontiguousarray(x, np.int32) for x in (*pages, *slots)]
+    r = None if rows is None else np.ascontiguousarray(rows, np.int32)
+    return L.calm_b200_seq_copy_units(len(pools), u, len(a[0]), a[0].ctypes.data, a[1].ctypes.data, None if r is None else r.ctypes.data, len(a[2]), a[2].ctypes.data, a[3].ctypes.data, None)
+
+
+def test_copy_refusals():
+    page = (4096, 4096, 64, 8, 10, 10, 0)
+    slot = (1 << 20, 1 << 20, 64, 0, 5, 5, 1)
+    for args, word in (((([page]), ([0], [10])), "page 10"), ((([page]), ([-1], [0])), "page -1"), ((([page]), ([0, 1], [3, 3])), "twice"), ((([page]), ([0, 1], [1, 2])), "read and written"),
+                       ((([page]), ([4], [4])), "read and written"), (([(4096, 4096, 64, 65, 10, 10, 0)], ([0], [1])), "rows"), (([(None, None, 64, 8, 10, 10, 0)], ([0], [1])), "memory"),
+                       (([(4096, 4096 + 64, 64, 8, 10, 10, 0)], ([0], [1])), "overlap"), (([(4096, 4096, 64, 8, 10, 10, 2)], ([0], [1])), "kind"), (([(4096, 4096, -1, 0, 10, 10, 0)], ([0], [1])), "negative"),
+                       (([(4096, 4096, 1 << 40, 0, 10, 10, 0)], ([0], [1])), "256 GB"), (([page, (4096, 1 << 22, 64, 8, 10, 3, 0)], ([0], [3])), "pool of 3")):
+        says(copy(*args), "copy", word)
+    says(copy([page], ([0], [1]), rows=[-1]), "rows")
+    says(copy([slot], slots=([0], [5])), "slot 5")
+    assert copy([page, slot]) == 0 and copy([]) == 0  # nothing to copy
+
+
+def cache8(**over):
+    f = dict(k=4096, k_scale=4096, v=4096, v_scale=4096, pages=10, heads=2, page=16, dim=64, table=4096, slots=3, table_pages=4)
+    f.update(over)
+    return seqops._Cache8(*[f[n] for n, _ in seqops._Cache8._fields_])
+
+
+def portions(**over):
+    f = dict(n=2, start=4096, count=4096, slot=4096, pos0=4096, longest=5)
+    f.update(over)
+    return seqops._Portions(*[f[n] for n, _ in seqops._Portions._fields_])
+
+
+def rows(**over):
+    f = dict(p=4096, type=0, row_stride=128, head_stride=64, rows=10)
+    f.update(over)
+    return seqops._Rows(*[f[n] for n, _ in seqops._Rows._fields_])
+
+
+def attend(c=None, p=None, **over):
+    f = dict(q=rows(), out=rows(), heads=4, scale=1.0, window=0, keep_first=0, chunk=0, softcap=0.0, sinks=None, slopes=None, gate=None, gate_row=0, gate_head=0, gate_dim=0, most_keys=100,
+             workspace=None, workspace_bytes=0)
+    f.update(over)
+    a = seqops._Attend8(*[f[n] for n, _ in seqops._Attend8._fields_])
+    return C.byref(c or cache8()), C.byref(p or portions()), C.byref(a)
+
+
+BAD_CACHES = ((dict(dim=0), "channels"), (dict(dim=24), "channels"), (dict(dim=272), "channels"), (dict(heads=0), "heads"), (dict(heads=5000), "heads"), (dict(page=0), "page"), (dict(page=1 << 20), "page"),
+              (dict(pages=-1), "pages"), (dict(k=None), "memory"), (dict(v_scale=None), "memory"), (dict(table=None), "table"), (dict(k=4104), "aligned"), (dict(k_scale=4097), "aligned"))
+BAD_BATCHES = ((dict(n=-1), "sequences"), (dict(n=70000), "sequences"), (dict(longest=-1), "longest"), (dict(start=None), "description"), (dict(pos0=None), "description"))
+
+
+def test_store_refusals():
+    def store(c=None, p=None, k=None, v=None):
+        return L.calm_b200_seq_cache8_store(C.byref(c or cache8()), C.byref(p or portions()), C.byref(k or rows()), C.byref(v or rows()), None)
+
+    for over, word in BAD_CACHES:
+        says(store(c=cache8(**over)), "store8", word)
+    for over, word in BAD_BATCHES:
+        says(store(p=portions(**over)), "store8", word)
+    for over, word in ((dict(type=7), "type"), (dict(p=None), "missing"), (dict(rows=-2), "missing"), (dict(p=4098), "aligned"), (dict(type=1), "values")):
+        says(store(k=rows(**over)), "store8", word)
+    says(L.calm_b200_seq_cache8_store(None, None, None, None, None), "no cache")
+    assert store(p=portions(n=0, start=None)) == 0 and store(p=portions(longest=0)) == 0
+
+
+def test_attend_refusals_and_workspace():
+    for over, word in BAD_CACHES:
+        says(L.calm_b200_seq_attend8(*attend(c=cache8(**over)), None), "attend8", word)
+    for over, word in BAD_BATCHES:
+        says(L.calm_b200_seq_attend8(*attend(p=portions(**over)), None), "attend8", word)
+    for over, word in ((dict(heads=3), "query heads"), (dict(heads=0), "query heads"), (dict(q=rows(type=4)), "type"), (dict(out=rows(type=2)), "type"), (dict(q=rows(type=1), out=rows(type=0)), "type"),
+                       (dict(out=rows(rows=9)), "rows"), (dict(window=-1), "range"), (dict(keep_first=-1), "range"), (dict(chunk=-3), "range"), (dict(softcap=-1.0), "range"),
+                       (dict(softcap=float("nan")), "range"), (dict(scale=float("nan")), "range"), (dict(q=rows(p=None)), "missing")):
+        says(L.calm_b200_seq_attend8(*attend(**over), None), "attend8", word)
+    one = portions(n=1, longest=1)
+    need = L.calm_b200_seq_attend8_workspace(*attend(p=one, most_keys=100000))
+    assert need > 0  # one sequence: its keys are divided
+    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000), None), "workspace")
+    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000, workspace=4096, workspace_bytes=need - 1), None), "workspace")
+    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000, workspace=4100, workspace_bytes=need), None), "workspace")
+    assert L.calm_b200_seq_attend8_workspace(*attend(p=portions(n=4000, longest=1))) == 0
+    assert L.calm_b200_seq_attend8(*attend(p=portions(n=0, start=None)), None) == 0
+
+
+def test_python_refusals():
+    x, s = torch.zeros(1, 2, 8), torch.zeros(1, 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        seqops.beam_select(x, s, 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        seqops.UnitPool([torch.zeros(2, 2, 2)])
+    with pytest.raises(ValueError, match="CUDA"):
+        seqops.Cache8(*[torch.zeros(1)] * 4)
+    for args in (([0, 0], [1, 1], [0, 0]), ([0], [1, 1], [0]), ([0], [-1], [0]), ([-1], [1], [0]), ([0], [1], [-1]), ([0], [1], [2 ** 31 - 1])):
+        with pytest.raises(ValueError):
+            seqops.Batch(*args, device="cpu")
+    seqops.UnitPool().copy()
+
+
+def test_the_plain_rounding_is_torchs():
+    """The statement that the GPU tests compare with, against the conversions of another implementation."""
+    rng = np.random.default_rng(0)
+    x = np.concatenate([rng.normal(0, 40, 20000), rng.normal(0, 0.02, 20000), plain.VALUES[:127] * 1.03125, plain.VALUES[:126] + np.diff(plain.VALUES[:127]) / 2]).clip(-448, 448).astype(np.float32)
+    t = torch.tensor(x).to(torch.float8_e4m3fn)
+    assert np.array_equal(plain.round_e4m3(x), t.float().double().numpy()) and np.array_equal(plain.VALUES[t.view(torch.uint8).numpy()], t.float().double().numpy())
+    for a in (0.0, 1.0, 448.0, 448.1, 449.0, 3e38, 1e-30, 2.0 ** -60):
+        e = plain.exponent(a)
+        assert a <= 448 * 2.0 ** e and (e == -64 or a > 448 * 2.0 ** (e - 1))
