@@ -2281,6 +2281,7 @@ struct QkArgs {
 	int pairs2 = 0;     // 1: rotation turns channels 2i and 2i + 1 together, 0: i and i + rot_dims/2
 	bf16* qb = nullptr; // given: the queries leave in the activation type for the product path instead, as they are (qsplit 0) or as
 	int qsplit = 0;     //        [hi | hi | lo] rows of `dim` columns each per head (see k_seq_split_q)
+	int by_token = 0;   // 1: kc and vc are the step's rows in the order of its tokens, to be stored in an 8-bit cache
 };
 // TH threads: 1024 where few tokens have a CTA each (16 tokens, 16 + 4 heads of 128 normed as a whole: 15.5 us with 256, most of it ten steps of two loads one after the other)
 template <int TH>
@@ -2294,7 +2295,7 @@ __global__ void __launch_bounds__(TH) k_seq_qk_rope(QkArgs a, SeqBatch sb) {
 	const int units = a.heads + a.kv_heads, per = (units + (int)gridDim.y - 1) / (int)gridDim.y; // this CTA's head vectors: query heads, then key heads
 	const int u0 = min(units, (int)blockIdx.y * per), u1 = min(units, u0 + per);
 	const int pos = sb.tpos[n];
-	const long row = cache_row(sb, sb.tslot[n], pos);
+	const long row = a.by_token ? n : cache_row(sb, sb.tslot[n], pos);
 	for (int i = tid; i < half; i += blockDim.x) {
 		double s, c;
 		sincos((double)pos * a.freq[i], &s, &c);

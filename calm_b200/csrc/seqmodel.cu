@@ -34,6 +34,9 @@ struct RunState {
 	bool readd = false;      // the embedding output is added to the stream right before this run
 	float* cache_a = nullptr; // SEQ_LATENT: latent rows (with the shared rotated key part behind each; an earlier layer's with kv_shared); SEQ_WINDOW / SEQ_GQA: key rows
 	float* cache_b = nullptr; // SEQ_WINDOW / SEQ_GQA: value rows
+	uint8_t *k8 = nullptr, *v8 = nullptr; // SEQ_GQA with cache8: codes [pages][kv_heads][page][dim] and scales [pages][kv_heads] in place of cache_a and cache_b
+	float *ks8 = nullptr, *vs8 = nullptr;
+	float* sinks = nullptr;   // SEQ_GQA with cache8 and add_one: a zero for every head
 	float* conv = nullptr;    // [slots][taps-1][channels]
 	bool cache_borrowed = false; // SEQ_LATENT with kv_shared: cache_a belongs to another run
 	float* delta = nullptr;   // SEQ_DELTA / SEQ_GLA: the recurrent state [slots][heads][dim][vdim]; SEQ_MINGRU: [slots][dim]
@@ -65,6 +68,7 @@ struct Seq {
 	// state manager
 	int n_pages = 0, max_pages = 0;
 	std::vector<int> free_pages;
+	std::vector<int> page_refs; // sequences that hold a page: full pages are shared by branches of one text
 	std::vector<Slot> slots;
 	std::vector<int> table; // host mirror of the page table
 	int* table_dev = nullptr;
@@ -119,6 +123,11 @@ struct Seq {
 	float* logits = nullptr;
 	void* hW = nullptr; // normed rows of the wanted tokens
 	int last_want = 0, last_tokens = 0;
+	float* kv = nullptr;                              // SEQ_GQA with cache8: the step's key and value rows before they are stored
+	size_t w_kv = 0;
+	// beams: page-locked scores in and picks out (written by the device), device scores and workspace
+	char *beam_host = nullptr, *beam_dev = nullptr;
+	size_t cap_beam_host = 0, cap_beam_dev = 0;
 
 	bool trace = false;
 	float* trace_buf = nullptr;
@@ -158,6 +167,21 @@ void run_kernel(Seq& s, int kind, double bytes, double flops, F&& launch) {
 		s.kind_ms[kind] += ms, s.kind_bytes[kind] += bytes, s.kind_flops[kind] += flops, ++s.kind_launches[kind];
 	}
 }
+
+// a call of an operator that counts its launches itself (seqops::launches); what it refuses here would be this file's own mistake
+template <typename F>
+void run_op(Seq& s, int kind, double bytes, double flops, F&& call) {
+	if (s.perf) CUDA_CHECK(cudaEventRecord(s.ev[0], s.stream));
+	if (call() != 0) CALM_FATAL("seq: %s", calm_b200_seq_error());
+	if (s.perf) {
+		CUDA_CHECK(cudaEventRecord(s.ev[1], s.stream));
+		CUDA_CHECK(cudaEventSynchronize(s.ev[1]));
+		float ms = 0;
+		CUDA_CHECK(cudaEventElapsedTime(&ms, s.ev[0], s.ev[1]));
+		s.kind_ms[kind] += ms, s.kind_bytes[kind] += bytes, s.kind_flops[kind] += flops, ++s.kind_launches[kind];
+	}
+}
+uint64_t all_launches() { return g_seq_launches + seqops::launches(); }
 
 // Every kernel goes out with programmatic stream serialization allowed: it may be launched while its predecessor still runs and
 // parks in pdl_enter() until that one has completed and flushed (a no-op attribute-less launch when CALM_B200_SEQ_PDL=0).
@@ -326,6 +350,7 @@ void validate_mixer(const Seq& s, int i, const SeqLayer& L, bool inner) {
 			CALM_FATAL("seq: layer %d: chunk, dist_bias, add_one, v_norm, qk_per_head and gate_per_head are options of SEQ_GQA", i);
 		if (L.type != SEQ_GQA && L.type != SEQ_LATENT && (L.no_gate || L.scores_f32)) CALM_FATAL("seq: layer %d: no_gate and scores_f32 are options of SEQ_GQA and SEQ_LATENT", i);
 		if (L.type != SEQ_GQA && (L.maps > 1 || L.v_from_k || L.rot_pairs || L.rot_kind)) CALM_FATAL("seq: layer %d: maps, v_from_k, rot_pairs and rot_kind are options of SEQ_GQA", i);
+		if (L.cache8 && (L.type != SEQ_GQA || L.maps > 1 || L.vdim != L.dim || L.dim % 16 || L.dim > 256)) CALM_FATAL("seq: layer %d: cache8 is an option of SEQ_GQA with one map and keys and values of one width, a multiple of 16 up to 256", i);
 		if (L.type != SEQ_LATENT && L.gate_channels) CALM_FATAL("seq: layer %d: gate_channels is an option of SEQ_LATENT", i);
 		if (L.type != SEQ_GQA && L.type != SEQ_LATENT && L.softcap != 0.f) CALM_FATAL("seq: layer %d: softcap is an option of SEQ_GQA and SEQ_LATENT", i);
 		if (L.type != SEQ_LATENT && L.kv_shared) CALM_FATAL("seq: layer %d: kv_shared is an option of SEQ_LATENT", i);
@@ -416,6 +441,7 @@ void reserve_tokens(Seq& s, int N, int B, int W) {
 		cudaFree(s.x), cudaFree(s.x0), cudaFree(s.proj), cudaFree(s.hA), cudaFree(s.a1), cudaFree(s.a2), cudaFree(s.a3), cudaFree(s.mo);
 		for (float*& p : s.f) cudaFree(p);
 		if (s.m.block != SEQ_BLOCK_SERIAL) s.mo = (float*)dalloc(cn * s.m.width * sizeof(float));
+		if (s.w_kv) cudaFree(s.kv), s.kv = (float*)dalloc(cn * s.w_kv * sizeof(float));
 		if (s.w_lin) cudaFree(s.lin), s.lin = (float*)dalloc(cn * s.w_lin * sizeof(float));
 		if (s.w_fsh) cudaFree(s.fsh), s.fsh = (float*)dalloc(cn * s.w_fsh * sizeof(float));
 		if (s.w_ah) cudaFree(s.ah), s.ah = dalloc(cn * s.w_ah * act_size(s));
@@ -812,6 +838,41 @@ void attention(Seq& s, int kind, AttArgs a, void* out, const SeqBatch& sb, doubl
 		});
 }
 
+// SEQ_GQA over an 8-bit cache: the operators that callers have for buffers of their own.  The keys that the split is planned for are rounded up to a few values per
+// octave: a decode graph is captured once per value.
+SeqCache8 cache8_of(const Seq& s, const SeqLayer& L, const RunState& r) {
+	return SeqCache8{r.k8, r.ks8, r.v8, r.vs8, s.n_pages, L.kv_heads, s.m.page, L.dim, s.table_dev, s.m.max_seqs, s.max_pages};
+}
+SeqAttend8 attend8_of(const Seq& s, const SeqLayer& L, const RunState& r, const float* gate, int ldg, void* out, int N, int longest) {
+	SeqAttend8 a = {};
+	a.q = SeqRows{s.f[0], SEQ_F32, (long long)L.heads * L.dim, L.dim, N};
+	a.out = SeqRows{out, s.m.exact ? SEQ_F32 : SEQ_BF16, (long long)L.heads * L.dim, L.dim, N};
+	a.heads = L.heads, a.scale = L.scale, a.window = std::max(L.window, 0), a.keep_first = L.window > 0 ? L.keep_first : 0, a.chunk = L.chunk, a.softcap = std::max(L.softcap, 0.f);
+	a.sinks = L.add_one ? r.sinks : nullptr, a.slopes = L.dist_bias ? r.slopes : nullptr;
+	a.gate = gate, a.gate_row = ldg, a.gate_head = L.gate_per_head ? 1 : L.dim, a.gate_dim = L.gate_per_head ? 0 : 1;
+	a.most_keys = round_split(cdiv(longest, 32)) * 32;
+	return a;
+}
+SeqPortions portions_of(const Seq& s, const SeqBatch& sb) {
+	int most = 0;
+	for (int b = 0; b < sb.B; ++b) most = std::max(most, s.hb_count[b]);
+	return SeqPortions{sb.B, sb.sstart, sb.scount, sb.sslot, sb.spos0, most};
+}
+void attention8(Seq& s, const SeqLayer& L, RunState& r, const float* kv, const float* gate, int ldg, void* out, const SeqBatch& sb, double kv_rows, int longest) {
+	const int N = sb.N, G = L.kv_heads, D = L.dim;
+	const SeqCache8 c = cache8_of(s, L, r);
+	const SeqPortions p = portions_of(s, sb);
+	const SeqRows k{const_cast<float*>(kv), SEQ_F32, (long long)G * D, D, N}, v{const_cast<float*>(kv) + (size_t)N * G * D, SEQ_F32, (long long)G * D, D, N};
+	run_op(s, KD_QK, (double)N * G * D * 10, 0, [&] { return calm_b200_seq_cache8_store(&c, &p, &k, &v, s.stream); });
+	SeqAttend8 a = attend8_of(s, L, r, gate, ldg, out, N, longest);
+	a.workspace_bytes = calm_b200_seq_attend8_workspace(&c, &p, &a);
+	ensure_part(s, a.workspace_bytes / sizeof(float));
+	a.workspace = s.part;
+	const int span = attn_span(L);
+	const double rows = span > 0 ? std::min(kv_rows, (double)N * span) : kv_rows;
+	run_op(s, KD_ATTN_WINDOW, rows * G * D * 2.0, 4.0 * rows * L.heads * D, [&] { return calm_b200_seq_attend8(&c, &p, &a, s.stream); });
+}
+
 void conv(Seq& s, const SeqLayer& L, RunState& r, ConvArgs& ca, const SeqBatch& sb, const float* proj, int ldp) {
 	const int units = ca.seg[0].heads + ca.seg[1].heads + ca.seg[2].heads;
 	ca.proj = proj, ca.ldp = ldp, ca.w = (const bf16*)L.conv, ca.taps = L.taps, ca.channels = conv_channels(L), ca.state = r.conv, ca.eps = s.m.eps;
@@ -1089,9 +1150,10 @@ void mixer_typed(Seq& s, const SeqLayer& L, RunState& r, const SeqBatch& sb, dou
 		qa.proj = proj, qa.ldp = P, qa.heads = H, qa.kv_heads = G, qa.vheads = Gv, qa.dim = D, qa.vdim = Dv, qa.qw = (const bf16*)L.q_norm, qa.kw = (const bf16*)L.k_norm, qa.eps = s.m.eps;
 		const auto rt = s.rot.find(&L);
 		qa.rot_dims = rt == s.rot.end() ? 0 : L.rot_dims, qa.freq = rt == s.rot.end() ? nullptr : rt->second.first, qa.mag = rt == s.rot.end() ? 1.f : rt->second.second, qa.q = s.f[0], qa.kc = r.cache_a, qa.vc = r.cache_b;
+		if (L.cache8) qa.kc = s.kv, qa.vc = s.kv + (size_t)N * G * D, qa.by_token = 1;
 		qa.v_norm = L.v_norm, qa.per_head = L.qk_per_head, qa.v_from_k = L.v_from_k, qa.pairs2 = L.rot_pairs;
 		// when all of the step's attention runs as products the queries go straight to the matrix those read: rounded, or as value and remainder
-		const bool direct = !s.m.exact && s.attn_products && s.n_on_products == sb.B;
+		const bool direct = !L.cache8 && !s.m.exact && s.attn_products && s.n_on_products == sb.B;
 		if (direct) qa.qb = (bf16*)s.a3, qa.qsplit = L.scores_f32;
 		// few tokens: their heads are shared out over several CTAs (a norm over the whole projection keeps them in one)
 		const int slices = L.q_norm && !L.qk_per_head ? 1 : std::max(1, std::min(cdiv(H + G, 8), 2 * s.sms / N));
@@ -1100,6 +1162,11 @@ void mixer_typed(Seq& s, const SeqLayer& L, RunState& r, const SeqBatch& sb, dou
 			if (slices == 1 && 2 * N <= s.sms) launch_k(s, k_seq_qk_rope<1024>, N, 1024, qk_smem, qa, sb);
 			else launch_k(s, k_seq_qk_rope<256>, dim3(N, slices), 256, qk_smem, qa, sb);
 		});
+		if (L.cache8) {
+			attention8(s, L, r, s.kv, L.no_gate ? nullptr : proj + H * D + G * D + Vn, P, a2, sb, kv_rows, longest);
+			out_product<AT>(s, a2, L.w_o, N, H * Dv, oe, L.b_o);
+			return;
+		}
 		AttArgs a;
 		a.q = s.f[0], a.kc = r.cache_a, a.vc = r.cache_b, a.kld = G * D, a.vld = Gv * Dv, a.heads = H, a.group = H / G, a.kd = D, a.vd = Dv, a.vshare = maps;
 		a.window = L.window, a.keep_first = L.window > 0 ? L.keep_first : 0, a.scale = L.scale, a.sink = nullptr;
@@ -1489,8 +1556,16 @@ void forward(Seq& s, const SeqBatch& sb, int n_want, double kv_rows, int longest
 void forward_decode_graph(Seq& s, const SeqBatch& sb, int n_want, double kv_rows, int longest) {
 	std::vector<int> key = {sb.N, n_want};
 	size_t part_need = 0;
-	auto one = [&](const SeqLayer& L) {
+	auto one = [&](const SeqLayer& L, const RunState& r) {
 		if (L.type != SEQ_LATENT && L.type != SEQ_WINDOW && L.type != SEQ_GQA) return; // recurrent mixers: nothing to share out
+		if (L.cache8) { // the workspace it needs tells the shares
+			const SeqCache8 c = cache8_of(s, L, r);
+			const SeqPortions p = portions_of(s, sb);
+			const SeqAttend8 a = attend8_of(s, L, r, nullptr, 0, s.a2, sb.N, longest);
+			const size_t need = calm_b200_seq_attend8_workspace(&c, &p, &a) / sizeof(float);
+			key.push_back((int)(need / ((size_t)sb.N * L.heads * (L.dim + 2)))), part_need = std::max(part_need, need);
+			return;
+		}
 		const bool lat = L.type == SEQ_LATENT;
 		const int group = lat ? L.heads : L.heads / L.kv_heads, kd = lat ? L.kv_rank + L.rot_dims : L.dim, vd = lat ? L.kv_rank : L.vdim;
 		const int heads = L.heads * att_maps(L), ns = attn_plan(s, group, kd, vd, lat, heads, sb.N, attn_span(L), longest, att_maps(L) > 1).nsplit;
@@ -1499,14 +1574,14 @@ void forward_decode_graph(Seq& s, const SeqBatch& sb, int n_want, double kv_rows
 	};
 	for (const RunState& r : s.runs) {
 		const SeqLayer& L = s.layers[r.layer];
-		if (L.type == SEQ_PAIR) one(L.pair[0]), one(L.pair[1]);
-		else one(L);
+		if (L.type == SEQ_PAIR) one(L.pair[0], r.sub[0]), one(L.pair[1], r.sub[1]);
+		else one(L, r);
 	}
 	ensure_part(s, part_need); // no allocation inside a capture
 	auto it = s.graphs.find(key);
 	if (it == s.graphs.end()) {
 		if (s.graphs.size() > 256) drop_graphs(s);
-		const uint64_t before = g_seq_launches;
+		const uint64_t before = all_launches();
 		cudaGraph_t graph = nullptr;
 		cudaGraphExec_t exec = nullptr;
 		++g_seq_routes[SEQ_ROUTE_CAPTURE];
@@ -1515,8 +1590,8 @@ void forward_decode_graph(Seq& s, const SeqBatch& sb, int n_want, double kv_rows
 		CUDA_CHECK(cudaStreamEndCapture(s.stream, &graph));
 		CUDA_CHECK(cudaGraphInstantiate(&exec, graph, 0));
 		CUDA_CHECK(cudaGraphDestroy(graph));
-		it = s.graphs.emplace(key, std::make_pair(exec, (int)(g_seq_launches - before))).first;
-		g_seq_launches = before;
+		it = s.graphs.emplace(key, std::make_pair(exec, (int)(all_launches() - before))).first;
+		g_seq_launches -= all_launches() - before; // captured, not launched
 	}
 	CUDA_CHECK(cudaGraphLaunch(it->second.first, s.stream));
 	g_seq_launches += it->second.second;
@@ -1532,7 +1607,7 @@ extern "C" void* calm_b200_seq_upload(const void* host, size_t size) {
 	return p;
 }
 extern "C" void calm_b200_seq_free(void* p) { cudaFree(p); }
-extern "C" uint64_t calm_b200_seq_launch_count(void) { return g_seq_launches + seqops::launches(); }
+extern "C" uint64_t calm_b200_seq_launch_count(void) { return all_launches(); }
 extern "C" uint64_t calm_b200_seq_route_count(int route) { return route >= SEQ_ROUTE_PAIRS ? (route < SEQ_ROUTE_PAIRS + TG_EPILOGUES ? g_tg.pair_launches[route - SEQ_ROUTE_PAIRS] : 0) : route >= 0 ? g_seq_routes[route] : 0; }
 extern "C" int calm_b200_seq_skinny_warps(int m, int k, int groups, int rows, int sms) { return skinny_warps(m, k, groups, rows, sms); }
 extern "C" int calm_b200_seq_delta_blocks_pay(int longest, int few, int heads, int vdim, int sms) { return delta_blocks_pay(longest, few, heads, vdim, sms); }
@@ -1588,6 +1663,7 @@ extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 	s.n_pages = cdiv(m.max_tokens, m.page) + m.max_seqs;
 	s.max_pages = s.n_pages;
 	for (int p = s.n_pages - 1; p >= 0; --p) s.free_pages.push_back(p);
+	s.page_refs.assign(s.n_pages, 0);
 	s.slots.resize(m.max_seqs);
 	s.table.assign((size_t)m.max_seqs * s.max_pages, 0);
 	s.table_dev = (int*)dalloc(s.table.size() * sizeof(int));
@@ -1608,7 +1684,16 @@ extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 			r.delta_per_slot = L.dim;
 			r.delta = (float*)dalloc(r.delta_per_slot * m.max_seqs * sizeof(float));
 		}
-		if (L.type == SEQ_WINDOW || L.type == SEQ_GQA) {
+		if (L.cache8) {
+			const size_t codes = rows * L.kv_heads * L.dim, scales = (size_t)s.n_pages * L.kv_heads * sizeof(float);
+			r.k8 = (uint8_t*)dalloc(codes), r.v8 = (uint8_t*)dalloc(codes), r.ks8 = (float*)dalloc(scales), r.vs8 = (float*)dalloc(scales);
+			for (uint8_t* c : {r.k8, r.v8}) CUDA_CHECK(cudaMemset(c, 0, codes));
+			for (float* c : {r.ks8, r.vs8}) CUDA_CHECK(cudaMemset(c, 0, scales));
+			if (L.add_one) {
+				r.sinks = (float*)dalloc(L.heads * sizeof(float));
+				CUDA_CHECK(cudaMemset(r.sinks, 0, L.heads * sizeof(float)));
+			}
+		} else if (L.type == SEQ_WINDOW || L.type == SEQ_GQA) {
 			r.cache_a = (float*)dalloc(rows * L.kv_heads * att_maps(L) * L.dim * sizeof(float));
 			r.cache_b = (float*)dalloc(rows * L.kv_heads * L.vdim * sizeof(float));
 		}
@@ -1701,6 +1786,7 @@ extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 			if (L.shared_ff > 0) s.w_fsh = std::max(s.w_fsh, (size_t)2 * L.shared_ff + 1 + L.experts + L.ident);
 			s.w_a = std::max(s.w_a, (size_t)L.shared_ff);
 		}
+		if (L.cache8) s.w_kv = std::max(s.w_kv, (size_t)2 * L.kv_heads * L.dim);
 		if (L.type == SEQ_GQA) s.w_f = std::max({s.w_f, (size_t)L.heads * att_maps(L) * L.dim, att_maps(L) > 1 ? (size_t)L.heads * 2 * L.vdim : 0}), s.w_a = std::max({s.w_a, (size_t)L.heads * L.vdim, (size_t)L.heads * att_maps(L) * L.dim * (L.scores_f32 ? 3 : 1)}); // a3 holds the queries (as value + remainder pairs when scores keep fp32 accuracy)
 		if (L.type == SEQ_GLA) s.w_f = std::max({s.w_f, (size_t)L.heads * L.dim, (size_t)L.heads * L.vdim}), s.w_a = std::max({s.w_a, (size_t)L.heads * L.vdim, (size_t)L.a_rank});
 		if (is_lin(L)) {
@@ -1722,7 +1808,7 @@ extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 	for (const SeqLayer& L : s.layers) {
 		if (L.type == SEQ_PAIR && L.ff > 0) { // the pair's own record carries the layer's feed-forward
 			SeqLayer ffonly = L;
-			ffonly.type = SEQ_GQA, ffonly.heads = ffonly.kv_heads = ffonly.dim = ffonly.vdim = 0, ffonly.no_gate = 1;
+			ffonly.cache8 = 0, ffonly.type = SEQ_GQA, ffonly.heads = ffonly.kv_heads = ffonly.dim = ffonly.vdim = 0, ffonly.no_gate = 1;
 			widths(ffonly);
 		}
 		widths(L);
@@ -1737,10 +1823,11 @@ extern "C" void calm_b200_seq_release(void* handle) {
 	drop_graphs(*s);
 	std::function<void(RunState&)> drop = [&](RunState& r) {
 		if (!r.cache_borrowed) cudaFree(r.cache_a);
-		cudaFree(r.cache_b), cudaFree(r.conv), cudaFree(r.delta), cudaFree(r.mstate), cudaFree(r.slopes);
+		cudaFree(r.cache_b), cudaFree(r.k8), cudaFree(r.v8), cudaFree(r.ks8), cudaFree(r.vs8), cudaFree(r.sinks), cudaFree(r.conv), cudaFree(r.delta), cudaFree(r.mstate), cudaFree(r.slopes);
 		for (RunState& q : r.sub) drop(q);
 	};
 	for (RunState& r : s->runs) drop(r);
+	cudaFree(s->kv), cudaFree(s->beam_dev), cudaFreeHost(s->beam_host);
 	cudaFree(s->lin), cudaFree(s->fsh), cudaFree(s->hist), cudaFree(s->carry), cudaFree(s->scan_ws), cudaFree(s->rope_cs);
 	cudaFree(s->table_dev), cudaFree(s->meta_dev), cudaFreeHost(s->meta), cudaFreeHost(s->picks), cudaFree(s->logits), cudaFree(s->hW);
 	cudaFree(s->part), cudaFree(s->a3), cudaFree(s->att_kb), cudaFree(s->att_vt), cudaFree(s->att_s), cudaFree(s->att_p), cudaFree(s->x), cudaFree(s->x0), cudaFree(s->proj), cudaFree(s->hA), cudaFree(s->a1), cudaFree(s->a2), cudaFree(s->trace_buf);
@@ -1770,11 +1857,165 @@ extern "C" int calm_b200_seq_open(void* handle) {
 	return -1;
 }
 
+// a sequence's pages go back, but for those that others still hold
+static void leave(Seq& s, Slot& sl) {
+	for (int p : sl.pages)
+		if (--s.page_refs[p] == 0) s.free_pages.push_back(p);
+	sl.pages.clear(), sl.open = false, sl.len = 0;
+}
+
 extern "C" int calm_b200_seq_close(void* handle, int slot) {
 	Seq& s = *(Seq*)handle;
 	if (slot < 0 || slot >= (int)s.slots.size() || !s.slots[slot].open) return -3;
-	for (int p : s.slots[slot].pages) s.free_pages.push_back(p);
-	s.slots[slot].pages.clear(), s.slots[slot].open = false, s.slots[slot].len = 0;
+	leave(s, s.slots[slot]);
+	return 0;
+}
+
+// What branches and resizing know of a model's buffers: f(pointer, bytes of a page, bytes of a page's row or 0, borrowed) for every cache ...
+template <typename F>
+static void each_cache(Seq& s, F&& f) {
+	std::function<void(RunState&, const SeqLayer&)> one = [&](RunState& r, const SeqLayer& L) {
+		if (L.type == SEQ_PAIR) {
+			one(r.sub[0], L.pair[0]), one(r.sub[1], L.pair[1]);
+			return;
+		}
+		const size_t page = s.m.page, a = L.type == SEQ_LATENT ? L.kv_rank + L.rot_dims : (size_t)L.kv_heads * att_maps(L) * L.dim, b = (size_t)L.kv_heads * L.vdim;
+		if (r.cache_a) f(r.cache_a, page * a * sizeof(float), a * sizeof(float), r.cache_borrowed);
+		if (r.cache_b) f(r.cache_b, page * b * sizeof(float), b * sizeof(float), false);
+		if (r.k8) f(r.k8, page * b, (size_t)0, false), f(r.v8, page * b, (size_t)0, false), f(r.ks8, L.kv_heads * sizeof(float), (size_t)0, false), f(r.vs8, L.kv_heads * sizeof(float), (size_t)0, false);
+	};
+	for (RunState& r : s.runs) one(r, s.layers[r.layer]);
+}
+// ... and f(pointer, bytes of a slot) for every recurrent state
+template <typename F>
+static void each_state(Seq& s, F&& f) {
+	std::function<void(RunState&)> one = [&](RunState& r) {
+		if (r.conv_per_slot) f(r.conv, r.conv_per_slot * sizeof(float));
+		if (r.delta_per_slot) f(r.delta, r.delta_per_slot * sizeof(float));
+		if (r.m_per_slot) f(r.mstate, r.m_per_slot * sizeof(float));
+		for (RunState& q : r.sub) one(q);
+	};
+	for (RunState& r : s.runs) one(r);
+}
+
+extern "C" int calm_b200_seq_branch(void* handle, int n_from, const int* from_slots, int n_to, const int* from_parents, int* out_slots) {
+	Seq& s = *(Seq*)handle;
+	const int page = s.m.page, S = (int)s.slots.size();
+	if (n_from < 1 || n_to < 0 || !from_slots || (n_to && (!from_parents || !out_slots))) return -3;
+	const std::vector<int> slots(from_slots, from_slots + n_from), parents(from_parents, from_parents + n_to); // (the result may go where they came from)
+	std::vector<int> kids(n_from, 0);
+	std::vector<char> named(S, 0);
+	for (int i = 0; i < n_from; ++i) {
+		if (slots[i] < 0 || slots[i] >= S || !s.slots[slots[i]].open || named[slots[i]]) return -3;
+		named[slots[i]] = 1;
+	}
+	for (int i = 0; i < n_to; ++i) {
+		if (parents[i] < 0 || parents[i] >= n_from) return -3;
+		++kids[parents[i]];
+	}
+	// room: slots and pages that ended sequences leave count; a page goes when the last of its sequences does
+	int places = 0, room = (int)s.free_pages.size(), more = 0, need = 0;
+	for (const Slot& sl : s.slots) places += !sl.open;
+	std::vector<int> left(s.page_refs);
+	for (int i = 0; i < n_from; ++i)
+		if (kids[i] == 0) {
+			++places;
+			for (int p : s.slots[slots[i]].pages) room += --left[p] == 0;
+		} else {
+			more += kids[i] - 1;
+			if (s.slots[slots[i]].len % page) need += kids[i] - 1;
+		}
+	if (more > places) return -1;
+	if (need > room) return -2;
+	std::vector<int> vacant;
+	for (int i = 0; i < n_from; ++i)
+		if (kids[i] == 0) leave(s, s.slots[slots[i]]), vacant.push_back(slots[i]);
+	for (int i = 0; i < S && (int)vacant.size() < more; ++i)
+		if (!s.slots[i].open && !named[i]) vacant.push_back(i);
+	// a sequence's first branch keeps its slot; the others share its full pages and get copies of what will still be written: the page in part filled, the recurrent state
+	std::vector<int> pf, pt, pr, sf, st;
+	std::vector<char> kept(n_from, 0);
+	size_t next = 0;
+	for (int i = 0; i < n_to; ++i) {
+		const int p = parents[i], from = slots[p];
+		if (!kept[p]) {
+			kept[p] = 1, out_slots[i] = from;
+			continue;
+		}
+		const int to = vacant[next++];
+		const Slot& a = s.slots[from];
+		Slot& b = s.slots[to];
+		b.open = true, b.len = a.len, b.last_tok = a.last_tok, b.pages = a.pages;
+		for (int q : b.pages) ++s.page_refs[q];
+		if (a.len % page) {
+			const int old = b.pages.back(), fresh = s.free_pages.back();
+			s.free_pages.pop_back();
+			--s.page_refs[old], s.page_refs[fresh] = 1, b.pages.back() = fresh;
+			pf.push_back(old), pt.push_back(fresh), pr.push_back(a.len % page);
+		}
+		const size_t row = (size_t)to * s.max_pages;
+		std::copy(b.pages.begin(), b.pages.end(), s.table.begin() + row);
+		if (!b.pages.empty()) CUDA_CHECK(cudaMemcpyAsync(s.table_dev + row, s.table.data() + row, b.pages.size() * sizeof(int), cudaMemcpyHostToDevice, s.stream));
+		sf.push_back(from), st.push_back(to), out_slots[i] = to;
+	}
+	if (sf.empty()) return 0;
+	std::vector<SeqUnits> pools;
+	each_cache(s, [&](auto*& p, size_t unit, size_t row, bool borrowed) {
+		if (!borrowed) pools.push_back(SeqUnits{p, p, (long long)unit, (long long)row, s.n_pages, s.n_pages, 0});
+	});
+	each_state(s, [&](void* p, size_t unit) { pools.push_back(SeqUnits{p, p, (long long)unit, 0, S, S, 1}); });
+	if (calm_b200_seq_copy_units((int)pools.size(), pools.data(), (int)pf.size(), pf.data(), pt.data(), pr.data(), (int)sf.size(), sf.data(), st.data(), s.stream) != 0)
+		CALM_FATAL("seq: %s", calm_b200_seq_error());
+	return 0;
+}
+
+extern "C" int calm_b200_seq_resize(void* handle, int max_tokens) {
+	Seq& s = *(Seq*)handle;
+	if (max_tokens < 1 || (long long)max_tokens + (long long)s.m.max_seqs * s.m.page > 0x7fffffff) return -3;
+	const int pages = cdiv(max_tokens, s.m.page) + s.m.max_seqs;
+	std::vector<int> from, to, place(s.n_pages, -1); // live pages, in order, go to the front
+	for (int p = 0; p < s.n_pages; ++p)
+		if (s.page_refs[p] > 0) place[p] = (int)from.size(), from.push_back(p), to.push_back(place[p]);
+	const int live = (int)from.size();
+	if (live > pages) return -2;
+	// all of the new memory first: when there is not enough, nothing has changed
+	std::vector<SeqUnits> pools;
+	std::map<void*, void*> moved;
+	bool fits = true;
+	auto get = [&](size_t bytes) {
+		void* p = nullptr;
+		if (fits && cudaMalloc(&p, bytes ? bytes : 16) != cudaSuccess) (void)cudaGetLastError(), fits = false, p = nullptr;
+		return p;
+	};
+	each_cache(s, [&](auto*& p, size_t unit, size_t row, bool borrowed) {
+		if (borrowed) return;
+		void* fresh = get(unit * pages);
+		moved[p] = fresh;
+		pools.push_back(SeqUnits{p, fresh, (long long)unit, (long long)row, s.n_pages, pages, 0});
+	});
+	int* table_dev = (int*)get((size_t)s.m.max_seqs * pages * sizeof(int));
+	if (!fits) {
+		for (auto& kv : moved) cudaFree(kv.second);
+		cudaFree(table_dev);
+		return -4;
+	}
+	if (calm_b200_seq_copy_units((int)pools.size(), pools.data(), live, from.data(), to.data(), nullptr, 0, nullptr, nullptr, s.stream) != 0) CALM_FATAL("seq: %s", calm_b200_seq_error());
+	std::vector<int> table((size_t)s.m.max_seqs * pages, 0), refs(pages, 0);
+	for (int i = 0; i < (int)s.slots.size(); ++i) {
+		Slot& sl = s.slots[i];
+		for (size_t k = 0; k < sl.pages.size(); ++k) sl.pages[k] = place[sl.pages[k]], table[(size_t)i * pages + k] = sl.pages[k];
+	}
+	for (int p = 0; p < s.n_pages; ++p)
+		if (place[p] >= 0) refs[place[p]] = s.page_refs[p];
+	CUDA_CHECK(cudaMemcpyAsync(table_dev, table.data(), table.size() * sizeof(int), cudaMemcpyHostToDevice, s.stream));
+	CUDA_CHECK(cudaStreamSynchronize(s.stream));
+	drop_graphs(s); // captured launches hold the old addresses
+	each_cache(s, [&](auto*& p, size_t, size_t, bool) { p = static_cast<std::remove_reference_t<decltype(p)>>(moved[p]); });
+	for (auto& kv : moved) cudaFree(kv.first);
+	cudaFree(s.table_dev);
+	s.table_dev = table_dev, s.table = std::move(table), s.page_refs = std::move(refs), s.n_pages = s.max_pages = pages, s.m.max_tokens = max_tokens;
+	s.free_pages.clear();
+	for (int p = pages - 1; p >= live; --p) s.free_pages.push_back(p);
 	return 0;
 }
 
@@ -1822,6 +2063,7 @@ extern "C" int calm_b200_seq_step(void* handle, int n_seq, const int* slots, con
 		const size_t had = sl.pages.size();
 		while ((int)sl.pages.size() * m.page < sl.len + counts[b]) {
 			s.table[(size_t)slots[b] * s.max_pages + sl.pages.size()] = s.free_pages.back();
+			s.page_refs[s.free_pages.back()] = 1;
 			sl.pages.push_back(s.free_pages.back()), s.free_pages.pop_back();
 		}
 		if (sl.pages.size() > had) { // only the new entries of this slot's row travel
@@ -1859,6 +2101,37 @@ extern "C" void calm_b200_seq_argmax(void* handle, int* out) {
 	++g_seq_launches;
 	CUDA_CHECK(cudaStreamSynchronize(s.stream));
 	std::copy(s.picks, s.picks + s.last_want, out);
+}
+extern "C" int calm_b200_seq_beams(void* handle, int row0, int groups, int beams, const float* scores, int n, int* tokens, int* parents, float* best) {
+	Seq& s = *(Seq*)handle;
+	if (row0 < 0 || groups < 1 || beams < 1 || beams > 64 || n < 1 || n > 64 || !scores || !tokens || !parents || !best || (long long)row0 + (long long)groups * beams > s.last_want) return -3;
+	const size_t rows = (size_t)groups * beams, picks = (size_t)groups * n, work = calm_b200_seq_beam_workspace(groups, beams, s.m.vocab, n);
+	if (!work) return -3;
+	const size_t host = rows * sizeof(float) + 3 * picks * sizeof(int), dev = work + rows * sizeof(float);
+	if (host > s.cap_beam_host || dev > s.cap_beam_dev) {
+		CUDA_CHECK(cudaStreamSynchronize(s.stream));
+		if (host > s.cap_beam_host) {
+			cudaFreeHost(s.beam_host);
+			s.cap_beam_host = 2 * host;
+			CUDA_CHECK(cudaHostAlloc((void**)&s.beam_host, s.cap_beam_host, cudaHostAllocMapped));
+		}
+		if (dev > s.cap_beam_dev) cudaFree(s.beam_dev), s.cap_beam_dev = 2 * dev, s.beam_dev = (char*)dalloc(s.cap_beam_dev);
+	}
+	float* const hs = (float*)s.beam_host;
+	int* const hp = (int*)(hs + rows); // tokens, parents, best
+	char* mapped = nullptr;
+	CUDA_CHECK(cudaHostGetDevicePointer((void**)&mapped, s.beam_host, 0));
+	int* const dp = (int*)(mapped + rows * sizeof(float));
+	std::copy(scores, scores + rows, hs);
+	CUDA_CHECK(cudaMemcpyAsync(s.beam_dev + work, hs, rows * sizeof(float), cudaMemcpyHostToDevice, s.stream));
+	SeqBeam q = {};
+	q.logits = s.logits + (size_t)row0 * s.m.vocab, q.type = SEQ_F32, q.row_stride = s.m.vocab, q.group_stride = (long long)beams * s.m.vocab, q.scores = (const float*)(s.beam_dev + work);
+	q.groups = groups, q.beams = beams, q.vocab = s.m.vocab, q.n = n, q.tokens = dp, q.parents = dp + picks, q.best = (float*)(dp + 2 * picks), q.workspace = s.beam_dev, q.workspace_bytes = work;
+	if (calm_b200_seq_beam_select(&q, s.stream) != 0) CALM_FATAL("seq: %s", calm_b200_seq_error());
+	CUDA_CHECK(cudaStreamSynchronize(s.stream));
+	std::copy(hp, hp + picks, tokens), std::copy(hp + picks, hp + 2 * picks, parents);
+	memcpy(best, hp + 2 * picks, picks * sizeof(float));
+	return 0;
 }
 extern "C" const float* calm_b200_seq_device_logits(void* handle) { return ((Seq*)handle)->logits; }
 

@@ -48,7 +48,7 @@ SeqLayer._fields_ = [(n, C.c_int) for n in ("type", "heads", "kv_heads", "dim", 
                                                                          ("expert_act", C.c_int), ("weight_input", C.c_int), ("shared_gate", C.c_int), ("kv_shared", C.c_int),
                                                                          ("dwa", C.c_void_p), ("w_rg2", C.c_void_p), ("b_rg2", C.c_void_p)] + [("glu_rows", C.c_int)] + \
                [("maps", C.c_int), ("diff_lambda", C.c_float), ("diff_mul", C.c_float), ("v_from_k", C.c_int), ("softcap", C.c_float), ("rot_pairs", C.c_int),
-                ("rot_kind", C.c_int), ("rot_low", C.c_float), ("rot_high", C.c_float), ("gate_channels", C.c_int)]
+                ("rot_kind", C.c_int), ("rot_low", C.c_float), ("rot_high", C.c_float), ("gate_channels", C.c_int), ("cache8", C.c_int)]
 
 
 class SeqModel(C.Structure):
@@ -79,6 +79,9 @@ def load() -> C.CDLL:
     L.calm_b200_seq_close.argtypes, L.calm_b200_seq_close.restype = [C.c_void_p, C.c_int], C.c_int
     L.calm_b200_seq_length.argtypes, L.calm_b200_seq_length.restype = [C.c_void_p, C.c_int], C.c_int
     L.calm_b200_seq_free_pages.argtypes, L.calm_b200_seq_free_pages.restype = [C.c_void_p], C.c_int
+    L.calm_b200_seq_branch.argtypes, L.calm_b200_seq_branch.restype = [C.c_void_p, C.c_int, _iptr, C.c_int, _iptr, _iptr], C.c_int
+    L.calm_b200_seq_resize.argtypes, L.calm_b200_seq_resize.restype = [C.c_void_p, C.c_int], C.c_int
+    L.calm_b200_seq_beams.argtypes, L.calm_b200_seq_beams.restype = [C.c_void_p, C.c_int, C.c_int, C.c_int, _fptr, C.c_int, _iptr, _iptr, _fptr], C.c_int
     L.calm_b200_seq_step.argtypes = [C.c_void_p, C.c_int, _iptr, _iptr, _iptr, C.c_int, _iptr, _fptr]
     L.calm_b200_seq_step.restype = C.c_int
     L.calm_b200_seq_argmax.argtypes, L.calm_b200_seq_argmax.restype = [C.c_void_p, _iptr], None
@@ -105,12 +108,25 @@ class SeqError(RuntimeError):
     pass
 
 
+def plain_mixers(layers: Sequence[Dict[str, object]]) -> List[Dict[str, object]]:
+    return [m for d in layers for m in (d["pair"] if d.get("pair") else [d])]
+
+
+def cache8_fits(d: Dict[str, object]) -> bool:
+    return d.get("type") == SEQ_GQA and d.get("maps", 0) < 2 and d["dim"] == d["vdim"] and d["dim"] % 16 == 0 and d["dim"] <= 256
+
+
 class SeqDeviceModel:
     """A layer-list model on the GPU.  `layers` are dicts of SeqLayer fields whose tensor-valued entries name tensors in
     `tensors` (host torch tensors, uploaded here); vimulorn.py, bovinex.py, zazilix.py, sopepel.py, fasulix.py and tabisun.py are the hosts that fill them from a checkpoint."""
 
     def __init__(self, head: Dict[str, object], layers: List[Dict[str, object]], tensors: Dict[str, "object"], exact: bool = False,
-                 max_tokens: int = 4096, max_seqs: int = 64, page: int = 16):
+                 max_tokens: int = 4096, max_seqs: int = 64, page: int = 16, cache_bits: int = 32):
+        """cache_bits 8: grouped-query layers with one map and keys and values of one width (a multiple of 16 up to 256) cache them in 8 bits; other layers' caches stay fp32."""
+        if cache_bits not in (8, 32):
+            raise ValueError("cache_bits must be 8 or 32")
+        if cache_bits == 8 and not any(cache8_fits(d) for d in plain_mixers(layers)):
+            raise ValueError("no layer of this model can cache in 8 bits")
         self.lib = load()
         self._uploaded: Dict[str, int] = {}
         self._keep = tensors
@@ -145,6 +161,8 @@ class SeqDeviceModel:
                     setattr(rec, k, ptr(v))
                 else:
                     setattr(rec, k, v)
+            if cache_bits == 8:
+                rec.cache8 = int(cache8_fits(d))
 
         self._layers = (SeqLayer * len(layers))()
         for rec, d in zip(self._layers, layers):
@@ -184,6 +202,27 @@ class SeqDeviceModel:
     def free_pages(self) -> int:
         return self.lib.calm_b200_seq_free_pages(self.handle)
 
+    def branch(self, slots: Sequence[int], parents: Sequence[int]) -> List[int]:
+        """Sequences that go on in several ways, or end: the slots of len(parents) sequences, the i-th going on from what slots[parents[i]] holds.  The first that names a
+        parent keeps its slot, the others share its full pages; a sequence that is not named is closed."""
+        sl, pa = np.ascontiguousarray(slots, np.int32), np.ascontiguousarray(parents, np.int32)
+        out = np.zeros(max(1, len(pa)), np.int32)
+        rc = self.lib.calm_b200_seq_branch(self.handle, len(sl), sl.ctypes.data_as(_iptr), len(pa), pa.ctypes.data_as(_iptr), out.ctypes.data_as(_iptr))
+        if rc != 0:
+            raise SeqError({-1: "no free sequence slot", -2: "the page pool is exhausted: more live tokens than max_tokens"}.get(rc, "bad branch: a slot that is not open or named twice, or a parent outside the list"))
+        return [int(x) for x in out[:len(pa)]]
+
+    def fork(self, slot: int, n: int) -> List[int]:
+        """n more sequences that go on from what `slot` holds (which stays open)."""
+        return self.branch([slot], [0] * (n + 1))[1:]
+
+    def resize(self, max_tokens: int) -> None:
+        """A cache for max_tokens live tokens from now on, smaller or larger; live sequences keep theirs."""
+        rc = self.lib.calm_b200_seq_resize(self.handle, int(max_tokens))
+        if rc != 0:
+            raise SeqError({-2: f"the live sequences hold more than {max_tokens} tokens", -4: "the device lacks the memory"}.get(rc, "max_tokens must be positive"))
+        self.desc.max_tokens = int(max_tokens)
+
     # ---- the step function
     def step(self, slots: Sequence[int], token_lists: Sequence[Sequence[int]], want: Sequence[int], fetch: bool = True) -> Optional[np.ndarray]:
         """Feed token_lists[i] to the sequence in slots[i]; `want` = packed indices whose logits are computed.  Returns
@@ -206,6 +245,19 @@ class SeqDeviceModel:
         out = np.zeros(n_want, np.int32)
         self.lib.calm_b200_seq_argmax(self.handle, out.ctypes.data_as(_iptr))
         return out
+
+    def beams(self, scores: np.ndarray, n: int, row0: int = 0):
+        """The n best continuations of every group of beams from the last step's logits, whose rows row0 .. are the groups' beams: scores [groups, beams] float32
+        -> tokens, parents, scores [groups, n] (see seqops.beam_select)."""
+        sc = np.ascontiguousarray(scores, np.float32)
+        if sc.ndim != 2:
+            raise ValueError("scores must be [groups, beams]")
+        G, K = sc.shape
+        tok, par, best = np.zeros((G, max(n, 1)), np.int32), np.zeros((G, max(n, 1)), np.int32), np.zeros((G, max(n, 1)), np.float32)
+        rc = self.lib.calm_b200_seq_beams(self.handle, row0, G, K, sc.ctypes.data_as(_fptr), n, tok.ctypes.data_as(_iptr), par.ctypes.data_as(_iptr), best.ctypes.data_as(_fptr))
+        if rc != 0:
+            raise SeqError("bad beams: rows that the last step did not want, or beams or n outside 1 .. 64")
+        return tok, par, best
 
     def set_trace(self, on: bool) -> None:
         self.lib.calm_b200_seq_set_trace(self.handle, int(on))

@@ -122,19 +122,19 @@ def plan(cfg: dict, tensors: Dict[str, torch.Tensor]) -> Tuple[dict, List[dict],
     return head, layers, up
 
 
-def load(folder: str, dtype: str = "bfloat16", max_tokens: int = 4096, max_seqs: int = 64, page: int = 16) -> seqlib.SeqDeviceModel:
+def load(folder: str, dtype: str = "bfloat16", max_tokens: int = 4096, max_seqs: int = 64, page: int = 16, cache_bits: int = 32) -> seqlib.SeqDeviceModel:
     """config.json + model.safetensors of `folder` onto the GPU."""
     with open(os.path.join(folder, "config.json")) as f:
         cfg = json.load(f)
     tensors, _ = container.read_tensors(os.path.join(folder, "model.safetensors"))
-    return from_tensors(cfg, tensors, dtype, max_tokens, max_seqs, page)
+    return from_tensors(cfg, tensors, dtype, max_tokens, max_seqs, page, cache_bits)
 
 
-def from_tensors(cfg: dict, tensors: Dict[str, torch.Tensor], dtype: str = "bfloat16", max_tokens: int = 4096, max_seqs: int = 64, page: int = 16):
+def from_tensors(cfg: dict, tensors: Dict[str, torch.Tensor], dtype: str = "bfloat16", max_tokens: int = 4096, max_seqs: int = 64, page: int = 16, cache_bits: int = 32):
     if dtype not in ("bfloat16", "float32"):
         raise ValueError("dtype must be bfloat16 or float32")
     head, layers, up = plan(cfg, tensors)
-    return seqlib.SeqDeviceModel(head, layers, up, exact=dtype == "float32", max_tokens=max_tokens, max_seqs=max_seqs, page=page)
+    return seqlib.SeqDeviceModel(head, layers, up, exact=dtype == "float32", max_tokens=max_tokens, max_seqs=max_seqs, page=page, cache_bits=cache_bits)
 
 
 # ---------------------------------------------------------------- synthetic checkpoints (tests, bench)

@@ -231,6 +231,7 @@ struct SeqLayer {
 	int rot_kind;          /* with rot_factor > 0: 0: ramp over the pair index between rot_fast and rot_slow turns (cos and sin rescaled too); 1: by wavelength */
 	float rot_low, rot_high;
 	int gate_channels;     /* SEQ_LATENT: 1: a gate per output channel instead of per head */
+	int cache8;            /* SEQ_GQA (one map, vdim = dim, a multiple of 16 up to 256): 1: keys and values are cached in 8 bits (struct SeqCache8; a page of the model is a page of it) */
 };
 
 struct SeqModel {
@@ -273,6 +274,13 @@ int calm_b200_seq_open(void* handle);
 int calm_b200_seq_close(void* handle, int slot);
 int calm_b200_seq_length(void* handle, int slot);
 int calm_b200_seq_free_pages(void* handle);
+/* Sequences that go on in several ways, or end: n_from open slots become n_to; out_slots[i] goes on from what slots[parents[i]] holds.  The first branch of a sequence keeps its slot, the
+ * others share its full pages and get a copy of the page in part filled and of its recurrent state; a sequence that no branch names is closed.  Returns 0, -1 when
+ * slots are missing, -2 when pages are, -3 for a bad slot or parent (nothing has changed then). */
+int calm_b200_seq_branch(void* handle, int n_from, const int* slots, int n_to, const int* parents, int* out_slots);
+/* A cache for max_tokens live tokens from now on: live pages move together at the front of new memory, the old goes back to the device.  Sequences live on.  Returns 0, -2 when
+ * the live pages do not fit, -3 for a bad size, -4 when the device lacks the memory (old and new exist side by side for a moment); nothing has changed then. */
+int calm_b200_seq_resize(void* handle, int max_tokens);
 
 /* One step over a batch: sequence i (slot slots[i]) is fed counts[i] new tokens, packed back to back in `tokens`.
  * `want` lists n_want packed token indices (ascending or not) whose logits are computed; they stay on the device and,
@@ -283,6 +291,9 @@ int calm_b200_seq_step(void* handle, int n_seq, const int* slots, const int* cou
 
 /* argmax (lowest index wins ties) of each row of the last step's logits -> out[n_want] */
 void calm_b200_seq_argmax(void* handle, int* out);
+/* calm_b200_seq_beam_select over rows row0 .. row0 + groups * beams - 1 of the last step's logits: scores [groups][beams] and the results [groups][n] on the host.
+ * Returns 0, or -3 for rows that the step did not want, beams or n outside 1 .. 64. */
+int calm_b200_seq_beams(void* handle, int row0, int groups, int beams, const float* scores, int n, int* tokens, int* parents, float* best);
 /* device pointer of the last step's logits, float[n_want][vocab] */
 const float* calm_b200_seq_device_logits(void* handle);
 
