@@ -8,16 +8,21 @@
 // token); beams are compared in 64 bits by scores + (x - log-sum).  Bound: the logits' way through memory; a single request's few rows, the latency of two
 // launches.
 #include "seqops.cuh"
+#include "tc05.cuh"
+
+#include <stddef.h>
 
 #include <algorithm>
 
 namespace seqops {
 namespace {
 
-constexpr int BM_THREADS = 256, BM_PER = 16, BM_TILE = BM_THREADS * BM_PER; // elements a thread and a CTA take at a time
+constexpr int BM_THREADS = 256, BM_PER = 16; // logits that a thread takes at a time
 constexpr int BM_MAX = 64;                                                  // n
-constexpr int BM_ROOM = 4;                                                  // keys wait for their order until there are more than BM_ROOM n
-constexpr int BM_KEYS = (BM_ROOM + BM_PER) * BM_MAX;                        // those and the ones of a tile that may join them
+constexpr int BM_LIST = 384;                                                // groups of four logits that may hold one of a slice's n highest
+constexpr int BM_KEYS = (1 + BM_PER) * BM_MAX;                              // single candidates, where the list overflows or is put in order
+constexpr int BM_WARPS = BM_THREADS / 32;
+constexpr int BM_RING = 4096;                                               // bytes that a warp has in flight
 constexpr int BM_LISTS = 256;                                               // slices of a group's rows
 constexpr int BM_CAND = 4096;                                               // candidates of a group that the merge compares with one another
 typedef unsigned long long u64;
@@ -51,33 +56,179 @@ __device__ __forceinline__ int rank_in(const u64* list, int c, u64 key) {
 	}
 	return r;
 }
-// The n highest of keys[0 .. c), in order, take the front; returns how many there are.  Keys differ, so their ranks do.
-__device__ int keep_best(u64* keys, int c, int n, u64* sorted) {
+// two fp32 operations in one instruction
+__device__ __forceinline__ u64 pair_of(float x, float y) {
+	u64 r;
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+	return r;
+}
+__device__ __forceinline__ float2 halves(u64 p) {
+	float2 r;
+	asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+	return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+	u64 r;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+	u64 r;
+	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+
+// What a CTA knows of its slice's highest logits.  Logits come in groups of four neighbours; a group whose highest is above tau joins the list (values as they are, so a thread spends
+// a few instructions on it), and now and then the list is cut down to the groups whose highest is among the n highest, the least of which is the new tau.  Only what is left at
+// the end becomes keys.  Tokens come in order, so a later value that equals tau is no candidate.
+struct BeamSlice {
+	alignas(128) unsigned char ring[BM_WARPS][BM_RING];
+	uint64_t full[BM_WARPS][4];
+	float4 quad[BM_LIST];
+	uint32_t token[BM_LIST]; // of the group's first value
+	alignas(16) float top[BM_LIST]; // (read four at a time, keys two at a time)
+	alignas(16) u64 key[BM_KEYS + 2];
+	alignas(16) u64 best[BM_THREADS];
+	u64 sorted[BM_MAX];
+	uint32_t least[BM_THREADS / 32];
+	float red[BM_THREADS / 32];
+	int count;
+	uint32_t low; // order bits
+	u64 bound;
+};
+// The n highest of key[0 .. c), in order, take the front; returns how many there are.  Keys differ, so their ranks do.
+__device__ __noinline__ int keep_best(BeamSlice& b, int c, int n) { // (functions of their own: the loop over the logits keeps its registers)
 	const int tid = threadIdx.x;
-	if (tid == 0 && (c & 1)) keys[c] = 0;
+	if (tid == 0 && (c & 1)) b.key[c] = 0;
 	__syncthreads();
 	for (int i = tid; i < c; i += BM_THREADS) {
-		const u64 k = keys[i];
-		const int r = rank_in(keys, c, k);
-		if (r < n) sorted[r] = k;
+		const u64 k = b.key[i];
+		const int r = rank_in(b.key, c, k);
+		if (r < n) b.sorted[r] = k;
 	}
 	__syncthreads();
 	const int have = min(c, n);
-	if (tid < have) keys[tid] = sorted[tid];
+	if (tid < have) b.key[tid] = b.sorted[tid];
 	__syncthreads();
 	return have;
 }
+// Cuts the list's c groups (c <= BM_LIST) down to those with fewer than n higher ones; returns how many are left, the least of which is b.low.
+__device__ __noinline__ int cut(BeamSlice& b, int c, int n) {
+	constexpr int EACH = (BM_LIST + BM_THREADS - 1) / BM_THREADS;
+	const int tid = threadIdx.x;
+	float4 quad[EACH];
+	uint32_t token[EACH];
+	float mine[EACH];
+#pragma unroll
+	for (int i = 0; i < EACH; ++i) {
+		const int at = i * BM_THREADS + tid;
+		mine[i] = -INFINITY;
+		if (at < c) quad[i] = b.quad[at], token[i] = b.token[at], mine[i] = fmaxf(fmaxf(quad[i].x, quad[i].y), fmaxf(quad[i].z, quad[i].w));
+		if (at < ((c + 3) & ~3)) b.top[at] = mine[i];
+	}
+	if (tid == 0) b.count = 0, b.low = 0xffffffffu;
+	__syncthreads();
+	if (tid < c) {
+		int higher[EACH] = {};
+		const float4* tops = reinterpret_cast<const float4*>(b.top);
+#pragma unroll 4
+		for (int k = 0; k < (c + 3) / 4; ++k) {
+			const float4 t = tops[k];
+#pragma unroll
+			for (int i = 0; i < EACH; ++i) higher[i] += (t.x > mine[i]) + (t.y > mine[i]) + (t.z > mine[i]) + (t.w > mine[i]);
+		}
+#pragma unroll
+		for (int i = 0; i < EACH; ++i)
+			if (i * BM_THREADS + tid < c && higher[i] < n) {
+				const int at = atomicAdd(&b.count, 1);
+				b.quad[at] = quad[i], b.token[at] = token[i];
+				atomicMin(&b.low, order_bits(mine[i]));
+			}
+	}
+	__syncthreads();
+	return b.count;
+}
+// Keys of the list's c groups, the n highest in order; returns how many there are.
+__device__ __noinline__ int list_keys(BeamSlice& b, int c, int n) {
+	const int tid = threadIdx.x;
+	int k = 0;
+	for (int first = 0; first < c; first += BM_MAX) { // 4 BM_MAX values at a time beside the n kept ones
+		if (tid == 0) b.count = k;
+		__syncthreads();
+		if (tid < min(c - first, BM_MAX)) {
+			const float4 q = b.quad[first + tid];
+			const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+			for (int e = 0; e < 4; ++e)
+				if (v[e] > -INFINITY) b.key[atomicAdd(&b.count, 1)] = beam_key(v[e], b.token[first + tid] + e);
+		}
+		__syncthreads();
+		k = keep_best(b, b.count, n);
+	}
+	return k;
+}
 
+// More groups than the list takes (rows in rising order, rows of few different values): the c groups listed before, and the tiles [v0, stop) since then once more, as
+// single candidates.  The n-th highest of the threads' highest values is no higher than the tile's n-th, and only n threads hold anything from it on: at most n * BM_PER values,
+// whatever the tile looks like.  The n highest become the list, as groups of one; returns how many there are.
 template <typename T>
-__global__ void __launch_bounds__(BM_THREADS) k_beam_slice(const BeamArgs a) {
+__device__ __noinline__ int slow_tiles(BeamSlice& b, const uint4* base, unsigned v0, unsigned stop, unsigned end, unsigned shift, unsigned total, int c, int n) {
 	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE;
-	constexpr float L2E = 1.4426950408889634f;
-	__shared__ __align__(16) u64 keys[BM_KEYS + 1], best[BM_THREADS], sorted[BM_MAX];
-	__shared__ int count;
-	__shared__ u64 bound;
-	__shared__ float red_m[BM_THREADS / 32], red_s[BM_THREADS / 32];
+	const int tid = threadIdx.x;
+	int k = list_keys(b, c, n);
+	for (; v0 < stop; v0 += NV * BM_THREADS) {
+		u64 key[BM_PER], mine = 0;
+#pragma unroll
+		for (int j = 0; j < NV; ++j) {
+			const unsigned o = v0 + j * BM_THREADS + tid;
+			uint4 w = make_uint4(0, 0, 0, 0);
+			if (o < end) w = ldg_stream(base + o);
+			float v[VE];
+			unpack16<T>(w, v);
+#pragma unroll
+			for (int e = 0; e < VE; ++e) {
+				const unsigned at = o * VE + e;
+				key[j * VE + e] = o < end && at >= shift && at < total ? beam_key(v[e], at - shift) : 0;
+				mine = max(mine, key[j * VE + e]);
+			}
+		}
+		b.best[tid] = mine;
+		if (tid == 0) b.bound = 1, b.count = k; // fewer than n threads with values: everything
+		const int valid = __syncthreads_count(mine != 0);
+		if (valid >= n && mine && rank_in(b.best, BM_THREADS, mine) == n - 1) b.bound = mine;
+		__syncthreads();
+		if (mine >= b.bound) {
+#pragma unroll
+			for (int i = 0; i < BM_PER; ++i)
+				if (key[i] >= b.bound) b.key[atomicAdd(&b.count, 1)] = key[i];
+		}
+		__syncthreads();
+		k = keep_best(b, b.count, n);
+	}
+	if (tid < k) {
+		b.quad[tid] = make_float4(order_value((uint32_t)(b.key[tid] >> 32)), -INFINITY, -INFINITY, -INFINITY);
+		b.token[tid] = ~(uint32_t)b.key[tid];
+	}
+	return k;
+}
+
+// Per logit: a maximum, a difference, a product, an exponential, an addition (with a fused multiply-add against the maximum times log2(e) a row of the type's lowest values, whose
+// product is infinite, would have no sum).
+constexpr float BM_L2E = 1.4426950408889634f;
+static_assert(offsetof(BeamSlice, top) % 16 == 0 && offsetof(BeamSlice, key) % 16 == 0 && offsetof(BeamSlice, best) % 16 == 0, "read 16 bytes at a time");
+template <typename T>
+__global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) {
+	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE, QUADS = BM_PER / 4, STAGES = BM_RING / (NV * 512);
+	constexpr unsigned WSTEP = NV * 32, STEP = WSTEP * BM_WARPS; // vectors of a warp's part of a tile, of a tile
+	extern __shared__ __align__(128) unsigned char slice_sm[];
+	BeamSlice& b = *reinterpret_cast<BeamSlice*>(slice_sm);
 	pdl_launch_next();
-	const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y, n = a.n;
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, slice = blockIdx.x, row = blockIdx.y, n = a.n;
 	u64* const out = a.keys + ((size_t)row * a.slices + slice) * n;
 	if (!(a.scores[row] > -INFINITY)) { // this beam is not there
 		for (int i = tid; i < n; i += BM_THREADS) out[i] = 0;
@@ -86,111 +237,150 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_slice(const BeamArgs a) {
 	}
 	// the row from the 16-byte boundary at or before its first element: elements [shift, total) of `base` are its own
 	const T* p = (const T*)a.logits + (long long)(row / a.beams) * a.group_stride + (long long)(row % a.beams) * a.row_stride;
-	const int shift = (int)(((uintptr_t)p & 15) / sizeof(T));
-	const T* base = p - shift;
-	const long long total = (long long)a.vocab + shift;
-	const long long vectors = (total + VE - 1) / VE, each = (vectors + a.slices - 1) / a.slices;
-	const long long begin = min(vectors, slice * each) * VE, end = min(total, (slice + 1) * each * VE);
-	float m = -INFINITY, s = 0.f, tau = -INFINITY; // the thread's maximum and sum; a later token counts only above tau
-	int c = 0;                                     // keys kept
-	bool first = true;
-	for (long long t0 = begin; t0 < end; t0 += BM_TILE) {
-		float v[BM_PER];
-		uint4 w[NV];
-#pragma unroll
-		for (int j = 0; j < NV; ++j) {
-			const long long o = t0 + (long long)(j * BM_THREADS + tid) * VE;
-			if (o < end) w[j] = ldg_stream(reinterpret_cast<const uint4*>(base + o));
+	const unsigned shift = (unsigned)(((uintptr_t)p & 15) / sizeof(T));
+	const uint4* const base = reinterpret_cast<const uint4*>(p - shift);
+	const unsigned total = a.vocab + shift, vectors = (total + VE - 1) / VE, each = (vectors + a.slices - 1) / a.slices;
+	const unsigned begin = min(vectors, slice * each), end = min(vectors, begin + each); // in vectors
+	// Each warp has a ring of its own, filled by bulk copies that run on while the block looks at its list.
+	uint64_t* const full = b.full[warp];
+	unsigned asked = begin + warp * WSTEP; // the warp's part of the next tile to request
+	const uint64_t policy = l2_policy_evict_first();
+	auto request = [&](int stage) {        // one lane
+		if (asked < end) {
+			const uint32_t bytes = min(end - asked, WSTEP) * 16;
+			mbar_expect_tx(full + stage, bytes);
+			tma_load_1d_hint(b.ring[warp] + stage * (NV * 512), base + asked, bytes, full + stage, policy);
 		}
+	};
+	if (lane == 0) {
 #pragma unroll
-		for (int j = 0; j < NV; ++j) {
-			const long long o = t0 + (long long)(j * BM_THREADS + tid) * VE;
-			float u[VE];
-			unpack16<T>(w[j], u);
-			const bool inside = o >= shift && o + VE <= end;
-#pragma unroll
-			for (int e = 0; e < VE; ++e) v[j * VE + e] = inside || (o + e >= shift && o + e < end) ? fmaxf(u[e], -INFINITY) : -INFINITY; // (fmaxf: a NaN becomes -inf)
-		}
-		float top = v[0];
-#pragma unroll
-		for (int i = 1; i < BM_PER; ++i) top = fmaxf(top, v[i]);
-		if (top > m) {
-			if (m > -INFINITY) s *= top == INFINITY ? 0.f : exp2f((m - top) * L2E);
-			m = top;
-		}
-		if (m < INFINITY) {
-			if (m > -INFINITY) {
-				float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-				for (int i = 0; i < BM_PER; ++i) part[i & 3] += exp2f((v[i] - m) * L2E);
-				s += (part[0] + part[1]) + (part[2] + part[3]);
-			}
-		} else {
-#pragma unroll
-			for (int i = 0; i < BM_PER; ++i) s += v[i] == INFINITY ? 1.f : 0.f;
-		}
-		auto index = [&](int i) { return (uint32_t)(t0 + (long long)((i / VE) * BM_THREADS + tid) * VE + i % VE - shift); };
-		if (!__syncthreads_or(top > tau)) continue;
-		bool pick = first;
-		if (!first) { // few values pass tau: they join the kept ones, unless there is no room for all
-			if (tid == 0) count = c;
-			__syncthreads();
-			if (top > tau) {
-#pragma unroll
-				for (int i = 0; i < BM_PER; ++i)
-					if (v[i] > tau) {
-						const int at = atomicAdd(&count, 1);
-						if (at < BM_KEYS) keys[at] = beam_key(v[i], index(i));
-					}
-			}
-			__syncthreads();
-			pick = count > BM_KEYS; // what was written behind the kept keys is forgotten
-			if (!pick) c = count;
-			__syncthreads();
-		}
-		if (pick) {
-			// The n-th highest of the threads' highest values is no higher than the tile's n-th, and only n threads hold anything from it on: at most
-			// n * BM_PER values, whatever the tile looks like.
-			u64 mine = 0;
-#pragma unroll
-			for (int i = 0; i < BM_PER; ++i) mine = max(mine, beam_key(v[i], index(i)));
-			best[tid] = mine;
-			if (tid == 0) bound = 1, count = c; // fewer than n threads with values: everything
-			const int valid = __syncthreads_count(mine != 0);
-			if (valid >= n && mine && rank_in(best, BM_THREADS, mine) == n - 1) bound = mine;
-			__syncthreads();
-			if (mine >= bound) {
-#pragma unroll
-				for (int i = 0; i < BM_PER; ++i) {
-					const u64 k = beam_key(v[i], index(i));
-					if (k >= bound) keys[atomicAdd(&count, 1)] = k;
-				}
-			}
-			__syncthreads();
-			c = count;
-			first = false;
-		}
-		if (pick || c > BM_ROOM * n) {
-			c = keep_best(keys, c, n, sorted);
-			tau = c == n ? order_value((uint32_t)(keys[n - 1] >> 32)) : -INFINITY;
-		}
+		for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1);
+		mbar_init_fence();
 	}
-	c = keep_best(keys, c, n, sorted);
-	for (int i = tid; i < n; i += BM_THREADS) out[i] = i < c ? keys[i] : 0;
-	const float wm = warp_max(m);
-	if ((tid & 31) == 0) red_m[tid >> 5] = wm;
-	__syncthreads();
-	float bm = red_m[0];
 #pragma unroll
-	for (int i = 1; i < BM_THREADS / 32; ++i) bm = fmaxf(bm, red_m[i]);
-	const float ws = warp_sum(m == bm ? s : m > -INFINITY ? s * exp2f((m - bm) * L2E) : 0.f);
-	if ((tid & 31) == 0) red_s[tid >> 5] = ws;
+	for (int i = 0; i < STAGES; ++i) {
+		if (lane == 0) request(i);
+		asked += STEP;
+	}
+	if (tid == 0) b.count = 0;
+	__syncwarp();
+	float m = -INFINITY, s = 0.f, tau = -INFINITY; // the thread's maximum and sum; a later group counts only above tau
+	int c = 0, stage = 0;                          // groups listed
+	uint32_t parity = 0;
+	bool lost = false; // a copy never came
+	auto spread = [&](unsigned v0, const uint4 (&w)[NV], float (&v)[BM_PER]) { // the tile's logits
+#pragma unroll
+		for (int j = 0; j < NV; ++j) unpack16<T>(w[j], *reinterpret_cast<float(*)[VE]>(v + j * VE));
+		if (v0 * VE < shift || v0 + STEP > end || (v0 + STEP) * VE > total) { // the row's first and last tile: places outside it
+#pragma unroll
+			for (int i = 0; i < BM_PER; ++i) {
+				const unsigned o = v0 + warp * WSTEP + (i / VE) * 32 + lane, e = o * VE + i % VE;
+				if (o >= end || e < shift || e >= total) v[i] = -INFINITY;
+			}
+		}
+	};
+	auto token = [&](unsigned v0, int i) { return (v0 + warp * WSTEP + (i / VE) * 32 + lane) * VE + i % VE - shift; };
+	unsigned next = begin, size = 1; // tiles between two looks at the list: more once few groups join it
+	while (next < end) {
+		const unsigned g0 = next, stop = g0 + size * STEP;
+		for (; next < end && next < stop; next += STEP) {
+			const unsigned v0 = next;
+			uint4 w[NV];
+			if (v0 + warp * WSTEP < end && !lost) {
+				lost = !mbar_wait_warp(full + stage, parity);
+				const uint4* const src = reinterpret_cast<const uint4*>(b.ring[warp] + stage * (NV * 512)) + lane;
+#pragma unroll
+				for (int j = 0; j < NV; ++j) w[j] = src[j * 32];
+			}
+			float v[BM_PER];
+			spread(v0, w, v);
+			__syncwarp(); // all lanes have read
+			if (lane == 0 && !lost) request(stage);
+			asked += STEP;
+			if (++stage == STAGES) stage = 0, parity ^= 1;
+			float quad[QUADS], top = -INFINITY; // (a NaN is passed over)
+#pragma unroll
+			for (int i = 0; i < QUADS; ++i) quad[i] = fmaxf(fmaxf(fmaxf(v[4 * i], v[4 * i + 1]), v[4 * i + 2]), v[4 * i + 3]);
+#pragma unroll
+			for (int i = 0; i < QUADS; i += 2) top = fmaxf(fmaxf(top, quad[i]), quad[i + 1]);
+			if (top > m) s = m > -INFINITY && top < INFINITY ? s * ex2((m - top) * BM_L2E) : 0.f, m = top;
+			u64 part[2] = {0, 0};
+			const u64 down = pair_of(-m, -m), l2e = pair_of(BM_L2E, BM_L2E);
+#pragma unroll
+			for (int i = 0; i < BM_PER / 2; ++i) {
+				const float2 y = halves(mul2(add2(pair_of(v[2 * i], v[2 * i + 1]), down), l2e));
+				part[i & 1] = add2(part[i & 1], pair_of(ex2(y.x), ex2(y.y)));
+			}
+			const float2 both = halves(add2(part[0], part[1]));
+			float sum = both.x + both.y;
+			if (!(sum < INFINITY)) { // a NaN among the logits, nothing but -inf so far, or +inf: rare
+				sum = 0.f;
+				if (m > -INFINITY)
+#pragma unroll
+					for (int i = 0; i < BM_PER; ++i) sum += m == INFINITY ? (v[i] == INFINITY ? 1.f : 0.f) : v[i] > -INFINITY ? ex2((v[i] - m) * BM_L2E) : 0.f;
+			}
+			s += sum;
+			if (v0 == begin) {
+				// where to start: the least, over the warps with logits, of the k-th highest of a warp's lanes, k warps >= n, has n values at or above it
+				uint32_t u = top > -INFINITY ? order_bits(top) : 0, x = 0;
+				const int warps = min(BM_WARPS, (int)((end - begin + WSTEP - 1) / WSTEP));
+				for (int k = (n + warps - 1) / warps; k > 0; --k) {
+					x = __reduce_max_sync(0xffffffffu, u);
+					if (__ffs(__ballot_sync(0xffffffffu, u == x)) - 1 == lane) u = 0;
+				}
+				if (lane == 0) b.least[warp] = x;
+				__syncthreads();
+				x = b.least[0];
+#pragma unroll
+				for (int i = 1; i < BM_WARPS; ++i)
+					if (i < warps) x = min(x, b.least[i]);
+				if (x) tau = nextafterf(order_value(x), -INFINITY);
+			}
+			if (top > tau)
+#pragma unroll
+				for (int q = 0; q < QUADS; ++q)
+					if (quad[q] > tau) {
+						const int at = atomicAdd(&b.count, 1);
+						if (at < BM_LIST) {
+							b.quad[at] = make_float4(fmaxf(v[4 * q], -INFINITY), fmaxf(v[4 * q + 1], -INFINITY), fmaxf(v[4 * q + 2], -INFINITY), fmaxf(v[4 * q + 3], -INFINITY));
+							b.token[at] = token(v0, 4 * q);
+						}
+					}
+		}
+		__syncthreads();
+		const int found = b.count;
+		__syncthreads();
+		if (found <= BM_LIST) {
+			c = found;
+			if (c > n) c = cut(b, c, n), tau = order_value(b.low);
+		} else {
+			const int k = slow_tiles<T>(b, base, g0, min(stop, end), end, shift, total, c, n);
+			c = k;
+			if (k == n) tau = order_value((uint32_t)(b.key[n - 1] >> 32));
+		}
+		__syncthreads();
+		if (tid == 0) b.count = c;
+		__syncthreads();
+		size = next == begin + STEP ? 3 : min(4 * size, 24); // 1, 3, 12, 24, ...
+	}
+	if (lost) mbar_wait_bounded(full + stage, parity); // (a copy that comes late lands in memory that is still the block's)
+	const int k = list_keys(b, c, n);
+	for (int i = tid; i < n; i += BM_THREADS) out[i] = i < k ? b.key[i] : 0;
+	const float wm = warp_max(m);
+	if (lane == 0) b.red[warp] = wm;
+	const bool broken = __syncthreads_or(lost);
+	float bm = b.red[0];
+#pragma unroll
+	for (int i = 1; i < BM_WARPS; ++i) bm = fmaxf(bm, b.red[i]);
+	const float ws = warp_sum(m == bm ? s : m > -INFINITY && bm < INFINITY ? s * ex2((m - bm) * BM_L2E) : 0.f);
+	__syncthreads();
+	if (lane == 0) b.red[warp] = ws;
 	__syncthreads();
 	if (tid == 0) {
-		float sum = red_s[0];
+		float sum = b.red[0];
 #pragma unroll
-		for (int i = 1; i < BM_THREADS / 32; ++i) sum += red_s[i];
-		a.sums[(size_t)row * a.slices + slice] = make_float2(bm, bm > -INFINITY ? sum : 0.f);
+		for (int i = 1; i < BM_WARPS; ++i) sum += b.red[i];
+		a.sums[(size_t)row * a.slices + slice] = make_float2(bm, broken ? NAN : bm > -INFINITY ? sum : 0.f); // (without a sum the row has no candidates)
 	}
 }
 
@@ -269,10 +459,10 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	for (int e = c + tid; e < n; e += BM_THREADS) a.tokens[base + e] = a.parents[base + e] = -1, a.best[base + e] = -INFINITY;
 }
 
-// Slices of a row: a tile each where rows are few, as many as keep all CTAs of one wave resident where they are many.
+// Slices of a row: 4096 logits each where rows are few, as many as two CTAs an SM hold at a time where they are many.
 int beam_slices(int groups, int beams, int vocab) {
-	const int rows = groups * beams, tiles = cdiv(vocab, BM_TILE);
-	return std::max(1, std::min({tiles, cdiv(148 * 6, rows), BM_LISTS / beams}));
+	const int rows = groups * beams, most = cdiv(vocab, 4096);
+	return std::max(1, std::min({most, 148 * 2 / rows, BM_LISTS / beams}));
 }
 size_t beam_keys(int groups, int beams, int vocab, int n) { return ((size_t)groups * beams * beam_slices(groups, beams, vocab) * n * sizeof(u64) + 15) & ~(size_t)15; }
 
@@ -310,7 +500,8 @@ extern "C" int calm_b200_seq_beam_select(const struct SeqBeam* q, void* stream) 
 	const cudaStream_t st = (cudaStream_t)stream;
 	const dim3 grid(a.slices, q->groups * q->beams);
 	auto kernel = q->type == SEQ_F32 ? k_beam_slice<float> : q->type == SEQ_BF16 ? k_beam_slice<__nv_bfloat16> : k_beam_slice<__half>;
-	cudaError_t e = launch(st, false, 1, kernel, grid, dim3(BM_THREADS), 0, a);
+	cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BeamSlice));
+	if (e == cudaSuccess) e = launch(st, false, 1, kernel, grid, dim3(BM_THREADS), sizeof(BeamSlice), a);
 	if (e != cudaSuccess) return failed("beam", e);
 	if ((e = cudaFuncSetAttribute(k_beam_merge, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BeamCand))) != cudaSuccess) return failed("beam", e);
 	e = launch(st, true, 1, k_beam_merge, dim3(q->groups), dim3(BM_THREADS), sizeof(BeamCand), a);
