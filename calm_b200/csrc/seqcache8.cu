@@ -18,6 +18,7 @@ struct C8 {
 	float *ks, *vs;
 	const int* table;
 	int pages, heads, page, dim, slots, table_pages;
+	int page_shift; // log2 of page, -1: no power of two
 	const int *start, *count, *slot, *pos0;
 };
 constexpr int C8_LEAST = -64; // exponent of the smallest scale
@@ -33,6 +34,17 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 	const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
 	return lo | hi << 16;
+}
+__device__ __forceinline__ int page_index(const C8& c, int pos) { return c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page; }
+__device__ __forceinline__ int page_row(const C8& c, int pos) { return c.page_shift >= 0 ? pos & (c.page - 1) : pos % c.page; }
+__device__ __forceinline__ float ex2(float x) {
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+// four codes as two pairs of fp16
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+	asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
 }
 // two codes (the lower byte first) as fp16
 __device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t codes) {
@@ -118,13 +130,16 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 
 // ---------------------------------------------------------------- attention
 // The rows of a CTA are 16 pairs (token, query head) of one sequence that read one key head, so a key is read once for all of them: row i of a sequence's tile is token
-// i / group, head i % group of the group.  Each warp walks its own chunks of 32 keys with a running maximum and sum of its own (no barrier between warps until the end),
+// i / group, head i % group of the group.  Each warp walks its own chunks of 32 keys with a running reference and sum of its own (no barrier between warps until the end),
 // fed by a ring of asynchronous copies; codes become fp16 in registers on their way into m16n8k16 products.  An e4m3 code is exact in fp16; scales do not enter the
-// products: a key's scale multiplies its scores, a value's scale s joins the exponent, w_j = exp2(z_j), z_j = log2(e) score_j + log2 s_j, whose running maximum bounds
-// the weights that are rounded to fp16; the denominator sums w_j / s_j.
+// products: a key's scale multiplies its scores, a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are
+// rounded to fp16 at 2^15 or less; the denominator sums w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z:
+// almost only in a warp's first chunks.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
+constexpr int AT_SHARES = 64; // of a tile's keys at most
 constexpr float AT_LOG2E = 1.4426950408889634f;
-constexpr int AT_LIFT = 15; // the largest query of a row and the largest weight stand at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of them
+constexpr int AT_LIFT = 15;                // the largest query of a tile stands at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of it
+constexpr float AT_MOST = 15.f, AT_SET = 10.f; // weights: at most 2^15, the largest at 2^10 or more
 
 struct Attend {
 	const void* q;
@@ -136,24 +151,27 @@ struct Attend {
 	int window, keep_first, chunk;
 	const float *sinks, *slopes, *gate;
 	long long gate_row, gate_head, gate_dim;
-	int shares;
-	float* part; // [rows][heads][shares][dim + 2]: sum, running maximum, denominator
+	int shares, each; // shares of a tile's keys at most, chunks of each
+	float* part;      // [rows][heads][shares][dim + 2]: sum, reference, denominator
 };
 
 template <int D>
 struct AtStage { // a warp's chunk
 	uint8_t k[AT_KEYS * D], v[AT_KEYS * D];
-	float ks[AT_KEYS], vs[AT_KEYS];
+	float ks[AT_KEYS], vs[AT_KEYS], ov[AT_KEYS]; // scales as they come; then factors on scores, log2 of the value scales and the inverse of those
 	uint32_t seen; // keys that are there
 	uint32_t pad[3];
 };
 template <int D>
-__host__ __device__ constexpr int at_stages() { return D == 64 ? 4 : D == 128 ? 3 : 2; }
+__host__ __device__ constexpr int at_stages() { return D == 64 ? 3 : 2; }
 template <int D, bool SPLIT>
 constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 16 * D * 2 + (size_t)AT_WARPS * at_stages<D>() * sizeof(AtStage<D>); }
 
-__device__ __forceinline__ void cp16(void* dst, const void* src, bool there) { // zeros where there is nothing to read
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) { // zeros where there is nothing to read
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp4(void* dst, const void* src, bool there) {
 	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
@@ -175,60 +193,84 @@ __device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) { /
 template <int D>
 __device__ __forceinline__ int at_place(int r, int piece) { return piece ^ (D == 64 ? (r >> 1) & 3 : r & 7); }
 
-struct AtSpan { // the positions that a tile of rows sees, in order: [0, kept), then [lo, last]
-	int lo, kept, total;
+// the positions that a tile of rows sees, in order: [0, kept), then [lo, last]
+struct AtSpan {
+	int first, last, lo, kept, total, chunks;
 };
 __device__ __forceinline__ int at_low(const Attend& a, int pos) {
 	int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
 	return a.chunk > 0 ? max(lo, pos / a.chunk * a.chunk) : lo;
 }
+__device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int rows, bool known) {
+	AtSpan s;
+	s.first = p0 + row0 / a.group, s.last = p0 + (row0 + rows - 1) / a.group;
+	s.lo = at_low(a, s.first), s.kept = min(a.keep_first, s.lo);
+	s.total = known ? s.kept + s.last - s.lo + 1 : 0;
+	s.chunks = (s.total + AT_KEYS - 1) / AT_KEYS;
+	return s;
+}
 
-template <int D, typename QT, typename OT>
-__global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const Attend a) {
-	constexpr bool SPLIT = sizeof(QT) == 4;
+// EXTRA: a soft cap or slopes
+template <int D, typename QT, typename OT, bool EXTRA>
+__global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(const C8 c, const Attend a) {
+	constexpr bool SPLIT = sizeof(QT) == 4, KEEP = !SPLIT && D <= 128; // KEEP: the queries' fragments stay in registers
 	constexpr int ST = at_stages<D>(), KS = D / 16, NT = D / 8, PIECES = D / 16;
 	extern __shared__ __align__(128) unsigned char at_sm[];
 	uint4* const qf = reinterpret_cast<uint4*>(at_sm); // A fragments [KS][32], then the remainders'
 	AtStage<D>* const ring = reinterpret_cast<AtStage<D>*>(at_sm + (size_t)(SPLIT ? 2 : 1) * 16 * D * 2);
-	__shared__ float qscale[16], fold_m[AT_WARPS][16], fold_l[AT_WARPS][16];
+	__shared__ float fold_m[AT_WARPS][16], fold_l[AT_WARPS][16], qtop[AT_WARPS];
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 	const int b = blockIdx.z, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = blockIdx.x;
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * 16 >= (long long)n * a.group) return;
-	const bool known = (unsigned)slot < (unsigned)c.slots;
 	const int row0 = tile * 16, rows = (int)min(16LL, (long long)n * a.group - row0);
-	const int first = p0 + row0 / a.group, last = p0 + (row0 + rows - 1) / a.group; // positions of the tile
-	const int lo = at_low(a, first), kept = min(a.keep_first, lo), total = known ? kept + last - lo + 1 : 0;
-	const int chunks = (total + AT_KEYS - 1) / AT_KEYS, each = (chunks + a.shares - 1) / a.shares;
-	const int begin = min(chunks, share * each), end = min(chunks, begin + each);
+	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
+	const int lo = sp.lo, kept = sp.kept, total = sp.total;
+	const int begin = share * a.each, end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
+	if (share > 0 && begin >= sp.chunks) return;
 	const int H = c.heads, dim = c.dim;
 
 	auto position = [&](int j) { return j < kept ? j : lo + (j - kept); };
 	auto page_of = [&](int chunk) { // the page of this lane's key, -1: none
 		const int j = chunk * AT_KEYS + lane;
 		if (chunk >= end || j >= total) return -1;
-		const int at = position(j) / c.page;
+		const int at = page_index(c, position(j));
 		if (at >= c.table_pages) return -1;
 		const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
 		return (unsigned)id < (unsigned)c.pages ? id : -1;
 	};
 	AtStage<D>* const mine = ring + warp * ST;
 	int next = begin + warp, next_page = page_of(next), stage_in = 0; // the chunk to request, its page
+	const int piece = lane % PIECES, prow = lane / PIECES;            // which piece of which row of a group of 32 pieces this lane copies
+	uint32_t swizzle[2];                                              // where, for rows that differ by 4 (by 2 where rows have 16 pieces: four of those)
+#pragma unroll
+	for (int i = 0; i < 2; ++i) swizzle[i] = at_place<D>(prow + i * 4, piece) * 16;
 	auto request = [&]() {
 		if (next < end) {
 			AtStage<D>& s = mine[stage_in];
-			const int at = position(min(next * AT_KEYS + lane, total - 1)) % c.page, id = next_page;
+			const int id = next_page;
 			const uint32_t seen = __ballot_sync(0xffffffffu, id >= 0);
-			const long long unit = (long long)max(id, 0) * H + kvh, off = (unit * c.page + at) * dim;
+			const int unit = max(id, 0) * H + kvh, row = unit * c.page + page_row(c, position(min(next * AT_KEYS + lane, total - 1))); // (rows of a pool: under 2^31)
 			if (lane == 0) s.seen = seen;
 			cp4(s.ks + lane, c.ks + unit, id >= 0), cp4(s.vs + lane, c.vs + unit, id >= 0);
+			const uint32_t kd = smem_u32(s.k) + prow * D, vd = smem_u32(s.v) + prow * D;
+			const uint8_t *const kp = c.k + piece * 16, *const vp = c.v + piece * 16;
+			if (seen == 0xffffffffu && dim == D) {
 #pragma unroll
-			for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
-				const int r = (i * 32 + lane) / PIECES, piece = (i * 32 + lane) % PIECES;
-				const long long o = __shfl_sync(0xffffffffu, off, r) + piece * 16;
-				const bool there = (seen >> r & 1) && piece * 16 < dim;
-				const int place = (r * PIECES + at_place<D>(r, piece)) * 16;
-				cp16(s.k + place, c.k + (there ? o : 0), there), cp16(s.v + place, c.v + (there ? o : 0), there);
+				for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
+					const long long o = (long long)__shfl_sync(0xffffffffu, row, i * (32 / PIECES) + prow) * D;
+					const uint32_t place = i * (32 / PIECES) * D + (D == 128 ? swizzle[i & 1] : at_place<D>(i * (32 / PIECES) + prow, piece) * 16);
+					cp16(kd + place, kp + o), cp16(vd + place, vp + o);
+				}
+			} else {
+#pragma unroll
+				for (int i = 0; i < PIECES; ++i) {
+					const int r = i * (32 / PIECES) + prow;
+					const long long o = (long long)__shfl_sync(0xffffffffu, row, r) * dim;
+					const bool there = (seen >> r & 1) && piece * 16 < dim;
+					const uint32_t place = i * (32 / PIECES) * D + at_place<D>(r, piece) * 16;
+					cp16(kd + place, there ? kp + o : c.k, there), cp16(vd + place, there ? vp + o : c.v, there);
+				}
 			}
 			stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
 			next += AT_WARPS, next_page = page_of(next);
@@ -238,52 +280,66 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 #pragma unroll
 	for (int i = 0; i < ST - 1; ++i) request();
 
-	// queries as A fragments: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a thread's codes of a key lie side by side)
-	for (int r = warp; r < 16; r += AT_WARPS) {
-		const QT* src = (const QT*)a.q + (long long)(start + (row0 + min(r, rows - 1)) / a.group) * a.q_row + (long long)(kvh * a.group + (row0 + min(r, rows - 1)) % a.group) * a.q_head;
-		float x[D / 32], top = 0.f;
+	// Queries as A fragments, times a power of two that is the tile's: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
+	// thread's codes of a key lie side by side).
+	float x[16 / AT_WARPS][D / 32], top = 0.f;
 #pragma unroll
-		for (int i = 0; i < D / 32; ++i) {
-			const int d = i * 32 + lane;
-			x[i] = r < rows && d < dim ? as_f32(src[d]) : 0.f;
-			top = fmaxf(top, fabsf(x[i]));
+	for (int i = 0; i < 16 / AT_WARPS; ++i) {
+		const int r = i * AT_WARPS + warp, rr = row0 + min(r, rows - 1);
+		const QT* src = (const QT*)a.q + (long long)(start + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head;
+#pragma unroll
+		for (int k = 0; k < D / 32; ++k) {
+			const int d = k * 32 + lane;
+			x[i][k] = r < rows && d < dim ? as_f32(src[d]) : 0.f;
+			top = fmaxf(top, fabsf(x[i][k]));
 		}
-		top = warp_max(top);
-		const int e = (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT; // the row's largest comes to 2^AT_LIFT
-		const float down = pow2f(-e);
+	}
+	top = warp_max(top);
+	if (lane == 0) qtop[warp] = top;
+	__syncthreads();
 #pragma unroll
-		for (int i = 0; i < D / 32; ++i) {
-			const int d = i * 32 + lane, dt = d / (D / 4), ds = d % (D / 4) / 4, de = d & 3;
+	for (int i = 0; i < AT_WARPS; ++i) top = fmaxf(top, qtop[i]);
+	const int qe = (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT; // top = m 2^(qe + AT_LIFT)
+	const float qdown = pow2f(-qe);
+#pragma unroll
+	for (int i = 0; i < 16 / AT_WARPS; ++i) {
+		const int r = i * AT_WARPS + warp;
+#pragma unroll
+		for (int k = 0; k < D / 32; ++k) {
+			const int d = k * 32 + lane, dt = d / (D / 4), ds = d % (D / 4) / 4, de = d & 3;
 			const int at = ((ds * 32 + (r & 7) * 4 + dt) * 4 + (de >> 1) * 2 + (r >> 3)) * 2 + (de & 1);
-			const float y = x[i] * down;
+			const float y = x[i][k] * qdown;
 			const __half hi = __float2half_rn(y);
 			reinterpret_cast<__half*>(qf)[at] = hi;
 			if (SPLIT) reinterpret_cast<__half*>(qf + KS * 32)[at] = __float2half_rn(y - __half2float(hi));
 		}
-		if (lane == 0) qscale[r] = a.scale * pow2f(e);
 	}
 	__syncthreads();
+	const float qscale = a.scale * pow2f(qe) * (EXTRA ? 1.f : AT_LOG2E);
+	uint4 qr[KEEP ? KS : 1];
+	if (KEEP) {
+#pragma unroll
+		for (int i = 0; i < KS; ++i) qr[i] = qf[i * 32 + lane];
+	}
 
-	float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // rows g and g + 8
+	float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // rows g and g + 8; m: the reference r
 #pragma unroll
 	for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-	int rpos[2], rlo[2];
-	float rs[2], slope[2];
-#pragma unroll
-	for (int i = 0; i < 2; ++i) {
-		const int r = g + 8 * i;
-		rpos[i] = r < rows ? p0 + (row0 + r) / a.group : -1, rlo[i] = r < rows ? at_low(a, rpos[i]) : 0, rs[i] = qscale[r];
-		slope[i] = a.slopes && r < rows ? a.slopes[kvh * a.group + (row0 + r) % a.group] : 0.f;
-	}
-	const int wide = at_low(a, last); // from here on, and before `first`, every row sees every key
+	const int rpos[2] = {g < rows ? p0 + (row0 + g) / a.group : -1, g + 8 < rows ? p0 + (row0 + g + 8) / a.group : -1};
+	const int wide = at_low(a, sp.last); // from here on, and up to `first`, every row sees every key
 
 	int stage = 0;
 	for (int chunk = begin + warp; chunk < end; chunk += AT_WARPS) {
 		asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
 		__syncwarp();
 		request(); // into the stage that was used up last
-		const AtStage<D>& s = mine[stage];
+		AtStage<D>& s = mine[stage];
 		stage = stage + 1 == ST ? 0 : stage + 1;
+		{ // a lane's key: factor on its scores, log2 and inverse of its value's scale
+			const float vscale = s.vs[lane];
+			const int ve = max((int)(__float_as_uint(vscale) >> 23) - 127, -126);
+			s.ks[lane] *= qscale, s.vs[lane] = (float)ve, s.ov[lane] = pow2f(-ve);
+		}
 		float z[4][4];
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
@@ -292,60 +348,68 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 			uint32_t w[KS];
 #pragma unroll
 			for (int i = 0; i < (KS + 3) / 4; ++i) {
-				const uint4 x = *reinterpret_cast<const uint4*>(s.k + (r * PIECES + at_place<D>(r, t * (PIECES / 4) + i)) * 16);
-				w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+				const uint4 y = *reinterpret_cast<const uint4*>(s.k + (r * PIECES + at_place<D>(r, t * (PIECES / 4) + i)) * 16);
+				w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
 			}
 #pragma unroll
 			for (int i = 0; i < KS; ++i) {
-				const uint32_t b0 = e4m3x2_to_f16(w[i]), b1 = e4m3x2_to_f16(w[i] >> 16);
-				mma_f16(z[j], qf[i * 32 + lane], b0, b1);
+				uint32_t b0, b1;
+				e4m3x4_to_f16(w[i], b0, b1);
+				mma_f16(z[j], KEEP ? qr[i] : qf[i * 32 + lane], b0, b1);
 				if (SPLIT) mma_f16(z[j], qf[(KS + i) * 32 + lane], b0, b1);
 			}
 		}
+		__syncwarp(); // the factors
 		// scores with the value's scale in the exponent
 		const uint32_t seen = s.seen;
 		const int j0 = chunk * AT_KEYS;
-		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= first;
-		float over[8]; // 1 / value scale
-		float top[2] = {-INFINITY, -INFINITY};
+		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= sp.first;
+		float tops[2] = {-INFINITY, -INFINITY};
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			const float2 ks = *reinterpret_cast<const float2*>(s.ks + 8 * j + 2 * t), vs = *reinterpret_cast<const float2*>(s.vs + 8 * j + 2 * t);
+			const float2 ks = *reinterpret_cast<const float2*>(s.ks + 8 * j + 2 * t), lv = *reinterpret_cast<const float2*>(s.vs + 8 * j + 2 * t);
+			if (EXTRA) {
 #pragma unroll
-			for (int e = 0; e < 4; ++e) {
-				const int i = e >> 1, key = 8 * j + 2 * t + (e & 1);
-				const float vscale = e & 1 ? vs.y : vs.x;
-				const int ve = (int)(__float_as_uint(vscale) >> 23) - 127;
-				if (i == 0) over[2 * j + (e & 1)] = pow2f(-max(ve, -126));
-				float x = z[j][e] * (rs[i] * (e & 1 ? ks.y : ks.x));
-				if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-				const int kp = position(j0 + key);
-				if (a.slopes) x -= slope[i] * (float)(rpos[i] - kp);
-				x = fmaf(x, AT_LOG2E, (float)ve);
-				if (!all && !((seen >> key & 1) && kp <= rpos[i] && (kp >= rlo[i] || kp < a.keep_first))) x = -INFINITY;
-				z[j][e] = x;
-				top[i] = fmaxf(top[i], x);
+				for (int e = 0; e < 4; ++e) {
+					const int i = e >> 1, r = g + 8 * i;
+					float y = z[j][e] * (e & 1 ? ks.y : ks.x);
+					if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
+					if (a.slopes && r < rows) y -= a.slopes[kvh * a.group + (row0 + r) % a.group] * (float)(rpos[i] - position(j0 + 8 * j + 2 * t + (e & 1)));
+					z[j][e] = fmaf(y, AT_LOG2E, e & 1 ? lv.y : lv.x);
+				}
+			} else z[j][0] = fmaf(z[j][0], ks.x, lv.x), z[j][1] = fmaf(z[j][1], ks.y, lv.y), z[j][2] = fmaf(z[j][2], ks.x, lv.x), z[j][3] = fmaf(z[j][3], ks.y, lv.y);
+			if (!all) {
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					const int i = e >> 1, key = 8 * j + 2 * t + (e & 1), kp = position(j0 + key);
+					if (!((seen >> key & 1) && kp <= rpos[i] && (kp >= at_low(a, rpos[i]) || kp < a.keep_first))) z[j][e] = -INFINITY;
+				}
 			}
+			tops[0] = fmaxf(fmaxf(tops[0], z[j][0]), z[j][1]), tops[1] = fmaxf(fmaxf(tops[1], z[j][2]), z[j][3]);
 		}
-		float f[2];
+		if (__any_sync(0xffffffffu, tops[0] > m[0] + AT_MOST || tops[1] > m[1] + AT_MOST)) { // references move
+			float f[2];
 #pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-			top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-			const float mn = fmaxf(m[i], top[i] - AT_LIFT);
-			f[i] = m[i] == -INFINITY ? 0.f : exp2f(m[i] - mn);
-			m[i] = mn, l[i] *= f[i];
+			for (int i = 0; i < 2; ++i) {
+				tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 1));
+				tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 2));
+				const float mn = tops[i] > m[i] + AT_MOST ? tops[i] - AT_SET : m[i];
+				f[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - mn);
+				m[i] = mn, l[i] *= f[i];
+			}
+#pragma unroll
+			for (int i = 0; i < NT; ++i) acc[i][0] *= f[0], acc[i][1] *= f[0], acc[i][2] *= f[1], acc[i][3] *= f[1];
 		}
 		const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-		for (int j = 0; j < 4; ++j)
+		for (int j = 0; j < 4; ++j) {
+			const float2 ov = *reinterpret_cast<const float2*>(s.ov + 8 * j + 2 * t);
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				const float w = exp2f(z[j][e] - base[e >> 1]);
-				z[j][e] = w, l[e >> 1] = fmaf(w, over[2 * j + (e & 1)], l[e >> 1]);
+				z[j][e] = ex2(z[j][e] - base[e >> 1]);
+				l[e >> 1] = fmaf(z[j][e], e & 1 ? ov.y : ov.x, l[e >> 1]);
 			}
-#pragma unroll
-		for (int i = 0; i < NT; ++i) acc[i][0] *= f[0], acc[i][1] *= f[0], acc[i][2] *= f[1], acc[i][3] *= f[1];
+		}
 		// values: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step kk is key 16 kk + 2t + {0, 1}, + 8; column g of product i is channel g * D / 8 + i
 #pragma unroll
 		for (int kk = 0; kk < 2; ++kk) {
@@ -356,18 +420,18 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 				pl.x = pack_rest(z[2 * kk][0], z[2 * kk][1], ph.x), pl.y = pack_rest(z[2 * kk][2], z[2 * kk][3], ph.y);
 				pl.z = pack_rest(z[2 * kk + 1][0], z[2 * kk + 1][1], ph.z), pl.w = pack_rest(z[2 * kk + 1][2], z[2 * kk + 1][3], ph.w);
 			}
-			uint32_t x[4][D / 32]; // this thread's channels of its four keys
+			uint32_t y[4][D / 32]; // this thread's channels of its four keys
 #pragma unroll
 			for (int u = 0; u < 4; ++u) {
 				const int r = 16 * kk + 2 * t + (u & 1) + (u >> 1) * 8;
 				if constexpr (D == 64) {
 					const uint2 w = *reinterpret_cast<const uint2*>(s.v + (r * PIECES + at_place<D>(r, g >> 1)) * 16 + (g & 1) * 8);
-					x[u][0] = w.x, x[u][1] = w.y;
+					y[u][0] = w.x, y[u][1] = w.y;
 				} else {
 #pragma unroll
 					for (int i = 0; i < D / 128; ++i) {
 						const uint4 w = *reinterpret_cast<const uint4*>(s.v + (r * PIECES + at_place<D>(r, g * (D / 128) + i)) * 16);
-						x[u][4 * i] = w.x, x[u][4 * i + 1] = w.y, x[u][4 * i + 2] = w.z, x[u][4 * i + 3] = w.w;
+						y[u][4 * i] = w.x, y[u][4 * i + 1] = w.y, y[u][4 * i + 2] = w.z, y[u][4 * i + 3] = w.w;
 					}
 				}
 			}
@@ -375,8 +439,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 			for (int i = 0; i < D / 32; ++i)
 #pragma unroll
 				for (int e = 0; e < 2; ++e) { // bytes 2e, 2e + 1 of the words
-					const uint32_t p = __byte_perm(x[0][i], x[1][i], e ? 0x7362 : 0x5140), q = __byte_perm(x[2][i], x[3][i], e ? 0x7362 : 0x5140);
-					const uint32_t b0 = e4m3x2_to_f16(p), b1 = e4m3x2_to_f16(q), b2 = e4m3x2_to_f16(p >> 16), b3 = e4m3x2_to_f16(q >> 16);
+					uint32_t b0, b1, b2, b3;
+					e4m3x4_to_f16(__byte_perm(y[0][i], y[1][i], e ? 0x7362 : 0x5140), b0, b2);
+					e4m3x4_to_f16(__byte_perm(y[2][i], y[3][i], e ? 0x7362 : 0x5140), b1, b3);
 					mma_f16(acc[4 * i + 2 * e], ph, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], ph, b2, b3);
 					if (SPLIT) mma_f16(acc[4 * i + 2 * e], pl, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], pl, b2, b3);
 				}
@@ -395,19 +460,20 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 		for (int e = 0; e < 4; ++e) sums[((warp * 16) + g + (e >> 1) * 8) * D + (2 * t + (e & 1)) * (D / 8) + i] = acc[i][e];
 	if (t == 0) fold_m[warp][g] = m[0], fold_m[warp][g + 8] = m[1], fold_l[warp][g] = l[0], fold_l[warp][g + 8] = l[1];
 	__syncthreads();
+	const bool whole = sp.chunks <= a.each || a.shares == 1; // no other share has keys
 	for (int r = warp; r < rows; r += AT_WARPS) {
 		float mx = fold_m[0][r], den = 0.f, wt[AT_WARPS];
 #pragma unroll
 		for (int w = 1; w < AT_WARPS; ++w) mx = fmaxf(mx, fold_m[w][r]);
 #pragma unroll
-		for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : exp2f(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
+		for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
 		const int token = start + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
-		float* const part = a.shares > 1 ? a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2) : nullptr;
+		float* const part = whole ? nullptr : a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2);
 		float norm = 0.f;
-		if (a.shares == 1) {
+		if (whole) {
 			if (a.sinks) { // one more term of the denominator
-				const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : exp2f(mx - mn);
-				den = den * down + exp2f(sk - mn), norm = down;
+				const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : ex2(mx - mn);
+				den = den * down + ex2(sk - mn), norm = down;
 			} else norm = 1.f;
 			norm = den > 0.f ? norm / den : den == 0.f ? 0.f : den; // (a NaN stays one)
 		} else if (lane == 0) part[dim] = mx, part[dim + 1] = den;
@@ -415,7 +481,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 			float v = 0.f;
 #pragma unroll
 			for (int w = 0; w < AT_WARPS; ++w) v = fmaf(wt[w], sums[(w * 16 + r) * D + d], v);
-			if (a.shares > 1) part[d] = v;
+			if (!whole) part[d] = v;
 			else {
 				v *= norm;
 				if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
@@ -425,30 +491,41 @@ __global__ void __launch_bounds__(32 * AT_WARPS) k_c8_attend(const C8 c, const A
 	}
 }
 
-// folds the shares of one (token, head), in share order
+// Folds the shares of one (token, head), in share order: a warp each, four channels a lane at a time.
 template <typename OT>
 __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	pdl_wait_prev();
-	const int b = blockIdx.z, head = blockIdx.y, n = c.count[b], start = c.start[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-	if (n < 1 || c.pos0[b] < 0 || c.pos0[b] > INT_MAX - n || start < 0 || n > a.rows - start) return;
-	for (int i = blockIdx.x * 4 + warp; i < n; i += gridDim.x * 4) {
-		const int token = start + i;
-		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * (c.dim + 2);
+	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start) return;
+	for (long long row = (long long)blockIdx.x * 4 + warp; row < (long long)n * a.group; row += gridDim.x * 4) {
+		const int row0 = (int)(row & ~15LL), rows = (int)min(16LL, (long long)n * a.group - row0);
+		const int shares = min(a.shares, (at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots).chunks + a.each - 1) / a.each);
+		if (shares <= 1) continue; // its one share has finished it
+		const int token = start + (int)(row / a.group), head = kvh * a.group + (int)(row % a.group), stride = c.dim + 2;
+		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * stride;
 		float mx = -INFINITY, den = 0.f;
-		for (int s = 0; s < a.shares; ++s) mx = fmaxf(mx, p[(size_t)s * (c.dim + 2) + c.dim]);
+		for (int s = lane; s < shares; s += 32) mx = fmaxf(mx, p[(size_t)s * stride + c.dim]);
+		mx = warp_max(mx);
 		const float sk = a.sinks ? a.sinks[head] * AT_LOG2E : -INFINITY, mn = fmaxf(mx, sk);
-		for (int s = 0; s < a.shares; ++s) {
-			const float* q = p + (size_t)s * (c.dim + 2) + c.dim;
-			den = fmaf(q[0] == -INFINITY ? 0.f : exp2f(q[0] - mn), q[1], den);
+		float w[AT_SHARES / 32]; // this lane's shares' weights
+#pragma unroll
+		for (int i = 0; i < AT_SHARES / 32; ++i) {
+			const int s = i * 32 + lane;
+			const float m = s < shares ? p[(size_t)s * stride + c.dim] : -INFINITY;
+			w[i] = m == -INFINITY ? 0.f : ex2(m - mn);
+			if (s < shares) den = fmaf(w[i], p[(size_t)s * stride + c.dim + 1], den);
 		}
-		if (a.sinks) den += exp2f(sk - mn);
-		const float norm = den > 0.f ? 1.f / den : den;
-		for (int d = lane; d < c.dim; d += 32) {
+		den = warp_sum(den);
+		if (a.sinks) den += ex2(sk - mn);
+		const float norm = den > 0.f ? 1.f / den : den; // (0: nothing was seen)
+		for (int d0 = 0; d0 < c.dim; d0 += 32) {
+			const int d = d0 + lane, dd = min(d, c.dim - 1);
 			float v = 0.f;
-			for (int s = 0; s < a.shares; ++s) {
-				const float* q = p + (size_t)s * (c.dim + 2);
-				v = fmaf(q[c.dim] == -INFINITY ? 0.f : exp2f(q[c.dim] - mn), q[d], v);
-			}
+#pragma unroll
+			for (int i = 0; i < AT_SHARES / 32; ++i)
+#pragma unroll 4
+				for (int s = i * 32; s < min(shares, i * 32 + 32); ++s) v = fmaf(__shfl_sync(0xffffffffu, w[i], s & 31), p[(size_t)s * stride + dd], v);
+			if (d >= c.dim) continue;
 			v *= norm;
 			if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
 			((OT*)a.out)[token * a.o_row + head * a.o_head + d] = from_f32<OT>(v);
@@ -460,6 +537,7 @@ int check_cache(const char* what, const SeqCache8* q, const SeqPortions* p) {
 	if (!q || !p) return refuse("%s: no cache or no batch", what);
 	if (q->pages < 0 || q->heads < 1 || q->page < 1 || q->slots < 0 || q->table_pages < 0) return refuse("%s: a cache of %d pages, %d heads, %d tokens a page", what, q->pages, q->heads, q->page);
 	if (q->heads > 4096 || q->page > 65536) return refuse("%s: at most 4096 heads and 65536 tokens a page", what);
+	if ((long long)q->pages * q->heads * q->page > INT_MAX) return refuse("%s: a pool of %d pages, %d heads, %d tokens a page has more than 2^31 rows", what, q->pages, q->heads, q->page);
 	if (q->dim < 16 || q->dim > 256 || q->dim % 16) return refuse("%s: rows of %d channels: a multiple of 16 up to 256 is served", what, q->dim);
 	if (p->n < 0 || p->longest < 0 || p->n > 65535) return refuse("%s: %d sequences (at most 65535), longest %d", what, p->n, p->longest);
 	if (p->n && (!p->start || !p->count || !p->slot || !p->pos0)) return refuse("%s: the batch's description is missing", what);
@@ -476,21 +554,32 @@ int check_rows(const char* what, const char* name, const SeqRows& r) {
 	return 0;
 }
 C8 describe(const SeqCache8& q, const SeqPortions& p) {
-	return C8{(uint8_t*)q.k, (uint8_t*)q.v, q.k_scale, q.v_scale, q.table, q.pages, q.heads, q.page, q.dim, q.slots, q.table_pages, p.start, p.count, p.slot, p.pos0};
+	int shift = 0;
+	while (1 << shift < q.page) ++shift;
+	return C8{(uint8_t*)q.k, (uint8_t*)q.v, q.k_scale, q.v_scale, q.table, q.pages, q.heads, q.page, q.dim, q.slots, q.table_pages, 1 << shift == q.page ? shift : -1, p.start, p.count, p.slot, p.pos0};
 }
 StoreRows store_rows(const SeqRows& r) {
 	const int bytes = 4 * type_size(r.type);
 	return StoreRows{r.p, r.row_stride, r.head_stride, r.rows, (uintptr_t)r.p % bytes == 0 && r.row_stride % 4 == 0 && r.head_stride % 4 == 0};
 }
 
-// CTAs that share the keys of a tile of rows: as many as the GPU has room for, four chunks for each at least
-int attend_shares(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
+// Shares of the keys of a tile of rows, and the chunks of each.  Sequences differ in length: shares of one length for all of them, short ones have fewer.  As many CTAs as the GPU
+// holds at a time where there are few; where there are more, shares that leave the last CTAs little to wait for; two chunks a warp at least.
+struct AtPlan {
+	int shares, each;
+};
+AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const int group = a.heads / c.heads;
-	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, 16) * c.heads, room = 148 * 2;
-	int keys = std::max(a.most_keys, 1);
-	if (a.window > 0) keys = (int)std::min<long long>(keys, (long long)a.window + a.keep_first + (p.longest > 1 ? 16 / group : 0));
-	if (a.chunk > 0) keys = (int)std::min<long long>(keys, (long long)a.chunk + a.keep_first);
-	return ctas >= room || ctas < 1 ? 1 : (int)std::max(1LL, std::min({room / ctas, (long long)cdiv(cdiv(keys, AT_KEYS), AT_WARPS), 64LL}));
+	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, 16) * c.heads, room = 148 * 3;
+	long long keys = std::max(a.most_keys, 1);
+	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + 16 / group);
+	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + 16 / group);
+	const int chunks = cdiv(keys, AT_KEYS);
+	if (ctas < 1) return AtPlan{1, chunks};
+	long long shares = ctas >= 4 * room ? 1 : ctas > room / 2 ? cdiv(4 * room, ctas) : room / ctas;
+	shares = std::max(1LL, std::min({shares, (long long)chunks / (2 * AT_WARPS), (long long)AT_SHARES}));
+	const int each = cdiv(chunks, shares);
+	return AtPlan{cdiv(chunks, each), each};
 }
 size_t attend_bytes(const SeqCache8& c, const SeqAttend8& a, int shares) { return shares > 1 ? (size_t)a.q.rows * a.heads * shares * (c.dim + 2) * sizeof(float) : 0; }
 
@@ -510,8 +599,9 @@ int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) 
 template <int D, typename QT, typename OT>
 cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	const size_t smem = at_smem<D, sizeof(QT) == 4>();
-	cudaError_t e = cudaFuncSetAttribute(k_c8_attend<D, QT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_attend<D, QT, OT>, grid, dim3(32 * AT_WARPS), smem, c, a);
+	auto kernel = a.softcap > 0.f || a.slopes ? k_c8_attend<D, QT, OT, true> : k_c8_attend<D, QT, OT, false>;
+	cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+	if (e == cudaSuccess) e = launch(st, false, 1, kernel, grid, dim3(32 * AT_WARPS), smem, c, a);
 	return e;
 }
 template <typename QT, typename OT>
@@ -542,14 +632,15 @@ extern "C" int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const s
 extern "C" size_t calm_b200_seq_attend8_workspace(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args) {
 	using namespace seqops;
 	if (check_attend(cache, batch, args)) return 0;
-	return attend_bytes(*cache, *args, attend_shares(*cache, *batch, *args));
+	return attend_bytes(*cache, *args, attend_plan(*cache, *batch, *args).shares);
 }
 
 extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* q, void* stream) {
 	using namespace seqops;
 	if (const int rc = check_attend(cache, batch, q)) return rc;
 	if (batch->n == 0 || batch->longest == 0) return 0;
-	const int shares = attend_shares(*cache, *batch, *q);
+	const AtPlan plan = attend_plan(*cache, *batch, *q);
+	const int shares = plan.shares;
 	const size_t need = attend_bytes(*cache, *q, shares);
 	if (need && (!q->workspace || (uintptr_t)q->workspace % 16 || q->workspace_bytes < need)) return refuse("attend8: the workspace has %zu bytes (16-byte aligned), %zu are needed", q->workspace ? q->workspace_bytes : (size_t)0, need);
 	const C8 c = describe(*cache, *batch);
@@ -558,8 +649,8 @@ extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct
 	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap;
 	a.window = q->window, a.keep_first = q->keep_first, a.chunk = q->chunk, a.sinks = q->sinks, a.slopes = q->slopes;
 	a.gate = q->gate, a.gate_row = q->gate_row, a.gate_head = q->gate_head, a.gate_dim = q->gate_dim;
-	a.shares = shares, a.part = (float*)q->workspace;
-	const dim3 grid(cdiv((long long)batch->longest * a.group, 16), cache->heads * shares, batch->n), fold(std::min(cdiv(batch->longest, 4), 65535), q->heads, batch->n);
+	a.shares = shares, a.each = plan.each, a.part = (float*)q->workspace;
+	const dim3 grid(cdiv((long long)batch->longest * a.group, 16), cache->heads * shares, batch->n), fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 	if (grid.y > 65535) return refuse("attend8: too many key heads");
 	const cudaStream_t st = (cudaStream_t)stream;
 	cudaError_t e;

@@ -106,7 +106,7 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
     kernel's arithmetic may add to it before the last rounding.
 
     Bound: a score is a sum over dim in steps of 16 whose fp32 additions may truncate (2^-23 of the terms' sum each), times factors (four roundings); queries and weights
-    enter as fp16 whose largest stands at 2^15 (2^-11 of a weight or 2^-25 2^-15 of the largest; 2^-22 as pairs).  A score's error d moves a weight by e^d; the numerator's sum and the denominator's add
+    enter as fp16, a tile's largest query at 2^15, a row's largest weight at 2^10 or more (2^-11 of a weight or 2^-25 2^-10 of the largest; 2^-22 as pairs).  A score's error d moves a weight by e^d; the numerator's sum and the denominator's add
     a rounding per 16 keys and per share."""
     T, Hq, D = q.shape
     pages, heads = ks.shape
@@ -137,7 +137,7 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
                 x = q[st + i, h]
                 s = k @ x * scale
                 mag = np.abs(k) @ np.abs(x) * abs(scale)
-                dq = (2.0 ** -22 if split else 0.0) * mag + 2.0 ** -40 * np.abs(x).max() * np.abs(k).sum(1) * abs(scale)
+                dq = (2.0 ** -22 if split else 0.0) * mag + 2.0 ** -40 * np.abs(q[st:st + n]).max() * np.abs(k).sum(1) * abs(scale)
                 ds = dq + (D / 16 * (2 if split else 1) + 6) * 2.0 ** -23 * mag
                 if softcap:
                     s = softcap * np.tanh(s / softcap)
@@ -154,8 +154,8 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
                 adds = (len(keys) / 16 * (2 if split else 1) + 80) * 2.0 ** -23
                 spread = p @ np.abs(v)
                 t = (p * ds) @ np.abs(v) + (p @ ds) * np.abs(o) + ((2.0 ** -22 if split else half) + adds) * spread + adds * np.abs(o)
-                # weights whose fp16 (or whose remainder's) is subnormal: half a step is 2^-25, the largest weight (times its value scale) stands at 2^14 at least
-                t = t + 2.0 ** -39 * np.abs(vv[ids, g, keys % page]).sum(0) * np.max(vs[ids, g] * w) / den
+                # weights whose fp16 (or whose remainder's) is subnormal: half a step is 2^-25, the largest weight (times its value scale) stands at 2^10 at least
+                t = t + 2.0 ** -35 * np.abs(vv[ids, g, keys % page]).sum(0) * np.max(vs[ids, g] * w) / den
                 # an exponential under 2^-126 may come out as zero: it multiplies sums of the values by weights of 2^15 at most, and den >= 1
                 t = t + 2.0 ** -111 * np.abs(v).sum(0)
                 if gate is not None:
