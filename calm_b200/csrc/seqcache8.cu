@@ -129,12 +129,12 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 }
 
 // ---------------------------------------------------------------- attention
-// The rows of a CTA are 16 pairs (token, query head) of one sequence that read one key head, so a key is read once for all of them: row i of a sequence's tile is token
-// i / group, head i % group of the group.  Each warp walks its own chunks of 32 keys with a running reference and sum of its own (no barrier between warps until the end),
-// fed by a ring of asynchronous copies; codes become fp16 in registers on their way into m16n8k16 products.  An e4m3 code is exact in fp16; scales do not enter the
-// products: a key's scale multiplies its scores, a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are
-// rounded to fp16 at 2^15 or less; the denominator sums w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z:
-// almost only in a warp's first chunks.
+// The rows of a CTA are 8 NQ pairs (token, query head) of one sequence that read one key head, so a key is read once for all of them: row i of a sequence's tile is token
+// i / group, head i % group of the group.  Each warp walks its own chunks of 32 keys with running references and sums of its own (no barrier between warps until the end),
+// fed by a ring of asynchronous copies; codes become fp16 in registers on their way into m16n8k16 products whose 16 rows are keys (scores: keys x queries) or channels (values:
+// channels x queries), so that eight rows of queries fill a product.  An e4m3 code is exact in fp16; scales do not enter the products: a key's scale multiplies its scores,
+// a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are rounded to fp16 at 2^15 or less; the denominator sums
+// w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z: almost only in a warp's first chunks.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
 constexpr int AT_SHARES = 64; // of a tile's keys at most
 constexpr float AT_LOG2E = 1.4426950408889634f;
@@ -146,11 +146,13 @@ struct Attend {
 	long long q_row, q_head;
 	void* out;
 	long long o_row, o_head;
+	int q_type, out_type;
 	int rows, heads, group;
 	float scale, softcap;
 	int window, keep_first, chunk;
 	const float *sinks, *slopes, *gate;
 	long long gate_row, gate_head, gate_dim;
+	int tile;         // rows of a CTA: 8 NQ
 	int shares, each; // shares of a tile's keys at most, chunks of each
 	float* part;      // [rows][heads][shares][dim + 2]: sum, reference, denominator
 };
@@ -158,14 +160,14 @@ struct Attend {
 template <int D>
 struct AtStage { // a warp's chunk
 	uint8_t k[AT_KEYS * D], v[AT_KEYS * D];
-	float ks[AT_KEYS], vs[AT_KEYS], ov[AT_KEYS]; // scales as they come; then factors on scores, log2 of the value scales and the inverse of those
+	float ks[AT_KEYS], vs[AT_KEYS];
 	uint32_t seen; // keys that are there
 	uint32_t pad[3];
 };
 template <int D>
 __host__ __device__ constexpr int at_stages() { return D == 64 ? 3 : 2; }
-template <int D, bool SPLIT>
-constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 16 * D * 2 + (size_t)AT_WARPS * at_stages<D>() * sizeof(AtStage<D>); }
+template <int D, bool SPLIT, int NQ>
+constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2 + (size_t)AT_WARPS * at_stages<D>() * sizeof(AtStage<D>); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -176,10 +178,16 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) 
 __device__ __forceinline__ void cp4(void* dst, const void* src, bool there) {
 	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
 	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-	             : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+	             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+// an 8 x 8 tile of fp16, a row's pair of neighbours a thread, with rows and columns exchanged
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+	uint32_t r;
+	asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+	return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
 	const __half2 h = __floats2half2_rn(x, y);
@@ -192,6 +200,14 @@ __device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) { /
 // 16-byte piece of a row of codes that is stored at place `piece` of row r: rows read together meet different banks
 template <int D>
 __device__ __forceinline__ int at_place(int r, int piece) { return piece ^ (D == 64 ? (r >> 1) & 3 : r & 7); }
+__device__ __forceinline__ float load_as_f32(const void* p, int type, long long i) {
+	return type == SEQ_F32 ? ((const float*)p)[i] : type == SEQ_BF16 ? as_f32(((const bf16*)p)[i]) : as_f32(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void store_f32(void* p, int type, long long i, float v) {
+	if (type == SEQ_F32) ((float*)p)[i] = v;
+	else if (type == SEQ_BF16) ((bf16*)p)[i] = __float2bfloat16_rn(v);
+	else ((__half*)p)[i] = __float2half_rn(v);
+}
 
 // the positions that a tile of rows sees, in order: [0, kept), then [lo, last]
 struct AtSpan {
@@ -209,21 +225,25 @@ __device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int
 	s.chunks = (s.total + AT_KEYS - 1) / AT_KEYS;
 	return s;
 }
+__device__ __forceinline__ void at_finish(const Attend& a, int token, int head, int d, float v) {
+	if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
+	store_f32(a.out, a.out_type, token * a.o_row + head * a.o_head + d, v);
+}
 
-// EXTRA: a soft cap or slopes
-template <int D, typename QT, typename OT, bool EXTRA>
-__global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(const C8 c, const Attend a) {
-	constexpr bool SPLIT = sizeof(QT) == 4, KEEP = !SPLIT && D <= 128; // KEEP: the queries' fragments stay in registers
-	constexpr int ST = at_stages<D>(), KS = D / 16, NT = D / 8, PIECES = D / 16;
+template <int D, bool SPLIT, int NQ>
+__global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 256 && D < 256 ? 3 : 2) k_c8_attend(const C8 c, const Attend a) {
+	constexpr bool KEEP = D * NQ * (SPLIT ? 2 : 1) <= 128; // the queries' fragments stay in registers
+	constexpr int ST = at_stages<D>(), KS = D / 16, MT = D / 16, PIECES = D / 16;
+	constexpr int FS = D == 256 ? 52 : 20, LD = 8 * FS + 4; // sums in shared memory: eight parts of a row FS apart, rows LD: 16-byte stores of eight lanes meet different banks
 	extern __shared__ __align__(128) unsigned char at_sm[];
-	uint4* const qf = reinterpret_cast<uint4*>(at_sm); // A fragments [KS][32], then the remainders'
-	AtStage<D>* const ring = reinterpret_cast<AtStage<D>*>(at_sm + (size_t)(SPLIT ? 2 : 1) * 16 * D * 2);
-	__shared__ float fold_m[AT_WARPS][16], fold_l[AT_WARPS][16], qtop[AT_WARPS];
+	uint2* const qf = reinterpret_cast<uint2*>(at_sm); // B fragments [KS][NQ][32], then the remainders'
+	AtStage<D>* const ring = reinterpret_cast<AtStage<D>*>(at_sm + (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2);
+	__shared__ float fold_m[AT_WARPS][8 * NQ], fold_l[AT_WARPS][8 * NQ], qtop[AT_WARPS];
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 	const int b = blockIdx.z, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = blockIdx.x;
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
-	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * 16 >= (long long)n * a.group) return;
-	const int row0 = tile * 16, rows = (int)min(16LL, (long long)n * a.group - row0);
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * (8 * NQ) >= (long long)n * a.group) return;
+	const int row0 = tile * (8 * NQ), rows = (int)min((long long)(8 * NQ), (long long)n * a.group - row0);
 	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
 	const int lo = sp.lo, kept = sp.kept, total = sp.total;
 	const int begin = share * a.each, end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
@@ -242,7 +262,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(c
 	AtStage<D>* const mine = ring + warp * ST;
 	int next = begin + warp, next_page = page_of(next), stage_in = 0; // the chunk to request, its page
 	const int piece = lane % PIECES, prow = lane / PIECES;            // which piece of which row of a group of 32 pieces this lane copies
-	uint32_t swizzle[2];                                              // where, for rows that differ by 4 (by 2 where rows have 16 pieces: four of those)
+	uint32_t swizzle[2];                                              // where, for even and odd groups (rows of 128 bytes)
 #pragma unroll
 	for (int i = 0; i < 2; ++i) swizzle[i] = at_place<D>(prow + i * 4, piece) * 16;
 	auto request = [&]() {
@@ -280,17 +300,17 @@ __global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(c
 #pragma unroll
 	for (int i = 0; i < ST - 1; ++i) request();
 
-	// Queries as A fragments, times a power of two that is the tile's: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
+	// Queries as B fragments, times a power of two that is the tile's: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
 	// thread's codes of a key lie side by side).
-	float x[16 / AT_WARPS][D / 32], top = 0.f;
+	float x[2 * NQ][D / 32], top = 0.f;
 #pragma unroll
-	for (int i = 0; i < 16 / AT_WARPS; ++i) {
+	for (int i = 0; i < 2 * NQ; ++i) {
 		const int r = i * AT_WARPS + warp, rr = row0 + min(r, rows - 1);
-		const QT* src = (const QT*)a.q + (long long)(start + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head;
+		const long long at = (long long)(start + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head;
 #pragma unroll
 		for (int k = 0; k < D / 32; ++k) {
 			const int d = k * 32 + lane;
-			x[i][k] = r < rows && d < dim ? as_f32(src[d]) : 0.f;
+			x[i][k] = r < rows && d < dim ? load_as_f32(a.q, a.q_type, at + d) : 0.f;
 			top = fmaxf(top, fabsf(x[i][k]));
 		}
 	}
@@ -302,30 +322,40 @@ __global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(c
 	const int qe = (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT; // top = m 2^(qe + AT_LIFT)
 	const float qdown = pow2f(-qe);
 #pragma unroll
-	for (int i = 0; i < 16 / AT_WARPS; ++i) {
+	for (int i = 0; i < 2 * NQ; ++i) {
 		const int r = i * AT_WARPS + warp;
 #pragma unroll
 		for (int k = 0; k < D / 32; ++k) {
 			const int d = k * 32 + lane, dt = d / (D / 4), ds = d % (D / 4) / 4, de = d & 3;
-			const int at = ((ds * 32 + (r & 7) * 4 + dt) * 4 + (de >> 1) * 2 + (r >> 3)) * 2 + (de & 1);
+			const int at = (((ds * NQ + (r >> 3)) * 32 + (r & 7) * 4 + dt) * 2 + (de >> 1)) * 2 + (de & 1);
 			const float y = x[i][k] * qdown;
 			const __half hi = __float2half_rn(y);
 			reinterpret_cast<__half*>(qf)[at] = hi;
-			if (SPLIT) reinterpret_cast<__half*>(qf + KS * 32)[at] = __float2half_rn(y - __half2float(hi));
+			if (SPLIT) reinterpret_cast<__half*>(qf + KS * NQ * 32)[at] = __float2half_rn(y - __half2float(hi));
 		}
 	}
 	__syncthreads();
-	const float qscale = a.scale * pow2f(qe) * (EXTRA ? 1.f : AT_LOG2E);
-	uint4 qr[KEEP ? KS : 1];
+	const bool extra = a.softcap > 0.f || a.slopes;
+	const float qscale = a.scale * pow2f(qe) * (extra ? 1.f : AT_LOG2E);
+	uint2 qr[KEEP ? (SPLIT ? 2 : 1) * KS * NQ : 1];
 	if (KEEP) {
 #pragma unroll
-		for (int i = 0; i < KS; ++i) qr[i] = qf[i * 32 + lane];
+		for (int i = 0; i < (SPLIT ? 2 : 1) * KS * NQ; ++i) qr[i] = qf[i * 32 + lane];
 	}
+	auto qfrag = [&](int i) { return KEEP ? qr[i] : qf[i * 32 + lane]; };
 
-	float acc[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // rows g and g + 8; m: the reference r
+	float acc[MT][NQ][4], m[NQ][2], l[NQ][2]; // queries 2t and 2t + 1 of each eight; m: the reference r
+	int rpos[NQ][2];
 #pragma unroll
-	for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-	const int rpos[2] = {g < rows ? p0 + (row0 + g) / a.group : -1, g + 8 < rows ? p0 + (row0 + g + 8) / a.group : -1};
+	for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+		for (int i = 0; i < MT; ++i) acc[i][q][0] = acc[i][q][1] = acc[i][q][2] = acc[i][q][3] = 0.f;
+#pragma unroll
+		for (int e = 0; e < 2; ++e) {
+			const int r = 8 * q + 2 * t + e;
+			m[q][e] = -INFINITY, l[q][e] = 0.f, rpos[q][e] = r < rows ? p0 + (row0 + r) / a.group : -1;
+		}
+	}
 	const int wide = at_low(a, sp.last); // from here on, and up to `first`, every row sees every key
 
 	int stage = 0;
@@ -333,93 +363,97 @@ __global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(c
 		asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
 		__syncwarp();
 		request(); // into the stage that was used up last
-		AtStage<D>& s = mine[stage];
+		const AtStage<D>& s = mine[stage];
 		stage = stage + 1 == ST ? 0 : stage + 1;
-		{ // a lane's key: factor on its scores, log2 and inverse of its value's scale
-			const float vscale = s.vs[lane];
-			const int ve = max((int)(__float_as_uint(vscale) >> 23) - 127, -126);
-			s.ks[lane] *= qscale, s.vs[lane] = (float)ve, s.ov[lane] = pow2f(-ve);
-		}
-		float z[4][4];
+		// scores: rows g and g + 8 of product i are keys 16 i + g, + 8
+		float z[2][NQ][4];
 #pragma unroll
-		for (int j = 0; j < 4; ++j) {
-			z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.f;
-			const int r = 8 * j + g;
-			uint32_t w[KS];
+		for (int i = 0; i < 2; ++i) {
 #pragma unroll
-			for (int i = 0; i < (KS + 3) / 4; ++i) {
-				const uint4 y = *reinterpret_cast<const uint4*>(s.k + (r * PIECES + at_place<D>(r, t * (PIECES / 4) + i)) * 16);
-				w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
+			for (int q = 0; q < NQ; ++q) z[i][q][0] = z[i][q][1] = z[i][q][2] = z[i][q][3] = 0.f;
+#pragma unroll
+			for (int k = 0; k < (KS + 3) / 4; ++k) {
+				const int r = 16 * i + g;
+				const uint4 u = *reinterpret_cast<const uint4*>(s.k + (r * PIECES + at_place<D>(r, t * (PIECES / 4) + k)) * 16);
+				const uint4 w = *reinterpret_cast<const uint4*>(s.k + ((r + 8) * PIECES + at_place<D>(r + 8, t * (PIECES / 4) + k)) * 16);
+				const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+				for (int f = 0; f < 4; ++f) {
+					uint32_t A[4];
+					e4m3x4_to_f16(us[f], A[0], A[2]), e4m3x4_to_f16(ws[f], A[1], A[3]);
+#pragma unroll
+					for (int q = 0; q < NQ; ++q) {
+						mma_f16(z[i][q], A, qfrag((4 * k + f) * NQ + q));
+						if (SPLIT) mma_f16(z[i][q], A, qfrag((KS + 4 * k + f) * NQ + q));
+					}
+				}
 			}
-#pragma unroll
-			for (int i = 0; i < KS; ++i) {
-				uint32_t b0, b1;
-				e4m3x4_to_f16(w[i], b0, b1);
-				mma_f16(z[j], KEEP ? qr[i] : qf[i * 32 + lane], b0, b1);
-				if (SPLIT) mma_f16(z[j], qf[(KS + i) * 32 + lane], b0, b1);
-			}
 		}
-		__syncwarp(); // the factors
-		// scores with the value's scale in the exponent
+		// with the value's scale in the exponent; this thread's keys are 8 j + g
 		const uint32_t seen = s.seen;
 		const int j0 = chunk * AT_KEYS;
 		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= sp.first;
-		float tops[2] = {-INFINITY, -INFINITY};
+		float over[4]; // 1 / value scale
+		bool move = false;
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			const float2 ks = *reinterpret_cast<const float2*>(s.ks + 8 * j + 2 * t), lv = *reinterpret_cast<const float2*>(s.vs + 8 * j + 2 * t);
-			if (EXTRA) {
+			const float kf = s.ks[8 * j + g] * qscale;
+			const int ve = max((int)(__float_as_uint(s.vs[8 * j + g]) >> 23) - 127, -126);
+			const float lv = (float)ve;
+			over[j] = pow2f(-ve);
+			const int kp = position(j0 + 8 * j + g);
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const int i = e >> 1, r = g + 8 * i;
-					float y = z[j][e] * (e & 1 ? ks.y : ks.x);
-					if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
-					if (a.slopes && r < rows) y -= a.slopes[kvh * a.group + (row0 + r) % a.group] * (float)(rpos[i] - position(j0 + 8 * j + 2 * t + (e & 1)));
-					z[j][e] = fmaf(y, AT_LOG2E, e & 1 ? lv.y : lv.x);
-				}
-			} else z[j][0] = fmaf(z[j][0], ks.x, lv.x), z[j][1] = fmaf(z[j][1], ks.y, lv.y), z[j][2] = fmaf(z[j][2], ks.x, lv.x), z[j][3] = fmaf(z[j][3], ks.y, lv.y);
-			if (!all) {
+			for (int q = 0; q < NQ; ++q)
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const int i = e >> 1, key = 8 * j + 2 * t + (e & 1), kp = position(j0 + key);
-					if (!((seen >> key & 1) && kp <= rpos[i] && (kp >= at_low(a, rpos[i]) || kp < a.keep_first))) z[j][e] = -INFINITY;
+				for (int e = 0; e < 2; ++e) {
+					float& y = z[j >> 1][q][(j & 1) * 2 + e];
+					if (extra) {
+						y *= kf;
+						if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
+						if (a.slopes) y -= a.slopes[kvh * a.group + (row0 + min(8 * q + 2 * t + e, rows - 1)) % a.group] * (float)(rpos[q][e] - kp);
+						y = fmaf(y, AT_LOG2E, lv);
+					} else y = fmaf(y, kf, lv);
+					if (!all && !((seen >> (8 * j + g) & 1) && kp <= rpos[q][e] && (kp >= at_low(a, rpos[q][e]) || kp < a.keep_first))) y = -INFINITY;
+					move |= y > m[q][e] + AT_MOST;
 				}
-			}
-			tops[0] = fmaxf(fmaxf(tops[0], z[j][0]), z[j][1]), tops[1] = fmaxf(fmaxf(tops[1], z[j][2]), z[j][3]);
 		}
-		if (__any_sync(0xffffffffu, tops[0] > m[0] + AT_MOST || tops[1] > m[1] + AT_MOST)) { // references move
-			float f[2];
+		if (__any_sync(0xffffffffu, move)) { // references move
+#pragma unroll
+			for (int q = 0; q < NQ; ++q) {
+				float f[2];
+#pragma unroll
+				for (int e = 0; e < 2; ++e) {
+					float top = fmaxf(fmaxf(z[0][q][e], z[0][q][2 + e]), fmaxf(z[1][q][e], z[1][q][2 + e]));
+#pragma unroll
+					for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+					const float mn = top > m[q][e] + AT_MOST ? top - AT_SET : m[q][e];
+					f[e] = m[q][e] == -INFINITY ? 0.f : ex2(m[q][e] - mn);
+					m[q][e] = mn, l[q][e] *= f[e];
+				}
+#pragma unroll
+				for (int i = 0; i < MT; ++i) acc[i][q][0] *= f[0], acc[i][q][1] *= f[1], acc[i][q][2] *= f[0], acc[i][q][3] *= f[1];
+			}
+		}
+		// weights, from keys x queries to the B fragments of queries x keys
+		uint2 ph[2][NQ], pl[2][SPLIT ? NQ : 1];
+#pragma unroll
+		for (int q = 0; q < NQ; ++q) {
+			const float base[2] = {m[q][0] == -INFINITY ? 0.f : m[q][0], m[q][1] == -INFINITY ? 0.f : m[q][1]};
 #pragma unroll
 			for (int i = 0; i < 2; ++i) {
-				tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 1));
-				tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 2));
-				const float mn = tops[i] > m[i] + AT_MOST ? tops[i] - AT_SET : m[i];
-				f[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - mn);
-				m[i] = mn, l[i] *= f[i];
-			}
 #pragma unroll
-			for (int i = 0; i < NT; ++i) acc[i][0] *= f[0], acc[i][1] *= f[0], acc[i][2] *= f[1], acc[i][3] *= f[1];
-		}
-		const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-		for (int j = 0; j < 4; ++j) {
-			const float2 ov = *reinterpret_cast<const float2*>(s.ov + 8 * j + 2 * t);
-#pragma unroll
-			for (int e = 0; e < 4; ++e) {
-				z[j][e] = ex2(z[j][e] - base[e >> 1]);
-				l[e >> 1] = fmaf(z[j][e], e & 1 ? ov.y : ov.x, l[e >> 1]);
+				for (int e = 0; e < 4; ++e) {
+					z[i][q][e] = ex2(z[i][q][e] - base[e & 1]);
+					l[q][e & 1] = fmaf(z[i][q][e], over[2 * i + (e >> 1)], l[q][e & 1]);
+				}
+				const uint32_t h0 = pack_f16(z[i][q][0], z[i][q][1]), h1 = pack_f16(z[i][q][2], z[i][q][3]);
+				ph[i][q] = make_uint2(transposed(h0), transposed(h1));
+				if (SPLIT) pl[i][q] = make_uint2(transposed(pack_rest(z[i][q][0], z[i][q][1], h0)), transposed(pack_rest(z[i][q][2], z[i][q][3], h1)));
 			}
 		}
-		// values: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step kk is key 16 kk + 2t + {0, 1}, + 8; column g of product i is channel g * D / 8 + i
+		// values: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step kk is key 16 kk + 2t + {0, 1}, + 8; rows g and g + 8 of product i are channels g * D / 8 + 2 i + {0, 1}
 #pragma unroll
 		for (int kk = 0; kk < 2; ++kk) {
-			uint4 ph, pl;
-			ph.x = pack_f16(z[2 * kk][0], z[2 * kk][1]), ph.y = pack_f16(z[2 * kk][2], z[2 * kk][3]);
-			ph.z = pack_f16(z[2 * kk + 1][0], z[2 * kk + 1][1]), ph.w = pack_f16(z[2 * kk + 1][2], z[2 * kk + 1][3]);
-			if (SPLIT) {
-				pl.x = pack_rest(z[2 * kk][0], z[2 * kk][1], ph.x), pl.y = pack_rest(z[2 * kk][2], z[2 * kk][3], ph.y);
-				pl.z = pack_rest(z[2 * kk + 1][0], z[2 * kk + 1][1], ph.z), pl.w = pack_rest(z[2 * kk + 1][2], z[2 * kk + 1][3], ph.w);
-			}
 			uint32_t y[4][D / 32]; // this thread's channels of its four keys
 #pragma unroll
 			for (int u = 0; u < 4; ++u) {
@@ -436,99 +470,111 @@ __global__ void __launch_bounds__(32 * AT_WARPS, D == 256 ? 2 : 3) k_c8_attend(c
 				}
 			}
 #pragma unroll
-			for (int i = 0; i < D / 32; ++i)
+			for (int i = 0; i < MT; ++i) { // bytes 2 (i & 1), + 1 of word i / 2
+				uint32_t A[4];
+				e4m3x4_to_f16(__byte_perm(y[0][i >> 1], y[1][i >> 1], i & 1 ? 0x7362 : 0x5140), A[0], A[1]);
+				e4m3x4_to_f16(__byte_perm(y[2][i >> 1], y[3][i >> 1], i & 1 ? 0x7362 : 0x5140), A[2], A[3]);
 #pragma unroll
-				for (int e = 0; e < 2; ++e) { // bytes 2e, 2e + 1 of the words
-					uint32_t b0, b1, b2, b3;
-					e4m3x4_to_f16(__byte_perm(y[0][i], y[1][i], e ? 0x7362 : 0x5140), b0, b2);
-					e4m3x4_to_f16(__byte_perm(y[2][i], y[3][i], e ? 0x7362 : 0x5140), b1, b3);
-					mma_f16(acc[4 * i + 2 * e], ph, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], ph, b2, b3);
-					if (SPLIT) mma_f16(acc[4 * i + 2 * e], pl, b0, b1), mma_f16(acc[4 * i + 2 * e + 1], pl, b2, b3);
+				for (int q = 0; q < NQ; ++q) {
+					mma_f16(acc[i][q], A, ph[kk][q]);
+					if (SPLIT) mma_f16(acc[i][q], A, pl[kk][q]);
 				}
+			}
 		}
 	}
-#pragma unroll
-	for (int i = 0; i < 2; ++i) l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1), l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-
-	// the warps' sums as one
 	asm volatile("cp.async.wait_group 0;" ::: "memory");
-	__syncthreads();
-	float* const sums = reinterpret_cast<float*>(ring); // [warps][16][D]
 #pragma unroll
-	for (int i = 0; i < NT; ++i)
+	for (int q = 0; q < NQ; ++q)
 #pragma unroll
-		for (int e = 0; e < 4; ++e) sums[((warp * 16) + g + (e >> 1) * 8) * D + (2 * t + (e & 1)) * (D / 8) + i] = acc[i][e];
-	if (t == 0) fold_m[warp][g] = m[0], fold_m[warp][g + 8] = m[1], fold_l[warp][g] = l[0], fold_l[warp][g + 8] = l[1];
-	__syncthreads();
+		for (int e = 0; e < 2; ++e) {
+#pragma unroll
+			for (int o = 4; o < 32; o *= 2) l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], o);
+			if (g == 0) fold_m[warp][8 * q + 2 * t + e] = m[q][e], fold_l[warp][8 * q + 2 * t + e] = l[q][e];
+		}
+
+	// the warps' sums as one, eight rows at a time
+	float* const sums = reinterpret_cast<float*>(ring); // [warps][8][LD]: channel d at d / (D / 8) * FS + d % (D / 8)
 	const bool whole = sp.chunks <= a.each || a.shares == 1; // no other share has keys
-	for (int r = warp; r < rows; r += AT_WARPS) {
-		float mx = fold_m[0][r], den = 0.f, wt[AT_WARPS];
 #pragma unroll
-		for (int w = 1; w < AT_WARPS; ++w) mx = fmaxf(mx, fold_m[w][r]);
+	for (int q = 0; q < NQ; ++q) {
+		if (8 * q >= rows) break;
+		__syncthreads();
 #pragma unroll
-		for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
-		const int token = start + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
-		float* const part = whole ? nullptr : a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2);
-		float norm = 0.f;
-		if (whole) {
-			if (a.sinks) { // one more term of the denominator
-				const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : ex2(mx - mn);
-				den = den * down + ex2(sk - mn), norm = down;
-			} else norm = 1.f;
-			norm = den > 0.f ? norm / den : den == 0.f ? 0.f : den; // (a NaN stays one)
-		} else if (lane == 0) part[dim] = mx, part[dim + 1] = den;
-		for (int d = lane; d < dim; d += 32) {
-			float v = 0.f;
+		for (int e = 0; e < 2; ++e) {
+			float* const to = sums + (warp * 8 + 2 * t + e) * LD + g * FS;
 #pragma unroll
-			for (int w = 0; w < AT_WARPS; ++w) v = fmaf(wt[w], sums[(w * 16 + r) * D + d], v);
-			if (!whole) part[d] = v;
-			else {
-				v *= norm;
-				if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
-				((OT*)a.out)[token * a.o_row + head * a.o_head + d] = from_f32<OT>(v);
+			for (int i = 0; i < MT; i += 2) *reinterpret_cast<float4*>(to + 2 * i) = make_float4(acc[i][q][e], acc[i][q][2 + e], acc[i + 1][q][e], acc[i + 1][q][2 + e]);
+		}
+		__syncthreads();
+		for (int rr = warp; rr < min(8, rows - 8 * q); rr += AT_WARPS) {
+			const int r = 8 * q + rr;
+			float mx = fold_m[0][r], den = 0.f, wt[AT_WARPS];
+#pragma unroll
+			for (int w = 1; w < AT_WARPS; ++w) mx = fmaxf(mx, fold_m[w][r]);
+#pragma unroll
+			for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
+			const int token = start + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
+			float* const part = whole ? nullptr : a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2);
+			float norm = 0.f;
+			if (whole) {
+				if (a.sinks) { // one more term of the denominator
+					const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : ex2(mx - mn);
+					den = den * down + ex2(sk - mn), norm = down;
+				} else norm = 1.f;
+				norm = den > 0.f ? norm / den : den == 0.f ? 0.f : den; // (a NaN stays one)
+			} else if (lane == 0) part[dim] = mx, part[dim + 1] = den;
+			for (int d = lane; d < dim; d += 32) {
+				float v = 0.f;
+#pragma unroll
+				for (int w = 0; w < AT_WARPS; ++w) v = fmaf(wt[w], sums[(w * 8 + rr) * LD + d / (D / 8) * FS + d % (D / 8)], v);
+				if (whole) at_finish(a, token, head, d, v * norm);
+				else part[d] = v;
 			}
 		}
 	}
 }
 
-// Folds the shares of one (token, head), in share order: a warp each, four channels a lane at a time.
-template <typename OT>
+// Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.
 __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	pdl_wait_prev();
 	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start) return;
 	for (long long row = (long long)blockIdx.x * 4 + warp; row < (long long)n * a.group; row += gridDim.x * 4) {
-		const int row0 = (int)(row & ~15LL), rows = (int)min(16LL, (long long)n * a.group - row0);
+		const int row0 = (int)(row / a.tile) * a.tile, rows = (int)min((long long)a.tile, (long long)n * a.group - row0);
 		const int shares = min(a.shares, (at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots).chunks + a.each - 1) / a.each);
 		if (shares <= 1) continue; // its one share has finished it
 		const int token = start + (int)(row / a.group), head = kvh * a.group + (int)(row % a.group), stride = c.dim + 2;
 		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * stride;
-		float mx = -INFINITY, den = 0.f;
-		for (int s = lane; s < shares; s += 32) mx = fmaxf(mx, p[(size_t)s * stride + c.dim]);
-		mx = warp_max(mx);
-		const float sk = a.sinks ? a.sinks[head] * AT_LOG2E : -INFINITY, mn = fmaxf(mx, sk);
-		float w[AT_SHARES / 32]; // this lane's shares' weights
+		const float sk = a.sinks ? a.sinks[head] * AT_LOG2E : -INFINITY;
+		float m[AT_SHARES / 32], w[AT_SHARES / 32], mx = sk, den = 0.f; // this lane's shares
 #pragma unroll
 		for (int i = 0; i < AT_SHARES / 32; ++i) {
 			const int s = i * 32 + lane;
-			const float m = s < shares ? p[(size_t)s * stride + c.dim] : -INFINITY;
-			w[i] = m == -INFINITY ? 0.f : ex2(m - mn);
-			if (s < shares) den = fmaf(w[i], p[(size_t)s * stride + c.dim + 1], den);
+			m[i] = s < shares ? p[(size_t)s * stride + c.dim] : -INFINITY, w[i] = s < shares ? p[(size_t)s * stride + c.dim + 1] : 0.f;
+			mx = fmaxf(mx, m[i]);
+		}
+		mx = warp_max(mx);
+#pragma unroll
+		for (int i = 0; i < AT_SHARES / 32; ++i) {
+			const float f = m[i] == -INFINITY ? 0.f : ex2(m[i] - mx);
+			den = fmaf(f, w[i], den), w[i] = f;
 		}
 		den = warp_sum(den);
-		if (a.sinks) den += ex2(sk - mn);
+		if (a.sinks) den += ex2(sk - mx);
 		const float norm = den > 0.f ? 1.f / den : den; // (0: nothing was seen)
-		for (int d0 = 0; d0 < c.dim; d0 += 32) {
-			const int d = d0 + lane, dd = min(d, c.dim - 1);
-			float v = 0.f;
+		for (int d0 = 0; d0 < c.dim; d0 += 128) {
+			float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 			for (int i = 0; i < AT_SHARES / 32; ++i)
-#pragma unroll 4
-				for (int s = i * 32; s < min(shares, i * 32 + 32); ++s) v = fmaf(__shfl_sync(0xffffffffu, w[i], s & 31), p[(size_t)s * stride + dd], v);
-			if (d >= c.dim) continue;
-			v *= norm;
-			if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
-			((OT*)a.out)[token * a.o_row + head * a.o_head + d] = from_f32<OT>(v);
+#pragma unroll 8
+				for (int s = i * 32; s < min(shares, i * 32 + 32); ++s) {
+					const float f = __shfl_sync(0xffffffffu, w[i], s & 31);
+#pragma unroll
+					for (int k = 0; k < 4; ++k) v[k] = fmaf(f, p[(size_t)s * stride + min(d0 + 32 * k + lane, c.dim - 1)], v[k]);
+				}
+#pragma unroll
+			for (int k = 0; k < 4; ++k)
+				if (d0 + 32 * k + lane < c.dim) at_finish(a, token, head, d0 + 32 * k + lane, v[k] * norm);
 		}
 	}
 }
@@ -568,12 +614,17 @@ StoreRows store_rows(const SeqRows& r) {
 struct AtPlan {
 	int shares, each;
 };
+// Rows of a CTA: eight fill a product; more where a sequence has more, so that codes are read and converted once for all of them, as far as registers hold their sums.
+int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
+	const long long rows = (long long)p.longest * (a.heads / c.heads);
+	return rows <= 8 ? 8 : rows <= 16 || c.dim > 128 ? 16 : 32;
+}
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
-	const int group = a.heads / c.heads;
-	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, 16) * c.heads, room = 148 * 3;
+	const int group = a.heads / c.heads, tile = attend_tile(c, p, a);
+	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, tile) * c.heads, room = 148 * 3;
 	long long keys = std::max(a.most_keys, 1);
-	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + 16 / group);
-	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + 16 / group);
+	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + tile / group);
+	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + tile / group);
 	const int chunks = cdiv(keys, AT_KEYS);
 	if (ctas < 1) return AtPlan{1, chunks};
 	long long shares = ctas >= 4 * room ? 1 : ctas > room / 2 ? cdiv(4 * room, ctas) : room / ctas;
@@ -596,19 +647,20 @@ int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) 
 	return 0;
 }
 
-template <int D, typename QT, typename OT>
+template <int D, bool SPLIT, int NQ>
 cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
-	const size_t smem = at_smem<D, sizeof(QT) == 4>();
-	auto kernel = a.softcap > 0.f || a.slopes ? k_c8_attend<D, QT, OT, true> : k_c8_attend<D, QT, OT, false>;
-	cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-	if (e == cudaSuccess) e = launch(st, false, 1, kernel, grid, dim3(32 * AT_WARPS), smem, c, a);
+	constexpr size_t smem = at_smem<D, SPLIT, NQ>();
+	cudaError_t e = cudaFuncSetAttribute(k_c8_attend<D, SPLIT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_attend<D, SPLIT, NQ>, grid, dim3(32 * AT_WARPS), smem, c, a);
 	return e;
 }
-template <typename QT, typename OT>
-cudaError_t attend_typed(const C8& c, const Attend& a, dim3 grid, dim3 fold, cudaStream_t st) {
-	cudaError_t e = c.dim <= 64 ? attend_launch<64, QT, OT>(c, a, grid, st) : c.dim <= 128 ? attend_launch<128, QT, OT>(c, a, grid, st) : attend_launch<256, QT, OT>(c, a, grid, st);
-	if (e == cudaSuccess && a.shares > 1) e = launch(st, true, 1, k_c8_fold<OT>, fold, dim3(128), 0, c, a);
-	return e;
+template <int D>
+cudaError_t attend_wide(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
+	const bool split = a.q_type == SEQ_F32;
+	if (a.tile == 8) return split ? attend_launch<D, true, 1>(c, a, grid, st) : attend_launch<D, false, 1>(c, a, grid, st);
+	if (D == 256 || a.tile == 16) return split ? attend_launch<D, true, 2>(c, a, grid, st) : attend_launch<D, false, 2>(c, a, grid, st);
+	constexpr int DD = D == 256 ? 128 : D; // (rows of 256 channels come in sixteens)
+	return split ? attend_launch<DD, true, 4>(c, a, grid, st) : attend_launch<DD, false, 4>(c, a, grid, st);
 }
 } // namespace
 } // namespace seqops
@@ -650,13 +702,11 @@ extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct
 	a.window = q->window, a.keep_first = q->keep_first, a.chunk = q->chunk, a.sinks = q->sinks, a.slopes = q->slopes;
 	a.gate = q->gate, a.gate_row = q->gate_row, a.gate_head = q->gate_head, a.gate_dim = q->gate_dim;
 	a.shares = shares, a.each = plan.each, a.part = (float*)q->workspace;
-	const dim3 grid(cdiv((long long)batch->longest * a.group, 16), cache->heads * shares, batch->n), fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
+	a.q_type = q->q.type, a.out_type = q->out.type, a.tile = attend_tile(*cache, *batch, *q);
+	const dim3 grid(cdiv((long long)batch->longest * a.group, a.tile), cache->heads * shares, batch->n), fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 	if (grid.y > 65535) return refuse("attend8: too many key heads");
 	const cudaStream_t st = (cudaStream_t)stream;
-	cudaError_t e;
-	if (q->q.type == SEQ_BF16) e = attend_typed<bf16, bf16>(c, a, grid, fold, st);
-	else if (q->q.type == SEQ_F16) e = attend_typed<__half, __half>(c, a, grid, fold, st);
-	else if (q->out.type == SEQ_BF16) e = attend_typed<float, bf16>(c, a, grid, fold, st);
-	else e = attend_typed<float, float>(c, a, grid, fold, st);
+	cudaError_t e = cache->dim <= 64 ? attend_wide<64>(c, a, grid, st) : cache->dim <= 128 ? attend_wide<128>(c, a, grid, st) : attend_wide<256>(c, a, grid, st);
+	if (e == cudaSuccess && shares > 1) e = launch(st, true, 1, k_c8_fold, fold, dim3(128), 0, c, a);
 	return e == cudaSuccess ? 0 : failed("attend8", e);
 }
