@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 // a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are rounded to fp16 at 2^15 or less; the denominator sums
 // w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z: almost only in a warp's first chunks.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
-constexpr int AT_SHARES = 64; // of a tile's keys at most
+constexpr int AT_SHARES = 64;  // of a tile's keys at most
+constexpr int AT_CLUSTER_ROWS = 16, AT_CLUSTER = 16; // shares that a thread-block cluster folds: of tiles of 16 rows at most, as many
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr int AT_LIFT = 15;                // the largest query of a tile stands at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of it
 constexpr float AT_MOST = 15.f, AT_SET = 10.f; // weights: at most 2^15, the largest at 2^10 or more
@@ -154,20 +155,23 @@ struct Attend {
 	long long gate_row, gate_head, gate_dim;
 	int tile;         // rows of a CTA: 8 NQ
 	int shares, each; // shares of a tile's keys at most, chunks of each
+	int cluster;      // 1: the shares of a tile are a cluster
 	float* part;      // [rows][heads][shares][dim + 2]: sum, reference, denominator
 };
 
 template <int D>
-struct AtStage { // a warp's chunk
+struct AtStage { // a warp's chunk: the next one's keys come while its values are used, the next one's values while their keys are
 	uint8_t k[AT_KEYS * D], v[AT_KEYS * D];
-	float ks[AT_KEYS], vs[AT_KEYS];
-	uint32_t seen; // keys that are there
-	uint32_t pad[3];
+	float ks[2][AT_KEYS], vs[2][AT_KEYS];
+	uint32_t seen[4]; // keys that are there, of this chunk and the next one
 };
 template <int D>
-__host__ __device__ constexpr int at_stages() { return D == 64 ? 3 : 2; }
+__host__ __device__ constexpr size_t at_ring() { // (the sums of the warps take its place)
+	const size_t a = (size_t)AT_WARPS * sizeof(AtStage<D>), b = (size_t)AT_WARPS * 8 * (8 * (D == 256 ? 52 : 20) + 4) * sizeof(float) + (size_t)AT_CLUSTER_ROWS * (D + 2) * sizeof(float);
+	return a > b ? a : b;
+}
 template <int D, bool SPLIT, int NQ>
-constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2 + (size_t)AT_WARPS * at_stages<D>() * sizeof(AtStage<D>); }
+constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2 + at_ring<D>(); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -231,9 +235,9 @@ __device__ __forceinline__ void at_finish(const Attend& a, int token, int head, 
 }
 
 template <int D, bool SPLIT, int NQ>
-__global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 256 && D < 256 ? 3 : 2) k_c8_attend(const C8 c, const Attend a) {
+__global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 256 ? 3 : 2) k_c8_attend(const C8 c, const Attend a) {
 	constexpr bool KEEP = D * NQ * (SPLIT ? 2 : 1) <= 128; // the queries' fragments stay in registers
-	constexpr int ST = at_stages<D>(), KS = D / 16, MT = D / 16, PIECES = D / 16;
+	constexpr int KS = D / 16, MT = D / 16, PIECES = D / 16;
 	constexpr int FS = D == 256 ? 52 : 20, LD = 8 * FS + 4; // sums in shared memory: eight parts of a row FS apart, rows LD: 16-byte stores of eight lanes meet different banks
 	extern __shared__ __align__(128) unsigned char at_sm[];
 	uint2* const qf = reinterpret_cast<uint2*>(at_sm); // B fragments [KS][NQ][32], then the remainders'
@@ -246,8 +250,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 	const int row0 = tile * (8 * NQ), rows = (int)min((long long)(8 * NQ), (long long)n * a.group - row0);
 	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
 	const int lo = sp.lo, kept = sp.kept, total = sp.total;
-	const int begin = share * a.each, end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
-	if (share > 0 && begin >= sp.chunks) return;
+	const int begin = min(sp.chunks, share * a.each), end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
+	if (share > 0 && begin >= sp.chunks && !a.cluster) return; // (a cluster stays together)
 	const int H = c.heads, dim = c.dim;
 
 	auto position = [&](int j) { return j < kept ? j : lo + (j - kept); };
@@ -259,46 +263,51 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 		const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
 		return (unsigned)id < (unsigned)c.pages ? id : -1;
 	};
-	AtStage<D>* const mine = ring + warp * ST;
-	int next = begin + warp, next_page = page_of(next), stage_in = 0; // the chunk to request, its page
-	const int piece = lane % PIECES, prow = lane / PIECES;            // which piece of which row of a group of 32 pieces this lane copies
-	uint32_t swizzle[2];                                              // where, for even and odd groups (rows of 128 bytes)
+	AtStage<D>& s = ring[warp];
+	int next = begin + warp, next_page = page_of(next), next_row = 0; // the chunk to request, the page and the row of this lane's key
+	uint32_t next_seen = 0;
+	const int piece = lane % PIECES, prow = lane / PIECES; // which piece of which row of a group of 32 pieces this lane copies
+	uint32_t swizzle[2];                                   // where, for even and odd groups (rows of 128 bytes)
 #pragma unroll
 	for (int i = 0; i < 2; ++i) swizzle[i] = at_place<D>(prow + i * 4, piece) * 16;
-	auto request = [&]() {
-		if (next < end) {
-			AtStage<D>& s = mine[stage_in];
-			const int id = next_page;
-			const uint32_t seen = __ballot_sync(0xffffffffu, id >= 0);
-			const int unit = max(id, 0) * H + kvh, row = unit * c.page + page_row(c, position(min(next * AT_KEYS + lane, total - 1))); // (rows of a pool: under 2^31)
-			if (lane == 0) s.seen = seen;
-			cp4(s.ks + lane, c.ks + unit, id >= 0), cp4(s.vs + lane, c.vs + unit, id >= 0);
-			const uint32_t kd = smem_u32(s.k) + prow * D, vd = smem_u32(s.v) + prow * D;
-			const uint8_t *const kp = c.k + piece * 16, *const vp = c.v + piece * 16;
-			if (seen == 0xffffffffu && dim == D) {
+	auto copy = [&](uint8_t* to, const uint8_t* from) { // the next chunk's keys or values
+		const uint32_t dst = smem_u32(to) + prow * D;
+		const uint8_t* const src = from + piece * 16;
+		if (next_seen == 0xffffffffu && dim == D) {
 #pragma unroll
-				for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
-					const long long o = (long long)__shfl_sync(0xffffffffu, row, i * (32 / PIECES) + prow) * D;
-					const uint32_t place = i * (32 / PIECES) * D + (D == 128 ? swizzle[i & 1] : at_place<D>(i * (32 / PIECES) + prow, piece) * 16);
-					cp16(kd + place, kp + o), cp16(vd + place, vp + o);
-				}
-			} else {
-#pragma unroll
-				for (int i = 0; i < PIECES; ++i) {
-					const int r = i * (32 / PIECES) + prow;
-					const long long o = (long long)__shfl_sync(0xffffffffu, row, r) * dim;
-					const bool there = (seen >> r & 1) && piece * 16 < dim;
-					const uint32_t place = i * (32 / PIECES) * D + at_place<D>(r, piece) * 16;
-					cp16(kd + place, there ? kp + o : c.k, there), cp16(vd + place, there ? vp + o : c.v, there);
-				}
+			for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
+				const long long o = (long long)__shfl_sync(0xffffffffu, next_row, i * (32 / PIECES) + prow) * D;
+				cp16(dst + i * (32 / PIECES) * D + (D == 128 ? swizzle[i & 1] : at_place<D>(i * (32 / PIECES) + prow, piece) * 16), src + o);
 			}
-			stage_in = stage_in + 1 == ST ? 0 : stage_in + 1;
+		} else {
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) {
+				const int r = i * (32 / PIECES) + prow;
+				const long long o = (long long)__shfl_sync(0xffffffffu, next_row, r) * dim;
+				const bool there = (next_seen >> r & 1) && piece * 16 < dim;
+				cp16(dst + i * (32 / PIECES) * D + at_place<D>(r, piece) * 16, there ? src + o : from, there);
+			}
+		}
+	};
+	auto request_keys = [&](int half) { // and both scales, in this half of their arrays
+		if (next < end) {
+			const int id = next_page, unit = max(id, 0) * H + kvh;
+			next_seen = __ballot_sync(0xffffffffu, id >= 0);
+			next_row = unit * c.page + page_row(c, position(min(next * AT_KEYS + lane, total - 1))); // (rows of a pool: under 2^31)
+			if (lane == 0) s.seen[half] = next_seen;
+			cp4(s.ks[half] + lane, c.ks + unit, id >= 0), cp4(s.vs[half] + lane, c.vs + unit, id >= 0);
+			copy(s.k, c.k);
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	};
+	auto request_values = [&]() { // of the chunk whose keys were requested last
+		if (next < end) {
+			copy(s.v, c.v);
 			next += AT_WARPS, next_page = page_of(next);
 		}
 		asm volatile("cp.async.commit_group;" ::: "memory");
 	};
-#pragma unroll
-	for (int i = 0; i < ST - 1; ++i) request();
+	request_keys(0), request_values();
 
 	// Queries as B fragments, times a power of two that is the tile's: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
 	// thread's codes of a key lie side by side).
@@ -358,13 +367,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 	}
 	const int wide = at_low(a, sp.last); // from here on, and up to `first`, every row sees every key
 
-	int stage = 0;
-	for (int chunk = begin + warp; chunk < end; chunk += AT_WARPS) {
-		asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+	int half = 0;
+	for (int chunk = begin + warp; chunk < end; chunk += AT_WARPS, half ^= 1) {
+		asm volatile("cp.async.wait_group 1;" ::: "memory"); // the keys; the values are the group behind them
 		__syncwarp();
-		request(); // into the stage that was used up last
-		const AtStage<D>& s = mine[stage];
-		stage = stage + 1 == ST ? 0 : stage + 1;
 		// scores: rows g and g + 8 of product i are keys 16 i + g, + 8
 		float z[2][NQ][4];
 #pragma unroll
@@ -390,33 +396,60 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 			}
 		}
 		// with the value's scale in the exponent; this thread's keys are 8 j + g
-		const uint32_t seen = s.seen;
+		__syncwarp(); // every lane has its keys
+		request_keys(half ^ 1);
+		const uint32_t seen = s.seen[half];
 		const int j0 = chunk * AT_KEYS;
 		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= sp.first;
 		float over[4]; // 1 / value scale
-		bool move = false;
+		if (extra) { // a soft cap or slopes
+#pragma unroll 1
+			for (int j = 0; j < 4; ++j) {
+				const int kp = position(j0 + 8 * j + g);
+				const float kf = s.ks[half][8 * j + g] * qscale;
+#pragma unroll
+				for (int q = 0; q < NQ; ++q)
+#pragma unroll
+					for (int e = 0; e < 2; ++e) {
+						float y = (j & 2 ? (j & 1 ? z[1][q][2 + e] : z[1][q][e]) : (j & 1 ? z[0][q][2 + e] : z[0][q][e])) * kf;
+						if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
+						if (a.slopes) y -= a.slopes[kvh * a.group + (row0 + min(8 * q + 2 * t + e, rows - 1)) % a.group] * (float)(rpos[q][e] - kp);
+						y *= AT_LOG2E;
+						if (j == 0) z[0][q][e] = y;
+						else if (j == 1) z[0][q][2 + e] = y;
+						else if (j == 2) z[1][q][e] = y;
+						else z[1][q][2 + e] = y;
+					}
+			}
+		}
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			const float kf = s.ks[8 * j + g] * qscale;
-			const int ve = max((int)(__float_as_uint(s.vs[8 * j + g]) >> 23) - 127, -126);
+			const float kf = extra ? 1.f : s.ks[half][8 * j + g] * qscale;
+			const int ve = max((int)(__float_as_uint(s.vs[half][8 * j + g]) >> 23) - 127, -126);
 			const float lv = (float)ve;
 			over[j] = pow2f(-ve);
-			const int kp = position(j0 + 8 * j + g);
 #pragma unroll
 			for (int q = 0; q < NQ; ++q)
 #pragma unroll
-				for (int e = 0; e < 2; ++e) {
-					float& y = z[j >> 1][q][(j & 1) * 2 + e];
-					if (extra) {
-						y *= kf;
-						if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
-						if (a.slopes) y -= a.slopes[kvh * a.group + (row0 + min(8 * q + 2 * t + e, rows - 1)) % a.group] * (float)(rpos[q][e] - kp);
-						y = fmaf(y, AT_LOG2E, lv);
-					} else y = fmaf(y, kf, lv);
-					if (!all && !((seen >> (8 * j + g) & 1) && kp <= rpos[q][e] && (kp >= at_low(a, rpos[q][e]) || kp < a.keep_first))) y = -INFINITY;
-					move |= y > m[q][e] + AT_MOST;
-				}
+				for (int e = 0; e < 2; ++e) z[j >> 1][q][(j & 1) * 2 + e] = fmaf(z[j >> 1][q][(j & 1) * 2 + e], kf, lv);
 		}
+		if (!all) { // some row does not see some key
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				const int kp = position(j0 + 8 * j + g);
+				const bool there = seen >> (8 * j + g) & 1, early = kp < a.keep_first;
+#pragma unroll
+				for (int q = 0; q < NQ; ++q)
+#pragma unroll
+					for (int e = 0; e < 2; ++e)
+						if (!(there && kp <= rpos[q][e] && (early || kp >= at_low(a, rpos[q][e])))) z[j >> 1][q][(j & 1) * 2 + e] = -INFINITY;
+			}
+		}
+		bool move = false;
+#pragma unroll
+		for (int q = 0; q < NQ; ++q)
+#pragma unroll
+			for (int e = 0; e < 2; ++e) move |= fmaxf(fmaxf(z[0][q][e], z[0][q][2 + e]), fmaxf(z[1][q][e], z[1][q][2 + e])) > m[q][e] + AT_MOST;
 		if (__any_sync(0xffffffffu, move)) { // references move
 #pragma unroll
 			for (int q = 0; q < NQ; ++q) {
@@ -451,6 +484,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 				if (SPLIT) pl[i][q] = make_uint2(transposed(pack_rest(z[i][q][0], z[i][q][1], h0)), transposed(pack_rest(z[i][q][2], z[i][q][3], h1)));
 			}
 		}
+		asm volatile("cp.async.wait_group 1;" ::: "memory"); // the values; the next keys are the group behind them
+		__syncwarp();
 		// values: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step kk is key 16 kk + 2t + {0, 1}, + 8; rows g and g + 8 of product i are channels g * D / 8 + 2 i + {0, 1}
 #pragma unroll
 		for (int kk = 0; kk < 2; ++kk) {
@@ -481,6 +516,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 				}
 			}
 		}
+		__syncwarp(); // every lane has its values
+		request_values();
 	}
 	asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
@@ -494,7 +531,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 
 	// the warps' sums as one, eight rows at a time
 	float* const sums = reinterpret_cast<float*>(ring); // [warps][8][LD]: channel d at d / (D / 8) * FS + d % (D / 8)
+	float* const own = sums + AT_WARPS * 8 * LD;              // [16][D + 2]: what this share of a cluster found
 	const bool whole = sp.chunks <= a.each || a.shares == 1; // no other share has keys
+	if (whole && share > 0) return;                          // (nor does any of the cluster wait)
 #pragma unroll
 	for (int q = 0; q < NQ; ++q) {
 		if (8 * q >= rows) break;
@@ -514,7 +553,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 #pragma unroll
 			for (int w = 0; w < AT_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
 			const int token = start + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
-			float* const part = whole ? nullptr : a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2);
+			float* const part = whole ? nullptr : a.cluster ? own + r * (D + 2) : a.part + (((size_t)token * a.heads + head) * a.shares + share) * (dim + 2);
 			float norm = 0.f;
 			if (whole) {
 				if (a.sinks) { // one more term of the denominator
@@ -532,6 +571,41 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 64 ? 4 : NQ * D <= 25
 			}
 		}
 	}
+	if (whole || !a.cluster) return;
+	// A cluster's shares: each CTA finishes its part of the outputs from all of them.
+	__shared__ float wz[AT_CLUSTER][AT_CLUSTER_ROWS], inv[AT_CLUSTER_ROWS];
+	const int shares = min(a.shares, (sp.chunks + a.each - 1) / a.each);
+	cluster_sync();
+	if (tid < rows) {
+		const int head = kvh * a.group + (row0 + tid) % a.group;
+		const float sk = a.sinks ? a.sinks[head] * AT_LOG2E : -INFINITY;
+		float ms[AT_CLUSTER], ls[AT_CLUSTER], mx = sk, den = 0.f;
+#pragma unroll
+		for (int k = 0; k < AT_CLUSTER; ++k) {
+			ms[k] = -INFINITY, ls[k] = 0.f;
+			if (k < shares) ms[k] = cluster_load_f32(cluster_addr(own + tid * (D + 2) + dim, k)), ls[k] = cluster_load_f32(cluster_addr(own + tid * (D + 2) + dim + 1, k));
+		}
+#pragma unroll
+		for (int k = 0; k < AT_CLUSTER; ++k) mx = fmaxf(mx, ms[k]);
+#pragma unroll
+		for (int k = 0; k < AT_CLUSTER; ++k)
+			if (k < shares) {
+				const float f = ms[k] == -INFINITY ? 0.f : ex2(ms[k] - mx);
+				wz[k][tid] = f, den = fmaf(f, ls[k], den);
+			}
+		if (a.sinks) den += ex2(sk - mx);
+		inv[tid] = den > 0.f ? 1.f / den : den; // (0: nothing was seen)
+	}
+	__syncthreads();
+	const int all = rows * dim, from = (int)((long long)all * share / a.shares), to = (int)((long long)all * (share + 1) / a.shares);
+	for (int e = from + tid; e < to; e += 32 * AT_WARPS) {
+		const int r = e / dim, d = e - r * dim;
+		float v = 0.f;
+#pragma unroll 8
+		for (int k = 0; k < shares; ++k) v = fmaf(cluster_load_f32(cluster_addr(own + r * (D + 2) + d, k)), wz[k][r], v);
+		at_finish(a, start + (row0 + r) / a.group, kvh * a.group + (row0 + r) % a.group, d, v * inv[r]);
+	}
+	cluster_sync(); // no CTA leaves while another reads what it found
 }
 
 // Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.
@@ -609,30 +683,38 @@ StoreRows store_rows(const SeqRows& r) {
 	return StoreRows{r.p, r.row_stride, r.head_stride, r.rows, (uintptr_t)r.p % bytes == 0 && r.row_stride % 4 == 0 && r.head_stride % 4 == 0};
 }
 
-// Shares of the keys of a tile of rows, and the chunks of each.  Sequences differ in length: shares of one length for all of them, short ones have fewer.  As many CTAs as the GPU
-// holds at a time where there are few; where there are more, shares that leave the last CTAs little to wait for; two chunks a warp at least.
+// How the work is cut: rows of a CTA; shares of a tile's keys and the chunks of each (sequences differ in length: shares of one length for all of them, short ones have fewer);
+// whether a cluster folds the shares.
 struct AtPlan {
-	int shares, each;
+	int tile, shares, each, cluster;
 };
-// Rows of a CTA: eight fill a product; more where a sequence has more, so that codes are read and converted once for all of them, as far as registers hold their sums.
+constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
+// Rows of a CTA: eight fill a product; more, where a sequence has more, read and convert the codes once for all of them, as far as registers hold their sums and CTAs are enough
+// for the GPU all the same.
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const long long rows = (long long)p.longest * (a.heads / c.heads);
-	return rows <= 8 ? 8 : rows <= 16 || c.dim > 128 ? 16 : 32;
+	auto ctas = [&](int tile) { return (long long)p.n * cdiv(rows, tile) * c.heads; };
+	if (rows > 16 && c.dim <= 128 && ctas(32) >= AT_ROOM) return 32;
+	return rows > 8 && ctas(16) >= AT_ROOM / 2 ? 16 : 8;
 }
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const int group = a.heads / c.heads, tile = attend_tile(c, p, a);
-	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, tile) * c.heads, room = 148 * 3;
+	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, tile) * c.heads, room = AT_ROOM;
 	long long keys = std::max(a.most_keys, 1);
 	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + tile / group);
 	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + tile / group);
 	const int chunks = cdiv(keys, AT_KEYS);
-	if (ctas < 1) return AtPlan{1, chunks};
-	long long shares = ctas >= 4 * room ? 1 : ctas > room / 2 ? cdiv(4 * room, ctas) : room / ctas;
-	shares = std::max(1LL, std::min({shares, (long long)chunks / (2 * AT_WARPS), (long long)AT_SHARES}));
+	if (ctas < 1) return AtPlan{tile, 1, chunks, 0};
+	// many CTAs: several rounds, so that the last one is short
+	long long shares = ctas >= 6 * room ? 1 : ctas > room / 2 ? cdiv(6 * room, ctas) : room / ctas;
+	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, ctas > room / 2 ? 2 * AT_WARPS : AT_WARPS), (long long)AT_SHARES}));
+	// one round: a cluster folds them, and the fold's launch is saved
+	const bool cluster = shares > 1 && ctas <= room / 2 && tile <= AT_CLUSTER_ROWS;
+	if (cluster) shares = shares >= 16 ? 16 : shares >= 8 ? 8 : shares >= 4 ? 4 : 2;
 	const int each = cdiv(chunks, shares);
-	return AtPlan{cdiv(chunks, each), each};
+	return AtPlan{tile, cluster ? (int)shares : cdiv(chunks, each), each, cluster};
 }
-size_t attend_bytes(const SeqCache8& c, const SeqAttend8& a, int shares) { return shares > 1 ? (size_t)a.q.rows * a.heads * shares * (c.dim + 2) * sizeof(float) : 0; }
+size_t attend_bytes(const SeqCache8& c, const SeqAttend8& a, const AtPlan& p) { return p.shares > 1 && !p.cluster ? (size_t)a.q.rows * a.heads * p.shares * (c.dim + 2) * sizeof(float) : 0; }
 
 int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) {
 	if (const int rc = check_cache("attend8", c, p)) return rc;
@@ -651,7 +733,8 @@ template <int D, bool SPLIT, int NQ>
 cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	constexpr size_t smem = at_smem<D, SPLIT, NQ>();
 	cudaError_t e = cudaFuncSetAttribute(k_c8_attend<D, SPLIT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_attend<D, SPLIT, NQ>, grid, dim3(32 * AT_WARPS), smem, c, a);
+	if (e == cudaSuccess && a.cluster && a.shares > 8) e = cudaFuncSetAttribute(k_c8_attend<D, SPLIT, NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+	if (e == cudaSuccess) e = launch(st, false, a.cluster ? a.shares : 1, k_c8_attend<D, SPLIT, NQ>, grid, dim3(32 * AT_WARPS), smem, c, a);
 	return e;
 }
 template <int D>
@@ -663,6 +746,11 @@ cudaError_t attend_wide(const C8& c, const Attend& a, dim3 grid, cudaStream_t st
 	return split ? attend_launch<DD, true, 4>(c, a, grid, st) : attend_launch<DD, false, 4>(c, a, grid, st);
 }
 } // namespace
+
+void attend8_plan(const SeqCache8& cache, const SeqPortions& batch, const SeqAttend8& args, int (&plan)[4]) {
+	const AtPlan p = attend_plan(cache, batch, args);
+	plan[0] = p.tile, plan[1] = p.shares, plan[2] = p.each, plan[3] = p.cluster;
+}
 } // namespace seqops
 
 extern "C" int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqRows* k, const struct SeqRows* v, void* stream) {
@@ -684,7 +772,7 @@ extern "C" int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const s
 extern "C" size_t calm_b200_seq_attend8_workspace(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args) {
 	using namespace seqops;
 	if (check_attend(cache, batch, args)) return 0;
-	return attend_bytes(*cache, *args, attend_plan(*cache, *batch, *args).shares);
+	return attend_bytes(*cache, *args, attend_plan(*cache, *batch, *args));
 }
 
 extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* q, void* stream) {
@@ -693,7 +781,7 @@ extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct
 	if (batch->n == 0 || batch->longest == 0) return 0;
 	const AtPlan plan = attend_plan(*cache, *batch, *q);
 	const int shares = plan.shares;
-	const size_t need = attend_bytes(*cache, *q, shares);
+	const size_t need = attend_bytes(*cache, *q, plan);
 	if (need && (!q->workspace || (uintptr_t)q->workspace % 16 || q->workspace_bytes < need)) return refuse("attend8: the workspace has %zu bytes (16-byte aligned), %zu are needed", q->workspace ? q->workspace_bytes : (size_t)0, need);
 	const C8 c = describe(*cache, *batch);
 	Attend a;
@@ -702,11 +790,11 @@ extern "C" int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct
 	a.window = q->window, a.keep_first = q->keep_first, a.chunk = q->chunk, a.sinks = q->sinks, a.slopes = q->slopes;
 	a.gate = q->gate, a.gate_row = q->gate_row, a.gate_head = q->gate_head, a.gate_dim = q->gate_dim;
 	a.shares = shares, a.each = plan.each, a.part = (float*)q->workspace;
-	a.q_type = q->q.type, a.out_type = q->out.type, a.tile = attend_tile(*cache, *batch, *q);
+	a.q_type = q->q.type, a.out_type = q->out.type, a.tile = plan.tile, a.cluster = plan.cluster;
 	const dim3 grid(cdiv((long long)batch->longest * a.group, a.tile), cache->heads * shares, batch->n), fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 	if (grid.y > 65535) return refuse("attend8: too many key heads");
 	const cudaStream_t st = (cudaStream_t)stream;
 	cudaError_t e = cache->dim <= 64 ? attend_wide<64>(c, a, grid, st) : cache->dim <= 128 ? attend_wide<128>(c, a, grid, st) : attend_wide<256>(c, a, grid, st);
-	if (e == cudaSuccess && shares > 1) e = launch(st, true, 1, k_c8_fold, fold, dim3(128), 0, c, a);
+	if (e == cudaSuccess && shares > 1 && !plan.cluster) e = launch(st, true, 1, k_c8_fold, fold, dim3(128), 0, c, a);
 	return e == cudaSuccess ? 0 : failed("attend8", e);
 }

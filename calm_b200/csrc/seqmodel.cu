@@ -1558,12 +1558,13 @@ void forward_decode_graph(Seq& s, const SeqBatch& sb, int n_want, double kv_rows
 	size_t part_need = 0;
 	auto one = [&](const SeqLayer& L, const RunState& r) {
 		if (L.type != SEQ_LATENT && L.type != SEQ_WINDOW && L.type != SEQ_GQA) return; // recurrent mixers: nothing to share out
-		if (L.cache8) { // the workspace it needs tells the shares
+		if (L.cache8) {
 			const SeqCache8 c = cache8_of(s, L, r);
 			const SeqPortions p = portions_of(s, sb);
 			const SeqAttend8 a = attend8_of(s, L, r, nullptr, 0, s.a2, sb.N, longest);
-			const size_t need = calm_b200_seq_attend8_workspace(&c, &p, &a) / sizeof(float);
-			key.push_back((int)(need / ((size_t)sb.N * L.heads * (L.dim + 2)))), part_need = std::max(part_need, need);
+			int plan[4];
+			seqops::attend8_plan(c, p, a, plan);
+			key.insert(key.end(), plan, plan + 4), part_need = std::max(part_need, calm_b200_seq_attend8_workspace(&c, &p, &a) / sizeof(float));
 			return;
 		}
 		const bool lat = L.type == SEQ_LATENT;

@@ -20,19 +20,22 @@ int sm_count(); // of the current device
 void count_launch();
 uint64_t launches(); // since the library was loaded
 
+// how calm_b200_seq_attend8 cuts its work (a captured call keeps it): rows of a CTA, shares of the keys, chunks of each, whether clusters fold them
+void attend8_plan(const SeqCache8& cache, const SeqPortions& batch, const SeqAttend8& args, int (&plan)[4]);
+
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// `after`: programmatic dependent launch behind the previous kernel of the stream, which the kernel waits for with pdl_wait_prev()
+// Clusters of cluster_y CTAs along y.  `after`: programmatic dependent launch behind the previous kernel of the stream, which the kernel waits for with pdl_wait_prev()
 template <typename... KArgs, typename... Args>
-cudaError_t launch(cudaStream_t st, bool after, int cluster_x, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
+cudaError_t launch(cudaStream_t st, bool after, int cluster_y, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
 	cudaLaunchAttribute at[2];
 	int n = 0;
 	if (after) at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[n++].val.programmaticStreamSerializationAllowed = 1;
-	if (cluster_x > 1) {
+	if (cluster_y > 1) {
 		at[n].id = cudaLaunchAttributeClusterDimension;
-		at[n].val.clusterDim.x = cluster_x, at[n].val.clusterDim.y = 1, at[n++].val.clusterDim.z = 1;
+		at[n].val.clusterDim.x = 1, at[n].val.clusterDim.y = cluster_y, at[n++].val.clusterDim.z = 1;
 	}
 	cfg.attrs = at, cfg.numAttrs = n;
 	count_launch();
