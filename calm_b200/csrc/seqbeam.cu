@@ -466,6 +466,13 @@ int beam_slices(int groups, int beams, int vocab) {
 }
 size_t beam_keys(int groups, int beams, int vocab, int n) { return ((size_t)groups * beams * beam_slices(groups, beams, vocab) * n * sizeof(u64) + 15) & ~(size_t)15; }
 
+template <typename T>
+cudaError_t beam_launch(const BeamArgs& a, dim3 grid, cudaStream_t st) {
+	static std::atomic<uint64_t> done{0};
+	const cudaError_t e = allow(k_beam_slice<T>, sizeof(BeamSlice), done);
+	return e == cudaSuccess ? launch(st, false, 1, k_beam_slice<T>, grid, dim3(BM_THREADS), sizeof(BeamSlice), a) : e;
+}
+
 int beam_check(int groups, int beams, int vocab, int n) {
 	if (groups < 0 || beams < 1 || beams > 64) return refuse("beam: %d groups of %d beams (at most 64 beams)", groups, beams);
 	if (vocab < 1 || (long long)beams * vocab >= (1LL << 31)) return refuse("beam: %d beams over %d tokens: at most 2^31 candidates", beams, vocab);
@@ -499,11 +506,10 @@ extern "C" int calm_b200_seq_beam_select(const struct SeqBeam* q, void* stream) 
 	a.keys = (u64*)q->workspace, a.sums = (float2*)((char*)q->workspace + beam_keys(q->groups, q->beams, q->vocab, q->n));
 	const cudaStream_t st = (cudaStream_t)stream;
 	const dim3 grid(a.slices, q->groups * q->beams);
-	auto kernel = q->type == SEQ_F32 ? k_beam_slice<float> : q->type == SEQ_BF16 ? k_beam_slice<__nv_bfloat16> : k_beam_slice<__half>;
-	cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BeamSlice));
-	if (e == cudaSuccess) e = launch(st, false, 1, kernel, grid, dim3(BM_THREADS), sizeof(BeamSlice), a);
+	cudaError_t e = q->type == SEQ_F32 ? beam_launch<float>(a, grid, st) : q->type == SEQ_BF16 ? beam_launch<__nv_bfloat16>(a, grid, st) : beam_launch<__half>(a, grid, st);
 	if (e != cudaSuccess) return failed("beam", e);
-	if ((e = cudaFuncSetAttribute(k_beam_merge, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BeamCand))) != cudaSuccess) return failed("beam", e);
-	e = launch(st, true, 1, k_beam_merge, dim3(q->groups), dim3(BM_THREADS), sizeof(BeamCand), a);
+	static std::atomic<uint64_t> done{0};
+	e = allow(k_beam_merge, sizeof(BeamCand), done);
+	if (e == cudaSuccess) e = launch(st, true, 1, k_beam_merge, dim3(q->groups), dim3(BM_THREADS), sizeof(BeamCand), a);
 	return e == cudaSuccess ? 0 : failed("beam", e);
 }

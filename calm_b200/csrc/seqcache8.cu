@@ -732,8 +732,8 @@ int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) 
 template <int D, bool SPLIT, int NQ>
 cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	constexpr size_t smem = at_smem<D, SPLIT, NQ>();
-	cudaError_t e = cudaFuncSetAttribute(k_c8_attend<D, SPLIT, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-	if (e == cudaSuccess && a.cluster && a.shares > 8) e = cudaFuncSetAttribute(k_c8_attend<D, SPLIT, NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+	static std::atomic<uint64_t> done{0};
+	cudaError_t e = allow(k_c8_attend<D, SPLIT, NQ>, smem, done, true);
 	if (e == cudaSuccess) e = launch(st, false, a.cluster ? a.shares : 1, k_c8_attend<D, SPLIT, NQ>, grid, dim3(32 * AT_WARPS), smem, c, a);
 	return e;
 }

@@ -7,6 +7,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/calm_b200_seq.h"
 #include "common.cuh"
 
@@ -40,6 +42,18 @@ cudaError_t launch(cudaStream_t st, bool after, int cluster_y, void (*kernel)(KA
 	cfg.attrs = at, cfg.numAttrs = n;
 	count_launch();
 	return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+// More than 48 KB of shared memory (and clusters of more than eight) for a kernel, asked for once on every device.
+template <typename... KArgs>
+cudaError_t allow(void (*kernel)(KArgs...), size_t smem, std::atomic<uint64_t>& done, bool wide_clusters = false) {
+	int dev = 0;
+	cudaError_t e = cudaGetDevice(&dev);
+	if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+	e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+	if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+	if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+	return e;
 }
 
 inline int type_size(int t) { return t == SEQ_F32 ? 4 : 2; }

@@ -7,6 +7,7 @@ ValueError before anything is launched.  Like everywhere in this package there i
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -72,31 +73,31 @@ def _check(rc: int) -> None:
     raise ValueError(text) if rc == -3 else seqlib.SeqError(text)
 
 
-class _on:
-    """The device of a call's tensors as the current one (most often it is already)."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *a):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _run(index: int, function, *args) -> None:
+    """One call of the library on torch's current stream of device `index`, with that as the current device (most often it is already)."""
+    if torch.cuda.current_device() == index:
+        _check(function(*args, _stream(index)))
+    else:
+        with torch.cuda.device(index):
+            _check(function(*args, _stream(index)))
 
 
-def _gpu(name: str, t: torch.Tensor, index: Optional[int] = None) -> int:
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+try:  # the handle itself; the stream object that carries it costs as much as a launch
+    from torch._C import _cuda_getCurrentRawStream as _stream
+except ImportError:
+
+    def _stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _gpu(name: str, t: torch.Tensor, index: int = -1) -> int:
+    """The tensor's device, which is to be `index`."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if index is not None and t.device.index != index:
+    at = t.get_device()
+    if index >= 0 and at != index:
         raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{index}")
-    return t.device.index
+    return at
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
@@ -105,37 +106,43 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, out: Optiona
     token's log-probability; where fewer than n candidates are above -inf the rest is token -1, parent -1, score -inf.  `out`: the three tensors to write."""
     index = _gpu("logits", logits)
     _gpu("scores", scores, index)
-    if logits.dim() != 3 or logits.dtype not in _TYPES or (logits.stride(2) != 1 and logits.shape[2] > 1):
+    kind = _TYPES.get(logits.dtype)
+    if logits.dim() != 3 or kind is None or (logits.stride(2) != 1 and logits.shape[2] > 1):
         raise ValueError("logits must be [groups, beams, vocab] in float32, bfloat16 or float16 with the vocabulary contiguous")
     G, K, V = logits.shape
     if scores.shape != (G, K) or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError(f"scores must be contiguous float32 [{G}, {K}]")
-    n = int(n)
-    L = _load()
-    with _on(index) as stream:
-        if out is None:
-            if not 1 <= n <= 64:
-                raise ValueError(f"beam: n = {n} is not in 1 .. 64")
-            both = torch.empty(2, G, n, dtype=torch.int32, device=logits.device)
-            tokens, parents, best = both[0], both[1], torch.empty(G, n, dtype=torch.float32, device=logits.device)
-        else:
-            tokens, parents, best = out
-            for name, t, dt in (("tokens", tokens, torch.int32), ("parents", parents, torch.int32), ("scores", best, torch.float32)):
-                _gpu(name, t, index)
-                if t.shape != (G, n) or t.dtype != dt or not t.is_contiguous():
-                    raise ValueError(f"{name} must be contiguous {dt} [{G}, {n}]")
-        work = torch.empty(max(16, L.calm_b200_seq_beam_workspace(G, K, V, n)), dtype=torch.uint8, device=logits.device)
-        a = _Beam(logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(), G, K, V, n, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(),
-                  work.data_ptr(), work.numel())
-        _check(L.calm_b200_seq_beam_select(C.byref(a), stream))
+    L, n = _load(), int(n)
+    need = L.calm_b200_seq_beam_workspace(G, K, V, n)
+    if not need and G:
+        _check(-3)
+    if out is None:
+        tokens, parents, best = torch.empty((3, G, n), dtype=torch.int32, device=logits.device).unbind(0)
+        best = best.view(torch.float32)
+    else:
+        tokens, parents, best = out
+        for name, t, dt in (("tokens", tokens, torch.int32), ("parents", parents, torch.int32), ("scores", best, torch.float32)):
+            _gpu(name, t, index)
+            if t.shape != (G, n) or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dt} [{G}, {n}]")
+    work = torch.empty(max(16, need), dtype=torch.uint8, device=logits.device)
+    a = _Beam(logits.data_ptr(), kind, logits.stride(0), logits.stride(1), scores.data_ptr(), G, K, V, n, tokens.data_ptr(), parents.data_ptr(), best.data_ptr(), work.data_ptr(), need)
+    _run(index, L.calm_b200_seq_beam_select, C.byref(a))
     return tokens, parents, best
 
 
-def _list(name: str, values) -> np.ndarray:
-    a = np.ascontiguousarray(values, np.int32)
-    if a.ndim != 1:
-        raise ValueError(f"{name} must be a list of numbers")
-    return a
+def _list(name: str, values) -> array:
+    """Host integers as a C array (an int32 numpy array is taken as it lies)."""
+    if isinstance(values, np.ndarray):
+        if values.ndim != 1 or values.dtype.kind not in "iu":
+            raise ValueError(f"{name} must be a list of whole numbers")
+        if len(values) and not -2 ** 31 <= int(values.min()) <= int(values.max()) < 2 ** 31:
+            raise ValueError(f"{name}: a number passes 32 bits")
+        return array("i", np.ascontiguousarray(values, np.int32).tobytes())
+    try:
+        return array("i", values)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{name} must be a list of whole numbers of 32 bits: {e}") from None
 
 
 class UnitPool:
@@ -147,7 +154,7 @@ class UnitPool:
         to = self.buffers if into is None else into.buffers
         if len(to) != len(self.buffers):
             raise ValueError("the pools hold different numbers of buffers")
-        self.index = None
+        self.index = -1
         self.units = (_Units * max(1, len(self.buffers)))()
         for i, ((t, kind), (d, dkind)) in enumerate(zip(self.buffers, to)):
             for x in (t, d):
@@ -169,13 +176,15 @@ class UnitPool:
         sf, st = _list("slots", slots[0]), _list("slots", slots[1])
         if len(pf) != len(pt) or len(sf) != len(st) or (pr is not None and len(pr) != len(pf)):
             raise ValueError("lists of one kind must have one length")
-        if pr is not None and len(pr) and pr.max() > self.rows:
+        if pr and max(pr) > self.rows:
             raise ValueError(f"a page has {self.rows} rows")
-        if self.index is None:
+        if self.index < 0:
             return
-        with _on(self.index) as stream:
-            _check(_load().calm_b200_seq_copy_units(len(self.buffers), self.units, len(pf), pf.ctypes.data, pt.ctypes.data, pr.ctypes.data if pr is not None else None, len(sf), sf.ctypes.data,
-                                                    st.ctypes.data, stream))
+
+        def at(a: Optional[array]) -> Optional[int]:
+            return a.buffer_info()[0] if a else None
+
+        _run(self.index, _load().calm_b200_seq_copy_units, len(self.buffers), self.units, len(pf), at(pf), at(pt), at(pr), len(sf), at(sf), at(st))
 
 
 class Batch:
@@ -183,7 +192,7 @@ class Batch:
     count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest`."""
 
     def __init__(self, slots: Sequence[int], counts: Sequence[int], before: Sequence[int], device=None):
-        sl, cn, at = _list("slots", list(slots)), _list("counts", counts), _list("before", before)
+        sl, cn, at = (np.array(_list(name, x), np.int32) for name, x in (("slots", slots), ("counts", counts), ("before", before)))
         if not len(sl) == len(cn) == len(at):
             raise ValueError("slots, counts and before must have one length")
         if len(cn) and (cn.min() < 0 or at.min() < 0 or sl.min() < 0):
@@ -201,10 +210,15 @@ class Batch:
         self.c = _Portions(len(sl), base, base + step, base + 2 * step, base + 3 * step, self.longest)
 
 
-def _rows(name: str, t: torch.Tensor, heads: int, dim: int) -> _Rows:
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.dtype not in _TYPES or (t.stride(2) != 1 and dim > 1):
+def _rows(name: str, t: torch.Tensor, index: int, heads: int, dim: int, least: int) -> _Rows:
+    _gpu(name, t, index)
+    kind, stride = _TYPES.get(t.dtype), t.stride()
+    if kind is None or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (stride[2] != 1 and dim > 1):
         raise ValueError(f"{name} must be [tokens, {heads}, {dim}] in float32, bfloat16 or float16 with the channels contiguous, not {list(t.shape)} {t.dtype}")
-    return _Rows(t.data_ptr(), _TYPES[t.dtype], t.stride(0), t.stride(1), t.shape[0])
+    n = t.shape[0]
+    if n < least:
+        raise ValueError(f"{name} has {n} rows for {least} tokens")
+    return _Rows(t.data_ptr(), kind, stride[0], stride[1], n)
 
 
 class Cache8:
@@ -223,6 +237,7 @@ class Cache8:
                 raise ValueError(f"scales must be contiguous float32 {list(k.shape[:2])}")
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
         self.pages, self.heads, self.page, self.dim = k.shape
+        self._pool = (k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), self.pages, self.heads, self.page, self.dim)
         if self.dim % 16 or not 16 <= self.dim <= 256:
             raise ValueError(f"rows of {self.dim} channels: a multiple of 16 up to 256 is served")
 
@@ -242,19 +257,15 @@ class Cache8:
             raise ValueError("the page table must be contiguous int32 [slots, pages of a slot]")
         if batch.index != self.index:
             raise ValueError(f"the batch is on cuda:{batch.index}, the cache on cuda:{self.index}")
-        return _Cache8(self.k.data_ptr(), self.k_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(), self.pages, self.heads, self.page, self.dim, table.data_ptr(), table.shape[0],
-                       table.shape[1])
+        slots, table_pages = table.shape
+        return _Cache8(*self._pool, table.data_ptr(), slots, table_pages)
 
     def store(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, batch: Batch) -> None:
         """The batch's key and value rows [tokens, heads, dim] into the pages that `table` (int32 [slots, pages of a slot]) names for their positions.  Scales grow to what
         the rows need, earlier rows of a page are rounded to the raised scale."""
-        c = self._with(table, batch)
-        _gpu("k", k, self.index), _gpu("v", v, self.index)
-        rk, rv = _rows("k", k, self.heads, self.dim), _rows("v", v, self.heads, self.dim)
-        if rk.rows < batch.tokens or rv.rows < batch.tokens:
-            raise ValueError(f"{min(rk.rows, rv.rows)} rows for {batch.tokens} tokens")
-        with _on(self.index) as stream:
-            _check(_load().calm_b200_seq_cache8_store(C.byref(c), C.byref(batch.c), C.byref(rk), C.byref(rv), stream))
+        c, n = self._with(table, batch), batch.tokens
+        rk, rv = _rows("k", k, self.index, self.heads, self.dim, n), _rows("v", v, self.index, self.heads, self.dim, n)
+        _run(self.index, _load().calm_b200_seq_cache8_store, C.byref(c), C.byref(batch.c), C.byref(rk), C.byref(rv))
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, batch: Batch, scale: float, window: int = 0, keep_first: int = 0, chunk: int = 0, softcap: float = 0.0,
                sink: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -262,35 +273,30 @@ class Cache8:
         to its own: the last `window` of them and the first `keep_first`, or those from its block of `chunk` positions on.  sink: float32 [query heads], one more logit in the
         softmax's denominator; slopes: float32 [query heads], times the distance taken off the scores; gate: float32 [tokens, query heads, dim] (strides as they are, 0 too), its
         sigmoid multiplies the result.  Rows of q behind the batch's tokens stay as they are in `out` (zero without one)."""
-        c = self._with(table, batch)
-        _gpu("q", q, self.index)
-        if q.dim() != 3:
+        c, index = self._with(table, batch), self.index
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q must be [tokens, query heads, dim]")
         heads = q.shape[1]
-        rq = _rows("q", q, heads, self.dim)
-        if rq.rows < batch.tokens:
-            raise ValueError(f"{rq.rows} rows for {batch.tokens} tokens")
+        rq = _rows("q", q, index, heads, self.dim, batch.tokens)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if rq.rows == batch.tokens else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        ro = _rows("out", out, index, heads, self.dim, rq.rows)
+        a = _Attend8(rq, ro, heads, scale, window, keep_first, chunk, softcap, None, None, None, 0, 0, 0, batch.most_keys, None, 0)
+        for name, t in (("sink", sink), ("slopes", slopes)):
+            if t is not None:
+                _gpu(name, t, index)
+                if t.shape != (heads,) or t.dtype != torch.float32 or not t.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous float32 [{heads}]")
+                setattr(a, "sinks" if name == "sink" else "slopes", t.data_ptr())
+        if gate is not None:
+            _gpu("gate", gate, index)
+            if gate.shape != q.shape or gate.dtype != torch.float32:
+                raise ValueError(f"gate must be float32 {list(q.shape)}")
+            a.gate, a.gate_row, a.gate_head, a.gate_dim = gate.data_ptr(), gate.stride(0), gate.stride(1), gate.stride(2)
         L = _load()
-        with _on(self.index) as stream:
-            if out is None:
-                out = (torch.empty if rq.rows == batch.tokens else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-            _gpu("out", out, self.index)
-            ro = _rows("out", out, heads, self.dim)
-            a = _Attend8(rq, ro, heads, scale, window, keep_first, chunk, softcap, None, None, None, 0, 0, 0, batch.most_keys, None, 0)
-            for name, t in (("sink", sink), ("slopes", slopes)):
-                if t is not None:
-                    _gpu(name, t, self.index)
-                    if t.shape != (heads,) or t.dtype != torch.float32 or not t.is_contiguous():
-                        raise ValueError(f"{name} must be contiguous float32 [{heads}]")
-                    setattr(a, "sinks" if name == "sink" else "slopes", t.data_ptr())
-            if gate is not None:
-                _gpu("gate", gate, self.index)
-                if gate.shape != q.shape or gate.dtype != torch.float32:
-                    raise ValueError(f"gate must be float32 {list(q.shape)}")
-                a.gate, a.gate_row, a.gate_head, a.gate_dim = gate.data_ptr(), gate.stride(0), gate.stride(1), gate.stride(2)
-            need = L.calm_b200_seq_attend8_workspace(C.byref(c), C.byref(batch.c), C.byref(a))
-            if need:
-                work = torch.empty(need, dtype=torch.uint8, device=q.device)
-                a.workspace, a.workspace_bytes = work.data_ptr(), need
-            _check(L.calm_b200_seq_attend8(C.byref(c), C.byref(batch.c), C.byref(a), stream))
+        need = L.calm_b200_seq_attend8_workspace(C.byref(c), C.byref(batch.c), C.byref(a))
+        if need:
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), need
+        _run(index, L.calm_b200_seq_attend8, C.byref(c), C.byref(batch.c), C.byref(a))
         return out

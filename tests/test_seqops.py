@@ -119,12 +119,13 @@ def test_attend_refusals_and_workspace():
                        (dict(out=rows(rows=9)), "rows"), (dict(window=-1), "range"), (dict(keep_first=-1), "range"), (dict(chunk=-3), "range"), (dict(softcap=-1.0), "range"),
                        (dict(softcap=float("nan")), "range"), (dict(scale=float("nan")), "range"), (dict(q=rows(p=None)), "missing")):
         says(L.calm_b200_seq_attend8(*attend(**over), None), "attend8", word)
-    one = portions(n=1, longest=1)
-    need = L.calm_b200_seq_attend8_workspace(*attend(p=one, most_keys=100000))
-    assert need > 0  # one sequence: its keys are divided
-    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000), None), "workspace")
-    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000, workspace=4096, workspace_bytes=need - 1), None), "workspace")
-    says(L.calm_b200_seq_attend8(*attend(p=one, most_keys=100000, workspace=4100, workspace_bytes=need), None), "workspace")
+    few, many = portions(n=1, longest=1), portions(n=150, longest=1)
+    assert L.calm_b200_seq_attend8_workspace(*attend(p=few, most_keys=100000)) == 0  # clusters fold their shares themselves
+    need = L.calm_b200_seq_attend8_workspace(*attend(p=many, most_keys=100000))
+    assert need > 0
+    says(L.calm_b200_seq_attend8(*attend(p=many, most_keys=100000), None), "workspace")
+    says(L.calm_b200_seq_attend8(*attend(p=many, most_keys=100000, workspace=4096, workspace_bytes=need - 1), None), "workspace")
+    says(L.calm_b200_seq_attend8(*attend(p=many, most_keys=100000, workspace=4100, workspace_bytes=need), None), "workspace")
     assert L.calm_b200_seq_attend8_workspace(*attend(p=portions(n=4000, longest=1))) == 0
     assert L.calm_b200_seq_attend8(*attend(p=portions(n=0, start=None)), None) == 0
 
