@@ -608,6 +608,388 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	cluster_sync(); // no CTA leaves while another reads what it found
 }
 
+// ---------------------------------------------------------------- attention of prompts
+// Where a sequence brings many rows, the products run on the fifth-generation tensor cores: a CTA takes 128 rows (pairs of token and head, as above) of one key head and walks
+// tiles of 64 keys.  Four warps read codes, a tile ahead, and lay them out in fp16 as the products' operands (keys as they are, values transposed); one thread issues
+// S = Q K^T of the next tile and O += P V of this one; four warps, a row a thread, take S from tensor memory, form the weights (exponents, references and denominators as
+// above) and write them to shared memory as the next product's operand.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.
+//   warps 0-3  softmax and output;  4, 5  keys;  6, 7  values;  8  products
+// Bound: for 128 channels a tile costs the tensor cores 512 cycles and the exponentials as many; two CTAs share an SM.
+constexpr int AP_ROWS = 128, AP_KEYS = 64, AP_THREADS = 288, C8_NONE = -1000;
+__device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
+	const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+	return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <int D, bool SPLIT>
+struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
+	static constexpr int PANELS = D / 64, PAIR = SPLIT ? 2 : 1;
+	unsigned char q[PAIR][PANELS][AP_ROWS * 128];
+	unsigned char k[2][PANELS][AP_KEYS * 128];
+	unsigned char v[2][D * 128];
+	unsigned char p[PAIR][AP_ROWS * 128];
+	float factor[2][AP_KEYS]; // of a tile's keys on their scores, in log2
+	float bias[2];            // log2 of the largest of the tile's value scales: its values come in units of that
+	uint32_t seen[2][2];      // keys that are there
+	uint64_t kv_full[2], kv_empty[2], s_full[2], s_empty[2], p_full, p_empty, done;
+	uint32_t tmem;
+	float top[4];
+	int lost;
+};
+// false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN
+__device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity, int* lost) {
+	for (unsigned spins = 0; spins < MBAR_SPINS; ++spins) {
+		if (mbar_try_wait(bar, parity)) return true;
+		if ((spins & 63) == 63 && *(volatile int*)lost) return false;
+	}
+	*(volatile int*)lost = 1;
+	return false;
+}
+__device__ __forceinline__ bool ap_wait_warp(uint64_t* bar, uint32_t parity, int* lost) { return __all_sync(0xffffffffu, ap_wait(bar, parity, lost)); }
+// eight neighbours as floats
+__device__ __forceinline__ void load8(const void* p, int type, long long i, bool vec, float (&x)[8]) {
+	if (!vec) {
+#pragma unroll
+		for (int k = 0; k < 8; ++k) x[k] = load_as_f32(p, type, i + k);
+	} else if (type == SEQ_F32) {
+		const float4 u = *reinterpret_cast<const float4*>((const float*)p + i), w = *reinterpret_cast<const float4*>((const float*)p + i + 4);
+		x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+	} else {
+		const uint4 w = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
+		if (type == SEQ_BF16) unpack16<bf16>(w, x);
+		else unpack16<__half>(w, x);
+	}
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+#define AP_R(i) "r"(__float_as_uint(v[i]))
+	asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+	             AP_R(0), AP_R(1), AP_R(2), AP_R(3), AP_R(4), AP_R(5), AP_R(6), AP_R(7), AP_R(8), AP_R(9), AP_R(10), AP_R(11), AP_R(12), AP_R(13), AP_R(14), AP_R(15), AP_R(16), AP_R(17),
+	             AP_R(18), AP_R(19), AP_R(20), AP_R(21), AP_R(22), AP_R(23), AP_R(24), AP_R(25), AP_R(26), AP_R(27), AP_R(28), AP_R(29), AP_R(30), AP_R(31)
+	             : "memory");
+#undef AP_R
+	asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ap_exponent(const float (&tops)[4]) { // queries times 2^-this stand at 2^AT_LIFT or less
+	const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+	return (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT;
+}
+template <int D, bool SPLIT>
+__global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C8 c, const Attend a) {
+	typedef ApShared<D, SPLIT> Shared;
+	constexpr int PANELS = Shared::PANELS, PIECES = D / 16;
+	extern __shared__ __align__(1024) unsigned char ap_raw[]; // (all of the kernel's shared memory: it starts where the swizzle's pattern does)
+	Shared& s = *reinterpret_cast<Shared*>(ap_raw);
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = gridDim.x - 1 - blockIdx.x; // (the longest rows first)
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * AP_ROWS >= (long long)n * a.group) return;
+	const int row0 = tile * AP_ROWS, rows = (int)min((long long)AP_ROWS, (long long)n * a.group - row0);
+	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
+	const int tiles = (sp.total + AP_KEYS - 1) / AP_KEYS;
+	auto position = [&](int j) { return j < sp.kept ? j : sp.lo + (j - sp.kept); };
+
+	if (warp == 8) tmem_alloc(&s.tmem, 256);
+	if (tid == 0) {
+		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 128), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1), mbar_init(s.s_empty + i, 128);
+		mbar_init(&s.p_full, 128), mbar_init(&s.p_empty, 1), mbar_init(&s.done, 1);
+		s.lost = 0;
+		mbar_init_fence();
+	}
+	// queries, times the tile's power of two
+	const int token = start + (row0 + min(tid, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(tid, rows - 1)) % a.group;
+	if (warp < 4) {
+		const long long at = token * a.q_row + head * a.q_head;
+		const int bytes = a.q_type == SEQ_F32 ? 4 : 2;
+		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * bytes) | (uintptr_t)(a.q_head * bytes)) % 16 == 0;
+		float x[8], top = 0.f;
+#pragma unroll 4
+		for (int piece = 0; piece < D / 8; ++piece) {
+			load8(a.q, a.q_type, at + piece * 8, vec, x);
+#pragma unroll
+			for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+		}
+		top = warp_max(top);
+		if (lane == 0) s.top[warp] = top;
+		asm volatile("bar.sync 1, 128;" ::: "memory");
+		const float down = tid < rows ? pow2f(-ap_exponent(s.top)) : 0.f;
+#pragma unroll 2
+		for (int piece = 0; piece < D / 8; ++piece) {
+			load8(a.q, a.q_type, at + piece * 8, vec, x);
+			uint32_t hi[4], rest[4];
+#pragma unroll
+			for (int i = 0; i < 4; ++i) hi[i] = pack_f16(x[2 * i] * down, x[2 * i + 1] * down), rest[i] = SPLIT ? pack_rest(x[2 * i] * down, x[2 * i + 1] * down, hi[i]) : 0;
+			const int place = tid * 128 + (((piece & 7) ^ (tid & 7)) << 4);
+			*reinterpret_cast<uint4*>(s.q[0][piece >> 3] + place) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+			if (SPLIT) *reinterpret_cast<uint4*>(s.q[Shared::PAIR - 1][piece >> 3] + place) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+		}
+		fence_async_smem();
+	}
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem = s.tmem; // scores: columns 0 .. 63 and 64 .. 127; sums from column 128
+	const float qscale = a.scale * pow2f(ap_exponent(s.top)) * AT_LOG2E;
+	float m = -INFINITY, l = 0.f;
+
+	if (warp < 4) {
+		const int rpos = tid < rows ? p0 + (row0 + tid) / a.group : -1, rlow = tid < rows ? at_low(a, rpos) : 0, wide = at_low(a, sp.last);
+		const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+		for (int i = 0; i < tiles; ++i) {
+			const int buf = i & 1;
+			const uint32_t parity = (i >> 1) & 1;
+			if (!ap_wait_warp(s.kv_full + buf, parity, &s.lost) || !ap_wait_warp(s.s_full + buf, parity, &s.lost)) break; // (the factors; the scores)
+			tc_fence_after();
+			const int j0 = i * AP_KEYS;
+			const uint32_t seen[2] = {s.seen[buf][0], s.seen[buf][1]};
+			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
+			const float bias = s.bias[buf];
+			float z[32];
+			auto scores = [&](int h) { // log2 of the weights of keys 32 h .. , not against the reference yet; returns the largest
+				tmem_ld32(tmem + lanes + buf * 64 + 32 * h, z);
+				float top = -INFINITY;
+#pragma unroll
+				for (int k = 0; k < 32; k += 4) {
+					const float4 f = *reinterpret_cast<const float4*>(s.factor[buf] + 32 * h + k);
+					z[k] = fmaf(z[k], f.x, bias), z[k + 1] = fmaf(z[k + 1], f.y, bias), z[k + 2] = fmaf(z[k + 2], f.z, bias), z[k + 3] = fmaf(z[k + 3], f.w, bias);
+				}
+				if (!all) {
+#pragma unroll
+					for (int k = 0; k < 32; ++k) {
+						const int kp = position(j0 + 32 * h + k);
+						if (!((seen[h] >> k & 1) && kp <= rpos && (kp >= rlow || kp < a.keep_first))) z[k] = -INFINITY;
+					}
+				}
+#pragma unroll
+				for (int k = 0; k < 32; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
+				return top;
+			};
+			float sum[2] = {0.f, 0.f};
+			auto weights = [&](int h) {
+				const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+				for (int k = 0; k < 32; k += 8) {
+					uint32_t hi[4], rest[4];
+#pragma unroll
+					for (int e = 0; e < 8; e += 2) {
+						const float w0 = ex2(z[k + e] - base), w1 = ex2(z[k + e + 1] - base);
+						sum[0] += w0, sum[1] += w1;
+						hi[e / 2] = pack_f16(w0, w1), rest[e / 2] = SPLIT ? pack_rest(w0, w1, hi[e / 2]) : 0;
+					}
+					const int place = tid * 128 + (((4 * h + k / 8) ^ (tid & 7)) << 4);
+					*reinterpret_cast<uint4*>(s.p[0] + place) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+					if (SPLIT) *reinterpret_cast<uint4*>(s.p[Shared::PAIR - 1] + place) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+				}
+			};
+			// half by half against the reference as it stands; where a row passes it, the warp looks at both halves, moves references and starts anew
+			bool moved = __any_sync(0xffffffffu, scores(0) > m + AT_MOST);
+			if (i > 0 && !ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break; // the product before has read the weights and left the sums
+			tc_fence_after();
+			if (!moved) {
+				weights(0);
+				moved = __any_sync(0xffffffffu, scores(1) > m + AT_MOST);
+			}
+			if (moved) {
+				const float top = fmaxf(scores(0), scores(1)), mn = top > m + AT_MOST ? top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn);
+				if (i > 0) { // (there are sums)
+#pragma unroll 1
+					for (int col = 0; col < D; col += 32) {
+						tmem_ld32(tmem + lanes + 128 + col, z);
+#pragma unroll
+						for (int k = 0; k < 32; ++k) z[k] *= f;
+						tmem_st32(tmem + lanes + 128 + col, z);
+					}
+				}
+				m = mn, l *= f, sum[0] = sum[1] = 0.f;
+				scores(0);
+				weights(0);
+				scores(1);
+			}
+			weights(1);
+			l = fmaf(sum[0] + sum[1], pow2f(-(int)bias), l); // the weights hold the value scale
+			tc_fence_before();
+			fence_async_smem();
+			mbar_arrive(s.s_empty + buf);
+			mbar_arrive(&s.p_full);
+		}
+		if (tiles > 0) ap_wait_warp(&s.p_empty, (tiles - 1) & 1, &s.lost);
+		tc_fence_after();
+		float norm = 1.f;
+		if (a.sinks && tid < rows) {
+			const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(m, sk), down = m == -INFINITY ? 0.f : ex2(m - mn);
+			l = l * down + ex2(sk - mn), norm = down;
+		}
+		norm = *(volatile int*)&s.lost ? NAN : l > 0.f ? norm / l : l == 0.f ? 0.f : l; // (0: nothing was seen; a NaN stays one)
+		const bool wide_store = a.out_type != SEQ_F32 && !a.gate && ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
+#pragma unroll 1
+		for (int col = 0; col < D; col += 32) {
+			float z[32];
+			__syncwarp(); // (rows behind the last one take part in the load)
+			if (tiles > 0) tmem_ld32(tmem + lanes + 128 + col, z);
+			else {
+#pragma unroll
+				for (int k = 0; k < 32; ++k) z[k] = 0.f;
+			}
+			if (tid < rows && wide_store) {
+				uint4* to = reinterpret_cast<uint4*>((uint16_t*)a.out + token * a.o_row + head * a.o_head + col);
+#pragma unroll
+				for (int k = 0; k < 32; k += 8) {
+					uint32_t w[4];
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						const float x = z[k + 2 * e] * norm, y = z[k + 2 * e + 1] * norm;
+						if (a.out_type == SEQ_BF16) {
+							const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+							w[e] = *reinterpret_cast<const uint32_t*>(&h);
+						} else w[e] = pack_f16(x, y);
+					}
+					to[k / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+				}
+			} else if (tid < rows) {
+#pragma unroll
+				for (int k = 0; k < 32; ++k) at_finish(a, token, head, col + k, z[k] * norm);
+			}
+		}
+	} else if (warp < 8) {
+		const bool keys = warp < 6;
+		const int t = tid - (keys ? 128 : 192); // 64 threads each
+		// keys: a thread has one key, all its channels.  values: a thread has eight keys, 16 channels (of 64 channels: two groups of eight threads have none)
+		const int group8 = t & 7, dims = t >> 3;
+		const bool works = keys || dims < PIECES;
+		auto page_of = [&](int j) {
+			if (j >= sp.total) return -1;
+			const int pos = position(j), at = page_index(c, pos);
+			if (at >= c.table_pages) return -1;
+			const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
+			return (unsigned)id < (unsigned)c.pages ? id : -1;
+		};
+		auto row_of = [&](int id, int j) { return id < 0 ? -1 : (id * c.heads + kvh) * c.page + page_row(c, position(j)); }; // (under 2^31; -1: none)
+		uint32_t next_seen = 0;
+		uint4 codes[8];
+		float scale = 0.f;                // keys: of this thread's key, 0: none
+		int exps[2] = {C8_NONE, C8_NONE}; // values: log2 of the scales of keys lane and lane + 32
+		auto load = [&](int i) {
+			if (keys) {
+				const int j = i * AP_KEYS + t, id = page_of(j);
+				scale = 0.f;
+#pragma unroll
+				for (int k = 0; k < PIECES; ++k) codes[k] = make_uint4(0, 0, 0, 0);
+				if (id >= 0) {
+					const uint4* src = reinterpret_cast<const uint4*>(c.k + (long long)row_of(id, j) * D);
+#pragma unroll
+					for (int k = 0; k < PIECES; ++k) codes[k] = __ldg(src + k);
+					scale = c.ks[id * c.heads + kvh];
+				}
+				const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
+				if (lane == 0) next_seen = there;
+			} else {
+				int row[2]; // of keys lane and lane + 32
+#pragma unroll
+				for (int h = 0; h < 2; ++h) {
+					const int j = i * AP_KEYS + 32 * h + lane, id = page_of(j);
+					row[h] = row_of(id, j);
+					exps[h] = id < 0 ? C8_NONE : max((int)(__float_as_uint(c.vs[id * c.heads + kvh]) >> 23) - 127, -126);
+				}
+#pragma unroll
+				for (int k = 0; k < 8; ++k) {
+					const int key = group8 * 8 + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
+					codes[k] = make_uint4(0, 0, 0, 0);
+					if (r >= 0 && works) codes[k] = __ldg(reinterpret_cast<const uint4*>(c.v + (long long)r * D) + dims);
+				}
+			}
+		};
+		if (tiles > 0) load(0);
+		for (int i = 0; i < tiles; ++i) {
+			const int st = i & 1;
+			if (!ap_wait_warp(s.kv_empty + st, ((i >> 1) & 1) ^ 1, &s.lost)) break;
+			if (keys) {
+				s.factor[st][t] = scale * qscale;
+				if (lane == 0) s.seen[st][warp - 4] = next_seen;
+#pragma unroll
+				for (int k = 0; k < PIECES; ++k) {
+					uint32_t w[8];
+					e4m3x4_to_f16(codes[k].x, w[0], w[1]), e4m3x4_to_f16(codes[k].y, w[2], w[3]), e4m3x4_to_f16(codes[k].z, w[4], w[5]), e4m3x4_to_f16(codes[k].w, w[6], w[7]);
+#pragma unroll
+					for (int e = 0; e < 2; ++e) {
+						const int piece = 2 * k + e;
+						*reinterpret_cast<uint4*>(s.k[st][piece >> 3] + t * 128 + (((piece & 7) ^ (t & 7)) << 4)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+					}
+				}
+			} else {
+				// values in units of the tile's largest scale: a smaller one's are shifted down (below 2^-24 of the largest nothing is left of a code)
+				int most = __reduce_max_sync(0xffffffffu, max(exps[0], exps[1]));
+				if (most == C8_NONE) most = 0;
+				const bool even = __all_sync(0xffffffffu, (exps[0] == most || exps[0] == C8_NONE) && (exps[1] == most || exps[1] == C8_NONE));
+				if (t == 0) s.bias[st] = (float)most;
+				uint32_t down[4]; // of the pairs of this thread's keys, as fp16
+#pragma unroll
+				for (int k = 0; k < 4; ++k) {
+					float f[2];
+#pragma unroll
+					for (int e = 0; e < 2; ++e) {
+						const int key = group8 * 8 + 2 * k + e, e0 = __shfl_sync(0xffffffffu, exps[0], key & 31), e1 = __shfl_sync(0xffffffffu, exps[1], key & 31);
+						f[e] = pow2f(max((key < 32 ? e0 : e1) - most, -126));
+					}
+					down[k] = pack_f16(f[0], f[1]);
+				}
+				const uint32_t* const x = reinterpret_cast<const uint32_t*>(codes); // x[4 key + word]
+				if (works) {
+#pragma unroll
+					for (int word = 0; word < 4; ++word)
+#pragma unroll
+						for (int e = 0; e < 2; ++e) { // channels 4 word + 2 e, + 1
+							uint32_t lo[4], hi[4];
+#pragma unroll
+							for (int k = 0; k < 4; ++k) {
+								e4m3x4_to_f16(__byte_perm(x[8 * k + word], x[8 * k + 4 + word], e ? 0x7362 : 0x5140), lo[k], hi[k]);
+								if (!even) lo[k] = mul_f16(lo[k], down[k]), hi[k] = mul_f16(hi[k], down[k]);
+							}
+							const int d = dims * 16 + 4 * word + 2 * e;
+							*reinterpret_cast<uint4*>(s.v[st] + d * 128 + ((group8 ^ (d & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+							*reinterpret_cast<uint4*>(s.v[st] + (d + 1) * 128 + ((group8 ^ ((d + 1) & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+						}
+				}
+			}
+			fence_async_smem();
+			mbar_arrive(s.kv_full + st);
+			if (i + 1 < tiles) load(i + 1);
+		}
+	} else if (lane == 0) {
+		constexpr uint32_t score = (1u << 4) | ((uint32_t)(AP_KEYS >> 3) << 17) | ((uint32_t)(AP_ROWS >> 4) << 24), value = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(AP_ROWS >> 4) << 24);
+		for (int i = 0; i <= tiles && tiles > 0; ++i) {
+			if (i < tiles) {
+				const int buf = i & 1;
+				const uint32_t parity = (i >> 1) & 1;
+				if (!ap_wait(s.kv_full + buf, parity, &s.lost) || !ap_wait(s.s_empty + buf, parity ^ 1, &s.lost)) break;
+				tc_fence_after();
+#pragma unroll
+				for (int h = 0; h < Shared::PAIR; ++h)
+#pragma unroll
+					for (int pn = 0; pn < PANELS; ++pn)
+#pragma unroll
+						for (int k = 0; k < 4; ++k)
+							umma_f16(tmem + buf * 64, umma_desc_sw128(s.q[h][pn]) + 2 * k, umma_desc_sw128(s.k[buf][pn]) + 2 * k, score, (h | pn | k) ? 1u : 0u);
+				umma_commit(s.s_full + buf);
+			}
+			if (i > 0) {
+				const int j = i - 1;
+				if (!ap_wait(&s.p_full, j & 1, &s.lost)) break;
+				tc_fence_after();
+#pragma unroll
+				for (int h = 0; h < Shared::PAIR; ++h)
+#pragma unroll
+					for (int k = 0; k < 4; ++k) umma_f16(tmem + 128, umma_desc_sw128(s.p[h]) + 2 * k, umma_desc_sw128(s.v[j & 1]) + 2 * k, value, (j | h | k) ? 1u : 0u);
+				umma_commit(s.kv_empty + (j & 1));
+				umma_commit(&s.p_empty);
+			}
+		}
+		umma_commit(&s.done); // nothing of this block's is left in the tensor core when its memory goes
+		mbar_wait_bounded(&s.done, 0);
+	}
+	__syncwarp();
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	if (warp == 8) tmem_dealloc(tmem, 256);
+}
+
 // Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.
 __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	pdl_wait_prev();
@@ -686,19 +1068,22 @@ StoreRows store_rows(const SeqRows& r) {
 // How the work is cut: rows of a CTA; shares of a tile's keys and the chunks of each (sequences differ in length: shares of one length for all of them, short ones have fewer);
 // whether a cluster folds the shares.
 struct AtPlan {
-	int tile, shares, each, cluster;
+	int tile, shares, each, cluster; // tile 128: the prompt kernel
 };
 constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
+constexpr int AP_CTAS = 48;      // of the prompt kernel, from which on it is the faster one
 // Rows of a CTA: eight fill a product; more, where a sequence has more, read and convert the codes once for all of them, as far as registers hold their sums and CTAs are enough
 // for the GPU all the same.
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const long long rows = (long long)p.longest * (a.heads / c.heads);
 	auto ctas = [&](int tile) { return (long long)p.n * cdiv(rows, tile) * c.heads; };
+	if (rows >= AP_ROWS / 2 && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(AP_ROWS) >= AP_CTAS) return AP_ROWS;
 	if (rows > 16 && c.dim <= 128 && ctas(32) >= AT_ROOM) return 32;
 	return rows > 8 && ctas(16) >= AT_ROOM / 2 ? 16 : 8;
 }
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const int group = a.heads / c.heads, tile = attend_tile(c, p, a);
+	if (tile == AP_ROWS) return AtPlan{tile, 1, cdiv(std::max(a.most_keys, 1), AT_KEYS), 0};
 	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, tile) * c.heads, room = AT_ROOM;
 	long long keys = std::max(a.most_keys, 1);
 	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + tile / group);
@@ -737,9 +1122,18 @@ cudaError_t attend_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t 
 	if (e == cudaSuccess) e = launch(st, false, a.cluster ? a.shares : 1, k_c8_attend<D, SPLIT, NQ>, grid, dim3(32 * AT_WARPS), smem, c, a);
 	return e;
 }
+template <int D, bool SPLIT>
+cudaError_t prompt_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
+	static std::atomic<uint64_t> done{0};
+	cudaError_t e = allow(k_c8_prompt<D, SPLIT>, sizeof(ApShared<D, SPLIT>), done);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_prompt<D, SPLIT>, grid, dim3(AP_THREADS), sizeof(ApShared<D, SPLIT>), c, a);
+	return e;
+}
 template <int D>
 cudaError_t attend_wide(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	const bool split = a.q_type == SEQ_F32;
+	if constexpr (D < 256)
+		if (a.tile == AP_ROWS) return split ? prompt_launch<D, true>(c, a, grid, st) : prompt_launch<D, false>(c, a, grid, st);
 	if (a.tile == 8) return split ? attend_launch<D, true, 1>(c, a, grid, st) : attend_launch<D, false, 1>(c, a, grid, st);
 	if (D == 256 || a.tile == 16) return split ? attend_launch<D, true, 2>(c, a, grid, st) : attend_launch<D, false, 2>(c, a, grid, st);
 	constexpr int DD = D == 256 ? 128 : D; // (rows of 256 channels come in sixteens)

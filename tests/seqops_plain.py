@@ -105,7 +105,8 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
     """q [tokens][Hq][dim]; kv, vv values of the codes [pages][heads][page][dim] -> out [tokens][Hq][dim] (NaN where no sequence has a row) and a bound of what the
     kernel's arithmetic may add to it before the last rounding.
 
-    Bound: a score is a sum over dim in steps of 16 whose fp32 additions may truncate (2^-23 of the terms' sum each), times factors (four roundings); queries and weights
+    Bound: a score is a sum over dim in steps of 16 products.  The tensor core aligns a step's products and the running sum to the largest of the 17 and may cut each off at its
+    2^-23: per step 2^-23 of the running sum and 17 times that of the largest product.  Then factors (four roundings); queries and weights
     enter as fp16, a tile's largest query at 2^15, a row's largest weight at 2^10 or more (2^-11 of a weight or 2^-25 2^-10 of the largest; 2^-22 as pairs).  A score's error d moves a weight by e^d; the numerator's sum and the denominator's add
     a rounding per 16 keys and per share."""
     T, Hq, D = q.shape
@@ -138,7 +139,7 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
                 s = k @ x * scale
                 mag = np.abs(k) @ np.abs(x) * abs(scale)
                 dq = (2.0 ** -22 if split else 0.0) * mag + 2.0 ** -40 * np.abs(q[st:st + n]).max() * np.abs(k).sum(1) * abs(scale)
-                ds = dq + (D / 16 * (2 if split else 1) + 6) * 2.0 ** -23 * mag
+                ds = dq + ((D / 16 * (2 if split else 1) + 6) * mag + D / 16 * (2 if split else 1) * 17 * (np.abs(k) * np.abs(x)).max(1) * abs(scale)) * 2.0 ** -23
                 if softcap:
                     s = softcap * np.tanh(s / softcap)
                     ds = ds + 8 * F32 * np.abs(s)
@@ -153,9 +154,14 @@ def attend(q, kv, ks, vv, vs, table, portions, page, scale, window=0, keep_first
                 o = p @ v
                 adds = (len(keys) / 16 * (2 if split else 1) + 80) * 2.0 ** -23
                 spread = p @ np.abs(v)
-                t = (p * ds) @ np.abs(v) + (p @ ds) * np.abs(o) + ((2.0 ** -22 if split else half) + adds) * spread + adds * np.abs(o)
-                # weights whose fp16 (or whose remainder's) is subnormal: half a step is 2^-25, the largest weight (times its value scale) stands at 2^10 at least
-                t = t + 2.0 ** -35 * np.abs(vv[ids, g, keys % page]).sum(0) * np.max(vs[ids, g] * w) / den
+                cut = len(keys) / 16 * (2 if split else 1) * 17 * 2.0 ** -23 * (p[:, None] * np.abs(v)).max(0)  # as for the scores
+                t = (p * ds) @ np.abs(v) + (p @ ds) * np.abs(o) + ((2.0 ** -22 if split else half) + adds) * spread + adds * np.abs(o) + cut
+                # weights whose fp16 (or whose remainder's) is subnormal: half a step is 2^-25, the largest weight (times the largest value scale beside it, in whose units a
+                # prompt's tile has its values) stands at 2^10 at least
+                t = t + 2.0 ** -35 * np.abs(vv[ids, g, keys % page]).sum(0) * np.max(vs[ids, g]) * np.max(w) / den
+                # codes in units of a scale that is 2^15 times their own or more fall under fp16's smallest step
+                if np.max(vs[ids, g]) > 2.0 ** 15 * np.min(vs[ids, g]):
+                    t = t + 2.0 ** -25 * np.max(vs[ids, g])
                 # an exponential under 2^-126 may come out as zero: it multiplies sums of the values by weights of 2^15 at most, and den >= 1
                 t = t + 2.0 ** -111 * np.abs(v).sum(0)
                 if gate is not None:

@@ -278,6 +278,34 @@ def test_attention_options(opt, dtype):
     check_attend(c, q, seqops.Batch([3, 1, 0, 2], counts, before), scale=0.2, **opt)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("page,dim,opt", [(16, 128, {}), (16, 64, {}), (13, 128, dict(window=70, keep_first=5)), (64, 64, dict(chunk=50)), (8, 128, dict(window=3, keep_first=90, sink=True, gate=True))])
+def test_attention_of_prompts(page, dim, opt, dtype):
+    """Rows enough for the tensor cores' tiles of 128: several sequences of different lengths, one token and none among them, tiles that end inside a token's heads."""
+    c = Cached(5, -(-330 // page), 8, page, dim, page + dim)
+    c.table[2, 3] = -1  # positions that are not there
+    c.dtable.copy_(torch.tensor(c.table))
+    g = torch.Generator(device="cuda").manual_seed(page)
+    counts, before = [100, 37, 1, 0, 77], [0, 50, 300, 5, 130]
+    q = torch.randn(sum(counts), 24, dim, generator=g, device="cuda").to(DT[dtype])
+    opt = dict(opt)
+    if opt.get("sink"):
+        opt["sink"] = torch.randn(24, generator=g, device="cuda") * 3
+    if opt.get("gate"):
+        opt["gate"] = torch.randn(sum(counts), 24, dim, generator=g, device="cuda")
+    check_attend(c, q, seqops.Batch([1, 2, 4, 0, 3], counts, before), scale=0.7 * dim ** -0.5, **opt)
+
+
+def test_prompt_rows_whose_scores_grow():
+    """Keys that grow along the sequence: references move in every tile and the sums are rescaled."""
+    c = Cached(1, 30, 8, 16, 128, 3)
+    for i in range(30):
+        c.scales[0, c.table[0, i]] = 2.0 ** (i / 2 - 14)
+    q = torch.randn(200, 32, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    check_attend(c, q.bfloat16(), seqops.Batch([0], [200], [270]), scale=0.1)
+    check_attend(c, q, seqops.Batch([0], [200], [0]), scale=0.1)
+
+
 def test_attention_of_one_token_over_many_keys():
     """Shares of the keys: single sequences whose keys many CTAs divide, lengths around their borders."""
     c = Cached(2, 200, 1, 16, 128, 21)
