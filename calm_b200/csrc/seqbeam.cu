@@ -25,8 +25,6 @@ constexpr int BM_WARPS = BM_THREADS / 32;
 constexpr int BM_RING = 4096;                                               // bytes that a warp has in flight
 constexpr int BM_LISTS = 256;                                               // slices of a group's rows
 constexpr int BM_CAND = 4096;                                               // candidates of a group that the merge compares with one another
-typedef unsigned long long u64;
-
 struct BeamArgs {
 	const void* logits;
 	long long group_stride, row_stride;
@@ -56,33 +54,6 @@ __device__ __forceinline__ int rank_in(const u64* list, int c, u64 key) {
 	}
 	return r;
 }
-// two fp32 operations in one instruction
-__device__ __forceinline__ u64 pair_of(float x, float y) {
-	u64 r;
-	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-	return r;
-}
-__device__ __forceinline__ float2 halves(u64 p) {
-	float2 r;
-	asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-	return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-	u64 r;
-	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-	return r;
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-	u64 r;
-	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-	return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-	float r;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-	return r;
-}
-
 // What a CTA knows of its slice's highest logits.  Logits come in groups of four neighbours; a group whose highest is above tau joins the list (values as they are, so a thread spends
 // a few instructions on it), and now and then the list is cut down to the groups whose highest is among the n highest, the least of which is the new tau.  Only what is left at
 // the end becomes keys.  Tokens come in order, so a later value that equals tau is no candidate.

@@ -37,11 +37,6 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 __device__ __forceinline__ int page_index(const C8& c, int pos) { return c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page; }
 __device__ __forceinline__ int page_row(const C8& c, int pos) { return c.page_shift >= 0 ? pos & (c.page - 1) : pos % c.page; }
-__device__ __forceinline__ float ex2(float x) {
-	float r;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-	return r;
-}
 // four codes as two pairs of fp16
 __device__ __forceinline__ void e4m3x4_to_f16(uint32_t codes, uint32_t& lo, uint32_t& hi) {
 	asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
@@ -613,7 +608,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // tiles of 64 keys.  Four warps read codes, a tile ahead, and lay them out in fp16 as the products' operands (keys as they are, values transposed); one thread issues
 // S = Q K^T of the next tile and O += P V of this one; four warps, a row a thread, take S from tensor memory, form the weights (exponents, references and denominators as
 // above) and write them to shared memory as the next product's operand.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.
-//   warps 0-3  softmax and output;  4, 5  keys;  6, 7  values;  8  products
+//   warps 0-3  softmax and output;  4-7  keys and values;  8  products
 // Bound: for 128 channels a tile costs the tensor cores 512 cycles and the exponentials as many; two CTAs share an SM.
 constexpr int AP_ROWS = 128, AP_KEYS = 64, AP_THREADS = 288, C8_NONE = -1000;
 __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
@@ -688,8 +683,8 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 
 	if (warp == 8) tmem_alloc(&s.tmem, 256);
 	if (tid == 0) {
-		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 128), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1), mbar_init(s.s_empty + i, 128);
-		mbar_init(&s.p_full, 128), mbar_init(&s.p_empty, 1), mbar_init(&s.done, 1);
+		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 4), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1), mbar_init(s.s_empty + i, 4); // (a warp arrives as one)
+		mbar_init(&s.p_full, 4), mbar_init(&s.p_empty, 1), mbar_init(&s.done, 1);
 		s.lost = 0;
 		mbar_init_fence();
 	}
@@ -741,14 +736,16 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			const uint32_t seen[2] = {s.seen[buf][0], s.seen[buf][1]};
 			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
 			const float bias = s.bias[buf];
-			float z[32];
-			auto scores = [&](int h) { // log2 of the weights of keys 32 h .. , not against the reference yet; returns the largest
+			float z[32], base = m == -INFINITY ? 0.f : m;
+			// log2 of the weights of keys 32 h .. against the reference (against 0 before there is one); returns the largest
+			auto scores = [&](int h) {
 				tmem_ld32(tmem + lanes + buf * 64 + 32 * h, z);
-				float top = -INFINITY;
+				const u64 off = pair_of(bias - base, bias - base);
 #pragma unroll
 				for (int k = 0; k < 32; k += 4) {
-					const float4 f = *reinterpret_cast<const float4*>(s.factor[buf] + 32 * h + k);
-					z[k] = fmaf(z[k], f.x, bias), z[k + 1] = fmaf(z[k + 1], f.y, bias), z[k + 2] = fmaf(z[k + 2], f.z, bias), z[k + 3] = fmaf(z[k + 3], f.w, bias);
+					const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[buf] + 32 * h + k);
+					const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), f.x, off)), y = halves(fma2(pair_of(z[k + 2], z[k + 3]), f.y, off));
+					z[k] = x.x, z[k + 1] = x.y, z[k + 2] = y.x, z[k + 3] = y.y;
 				}
 				if (!all) {
 #pragma unroll
@@ -757,20 +754,20 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 						if (!((seen[h] >> k & 1) && kp <= rpos && (kp >= rlow || kp < a.keep_first))) z[k] = -INFINITY;
 					}
 				}
+				float top = -INFINITY;
 #pragma unroll
 				for (int k = 0; k < 32; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
 				return top;
 			};
-			float sum[2] = {0.f, 0.f};
+			u64 sum = 0;
 			auto weights = [&](int h) {
-				const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
 				for (int k = 0; k < 32; k += 8) {
 					uint32_t hi[4], rest[4];
 #pragma unroll
 					for (int e = 0; e < 8; e += 2) {
-						const float w0 = ex2(z[k + e] - base), w1 = ex2(z[k + e + 1] - base);
-						sum[0] += w0, sum[1] += w1;
+						const float w0 = ex2(z[k + e]), w1 = ex2(z[k + e + 1]);
+						sum = add2(sum, pair_of(w0, w1));
 						hi[e / 2] = pack_f16(w0, w1), rest[e / 2] = SPLIT ? pack_rest(w0, w1, hi[e / 2]) : 0;
 					}
 					const int place = tid * 128 + (((4 * h + k / 8) ^ (tid & 7)) << 4);
@@ -779,15 +776,16 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 				}
 			};
 			// half by half against the reference as it stands; where a row passes it, the warp looks at both halves, moves references and starts anew
-			bool moved = __any_sync(0xffffffffu, scores(0) > m + AT_MOST);
+			const float most = m == -INFINITY ? -INFINITY : AT_MOST;
+			bool moved = __any_sync(0xffffffffu, scores(0) > most);
 			if (i > 0 && !ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break; // the product before has read the weights and left the sums
 			tc_fence_after();
 			if (!moved) {
 				weights(0);
-				moved = __any_sync(0xffffffffu, scores(1) > m + AT_MOST);
+				moved = __any_sync(0xffffffffu, scores(1) > most);
 			}
 			if (moved) {
-				const float top = fmaxf(scores(0), scores(1)), mn = top > m + AT_MOST ? top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn);
+				const float top = fmaxf(scores(0), scores(1)), mn = top > most ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn);
 				if (i > 0) { // (there are sums)
 #pragma unroll 1
 					for (int col = 0; col < D; col += 32) {
@@ -797,17 +795,18 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 						tmem_st32(tmem + lanes + 128 + col, z);
 					}
 				}
-				m = mn, l *= f, sum[0] = sum[1] = 0.f;
+				m = mn, l *= f, sum = 0, base = m == -INFINITY ? 0.f : m;
 				scores(0);
 				weights(0);
 				scores(1);
 			}
 			weights(1);
-			l = fmaf(sum[0] + sum[1], pow2f(-(int)bias), l); // the weights hold the value scale
+			const float2 sums = halves(sum);
+			l = fmaf(sums.x + sums.y, pow2f(-(int)bias), l); // the weights hold the value scale
 			tc_fence_before();
 			fence_async_smem();
-			mbar_arrive(s.s_empty + buf);
-			mbar_arrive(&s.p_full);
+			__syncwarp();
+			if (lane == 0) mbar_arrive(s.s_empty + buf), mbar_arrive(&s.p_full);
 		}
 		if (tiles > 0) ap_wait_warp(&s.p_empty, (tiles - 1) & 1, &s.lost);
 		tc_fence_after();
@@ -848,107 +847,108 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			}
 		}
 	} else if (warp < 8) {
-		const bool keys = warp < 6;
-		const int t = tid - (keys ? 128 : 192); // 64 threads each
-		// keys: a thread has one key, all its channels.  values: a thread has eight keys, 16 channels (of 64 channels: two groups of eight threads have none)
-		const int group8 = t & 7, dims = t >> 3;
-		const bool works = keys || dims < PIECES;
-		auto page_of = [&](int j) {
-			if (j >= sp.total) return -1;
-			const int pos = position(j), at = page_index(c, pos);
-			if (at >= c.table_pages) return -1;
-			const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
-			return (unsigned)id < (unsigned)c.pages ? id : -1;
+		// Every thread takes pieces of keys' rows (PIECES lanes read a row) and eight channels of eight keys' values.
+		constexpr int KROWS = 32 / PIECES, KEACH = AP_KEYS / (4 * KROWS);
+		const int t = tid - 128, group8 = t & 7, dims = (t >> 3) * 8;
+		const bool works = dims < D;
+		auto page_of = [&](int j) { // as the table has it: looked at where it is used, a tile later
+			const int at = page_index(c, position(min(j, sp.total - 1)));
+			return j < sp.total && at < c.table_pages ? __ldg(c.table + (size_t)slot * c.table_pages + at) : -1;
 		};
-		auto row_of = [&](int id, int j) { return id < 0 ? -1 : (id * c.heads + kvh) * c.page + page_row(c, position(j)); }; // (under 2^31; -1: none)
-		uint32_t next_seen = 0;
-		uint4 codes[8];
-		float scale = 0.f;                // keys: of this thread's key, 0: none
-		int exps[2] = {C8_NONE, C8_NONE}; // values: log2 of the scales of keys lane and lane + 32
+		int ahead[2] = {-1, -1}, exps[2] = {0, 0}; // of keys lane and lane + 32: the pages of the tile to load next; the values' scales of the loaded one, as they come
+		bool have[2] = {false, false};
+		float scale = 0.f; // of key t, the keys'
+		uint4 kw[KEACH];
+		uint2 vw[8];
+		auto look = [&](int i) { ahead[0] = page_of(i * AP_KEYS + lane), ahead[1] = page_of(i * AP_KEYS + 32 + lane); };
 		auto load = [&](int i) {
-			if (keys) {
-				const int j = i * AP_KEYS + t, id = page_of(j);
-				scale = 0.f;
+			int row[2];
 #pragma unroll
-				for (int k = 0; k < PIECES; ++k) codes[k] = make_uint4(0, 0, 0, 0);
-				if (id >= 0) {
-					const uint4* src = reinterpret_cast<const uint4*>(c.k + (long long)row_of(id, j) * D);
-#pragma unroll
-					for (int k = 0; k < PIECES; ++k) codes[k] = __ldg(src + k);
-					scale = c.ks[id * c.heads + kvh];
-				}
-				const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-				if (lane == 0) next_seen = there;
-			} else {
-				int row[2]; // of keys lane and lane + 32
-#pragma unroll
-				for (int h = 0; h < 2; ++h) {
-					const int j = i * AP_KEYS + 32 * h + lane, id = page_of(j);
-					row[h] = row_of(id, j);
-					exps[h] = id < 0 ? C8_NONE : max((int)(__float_as_uint(c.vs[id * c.heads + kvh]) >> 23) - 127, -126);
-				}
-#pragma unroll
-				for (int k = 0; k < 8; ++k) {
-					const int key = group8 * 8 + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
-					codes[k] = make_uint4(0, 0, 0, 0);
-					if (r >= 0 && works) codes[k] = __ldg(reinterpret_cast<const uint4*>(c.v + (long long)r * D) + dims);
-				}
+			for (int h = 0; h < 2; ++h) {
+				const int id = (unsigned)ahead[h] < (unsigned)c.pages ? ahead[h] : -1, unit = id * c.heads + kvh;
+				have[h] = id >= 0;
+				row[h] = have[h] ? unit * c.page + page_row(c, position(i * AP_KEYS + 32 * h + lane)) : -1; // (under 2^31)
+				if (have[h]) exps[h] = __float_as_int(__ldg(c.vs + unit));
+				if (have[h] && h == warp - 4) scale = __ldg(c.ks + unit);
 			}
+#pragma unroll
+			for (int k = 0; k < KEACH; ++k) {
+				const int key = (k * 4 + warp - 4) * KROWS + lane / PIECES, r = __shfl_sync(0xffffffffu, (k * 4 + warp - 4) * KROWS < 32 ? row[0] : row[1], key & 31);
+				kw[k] = make_uint4(0, 0, 0, 0);
+				if (r >= 0) kw[k] = ldg_stream(reinterpret_cast<const uint4*>(c.k + (long long)r * D) + lane % PIECES);
+			}
+#pragma unroll
+			for (int k = 0; k < 8; ++k) {
+				const int key = group8 * 8 + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
+				vw[k] = make_uint2(0, 0);
+				if (r >= 0 && works) vw[k] = ldg_stream8(reinterpret_cast<const uint2*>(c.v + (long long)r * D + dims));
+			}
+			look(i + 1);
 		};
+		look(0);
 		if (tiles > 0) load(0);
 		for (int i = 0; i < tiles; ++i) {
 			const int st = i & 1;
 			if (!ap_wait_warp(s.kv_empty + st, ((i >> 1) & 1) ^ 1, &s.lost)) break;
-			if (keys) {
-				s.factor[st][t] = scale * qscale;
-				if (lane == 0) s.seen[st][warp - 4] = next_seen;
+			if (t < AP_KEYS) {
+				const bool there = warp == 4 ? have[0] : have[1];
+				s.factor[st][t] = there ? scale * qscale : 0.f;
+				const uint32_t seen = __ballot_sync(0xffffffffu, there);
+				if (lane == 0) s.seen[st][warp - 4] = seen;
+			}
 #pragma unroll
-				for (int k = 0; k < PIECES; ++k) {
-					uint32_t w[8];
-					e4m3x4_to_f16(codes[k].x, w[0], w[1]), e4m3x4_to_f16(codes[k].y, w[2], w[3]), e4m3x4_to_f16(codes[k].z, w[4], w[5]), e4m3x4_to_f16(codes[k].w, w[6], w[7]);
+			for (int k = 0; k < KEACH; ++k) {
+				const int key = (k * 4 + warp - 4) * KROWS + lane / PIECES, piece = lane % PIECES;
+				uint32_t w[8];
+				e4m3x4_to_f16(kw[k].x, w[0], w[1]), e4m3x4_to_f16(kw[k].y, w[2], w[3]), e4m3x4_to_f16(kw[k].z, w[4], w[5]), e4m3x4_to_f16(kw[k].w, w[6], w[7]);
+				unsigned char* const to = s.k[st][piece >> 2] + key * 128;
+				const bool odd = piece & 4; // (lanes of the second panel store their second half first: eight lanes meet different banks)
+				const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
+				const int at = (2 * piece & 7) ^ (key & 7);
+				*reinterpret_cast<uint4*>(to + ((odd ? at ^ 1 : at) << 4)) = odd ? hi : lo;
+				*reinterpret_cast<uint4*>(to + ((odd ? at : at ^ 1) << 4)) = odd ? lo : hi;
+			}
+			// values in units of the tile's largest scale: a smaller one's are shifted down (below 2^-24 of the largest nothing is left of a code)
+			int e[2];
 #pragma unroll
-					for (int e = 0; e < 2; ++e) {
-						const int piece = 2 * k + e;
-						*reinterpret_cast<uint4*>(s.k[st][piece >> 3] + t * 128 + (((piece & 7) ^ (t & 7)) << 4)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-					}
-				}
-			} else {
-				// values in units of the tile's largest scale: a smaller one's are shifted down (below 2^-24 of the largest nothing is left of a code)
-				int most = __reduce_max_sync(0xffffffffu, max(exps[0], exps[1]));
-				if (most == C8_NONE) most = 0;
-				const bool even = __all_sync(0xffffffffu, (exps[0] == most || exps[0] == C8_NONE) && (exps[1] == most || exps[1] == C8_NONE));
-				if (t == 0) s.bias[st] = (float)most;
-				uint32_t down[4]; // of the pairs of this thread's keys, as fp16
+			for (int h = 0; h < 2; ++h) e[h] = have[h] ? max((exps[h] >> 23 & 255) - 127, -126) : C8_NONE;
+			int most = __reduce_max_sync(0xffffffffu, max(e[0], e[1]));
+			if (most == C8_NONE) most = 0;
+			if (t == 0) s.bias[st] = (float)most;
+			const bool even = __all_sync(0xffffffffu, (e[0] == most || e[0] == C8_NONE) && (e[1] == most || e[1] == C8_NONE));
+			uint32_t down[4]; // of the pairs of this thread's keys, as fp16
+			if (!even) {
 #pragma unroll
 				for (int k = 0; k < 4; ++k) {
 					float f[2];
 #pragma unroll
-					for (int e = 0; e < 2; ++e) {
-						const int key = group8 * 8 + 2 * k + e, e0 = __shfl_sync(0xffffffffu, exps[0], key & 31), e1 = __shfl_sync(0xffffffffu, exps[1], key & 31);
-						f[e] = pow2f(max((key < 32 ? e0 : e1) - most, -126));
+					for (int u = 0; u < 2; ++u) {
+						const int key = group8 * 8 + 2 * k + u, e0 = __shfl_sync(0xffffffffu, e[0], key & 31), e1 = __shfl_sync(0xffffffffu, e[1], key & 31);
+						f[u] = pow2f(max((key < 32 ? e0 : e1) - most, -126));
 					}
 					down[k] = pack_f16(f[0], f[1]);
 				}
-				const uint32_t* const x = reinterpret_cast<const uint32_t*>(codes); // x[4 key + word]
-				if (works) {
+			}
+			if (works) {
 #pragma unroll
-					for (int word = 0; word < 4; ++word)
+				for (int word = 0; word < 2; ++word)
 #pragma unroll
-						for (int e = 0; e < 2; ++e) { // channels 4 word + 2 e, + 1
-							uint32_t lo[4], hi[4];
+					for (int u = 0; u < 2; ++u) { // channels dims + 4 word + 2 u, + 1
+						uint32_t lo[4], hi[4];
 #pragma unroll
-							for (int k = 0; k < 4; ++k) {
-								e4m3x4_to_f16(__byte_perm(x[8 * k + word], x[8 * k + 4 + word], e ? 0x7362 : 0x5140), lo[k], hi[k]);
-								if (!even) lo[k] = mul_f16(lo[k], down[k]), hi[k] = mul_f16(hi[k], down[k]);
-							}
-							const int d = dims * 16 + 4 * word + 2 * e;
-							*reinterpret_cast<uint4*>(s.v[st] + d * 128 + ((group8 ^ (d & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-							*reinterpret_cast<uint4*>(s.v[st] + (d + 1) * 128 + ((group8 ^ ((d + 1) & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+						for (int k = 0; k < 4; ++k) {
+							const uint32_t x = word ? vw[2 * k].y : vw[2 * k].x, y = word ? vw[2 * k + 1].y : vw[2 * k + 1].x;
+							e4m3x4_to_f16(__byte_perm(x, y, u ? 0x7362 : 0x5140), lo[k], hi[k]);
+							if (!even) lo[k] = mul_f16(lo[k], down[k]), hi[k] = mul_f16(hi[k], down[k]);
 						}
-				}
+						const int d = dims + 4 * word + 2 * u;
+						*reinterpret_cast<uint4*>(s.v[st] + d * 128 + ((group8 ^ (d & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+						*reinterpret_cast<uint4*>(s.v[st] + (d + 1) * 128 + ((group8 ^ ((d + 1) & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+					}
 			}
 			fence_async_smem();
-			mbar_arrive(s.kv_full + st);
+			__syncwarp();
+			if (lane == 0) mbar_arrive(s.kv_full + st);
 			if (i + 1 < tiles) load(i + 1);
 		}
 	} else if (lane == 0) {

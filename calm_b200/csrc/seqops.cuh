@@ -62,6 +62,40 @@ inline bool type_ok(int t) { return t == SEQ_F32 || t == SEQ_BF16 || t == SEQ_F1
 __device__ __forceinline__ float as_f32(float v) { return v; }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
+typedef unsigned long long u64;
+// two fp32 operations in one instruction
+__device__ __forceinline__ u64 pair_of(float x, float y) {
+	u64 r;
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+	return r;
+}
+__device__ __forceinline__ float2 halves(u64 p) {
+	float2 r;
+	asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+	return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+	u64 r;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+	u64 r;
+	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+	u64 r;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+	return r;
+}
+// 2^x to two steps; under 2^-126 zero
+__device__ __forceinline__ float ex2(float x) {
+	float r;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
