@@ -20,6 +20,7 @@ struct C8 {
 	int pages, heads, page, dim, slots, table_pages;
 	int page_shift; // log2 of page, -1: no power of two
 	const int *start, *count, *slot, *pos0;
+	__device__ __forceinline__ bool known(int slot) const { return (unsigned)slot < (unsigned)slots && pages > 0 && table_pages > 0; } // something may be there
 };
 constexpr int C8_LEAST = -64; // exponent of the smallest scale
 
@@ -243,20 +244,19 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * (8 * NQ) >= (long long)n * a.group) return;
 	const int row0 = tile * (8 * NQ), rows = (int)min((long long)(8 * NQ), (long long)n * a.group - row0);
-	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
+	const AtSpan sp = at_span(a, p0, row0, rows, c.known(slot));
 	const int lo = sp.lo, kept = sp.kept, total = sp.total;
 	const int begin = min(sp.chunks, share * a.each), end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
 	if (share > 0 && begin >= sp.chunks && !a.cluster) return; // (a cluster stays together)
 	const int H = c.heads, dim = c.dim;
 
 	auto position = [&](int j) { return j < kept ? j : lo + (j - kept); };
-	auto page_of = [&](int chunk) { // the page of this lane's key, -1: none
-		const int j = chunk * AT_KEYS + lane;
-		if (chunk >= end || j >= total) return -1;
-		const int at = page_index(c, position(j));
-		if (at >= c.table_pages) return -1;
-		const int id = __ldg(c.table + (size_t)slot * c.table_pages + at);
-		return (unsigned)id < (unsigned)c.pages ? id : -1;
+	// The page of this lane's key, as the table has it: a load that nothing waits for here, looked at a chunk later (page_ok: whether there was one to look for).
+	bool page_ok = false;
+	auto page_of = [&](int chunk) {
+		const int j = chunk * AT_KEYS + lane, at = page_index(c, position(min(j, max(total - 1, 0))));
+		page_ok = chunk < end && j < total && at < c.table_pages;
+		return total > 0 ? __ldg(c.table + (size_t)slot * c.table_pages + min(at, c.table_pages - 1)) : 0;
 	};
 	AtStage<D>& s = ring[warp];
 	int next = begin + warp, next_page = page_of(next), next_row = 0; // the chunk to request, the page and the row of this lane's key
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	};
 	auto request_keys = [&](int half) { // and both scales, in this half of their arrays
 		if (next < end) {
-			const int id = next_page, unit = max(id, 0) * H + kvh;
+			const int id = page_ok && (unsigned)next_page < (unsigned)c.pages ? next_page : -1, unit = max(id, 0) * H + kvh;
 			next_seen = __ballot_sync(0xffffffffu, id >= 0);
 			next_row = unit * c.page + page_row(c, position(min(next * AT_KEYS + lane, total - 1))); // (rows of a pool: under 2^31)
 			if (lane == 0) s.seen[half] = next_seen;
@@ -674,10 +674,11 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 	extern __shared__ __align__(1024) unsigned char ap_raw[]; // (all of the kernel's shared memory: it starts where the swizzle's pattern does)
 	Shared& s = *reinterpret_cast<Shared*>(ap_raw);
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = gridDim.x - 1 - blockIdx.x; // (the longest rows first)
-	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * AP_ROWS >= (long long)n * a.group) return;
+	const int b = blockIdx.y, kvh = blockIdx.x, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b];
+	const int tile = (int)min((long long)gridDim.z, ((long long)n * a.group + AP_ROWS - 1) / AP_ROWS) - 1 - (int)blockIdx.z; // (every sequence's longest rows first)
+	if (tile < 0 || n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * AP_ROWS >= (long long)n * a.group) return;
 	const int row0 = tile * AP_ROWS, rows = (int)min((long long)AP_ROWS, (long long)n * a.group - row0);
-	const AtSpan sp = at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots);
+	const AtSpan sp = at_span(a, p0, row0, rows, c.known(slot));
 	const int tiles = (sp.total + AP_KEYS - 1) / AP_KEYS;
 	auto position = [&](int j) { return j < sp.kept ? j : sp.lo + (j - sp.kept); };
 
@@ -851,42 +852,46 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 		constexpr int KROWS = 32 / PIECES, KEACH = AP_KEYS / (4 * KROWS);
 		const int t = tid - 128, group8 = t & 7, dims = (t >> 3) * 8;
 		const bool works = dims < D;
-		auto page_of = [&](int j) { // as the table has it: looked at where it is used, a tile later
-			const int at = page_index(c, position(min(j, sp.total - 1)));
-			return j < sp.total && at < c.table_pages ? __ldg(c.table + (size_t)slot * c.table_pages + at) : -1;
-		};
-		int ahead[2] = {-1, -1}, exps[2] = {0, 0}; // of keys lane and lane + 32: the pages of the tile to load next; the values' scales of the loaded one, as they come
-		bool have[2] = {false, false};
-		float scale = 0.f; // of key t, the keys'
+		// Nothing below waits for a load where it asks for it: keys that are not there read row 0 of the pool and the table's last entry, and are sorted out a tile later.
+		int ahead[2], exps[2];     // of keys lane and lane + 32: the pages of the tile to load next, as the table has them; the values' scales of the loaded one
+		bool asked[2], have[2];    // whether there was a page to look for; whether the key is there
+		float scale;               // of key t, the keys'
 		uint4 kw[KEACH];
 		uint2 vw[8];
-		auto look = [&](int i) { ahead[0] = page_of(i * AP_KEYS + lane), ahead[1] = page_of(i * AP_KEYS + 32 + lane); };
+		uint32_t mine = 0;         // this thread's values that are there
+		auto look = [&](int i) {
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+				const int j = i * AP_KEYS + 32 * h + lane, at = page_index(c, position(min(j, sp.total - 1)));
+				asked[h] = j < sp.total && at < c.table_pages;
+				ahead[h] = __ldg(c.table + (size_t)slot * c.table_pages + min(at, c.table_pages - 1));
+			}
+		};
 		auto load = [&](int i) {
 			int row[2];
 #pragma unroll
 			for (int h = 0; h < 2; ++h) {
-				const int id = (unsigned)ahead[h] < (unsigned)c.pages ? ahead[h] : -1, unit = id * c.heads + kvh;
-				have[h] = id >= 0;
+				have[h] = asked[h] && (unsigned)ahead[h] < (unsigned)c.pages;
+				const int unit = (have[h] ? ahead[h] : 0) * c.heads + kvh;
 				row[h] = have[h] ? unit * c.page + page_row(c, position(i * AP_KEYS + 32 * h + lane)) : -1; // (under 2^31)
-				if (have[h]) exps[h] = __float_as_int(__ldg(c.vs + unit));
-				if (have[h] && h == warp - 4) scale = __ldg(c.ks + unit);
+				exps[h] = __float_as_int(__ldg(c.vs + unit));
+				if (h == (warp & 1)) scale = __ldg(c.ks + unit);
 			}
 #pragma unroll
 			for (int k = 0; k < KEACH; ++k) {
 				const int key = (k * 4 + warp - 4) * KROWS + lane / PIECES, r = __shfl_sync(0xffffffffu, (k * 4 + warp - 4) * KROWS < 32 ? row[0] : row[1], key & 31);
-				kw[k] = make_uint4(0, 0, 0, 0);
-				if (r >= 0) kw[k] = ldg_stream(reinterpret_cast<const uint4*>(c.k + (long long)r * D) + lane % PIECES);
+				kw[k] = ldg_stream(reinterpret_cast<const uint4*>(c.k + (long long)max(r, 0) * D) + lane % PIECES);
 			}
+			mine = 0;
 #pragma unroll
 			for (int k = 0; k < 8; ++k) {
 				const int key = group8 * 8 + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
-				vw[k] = make_uint2(0, 0);
-				if (r >= 0 && works) vw[k] = ldg_stream8(reinterpret_cast<const uint2*>(c.v + (long long)r * D + dims));
+				vw[k] = ldg_stream8(reinterpret_cast<const uint2*>(c.v + (long long)max(r, 0) * D + (works ? dims : 0)));
+				mine |= (r >= 0 ? 1u : 0u) << k;
 			}
 			look(i + 1);
 		};
-		look(0);
-		if (tiles > 0) load(0);
+		if (tiles > 0) look(0), load(0);
 		for (int i = 0; i < tiles; ++i) {
 			const int st = i & 1;
 			if (!ap_wait_warp(s.kv_empty + st, ((i >> 1) & 1) ^ 1, &s.lost)) break;
@@ -916,6 +921,11 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			if (most == C8_NONE) most = 0;
 			if (t == 0) s.bias[st] = (float)most;
 			const bool even = __all_sync(0xffffffffu, (e[0] == most || e[0] == C8_NONE) && (e[1] == most || e[1] == C8_NONE));
+			if (mine != 0xff) { // (a code that is no number would spoil rows that do not see it)
+#pragma unroll
+				for (int k = 0; k < 8; ++k)
+					if (!(mine >> k & 1)) vw[k] = make_uint2(0, 0);
+			}
 			uint32_t down[4]; // of the pairs of this thread's keys, as fp16
 			if (!even) {
 #pragma unroll
@@ -997,7 +1007,7 @@ __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start) return;
 	for (long long row = (long long)blockIdx.x * 4 + warp; row < (long long)n * a.group; row += gridDim.x * 4) {
 		const int row0 = (int)(row / a.tile) * a.tile, rows = (int)min((long long)a.tile, (long long)n * a.group - row0);
-		const int shares = min(a.shares, (at_span(a, p0, row0, rows, (unsigned)slot < (unsigned)c.slots).chunks + a.each - 1) / a.each);
+		const int shares = min(a.shares, (at_span(a, p0, row0, rows, c.known(slot)).chunks + a.each - 1) / a.each);
 		if (shares <= 1) continue; // its one share has finished it
 		const int token = start + (int)(row / a.group), head = kvh * a.group + (int)(row % a.group), stride = c.dim + 2;
 		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * stride;
@@ -1071,7 +1081,7 @@ struct AtPlan {
 	int tile, shares, each, cluster; // tile 128: the prompt kernel
 };
 constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
-constexpr int AP_CTAS = 48;      // of the prompt kernel, from which on it is the faster one
+constexpr int AP_CTAS = 64;      // of the prompt kernel, from which on it is the faster one: 32 CTAs 47 us and 31 with the other, 75 43 and 50, 80 46 and 48, 256 54 and 131
 // Rows of a CTA: eight fill a product; more, where a sequence has more, read and convert the codes once for all of them, as far as registers hold their sums and CTAs are enough
 // for the GPU all the same.
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
@@ -1126,7 +1136,7 @@ template <int D, bool SPLIT>
 cudaError_t prompt_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	static std::atomic<uint64_t> done{0};
 	cudaError_t e = allow(k_c8_prompt<D, SPLIT>, sizeof(ApShared<D, SPLIT>), done);
-	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_prompt<D, SPLIT>, grid, dim3(AP_THREADS), sizeof(ApShared<D, SPLIT>), c, a);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_prompt<D, SPLIT>, dim3(grid.y, grid.z, grid.x), dim3(AP_THREADS), sizeof(ApShared<D, SPLIT>), c, a);
 	return e;
 }
 template <int D>
