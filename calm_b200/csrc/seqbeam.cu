@@ -5,8 +5,10 @@
 // from their lists.
 //   log sum_u exp x_u = m + log sum_s exp(m_s - m) S_s,   S_s = sum_(u in s) exp(x_u - m_s),   m = max m_s
 // Inside a row the order of scores is the order of logits, so a slice compares logits, as they are, and tokens (64-bit keys: ordered bits of the logit, then the lower
-// token); beams are compared in 64 bits by scores + (x - log-sum).  Bound: the logits' way through memory; a single request's few rows, the latency of two
-// launches.
+// token); beams are compared in 64 bits by scores + (x - log-sum).
+// Four beams of 32000 fp32 logits take 9.0 us (0.08 of bytes), 256 rows of 128256 32.2 us (4.1 TB/s; 20.1 of bytes), 400 rows of 128256 bf16 50.6 us.  Bound: few rows, the
+// latency of two launches and of a slice's end (the looks at its chunks, about 4 us); many, the latency of a warp's chunk - copy, maximum, sum - with 16 to 24 warps an SM, and a
+// 16-bit row the instructions of a logit.  Twice the bytes in flight a warp leaves two CTAs an SM: 160 rows 32.2 for 24.2 us.
 #include "seqops.cuh"
 #include "tc05.cuh"
 
@@ -17,14 +19,16 @@
 namespace seqops {
 namespace {
 
-constexpr int BM_THREADS = 256, BM_PER = 16; // logits that a thread takes at a time
-constexpr int BM_MAX = 64;                                                  // n
-constexpr int BM_LIST = 384;                                                // groups of four logits that may hold one of a slice's n highest
-constexpr int BM_KEYS = (1 + BM_PER) * BM_MAX;                              // single candidates, where the list overflows or is put in order
-constexpr int BM_WARPS = BM_THREADS / 32;
-constexpr int BM_RING = 4096;                                               // bytes that a warp has in flight
-constexpr int BM_LISTS = 256;                                               // slices of a group's rows
-constexpr int BM_CAND = 4096;                                               // candidates of a group that the merge compares with one another
+constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32, BM_PER = 16; // logits that a thread takes at a time: a chunk
+constexpr int BM_TILE = BM_THREADS * BM_PER, BM_SLICE = 64, BM_TILES = 160; // a CTA's at a time; tiles that a slice should have at most, and has at most
+constexpr int BM_RING = 4096;                                            // bytes that a warp has in flight
+constexpr int BM_MAX = 64;                                               // n
+constexpr int BM_LIST = 1024;                                            // chunks that may hold one of a slice's n highest
+constexpr int BM_KEYS = (1 + BM_PER) * BM_MAX;                           // single candidates
+constexpr int BM_LISTS = 256;                                            // slices of a group's rows
+constexpr int BM_MOST = 1 << 27;                                         // candidates of a group: so many fit BM_LISTS / beams slices of BM_TILES - 1 tiles, whatever the beams
+constexpr int BM_CAND = 4096;                                            // candidates of a group that the merge compares with one another
+
 struct BeamArgs {
 	const void* logits;
 	long long group_stride, row_stride;
@@ -54,105 +58,51 @@ __device__ __forceinline__ int rank_in(const u64* list, int c, u64 key) {
 	}
 	return r;
 }
-// What a CTA knows of its slice's highest logits.  Logits come in groups of four neighbours; a group whose highest is above tau joins the list (values as they are, so a thread spends
-// a few instructions on it), and now and then the list is cut down to the groups whose highest is among the n highest, the least of which is the new tau.  Only what is left at
-// the end becomes keys.  Tokens come in order, so a later value that equals tau is no candidate.
-struct BeamSlice {
-	alignas(128) unsigned char ring[BM_WARPS][BM_RING];
-	uint64_t full[BM_WARPS][4];
-	float4 quad[BM_LIST];
-	uint32_t token[BM_LIST]; // of the group's first value
+// A CTA's shared memory: rings of bulk copies while it reads its slice, then what it finds the slice's n highest with; behind it the highest logit of every chunk, [tiles][threads].
+struct BeamEnd {
 	alignas(16) float top[BM_LIST]; // (read four at a time, keys two at a time)
+	uint32_t chunk[BM_LIST];
 	alignas(16) u64 key[BM_KEYS + 2];
 	alignas(16) u64 best[BM_THREADS];
 	u64 sorted[BM_MAX];
-	uint32_t least[BM_THREADS / 32];
-	float red[BM_THREADS / 32];
+};
+struct BeamSlice {
+	union {
+		alignas(128) unsigned char ring[BM_WARPS][BM_RING];
+		BeamEnd end;
+	};
+	uint64_t full[BM_WARPS][4];
+	uint32_t least[BM_WARPS], low; // order bits
+	float red[BM_WARPS];
 	int count;
-	uint32_t low; // order bits
 	u64 bound;
 };
+static_assert(offsetof(BeamEnd, key) % 16 == 0 && offsetof(BeamEnd, best) % 16 == 0 && sizeof(BeamSlice) % 16 == 0, "read 16 bytes at a time");
+
 // The n highest of key[0 .. c), in order, take the front; returns how many there are.  Keys differ, so their ranks do.
 __device__ __noinline__ int keep_best(BeamSlice& b, int c, int n) { // (functions of their own: the loop over the logits keeps its registers)
 	const int tid = threadIdx.x;
-	if (tid == 0 && (c & 1)) b.key[c] = 0;
+	if (tid == 0 && (c & 1)) b.end.key[c] = 0;
 	__syncthreads();
 	for (int i = tid; i < c; i += BM_THREADS) {
-		const u64 k = b.key[i];
-		const int r = rank_in(b.key, c, k);
-		if (r < n) b.sorted[r] = k;
+		const u64 k = b.end.key[i];
+		const int r = rank_in(b.end.key, c, k);
+		if (r < n) b.end.sorted[r] = k;
 	}
 	__syncthreads();
 	const int have = min(c, n);
-	if (tid < have) b.key[tid] = b.sorted[tid];
+	if (tid < have) b.end.key[tid] = b.end.sorted[tid];
 	__syncthreads();
 	return have;
 }
-// Cuts the list's c groups (c <= BM_LIST) down to those with fewer than n higher ones; returns how many are left, the least of which is b.low.
-__device__ __noinline__ int cut(BeamSlice& b, int c, int n) {
-	constexpr int EACH = (BM_LIST + BM_THREADS - 1) / BM_THREADS;
-	const int tid = threadIdx.x;
-	float4 quad[EACH];
-	uint32_t token[EACH];
-	float mine[EACH];
-#pragma unroll
-	for (int i = 0; i < EACH; ++i) {
-		const int at = i * BM_THREADS + tid;
-		mine[i] = -INFINITY;
-		if (at < c) quad[i] = b.quad[at], token[i] = b.token[at], mine[i] = fmaxf(fmaxf(quad[i].x, quad[i].y), fmaxf(quad[i].z, quad[i].w));
-		if (at < ((c + 3) & ~3)) b.top[at] = mine[i];
-	}
-	if (tid == 0) b.count = 0, b.low = 0xffffffffu;
-	__syncthreads();
-	if (tid < c) {
-		int higher[EACH] = {};
-		const float4* tops = reinterpret_cast<const float4*>(b.top);
-#pragma unroll 4
-		for (int k = 0; k < (c + 3) / 4; ++k) {
-			const float4 t = tops[k];
-#pragma unroll
-			for (int i = 0; i < EACH; ++i) higher[i] += (t.x > mine[i]) + (t.y > mine[i]) + (t.z > mine[i]) + (t.w > mine[i]);
-		}
-#pragma unroll
-		for (int i = 0; i < EACH; ++i)
-			if (i * BM_THREADS + tid < c && higher[i] < n) {
-				const int at = atomicAdd(&b.count, 1);
-				b.quad[at] = quad[i], b.token[at] = token[i];
-				atomicMin(&b.low, order_bits(mine[i]));
-			}
-	}
-	__syncthreads();
-	return b.count;
-}
-// Keys of the list's c groups, the n highest in order; returns how many there are.
-__device__ __noinline__ int list_keys(BeamSlice& b, int c, int n) {
-	const int tid = threadIdx.x;
-	int k = 0;
-	for (int first = 0; first < c; first += BM_MAX) { // 4 BM_MAX values at a time beside the n kept ones
-		if (tid == 0) b.count = k;
-		__syncthreads();
-		if (tid < min(c - first, BM_MAX)) {
-			const float4 q = b.quad[first + tid];
-			const float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-			for (int e = 0; e < 4; ++e)
-				if (v[e] > -INFINITY) b.key[atomicAdd(&b.count, 1)] = beam_key(v[e], b.token[first + tid] + e);
-		}
-		__syncthreads();
-		k = keep_best(b, b.count, n);
-	}
-	return k;
-}
-
-// More groups than the list takes (rows in rising order, rows of few different values): the c groups listed before, and the tiles [v0, stop) since then once more, as
-// single candidates.  The n-th highest of the threads' highest values is no higher than the tile's n-th, and only n threads hold anything from it on: at most n * BM_PER values,
-// whatever the tile looks like.  The n highest become the list, as groups of one; returns how many there are.
+// The slice's n highest where too many values are as high as the n-th (rows of few different values): all of it once more, tile by tile.  The n-th highest of the threads' highest
+// values is no higher than the tile's n-th, and only n threads hold anything from it on: at most n * BM_PER values, whatever the tile looks like.
 template <typename T>
-__device__ __noinline__ int slow_tiles(BeamSlice& b, const uint4* base, unsigned v0, unsigned stop, unsigned end, unsigned shift, unsigned total, int c, int n) {
+__device__ __noinline__ int slow_tiles(BeamSlice& b, const uint4* base, unsigned begin, unsigned end, unsigned shift, unsigned total, int n) {
 	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE;
 	const int tid = threadIdx.x;
-	int k = list_keys(b, c, n);
-	for (; v0 < stop; v0 += NV * BM_THREADS) {
+	int k = 0;
+	for (unsigned v0 = begin; v0 < end; v0 += NV * BM_THREADS) {
 		u64 key[BM_PER], mine = 0;
 #pragma unroll
 		for (int j = 0; j < NV; ++j) {
@@ -168,36 +118,112 @@ __device__ __noinline__ int slow_tiles(BeamSlice& b, const uint4* base, unsigned
 				mine = max(mine, key[j * VE + e]);
 			}
 		}
-		b.best[tid] = mine;
+		b.end.best[tid] = mine;
 		if (tid == 0) b.bound = 1, b.count = k; // fewer than n threads with values: everything
 		const int valid = __syncthreads_count(mine != 0);
-		if (valid >= n && mine && rank_in(b.best, BM_THREADS, mine) == n - 1) b.bound = mine;
+		if (valid >= n && mine && rank_in(b.end.best, BM_THREADS, mine) == n - 1) b.bound = mine;
 		__syncthreads();
 		if (mine >= b.bound) {
 #pragma unroll
 			for (int i = 0; i < BM_PER; ++i)
-				if (key[i] >= b.bound) b.key[atomicAdd(&b.count, 1)] = key[i];
+				if (key[i] >= b.bound) b.end.key[atomicAdd(&b.count, 1)] = key[i];
 		}
 		__syncthreads();
 		k = keep_best(b, b.count, n);
 	}
-	if (tid < k) {
-		b.quad[tid] = make_float4(order_value((uint32_t)(b.key[tid] >> 32)), -INFINITY, -INFINITY, -INFINITY);
-		b.token[tid] = ~(uint32_t)b.key[tid];
-	}
 	return k;
+}
+// The slice's n highest from the highest logits of its chunks: the n-th highest of those is no higher than the slice's n-th, so the n highest lie in the chunks from it on.  m: the
+// thread's highest logit.  Returns how many there are, in order at the front of key.
+template <typename T>
+__device__ __noinline__ int slice_best(BeamSlice& b, const float* tops, int tiles, float m, const uint4* base, unsigned begin, unsigned end, unsigned shift, unsigned total, int n) {
+	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE;
+	constexpr unsigned WSTEP = NV * 32, STEP = WSTEP * BM_WARPS;
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+	// a value that n chunks reach: the least, over the warps with logits, of the k-th highest of a warp's threads, k warps >= n
+	const int warps = min(BM_WARPS, (int)((end - begin + WSTEP - 1) / WSTEP));
+	uint32_t u = m > -INFINITY ? order_bits(m) : 0, x = 0;
+	for (int k = (n + warps - 1) / warps; k > 0; --k) {
+		x = __reduce_max_sync(0xffffffffu, u);
+		if (__ffs(__ballot_sync(0xffffffffu, u == x)) - 1 == lane) u = 0;
+	}
+	if (lane == 0) b.least[warp] = x;
+	if (tid == 0) b.count = 0, b.low = 0xffffffffu;
+	__syncthreads();
+	uint32_t from = b.least[0];
+#pragma unroll
+	for (int i = 1; i < BM_WARPS; ++i)
+		if (i < warps) from = min(from, b.least[i]);
+	const float least = from ? order_value(from) : -INFINITY;
+	if (m >= least && m > -INFINITY)
+		for (int i = 0; i < tiles; ++i) {
+			const float v = tops[i * BM_THREADS + tid];
+			if (v >= least && v > -INFINITY) {
+				const int at = atomicAdd(&b.count, 1);
+				if (at < BM_LIST) b.end.top[at] = v, b.end.chunk[at] = i * BM_THREADS + tid;
+			}
+		}
+	__syncthreads();
+	const int c = b.count;
+	__syncthreads();
+	if (c > BM_LIST) return slow_tiles<T>(b, base, begin, end, shift, total, n);
+	// chunks with fewer than n higher ones
+	if (tid < (-c & 3)) b.end.top[c + tid] = -INFINITY;
+	if (tid == 0) b.count = 0;
+	__syncthreads();
+	for (int i = tid; i < c; i += BM_THREADS) {
+		const float mine = b.end.top[i];
+		int higher = 0;
+#pragma unroll 4
+		for (int k = 0; k < (c + 3) / 4; ++k) {
+			const float4 t = reinterpret_cast<const float4*>(b.end.top)[k];
+			higher += (t.x > mine) + (t.y > mine) + (t.z > mine) + (t.w > mine);
+		}
+		if (higher < n) {
+			const int at = atomicAdd(&b.count, 1);
+			if (at < BM_THREADS) reinterpret_cast<uint32_t*>(b.end.best)[at] = b.end.chunk[i];
+			atomicMin(&b.low, order_bits(mine));
+		}
+	}
+	__syncthreads();
+	const int left = b.count;
+	const float low = left >= n ? order_value(b.low) : -INFINITY;
+	__syncthreads();
+	if (left > BM_THREADS) return slow_tiles<T>(b, base, begin, end, shift, total, n);
+	// their logits, from memory once more
+	if (tid == 0) b.count = 0;
+	__syncthreads();
+	for (int i = tid; i < left * NV; i += BM_THREADS) {
+		const unsigned chunk = reinterpret_cast<const uint32_t*>(b.end.best)[i / NV], owner = chunk % BM_THREADS;
+		const unsigned o = begin + chunk / BM_THREADS * STEP + owner / 32 * WSTEP + i % NV * 32 + owner % 32;
+		if (o >= end) continue;
+		float v[VE];
+		unpack16<T>(ldg_stream(base + o), v);
+#pragma unroll
+		for (int e = 0; e < VE; ++e) {
+			const unsigned at = o * VE + e;
+			if (v[e] >= low && v[e] > -INFINITY && at >= shift && at < total) {
+				const int to = atomicAdd(&b.count, 1);
+				if (to < BM_KEYS) b.end.key[to] = beam_key(v[e], at - shift);
+			}
+		}
+	}
+	__syncthreads();
+	const int keys = b.count;
+	__syncthreads();
+	return keys > BM_KEYS ? slow_tiles<T>(b, base, begin, end, shift, total, n) : keep_best(b, keys, n);
 }
 
 // Per logit: a maximum, a difference, a product, an exponential, an addition (with a fused multiply-add against the maximum times log2(e) a row of the type's lowest values, whose
-// product is infinite, would have no sum).
+// product is infinite, would have no sum); per chunk one value kept.  No barrier between warps until the slice has been read.
 constexpr float BM_L2E = 1.4426950408889634f;
-static_assert(offsetof(BeamSlice, top) % 16 == 0 && offsetof(BeamSlice, key) % 16 == 0 && offsetof(BeamSlice, best) % 16 == 0, "read 16 bytes at a time");
 template <typename T>
-__global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) {
-	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE, QUADS = BM_PER / 4, STAGES = BM_RING / (NV * 512);
+__global__ void __launch_bounds__(BM_THREADS, 4) k_beam_slice(const BeamArgs a) {
+	constexpr int VE = 16 / sizeof(T), NV = BM_PER / VE, STAGES = BM_RING / (NV * 512);
 	constexpr unsigned WSTEP = NV * 32, STEP = WSTEP * BM_WARPS; // vectors of a warp's part of a tile, of a tile
 	extern __shared__ __align__(128) unsigned char slice_sm[];
 	BeamSlice& b = *reinterpret_cast<BeamSlice*>(slice_sm);
+	float* const tops = reinterpret_cast<float*>(slice_sm + sizeof(BeamSlice));
 	pdl_launch_next();
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, slice = blockIdx.x, row = blockIdx.y, n = a.n;
 	u64* const out = a.keys + ((size_t)row * a.slices + slice) * n;
@@ -212,11 +238,11 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) 
 	const uint4* const base = reinterpret_cast<const uint4*>(p - shift);
 	const unsigned total = a.vocab + shift, vectors = (total + VE - 1) / VE, each = (vectors + a.slices - 1) / a.slices;
 	const unsigned begin = min(vectors, slice * each), end = min(vectors, begin + each); // in vectors
-	// Each warp has a ring of its own, filled by bulk copies that run on while the block looks at its list.
+	// each warp has a ring of its own
 	uint64_t* const full = b.full[warp];
 	unsigned asked = begin + warp * WSTEP; // the warp's part of the next tile to request
 	const uint64_t policy = l2_policy_evict_first();
-	auto request = [&](int stage) {        // one lane
+	auto request = [&](int stage) { // one lane
 		if (asked < end) {
 			const uint32_t bytes = min(end - asked, WSTEP) * 16;
 			mbar_expect_tx(full + stage, bytes);
@@ -233,29 +259,14 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) 
 		if (lane == 0) request(i);
 		asked += STEP;
 	}
-	if (tid == 0) b.count = 0;
 	__syncwarp();
-	float m = -INFINITY, s = 0.f, tau = -INFINITY; // the thread's maximum and sum; a later group counts only above tau
-	int c = 0, stage = 0;                          // groups listed
+	float m = -INFINITY, s = 0.f; // the thread's maximum and sum
+	int stage = 0, tiles = 0;
 	uint32_t parity = 0;
 	bool lost = false; // a copy never came
-	auto spread = [&](unsigned v0, const uint4 (&w)[NV], float (&v)[BM_PER]) { // the tile's logits
-#pragma unroll
-		for (int j = 0; j < NV; ++j) unpack16<T>(w[j], *reinterpret_cast<float(*)[VE]>(v + j * VE));
-		if (v0 * VE < shift || v0 + STEP > end || (v0 + STEP) * VE > total) { // the row's first and last tile: places outside it
-#pragma unroll
-			for (int i = 0; i < BM_PER; ++i) {
-				const unsigned o = v0 + warp * WSTEP + (i / VE) * 32 + lane, e = o * VE + i % VE;
-				if (o >= end || e < shift || e >= total) v[i] = -INFINITY;
-			}
-		}
-	};
-	auto token = [&](unsigned v0, int i) { return (v0 + warp * WSTEP + (i / VE) * 32 + lane) * VE + i % VE - shift; };
-	unsigned next = begin, size = 1; // tiles between two looks at the list: more once few groups join it
-	while (next < end) {
-		const unsigned g0 = next, stop = g0 + size * STEP;
-		for (; next < end && next < stop; next += STEP) {
-			const unsigned v0 = next;
+	for (unsigned v0 = begin; v0 < end; v0 += STEP, ++tiles) {
+		float v[BM_PER];
+		{
 			uint4 w[NV];
 			if (v0 + warp * WSTEP < end && !lost) {
 				lost = !mbar_wait_warp(full + stage, parity);
@@ -263,80 +274,43 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) 
 #pragma unroll
 				for (int j = 0; j < NV; ++j) w[j] = src[j * 32];
 			}
-			float v[BM_PER];
-			spread(v0, w, v);
-			__syncwarp(); // all lanes have read
-			if (lane == 0 && !lost) request(stage);
-			asked += STEP;
-			if (++stage == STAGES) stage = 0, parity ^= 1;
-			float quad[QUADS], top = -INFINITY; // (a NaN is passed over)
 #pragma unroll
-			for (int i = 0; i < QUADS; ++i) quad[i] = fmaxf(fmaxf(fmaxf(v[4 * i], v[4 * i + 1]), v[4 * i + 2]), v[4 * i + 3]);
-#pragma unroll
-			for (int i = 0; i < QUADS; i += 2) top = fmaxf(fmaxf(top, quad[i]), quad[i + 1]);
-			if (top > m) s = m > -INFINITY && top < INFINITY ? s * ex2((m - top) * BM_L2E) : 0.f, m = top;
-			u64 part[2] = {0, 0};
-			const u64 down = pair_of(-m, -m), l2e = pair_of(BM_L2E, BM_L2E);
-#pragma unroll
-			for (int i = 0; i < BM_PER / 2; ++i) {
-				const float2 y = halves(mul2(add2(pair_of(v[2 * i], v[2 * i + 1]), down), l2e));
-				part[i & 1] = add2(part[i & 1], pair_of(ex2(y.x), ex2(y.y)));
-			}
-			const float2 both = halves(add2(part[0], part[1]));
-			float sum = both.x + both.y;
-			if (!(sum < INFINITY)) { // a NaN among the logits, nothing but -inf so far, or +inf: rare
-				sum = 0.f;
-				if (m > -INFINITY)
-#pragma unroll
-					for (int i = 0; i < BM_PER; ++i) sum += m == INFINITY ? (v[i] == INFINITY ? 1.f : 0.f) : v[i] > -INFINITY ? ex2((v[i] - m) * BM_L2E) : 0.f;
-			}
-			s += sum;
-			if (v0 == begin) {
-				// where to start: the least, over the warps with logits, of the k-th highest of a warp's lanes, k warps >= n, has n values at or above it
-				uint32_t u = top > -INFINITY ? order_bits(top) : 0, x = 0;
-				const int warps = min(BM_WARPS, (int)((end - begin + WSTEP - 1) / WSTEP));
-				for (int k = (n + warps - 1) / warps; k > 0; --k) {
-					x = __reduce_max_sync(0xffffffffu, u);
-					if (__ffs(__ballot_sync(0xffffffffu, u == x)) - 1 == lane) u = 0;
-				}
-				if (lane == 0) b.least[warp] = x;
-				__syncthreads();
-				x = b.least[0];
-#pragma unroll
-				for (int i = 1; i < BM_WARPS; ++i)
-					if (i < warps) x = min(x, b.least[i]);
-				if (x) tau = nextafterf(order_value(x), -INFINITY);
-			}
-			if (top > tau)
-#pragma unroll
-				for (int q = 0; q < QUADS; ++q)
-					if (quad[q] > tau) {
-						const int at = atomicAdd(&b.count, 1);
-						if (at < BM_LIST) {
-							b.quad[at] = make_float4(fmaxf(v[4 * q], -INFINITY), fmaxf(v[4 * q + 1], -INFINITY), fmaxf(v[4 * q + 2], -INFINITY), fmaxf(v[4 * q + 3], -INFINITY));
-							b.token[at] = token(v0, 4 * q);
-						}
-					}
+			for (int j = 0; j < NV; ++j) unpack16<T>(w[j], *reinterpret_cast<float(*)[VE]>(v + j * VE));
 		}
-		__syncthreads();
-		const int found = b.count;
-		__syncthreads();
-		if (found <= BM_LIST) {
-			c = found;
-			if (c > n) c = cut(b, c, n), tau = order_value(b.low);
-		} else {
-			const int k = slow_tiles<T>(b, base, g0, min(stop, end), end, shift, total, c, n);
-			c = k;
-			if (k == n) tau = order_value((uint32_t)(b.key[n - 1] >> 32));
+		if (v0 * VE < shift || v0 + STEP > end || (v0 + STEP) * VE > total) { // the row's first and last tile: places outside it
+#pragma unroll
+			for (int i = 0; i < BM_PER; ++i) {
+				const unsigned o = v0 + warp * WSTEP + (i / VE) * 32 + lane, e = o * VE + i % VE;
+				if (o >= end || e < shift || e >= total) v[i] = -INFINITY;
+			}
 		}
-		__syncthreads();
-		if (tid == 0) b.count = c;
-		__syncthreads();
-		size = next == begin + STEP ? 3 : min(4 * size, 24); // 1, 3, 12, 24, ...
+		__syncwarp(); // all lanes have read
+		if (lane == 0 && !lost) request(stage);
+		asked += STEP;
+		if (++stage == STAGES) stage = 0, parity ^= 1;
+		float top = -INFINITY; // (a NaN is passed over)
+#pragma unroll
+		for (int i = 0; i < BM_PER; i += 2) top = fmaxf(fmaxf(top, v[i]), v[i + 1]);
+		tops[tiles * BM_THREADS + tid] = top;
+		if (top > m) s = m > -INFINITY && top < INFINITY ? s * ex2((m - top) * BM_L2E) : 0.f, m = top;
+		u64 part[2] = {0, 0};
+		const u64 down = pair_of(-m, -m), l2e = pair_of(BM_L2E, BM_L2E);
+#pragma unroll
+		for (int i = 0; i < BM_PER / 2; ++i) {
+			const float2 y = halves(mul2(add2(pair_of(v[2 * i], v[2 * i + 1]), down), l2e));
+			part[i & 1] = add2(part[i & 1], pair_of(ex2(y.x), ex2(y.y)));
+		}
+		const float2 both = halves(add2(part[0], part[1]));
+		float sum = both.x + both.y;
+		if (!(sum < INFINITY)) { // a NaN among the logits, nothing but -inf so far, or +inf: rare
+			sum = 0.f;
+			if (m > -INFINITY)
+#pragma unroll
+				for (int i = 0; i < BM_PER; ++i) sum += m == INFINITY ? (v[i] == INFINITY ? 1.f : 0.f) : v[i] > -INFINITY ? ex2((v[i] - m) * BM_L2E) : 0.f;
+		}
+		s += sum;
 	}
 	if (lost) mbar_wait_bounded(full + stage, parity); // (a copy that comes late lands in memory that is still the block's)
-	const int k = list_keys(b, c, n);
-	for (int i = tid; i < n; i += BM_THREADS) out[i] = i < k ? b.key[i] : 0;
 	const float wm = warp_max(m);
 	if (lane == 0) b.red[warp] = wm;
 	const bool broken = __syncthreads_or(lost);
@@ -346,6 +320,8 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_slice(const BeamArgs a) 
 	const float ws = warp_sum(m == bm ? s : m > -INFINITY && bm < INFINITY ? s * ex2((m - bm) * BM_L2E) : 0.f);
 	__syncthreads();
 	if (lane == 0) b.red[warp] = ws;
+	const int k = begin < end ? slice_best<T>(b, tops, tiles, m, base, begin, end, shift, total, n) : 0;
+	for (int i = tid; i < n; i += BM_THREADS) out[i] = i < k ? b.end.key[i] : 0;
 	__syncthreads();
 	if (tid == 0) {
 		float sum = b.red[0];
@@ -368,8 +344,8 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	__shared__ float row_max[BM_MAX];
 	__shared__ uint32_t head_i[BM_THREADS];
 	__shared__ int count;
-	__shared__ double bound_d;
-	__shared__ uint32_t bound_i;
+	__shared__ double bound_d[BM_THREADS / 64];
+	__shared__ uint32_t bound_i[BM_THREADS / 64];
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = blockIdx.x, n = a.n, K = a.beams, S = a.slices, lists = K * S;
 	if (tid == 0) count = 0;
 	pdl_wait_prev();
@@ -397,24 +373,31 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 		i = (uint32_t)b * (uint32_t)a.vocab + ~(uint32_t)k;
 		return k != 0 && d > -INFINITY;
 	};
-	// Lists are in order.  Of the values at one depth of all lists the r-th highest, r (depth + 1) >= n, has n values at or above it; at most r lists reach it
-	// there, so what is at or above it is at most r n values and the others' first `depth`: n lists' worth.
-	const int depth = max(0, (n + lists - 1) / lists - 1), r = (n + depth) / (depth + 1);
+	// Lists are in order.  Of the values at one depth of all lists the r-th highest, r (depth + 1) >= n, has n values at or above it; at the least such depth at most r lists reach
+	// it there, so what is at or above it is at most r n values and the others' first `depth`: n lists' worth.  Where lists are few, other threads look at twice that depth, four
+	// times, ...: the highest of the bounds leaves far fewer (64 lists of 64 values: the lowest list's head bounds nothing).
+	int width = 64;
+	while (width < lists) width *= 2;
+	const int set = tid / width, list = tid % width, depth = ((n + lists - 1) / lists << set) - 1, r = (n + depth) / (depth + 1);
 	double d = 0.;
 	uint32_t i = 0;
-	const bool have = tid < lists && value(tid, depth, d, i);
+	const bool have = list < lists && depth < n && value(list, depth, d, i);
 	head_d[tid] = have ? d : -INFINITY, head_i[tid] = have ? i : 0xffffffffu;
-	if (tid == 0) bound_d = -INFINITY, bound_i = 0xffffffffu; // fewer than r lists reach the depth: everything
-	const int valid = __syncthreads_count(have);
-	if (have && valid >= r) {
+	if (list == 0) bound_d[set] = -INFINITY, bound_i[set] = 0xffffffffu; // fewer than r lists reach the depth: everything
+	__syncthreads();
+	if (have) {
 		int rank = 0;
 #pragma unroll 8
-		for (int k = 0; k < lists; ++k) rank += above(head_d[k], head_i[k], d, i);
-		if (rank == r - 1) bound_d = d, bound_i = i;
+		for (int k = 0; k < lists; ++k) rank += above(head_d[set * width + k], head_i[set * width + k], d, i);
+		if (rank == r - 1) bound_d[set] = d, bound_i[set] = i;
 	}
 	__syncthreads();
+	double low_d = bound_d[0];
+	uint32_t low_i = bound_i[0];
+	for (int k = 1; k < BM_THREADS / width; ++k)
+		if (above(bound_d[k], bound_i[k], low_d, low_i)) low_d = bound_d[k], low_i = bound_i[k];
 	for (int e = tid; e < lists * n; e += BM_THREADS)
-		if (value(e / n, e % n, d, i) && !above(bound_d, bound_i, d, i)) {
+		if (value(e / n, e % n, d, i) && !above(low_d, low_i, d, i)) {
 			const int at = atomicAdd(&count, 1);
 			if (at < BM_CAND) cand.d[at] = d, cand.i[at] = i;
 		}
@@ -430,23 +413,28 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	for (int e = c + tid; e < n; e += BM_THREADS) a.tokens[base + e] = a.parents[base + e] = -1, a.best[base + e] = -INFINITY;
 }
 
-// Slices of a row: 4096 logits each where rows are few, as many as two CTAs an SM hold at a time where they are many.
+// Slices of a row: a tile each where rows are few, three CTAs an SM in all where they are many (148 / 296 / 444 / 592 CTAs in all: 160 rows of 128256 fp32 30.5 / 30.9 / 24.2 /
+// 34.7 us, 100 rows 26.4 / 20.3 / 18.1 / 24.1, 64 rows 18.2 / 15.9 / 16.5 / 18.2: a slice's end costs about the same whatever its length), two an SM for the longest rows.
 int beam_slices(int groups, int beams, int vocab) {
-	const int rows = groups * beams, most = cdiv(vocab, 4096);
-	return std::max(1, std::min({most, 148 * 2 / rows, BM_LISTS / beams}));
+	const int want = std::max(std::min(cdiv(vocab, BM_TILE), 148 * 3 / (groups * beams)), cdiv(vocab, BM_TILE * BM_SLICE));
+	return std::max(cdiv(vocab, BM_TILE * (BM_TILES - 1)), std::min(want, BM_LISTS / beams)); // (a row that starts behind a 16-byte boundary may reach into one tile more)
+}
+size_t beam_shared(const BeamArgs& a, int size) { // tiles of a slice, as the kernel cuts them at the worst alignment
+	const int ve = 16 / size, each = cdiv(cdiv(a.vocab + ve - 1, ve), a.slices);
+	return sizeof(BeamSlice) + (size_t)cdiv(each, BM_TILE / ve) * BM_THREADS * sizeof(float);
 }
 size_t beam_keys(int groups, int beams, int vocab, int n) { return ((size_t)groups * beams * beam_slices(groups, beams, vocab) * n * sizeof(u64) + 15) & ~(size_t)15; }
 
 template <typename T>
 cudaError_t beam_launch(const BeamArgs& a, dim3 grid, cudaStream_t st) {
 	static std::atomic<uint64_t> done{0};
-	const cudaError_t e = allow(k_beam_slice<T>, sizeof(BeamSlice), done);
-	return e == cudaSuccess ? launch(st, false, 1, k_beam_slice<T>, grid, dim3(BM_THREADS), sizeof(BeamSlice), a) : e;
+	const cudaError_t e = allow(k_beam_slice<T>, sizeof(BeamSlice) + BM_TILES * BM_THREADS * sizeof(float), done);
+	return e == cudaSuccess ? launch(st, false, 1, k_beam_slice<T>, grid, dim3(BM_THREADS), beam_shared(a, sizeof(T)), a) : e;
 }
 
 int beam_check(int groups, int beams, int vocab, int n) {
 	if (groups < 0 || beams < 1 || beams > 64) return refuse("beam: %d groups of %d beams (at most 64 beams)", groups, beams);
-	if (vocab < 1 || (long long)beams * vocab >= (1LL << 31)) return refuse("beam: %d beams over %d tokens: at most 2^31 candidates", beams, vocab);
+	if (vocab < 1 || (long long)beams * vocab > BM_MOST) return refuse("beam: %d beams over %d tokens: at most 2^27 candidates a group", beams, vocab);
 	if (n < 1 || n > BM_MAX) return refuse("beam: n = %d is not in 1 .. %d", n, BM_MAX);
 	if ((long long)groups * beams > 65535) return refuse("beam: %d rows in all, at most 65535", groups * beams);
 	return 0;

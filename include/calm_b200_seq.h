@@ -350,7 +350,7 @@ struct SeqBeam {
 	int type;            /* enum SeqType */
 	long long group_stride, row_stride; /* in elements */
 	const float* scores; /* [groups][beams] */
-	int groups, beams, vocab, n; /* 1 <= beams <= 64, 1 <= n <= 64, beams * vocab < 2^31 */
+	int groups, beams, vocab, n; /* 1 <= beams <= 64, 1 <= n <= 64, beams * vocab <= 2^27 */
 	int* tokens;         /* [groups][n] */
 	int* parents;        /* [groups][n]: beam of the group */
 	float* best;         /* [groups][n] */

@@ -34,7 +34,7 @@ def beam(**over):
 
 def test_beam_refusals():
     says(L.calm_b200_seq_beam_select(None, None), "no arguments")
-    for over, word in ((dict(beams=0), "beams"), (dict(beams=65), "64"), (dict(groups=-1), "groups"), (dict(vocab=0), "tokens"), (dict(vocab=1 << 30), "2^31"), (dict(n=0), "n = 0"),
+    for over, word in ((dict(beams=0), "beams"), (dict(beams=65), "64"), (dict(groups=-1), "groups"), (dict(vocab=0), "tokens"), (dict(vocab=1 << 30), "2^27"), (dict(n=0), "n = 0"),
                        (dict(n=65), "n = 65"), (dict(groups=20000), "65535"), (dict(type=3), "type"), (dict(logits=None), "pointer"), (dict(scores=None), "pointer"), (dict(tokens=None), "pointer"),
                        (dict(parents=None), "pointer"), (dict(best=None), "pointer"), (dict(workspace=None), "pointer"), (dict(logits=4098), "aligned"), (dict(workspace=4104), "aligned"),
                        (dict(workspace_bytes=8), "are needed"), (dict(type=1, logits=4097), "aligned")):

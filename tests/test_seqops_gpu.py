@@ -36,7 +36,8 @@ def check_beam(logits, scores, n, got=None):
 
 @pytest.mark.parametrize("groups,beams,vocab,n,dtype", [
     (1, 1, 1, 1, "fp32"), (1, 1, 1, 5, "bf16"), (1, 1, 17, 20, "fp32"), (2, 3, 257, 6, "fp32"), (1, 4, 4096, 8, "fp32"), (1, 4, 4097, 8, "fp16"), (3, 5, 4099, 10, "bf16"),
-    (1, 1, 50257, 64, "fp32"), (1, 64, 700, 64, "fp32"), (7, 16, 1000, 16, "fp16"), (2, 2, 131072, 3, "bf16"), (40, 8, 9001, 16, "fp32"), (300, 1, 33, 2, "fp32")])
+    (1, 1, 50257, 64, "fp32"), (1, 64, 700, 64, "fp32"), (7, 16, 1000, 16, "fp16"), (2, 2, 131072, 3, "bf16"), (40, 8, 9001, 16, "fp32"), (300, 1, 33, 2, "fp32"),
+    (150, 3, 40001, 10, "fp16"), (4, 64, 20000, 64, "fp32"), (1, 1, 3000000, 3, "bf16")])
 def test_beams_of_random_logits(groups, beams, vocab, n, dtype):
     g = torch.Generator(device="cuda").manual_seed(vocab + n)
     logits = (torch.randn(groups, beams, vocab, generator=g, device="cuda") * 3).to(DT[dtype])
@@ -52,6 +53,19 @@ def test_beams_of_ordered_rows(order, n):
     row = {"equal": torch.zeros_like(i), "rising": i * 1e-3, "falling": -i * 1e-3, "late": torch.where(i > V - 100, 5.0, i * 1e-5), "two values": torch.where(i % 2 == 1, 1.0, -1.0)}[order]
     logits = torch.stack([row, row - 1.0]).expand(2, 2, V)
     check_beam(logits, torch.tensor([[-1.0, -1.25], [-3.0, -2.5]], device="cuda"), n)
+
+
+def test_beams_of_the_longest_rows():
+    V = 1 << 21  # (2^27 candidates a group)
+    row = torch.randperm(V, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").float() / (1 << 18)
+    scores = torch.full((1, 64), -100.0, device="cuda")  # only beam 5 counts: no other beam's best reaches its 64th
+    scores[0, 5] = -1.0
+    tok, par, best = seqops.beam_select(row.expand(1, 64, V), scores, 64)
+    top = torch.argsort(row, descending=True)[:64]
+    assert torch.equal(tok[0].long(), top) and (par == 5).all()
+    want = row[top].double() - torch.logsumexp(row.double(), 0) - 1.0
+    off = (best[0].double() - want).abs()
+    assert (off <= plain.F32 * want.abs() + plain.log_sum_bound(V)).all(), off.max()
 
 
 def test_beams_with_rows_that_leave_nothing_and_special_values():
