@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // Where a sequence brings many rows, the products run on the fifth-generation tensor cores: a CTA takes 128 rows (pairs of token and head, as above) of one key head and walks
 // tiles of 64 keys.  Four warps read codes, a tile ahead, and lay them out in fp16 as the products' operands (keys as they are, values transposed); one thread issues
 // S = Q K^T of the next tile and O += P V of this one; four warps, a row a thread, take S from tensor memory, form the weights (exponents, references and denominators as
-// above) and write them to shared memory as the next product's operand.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.
+// above) and write them back where the scores stood: the next product's operand.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.
 //   warps 0-3  softmax and output;  4-7  keys and values;  8  products
 // Bound: for 128 channels a tile costs the tensor cores 512 cycles and the exponentials as many; two CTAs share an SM.
 constexpr int AP_ROWS = 128, AP_KEYS = 64, AP_THREADS = 288, C8_NONE = -1000;
@@ -621,11 +621,10 @@ struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	unsigned char q[PAIR][PANELS][AP_ROWS * 128];
 	unsigned char k[2][PANELS][AP_KEYS * 128];
 	unsigned char v[2][D * 128];
-	unsigned char p[PAIR][AP_ROWS * 128];
 	float factor[2][AP_KEYS]; // of a tile's keys on their scores, in log2
 	float bias[2];            // log2 of the largest of the tile's value scales: its values come in units of that
 	uint32_t seen[2][2];      // keys that are there
-	uint64_t kv_full[2], kv_empty[2], s_full[2], s_empty[2], p_full, p_empty, done;
+	uint64_t kv_full[2], kv_empty[2], s_full[2], p_full, p_empty, done;
 	uint32_t tmem;
 	float top[4];
 	int lost;
@@ -654,14 +653,30 @@ __device__ __forceinline__ void load8(const void* p, int type, long long i, bool
 		else unpack16<__half>(w, x);
 	}
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-#define AP_R(i) "r"(__float_as_uint(v[i]))
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) { // (tcgen05.wait::st is the caller's)
 	asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-	             AP_R(0), AP_R(1), AP_R(2), AP_R(3), AP_R(4), AP_R(5), AP_R(6), AP_R(7), AP_R(8), AP_R(9), AP_R(10), AP_R(11), AP_R(12), AP_R(13), AP_R(14), AP_R(15), AP_R(16), AP_R(17),
-	             AP_R(18), AP_R(19), AP_R(20), AP_R(21), AP_R(22), AP_R(23), AP_R(24), AP_R(25), AP_R(26), AP_R(27), AP_R(28), AP_R(29), AP_R(30), AP_R(31)
+	             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+	             "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
 	             : "memory");
-#undef AP_R
-	asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// 32 lanes x 8 columns times f
+__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
+	float v[8];
+	asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+	             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+	asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+	             "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f), "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f)
+	             : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] . B[smem]^T: A's rows are lanes, a column holds two neighbouring fp16 of a row
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+	asm volatile(
+	    "{\n\t.reg .pred p;\n\t"
+	    "setp.ne.b32 p, %4, 0;\n\t"
+	    "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+	    ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+	    : "memory");
 }
 __device__ __forceinline__ int ap_exponent(const float (&tops)[4]) { // queries times 2^-this stand at 2^AT_LIFT or less
 	const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 
 	if (warp == 8) tmem_alloc(&s.tmem, 256);
 	if (tid == 0) {
-		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 4), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1), mbar_init(s.s_empty + i, 4); // (a warp arrives as one)
+		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 4), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1); // (a warp arrives as one)
 		mbar_init(&s.p_full, 4), mbar_init(&s.p_empty, 1), mbar_init(&s.done, 1);
 		s.lost = 0;
 		mbar_init_fence();
@@ -737,77 +752,56 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			const uint32_t seen[2] = {s.seen[buf][0], s.seen[buf][1]};
 			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
 			const float bias = s.bias[buf];
-			float z[32], base = m == -INFINITY ? 0.f : m;
-			// log2 of the weights of keys 32 h .. against the reference (against 0 before there is one); returns the largest
-			auto scores = [&](int h) {
-				tmem_ld32(tmem + lanes + buf * 64 + 32 * h, z);
-				const u64 off = pair_of(bias - base, bias - base);
+			const float base = m == -INFINITY ? 0.f : m, most = m == -INFINITY ? -INFINITY : AT_MOST;
+			float z[64], top = -INFINITY; // log2 of the weights against the reference as it stands (against 0 before there is one)
+			tmem_ld32(tmem + lanes + buf * 64, *reinterpret_cast<float(*)[32]>(z));
+			tmem_ld32(tmem + lanes + buf * 64 + 32, *reinterpret_cast<float(*)[32]>(z + 32));
+			const u64 off = pair_of(bias - base, bias - base);
 #pragma unroll
-				for (int k = 0; k < 32; k += 4) {
-					const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[buf] + 32 * h + k);
-					const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), f.x, off)), y = halves(fma2(pair_of(z[k + 2], z[k + 3]), f.y, off));
-					z[k] = x.x, z[k + 1] = x.y, z[k + 2] = y.x, z[k + 3] = y.y;
-				}
-				if (!all) {
-#pragma unroll
-					for (int k = 0; k < 32; ++k) {
-						const int kp = position(j0 + 32 * h + k);
-						if (!((seen[h] >> k & 1) && kp <= rpos && (kp >= rlow || kp < a.keep_first))) z[k] = -INFINITY;
-					}
-				}
-				float top = -INFINITY;
-#pragma unroll
-				for (int k = 0; k < 32; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
-				return top;
-			};
-			u64 sum = 0;
-			auto weights = [&](int h) {
-#pragma unroll
-				for (int k = 0; k < 32; k += 8) {
-					uint32_t hi[4], rest[4];
-#pragma unroll
-					for (int e = 0; e < 8; e += 2) {
-						const float w0 = ex2(z[k + e]), w1 = ex2(z[k + e + 1]);
-						sum = add2(sum, pair_of(w0, w1));
-						hi[e / 2] = pack_f16(w0, w1), rest[e / 2] = SPLIT ? pack_rest(w0, w1, hi[e / 2]) : 0;
-					}
-					const int place = tid * 128 + (((4 * h + k / 8) ^ (tid & 7)) << 4);
-					*reinterpret_cast<uint4*>(s.p[0] + place) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-					if (SPLIT) *reinterpret_cast<uint4*>(s.p[Shared::PAIR - 1] + place) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-				}
-			};
-			// half by half against the reference as it stands; where a row passes it, the warp looks at both halves, moves references and starts anew
-			const float most = m == -INFINITY ? -INFINITY : AT_MOST;
-			bool moved = __any_sync(0xffffffffu, scores(0) > most);
-			if (i > 0 && !ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break; // the product before has read the weights and left the sums
-			tc_fence_after();
-			if (!moved) {
-				weights(0);
-				moved = __any_sync(0xffffffffu, scores(1) > most);
+			for (int k = 0; k < 64; k += 4) {
+				const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[buf] + k);
+				const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), f.x, off)), y = halves(fma2(pair_of(z[k + 2], z[k + 3]), f.y, off));
+				z[k] = x.x, z[k + 1] = x.y, z[k + 2] = y.x, z[k + 3] = y.y;
 			}
-			if (moved) {
-				const float top = fmaxf(scores(0), scores(1)), mn = top > most ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn);
-				if (i > 0) { // (there are sums)
+			if (!all) {
+#pragma unroll
+				for (int k = 0; k < 64; ++k) {
+					const int kp = position(j0 + k);
+					if (!((seen[k / 32] >> (k & 31) & 1) && kp <= rpos && (kp >= rlow || kp < a.keep_first))) z[k] = -INFINITY;
+				}
+			}
+#pragma unroll
+			for (int k = 0; k < 64; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
+			if (__any_sync(0xffffffffu, top > most)) { // references move
+				const float mn = top > most ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
+#pragma unroll
+				for (int k = 0; k < 64; ++k) z[k] += by;
+				m = mn, l *= f;
+				if (i > 0) { // there are sums
+					if (!ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break;
+					tc_fence_after();
 #pragma unroll 1
-					for (int col = 0; col < D; col += 32) {
-						tmem_ld32(tmem + lanes + 128 + col, z);
-#pragma unroll
-						for (int k = 0; k < 32; ++k) z[k] *= f;
-						tmem_st32(tmem + lanes + 128 + col, z);
-					}
+					for (int col = 0; col < D; col += 8) tmem_scale8(tmem + lanes + 128 + col, f);
+					tmem_st_wait();
 				}
-				m = mn, l *= f, sum = 0, base = m == -INFINITY ? 0.f : m;
-				scores(0);
-				weights(0);
-				scores(1);
 			}
-			weights(1);
+			u64 sum = 0;
+			uint32_t hi[32], rest[32];
+#pragma unroll
+			for (int k = 0; k < 64; k += 2) {
+				const float w0 = ex2(z[k]), w1 = ex2(z[k + 1]);
+				sum = add2(sum, pair_of(w0, w1));
+				hi[k / 2] = pack_f16(w0, w1), rest[k / 2] = SPLIT ? pack_rest(w0, w1, hi[k / 2]) : 0;
+			}
+			tmem_st32(tmem + lanes + buf * 64, hi); // where the scores were
+			if (SPLIT) tmem_st32(tmem + lanes + buf * 64 + 32, rest);
 			const float2 sums = halves(sum);
 			l = fmaf(sums.x + sums.y, pow2f(-(int)bias), l); // the weights hold the value scale
+			tmem_st_wait();
+			if (i > 0 && !ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break; // (long done: the barrier's phases stay in step)
 			tc_fence_before();
-			fence_async_smem();
 			__syncwarp();
-			if (lane == 0) mbar_arrive(s.s_empty + buf), mbar_arrive(&s.p_full);
+			if (lane == 0) mbar_arrive(&s.p_full);
 		}
 		if (tiles > 0) ap_wait_warp(&s.p_empty, (tiles - 1) & 1, &s.lost);
 		tc_fence_after();
@@ -967,7 +961,7 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			if (i < tiles) {
 				const int buf = i & 1;
 				const uint32_t parity = (i >> 1) & 1;
-				if (!ap_wait(s.kv_full + buf, parity, &s.lost) || !ap_wait(s.s_empty + buf, parity ^ 1, &s.lost)) break;
+				if (!ap_wait(s.kv_full + buf, parity, &s.lost)) break; // (the scores' columns: the product of the tile before the last, which read weights there, was issued earlier)
 				tc_fence_after();
 #pragma unroll
 				for (int h = 0; h < Shared::PAIR; ++h)
@@ -985,7 +979,7 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 #pragma unroll
 				for (int h = 0; h < Shared::PAIR; ++h)
 #pragma unroll
-					for (int k = 0; k < 4; ++k) umma_f16(tmem + 128, umma_desc_sw128(s.p[h]) + 2 * k, umma_desc_sw128(s.v[j & 1]) + 2 * k, value, (j | h | k) ? 1u : 0u);
+					for (int k = 0; k < 4; ++k) umma_f16_ts(tmem + 128, tmem + (j & 1) * 64 + 32 * h + 8 * k, umma_desc_sw128(s.v[j & 1]) + 2 * k, value, (j | h | k) ? 1u : 0u);
 				umma_commit(s.kv_empty + (j & 1));
 				umma_commit(&s.p_empty);
 			}
