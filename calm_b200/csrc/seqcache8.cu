@@ -51,8 +51,8 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t codes) {
 
 // ---------------------------------------------------------------- storing
 // A warp takes one page of a sequence's new rows, one head, keys or values: the largest finite value, the scale, the codes of earlier rows where the scale grew, the codes
-// of the new rows.  Pages are independent, so a prompt's run side by side.  Bound: memory for prompts (rows read once from DRAM, once more from L1),
-// latency for single tokens.
+// of the new rows.  Pages are independent, so a prompt's run side by side.  Bound: memory for prompts (rows read once from DRAM, once more from L1: 3990 rows of 8 heads of 128
+// fp32 channels 11.2 us, 4.6 TB/s), latency for single tokens (32 of them 2.8 us: the page's number, its scale, its rows one after another).
 constexpr int ST_WARPS = 4;
 struct StoreRows {
 	const void* p;
@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 // channels x queries), so that eight rows of queries fill a product.  An e4m3 code is exact in fp16; scales do not enter the products: a key's scale multiplies its scores,
 // a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are rounded to fp16 at 2^15 or less; the denominator sums
 // w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z: almost only in a warp's first chunks.
+// 64 tokens of 32 heads over 2000 to 8000 keys of 8 heads of 128 channels (656 MB): 125 us, 5.3 TB/s; one over 4000 keys 10.8 us.  Bound: with many CTAs issue and the latency of
+// a warp's chunk (1.7 warp instructions a cycle; 49 million in all), with few the latency of copy, products, softmax and the cluster's fold.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
 constexpr int AT_SHARES = 64;  // of a tile's keys at most
 constexpr int AT_CLUSTER_ROWS = 16, AT_CLUSTER = 16; // shares that a thread-block cluster folds: of tiles of 16 rows at most, as many
@@ -604,29 +606,34 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 }
 
 // ---------------------------------------------------------------- attention of prompts
-// Where a sequence brings many rows, the products run on the fifth-generation tensor cores: a CTA takes 128 rows (pairs of token and head, as above) of one key head and walks
-// tiles of 64 keys.  Four warps read codes, a tile ahead, and lay them out in fp16 as the products' operands (keys as they are, values transposed); one thread issues
-// S = Q K^T of the next tile and O += P V of this one; four warps, a row a thread, take S from tensor memory, form the weights (exponents, references and denominators as
-// above) and write them back where the scores stood: the next product's operand.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.
-//   warps 0-3  softmax and output;  4-7  keys and values;  8  products
-// Bound: for 128 channels a tile costs the tensor cores 512 cycles and the exponentials as many; two CTAs share an SM.
-constexpr int AP_ROWS = 128, AP_KEYS = 64, AP_THREADS = 288, C8_NONE = -1000;
+// Where a sequence brings many rows, the products run on the fifth-generation tensor cores: a CTA takes two groups of 128 rows (pairs of token and head, as above; one group where
+// queries are pairs) of one key head and walks tiles of 64 keys.  Four warps a group read codes, a tile ahead, and lay them out in fp16 as the products' operands (keys as they are,
+// values transposed), once for both groups; one thread issues S = Q K^T of the next tile and O += P V of this one; four warps a group, a row a thread, take S from tensor memory, form
+// the weights (exponents, references and denominators as above) and write them back where the scores stood: the next product's operand.  O stays in tensor memory; it is rescaled
+// in the rare case that a row's reference moves.
+//   warps, in fours: softmax and output of each group; keys and values; a warp for the products
+// 1500 and 700 queries of 16 heads behind 700 and 300 keys of 128 channels: 77 us (one group a CTA and two CTAs an SM 86, with the weights through shared memory 95).  Bound: the way of a tile
+// through its roles, about 3900 cycles, of which a softmax warp works 3000 (its exponentials keep the units busy for 1024 of them, the tensor cores are for about 1300); registers
+// hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86), registers moved from them to the softmax 76.
+constexpr int AP_KEYS = 64, C8_NONE = -1000;
+constexpr int ap_groups(bool split) { return split ? 1 : 2; } // of 128 rows
+constexpr int ap_threads(bool split) { return 256 * ap_groups(split) + 32; }
 __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
 	const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
 	return *reinterpret_cast<const uint32_t*>(&r);
 }
 template <int D, bool SPLIT>
 struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
-	static constexpr int PANELS = D / 64, PAIR = SPLIT ? 2 : 1;
-	unsigned char q[PAIR][PANELS][AP_ROWS * 128];
-	unsigned char k[2][PANELS][AP_KEYS * 128];
-	unsigned char v[2][D * 128];
-	float factor[2][AP_KEYS]; // of a tile's keys on their scores, in log2
-	float bias[2];            // log2 of the largest of the tile's value scales: its values come in units of that
-	uint32_t seen[2][2];      // keys that are there
-	uint64_t kv_full[2], kv_empty[2], s_full[2], p_full, p_empty, done;
+	static constexpr int PANELS = D / 64, PAIR = SPLIT ? 2 : 1, GROUPS = ap_groups(SPLIT), STAGES = 2 + (GROUPS > 1);
+	unsigned char q[GROUPS][PAIR][PANELS][128 * 128];
+	unsigned char k[STAGES][PANELS][AP_KEYS * 128];
+	unsigned char v[STAGES][D * 128];
+	float factor[STAGES][AP_KEYS]; // of a tile's keys on their scores, in log2
+	float bias[STAGES];            // log2 of the largest of the tile's value scales: its values come in units of that
+	uint32_t seen[STAGES][2];      // keys that are there
+	uint64_t kv_full[STAGES], kv_empty[STAGES], s_full[GROUPS][2], p_full[GROUPS], p_empty[GROUPS], done;
 	uint32_t tmem;
-	float top[4];
+	float top[4 * GROUPS];
 	int lost;
 };
 // false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN
@@ -678,35 +685,41 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
 	    ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
 	    : "memory");
 }
-__device__ __forceinline__ int ap_exponent(const float (&tops)[4]) { // queries times 2^-this stand at 2^AT_LIFT or less
-	const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+template <int N>
+__device__ __forceinline__ int ap_exponent(const float (&tops)[N]) { // queries times 2^-this stand at 2^AT_LIFT or less
+	float top = tops[0];
+#pragma unroll
+	for (int i = 1; i < N; ++i) top = fmaxf(top, tops[i]);
 	return (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT;
 }
 template <int D, bool SPLIT>
-__global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C8 c, const Attend a) {
+__global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, const Attend a) {
 	typedef ApShared<D, SPLIT> Shared;
-	constexpr int PANELS = Shared::PANELS, PIECES = D / 16;
+	constexpr int PANELS = Shared::PANELS, PIECES = D / 16, GROUPS = Shared::GROUPS, STAGES = Shared::STAGES, WARPS = 4 * GROUPS, ROWS = 128 * GROUPS; // WARPS: of the softmax, and as many of the codes
+	constexpr uint32_t S_COLS = 64 * GROUPS, O_COL = 2 * S_COLS;
 	extern __shared__ __align__(1024) unsigned char ap_raw[]; // (all of the kernel's shared memory: it starts where the swizzle's pattern does)
 	Shared& s = *reinterpret_cast<Shared*>(ap_raw);
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	const int b = blockIdx.y, kvh = blockIdx.x, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b];
-	const int tile = (int)min((long long)gridDim.z, ((long long)n * a.group + AP_ROWS - 1) / AP_ROWS) - 1 - (int)blockIdx.z; // (every sequence's longest rows first)
-	if (tile < 0 || n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * AP_ROWS >= (long long)n * a.group) return;
-	const int row0 = tile * AP_ROWS, rows = (int)min((long long)AP_ROWS, (long long)n * a.group - row0);
+	const int tile = (int)min((long long)gridDim.z, ((long long)n * a.group + ROWS - 1) / ROWS) - 1 - (int)blockIdx.z; // (every sequence's longest rows first)
+	if (tile < 0 || n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * ROWS >= (long long)n * a.group) return;
+	const int row0 = tile * ROWS, rows = (int)min((long long)ROWS, (long long)n * a.group - row0);
 	const AtSpan sp = at_span(a, p0, row0, rows, c.known(slot));
 	const int tiles = (sp.total + AP_KEYS - 1) / AP_KEYS;
 	auto position = [&](int j) { return j < sp.kept ? j : sp.lo + (j - sp.kept); };
 
-	if (warp == 8) tmem_alloc(&s.tmem, 256);
+	const int groups = rows > 128 ? GROUPS : 1;
+	if (warp == 2 * WARPS) tmem_alloc(&s.tmem, 256 * GROUPS);
 	if (tid == 0) {
-		for (int i = 0; i < 2; ++i) mbar_init(s.kv_full + i, 4), mbar_init(s.kv_empty + i, 1), mbar_init(s.s_full + i, 1); // (a warp arrives as one)
-		mbar_init(&s.p_full, 4), mbar_init(&s.p_empty, 1), mbar_init(&s.done, 1);
+		for (int i = 0; i < STAGES; ++i) mbar_init(s.kv_full + i, WARPS), mbar_init(s.kv_empty + i, 1); // (a warp arrives as one)
+		for (int g = 0; g < GROUPS; ++g) mbar_init(s.s_full[g], 1), mbar_init(s.s_full[g] + 1, 1), mbar_init(s.p_full + g, 4), mbar_init(s.p_empty + g, 1);
+		mbar_init(&s.done, 1);
 		s.lost = 0;
 		mbar_init_fence();
 	}
 	// queries, times the tile's power of two
 	const int token = start + (row0 + min(tid, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(tid, rows - 1)) % a.group;
-	if (warp < 4) {
+	if (warp < WARPS) {
 		const long long at = token * a.q_row + head * a.q_head;
 		const int bytes = a.q_type == SEQ_F32 ? 4 : 2;
 		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * bytes) | (uintptr_t)(a.q_head * bytes)) % 16 == 0;
@@ -719,7 +732,7 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 		}
 		top = warp_max(top);
 		if (lane == 0) s.top[warp] = top;
-		asm volatile("bar.sync 1, 128;" ::: "memory");
+		asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
 		const float down = tid < rows ? pow2f(-ap_exponent(s.top)) : 0.f;
 #pragma unroll 2
 		for (int piece = 0; piece < D / 8; ++piece) {
@@ -727,39 +740,41 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			uint32_t hi[4], rest[4];
 #pragma unroll
 			for (int i = 0; i < 4; ++i) hi[i] = pack_f16(x[2 * i] * down, x[2 * i + 1] * down), rest[i] = SPLIT ? pack_rest(x[2 * i] * down, x[2 * i + 1] * down, hi[i]) : 0;
-			const int place = tid * 128 + (((piece & 7) ^ (tid & 7)) << 4);
-			*reinterpret_cast<uint4*>(s.q[0][piece >> 3] + place) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-			if (SPLIT) *reinterpret_cast<uint4*>(s.q[Shared::PAIR - 1][piece >> 3] + place) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+			const int place = (tid & 127) * 128 + (((piece & 7) ^ (tid & 7)) << 4);
+			*reinterpret_cast<uint4*>(s.q[tid >> 7][0][piece >> 3] + place) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+			if (SPLIT) *reinterpret_cast<uint4*>(s.q[tid >> 7][Shared::PAIR - 1][piece >> 3] + place) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
 		}
 		fence_async_smem();
 	}
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
-	const uint32_t tmem = s.tmem; // scores: columns 0 .. 63 and 64 .. 127; sums from column 128
+	const uint32_t tmem = s.tmem; // scores of even tiles, a group's 64 columns beside another's, of odd ones, sums: 128 columns a group
 	const float qscale = a.scale * pow2f(ap_exponent(s.top)) * AT_LOG2E;
 	float m = -INFINITY, l = 0.f;
 
-	if (warp < 4) {
+	if (warp < WARPS) {
+		const int group = warp / 4;
 		const int rpos = tid < rows ? p0 + (row0 + tid) / a.group : -1, rlow = tid < rows ? at_low(a, rpos) : 0, wide = at_low(a, sp.last);
-		const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-		for (int i = 0; i < tiles; ++i) {
-			const int buf = i & 1;
-			const uint32_t parity = (i >> 1) & 1;
-			if (!ap_wait_warp(s.kv_full + buf, parity, &s.lost) || !ap_wait_warp(s.s_full + buf, parity, &s.lost)) break; // (the factors; the scores)
+		const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), sums_at = lanes + O_COL + 128 * group;
+		int st = 0;
+		uint32_t round = 0;
+		for (int i = 0; i < tiles && group < groups; ++i) {
+			const uint32_t scores_at = lanes + (i & 1) * S_COLS + 64 * group;
+			if (!ap_wait_warp(s.kv_full + st, round, &s.lost) || !ap_wait_warp(s.s_full[group] + (i & 1), (i >> 1) & 1, &s.lost)) break; // (the factors; the scores)
 			tc_fence_after();
 			const int j0 = i * AP_KEYS;
-			const uint32_t seen[2] = {s.seen[buf][0], s.seen[buf][1]};
+			const uint32_t seen[2] = {s.seen[st][0], s.seen[st][1]};
 			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
-			const float bias = s.bias[buf];
+			const float bias = s.bias[st];
 			const float base = m == -INFINITY ? 0.f : m, most = m == -INFINITY ? -INFINITY : AT_MOST;
 			float z[64], top = -INFINITY; // log2 of the weights against the reference as it stands (against 0 before there is one)
-			tmem_ld32(tmem + lanes + buf * 64, *reinterpret_cast<float(*)[32]>(z));
-			tmem_ld32(tmem + lanes + buf * 64 + 32, *reinterpret_cast<float(*)[32]>(z + 32));
+			tmem_ld32(scores_at, *reinterpret_cast<float(*)[32]>(z));
+			tmem_ld32(scores_at + 32, *reinterpret_cast<float(*)[32]>(z + 32));
 			const u64 off = pair_of(bias - base, bias - base);
 #pragma unroll
 			for (int k = 0; k < 64; k += 4) {
-				const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[buf] + k);
+				const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[st] + k);
 				const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), f.x, off)), y = halves(fma2(pair_of(z[k + 2], z[k + 3]), f.y, off));
 				z[k] = x.x, z[k + 1] = x.y, z[k + 2] = y.x, z[k + 3] = y.y;
 			}
@@ -770,18 +785,20 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 					if (!((seen[k / 32] >> (k & 31) & 1) && kp <= rpos && (kp >= rlow || kp < a.keep_first))) z[k] = -INFINITY;
 				}
 			}
+			float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-			for (int k = 0; k < 64; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
+			for (int k = 0; k < 64; k += 2) tops[k / 2 % 4] = fmaxf(fmaxf(tops[k / 2 % 4], z[k]), z[k + 1]);
+			top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 			if (__any_sync(0xffffffffu, top > most)) { // references move
 				const float mn = top > most ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
 #pragma unroll
 				for (int k = 0; k < 64; ++k) z[k] += by;
 				m = mn, l *= f;
 				if (i > 0) { // there are sums
-					if (!ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break;
+					if (!ap_wait_warp(s.p_empty + group, (i - 1) & 1, &s.lost)) break;
 					tc_fence_after();
 #pragma unroll 1
-					for (int col = 0; col < D; col += 8) tmem_scale8(tmem + lanes + 128 + col, f);
+					for (int col = 0; col < D; col += 8) tmem_scale8(sums_at + col, f);
 					tmem_st_wait();
 				}
 			}
@@ -793,17 +810,18 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 				sum = add2(sum, pair_of(w0, w1));
 				hi[k / 2] = pack_f16(w0, w1), rest[k / 2] = SPLIT ? pack_rest(w0, w1, hi[k / 2]) : 0;
 			}
-			tmem_st32(tmem + lanes + buf * 64, hi); // where the scores were
-			if (SPLIT) tmem_st32(tmem + lanes + buf * 64 + 32, rest);
+			tmem_st32(scores_at, hi); // where the scores were
+			if (SPLIT) tmem_st32(scores_at + 32, rest);
 			const float2 sums = halves(sum);
 			l = fmaf(sums.x + sums.y, pow2f(-(int)bias), l); // the weights hold the value scale
 			tmem_st_wait();
-			if (i > 0 && !ap_wait_warp(&s.p_empty, (i - 1) & 1, &s.lost)) break; // (long done: the barrier's phases stay in step)
+			if (i > 0 && !ap_wait_warp(s.p_empty + group, (i - 1) & 1, &s.lost)) break; // (long done: the barrier's phases stay in step)
 			tc_fence_before();
 			__syncwarp();
-			if (lane == 0) mbar_arrive(&s.p_full);
+			if (lane == 0) mbar_arrive(s.p_full + group);
+			if (++st == STAGES) st = 0, round ^= 1;
 		}
-		if (tiles > 0) ap_wait_warp(&s.p_empty, (tiles - 1) & 1, &s.lost);
+		if (tiles > 0 && group < groups) ap_wait_warp(s.p_empty + group, (tiles - 1) & 1, &s.lost);
 		tc_fence_after();
 		float norm = 1.f;
 		if (a.sinks && tid < rows) {
@@ -813,10 +831,10 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 		norm = *(volatile int*)&s.lost ? NAN : l > 0.f ? norm / l : l == 0.f ? 0.f : l; // (0: nothing was seen; a NaN stays one)
 		const bool wide_store = a.out_type != SEQ_F32 && !a.gate && ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
 #pragma unroll 1
-		for (int col = 0; col < D; col += 32) {
+		for (int col = 0; col < D && group < groups; col += 32) {
 			float z[32];
 			__syncwarp(); // (rows behind the last one take part in the load)
-			if (tiles > 0) tmem_ld32(tmem + lanes + 128 + col, z);
+			if (tiles > 0) tmem_ld32(sums_at + col, z);
 			else {
 #pragma unroll
 				for (int k = 0; k < 32; ++k) z[k] = 0.f;
@@ -841,17 +859,17 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 				for (int k = 0; k < 32; ++k) at_finish(a, token, head, col + k, z[k] * norm);
 			}
 		}
-	} else if (warp < 8) {
-		// Every thread takes pieces of keys' rows (PIECES lanes read a row) and eight channels of eight keys' values.
-		constexpr int KROWS = 32 / PIECES, KEACH = AP_KEYS / (4 * KROWS);
-		const int t = tid - 128, group8 = t & 7, dims = (t >> 3) * 8;
+	} else if (warp < 2 * WARPS) {
+		// Every thread takes pieces of keys' rows (PIECES lanes read a row) and eight channels of VKEYS keys' values.
+		constexpr int KROWS = 32 / PIECES, KEACH = AP_KEYS / (WARPS * KROWS), VKEYS = 8 / GROUPS, VGROUPS = AP_KEYS / VKEYS;
+		const int t = tid - 32 * WARPS, own = warp - WARPS, vgroup = t % VGROUPS, dims = t / VGROUPS * 8;
 		const bool works = dims < D;
 		// Nothing below waits for a load where it asks for it: keys that are not there read row 0 of the pool and the table's last entry, and are sorted out a tile later.
 		int ahead[2], exps[2];     // of keys lane and lane + 32: the pages of the tile to load next, as the table has them; the values' scales of the loaded one
 		bool asked[2], have[2];    // whether there was a page to look for; whether the key is there
 		float scale;               // of key t, the keys'
 		uint4 kw[KEACH];
-		uint2 vw[8];
+		uint2 vw[VKEYS];
 		uint32_t mine = 0;         // this thread's values that are there
 		auto look = [&](int i) {
 #pragma unroll
@@ -869,35 +887,36 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 				const int unit = (have[h] ? ahead[h] : 0) * c.heads + kvh;
 				row[h] = have[h] ? unit * c.page + page_row(c, position(i * AP_KEYS + 32 * h + lane)) : -1; // (under 2^31)
 				exps[h] = __float_as_int(__ldg(c.vs + unit));
-				if (h == (warp & 1)) scale = __ldg(c.ks + unit);
+				if (h == (own & 1)) scale = __ldg(c.ks + unit);
 			}
 #pragma unroll
 			for (int k = 0; k < KEACH; ++k) {
-				const int key = (k * 4 + warp - 4) * KROWS + lane / PIECES, r = __shfl_sync(0xffffffffu, (k * 4 + warp - 4) * KROWS < 32 ? row[0] : row[1], key & 31);
+				const int key = (k * WARPS + own) * KROWS + lane / PIECES, r = __shfl_sync(0xffffffffu, (k * WARPS + own) * KROWS < 32 ? row[0] : row[1], key & 31);
 				kw[k] = ldg_stream(reinterpret_cast<const uint4*>(c.k + (long long)max(r, 0) * D) + lane % PIECES);
 			}
 			mine = 0;
 #pragma unroll
-			for (int k = 0; k < 8; ++k) {
-				const int key = group8 * 8 + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
+			for (int k = 0; k < VKEYS; ++k) {
+				const int key = vgroup * VKEYS + k, r0 = __shfl_sync(0xffffffffu, row[0], key & 31), r1 = __shfl_sync(0xffffffffu, row[1], key & 31), r = key < 32 ? r0 : r1;
 				vw[k] = ldg_stream8(reinterpret_cast<const uint2*>(c.v + (long long)max(r, 0) * D + (works ? dims : 0)));
 				mine |= (r >= 0 ? 1u : 0u) << k;
 			}
 			look(i + 1);
 		};
+		int st = 0;
+		uint32_t round = 0;
 		if (tiles > 0) look(0), load(0);
 		for (int i = 0; i < tiles; ++i) {
-			const int st = i & 1;
-			if (!ap_wait_warp(s.kv_empty + st, ((i >> 1) & 1) ^ 1, &s.lost)) break;
+			if (!ap_wait_warp(s.kv_empty + st, round ^ 1, &s.lost)) break;
 			if (t < AP_KEYS) {
-				const bool there = warp == 4 ? have[0] : have[1];
+				const bool there = own == 0 ? have[0] : have[1];
 				s.factor[st][t] = there ? scale * qscale : 0.f;
 				const uint32_t seen = __ballot_sync(0xffffffffu, there);
-				if (lane == 0) s.seen[st][warp - 4] = seen;
+				if (lane == 0) s.seen[st][own] = seen;
 			}
 #pragma unroll
 			for (int k = 0; k < KEACH; ++k) {
-				const int key = (k * 4 + warp - 4) * KROWS + lane / PIECES, piece = lane % PIECES;
+				const int key = (k * WARPS + own) * KROWS + lane / PIECES, piece = lane % PIECES;
 				uint32_t w[8];
 				e4m3x4_to_f16(kw[k].x, w[0], w[1]), e4m3x4_to_f16(kw[k].y, w[2], w[3]), e4m3x4_to_f16(kw[k].z, w[4], w[5]), e4m3x4_to_f16(kw[k].w, w[6], w[7]);
 				unsigned char* const to = s.k[st][piece >> 2] + key * 128;
@@ -915,19 +934,19 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 			if (most == C8_NONE) most = 0;
 			if (t == 0) s.bias[st] = (float)most;
 			const bool even = __all_sync(0xffffffffu, (e[0] == most || e[0] == C8_NONE) && (e[1] == most || e[1] == C8_NONE));
-			if (mine != 0xff) { // (a code that is no number would spoil rows that do not see it)
+			if (mine != (1u << VKEYS) - 1) { // (a code that is no number would spoil rows that do not see it)
 #pragma unroll
-				for (int k = 0; k < 8; ++k)
+				for (int k = 0; k < VKEYS; ++k)
 					if (!(mine >> k & 1)) vw[k] = make_uint2(0, 0);
 			}
-			uint32_t down[4]; // of the pairs of this thread's keys, as fp16
+			uint32_t down[VKEYS / 2]; // of the pairs of this thread's keys, as fp16
 			if (!even) {
 #pragma unroll
-				for (int k = 0; k < 4; ++k) {
+				for (int k = 0; k < VKEYS / 2; ++k) {
 					float f[2];
 #pragma unroll
 					for (int u = 0; u < 2; ++u) {
-						const int key = group8 * 8 + 2 * k + u, e0 = __shfl_sync(0xffffffffu, e[0], key & 31), e1 = __shfl_sync(0xffffffffu, e[1], key & 31);
+						const int key = vgroup * VKEYS + 2 * k + u, e0 = __shfl_sync(0xffffffffu, e[0], key & 31), e1 = __shfl_sync(0xffffffffu, e[1], key & 31);
 						f[u] = pow2f(max((key < 32 ? e0 : e1) - most, -126));
 					}
 					down[k] = pack_f16(f[0], f[1]);
@@ -938,51 +957,64 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 				for (int word = 0; word < 2; ++word)
 #pragma unroll
 					for (int u = 0; u < 2; ++u) { // channels dims + 4 word + 2 u, + 1
-						uint32_t lo[4], hi[4];
+						uint32_t lo[VKEYS / 2], hi[VKEYS / 2];
 #pragma unroll
-						for (int k = 0; k < 4; ++k) {
+						for (int k = 0; k < VKEYS / 2; ++k) {
 							const uint32_t x = word ? vw[2 * k].y : vw[2 * k].x, y = word ? vw[2 * k + 1].y : vw[2 * k + 1].x;
 							e4m3x4_to_f16(__byte_perm(x, y, u ? 0x7362 : 0x5140), lo[k], hi[k]);
 							if (!even) lo[k] = mul_f16(lo[k], down[k]), hi[k] = mul_f16(hi[k], down[k]);
 						}
 						const int d = dims + 4 * word + 2 * u;
-						*reinterpret_cast<uint4*>(s.v[st] + d * 128 + ((group8 ^ (d & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-						*reinterpret_cast<uint4*>(s.v[st] + (d + 1) * 128 + ((group8 ^ ((d + 1) & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+						auto put = [&](int d, const uint32_t (&w)[VKEYS / 2]) {
+							unsigned char* const to = s.v[st] + d * 128 + (((vgroup * VKEYS / 8) ^ (d & 7)) << 4) + vgroup * VKEYS % 8 * 2;
+							if constexpr (VKEYS == 8) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+							else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+						};
+						put(d, lo), put(d + 1, hi);
 					}
 			}
 			fence_async_smem();
 			__syncwarp();
 			if (lane == 0) mbar_arrive(s.kv_full + st);
 			if (i + 1 < tiles) load(i + 1);
+			if (++st == STAGES) st = 0, round ^= 1;
 		}
 	} else if (lane == 0) {
-		constexpr uint32_t score = (1u << 4) | ((uint32_t)(AP_KEYS >> 3) << 17) | ((uint32_t)(AP_ROWS >> 4) << 24), value = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(AP_ROWS >> 4) << 24);
-		for (int i = 0; i <= tiles && tiles > 0; ++i) {
+		constexpr uint32_t score = (1u << 4) | ((uint32_t)(AP_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows
+		int st = 0, behind = 0; // stages of this tile's keys, of the values of the one before
+		uint32_t round = 0;
+		bool there = true;
+		for (int i = 0; i <= tiles && tiles > 0 && there; ++i) {
 			if (i < tiles) {
-				const int buf = i & 1;
-				const uint32_t parity = (i >> 1) & 1;
-				if (!ap_wait(s.kv_full + buf, parity, &s.lost)) break; // (the scores' columns: the product of the tile before the last, which read weights there, was issued earlier)
+				if (!ap_wait(s.kv_full + st, round, &s.lost)) break; // (the scores' columns: the product of the tile before the last, which read weights there, was issued earlier)
 				tc_fence_after();
+				for (int g = 0; g < groups; ++g) {
 #pragma unroll
-				for (int h = 0; h < Shared::PAIR; ++h)
+					for (int h = 0; h < Shared::PAIR; ++h)
 #pragma unroll
-					for (int pn = 0; pn < PANELS; ++pn)
+						for (int pn = 0; pn < PANELS; ++pn)
 #pragma unroll
-						for (int k = 0; k < 4; ++k)
-							umma_f16(tmem + buf * 64, umma_desc_sw128(s.q[h][pn]) + 2 * k, umma_desc_sw128(s.k[buf][pn]) + 2 * k, score, (h | pn | k) ? 1u : 0u);
-				umma_commit(s.s_full + buf);
+							for (int k = 0; k < 4; ++k)
+								umma_f16(tmem + (i & 1) * S_COLS + 64 * g, umma_desc_sw128(s.q[g][h][pn]) + 2 * k, umma_desc_sw128(s.k[st][pn]) + 2 * k, score, (h | pn | k) ? 1u : 0u);
+					umma_commit(s.s_full[g] + (i & 1));
+				}
 			}
 			if (i > 0) {
 				const int j = i - 1;
-				if (!ap_wait(&s.p_full, j & 1, &s.lost)) break;
-				tc_fence_after();
+				for (int g = 0; g < groups; ++g) {
+					if (!(there = ap_wait(s.p_full + g, j & 1, &s.lost))) break;
+					tc_fence_after();
 #pragma unroll
-				for (int h = 0; h < Shared::PAIR; ++h)
+					for (int h = 0; h < Shared::PAIR; ++h)
 #pragma unroll
-					for (int k = 0; k < 4; ++k) umma_f16_ts(tmem + 128, tmem + (j & 1) * 64 + 32 * h + 8 * k, umma_desc_sw128(s.v[j & 1]) + 2 * k, value, (j | h | k) ? 1u : 0u);
-				umma_commit(s.kv_empty + (j & 1));
-				umma_commit(&s.p_empty);
+						for (int k = 0; k < 4; ++k)
+							umma_f16_ts(tmem + O_COL + 128 * g, tmem + (j & 1) * S_COLS + 64 * g + 32 * h + 8 * k, umma_desc_sw128(s.v[behind]) + 2 * k, value, (j | h | k) ? 1u : 0u);
+					umma_commit(s.p_empty + g);
+				}
+				umma_commit(s.kv_empty + behind);
 			}
+			behind = st;
+			if (++st == STAGES) st = 0, round ^= 1;
 		}
 		umma_commit(&s.done); // nothing of this block's is left in the tensor core when its memory goes
 		mbar_wait_bounded(&s.done, 0);
@@ -991,10 +1023,10 @@ __global__ void __launch_bounds__(AP_THREADS, SPLIT ? 1 : 2) k_c8_prompt(const C
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
-	if (warp == 8) tmem_dealloc(tmem, 256);
+	if (warp == 2 * WARPS) tmem_dealloc(tmem, 256 * GROUPS);
 }
 
-// Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.
+// Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.  9 us for 2048 rows of 6 shares: latency, launched while the shares still run.
 __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	pdl_wait_prev();
 	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1075,19 +1107,23 @@ struct AtPlan {
 	int tile, shares, each, cluster; // tile 128: the prompt kernel
 };
 constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
-constexpr int AP_CTAS = 64;      // of the prompt kernel, from which on it is the faster one: 32 CTAs 47 us and 31 with the other, 75 43 and 50, 80 46 and 48, 256 54 and 131
+constexpr int AP_TILE = 128;     // stands for the prompt kernel
+// 128s of rows from which on the prompt kernel is the faster one (us, and with the other).  Its time is that of a CTA's tiles one after another, whatever the channels; the other's
+// work halves with them.  128 channels, 16 bits: 32 46 / 31 and 48 / 46, 48 47 / 46, 64 42 / 61, 80 48 / 58, 128 41 / 101, 256 44 / 133; fp32 80 44 / 48.
+// 64 channels, 16 bits: 64 72 / 48, 128 27 / 39; fp32 88 30 / 40.
+constexpr int ap_least(bool split, int dim) { return split || dim > 64 ? 64 : 96; }
 // Rows of a CTA: eight fill a product; more, where a sequence has more, read and convert the codes once for all of them, as far as registers hold their sums and CTAs are enough
 // for the GPU all the same.
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const long long rows = (long long)p.longest * (a.heads / c.heads);
 	auto ctas = [&](int tile) { return (long long)p.n * cdiv(rows, tile) * c.heads; };
-	if (rows >= AP_ROWS / 2 && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(AP_ROWS) >= AP_CTAS) return AP_ROWS;
+	if (rows >= 64 && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(128) >= ap_least(a.q.type == SEQ_F32, c.dim)) return AP_TILE;
 	if (rows > 16 && c.dim <= 128 && ctas(32) >= AT_ROOM) return 32;
 	return rows > 8 && ctas(16) >= AT_ROOM / 2 ? 16 : 8;
 }
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const int group = a.heads / c.heads, tile = attend_tile(c, p, a);
-	if (tile == AP_ROWS) return AtPlan{tile, 1, cdiv(std::max(a.most_keys, 1), AT_KEYS), 0};
+	if (tile == AP_TILE) return AtPlan{tile, 1, cdiv(std::max(a.most_keys, 1), AT_KEYS), 0};
 	const long long ctas = (long long)p.n * cdiv((long long)p.longest * group, tile) * c.heads, room = AT_ROOM;
 	long long keys = std::max(a.most_keys, 1);
 	if (a.window > 0) keys = std::min(keys, (long long)a.window + a.keep_first + tile / group);
@@ -1130,14 +1166,14 @@ template <int D, bool SPLIT>
 cudaError_t prompt_launch(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	static std::atomic<uint64_t> done{0};
 	cudaError_t e = allow(k_c8_prompt<D, SPLIT>, sizeof(ApShared<D, SPLIT>), done);
-	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_prompt<D, SPLIT>, dim3(grid.y, grid.z, grid.x), dim3(AP_THREADS), sizeof(ApShared<D, SPLIT>), c, a);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c8_prompt<D, SPLIT>, dim3(grid.y, grid.z, cdiv(grid.x, ap_groups(SPLIT))), dim3(ap_threads(SPLIT)), sizeof(ApShared<D, SPLIT>), c, a);
 	return e;
 }
 template <int D>
 cudaError_t attend_wide(const C8& c, const Attend& a, dim3 grid, cudaStream_t st) {
 	const bool split = a.q_type == SEQ_F32;
 	if constexpr (D < 256)
-		if (a.tile == AP_ROWS) return split ? prompt_launch<D, true>(c, a, grid, st) : prompt_launch<D, false>(c, a, grid, st);
+		if (a.tile == AP_TILE) return split ? prompt_launch<D, true>(c, a, grid, st) : prompt_launch<D, false>(c, a, grid, st);
 	if (a.tile == 8) return split ? attend_launch<D, true, 1>(c, a, grid, st) : attend_launch<D, false, 1>(c, a, grid, st);
 	if (D == 256 || a.tile == 16) return split ? attend_launch<D, true, 2>(c, a, grid, st) : attend_launch<D, false, 2>(c, a, grid, st);
 	constexpr int DD = D == 256 ? 128 : D; // (rows of 256 channels come in sixteens)
