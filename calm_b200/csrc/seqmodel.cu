@@ -4,6 +4,7 @@
 
 #include "../../include/calm_b200_seq.h"
 
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 
@@ -11,6 +12,7 @@
 #include <array>
 #include <functional>
 #include <map>
+#include <new>
 #include <type_traits>
 #include <vector>
 
@@ -1614,6 +1616,13 @@ extern "C" int calm_b200_seq_skinny_warps(int m, int k, int groups, int rows, in
 extern "C" int calm_b200_seq_delta_blocks_pay(int longest, int few, int heads, int vdim, int sms) { return delta_blocks_pay(longest, few, heads, vdim, sms); }
 extern "C" int calm_b200_seq_pairs_pay(int rows, int tokens, int k, int epi, int pairs) { return tg_pairs_pay(rows, tokens, k, epi, pairs); }
 
+// whether the operators over 8-bit caches take pools of so many pages
+static bool cache8_holds(const Seq& s, int pages) {
+	auto one = [&](const SeqLayer& L) { return !L.cache8 || (s.m.page <= 65536 && (long long)pages * L.kv_heads * s.m.page <= INT_MAX); };
+	for (const SeqLayer& L : s.layers)
+		if (L.type == SEQ_PAIR ? !one(L.pair[0]) || !one(L.pair[1]) : !one(L)) return false;
+	return true;
+}
 extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 	int count = 0;
 	if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) CALM_FATAL("no CUDA device available; this backend has no CPU fallback");
@@ -1662,6 +1671,7 @@ extern "C" void* calm_b200_seq_prepare(const struct SeqModel* model) {
 
 	// pages: every live token, one partly filled page per sequence
 	s.n_pages = cdiv(m.max_tokens, m.page) + m.max_seqs;
+	if (!cache8_holds(s, s.n_pages)) CALM_FATAL("seq: an 8-bit cache of %d pages of %d tokens: a layer holds at most 2^31 rows in pages of at most 65536", s.n_pages, m.page);
 	s.max_pages = s.n_pages;
 	for (int p = s.n_pages - 1; p >= 0; --p) s.free_pages.push_back(p);
 	s.page_refs.assign(s.n_pages, 0);
@@ -1902,7 +1912,8 @@ static void each_state(Seq& s, F&& f) {
 extern "C" int calm_b200_seq_branch(void* handle, int n_from, const int* from_slots, int n_to, const int* from_parents, int* out_slots) {
 	Seq& s = *(Seq*)handle;
 	const int page = s.m.page, S = (int)s.slots.size();
-	if (n_from < 1 || n_to < 0 || !from_slots || (n_to && (!from_parents || !out_slots))) return -3;
+	if (n_from < 1 || n_from > S || n_to < 0 || !from_slots || (n_to && (!from_parents || !out_slots))) return -3;
+	if (n_to > S) return -1;
 	const std::vector<int> slots(from_slots, from_slots + n_from), parents(from_parents, from_parents + n_to); // (the result may go where they came from)
 	std::vector<int> kids(n_from, 0);
 	std::vector<char> named(S, 0);
@@ -1974,6 +1985,13 @@ extern "C" int calm_b200_seq_resize(void* handle, int max_tokens) {
 	Seq& s = *(Seq*)handle;
 	if (max_tokens < 1 || (long long)max_tokens + (long long)s.m.max_seqs * s.m.page > 0x7fffffff) return -3;
 	const int pages = cdiv(max_tokens, s.m.page) + s.m.max_seqs;
+	if (!cache8_holds(s, pages)) return -3;
+	std::vector<int> table, refs;
+	try {
+		table.assign((size_t)s.m.max_seqs * pages, 0), refs.assign(pages, 0);
+	} catch (const std::bad_alloc&) {
+		return -4;
+	}
 	std::vector<int> from, to, place(s.n_pages, -1); // live pages, in order, go to the front
 	for (int p = 0; p < s.n_pages; ++p)
 		if (s.page_refs[p] > 0) place[p] = (int)from.size(), from.push_back(p), to.push_back(place[p]);
@@ -2001,7 +2019,6 @@ extern "C" int calm_b200_seq_resize(void* handle, int max_tokens) {
 		return -4;
 	}
 	if (calm_b200_seq_copy_units((int)pools.size(), pools.data(), live, from.data(), to.data(), nullptr, 0, nullptr, nullptr, s.stream) != 0) CALM_FATAL("seq: %s", calm_b200_seq_error());
-	std::vector<int> table((size_t)s.m.max_seqs * pages, 0), refs(pages, 0);
 	for (int i = 0; i < (int)s.slots.size(); ++i) {
 		Slot& sl = s.slots[i];
 		for (size_t k = 0; k < sl.pages.size(); ++k) sl.pages[k] = place[sl.pages[k]], table[(size_t)i * pages + k] = sl.pages[k];

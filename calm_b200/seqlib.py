@@ -220,7 +220,7 @@ class SeqDeviceModel:
         """A cache for max_tokens live tokens from now on, smaller or larger; live sequences keep theirs."""
         rc = self.lib.calm_b200_seq_resize(self.handle, int(max_tokens))
         if rc != 0:
-            raise SeqError({-2: f"the live sequences hold more than {max_tokens} tokens", -4: "the device lacks the memory"}.get(rc, "max_tokens must be positive"))
+            raise SeqError({-2: f"the live sequences hold more than {max_tokens} tokens", -4: "the device lacks the memory"}.get(rc, "max_tokens must be positive and within what the caches can hold"))
         self.desc.max_tokens = int(max_tokens)
 
     # ---- the step function

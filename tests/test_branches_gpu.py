@@ -150,6 +150,22 @@ def test_refused_branches_and_sizes_change_nothing():
         assert m.branch([a, b, 3], []) == [] and m.free_pages() == 14
 
 
+def test_more_branches_than_slots_and_pools_past_an_operators_range_are_refused():
+    with build("bovinex", max_tokens=40, max_seqs=4, cache_bits=8) as m:
+        a = m.open()
+        m.step([a], [text(20, 1)], [])
+        with pytest.raises(seqlib.SeqError, match="slot"):
+            m.branch([a], [0] * 1000)
+        with pytest.raises(seqlib.SeqError, match="bad branch"):
+            m.branch([a] * 1000, [0])
+        with pytest.raises(seqlib.SeqError):  # more rows than the operators over 8-bit caches take
+            m.resize(2 ** 31 - 200)
+        with build("bovinex", max_tokens=40, max_seqs=4, cache_bits=8) as twin:
+            x = twin.open()
+            twin.step([x], [text(20, 1)], [])
+            assert np.array_equal(m.step([a], [[7]], [0]), twin.step([x], [[7]], [0]))
+
+
 def test_a_pool_made_smaller_gives_memory_back():
     with build("bovinex", max_tokens=400000, page=16) as m:
         s = m.open()
