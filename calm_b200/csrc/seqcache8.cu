@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 // a warp's chunk (1.7 warp instructions a cycle; 49 million in all), with few the latency of copy, products, softmax and the cluster's fold.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
 constexpr int AT_SHARES = 64;  // of a tile's keys at most
-constexpr int AT_CLUSTER_ROWS = 16, AT_CLUSTER = 16; // shares that a thread-block cluster folds: of tiles of 16 rows at most, as many
+constexpr int AT_TILE = 16, AT_CLUSTER = 16; // rows of a CTA at most; shares that a thread-block cluster folds at most
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr int AT_LIFT = 15;                // the largest query of a tile stands at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of it
 constexpr float AT_MOST = 15.f, AT_SET = 10.f; // weights: at most 2^15, the largest at 2^10 or more
@@ -165,7 +165,7 @@ struct AtStage { // a warp's chunk: the next one's keys come while its values ar
 };
 template <int D>
 __host__ __device__ constexpr size_t at_ring() { // (the sums of the warps take its place)
-	const size_t a = (size_t)AT_WARPS * sizeof(AtStage<D>), b = (size_t)AT_WARPS * 8 * (8 * (D == 256 ? 52 : 20) + 4) * sizeof(float) + (size_t)AT_CLUSTER_ROWS * (D + 2) * sizeof(float);
+	const size_t a = (size_t)AT_WARPS * sizeof(AtStage<D>), b = (size_t)AT_WARPS * 8 * (8 * (D == 256 ? 52 : 20) + 4) * sizeof(float) + (size_t)AT_TILE * (D + 2) * sizeof(float);
 	return a > b ? a : b;
 }
 template <int D, bool SPLIT, int NQ>
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	}
 	if (whole || !a.cluster) return;
 	// A cluster's shares: each CTA finishes its part of the outputs from all of them.
-	__shared__ float wz[AT_CLUSTER][AT_CLUSTER_ROWS], inv[AT_CLUSTER_ROWS];
+	__shared__ float wz[AT_CLUSTER][AT_TILE], inv[AT_TILE];
 	const int shares = min(a.shares, (sp.chunks + a.each - 1) / a.each);
 	cluster_sync();
 	if (tid < rows) {
@@ -1112,14 +1112,14 @@ constexpr int AP_TILE = 128;     // stands for the prompt kernel
 // work halves with them.  128 channels, 16 bits: 32 46 / 31 and 48 / 46, 48 47 / 46, 64 42 / 61, 80 48 / 58, 128 41 / 101, 256 44 / 133; fp32 80 44 / 48.
 // 64 channels, 16 bits: 64 72 / 48, 128 27 / 39; fp32 88 30 / 40.
 constexpr int ap_least(bool split, int dim) { return split || dim > 64 ? 64 : 96; }
-// Rows of a CTA: eight fill a product; more, where a sequence has more, read and convert the codes once for all of them, as far as registers hold their sums and CTAs are enough
-// for the GPU all the same.
+// Rows of a CTA: eight fill a product; sixteen read and convert the codes once for all of them, with fewer CTAs an SM.  They pay with many rows a sequence (us with 8 and 16 rows:
+// 6000 rows of 80 channels 237 / 176, of 256 438 / 339; 16 and 32 rows, 64 sequences: 60 / 69 and 94 / 108), with 64 channels (64 sequences of 63 rows 46 / 43), and where
+// they bring the CTAs down to what clusters serve (1600 rows 31 / 23, 16 sequences of 16 rows 24 / 21); not where CTAs are few (80 of 8 rows 16.5 / 17.4).
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const long long rows = (long long)p.longest * (a.heads / c.heads);
 	auto ctas = [&](int tile) { return (long long)p.n * cdiv(rows, tile) * c.heads; };
 	if (rows >= 64 && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(128) >= ap_least(a.q.type == SEQ_F32, c.dim)) return AP_TILE;
-	if (rows > 16 && c.dim <= 128 && ctas(32) >= AT_ROOM) return 32;
-	return rows > 8 && ctas(16) >= AT_ROOM / 2 ? 16 : 8;
+	return rows > 8 && ctas(8) > AT_ROOM / 2 && (rows >= 64 || c.dim <= 64 || ctas(16) <= AT_ROOM / 2) ? 16 : 8;
 }
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const int group = a.heads / c.heads, tile = attend_tile(c, p, a);
@@ -1133,8 +1133,8 @@ AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a
 	// many CTAs: several rounds, so that the last one is short
 	long long shares = ctas >= 6 * room ? 1 : ctas > room / 2 ? cdiv(6 * room, ctas) : room / ctas;
 	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, ctas > room / 2 ? 2 * AT_WARPS : AT_WARPS), (long long)AT_SHARES}));
-	// one round: a cluster folds them, and the fold's launch is saved
-	const bool cluster = shares > 1 && ctas <= room / 2 && tile <= AT_CLUSTER_ROWS;
+	// one round: a cluster folds them, and the fold's launch is saved (one token over 4000 keys 11.0 us and 32.2 without, four 14.1 and 21.9)
+	const bool cluster = shares > 1 && ctas <= room / 2;
 	if (cluster) shares = shares >= 16 ? 16 : shares >= 8 ? 8 : shares >= 4 ? 4 : 2;
 	const int each = cdiv(chunks, shares);
 	return AtPlan{tile, cluster ? (int)shares : cdiv(chunks, each), each, cluster};
@@ -1175,9 +1175,7 @@ cudaError_t attend_wide(const C8& c, const Attend& a, dim3 grid, cudaStream_t st
 	if constexpr (D < 256)
 		if (a.tile == AP_TILE) return split ? prompt_launch<D, true>(c, a, grid, st) : prompt_launch<D, false>(c, a, grid, st);
 	if (a.tile == 8) return split ? attend_launch<D, true, 1>(c, a, grid, st) : attend_launch<D, false, 1>(c, a, grid, st);
-	if (D == 256 || a.tile == 16) return split ? attend_launch<D, true, 2>(c, a, grid, st) : attend_launch<D, false, 2>(c, a, grid, st);
-	constexpr int DD = D == 256 ? 128 : D; // (rows of 256 channels come in sixteens)
-	return split ? attend_launch<DD, true, 4>(c, a, grid, st) : attend_launch<DD, false, 4>(c, a, grid, st);
+	return split ? attend_launch<D, true, 2>(c, a, grid, st) : attend_launch<D, false, 2>(c, a, grid, st);
 }
 } // namespace
 
