@@ -1109,8 +1109,8 @@ struct AtPlan {
 constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
 constexpr int AP_TILE = 128;     // stands for the prompt kernel
 // 128s of rows from which on the prompt kernel is the faster one (us, and with the other).  Its time is that of a CTA's tiles one after another, whatever the channels; the other's
-// work halves with them.  128 channels, 16 bits: 32 46 / 31 and 48 / 46, 48 47 / 46, 64 42 / 61, 80 48 / 58, 128 41 / 101, 256 44 / 133; fp32 80 44 / 48.
-// 64 channels, 16 bits: 64 72 / 48, 128 27 / 39; fp32 88 30 / 40.
+// work halves with them.  128 channels, 16 bits: 32 46 / 31 and 48 / 46, 48 47 / 46, 64 42 / 61, 80 48 / 58, 128 41 / 79, 256 44 / 90; fp32 80 43 / 48.
+// 64 channels, 16 bits: 64 72 / 48, 128 27 / 39; fp32 88 28 / 40.
 constexpr int ap_least(bool split, int dim) { return split || dim > 64 ? 64 : 96; }
 // Rows of a CTA: eight fill a product; sixteen read and convert the codes once for all of them, with fewer CTAs an SM.  They pay with many rows a sequence (us with 8 and 16 rows:
 // 6000 rows of 80 channels 237 / 176, of 256 438 / 339; 16 and 32 rows, 64 sequences: 60 / 69 and 94 / 108), with 64 channels (64 sequences of 63 rows 46 / 43), and where
@@ -1130,7 +1130,7 @@ AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a
 	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + tile / group);
 	const int chunks = cdiv(keys, AT_KEYS);
 	if (ctas < 1) return AtPlan{tile, 1, chunks, 0};
-	// many CTAs: several rounds, so that the last one is short
+	// many CTAs: several rounds, so that the last one is short (64 tokens over 2000 to 8000 keys: two rounds 140 us, six 126, eight 126, twelve 139)
 	long long shares = ctas >= 6 * room ? 1 : ctas > room / 2 ? cdiv(6 * room, ctas) : room / ctas;
 	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, ctas > room / 2 ? 2 * AT_WARPS : AT_WARPS), (long long)AT_SHARES}));
 	// one round: a cluster folds them, and the fold's launch is saved (one token over 4000 keys 11.0 us and 32.2 without, four 14.1 and 21.9)
