@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(BM_THREADS, 4) k_beam_slice(const BeamArgs a) 
 	pdl_launch_next();
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, slice = blockIdx.x, row = blockIdx.y, n = a.n;
 	u64* const out = a.keys + ((size_t)row * a.slices + slice) * n;
-	if (!(a.scores[row] > -INFINITY)) { // this beam is not there
+	if (!(fabsf(a.scores[row]) < INFINITY)) { // this beam is not there
 		for (int i = tid; i < n; i += BM_THREADS) out[i] = 0;
 		if (tid == 0) a.sums[(size_t)row * a.slices + slice] = make_float2(-INFINITY, 0.f);
 		return;

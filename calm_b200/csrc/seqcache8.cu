@@ -20,7 +20,7 @@ struct C8 {
 	int pages, heads, page, dim, slots, table_pages;
 	int page_shift; // log2 of page, -1: no power of two
 	const int *start, *count, *slot, *pos0;
-	__device__ __forceinline__ bool known(int slot) const { return (unsigned)slot < (unsigned)slots && pages > 0 && table_pages > 0; } // something may be there
+	__device__ __forceinline__ int reach(int slot) const { return (unsigned)slot < (unsigned)slots && pages > 0 ? (int)min((long long)table_pages * page, INT_MAX - 128LL) : 0; } // positions that the table has
 };
 constexpr int C8_LEAST = -64; // exponent of the smallest scale
 
@@ -51,8 +51,8 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t codes) {
 
 // ---------------------------------------------------------------- storing
 // A warp takes one page of a sequence's new rows, one head, keys or values: the largest finite value, the scale, the codes of earlier rows where the scale grew, the codes
-// of the new rows.  Pages are independent, so a prompt's run side by side.  Bound: memory for prompts (rows read once from DRAM, once more from L1: 3990 rows of 8 heads of 128
-// fp32 channels 11.2 us, 4.6 TB/s), latency for single tokens (32 of them 2.8 us: the page's number, its scale, its rows one after another).
+// of the new rows.  Pages are independent, so a prompt's run side by side.  Bound: memory for prompts (rows read once from DRAM, once more from L1: 4955 rows of 8 heads of 128
+// fp32 channels 11.2 us, 4.5 TB/s), latency for single tokens (32 of them 2.8 us: the page's number, its scale, its rows one after another).
 constexpr int ST_WARPS = 4;
 struct StoreRows {
 	const void* p;
@@ -80,8 +80,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 	const int h = isv ? unit - c.heads : unit, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b];
 	const StoreRows& r = isv ? rv : rk;
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || (unsigned)slot >= (unsigned)c.slots || start < 0 || n > r.rows - start) return;
-	const int block = p0 / c.page + blockIdx.x;
-	const long long page0 = (long long)block * c.page;
+	const long long block = p0 / c.page + (long long)blockIdx.x, page0 = block * c.page;
 	if (block >= c.table_pages || page0 >= (long long)p0 + n) return;
 	const int id = c.table[(size_t)slot * c.table_pages + block];
 	if ((unsigned)id >= (unsigned)c.pages) return;
@@ -219,11 +218,11 @@ __device__ __forceinline__ int at_low(const Attend& a, int pos) {
 	int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
 	return a.chunk > 0 ? max(lo, pos / a.chunk * a.chunk) : lo;
 }
-__device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int rows, bool known) {
+__device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int rows, int reach) {
 	AtSpan s;
 	s.first = p0 + row0 / a.group, s.last = p0 + (row0 + rows - 1) / a.group;
-	s.lo = at_low(a, s.first), s.kept = min(a.keep_first, s.lo);
-	s.total = known ? s.kept + s.last - s.lo + 1 : 0;
+	s.lo = at_low(a, s.first), s.kept = min(min(a.keep_first, s.lo), reach);
+	s.total = s.kept + max(min(s.last, reach - 1) - s.lo + 1, 0); // (no walk over positions that the table does not have)
 	s.chunks = (s.total + AT_KEYS - 1) / AT_KEYS;
 	return s;
 }
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * (8 * NQ) >= (long long)n * a.group) return;
 	const int row0 = tile * (8 * NQ), rows = (int)min((long long)(8 * NQ), (long long)n * a.group - row0);
-	const AtSpan sp = at_span(a, p0, row0, rows, c.known(slot));
+	const AtSpan sp = at_span(a, p0, row0, rows, c.reach(slot));
 	const int lo = sp.lo, kept = sp.kept, total = sp.total;
 	const int begin = min(sp.chunks, share * a.each), end = share == a.shares - 1 ? sp.chunks : min(sp.chunks, begin + a.each); // (more keys than were planned for: the last share's)
 	if (share > 0 && begin >= sp.chunks && !a.cluster) return; // (a cluster stays together)
@@ -612,9 +611,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // the weights (exponents, references and denominators as above) and write them back where the scores stood: the next product's operand.  O stays in tensor memory; it is rescaled
 // in the rare case that a row's reference moves.
 //   warps, in fours: softmax and output of each group; keys and values; a warp for the products
-// 1500 and 700 queries of 16 heads behind 700 and 300 keys of 128 channels: 77 us (one group a CTA and two CTAs an SM 86, with the weights through shared memory 95).  Bound: the way of a tile
+// 1500 and 805 queries of 16 heads behind 700 and 376 keys of 128 channels, 148 CTAs: 76 us (one group a CTA and two CTAs an SM 86, with the weights through shared memory 95).  Bound: the way of a tile
 // through its roles, about 3900 cycles, of which a softmax warp works 3000 (its exponentials keep the units busy for 1024 of them, the tensor cores are for about 1300); registers
-// hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86), registers moved from them to the softmax 76.
+// hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86).
 constexpr int AP_KEYS = 64, C8_NONE = -1000;
 constexpr int ap_groups(bool split) { return split ? 1 : 2; } // of 128 rows
 constexpr int ap_threads(bool split) { return 256 * ap_groups(split) + 32; }
@@ -704,7 +703,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 	const int tile = (int)min((long long)gridDim.z, ((long long)n * a.group + ROWS - 1) / ROWS) - 1 - (int)blockIdx.z; // (every sequence's longest rows first)
 	if (tile < 0 || n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || (long long)tile * ROWS >= (long long)n * a.group) return;
 	const int row0 = tile * ROWS, rows = (int)min((long long)ROWS, (long long)n * a.group - row0);
-	const AtSpan sp = at_span(a, p0, row0, rows, c.known(slot));
+	const AtSpan sp = at_span(a, p0, row0, rows, c.reach(slot));
 	const int tiles = (sp.total + AP_KEYS - 1) / AP_KEYS;
 	auto position = [&](int j) { return j < sp.kept ? j : sp.lo + (j - sp.kept); };
 
@@ -753,7 +752,9 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 	const float qscale = a.scale * pow2f(ap_exponent(s.top)) * AT_LOG2E;
 	float m = -INFINITY, l = 0.f;
 
+	// registers go from the warps of keys and values to those of the softmax: 8 x 112 + 8 x 80 + 96 = 17 x 96, what the block was launched with
 	if (warp < WARPS) {
+		if (!SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
 		const int group = warp / 4;
 		const int rpos = tid < rows ? p0 + (row0 + tid) / a.group : -1, rlow = tid < rows ? at_low(a, rpos) : 0, wide = at_low(a, sp.last);
 		const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), sums_at = lanes + O_COL + 128 * group;
@@ -860,6 +861,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			}
 		}
 	} else if (warp < 2 * WARPS) {
+		if (!SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 		// Every thread takes pieces of keys' rows (PIECES lanes read a row) and eight channels of VKEYS keys' values.
 		constexpr int KROWS = 32 / PIECES, KEACH = AP_KEYS / (WARPS * KROWS), VKEYS = 8 / GROUPS, VGROUPS = AP_KEYS / VKEYS;
 		const int t = tid - 32 * WARPS, own = warp - WARPS, vgroup = t % VGROUPS, dims = t / VGROUPS * 8;
@@ -1033,7 +1035,7 @@ __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start) return;
 	for (long long row = (long long)blockIdx.x * 4 + warp; row < (long long)n * a.group; row += gridDim.x * 4) {
 		const int row0 = (int)(row / a.tile) * a.tile, rows = (int)min((long long)a.tile, (long long)n * a.group - row0);
-		const int shares = min(a.shares, (at_span(a, p0, row0, rows, c.known(slot)).chunks + a.each - 1) / a.each);
+		const int shares = min(a.shares, (at_span(a, p0, row0, rows, c.reach(slot)).chunks + a.each - 1) / a.each);
 		if (shares <= 1) continue; // its one share has finished it
 		const int token = start + (int)(row / a.group), head = kvh * a.group + (int)(row % a.group), stride = c.dim + 2;
 		const float* p = a.part + ((size_t)token * a.heads + head) * a.shares * stride;
@@ -1109,16 +1111,17 @@ struct AtPlan {
 constexpr int AT_ROOM = 148 * 3; // CTAs that run at a time
 constexpr int AP_TILE = 128;     // stands for the prompt kernel
 // 128s of rows from which on the prompt kernel is the faster one (us, and with the other).  Its time is that of a CTA's tiles one after another, whatever the channels; the other's
-// work halves with them.  128 channels, 16 bits: 32 46 / 31 and 48 / 46, 48 47 / 46, 64 42 / 61, 80 48 / 58, 128 41 / 79, 256 44 / 90; fp32 80 43 / 48.
-// 64 channels, 16 bits: 64 72 / 48, 128 27 / 39; fp32 88 28 / 40.
-constexpr int ap_least(bool split, int dim) { return split || dim > 64 ? 64 : 96; }
+// work halves with them.  128 channels, 16 bits: 32 46 / 24, 64 42 / 44, 80 21 / 29 and 47 / 30, 100 35 / 41 and 93 / 107, 104 35 / 35, 128 40 / 60 and 31 / 36, 256 43 / 55, 376 76 / 167.
+// 64 channels: 64 72 / 33, 128 26 / 18, 200 49 / 66, 224 30 / 33, 256 27 / 31 and 83 / 138.  fp32 (a group of rows a CTA): 80 43 / 34, 104 44 / 38, 128 52 / 67, 224 47 / 37 and
+// 74 / 63, 384 52 / 76.
+constexpr int ap_least(bool split, int dim) { return split ? 192 : dim > 64 ? 100 : 200; }
 // Rows of a CTA: eight fill a product; sixteen read and convert the codes once for all of them, with fewer CTAs an SM.  They pay with many rows a sequence (us with 8 and 16 rows:
 // 6000 rows of 80 channels 237 / 176, of 256 438 / 339; 16 and 32 rows, 64 sequences: 60 / 69 and 94 / 108), with 64 channels (64 sequences of 63 rows 46 / 43), and where
 // they bring the CTAs down to what clusters serve (1600 rows 31 / 23, 16 sequences of 16 rows 24 / 21); not where CTAs are few (80 of 8 rows 16.5 / 17.4).
 int attend_tile(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
 	const long long rows = (long long)p.longest * (a.heads / c.heads);
 	auto ctas = [&](int tile) { return (long long)p.n * cdiv(rows, tile) * c.heads; };
-	if (rows >= 64 && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(128) >= ap_least(a.q.type == SEQ_F32, c.dim)) return AP_TILE;
+	if (rows >= 64 && rows <= 65535 * 128LL && (c.dim == 64 || c.dim == 128) && !(a.softcap > 0.f) && !a.slopes && ctas(128) >= ap_least(a.q.type == SEQ_F32, c.dim)) return AP_TILE;
 	return rows > 8 && ctas(8) > AT_ROOM / 2 && (rows >= 64 || c.dim <= 64 || ctas(16) <= AT_ROOM / 2) ? 16 : 8;
 }
 AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a) {
@@ -1130,8 +1133,10 @@ AtPlan attend_plan(const SeqCache8& c, const SeqPortions& p, const SeqAttend8& a
 	if (a.chunk > 0) keys = std::min(keys, (long long)a.chunk + a.keep_first + tile / group);
 	const int chunks = cdiv(keys, AT_KEYS);
 	if (ctas < 1) return AtPlan{tile, 1, chunks, 0};
-	// many CTAs: several rounds, so that the last one is short (64 tokens over 2000 to 8000 keys: two rounds 140 us, six 126, eight 126, twelve 139)
-	long long shares = ctas >= 6 * room ? 1 : ctas > room / 2 ? cdiv(6 * room, ctas) : room / ctas;
+	// many CTAs: several rounds, so that the last one is short (64 tokens over 2000 to 8000 keys: two rounds 140 us, six 126, eight 126, twelve 139); one where tokens are many, whose
+	// shares would be as many rows to write and to fold (us with one and six: 2000 rows 44 / 63, 8 sequences of 400 34 / 53, 4 of 256 24 / 32)
+	const int rounds = (long long)p.longest * group >= 64 ? 1 : 6;
+	long long shares = ctas >= rounds * room ? 1 : ctas > room / 2 ? cdiv(rounds * room, ctas) : room / ctas;
 	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, ctas > room / 2 ? 2 * AT_WARPS : AT_WARPS), (long long)AT_SHARES}));
 	// one round: a cluster folds them, and the fold's launch is saved (one token over 4000 keys 11.0 us and 32.2 without, four 14.1 and 21.9)
 	const bool cluster = shares > 1 && ctas <= room / 2;

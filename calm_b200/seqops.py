@@ -102,7 +102,7 @@ def _gpu(name: str, t: torch.Tensor, index: int = -1) -> int:
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
     """The n best continuations of every group of beams: logits [groups, beams, vocab] (float32, bfloat16 or float16, the last axis contiguous), scores [groups,
-    beams] float32 (-inf: no beam there) -> tokens int32, parents int32, scores float32, each [groups, n], best first.  A candidate's score is its beam's plus the
+    beams] float32 (-inf, or not finite: no beam there) -> tokens int32, parents int32, scores float32, each [groups, n], best first.  A candidate's score is its beam's plus the
     token's log-probability; where fewer than n candidates are above -inf the rest is token -1, parent -1, score -inf.  `out`: the three tensors to write."""
     index = _gpu("logits", logits)
     _gpu("scores", scores, index)

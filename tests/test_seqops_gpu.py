@@ -90,6 +90,12 @@ def test_beams_with_rows_that_leave_nothing_and_special_values():
     check_beam(x, s, 6)
 
 
+def test_beams_whose_score_is_not_finite_are_not_there():
+    x = torch.randn(2, 4, 500, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    s = torch.tensor([[-1.0, math.inf, math.nan, -2.0], [math.inf, math.inf, -math.inf, math.nan]], device="cuda")
+    check_beam(x, torch.where(s.isfinite(), s, -math.inf), 12, seqops.beam_select(x, s, 12))
+
+
 def test_beams_strides_streams_outputs_and_replay():
     g = torch.Generator(device="cuda").manual_seed(5)
     wide = torch.randn(3, 4, 1111, generator=g, device="cuda", dtype=torch.float32).bfloat16()
@@ -296,28 +302,28 @@ def test_attention_options(opt, dtype):
 @pytest.mark.parametrize("page,dim,opt", [(16, 128, {}), (16, 64, {}), (13, 128, dict(window=70, keep_first=5)), (64, 64, dict(chunk=50)), (8, 128, dict(window=3, keep_first=90, sink=True, gate=True))])
 def test_attention_of_prompts(page, dim, opt, dtype):
     """Rows enough for the tensor cores' tiles of 128: several sequences of different lengths, one token and none among them, tiles that end inside a token's heads."""
-    c = Cached(5, -(-330 // page), 8, page, dim, page + dim)
+    c = Cached(5, -(-330 // page), 16, page, dim, page + dim)
     c.table[2, 3] = -1  # positions that are not there
     c.dtable.copy_(torch.tensor(c.table))
     g = torch.Generator(device="cuda").manual_seed(page)
     counts, before = [100, 37, 1, 0, 77], [0, 50, 300, 5, 130]
-    q = torch.randn(sum(counts), 24, dim, generator=g, device="cuda").to(DT[dtype])
+    q = torch.randn(sum(counts), 48, dim, generator=g, device="cuda").to(DT[dtype])
     opt = dict(opt)
     if opt.get("sink"):
-        opt["sink"] = torch.randn(24, generator=g, device="cuda") * 3
+        opt["sink"] = torch.randn(48, generator=g, device="cuda") * 3
     if opt.get("gate"):
-        opt["gate"] = torch.randn(sum(counts), 24, dim, generator=g, device="cuda")
+        opt["gate"] = torch.randn(sum(counts), 48, dim, generator=g, device="cuda")
     check_attend(c, q, seqops.Batch([1, 2, 4, 0, 3], counts, before), scale=0.7 * dim ** -0.5, **opt)
 
 
 def test_prompt_rows_whose_scores_grow():
     """Keys that grow along the sequence: references move in every tile and the sums are rescaled."""
-    c = Cached(1, 30, 8, 16, 128, 3)
+    c = Cached(1, 30, 2, 16, 128, 3)
     for i in range(30):
         c.scales[0, c.table[0, i]] = 2.0 ** (i / 2 - 14)
-    q = torch.randn(200, 32, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
-    check_attend(c, q.bfloat16(), seqops.Batch([0], [200], [270]), scale=0.1)
-    check_attend(c, q, seqops.Batch([0], [200], [0]), scale=0.1)
+    q = torch.randn(130, 200, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    check_attend(c, q.bfloat16(), seqops.Batch([0], [130], [340]), scale=0.1)
+    check_attend(c, q, seqops.Batch([0], [130], [0]), scale=0.1)
 
 
 def test_attention_of_one_token_over_many_keys():
@@ -365,6 +371,29 @@ def test_attention_does_not_see_what_is_not_there():
     check_attend(c, q, seqops.Batch([0, 2, 1], [3, 5, 1], [37, 44, 9]), scale=0.2, window=30)  # past the table's end
     b.data[2, 0], b.data[0, 1], b.data[3, 2] = 9, 16, -1
     check_attend(c, q, b, out=torch.full((16, 4, 32), 5.0, device="cuda"), scale=0.2)
+
+
+@pytest.mark.parametrize("tokens", [1, 800])
+@pytest.mark.parametrize("page", [8, 1])
+def test_positions_far_behind_the_table(tokens, page):
+    """Device arrays may hold any position: what lies behind the table is neither walked over nor stored, what is in it is still seen."""
+    c = Cached(2, 32 // page, 2, page, 64, 10)  # 32 positions a slot
+    one = torch.randn(1, 16, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).bfloat16()
+    q, rows = one.expand(2 * tokens, 16, 64).contiguous(), torch.ones(2 * tokens, 2, 64, device="cuda")
+    want = c.cache.attend(torch.cat([one, one]), c.dtable, seqops.Batch([0, 1], [1, 1], [31, 31]), 0.2).float()
+    codes, scales = c.values()
+    top = float((np.nan_to_num(np.abs(codes[1])).max((2, 3)) * scales[1]).max())
+    # each of the two is off by half a bf16 step and by its weights' fp16 rounding, in numerator and denominator
+    bound = 2 * (plain.BF16 * want.abs() + 2 * plain.F16 * top)
+    b = seqops.Batch([0, 1], [tokens, tokens], [20, 20])
+    for far in (2 ** 31 - 1 - tokens, 2 ** 30):
+        b.data[3] = far
+        before = [x.clone() for x in c.cache.buffers()]
+        c.cache.store(rows, rows, c.dtable, b)
+        assert all(torch.equal(x, y) for x, y in zip(before, c.cache.buffers()))
+        got = c.cache.attend(q, c.dtable, b, 0.2).float().view(2, tokens, 16, 64)
+        assert ((got - want[:, None]).abs() <= bound[:, None]).all()
+        assert (c.cache.attend(q, c.dtable, b, 0.2, window=16) == 0).all()
 
 
 def test_a_later_tokens_codes_reach_no_earlier_one():
