@@ -317,13 +317,13 @@ def test_attention_of_prompts(page, dim, opt, dtype):
 
 
 def test_prompt_rows_whose_scores_grow():
-    """Keys that grow along the sequence: references move in every tile and the sums are rescaled."""
-    c = Cached(1, 30, 2, 16, 128, 3)
+    """Keys that grow along the sequence: references move in every tile and the sums are rescaled.  (Single tokens beside it make the batch one for the tensor cores' tiles.)"""
+    c = Cached(8, 30, 2, 16, 128, 3)
     for i in range(30):
         c.scales[0, c.table[0, i]] = 2.0 ** (i / 2 - 14)
-    q = torch.randn(130, 200, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
-    check_attend(c, q.bfloat16(), seqops.Batch([0], [130], [340]), scale=0.1)
-    check_attend(c, q, seqops.Batch([0], [130], [0]), scale=0.1)
+    q = torch.randn(137, 32, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    check_attend(c, q.bfloat16(), seqops.Batch(list(range(8)), [130] + 7 * [1], [340] + 7 * [40]), scale=0.1)
+    check_attend(c, q, seqops.Batch(list(range(8)), [130] + 7 * [1], 8 * [0]), scale=0.1)
 
 
 def test_attention_of_one_token_over_many_keys():
