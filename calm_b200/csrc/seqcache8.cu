@@ -137,6 +137,8 @@ constexpr int AT_SHARES = 64;  // of a tile's keys at most
 constexpr int AT_TILE = 16, AT_CLUSTER = 16; // rows of a CTA at most; shares that a thread-block cluster folds at most
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr int AT_LIFT = 15;                // the largest query of a tile stands at 2^15 in fp16, so that what rounds as a subnormal is 2^-40 of it
+constexpr int AT_ALIKE = 12;               // rows whose largest elements lie further apart (2^this) have a power of two each; nearer ones share the tile's: no factor a score
+constexpr int AT_NO_ROW = -1000;           // exponent of a row of zeros
 constexpr float AT_MOST = 15.f, AT_SET = 10.f; // weights: at most 2^15, the largest at 2^10 or more
 
 struct Attend {
@@ -210,6 +212,14 @@ __device__ __forceinline__ void store_f32(void* p, int type, long long i, float 
 	else ((__half*)p)[i] = __float2half_rn(v);
 }
 
+// Queries times 2^-exponent stand at 2^AT_LIFT or less.  What is not finite does not count: it spoils its own row and no other.
+__device__ __forceinline__ uint32_t at_size(float x) { // |x| as bits, which are in the order of the values
+	const uint32_t a = __float_as_uint(x) & 0x7fffffff;
+	return a < 0x7f800000 ? a : 0;
+}
+__device__ __forceinline__ int at_exponent(uint32_t top) { return top ? min(max((int)(top >> 23) - 126, -85), 115) - AT_LIFT : AT_NO_ROW; } // top = m 2^(result + AT_LIFT)
+__device__ __forceinline__ float at_factor(int e) { return pow2f(e >> 1) * pow2f(e - (e >> 1)); } // 2^e, -200 <= e <= 0: under 2^-149 zero
+
 // the positions that a tile of rows sees, in order: [0, kept), then [lo, last]
 struct AtSpan {
 	int first, last, lo, kept, total, chunks;
@@ -239,7 +249,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	extern __shared__ __align__(128) unsigned char at_sm[];
 	uint2* const qf = reinterpret_cast<uint2*>(at_sm); // B fragments [KS][NQ][32], then the remainders'
 	AtStage<D>* const ring = reinterpret_cast<AtStage<D>*>(at_sm + (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2);
-	__shared__ float fold_m[AT_WARPS][8 * NQ], fold_l[AT_WARPS][8 * NQ], qtop[AT_WARPS];
+	__shared__ float fold_m[AT_WARPS][8 * NQ], fold_l[AT_WARPS][8 * NQ], qown[8 * NQ];
+	__shared__ uint32_t qsize[8 * NQ];
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 	const int b = blockIdx.z, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], tile = blockIdx.x;
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
@@ -305,30 +316,31 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 	};
 	request_keys(0), request_values();
 
-	// Queries as B fragments, times a power of two that is the tile's: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
+	// Queries as B fragments, times a power of two that is the tile's, or a row's own: k index 2t + {0, 1}, 2t + 8 + {0, 1} of step s is channel t * D / 4 + 4 s + {0, 1}, {2, 3} (so that a
 	// thread's codes of a key lie side by side).
-	float x[2 * NQ][D / 32], top = 0.f;
+	float x[2 * NQ][D / 32];
 #pragma unroll
 	for (int i = 0; i < 2 * NQ; ++i) {
 		const int r = i * AT_WARPS + warp, rr = row0 + min(r, rows - 1);
 		const long long at = (long long)(start + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head;
+		uint32_t top = 0;
 #pragma unroll
 		for (int k = 0; k < D / 32; ++k) {
 			const int d = k * 32 + lane;
 			x[i][k] = r < rows && d < dim ? load_as_f32(a.q, a.q_type, at + d) : 0.f;
-			top = fmaxf(top, fabsf(x[i][k]));
+			top = max(top, at_size(x[i][k]));
 		}
+		top = __reduce_max_sync(0xffffffffu, top);
+		if (lane == 0) qsize[r] = top;
 	}
-	top = warp_max(top);
-	if (lane == 0) qtop[warp] = top;
 	__syncthreads();
-#pragma unroll
-	for (int i = 0; i < AT_WARPS; ++i) top = fmaxf(top, qtop[i]);
-	const int qe = (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT; // top = m 2^(qe + AT_LIFT)
-	const float qdown = pow2f(-qe);
+	const int row_e = at_exponent(qsize[lane % (8 * NQ)]), tile_e = __reduce_max_sync(0xffffffffu, row_e), qe = tile_e == AT_NO_ROW ? 0 : tile_e;
+	const bool alike = __all_sync(0xffffffffu, row_e == AT_NO_ROW || row_e >= qe - AT_ALIKE);
+	if (tid < 8 * NQ) qown[tid] = row_e == AT_NO_ROW ? 1.f : at_factor(row_e - qe);
 #pragma unroll
 	for (int i = 0; i < 2 * NQ; ++i) {
-		const int r = i * AT_WARPS + warp;
+		const int r = i * AT_WARPS + warp, own = __shfl_sync(0xffffffffu, row_e, r);
+		const float qdown = pow2f(-(alike || own == AT_NO_ROW ? qe : own));
 #pragma unroll
 		for (int k = 0; k < D / 32; ++k) {
 			const int d = k * 32 + lane, dt = d / (D / 4), ds = d % (D / 4) / 4, de = d & 3;
@@ -340,7 +352,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 		}
 	}
 	__syncthreads();
-	const bool extra = a.softcap > 0.f || a.slopes;
+	const bool extra = a.softcap > 0.f || a.slopes || !alike;
 	const float qscale = a.scale * pow2f(qe) * (extra ? 1.f : AT_LOG2E);
 	uint2 qr[KEEP ? (SPLIT ? 2 : 1) * KS * NQ : 1];
 	if (KEEP) {
@@ -398,7 +410,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 		const int j0 = chunk * AT_KEYS;
 		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= sp.first;
 		float over[4]; // 1 / value scale
-		if (extra) { // a soft cap or slopes
+		if (extra) { // a soft cap, slopes or rows with powers of two of their own
 #pragma unroll 1
 			for (int j = 0; j < 4; ++j) {
 				const int kp = position(j0 + 8 * j + g);
@@ -407,7 +419,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 				for (int q = 0; q < NQ; ++q)
 #pragma unroll
 					for (int e = 0; e < 2; ++e) {
-						float y = (j & 2 ? (j & 1 ? z[1][q][2 + e] : z[1][q][e]) : (j & 1 ? z[0][q][2 + e] : z[0][q][e])) * kf;
+						float y = (j & 2 ? (j & 1 ? z[1][q][2 + e] : z[1][q][e]) : (j & 1 ? z[0][q][2 + e] : z[0][q][e]));
+						if (!alike) y *= qown[8 * q + 2 * t + e];
+						y *= kf;
 						if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
 						if (a.slopes) y -= a.slopes[kvh * a.group + (row0 + min(8 * q + 2 * t + e, rows - 1)) % a.group] * (float)(rpos[q][e] - kp);
 						y *= AT_LOG2E;
@@ -632,7 +646,7 @@ struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	uint32_t seen[STAGES][2];      // keys that are there
 	uint64_t kv_full[STAGES], kv_empty[STAGES], s_full[GROUPS][2], p_full[GROUPS], p_empty[GROUPS], done;
 	uint32_t tmem;
-	float top[4 * GROUPS];
+	int tops[4 * GROUPS], least[4 * GROUPS]; // exponents of the queries: the largest and the smallest row of a warp's
 	int lost;
 };
 // false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN
@@ -685,11 +699,18 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
 	    : "memory");
 }
 template <int N>
-__device__ __forceinline__ int ap_exponent(const float (&tops)[N]) { // queries times 2^-this stand at 2^AT_LIFT or less
-	float top = tops[0];
+__device__ __forceinline__ int ap_tile_exponent(const int (&tops)[N]) {
+	int e = tops[0];
 #pragma unroll
-	for (int i = 1; i < N; ++i) top = fmaxf(top, tops[i]);
-	return (top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 126, -85), 115) : 0) - AT_LIFT;
+	for (int i = 1; i < N; ++i) e = max(e, tops[i]);
+	return e == AT_NO_ROW ? 0 : e;
+}
+template <int N>
+__device__ __forceinline__ bool ap_alike(const int (&least)[N], int tile_e) {
+	int e = least[0];
+#pragma unroll
+	for (int i = 1; i < N; ++i) e = min(e, least[i]);
+	return e >= tile_e - AT_ALIKE;
 }
 template <int D, bool SPLIT>
 __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, const Attend a) {
@@ -716,23 +737,28 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 		s.lost = 0;
 		mbar_init_fence();
 	}
-	// queries, times the tile's power of two
+	// queries, times the tile's power of two, or the row's own
+	int row_e = 0;
 	const int token = start + (row0 + min(tid, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(tid, rows - 1)) % a.group;
 	if (warp < WARPS) {
 		const long long at = token * a.q_row + head * a.q_head;
 		const int bytes = a.q_type == SEQ_F32 ? 4 : 2;
 		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * bytes) | (uintptr_t)(a.q_head * bytes)) % 16 == 0;
-		float x[8], top = 0.f;
+		float x[8];
+		uint32_t top = 0;
 #pragma unroll 4
 		for (int piece = 0; piece < D / 8; ++piece) {
 			load8(a.q, a.q_type, at + piece * 8, vec, x);
 #pragma unroll
-			for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+			for (int i = 0; i < 8; ++i) top = max(top, at_size(x[i]));
 		}
-		top = warp_max(top);
-		if (lane == 0) s.top[warp] = top;
+		row_e = at_exponent(top); // (a thread's own row; behind the last one that once more)
+		const int most = __reduce_max_sync(0xffffffffu, row_e), least = __reduce_min_sync(0xffffffffu, row_e == AT_NO_ROW ? -AT_NO_ROW : row_e);
+		if (lane == 0) s.tops[warp] = most, s.least[warp] = least;
 		asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
-		const float down = tid < rows ? pow2f(-ap_exponent(s.top)) : 0.f;
+		const int tile_e = ap_tile_exponent(s.tops);
+		if (row_e == AT_NO_ROW || ap_alike(s.least, tile_e)) row_e = tile_e;
+		const float down = tid < rows ? pow2f(-row_e) : 0.f;
 #pragma unroll 2
 		for (int piece = 0; piece < D / 8; ++piece) {
 			load8(a.q, a.q_type, at + piece * 8, vec, x);
@@ -749,7 +775,8 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = s.tmem; // scores of even tiles, a group's 64 columns beside another's, of odd ones, sums: 128 columns a group
-	const float qscale = a.scale * pow2f(ap_exponent(s.top)) * AT_LOG2E;
+	const int tile_e = ap_tile_exponent(s.tops);
+	const float qscale = a.scale * pow2f(tile_e) * AT_LOG2E;
 	float m = -INFINITY, l = 0.f;
 
 	// registers go from the warps of keys and values to those of the softmax: 8 x 112 + 8 x 80 + 96 = 17 x 96, what the block was launched with
@@ -758,6 +785,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 		const int group = warp / 4;
 		const int rpos = tid < rows ? p0 + (row0 + tid) / a.group : -1, rlow = tid < rows ? at_low(a, rpos) : 0, wide = at_low(a, sp.last);
 		const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), sums_at = lanes + O_COL + 128 * group;
+		const float own = ap_alike(s.least, tile_e) ? 1.f : at_factor(row_e - tile_e);
 		int st = 0;
 		uint32_t round = 0;
 		for (int i = 0; i < tiles && group < groups; ++i) {
@@ -772,6 +800,13 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			float z[64], top = -INFINITY; // log2 of the weights against the reference as it stands (against 0 before there is one)
 			tmem_ld32(scores_at, *reinterpret_cast<float(*)[32]>(z));
 			tmem_ld32(scores_at + 32, *reinterpret_cast<float(*)[32]>(z + 32));
+			if (own != 1.f) { // a row with a power of two of its own
+#pragma unroll
+				for (int k = 0; k < 64; k += 2) {
+					const float2 x = halves(mul2(pair_of(z[k], z[k + 1]), pair_of(own, own)));
+					z[k] = x.x, z[k + 1] = x.y;
+				}
+			}
 			const u64 off = pair_of(bias - base, bias - base);
 #pragma unroll
 			for (int k = 0; k < 64; k += 4) {

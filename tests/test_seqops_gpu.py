@@ -476,3 +476,67 @@ def test_store_and_attention_as_they_are_used():
                 # a code is off by 2^-4 of its value at most: scores by 2^-4 sum |q k|, values by 2^-4, typically a quarter of the random sums of these
                 ds = 2.0 ** -4 * np.sqrt(((k[:, h] * as64(rows[s, p, 2, h])) ** 2).sum(1).max()) * dim ** -0.5
                 assert np.abs(as64(o[s, h]) - want).max() <= 4 * (2.0 ** -4 + ds) * np.abs(v[:, h]).max()
+
+
+def check_rows_beside(c, q, odd, batch, opt, heads, near=None):
+    """Attention of all of q, then the rows that are not odd against the definition, which works on each by itself: their reference and their bound come from queries without the odd
+    ones.  heads: the key heads looked at."""
+    o = c.cache.attend(q, c.dtable, batch, **opt)
+    group = q.shape[1] // c.heads
+    clean = q.masked_fill(odd[:, :, None], 0.0)
+    values, scales = c.values()
+    for h in heads:
+        mine = slice(h * group, (h + 1) * group)
+        kw = {k: (as64(v)[mine] if isinstance(v, torch.Tensor) else v) for k, v in opt.items()}
+        ref, tol = plain.attend(as64(clean[:, mine]), values[0][:, h:h + 1], scales[0][:, h:h + 1], values[1][:, h:h + 1], scales[1][:, h:h + 1], c.table, portions_of(batch), c.page,
+                                split=q.dtype == torch.float32, **kw)
+        got, there = as64(o[:, mine]), ~odd[:, mine].cpu().numpy()
+        if near is not None:
+            there &= near(h)[:, None]
+        bound = tol + plain.half_step(o.dtype) * (np.abs(ref) + tol) + (2.0 ** -24 if o.dtype == torch.float16 else 0.0)
+        assert there.any() and np.isfinite(got[there]).all() and (np.abs(got - ref)[there] <= bound[there]).all(), (h, np.abs(got - ref)[there].max())
+    return o
+
+
+ODD = {"inf": math.inf, "nan": math.nan, "2^40": 2.0 ** 40, "2^-30 2^100": 2.0 ** 100}
+
+
+@pytest.mark.parametrize("odd", list(ODD))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("dim,opt", [(128, {}), (64, {}), (256, dict(softcap=4.0)), (80, dict(slopes=True))])
+def test_odd_queries_beside_ordinary_ones(dim, opt, dtype, odd):
+    """One element of one head's query is infinite, no number, or far above what the others hold: the other heads and tokens keep their values (tiles of eight and of sixteen rows)."""
+    if dtype == "fp16" and "2^" in odd:
+        pytest.skip("not a value of the type")
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    for seqs, tokens in ((3, 1), (30, 5)):
+        c = Cached(seqs, 6, 2, 16, dim, dim + seqs)
+        q = torch.randn(seqs * tokens, 12, dim, generator=g, device="cuda").to(DT[dtype])
+        if "2^-30" in odd:
+            q = q * 2.0 ** -30
+        at = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+        for token, head in ((0, 7), (seqs * tokens - 1, 11)):
+            q[token, head, 5], at[token, head] = ODD[odd] * (-1) ** token, True
+        kw = dict(scale=0.2 * (2.0 ** 30 if "2^-30" in odd else 1.0), **opt)
+        if "slopes" in opt:
+            kw["slopes"] = torch.rand(12, generator=g, device="cuda") * 0.1
+        check_rows_beside(c, q, at, seqops.Batch(range(seqs), [tokens] * seqs, [60 + i % 30 for i in range(seqs)]), kw, [1])
+
+
+@pytest.mark.parametrize("odd", list(ODD))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_odd_queries_in_a_prompt(dim, dtype, odd):
+    """The same in the tensor cores' tiles of 128: a later token's query reaches neither earlier tokens nor other heads."""
+    if dtype == "fp16" and "2^" in odd:
+        pytest.skip("not a value of the type")
+    c = Cached(5, 21, 16, 16, dim, dim)
+    g = torch.Generator(device="cuda").manual_seed(dim + 1)
+    counts, before = [100, 37, 1, 0, 77], [0, 50, 300, 5, 130]
+    q = torch.randn(sum(counts), 48, dim, generator=g, device="cuda").to(DT[dtype])
+    if "2^-30" in odd:
+        q = q * 2.0 ** -30
+    at = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for token, head in ((60, 7), (99, 6), (120, 47), (214, 8)):
+        q[token, head, 3], at[token, head] = ODD[odd], True
+    check_rows_beside(c, q, at, seqops.Batch([1, 2, 4, 0, 3], counts, before), dict(scale=0.7 * dim ** -0.5 * (2.0 ** 30 if "2^-30" in odd else 1.0)), [2, 15])
