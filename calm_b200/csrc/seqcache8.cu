@@ -244,6 +244,7 @@ __device__ __forceinline__ void at_finish(const Attend& a, int token, int head, 
 template <int D, bool SPLIT, int NQ>
 __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 256 ? 3 : 2) k_c8_attend(const C8 c, const Attend a) {
 	constexpr bool KEEP = D * NQ * (SPLIT ? 2 : 1) <= 128; // the queries' fragments stay in registers
+	constexpr bool OWN_LATE = SPLIT && D * NQ > 256; // rows' own factors a key at a time: 129 us for 138 where registers are all in use, else all at once (soft-capped prompts 97 for 101)
 	constexpr int KS = D / 16, MT = D / 16, PIECES = D / 16;
 	constexpr int FS = D == 256 ? 52 : 20, LD = 8 * FS + 4; // sums in shared memory: eight parts of a row FS apart, rows LD: 16-byte stores of eight lanes meet different banks
 	extern __shared__ __align__(128) unsigned char at_sm[];
@@ -411,6 +412,12 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 		const bool all = seen == 0xffffffffu && j0 >= kept && position(j0) >= wide && position(j0 + AT_KEYS - 1) <= sp.first;
 		float over[4]; // 1 / value scale
 		if (extra) { // a soft cap, slopes or rows with powers of two of their own
+			if (!OWN_LATE && !alike)
+#pragma unroll
+				for (int i = 0; i < 2 * NQ; ++i) {
+					const float f = qown[8 * (i >> 1) + 2 * t + (i & 1)];
+					z[0][i >> 1][i & 1] *= f, z[0][i >> 1][2 + (i & 1)] *= f, z[1][i >> 1][i & 1] *= f, z[1][i >> 1][2 + (i & 1)] *= f;
+				}
 #pragma unroll 1
 			for (int j = 0; j < 4; ++j) {
 				const int kp = position(j0 + 8 * j + g);
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 #pragma unroll
 					for (int e = 0; e < 2; ++e) {
 						float y = (j & 2 ? (j & 1 ? z[1][q][2 + e] : z[1][q][e]) : (j & 1 ? z[0][q][2 + e] : z[0][q][e]));
-						if (!alike) y *= qown[8 * q + 2 * t + e];
+						if (OWN_LATE && !alike) y *= qown[8 * q + 2 * t + e];
 						y *= kf;
 						if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
 						if (a.slopes) y -= a.slopes[kvh * a.group + (row0 + min(8 * q + 2 * t + e, rows - 1)) % a.group] * (float)(rpos[q][e] - kp);
