@@ -636,6 +636,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // through its roles, about 3900 cycles, of which a softmax warp works 3000 (its exponentials keep the units busy for 1024 of them, the tensor cores are for about 1300); registers
 // hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86).
 constexpr int AP_KEYS = 64, C8_NONE = -1000;
+// Value scales that go through the products together lie within 2^AP_NEAR; a tile whose scales lie further apart comes several times, each time with the keys of one such range.  Codes
+// stay exact in units of the largest scale.  Where a row may not see the key that has it, the row's reference goes by what it sees, weights times their keys' own scales (AP_NEAR more
+// than AT_SET is still under AT_MOST): what is rounded as a subnormal is 2^-35 of the largest weight times the largest scale that the row sees.
+constexpr int AP_NEAR = 4;
 constexpr int ap_groups(bool split) { return split ? 1 : 2; } // of 128 rows
 constexpr int ap_threads(bool split) { return 256 * ap_groups(split) + 32; }
 __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
@@ -649,8 +653,10 @@ struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	unsigned char k[STAGES][PANELS][AP_KEYS * 128];
 	unsigned char v[STAGES][D * 128];
 	float factor[STAGES][AP_KEYS]; // of a tile's keys on their scores, in log2
+	alignas(16) float lower[STAGES][AP_KEYS]; // log2 of their value scales against the largest, where they differ
 	float bias[STAGES];            // log2 of the largest of the tile's value scales: its values come in units of that
 	uint32_t seen[STAGES][2];      // keys that are there
+	int tile[STAGES], last[STAGES], even[STAGES]; // which 64 keys; whether nothing comes behind them; whether their value scales are one
 	uint64_t kv_full[STAGES], kv_empty[STAGES], s_full[GROUPS][2], p_full[GROUPS], p_empty[GROUPS], done;
 	uint32_t tmem;
 	int tops[4 * GROUPS], least[4 * GROUPS]; // exponents of the queries: the largest and the smallest row of a warp's
@@ -793,13 +799,14 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 		const int rpos = tid < rows ? p0 + (row0 + tid) / a.group : -1, rlow = tid < rows ? at_low(a, rpos) : 0, wide = at_low(a, sp.last);
 		const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), sums_at = lanes + O_COL + 128 * group;
 		const float own = ap_alike(s.least, tile_e) ? 1.f : at_factor(row_e - tile_e);
-		int st = 0;
+		int st = 0, i = 0;
 		uint32_t round = 0;
-		for (int i = 0; i < tiles && group < groups; ++i) {
+		for (bool last = tiles == 0 || group >= groups; !last; ++i) {
 			const uint32_t scores_at = lanes + (i & 1) * S_COLS + 64 * group;
 			if (!ap_wait_warp(s.kv_full + st, round, &s.lost) || !ap_wait_warp(s.s_full[group] + (i & 1), (i >> 1) & 1, &s.lost)) break; // (the factors; the scores)
 			tc_fence_after();
-			const int j0 = i * AP_KEYS;
+			const int j0 = s.tile[st] * AP_KEYS;
+			last = s.last[st];
 			const uint32_t seen[2] = {s.seen[st][0], s.seen[st][1]};
 			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
 			const float bias = s.bias[st];
@@ -833,7 +840,16 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			for (int k = 0; k < 64; k += 2) tops[k / 2 % 4] = fmaxf(fmaxf(tops[k / 2 % 4], z[k]), z[k + 1]);
 			top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 			if (__any_sync(0xffffffffu, top > most)) { // references move
-				const float mn = top > most ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
+				const bool moves = top > most;
+				if (!all && !s.even[st]) {
+					top = -INFINITY;
+#pragma unroll
+					for (int k = 0; k < 64; k += 4) {
+						const float4 u = *reinterpret_cast<const float4*>(s.lower[st] + k);
+						top = fmaxf(fmaxf(top, fmaxf(z[k] + u.x, z[k + 1] + u.y)), fmaxf(z[k + 2] + u.z, z[k + 3] + u.w));
+					}
+				}
+				const float mn = moves ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
 #pragma unroll
 				for (int k = 0; k < 64; ++k) z[k] += by;
 				m = mn, l *= f;
@@ -864,7 +880,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			if (lane == 0) mbar_arrive(s.p_full + group);
 			if (++st == STAGES) st = 0, round ^= 1;
 		}
-		if (tiles > 0 && group < groups) ap_wait_warp(s.p_empty + group, (tiles - 1) & 1, &s.lost);
+		if (i > 0) ap_wait_warp(s.p_empty + group, (i - 1) & 1, &s.lost);
 		tc_fence_after();
 		float norm = 1.f;
 		if (a.sinks && tid < rows) {
@@ -950,14 +966,9 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 		int st = 0;
 		uint32_t round = 0;
 		if (tiles > 0) look(0), load(0);
-		for (int i = 0; i < tiles; ++i) {
+		for (int i = 0; i < tiles;) {
 			if (!ap_wait_warp(s.kv_empty + st, round ^ 1, &s.lost)) break;
-			if (t < AP_KEYS) {
-				const bool there = own == 0 ? have[0] : have[1];
-				s.factor[st][t] = there ? scale * qscale : 0.f;
-				const uint32_t seen = __ballot_sync(0xffffffffu, there);
-				if (lane == 0) s.seen[st][own] = seen;
-			}
+			if (t < AP_KEYS) s.factor[st][t] = (own == 0 ? have[0] : have[1]) ? scale * qscale : 0.f;
 #pragma unroll
 			for (int k = 0; k < KEACH; ++k) {
 				const int key = (k * WARPS + own) * KROWS + lane / PIECES, piece = lane % PIECES;
@@ -970,14 +981,21 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 				*reinterpret_cast<uint4*>(to + ((odd ? at ^ 1 : at) << 4)) = odd ? hi : lo;
 				*reinterpret_cast<uint4*>(to + ((odd ? at : at ^ 1) << 4)) = odd ? lo : hi;
 			}
-			// values in units of the tile's largest scale: a smaller one's are shifted down (below 2^-24 of the largest nothing is left of a code)
+			// values in units of the largest scale, a smaller one's shifted down, exactly
 			int e[2];
 #pragma unroll
 			for (int h = 0; h < 2; ++h) e[h] = have[h] ? max((exps[h] >> 23 & 255) - 127, -126) : C8_NONE;
 			int most = __reduce_max_sync(0xffffffffu, max(e[0], e[1]));
 			if (most == C8_NONE) most = 0;
-			if (t == 0) s.bias[st] = (float)most;
-			const bool even = __all_sync(0xffffffffu, (e[0] == most || e[0] == C8_NONE) && (e[1] == most || e[1] == C8_NONE));
+			const int least = __reduce_min_sync(0xffffffffu, min(e[0] == C8_NONE ? INT_MAX : e[0], e[1] == C8_NONE ? INT_MAX : e[1]));
+			const bool even = least >= most, more = least < most - AP_NEAR; // more: the keys with smaller scales come after these
+			if (t < AP_KEYS) {
+				const int own_e = own == 0 ? e[0] : e[1];
+				const uint32_t seen = __ballot_sync(0xffffffffu, own_e >= most - AP_NEAR);
+				if (lane == 0) s.seen[st][own] = seen;
+				if (!even) s.lower[st][t] = (float)(own_e - most);
+			}
+			if (t == 0) s.bias[st] = (float)most, s.even[st] = even, s.tile[st] = i, s.last[st] = i == tiles - 1 && !more;
 			if (mine != (1u << VKEYS) - 1) { // (a code that is no number would spoil rows that do not see it)
 #pragma unroll
 				for (int k = 0; k < VKEYS; ++k)
@@ -1020,18 +1038,21 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			fence_async_smem();
 			__syncwarp();
 			if (lane == 0) mbar_arrive(s.kv_full + st);
-			if (i + 1 < tiles) load(i + 1);
+			if (more) have[0] = have[0] && e[0] < most - AP_NEAR, have[1] = have[1] && e[1] < most - AP_NEAR;
+			else if (++i < tiles) load(i);
 			if (++st == STAGES) st = 0, round ^= 1;
 		}
 	} else if (lane == 0) {
 		constexpr uint32_t score = (1u << 4) | ((uint32_t)(AP_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows
 		int st = 0, behind = 0; // stages of this tile's keys, of the values of the one before
 		uint32_t round = 0;
-		bool there = true;
-		for (int i = 0; i <= tiles && tiles > 0 && there; ++i) {
-			if (i < tiles) {
+		bool there = tiles > 0, last = false;
+		for (int i = 0; there; ++i) {
+			if (last) there = false; // the last tile's values are left
+			else {
 				if (!ap_wait(s.kv_full + st, round, &s.lost)) break; // (the scores' columns: the product of the tile before the last, which read weights there, was issued earlier)
 				tc_fence_after();
+				last = s.last[st];
 				for (int g = 0; g < groups; ++g) {
 #pragma unroll
 					for (int h = 0; h < Shared::PAIR; ++h)
@@ -1046,7 +1067,10 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			if (i > 0) {
 				const int j = i - 1;
 				for (int g = 0; g < groups; ++g) {
-					if (!(there = ap_wait(s.p_full + g, j & 1, &s.lost))) break;
+					if (!ap_wait(s.p_full + g, j & 1, &s.lost)) {
+						there = false;
+						break;
+					}
 					tc_fence_after();
 #pragma unroll
 					for (int h = 0; h < Shared::PAIR; ++h)

@@ -410,8 +410,8 @@ int calm_b200_seq_cache8_store(const struct SeqCache8* cache, const struct SeqPo
  * ones, lo = max(p - window + 1 with window > 0, floor(p / chunk) * chunk with chunk > 0, 0); query head h reads key head h / group.
  *   s_j = softcap(scale q . k_j) - slopes[h] (p - j);  out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h])), times sigmoid(gate) where given.
  * Scores, softmax and sums are fp32; queries and softmax weights enter the tensor cores as fp16 (queries scaled by a power of two: one for those that are
- * worked on together, at most 256 rows of one sequence, where their largest elements lie within 2^12 of each other, else one a row; elements that are not finite spoil their own row alone), as a pair of fp16 value and remainder where the queries are fp32; codes enter exactly (where a prompt's 64 keys have values of different scales, those enter as multiples of the largest one's
- * 2^-24 times its scale).   Codes of a page that some token sees are finite: a NaN among them may reach rows that do not see it.
+ * worked on together, at most 256 rows of one sequence, where their largest elements lie within 2^12 of each other, else one a row; elements that are not finite spoil their own row alone), as a pair of fp16 value and remainder where the queries are fp32; codes enter exactly. The value scales of the keys
+ * that a token sees lie within 2^112 of one another (else a weight may be missing from its denominator). Codes of a page that some token sees are finite: a NaN among them may reach rows that do not see it.
  * A token that sees nothing gets zeros. */
 struct SeqAttend8 {
 	struct SeqRows q, out;   /* out.type: as q's, or SEQ_BF16 where the queries are fp32 */

@@ -540,3 +540,49 @@ def test_odd_queries_in_a_prompt(dim, dtype, odd):
     for token, head in ((60, 7), (99, 6), (120, 47), (214, 8)):
         q[token, head, 3], at[token, head] = ODD[odd], True
     check_rows_beside(c, q, at, seqops.Batch([1, 2, 4, 0, 3], counts, before), dict(scale=0.7 * dim ** -0.5 * (2.0 ** 30 if "2^-30" in odd else 1.0)), [2, 15])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("far", [14, 18, 40, 110])
+def test_values_that_a_prompts_rows_do_not_see(dim, far, dtype):
+    """Pages whose value scale is 2^far times the others', ahead of some rows and behind the window of others that share their tiles of keys: those rows' results know nothing of it."""
+    c = Cached(5, 21, 16, 16, dim, dim + far)
+    for slot in (0, 1):
+        c.scales[1, c.table[slot, 3]] *= 2.0 ** far
+    g = torch.Generator(device="cuda").manual_seed(far)
+    counts, before = [100, 100, 1, 1, 77], [0, 0, 300, 5, 130]
+    q = torch.randn(sum(counts), 48, dim, generator=g, device="cuda").to(DT[dtype])
+    none = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    batch = seqops.Batch([0, 1, 2, 3, 4], counts, before)
+    check_rows_beside(c, q, none, batch, dict(scale=dim ** -0.5), [0, 7], near=lambda h: np.arange(sum(counts)) % 100 < 48)
+    pos = np.concatenate([b + np.arange(n) for n, b in zip(counts, before)])
+    check_rows_beside(c, q, none, batch, dict(scale=dim ** -0.5, window=10), [0, 7], near=lambda h: (pos < 48) | (pos >= 64 + 9))
+    check_rows_beside(c, q, none, batch, dict(scale=dim ** -0.5), [0, 7])  # and those that see it, within what their own bound says
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("far", [17, 60])
+def test_small_values_that_take_a_prompts_weights(dim, far, dtype):
+    """Keys with small values score far above keys with large ones: the result is the small values' mean, as if the others were not there (their weights are e^-100 2^far at most)."""
+    c = Cached(5, 21, 16, 16, dim, dim + far)
+    g = torch.Generator(device="cuda").manual_seed(far)
+    counts, before = [100, 37, 1, 0, 77], [0, 50, 300, 5, 130]
+    batch = seqops.Batch([1, 2, 4, 0, 3], counts, before)
+    q = (1.0 + 0.05 * torch.rand(sum(counts), 48, dim, generator=g, device="cuda")).to(DT[dtype])
+    c.codes[0], c.scales[0] = 0x38, 1.0  # keys of ones (1.0 is code 0x38)
+    seen = c.table.copy()
+    for slot in range(5):
+        for block in range(1, 21, 3):
+            p = c.table[slot, block]
+            c.codes[0, p], c.scales[1, p] = 0xB8, c.scales[1, p] * 2.0 ** far  # minus ones
+            seen[slot, block] = -1
+    o = as64(c.cache.attend(q, c.dtable, batch, scale=100.0 / dim))
+    values, scales = c.values()
+    for h in (0, 9):
+        mine = slice(3 * h, 3 * h + 3)
+        ref, tol = plain.attend(as64(q[:, mine]), *[x[:, h:h + 1] for x in (values[0], scales[0], values[1], scales[1])], seen, portions_of(batch), c.page, 100.0 / dim, split=dtype == "fp32")
+        rest = 2.0 ** (far - 2 * 100 / math.log(2)) * 448.0 * 330
+        bound = tol + plain.half_step(DT[dtype]) * (np.abs(ref) + tol) + rest
+        assert (np.abs(o[:, mine] - ref) <= bound).all(), np.abs(o[:, mine] - ref).max()
