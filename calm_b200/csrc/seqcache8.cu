@@ -236,6 +236,8 @@ __device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int
 	s.chunks = (s.total + AT_KEYS - 1) / AT_KEYS;
 	return s;
 }
+// a sink's term of the denominator against a reference that is no lower: none for -inf, all of it for +inf
+__device__ __forceinline__ float at_sink(float sk, float top) { return sk == -INFINITY ? 0.f : sk == top ? 1.f : ex2(sk - top); }
 __device__ __forceinline__ void at_finish(const Attend& a, int token, int head, int d, float v) {
 	if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
 	store_f32(a.out, a.out_type, token * a.o_row + head * a.o_head + d, v);
@@ -575,7 +577,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 			if (whole) {
 				if (a.sinks) { // one more term of the denominator
 					const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(mx, sk), down = mx == -INFINITY ? 0.f : ex2(mx - mn);
-					den = den * down + ex2(sk - mn), norm = down;
+					den = den * down + at_sink(sk, mn), norm = down;
 				} else norm = 1.f;
 				norm = den > 0.f ? norm / den : den == 0.f ? 0.f : den; // (a NaN stays one)
 			} else if (lane == 0) part[dim] = mx, part[dim + 1] = den;
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 				const float f = ms[k] == -INFINITY ? 0.f : ex2(ms[k] - mx);
 				wz[k][tid] = f, den = fmaf(f, ls[k], den);
 			}
-		if (a.sinks) den += ex2(sk - mx);
+		if (a.sinks) den += at_sink(sk, mx);
 		inv[tid] = den > 0.f ? 1.f / den : den; // (0: nothing was seen)
 	}
 	__syncthreads();
@@ -885,7 +887,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 		float norm = 1.f;
 		if (a.sinks && tid < rows) {
 			const float sk = a.sinks[head] * AT_LOG2E, mn = fmaxf(m, sk), down = m == -INFINITY ? 0.f : ex2(m - mn);
-			l = l * down + ex2(sk - mn), norm = down;
+			l = l * down + at_sink(sk, mn), norm = down;
 		}
 		norm = *(volatile int*)&s.lost ? NAN : l > 0.f ? norm / l : l == 0.f ? 0.f : l; // (0: nothing was seen; a NaN stays one)
 		const bool wide_store = a.out_type != SEQ_F32 && !a.gate && ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
@@ -1120,7 +1122,7 @@ __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 			den = fmaf(f, w[i], den), w[i] = f;
 		}
 		den = warp_sum(den);
-		if (a.sinks) den += ex2(sk - mx);
+		if (a.sinks) den += at_sink(sk, mx);
 		const float norm = den > 0.f ? 1.f / den : den; // (0: nothing was seen)
 		for (int d0 = 0; d0 < c.dim; d0 += 128) {
 			float v[4] = {0.f, 0.f, 0.f, 0.f};

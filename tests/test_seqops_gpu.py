@@ -586,3 +586,21 @@ def test_small_values_that_take_a_prompts_weights(dim, far, dtype):
         rest = 2.0 ** (far - 2 * 100 / math.log(2)) * 448.0 * 330
         bound = tol + plain.half_step(DT[dtype]) * (np.abs(ref) + tol) + rest
         assert (np.abs(o[:, mine] - ref) <= bound).all(), np.abs(o[:, mine] - ref).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("seqs,tokens,before", [(2, 1, 20), (1, 1, 300), (150, 1, 300), (5, 60, 200)])
+def test_sinks_that_are_infinite(seqs, tokens, before, dtype):
+    """exp(-inf) = 0 adds nothing, also where a token sees nothing; exp(+inf) takes everything.  (One share, a cluster's, shares through memory, a prompt's tiles.)"""
+    c = Cached(seqs, 23, 16, 16, 128, seqs)
+    c.table[0] = -1
+    c.dtable.copy_(torch.tensor(c.table))
+    q = torch.randn(seqs * tokens, 48, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(DT[dtype])
+    b = seqops.Batch(range(seqs), [tokens] * seqs, [before] * seqs)
+    sink = torch.zeros(48, device="cuda")
+    sink[::3], sink[1::3] = -math.inf, math.inf
+    got, free = c.cache.attend(q, c.dtable, b, 0.1, sink=sink), c.cache.attend(q, c.dtable, b, 0.1)
+    assert (got[:tokens] == 0).all() and (got[:, 1::3] == 0).all() and (free[:tokens] == 0).all()
+    # the same weights over the same denominator: a rounding each where the factor 1 is applied, and the output's own
+    off = (got[:, ::3].double() - free[:, ::3].double()).abs()
+    assert (off <= (2 * plain.half_step(DT[dtype]) + 4 * plain.F32) * free[:, ::3].double().abs()).all()
