@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 // Slices of a row: a tile each where rows are few, three CTAs an SM in all where they are many (148 / 296 / 444 / 592 CTAs in all: 160 rows of 128256 fp32 30.5 / 30.9 / 24.2 /
 // 34.7 us, 100 rows 26.4 / 20.3 / 18.1 / 24.1, 64 rows 18.2 / 15.9 / 16.5 / 18.2: a slice's end costs about the same whatever its length), two an SM for the longest rows.
 int beam_slices(int groups, int beams, int vocab) {
-	const int want = std::max(std::min(cdiv(vocab, BM_TILE), 148 * 3 / (groups * beams)), cdiv(vocab, BM_TILE * BM_SLICE));
+	const int want = std::max(std::min(cdiv(vocab, BM_TILE), 148 * 3 / std::max(1, groups * beams)), cdiv(vocab, BM_TILE * BM_SLICE));
 	return std::max(cdiv(vocab, BM_TILE * (BM_TILES - 1)), std::min(want, BM_LISTS / beams)); // (a row that starts behind a 16-byte boundary may reach into one tile more)
 }
 size_t beam_shared(const BeamArgs& a, int size) { // tiles of a slice, as the kernel cuts them at the worst alignment

@@ -153,3 +153,10 @@ def test_the_plain_rounding_is_torchs():
     for a in (0.0, 1.0, 448.0, 448.1, 449.0, 3e38, 1e-30, 2.0 ** -60):
         e = plain.exponent(a)
         assert a <= 448 * 2.0 ** e and (e == -64 or a > 448 * 2.0 ** (e - 1))
+
+
+def test_a_batch_without_groups():
+    """Nothing to select, nothing to hold; what is refused with groups is refused without."""
+    for beams in (1, 4, 64):
+        assert L.calm_b200_seq_beam_workspace(0, beams, 100, 3) == 0 and beam(groups=0, beams=beams) == 0
+    says(beam(groups=0, beams=65), "beam", "64")

@@ -604,3 +604,8 @@ def test_sinks_that_are_infinite(seqs, tokens, before, dtype):
     # the same weights over the same denominator: a rounding each where the factor 1 is applied, and the output's own
     off = (got[:, ::3].double() - free[:, ::3].double()).abs()
     assert (off <= (2 * plain.half_step(DT[dtype]) + 4 * plain.F32) * free[:, ::3].double().abs()).all()
+
+
+def test_beams_of_no_groups():
+    tok, par, best = seqops.beam_select(torch.zeros(0, 3, 50, device="cuda"), torch.zeros(0, 3, device="cuda"), 4)
+    assert tok.shape == par.shape == best.shape == (0, 4)
