@@ -5,7 +5,7 @@
 // from their lists.
 //   log sum_u exp x_u = m + log sum_s exp(m_s - m) S_s,   S_s = sum_(u in s) exp(x_u - m_s),   m = max m_s
 // Inside a row the order of scores is the order of logits, so a slice compares logits, as they are, and tokens (64-bit keys: ordered bits of the logit, then the lower
-// token); beams are compared in 64 bits by scores + (x - log-sum).
+// token), and so does the merge; beams are compared in 64 bits by scores + (x - log-sum).
 // Four beams of 32000 fp32 logits take 9.0 us (0.08 of bytes), 256 rows of 128256 32.2 us (4.1 TB/s; 20.1 of bytes), 400 rows of 128256 bf16 50.6 us.  Bound: few rows, the
 // latency of two launches and of a slice's end (the looks at its chunks, about 4 us); many, the latency of a warp's chunk - copy, maximum, sum - with 16 to 24 warps an SM, and a
 // 16-bit row the instructions of a logit.  Twice the bytes in flight a warp leaves two CTAs an SM: 160 rows 32.2 for 24.2 us.
@@ -331,21 +331,23 @@ __global__ void __launch_bounds__(BM_THREADS, 4) k_beam_slice(const BeamArgs a) 
 	}
 }
 
+// A candidate's score and, as one number that is higher for what comes first among equal scores, its beam, its logit and its token: of one beam the higher logit comes first
+// also where 64 bits do not tell the scores apart (a logit of 1e-20 and one of 2e-20 beside a maximum of 5).
 struct BeamCand {
 	double d[BM_CAND];
-	uint32_t i[BM_CAND];
+	u64 i[BM_CAND];
 };
-__device__ __forceinline__ bool above(double d, uint32_t i, double e, uint32_t j) { return d > e || (d == e && i < j); }
+__device__ __forceinline__ bool above(double d, u64 i, double e, u64 j) { return d > e || (d == e && i > j); }
 
 __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	extern __shared__ __align__(16) unsigned char merge_sm[];
 	BeamCand& cand = *reinterpret_cast<BeamCand*>(merge_sm);
 	__shared__ double log_sum[BM_MAX], head_d[BM_THREADS];
 	__shared__ float row_max[BM_MAX];
-	__shared__ uint32_t head_i[BM_THREADS];
+	__shared__ u64 head_i[BM_THREADS];
 	__shared__ int count;
 	__shared__ double bound_d[BM_THREADS / 64];
-	__shared__ uint32_t bound_i[BM_THREADS / 64];
+	__shared__ u64 bound_i[BM_THREADS / 64];
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = blockIdx.x, n = a.n, K = a.beams, S = a.slices, lists = K * S;
 	if (tid == 0) count = 0;
 	pdl_wait_prev();
@@ -365,14 +367,14 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	}
 	__syncthreads();
 	const u64* const keys = a.keys + (size_t)g * lists * n;
-	auto value = [&](int list, int at, double& d, uint32_t& i) { // candidate `at` of a list; false: there is none
-		const u64 k = keys[(size_t)list * n + at];
+	const int bits = 32 - __clz(a.vocab - 1); // of a token; beams and tokens have 28 together at most
+	auto value = [&](int list, u64 k, double& d) { // a candidate of a list; false: it is none
 		const int b = list / S;
 		const float x = order_value((uint32_t)(k >> 32)), m = row_max[b];
 		d = (double)a.scores[g * K + b] + ((x == m ? 0. : (double)x - (double)m) - log_sum[b]);
-		i = (uint32_t)b * (uint32_t)a.vocab + ~(uint32_t)k;
 		return k != 0 && d > -INFINITY;
 	};
+	auto place = [&](int list, u64 k) { return (u64)(K - 1 - list / S) << (32 + bits) | k >> 32 << bits | (uint32_t)(a.vocab - 1 - (int)~(uint32_t)k); };
 	// Lists are in order.  Of the values at one depth of all lists the r-th highest, r (depth + 1) >= n, has n values at or above it; at the least such depth at most r lists reach
 	// it there, so what is at or above it is at most r n values and the others' first `depth`: n lists' worth.  Where lists are few, other threads look at twice that depth, four
 	// times, ...: the highest of the bounds leaves far fewer (64 lists of 64 values: the lowest list's head bounds nothing).
@@ -380,10 +382,11 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	while (width < lists) width *= 2;
 	const int set = tid / width, list = tid % width, depth = ((n + lists - 1) / lists << set) - 1, r = (n + depth) / (depth + 1);
 	double d = 0.;
-	uint32_t i = 0;
-	const bool have = list < lists && depth < n && value(list, depth, d, i);
-	head_d[tid] = have ? d : -INFINITY, head_i[tid] = have ? i : 0xffffffffu;
-	if (list == 0) bound_d[set] = -INFINITY, bound_i[set] = 0xffffffffu; // fewer than r lists reach the depth: everything
+	const u64 head = list < lists && depth < n ? keys[list * n + depth] : 0;
+	const bool have = value(min(list, lists - 1), head, d);
+	u64 i = have ? place(list, head) : 0;
+	head_d[tid] = have ? d : -INFINITY, head_i[tid] = i;
+	if (list == 0) bound_d[set] = -INFINITY, bound_i[set] = 0; // fewer than r lists reach the depth: everything
 	__syncthreads();
 	if (have) {
 		int rank = 0;
@@ -393,22 +396,35 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_merge(const BeamArgs a) {
 	}
 	__syncthreads();
 	double low_d = bound_d[0];
-	uint32_t low_i = bound_i[0];
+	u64 low_i = bound_i[0];
 	for (int k = 1; k < BM_THREADS / width; ++k)
 		if (above(bound_d[k], bound_i[k], low_d, low_i)) low_d = bound_d[k], low_i = bound_i[k];
-	for (int e = tid; e < lists * n; e += BM_THREADS)
-		if (value(e / n, e % n, d, i) && !above(low_d, low_i, d, i)) {
-			const int at = atomicAdd(&count, 1);
-			if (at < BM_CAND) cand.d[at] = d, cand.i[at] = i;
+	for (int e0 = tid; e0 < lists * n; e0 += 4 * BM_THREADS) {
+		u64 k[4];
+#pragma unroll
+		for (int u = 0; u < 4; ++u) k[u] = e0 + u * BM_THREADS < lists * n ? keys[e0 + u * BM_THREADS] : 0;
+#pragma unroll
+		for (int u = 0; u < 4; ++u) {
+			if (e0 - tid + u * BM_THREADS >= lists * n) break;
+			const int from = min((e0 + u * BM_THREADS) / n, lists - 1);
+			if (value(from, k[u], d) && d >= low_d && (d > low_d || place(from, k[u]) >= low_i)) {
+				const int at = atomicAdd(&count, 1);
+				if (at < BM_CAND) cand.d[at] = d, cand.i[at] = place(from, k[u]);
+			}
 		}
+	}
 	__syncthreads();
 	const int c = min(count, BM_CAND), base = g * n;
 	for (int e = tid; e < c; e += BM_THREADS) {
 		d = cand.d[e], i = cand.i[e];
 		int rank = 0;
 #pragma unroll 8
-		for (int k = 0; k < c; ++k) rank += above(cand.d[k], cand.i[k], d, i);
-		if (rank < n) a.tokens[base + rank] = (int)(i % (uint32_t)a.vocab), a.parents[base + rank] = (int)(i / (uint32_t)a.vocab), a.best[base + rank] = (float)d;
+		for (int k = 0; k < c; ++k) {
+			const double o = cand.d[k];
+			rank += o > d;
+			if (o == d && k != e) rank += cand.i[k] > i; // (seldom)
+		}
+		if (rank < n) a.tokens[base + rank] = a.vocab - 1 - (int)(i & ((1ull << bits) - 1)), a.parents[base + rank] = K - 1 - (int)(i >> (32 + bits)), a.best[base + rank] = (float)d;
 	}
 	for (int e = c + tid; e < n; e += BM_THREADS) a.tokens[base + e] = a.parents[base + e] = -1, a.best[base + e] = -INFINITY;
 }

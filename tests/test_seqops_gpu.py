@@ -609,3 +609,22 @@ def test_sinks_that_are_infinite(seqs, tokens, before, dtype):
 def test_beams_of_no_groups():
     tok, par, best = seqops.beam_select(torch.zeros(0, 3, 50, device="cuda"), torch.zeros(0, 3, device="cuda"), 4)
     assert tok.shape == par.shape == best.shape == (0, 4)
+
+
+def test_tokens_of_one_beam_come_in_their_logits_order():
+    """Logits whose difference is lost beside the row's maximum, or beside the beam's score, in 64 bits: n = 1, 2, ... continuations are prefixes of one order, in and across slices."""
+    V = 20000
+    x = torch.full((1, 3, V), -50.0, device="cuda")
+    x[0, 0, 7] = 5.0
+    low = torch.tensor([3, 19000, 9000, 4, 12000, 18999], device="cuda")
+    x[0, 0, low] = torch.arange(1, 7, device="cuda") * 1e-20
+    x[0, 1:, :8] = torch.arange(8, device="cuda") * 2.0 ** -24 - 0.25  # (fp32 holds the steps, a score of -2^40 beside them does not)
+    s = torch.tensor([[-1.0, -2.0 ** 40, -2.0 ** 40]], device="cuda")
+    want = [7] + low.flip(0).tolist()
+    for n in range(1, 8):
+        tok, par, _ = seqops.beam_select(x, s, n)
+        assert tok[0].tolist() == want[:n] and (par == 0).all(), (n, tok)
+    s[0, 0] = -math.inf
+    for n in range(1, 17):
+        tok, par, _ = seqops.beam_select(x, s, n)
+        assert tok[0].tolist() == (2 * list(range(7, -1, -1)))[:n] and par[0].tolist() == (8 * [1] + 8 * [2])[:n], (n, tok, par)
