@@ -214,6 +214,15 @@ __device__ __noinline__ int slice_best(BeamSlice& b, const float* tops, int tile
 	return keys > BM_KEYS ? slow_tiles<T>(b, base, begin, end, shift, total, n) : keep_best(b, keys, n);
 }
 
+// After a wait that gave up: waits, bounded again, for the copies in flight - of this tile and of those requested ahead - before their memory becomes something else.
+template <int STAGES>
+__device__ __noinline__ void beam_drain(uint64_t* full, int stage, uint32_t parity, unsigned at, unsigned end, unsigned step) {
+	for (int k = 0; k < STAGES && at < end; ++k, at += step) {
+		mbar_wait_warp(full + stage, parity);
+		if (++stage == STAGES) stage = 0, parity ^= 1;
+	}
+}
+
 // Per logit: a maximum, a difference, a product, an exponential, an addition (with a fused multiply-add against the maximum times log2(e) a row of the type's lowest values, whose
 // product is infinite, would have no sum); per chunk one value kept.  No barrier between warps until the slice has been read.
 constexpr float BM_L2E = 1.4426950408889634f;
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__(BM_THREADS, 4) k_beam_slice(const BeamArgs a) 
 		{
 			uint4 w[NV];
 			if (v0 + warp * WSTEP < end && !lost) {
-				lost = !mbar_wait_warp(full + stage, parity);
+				if (!mbar_wait_warp(full + stage, parity)) lost = true, beam_drain<STAGES>(full, stage, parity, v0 + warp * WSTEP, end, STEP);
 				const uint4* const src = reinterpret_cast<const uint4*>(b.ring[warp] + stage * (NV * 512)) + lane;
 #pragma unroll
 				for (int j = 0; j < NV; ++j) w[j] = src[j * 32];
@@ -310,7 +319,6 @@ __global__ void __launch_bounds__(BM_THREADS, 4) k_beam_slice(const BeamArgs a) 
 		}
 		s += sum;
 	}
-	if (lost) mbar_wait_bounded(full + stage, parity); // (a copy that comes late lands in memory that is still the block's)
 	const float wm = warp_max(m);
 	if (lane == 0) b.red[warp] = wm;
 	const bool broken = __syncthreads_or(lost);

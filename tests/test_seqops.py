@@ -160,3 +160,35 @@ def test_a_batch_without_groups():
     for beams in (1, 4, 64):
         assert L.calm_b200_seq_beam_workspace(0, beams, 100, 3) == 0 and beam(groups=0, beams=beams) == 0
     says(beam(groups=0, beams=65), "beam", "64")
+
+
+def test_a_slice_that_gives_up_waits_for_every_copy_that_it_asked_for():
+    """k_beam_slice: a warp that gives up on a tile has the copies of that tile and of the stages behind it in flight, into memory that the block uses for other things next."""
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "calm_b200", "csrc", "seqbeam.cu")).read()
+    drain = src[src.index("void beam_drain("):]
+    drain = drain[:drain.index("\n}\n")]
+    assert "for (int k = 0; k < STAGES && at < end; ++k, at += step) {\n\t\tmbar_wait_warp(full + stage, parity);\n\t\tif (++stage == STAGES) stage = 0, parity ^= 1;" in drain
+    loop = src[src.index("bool lost = false;"):]
+    loop = loop[:loop.index("\n\t}\n")]
+    gave_up = loop.index("if (!mbar_wait_warp(full + stage, parity)) lost = true, beam_drain<STAGES>(full, stage, parity, v0 + warp * WSTEP, end, STEP);")
+    assert gave_up < loop.index("if (lane == 0 && !lost) request(stage);") and "&& !lost)" in loop[:gave_up]
+    # the loop's requests and the drain's waits, tile by tile
+    for stages in (2, 4):
+        for tiles in range(1, 12):
+            for lost in range(tiles):
+                asked, done = set(range(min(stages, tiles))), set()
+                for i in range(lost):
+                    done.add(i)
+                    if i + stages < tiles:
+                        asked.add(i + stages)
+                stage, parity, waited = lost % stages, lost // stages & 1, set()
+                for k in range(stages):
+                    if lost + k >= tiles:
+                        break
+                    t = lost + k
+                    assert (stage, parity) == (t % stages, t // stages & 1)
+                    waited.add(t)
+                    stage += 1
+                    if stage == stages:
+                        stage, parity = 0, parity ^ 1
+                assert waited == asked - done
