@@ -628,3 +628,22 @@ def test_tokens_of_one_beam_come_in_their_logits_order():
     for n in range(1, 17):
         tok, par, _ = seqops.beam_select(x, s, n)
         assert tok[0].tolist() == (2 * list(range(7, -1, -1)))[:n] and par[0].tolist() == (8 * [1] + 8 * [2])[:n], (n, tok, par)
+
+
+@pytest.mark.parametrize("vocab", [97, 32000, 128256])
+def test_beams_that_lie_just_apart(vocab):
+    """Two beams with the same logits in different places, their scores further apart than the two log-sums' bounds: every candidate of the higher beam comes before the other's same one."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    row = torch.randn(vocab, generator=g, device="cuda") * 3
+    row[:8] = 20.0 + torch.arange(8, device="cuda")
+    for seed in range(8):
+        g.manual_seed(seed)
+        place = [torch.randperm(vocab, generator=g, device="cuda") for _ in range(2)]
+        x = torch.stack([row[p] for p in place])[None]
+        apart = 2.02 * (2.0 ** -22 + (25 + math.ceil(vocab / 4096)) * 2.0 ** -24)  # what is documented, and a little
+        for high in (0, 1):
+            s = torch.zeros(1, 2, device="cuda")
+            s[0, 1 - high] = -apart
+            tok, par, _ = seqops.beam_select(x, s, 16)
+            assert par[0].tolist() == [high, 1 - high] * 8
+            assert [int(place[p][t]) for t, p in zip(tok[0].tolist(), par[0].tolist())] == [i for i in range(7, -1, -1) for _ in range(2)]
