@@ -647,3 +647,19 @@ def test_beams_that_lie_just_apart(vocab):
             tok, par, _ = seqops.beam_select(x, s, 16)
             assert par[0].tolist() == [high, 1 - high] * 8
             assert [int(place[p][t]) for t, p in zip(tok[0].tolist(), par[0].tolist())] == [i for i in range(7, -1, -1) for _ in range(2)]
+
+
+def test_pages_of_an_8_bit_cache_are_copied_whole():
+    """Their second axis is heads, not tokens: a copy of a page's first rows is refused, alone and beside a wide cache, and nothing is copied then."""
+    c = Cached(1, 6, 3, 8, 32, 5)
+    wide = torch.randn(8, 8, 4, device="cuda")
+    for pool in (seqops.UnitPool(c.cache.buffers()), seqops.UnitPool([wide] + c.cache.buffers())):
+        before = [x.clone() for x in (wide, c.codes, c.scales)]
+        with pytest.raises(ValueError, match="rows"):
+            pool.copy(pages=([0], [1], [3]))
+        assert all(torch.equal(x, y) for x, y in zip(before, (wide, c.codes, c.scales)))
+        pool.copy(pages=([0, 2], [1, 3]))
+        for t in (*c.codes, *c.scales):
+            assert torch.equal(t[0], t[1]) and torch.equal(t[2], t[3])
+    assert torch.equal(wide[0], wide[1]) and torch.equal(wide[2], wide[3])
+    assert all(x.shape[0] == 0 for x in seqops.Cache8.empty(0, 3, 8, 32).buffers())
