@@ -214,6 +214,8 @@ class SeqDeviceModel:
 
     def fork(self, slot: int, n: int) -> List[int]:
         """n more sequences that go on from what `slot` holds (which stays open)."""
+        if n < 0:
+            raise SeqError(f"bad branch: {n} more sequences")
         return self.branch([slot], [0] * (n + 1))[1:]
 
     def resize(self, max_tokens: int) -> None:

@@ -192,3 +192,28 @@ def test_a_slice_that_gives_up_waits_for_every_copy_that_it_asked_for():
                     if stage == stages:
                         stage, parity = 0, parity ^ 1
                 assert waited == asked - done
+
+
+def test_a_fork_into_fewer_than_no_sequences_is_refused():
+    """It would be a branch without children, which closes the sequence."""
+    from calm_b200 import seqlib
+
+    asked = []
+
+    class Model(seqlib.SeqDeviceModel):
+        def __init__(self):
+            pass
+
+        def branch(self, slots, parents):
+            asked.append((list(slots), list(parents)))
+            return list(range(len(parents)))
+
+        def __del__(self):
+            pass
+
+    m = Model()
+    assert m.fork(3, 0) == [] and m.fork(3, 2) == [1, 2] and asked == [([3], [0]), ([3], [0, 0, 0])]
+    for n in (-1, -2, -100):
+        with pytest.raises(seqlib.SeqError, match="bad branch"):
+            m.fork(3, n)
+    assert len(asked) == 2
