@@ -117,7 +117,7 @@ class Scheduler:
                 every = self._sample([], len(slots), None)
                 toks = [every[k] for k in took]
             else:
-                toks = self._sample([live[i] for i in single], len(took), logits[took])
+                toks = self._sample([live[i] for i in single], len(took), logits[took] if beams else logits)  # (a choice of rows is a copy of them)
             for i, tok in zip(single, toks):
                 r = live[i]
                 r.out.append(tok)

@@ -177,3 +177,34 @@ def test_refused_requests():
     for kw in (dict(beams=0), dict(beams=65), dict(beams=33, eos=1), dict(beams=2, temperature=0.5), dict(beams=5)):
         with pytest.raises(ValueError):
             s.add(serving.Request("a", [1], 3, **kw))
+
+
+def test_sampled_batches_hand_the_steps_own_logits_on():
+    """Without beams every row is a request's: the array goes to the sampler as the step gave it, not a copy of a vocabulary a request; beside beams the rows are the requests'."""
+
+    class Sampled(serving.Scheduler):
+        def _sample(self, reqs, n, logits):
+            seen.append((len(reqs), n, logits is m.given[-1] if logits is not None else None, None if logits is None else np.array(logits)))
+            return [int(r.argmax()) for r in logits]
+
+    class Keeping(TextModel):
+        given = None
+
+        def step(self, *a, **kw):
+            out = super().step(*a, **kw)
+            self.given = (self.given or []) + [out]
+            return out
+
+    m, seen = Keeping(), []
+    s = Sampled(m)
+    for i in range(3):
+        s.add(serving.Request(str(i), [i, 4], 3, temperature=0.7))
+    s.run()
+    assert len(seen) == 3 and all(x[:3] == (3, 3, True) for x in seen)
+    m, seen = Keeping(), []
+    s = Sampled(m)
+    s.add(serving.Request("b", [5], 3, beams=2))
+    s.add(serving.Request("a", [7, 4], 3, temperature=0.7))
+    s.run()
+    assert [x[:3] for x in seen] == [(1, 1, False)] * 3
+    assert np.array_equal(seen[0][3][0], m.logits_of([7, 4])) and np.array_equal(seen[1][3][0], m.given[1][-1])
