@@ -205,6 +205,8 @@ class SeqDeviceModel:
     def branch(self, slots: Sequence[int], parents: Sequence[int]) -> List[int]:
         """Sequences that go on in several ways, or end: the slots of len(parents) sequences, the i-th going on from what slots[parents[i]] holds.  The first that names a
         parent keeps its slot, the others share its full pages; a sequence that is not named is closed."""
+        if not all(-2 ** 31 <= int(x) < 2 ** 31 for x in (*slots, *parents)):  # (numpy or ctypes would cut them off)
+            raise SeqError("bad branch: a number that passes 32 bits")
         sl, pa = np.ascontiguousarray(slots, np.int32), np.ascontiguousarray(parents, np.int32)
         out = np.zeros(max(1, len(pa)), np.int32)
         rc = self.lib.calm_b200_seq_branch(self.handle, len(sl), sl.ctypes.data_as(_iptr), len(pa), pa.ctypes.data_as(_iptr), out.ctypes.data_as(_iptr))
@@ -220,7 +222,7 @@ class SeqDeviceModel:
 
     def resize(self, max_tokens: int) -> None:
         """A cache for max_tokens live tokens from now on, smaller or larger; live sequences keep theirs."""
-        rc = self.lib.calm_b200_seq_resize(self.handle, int(max_tokens))
+        rc = self.lib.calm_b200_seq_resize(self.handle, int(max_tokens)) if int(max_tokens) < 2 ** 31 else -3
         if rc != 0:
             raise SeqError({-2: f"the live sequences hold more than {max_tokens} tokens", -4: "the device lacks the memory"}.get(rc, "max_tokens must be positive and within what the caches can hold"))
         self.desc.max_tokens = int(max_tokens)
@@ -254,8 +256,10 @@ class SeqDeviceModel:
         sc = np.ascontiguousarray(scores, np.float32)
         if sc.ndim != 2:
             raise ValueError("scores must be [groups, beams]")
+        if not 0 <= row0 < 2 ** 31 or not 1 <= n <= 64:
+            raise SeqError("bad beams: rows that the last step did not want, or beams or n outside 1 .. 64")
         G, K = sc.shape
-        tok, par, best = np.zeros((G, max(n, 1)), np.int32), np.zeros((G, max(n, 1)), np.int32), np.zeros((G, max(n, 1)), np.float32)
+        tok, par, best = np.zeros((G, n), np.int32), np.zeros((G, n), np.int32), np.zeros((G, n), np.float32)
         rc = self.lib.calm_b200_seq_beams(self.handle, row0, G, K, sc.ctypes.data_as(_fptr), n, tok.ctypes.data_as(_iptr), par.ctypes.data_as(_iptr), best.ctypes.data_as(_fptr))
         if rc != 0:
             raise SeqError("bad beams: rows that the last step did not want, or beams or n outside 1 .. 64")

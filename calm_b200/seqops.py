@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 from array import array
+from operator import index as index_of
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -100,6 +101,17 @@ def _gpu(name: str, t: torch.Tensor, index: int = -1) -> int:
     return at
 
 
+def _whole(name: str, value) -> int:
+    """A whole number that the library's 32 bits hold (ctypes would cut a larger one off)."""
+    try:
+        v = index_of(value)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number, not {value!r}") from None
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{name} = {v} passes 32 bits")
+    return v
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
     """The n best continuations of every group of beams: logits [groups, beams, vocab] (float32, bfloat16 or float16, the last axis contiguous), scores [groups,
     beams] float32 (-inf, or not finite: no beam there) -> tokens int32, parents int32, scores float32, each [groups, n], best first.  A candidate's score is its beam's plus the
@@ -112,9 +124,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, out: Optiona
     G, K, V = logits.shape
     if scores.shape != (G, K) or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError(f"scores must be contiguous float32 [{G}, {K}]")
-    L, n = _load(), int(n)
+    L, n = _load(), _whole("n", n)
+    for name, v in (("groups", G), ("beams", K), ("vocabulary", V)):
+        _whole(name, v)
     need = L.calm_b200_seq_beam_workspace(G, K, V, n)
-    if not need and G:
+    if not need and (G or not 1 <= n <= 64):
         _check(-3)
     if out is None:
         tokens, parents, best = torch.empty((3, G, n), dtype=torch.int32, device=logits.device).unbind(0)
@@ -218,7 +232,7 @@ def _rows(name: str, t: torch.Tensor, index: int, heads: int, dim: int, least: i
     n = t.shape[0]
     if n < least:
         raise ValueError(f"{name} has {n} rows for {least} tokens")
-    return _Rows(t.data_ptr(), kind, stride[0], stride[1], n)
+    return _Rows(t.data_ptr(), kind, stride[0], stride[1], min(n, 2 ** 31 - 1))
 
 
 class Cache8:
@@ -281,7 +295,7 @@ class Cache8:
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if rq.rows == batch.tokens else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         ro = _rows("out", out, index, heads, self.dim, rq.rows)
-        a = _Attend8(rq, ro, heads, scale, window, keep_first, chunk, softcap, None, None, None, 0, 0, 0, batch.most_keys, None, 0)
+        a = _Attend8(rq, ro, heads, scale, _whole("window", window), _whole("keep_first", keep_first), _whole("chunk", chunk), softcap, None, None, None, 0, 0, 0, batch.most_keys, None, 0)
         for name, t in (("sink", sink), ("slopes", slopes)):
             if t is not None:
                 _gpu(name, t, index)

@@ -217,3 +217,27 @@ def test_a_fork_into_fewer_than_no_sequences_is_refused():
         with pytest.raises(seqlib.SeqError, match="bad branch"):
             m.fork(3, n)
     assert len(asked) == 2
+
+
+def test_numbers_past_32_bits_are_refused_and_not_cut_off():
+    from calm_b200 import seqlib
+
+    for v in (2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1, 10 ** 30, 1.5, "3", None):
+        with pytest.raises(ValueError, match="window"):
+            seqops._whole("window", v)
+    assert [seqops._whole("n", v) for v in (0, -1, 2 ** 31 - 1, np.int64(7), True)] == [0, -1, 2 ** 31 - 1, 7, 1]
+
+    class Library:  # the library as it would answer what it is asked
+        def __getattr__(self, name):
+            return lambda *a: asked.append((name, a)) or 0
+
+    asked, m = [], seqlib.SeqDeviceModel.__new__(seqlib.SeqDeviceModel)
+    m.lib, m.handle, m.desc = Library(), None, type("D", (), {})()
+    for call in (lambda: m.resize(2 ** 32 + 100), lambda: m.branch([2 ** 32], [0]), lambda: m.branch(np.array([2 ** 32 + 1]), [0]), lambda: m.branch([0], np.array([-2 ** 32])),
+                 lambda: m.beams(np.zeros((1, 1), np.float32), 3, row0=2 ** 32), lambda: m.beams(np.zeros((1, 1), np.float32), 2 ** 32 + 1)):
+        with pytest.raises(seqlib.SeqError):
+            call()
+    assert not asked
+    m.resize(100), m.branch(np.array([1, 0]), [1, 1]), m.beams(np.zeros((1, 1), np.float32), 3, row0=1)
+    assert [a[0] for a in asked] == ["calm_b200_seq_resize", "calm_b200_seq_branch", "calm_b200_seq_beams"]
+    m.close = lambda: None

@@ -663,3 +663,19 @@ def test_pages_of_an_8_bit_cache_are_copied_whole():
             assert torch.equal(t[0], t[1]) and torch.equal(t[2], t[3])
     assert torch.equal(wide[0], wide[1]) and torch.equal(wide[2], wide[3])
     assert all(x.shape[0] == 0 for x in seqops.Cache8.empty(0, 3, 8, 32).buffers())
+
+
+def test_whole_numbers_that_pass_32_bits_are_refused():
+    c = Cached(1, 4, 1, 16, 64, 5)
+    q, b = torch.zeros(1, 2, 64, device="cuda"), seqops.Batch([0], [1], [30])
+    for name in ("window", "keep_first", "chunk"):
+        for v in (2 ** 32 + 5, -1, 1.5):
+            with pytest.raises(ValueError, match=name):
+                c.cache.attend(q, c.dtable, b, 0.1, **{name: v})
+    x, s = torch.zeros(1, 2, 8, device="cuda"), torch.zeros(1, 2, device="cuda")
+    for n in (2 ** 32 + 3, 0, 65, -1, 2.5):
+        for groups in (1, 0):
+            with pytest.raises(ValueError, match="n"):
+                seqops.beam_select(x[:groups], s[:groups], n)
+    with pytest.raises(ValueError, match="vocabulary"):
+        seqops.beam_select(torch.empty(1, 1, 2 ** 32 + 5, dtype=torch.bfloat16, device="cuda"), s[:, :1].contiguous(), 2)
