@@ -480,6 +480,7 @@ extern "C" int calm_b200_seq_beam_select(const struct SeqBeam* q, void* stream) 
 	if (q->groups == 0) return 0;
 	if (!q->logits || !q->scores || !q->tokens || !q->parents || !q->best || !q->workspace) return refuse("beam: a pointer is missing");
 	if ((uintptr_t)q->logits % type_size(q->type)) return refuse("beam: the logits are not aligned to their type");
+	if (((uintptr_t)q->scores | (uintptr_t)q->tokens | (uintptr_t)q->parents | (uintptr_t)q->best) % 4) return refuse("beam: scores or results are not aligned to 4 bytes");
 	if ((uintptr_t)q->workspace % 16) return refuse("beam: the workspace is not aligned to 16 bytes");
 	if (q->workspace_bytes < calm_b200_seq_beam_workspace(q->groups, q->beams, q->vocab, q->n)) return refuse("beam: the workspace has %zu bytes, %zu are needed", q->workspace_bytes, calm_b200_seq_beam_workspace(q->groups, q->beams, q->vocab, q->n));
 	BeamArgs a;

@@ -1152,6 +1152,7 @@ int check_cache(const char* what, const SeqCache8* q, const SeqPortions* p) {
 	if (q->pages && (!q->k || !q->v || !q->k_scale || !q->v_scale)) return refuse("%s: the cache has no memory", what);
 	if (q->slots > 0 && q->table_pages > 0 && !q->table) return refuse("%s: the page table is missing", what);
 	if (((uintptr_t)q->k | (uintptr_t)q->v) % 16) return refuse("%s: codes are not aligned to 16 bytes", what);
+	if (((uintptr_t)q->table | (uintptr_t)p->start | (uintptr_t)p->count | (uintptr_t)p->slot | (uintptr_t)p->pos0) % 4) return refuse("%s: the page table or the batch's description is not aligned to 4 bytes", what);
 	if (((uintptr_t)q->k_scale | (uintptr_t)q->v_scale) % 4) return refuse("%s: scales are not aligned to 4 bytes", what);
 	return 0;
 }
@@ -1223,6 +1224,7 @@ int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) 
 	if (a->heads > 65535) return refuse("attend8: at most 65535 query heads");
 	if (a->out.type != a->q.type && !(a->q.type == SEQ_F32 && a->out.type == SEQ_BF16)) return refuse("attend8: out has type %d, q %d", a->out.type, a->q.type);
 	if (a->out.rows < a->q.rows) return refuse("attend8: out has %d rows, q %d", a->out.rows, a->q.rows);
+	if (((uintptr_t)a->sinks | (uintptr_t)a->slopes | (uintptr_t)a->gate) % 4) return refuse("attend8: sinks, slopes or gate are not aligned to 4 bytes");
 	if (!(a->scale == a->scale) || a->window < 0 || a->keep_first < 0 || a->chunk < 0 || !(a->softcap >= 0.f)) return refuse("attend8: scale, window, keep_first, chunk or softcap out of range");
 	return 0;
 }

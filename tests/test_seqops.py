@@ -241,3 +241,15 @@ def test_numbers_past_32_bits_are_refused_and_not_cut_off():
     m.resize(100), m.branch(np.array([1, 0]), [1, 1]), m.beams(np.zeros((1, 1), np.float32), 3, row0=1)
     assert [a[0] for a in asked] == ["calm_b200_seq_resize", "calm_b200_seq_branch", "calm_b200_seq_beams"]
     m.close = lambda: None
+
+
+def test_pointers_that_a_kernel_could_not_read_through_are_refused():
+    """Four bytes at an odd address are a fault on the device."""
+    for name in ("scores", "tokens", "parents", "best"):
+        says(beam(**{name: 4098}), "beam", "aligned")
+    store = lambda c, p: L.calm_b200_seq_cache8_store(C.byref(c), C.byref(p), C.byref(rows()), C.byref(rows()), None)
+    for c, p in [(cache8(table=4097), portions())] + [(cache8(), portions(**{name: 4098})) for name in ("start", "count", "slot", "pos0")]:
+        says(store(c, p), "store8", "aligned")
+        says(L.calm_b200_seq_attend8(*attend(c=c, p=p), None), "attend8", "aligned")
+    for name in ("sinks", "slopes", "gate"):
+        says(L.calm_b200_seq_attend8(*attend(**{name: 4099}), None), "attend8", "aligned")
