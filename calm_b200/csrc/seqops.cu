@@ -153,8 +153,9 @@ int copy_units(int n_pools, const SeqUnits* pools, int np, const int* pf, const 
 		if (u.unit_bytes < 0 || u.row_bytes < 0 || u.row_bytes > u.unit_bytes || u.src_units < 0 || u.dst_units < 0) return refuse("copy: pool %d has negative sizes, or rows wider than its units", i);
 		if (pairs && u.unit_bytes && (!u.src || !u.dst)) return refuse("copy: pool %d has no memory", i);
 		if (u.unit_bytes > (1LL << 38)) return refuse("copy: units of pool %d are larger than 256 GB", i);
-		const char *s0 = (const char*)u.src, *d0 = (const char*)u.dst;
-		if (s0 != d0 && s0 < d0 + u.unit_bytes * u.dst_units && d0 < s0 + u.unit_bytes * u.src_units) return refuse("copy: source and destination of pool %d overlap", i);
+		const uintptr_t s0 = (uintptr_t)u.src, d0 = (uintptr_t)u.dst;
+		const unsigned __int128 sn = (unsigned __int128)u.unit_bytes * u.src_units, dn = (unsigned __int128)u.unit_bytes * u.dst_units; // (units that are not used may be named beyond what 64 bits count)
+		if (s0 != d0 && s0 < d0 + dn && d0 < s0 + sn) return refuse("copy: source and destination of pool %d overlap", i);
 		bool known = false; // pools of one shape are checked once
 		for (int j = 0; j < i && !known; ++j)
 			known = pools[j].kind == u.kind && pools[j].src_units == u.src_units && pools[j].dst_units == u.dst_units && (pools[j].src == pools[j].dst) == (u.src == u.dst);

@@ -253,3 +253,9 @@ def test_pointers_that_a_kernel_could_not_read_through_are_refused():
         says(L.calm_b200_seq_attend8(*attend(c=c, p=p), None), "attend8", "aligned")
     for name in ("sinks", "slopes", "gate"):
         says(L.calm_b200_seq_attend8(*attend(**{name: 4099}), None), "attend8", "aligned")
+
+
+def test_pools_that_overlap_are_found_whatever_their_size():
+    for unit, n in ((1 << 38, 1 << 26), (1 << 38, (1 << 26) + 1), (1 << 36, 1 << 27), (1 << 38, 2 ** 31 - 1)):
+        says(copy([(4096, 4096 + 64, unit, 0, n, n, 0)], ([0], [1])), "copy", "overlap")
+        says(copy([(4096 + 64, 4096, unit, 0, n, n, 1)], slots=([0], [1])), "copy", "overlap")
