@@ -1222,6 +1222,7 @@ int check_attend(const SeqCache8* c, const SeqPortions* p, const SeqAttend8* a) 
 	if (const int rc = check_rows("attend8", "out", a->out)) return rc;
 	if (a->heads < 1 || a->heads % c->heads) return refuse("attend8: %d query heads over %d key heads", a->heads, c->heads);
 	if (a->heads > 65535) return refuse("attend8: at most 65535 query heads");
+	if ((long long)p->longest * (a->heads / c->heads) > INT_MAX - 256) return refuse("attend8: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence", p->longest, a->heads / c->heads);
 	if (a->out.type != a->q.type && !(a->q.type == SEQ_F32 && a->out.type == SEQ_BF16)) return refuse("attend8: out has type %d, q %d", a->out.type, a->q.type);
 	if (a->out.rows < a->q.rows) return refuse("attend8: out has %d rows, q %d", a->out.rows, a->q.rows);
 	if (((uintptr_t)a->sinks | (uintptr_t)a->slopes | (uintptr_t)a->gate) % 4) return refuse("attend8: sinks, slopes or gate are not aligned to 4 bytes");

@@ -259,3 +259,13 @@ def test_pools_that_overlap_are_found_whatever_their_size():
     for unit, n in ((1 << 38, 1 << 26), (1 << 38, (1 << 26) + 1), (1 << 36, 1 << 27), (1 << 38, 2 ** 31 - 1)):
         says(copy([(4096, 4096 + 64, unit, 0, n, n, 0)], ([0], [1])), "copy", "overlap")
         says(copy([(4096 + 64, 4096, unit, 0, n, n, 1)], slots=([0], [1])), "copy", "overlap")
+
+
+def test_more_pairs_of_token_and_head_than_are_counted_are_refused():
+    """Rows of a sequence are numbered in 31 bits: 2^30 tokens of 36 heads came out as a grid of an eighth of them."""
+    for longest, heads in ((1 << 30, 72), (2 ** 31 - 1, 4), (1 << 26, 64)):
+        a = attend(p=portions(longest=longest), heads=heads)
+        says(L.calm_b200_seq_attend8(*a, None), "attend8", "pairs")
+        assert L.calm_b200_seq_attend8_workspace(*a) == 0
+    for longest, heads in ((1 << 29, 4), (2 ** 31 - 300, 2)):
+        assert L.calm_b200_seq_attend8(*attend(p=portions(longest=longest, n=0, start=None), heads=heads), None) == 0
