@@ -211,6 +211,8 @@ def main(argv=None) -> int:
     ap.add_argument("--length-penalty", type=float, default=1.0, help="exponent of a hypothesis's length in its score")
     ap.add_argument("--cache-bits", type=int, default=32, choices=[8, 32], help="8: grouped-query layers cache keys and values in 8 bits")
     a = ap.parse_args(argv)
+    if a.beams < 1:
+        ap.error("--beams must be at least 1")
     from . import registry
 
     prompts = [[int(x) for x in p.split(",")] for p in a.tokens]

@@ -208,3 +208,11 @@ def test_sampled_batches_hand_the_steps_own_logits_on():
     s.run()
     assert [x[:3] for x in seen] == [(1, 1, False)] * 3
     assert np.array_equal(seen[0][3][0], m.logits_of([7, 4])) and np.array_equal(seen[1][3][0], m.given[1][-1])
+
+
+def test_the_command_line_refuses_a_number_of_beams_that_is_none(capsys):
+    """Before a model of no tokens and no slots is prepared, which ends the process."""
+    for beams in ("0", "-2"):
+        with pytest.raises(SystemExit) as e:
+            serving.main(["nowhere", "--tokens", "1,2", "--beams", beams])
+        assert e.value.code == 2 and "--beams" in capsys.readouterr().err
