@@ -639,9 +639,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86).
 constexpr int AP_KEYS = 64, C8_NONE = -1000;
 // Value scales that go through the products together lie within 2^AP_NEAR; a tile whose scales lie further apart comes several times, each time with the keys of one such range.  Codes
-// stay exact in units of the largest scale.  Where a row may not see the key that has it, the row's reference goes by what it sees, weights times their keys' own scales (AP_NEAR more
-// than AT_SET is still under AT_MOST): what is rounded as a subnormal is 2^-35 of the largest weight times the largest scale that the row sees.
+// stay exact in units of the largest scale.  Where a row may not see the key that has it, the row's weights would stand as many bits lower as the tile's scales lie apart: references
+// are set that much lower there (AT_SET + AP_NEAR is still under AT_MOST).  So what is rounded as a subnormal is 2^-35 of the largest weight times the largest scale that the row sees.
 constexpr int AP_NEAR = 4;
+static_assert(AP_NEAR < 8 && AT_SET + AP_NEAR < AT_MOST, "three bits; references that are set do not move at once");
 constexpr int ap_groups(bool split) { return split ? 1 : 2; } // of 128 rows
 constexpr int ap_threads(bool split) { return 256 * ap_groups(split) + 32; }
 __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
@@ -655,10 +656,9 @@ struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	unsigned char k[STAGES][PANELS][AP_KEYS * 128];
 	unsigned char v[STAGES][D * 128];
 	float factor[STAGES][AP_KEYS]; // of a tile's keys on their scores, in log2
-	alignas(16) float lower[STAGES][AP_KEYS]; // log2 of their value scales against the largest, where they differ
-	float bias[STAGES];            // log2 of the largest of the tile's value scales: its values come in units of that
+	int units[STAGES]; // 8 times log2 of the largest of the tile's value scales, in units of which its values come, plus that many bits that they lie apart (one number: a register)
 	uint32_t seen[STAGES][2];      // keys that are there
-	int tile[STAGES], last[STAGES], even[STAGES]; // which 64 keys; whether nothing comes behind them; whether their value scales are one
+	int tile[STAGES], last[STAGES]; // which 64 keys; whether nothing comes behind them
 	uint64_t kv_full[STAGES], kv_empty[STAGES], s_full[GROUPS][2], p_full[GROUPS], p_empty[GROUPS], done;
 	uint32_t tmem;
 	int tops[4 * GROUPS], least[4 * GROUPS]; // exponents of the queries: the largest and the smallest row of a warp's
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			last = s.last[st];
 			const uint32_t seen[2] = {s.seen[st][0], s.seen[st][1]};
 			const bool all = (seen[0] & seen[1]) == 0xffffffffu && j0 >= sp.kept && position(j0) >= wide && position(j0 + AP_KEYS - 1) <= sp.first;
-			const float bias = s.bias[st];
+			const int units = s.units[st];
 			const float base = m == -INFINITY ? 0.f : m, most = m == -INFINITY ? -INFINITY : AT_MOST;
 			float z[64], top = -INFINITY; // log2 of the weights against the reference as it stands (against 0 before there is one)
 			tmem_ld32(scores_at, *reinterpret_cast<float(*)[32]>(z));
@@ -823,7 +823,8 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 					z[k] = x.x, z[k + 1] = x.y;
 				}
 			}
-			const u64 off = pair_of(bias - base, bias - base);
+			const float lift = (float)(units >> 3) - base;
+			const u64 off = pair_of(lift, lift);
 #pragma unroll
 			for (int k = 0; k < 64; k += 4) {
 				const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s.factor[st] + k);
@@ -842,16 +843,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			for (int k = 0; k < 64; k += 2) tops[k / 2 % 4] = fmaxf(fmaxf(tops[k / 2 % 4], z[k]), z[k + 1]);
 			top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 			if (__any_sync(0xffffffffu, top > most)) { // references move
-				const bool moves = top > most;
-				if (!all && !s.even[st]) {
-					top = -INFINITY;
-#pragma unroll
-					for (int k = 0; k < 64; k += 4) {
-						const float4 u = *reinterpret_cast<const float4*>(s.lower[st] + k);
-						top = fmaxf(fmaxf(top, fmaxf(z[k] + u.x, z[k + 1] + u.y)), fmaxf(z[k + 2] + u.z, z[k + 3] + u.w));
-					}
-				}
-				const float mn = moves ? base + top - AT_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
+				const float set = all ? AT_SET : AT_SET + (float)(units & 7), mn = top > most ? base + top - set : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = base - (mn == -INFINITY ? 0.f : mn);
 #pragma unroll
 				for (int k = 0; k < 64; ++k) z[k] += by;
 				m = mn, l *= f;
@@ -874,7 +866,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			tmem_st32(scores_at, hi); // where the scores were
 			if (SPLIT) tmem_st32(scores_at + 32, rest);
 			const float2 sums = halves(sum);
-			l = fmaf(sums.x + sums.y, pow2f(-(int)bias), l); // the weights hold the value scale
+			l = fmaf(sums.x + sums.y, pow2f(-(units >> 3)), l); // the weights hold the value scale
 			tmem_st_wait();
 			if (i > 0 && !ap_wait_warp(s.p_empty + group, (i - 1) & 1, &s.lost)) break; // (long done: the barrier's phases stay in step)
 			tc_fence_before();
@@ -983,21 +975,21 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 				*reinterpret_cast<uint4*>(to + ((odd ? at ^ 1 : at) << 4)) = odd ? hi : lo;
 				*reinterpret_cast<uint4*>(to + ((odd ? at : at ^ 1) << 4)) = odd ? lo : hi;
 			}
-			// values in units of the largest scale, a smaller one's shifted down, exactly
+			// values in units of the largest scale, a smaller one's shifted down, exactly; keys whose scales are far smaller are left for the next round
 			int e[2];
 #pragma unroll
 			for (int h = 0; h < 2; ++h) e[h] = have[h] ? max((exps[h] >> 23 & 255) - 127, -126) : C8_NONE;
 			int most = __reduce_max_sync(0xffffffffu, max(e[0], e[1]));
 			if (most == C8_NONE) most = 0;
 			const int least = __reduce_min_sync(0xffffffffu, min(e[0] == C8_NONE ? INT_MAX : e[0], e[1] == C8_NONE ? INT_MAX : e[1]));
-			const bool even = least >= most, more = least < most - AP_NEAR; // more: the keys with smaller scales come after these
+			const bool even = least >= most, more = least < most - AP_NEAR;
+			have[0] = have[0] && e[0] < most - AP_NEAR, have[1] = have[1] && e[1] < most - AP_NEAR;
 			if (t < AP_KEYS) {
 				const int own_e = own == 0 ? e[0] : e[1];
 				const uint32_t seen = __ballot_sync(0xffffffffu, own_e >= most - AP_NEAR);
 				if (lane == 0) s.seen[st][own] = seen;
-				if (!even) s.lower[st][t] = (float)(own_e - most);
 			}
-			if (t == 0) s.bias[st] = (float)most, s.even[st] = even, s.tile[st] = i, s.last[st] = i == tiles - 1 && !more;
+			if (t == 0) s.units[st] = most * 8 + (more ? AP_NEAR : even ? 0 : most - least), s.tile[st] = i, s.last[st] = i == tiles - 1 && !more;
 			if (mine != (1u << VKEYS) - 1) { // (a code that is no number would spoil rows that do not see it)
 #pragma unroll
 				for (int k = 0; k < VKEYS; ++k)
@@ -1040,8 +1032,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 			fence_async_smem();
 			__syncwarp();
 			if (lane == 0) mbar_arrive(s.kv_full + st);
-			if (more) have[0] = have[0] && e[0] < most - AP_NEAR, have[1] = have[1] && e[1] < most - AP_NEAR;
-			else if (++i < tiles) load(i);
+			if (!more && ++i < tiles) load(i);
 			if (++st == STAGES) st = 0, round ^= 1;
 		}
 	} else if (lane == 0) {
