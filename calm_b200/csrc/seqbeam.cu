@@ -6,8 +6,8 @@
 //   log sum_u exp x_u = m + log sum_s exp(m_s - m) S_s,   S_s = sum_(u in s) exp(x_u - m_s),   m = max m_s
 // Inside a row the order of scores is the order of logits, so a slice compares logits, as they are, and tokens (64-bit keys: ordered bits of the logit, then the lower
 // token), and so does the merge; beams are compared in 64 bits by scores + (x - log-sum).
-// Four beams of 32000 fp32 logits take 9.0 us (0.08 of bytes), 256 rows of 128256 32.2 us (4.1 TB/s; 20.1 of bytes), 400 rows of 128256 bf16 50.6 us.  Bound: few rows, the
-// latency of two launches and of a slice's end (the looks at its chunks, about 4 us); many, the latency of a warp's chunk - copy, maximum, sum - with 16 to 24 warps an SM, and a
+// Four beams of 32000 fp32 logits take 9.0 us (0.08 of bytes), 256 rows of 128256 32.2 us (4.1 TB/s; 20.1 of bytes), 400 rows of 128256 bf16 51.5 us.  Bound: few rows, the
+// latency of two launches and of a slice's end (the looks at its chunks, about 4 us); many, the latency of a warp's chunk - copy, maximum, sum - with 13.7 warps an SM in the mean (whole rows a CTA: two on 108 SMs, one on 40), and a
 // 16-bit row the instructions of a logit.  Twice the bytes in flight a warp leaves two CTAs an SM: 160 rows 32.2 for 24.2 us.
 #include "seqops.cuh"
 #include "tc05.cuh"

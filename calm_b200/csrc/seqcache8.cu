@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) k_c8_store(const C8 c, const St
 // channels x queries), so that eight rows of queries fill a product.  An e4m3 code is exact in fp16; scales do not enter the products: a key's scale multiplies its scores,
 // a value's scale s joins the exponent, w_j = 2^(z_j - r), z_j = log2(e) score_j + log2 s_j, where r keeps the weights that are rounded to fp16 at 2^15 or less; the denominator sums
 // w_j / s_j.  r moves (and the sums are rescaled) when a chunk's largest z passes it by 15, to 10 below that z: almost only in a warp's first chunks.
-// 64 tokens of 32 heads over 2000 to 8000 keys of 8 heads of 128 channels (656 MB): 125 us, 5.3 TB/s; one over 4000 keys 10.8 us.  Bound: with many CTAs issue and the latency of
+// 64 tokens of 32 heads over 2000 to 8000 keys of 8 heads of 128 channels (656 MB): 125 us, 5.3 TB/s; one over 4000 keys 11.1 us.  Bound: with many CTAs issue and the latency of
 // a warp's chunk (1.7 warp instructions a cycle; 49 million in all), with few the latency of copy, products, softmax and the cluster's fold.
 constexpr int AT_WARPS = 4, AT_KEYS = 32;
 constexpr int AT_SHARES = 64;  // of a tile's keys at most
@@ -634,7 +634,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, NQ * D <= 128 ? 4 : NQ * D <= 2
 // the weights (exponents, references and denominators as above) and write them back where the scores stood: the next product's operand.  O stays in tensor memory; it is rescaled
 // in the rare case that a row's reference moves.
 //   warps, in fours: softmax and output of each group; keys and values; a warp for the products
-// 1500 and 805 queries of 16 heads behind 700 and 376 keys of 128 channels, 148 CTAs: 76 us (one group a CTA and two CTAs an SM 86, with the weights through shared memory 95).  Bound: the way of a tile
+// 1500 and 805 queries of 16 heads behind 700 and 376 keys of 128 channels, 148 CTAs: 78 us (one group a CTA and two CTAs an SM 86, with the weights through shared memory 95).  Bound: the longest CTA, which
+// walks 35 tiles where the mean is 19.8, and the way of a tile
 // through its roles, about 3900 cycles, of which a softmax warp works 3000 (its exponentials keep the units busy for 1024 of them, the tensor cores are for about 1300); registers
 // hold 17 warps.  Not better: values freed apart from keys 93, loads two tiles ahead 84, four warps for keys and values 75 (92 with a cold L2 for 86).
 constexpr int AP_KEYS = 64, C8_NONE = -1000;
@@ -1087,7 +1088,7 @@ __global__ void __launch_bounds__(ap_threads(SPLIT), 1) k_c8_prompt(const C8 c, 
 	if (warp == 2 * WARPS) tmem_dealloc(tmem, 256 * GROUPS);
 }
 
-// Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.  9 us for 2048 rows of 6 shares: latency, launched while the shares still run.
+// Folds the shares of one (token, head), in share order: a warp for each, all of a lane's shares read at once.  9 us for 2048 rows of 6 shares: latency (the shares do not announce it early, so it starts when the last of them has ended).
 __global__ void __launch_bounds__(128) k_c8_fold(const C8 c, const Attend a) {
 	pdl_wait_prev();
 	const int b = blockIdx.z, kvh = blockIdx.y, n = c.count[b], p0 = c.pos0[b], start = c.start[b], slot = c.slot[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -29,15 +29,6 @@ int failed(const char* what, cudaError_t e) {
 	(void)cudaGetLastError(); // a launch that was turned down is not found again by the next call
 	return -4;
 }
-int sm_count() {
-	static std::atomic<int> known[64];
-	int dev = 0, n = 0;
-	if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-	if (dev < 64 && (n = known[dev].load()) > 0) return n;
-	if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
-	if (dev < 64) known[dev].store(n);
-	return n;
-}
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 uint64_t launches() { return g_launches.load(std::memory_order_relaxed); }
 

@@ -1,4 +1,4 @@
-// seqops.cuh -- what the operators on callers' device memory (seqbeam.cu, seqcopy.cu, seqcache8.cu; entry points in include/calm_b200_seq.h) share:
+// seqops.cuh -- what the operators on callers' device memory (seqops.cu, seqbeam.cu, seqcache8.cu; entry points in include/calm_b200_seq.h) share:
 // refusals that leave a message instead of ending the process, launches that report their error, element types.
 #pragma once
 
@@ -18,7 +18,6 @@ namespace seqops {
 int refuse(const char* fmt, ...);
 int failed(const char* what, cudaError_t e);
 
-int sm_count(); // of the current device
 void count_launch();
 uint64_t launches(); // since the library was loaded
 
