@@ -263,7 +263,7 @@ class Cache8:
 
     def buffers(self) -> List[torch.Tensor]:
         """The four tensors as page buffers of a UnitPool: views [pages, 1, ...], since a page's first tokens are not its front (heads come first) and pages are copied whole."""
-        return [t.view(self.pages, 1, n) for t, n in ((self.k, self.heads * self.page * self.dim), (self.k_scale, self.heads), (self.v, self.heads * self.page * self.dim), (self.v_scale, self.heads))]
+        return [t.unsqueeze(1) for t in (self.k, self.k_scale, self.v, self.v_scale)]
 
     def _with(self, table: torch.Tensor, batch: Batch) -> _Cache8:
         _gpu("the page table", table, self.index)

@@ -679,3 +679,9 @@ def test_whole_numbers_that_pass_32_bits_are_refused():
                 seqops.beam_select(x[:groups], s[:groups], n)
     with pytest.raises(ValueError, match="vocabulary"):
         seqops.beam_select(torch.empty(1, 1, 2 ** 32 + 5, dtype=torch.bfloat16, device="cuda"), s[:, :1].contiguous(), 2)
+
+
+def test_8_bit_pages_of_other_shapes_are_refused_as_a_destination():
+    a, b = seqops.Cache8.empty(4, 2, 16, 64), seqops.Cache8.empty(4, 2, 64, 16)  # as many bytes a page
+    with pytest.raises(ValueError, match="shape"):
+        seqops.UnitPool(a.buffers(), into=seqops.UnitPool(b.buffers()))
