@@ -16,8 +16,8 @@ INCLUDE = os.path.join(HERE, "..", "include")
 TARGETS = {
     "engine": {"lib": os.path.join(HERE, "libcalm_b200.so"), "sources": ["engine.cu"],
                "deps": ["attn.cuh", "common.cuh", "tc05.cuh", "prefill.cuh", "ring.cuh", "cols.cuh", "stages.cuh", os.path.join(INCLUDE, "calm_b200.h"), os.path.join(INCLUDE, "calm_model.h")]},
-    "seq": {"lib": os.path.join(HERE, "libcalm_b200_seq.so"), "sources": ["seqmodel.cu", "seqops.cu", "seqbeam.cu", "seqcache8.cu"],
-            "deps": ["common.cuh", "tc05.cuh", "seqkernels.cuh", "seqgemm_tc.cuh", "seqops.cuh", os.path.join(INCLUDE, "calm_b200_seq.h")]},
+    "seq": {"lib": os.path.join(HERE, "libcalm_b200_seq.so"), "sources": ["seqmodel.cu", "seqops.cu", "seqbeam.cu", "seqcache8.cu", "seqrotate.cu", "seqattend16.cu"],
+            "deps": ["common.cuh", "tc05.cuh", "seqkernels.cuh", "seqgemm_tc.cuh", "seqops.cuh", "seqcache16.cuh", os.path.join(INCLUDE, "calm_b200_seq.h")]},
 }
 LIB = TARGETS["engine"]["lib"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

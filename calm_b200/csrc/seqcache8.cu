@@ -24,7 +24,6 @@ struct C8 {
 };
 constexpr int C8_LEAST = -64; // exponent of the smallest scale
 
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); } // -126 <= e <= 127
 __device__ __forceinline__ int pow2_of(float scale) { return max((int)(__float_as_uint(scale) >> 23 & 255) - 127, C8_LEAST); }
 // the least e >= C8_LEAST with amax <= 448 * 2^e: amax = m 2^x with 1/2 <= m < 1, 448 = 0.875 * 2^9
 __device__ __forceinline__ int scale_exponent(float amax) {
@@ -172,12 +171,6 @@ __host__ __device__ constexpr size_t at_ring() { // (the sums of the warps take 
 template <int D, bool SPLIT, int NQ>
 constexpr size_t at_smem() { return (size_t)(SPLIT ? 2 : 1) * 8 * NQ * D * 2 + at_ring<D>(); }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) { // zeros where there is nothing to read
-	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp4(void* dst, const void* src, bool there) {
 	asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
@@ -185,12 +178,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 	             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-}
-// an 8 x 8 tile of fp16, a row's pair of neighbours a thread, with rows and columns exchanged
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
-	uint32_t r;
-	asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-	return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
 	const __half2 h = __floats2half2_rn(x, y);
@@ -203,15 +190,6 @@ __device__ __forceinline__ uint32_t pack_rest(float x, float y, uint32_t hi) { /
 // 16-byte piece of a row of codes that is stored at place `piece` of row r: rows read together meet different banks
 template <int D>
 __device__ __forceinline__ int at_place(int r, int piece) { return piece ^ (D == 64 ? (r >> 1) & 3 : r & 7); }
-__device__ __forceinline__ float load_as_f32(const void* p, int type, long long i) {
-	return type == SEQ_F32 ? ((const float*)p)[i] : type == SEQ_BF16 ? as_f32(((const bf16*)p)[i]) : as_f32(((const __half*)p)[i]);
-}
-__device__ __forceinline__ void store_f32(void* p, int type, long long i, float v) {
-	if (type == SEQ_F32) ((float*)p)[i] = v;
-	else if (type == SEQ_BF16) ((bf16*)p)[i] = __float2bfloat16_rn(v);
-	else ((__half*)p)[i] = __float2half_rn(v);
-}
-
 // Queries times 2^-exponent stand at 2^AT_LIFT or less.  What is not finite does not count: it spoils its own row and no other.
 __device__ __forceinline__ uint32_t at_size(float x) { // |x| as bits, which are in the order of the values
 	const uint32_t a = __float_as_uint(x) & 0x7fffffff;
@@ -236,8 +214,6 @@ __device__ __forceinline__ AtSpan at_span(const Attend& a, int p0, int row0, int
 	s.chunks = (s.total + AT_KEYS - 1) / AT_KEYS;
 	return s;
 }
-// a sink's term of the denominator against a reference that is no lower: none for -inf, all of it for +inf
-__device__ __forceinline__ float at_sink(float sk, float top) { return sk == -INFINITY ? 0.f : sk == top ? 1.f : ex2(sk - top); }
 __device__ __forceinline__ void at_finish(const Attend& a, int token, int head, int d, float v) {
 	if (a.gate) v *= 1.f / (1.f + expf(-a.gate[token * a.gate_row + head * a.gate_head + d * a.gate_dim]));
 	store_f32(a.out, a.out_type, token * a.o_row + head * a.o_head + d, v);
@@ -665,16 +641,6 @@ struct ApShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	int tops[4 * GROUPS], least[4 * GROUPS]; // exponents of the queries: the largest and the smallest row of a warp's
 	int lost;
 };
-// false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN
-__device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity, int* lost) {
-	for (unsigned spins = 0; spins < MBAR_SPINS; ++spins) {
-		if (mbar_try_wait(bar, parity)) return true;
-		if ((spins & 63) == 63 && *(volatile int*)lost) return false;
-	}
-	*(volatile int*)lost = 1;
-	return false;
-}
-__device__ __forceinline__ bool ap_wait_warp(uint64_t* bar, uint32_t parity, int* lost) { return __all_sync(0xffffffffu, ap_wait(bar, parity, lost)); }
 // eight neighbours as floats
 __device__ __forceinline__ void load8(const void* p, int type, long long i, bool vec, float (&x)[8]) {
 	if (!vec) {
@@ -688,31 +654,6 @@ __device__ __forceinline__ void load8(const void* p, int type, long long i, bool
 		if (type == SEQ_BF16) unpack16<bf16>(w, x);
 		else unpack16<__half>(w, x);
 	}
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) { // (tcgen05.wait::st is the caller's)
-	asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-	             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
-	             "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-	             : "memory");
-}
-// 32 lanes x 8 columns times f
-__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
-	float v[8];
-	asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-	             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
-	asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
-	             "f"(v[0] * f), "f"(v[1] * f), "f"(v[2] * f), "f"(v[3] * f), "f"(v[4] * f), "f"(v[5] * f), "f"(v[6] * f), "f"(v[7] * f)
-	             : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem] (+)= A[tmem] . B[smem]^T: A's rows are lanes, a column holds two neighbouring fp16 of a row
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-	asm volatile(
-	    "{\n\t.reg .pred p;\n\t"
-	    "setp.ne.b32 p, %4, 0;\n\t"
-	    "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-	    ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-	    : "memory");
 }
 template <int N>
 __device__ __forceinline__ int ap_tile_exponent(const int (&tops)[N]) {
@@ -1146,12 +1087,6 @@ int check_cache(const char* what, const SeqCache8* q, const SeqPortions* p) {
 	if (((uintptr_t)q->k | (uintptr_t)q->v) % 16) return refuse("%s: codes are not aligned to 16 bytes", what);
 	if (((uintptr_t)q->table | (uintptr_t)p->start | (uintptr_t)p->count | (uintptr_t)p->slot | (uintptr_t)p->pos0) % 4) return refuse("%s: the page table or the batch's description is not aligned to 4 bytes", what);
 	if (((uintptr_t)q->k_scale | (uintptr_t)q->v_scale) % 4) return refuse("%s: scales are not aligned to 4 bytes", what);
-	return 0;
-}
-int check_rows(const char* what, const char* name, const SeqRows& r) {
-	if (!type_ok(r.type)) return refuse("%s: %s has type %d", what, name, r.type);
-	if (r.rows < 0 || (r.rows && !r.p)) return refuse("%s: %s is missing", what, name);
-	if ((uintptr_t)r.p % type_size(r.type)) return refuse("%s: %s is not aligned to its type", what, name);
 	return 0;
 }
 C8 describe(const SeqCache8& q, const SeqPortions& p) {

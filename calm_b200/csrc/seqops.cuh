@@ -11,6 +11,7 @@
 
 #include "../../include/calm_b200_seq.h"
 #include "common.cuh"
+#include "tc05.cuh"
 
 namespace seqops {
 
@@ -57,6 +58,13 @@ cudaError_t allow(void (*kernel)(KArgs...), size_t smem, std::atomic<uint64_t>& 
 
 inline int type_size(int t) { return t == SEQ_F32 ? 4 : 2; }
 inline bool type_ok(int t) { return t == SEQ_F32 || t == SEQ_BF16 || t == SEQ_F16; }
+
+inline int check_rows(const char* what, const char* name, const SeqRows& r) {
+	if (!type_ok(r.type)) return refuse("%s: %s has type %d", what, name, r.type);
+	if (r.rows < 0 || (r.rows && !r.p)) return refuse("%s: %s is missing", what, name);
+	if ((uintptr_t)r.p % type_size(r.type)) return refuse("%s: %s is not aligned to its type", what, name);
+	return 0;
+}
 
 __device__ __forceinline__ float as_f32(float v) { return v; }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -110,5 +118,40 @@ __device__ __forceinline__ void unpack16(const uint4& w, float (&v)[16 / sizeof(
 #pragma unroll
 	for (int i = 0; i < (int)(16 / sizeof(T)); ++i) v[i] = as_f32(p[i]);
 }
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); } // -126 <= e <= 127
+__device__ __forceinline__ float load_as_f32(const void* p, int type, long long i) {
+	return type == SEQ_F32 ? ((const float*)p)[i] : type == SEQ_BF16 ? as_f32(((const __nv_bfloat16*)p)[i]) : as_f32(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void store_f32(void* p, int type, long long i, float v) {
+	if (type == SEQ_F32) ((float*)p)[i] = v;
+	else if (type == SEQ_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+	else ((__half*)p)[i] = __float2half_rn(v);
+}
+// a sink's term of the denominator against a reference that is no lower: none for -inf, all of it for +inf
+__device__ __forceinline__ float at_sink(float sk, float top) { return sk == -INFINITY ? 0.f : sk == top ? 1.f : ex2(sk - top); }
+// 16 bytes into shared memory, asynchronously
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) { // zeros where there is nothing to read
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// an 8 x 8 tile of fp16, a row's pair of neighbours a thread, with rows and columns exchanged
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+	uint32_t r;
+	asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+	return r;
+}
+// false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN
+__device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity, int* lost) {
+	for (unsigned spins = 0; spins < MBAR_SPINS; ++spins) {
+		if (mbar_try_wait(bar, parity)) return true;
+		if ((spins & 63) == 63 && *(volatile int*)lost) return false;
+	}
+	*(volatile int*)lost = 1;
+	return false;
+}
+__device__ __forceinline__ bool ap_wait_warp(uint64_t* bar, uint32_t parity, int* lost) { return __all_sync(0xffffffffu, ap_wait(bar, parity, lost)); }
 
 } // namespace seqops

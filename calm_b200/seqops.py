@@ -1,5 +1,5 @@
 """Operators of the layer-list library on the caller's own GPU tensors (include/calm_b200_seq.h, second half): the n best continuations of beams, copies of
-cache pages and state slots, a cache of keys and values in 8 bits and attention over it.  The serving runtime (seqlib.SeqDeviceModel, serving.Scheduler) runs
+cache pages and state slots, caches of keys and values in 8 and in 16 bits and attention over them, prefixes that sequences share, rotary positions.  The serving runtime (seqlib.SeqDeviceModel, serving.Scheduler) runs
 on the same kernels.
 
 Calls run on torch's current stream of the tensors' device, return before the work is done and can be captured into CUDA graphs.  What a call refuses raises
@@ -7,6 +7,7 @@ ValueError before anything is launched.  Like everywhere in this package there i
 from __future__ import annotations
 
 import ctypes as C
+import math
 from array import array
 from operator import index as index_of
 from typing import List, Optional, Sequence, Tuple
@@ -47,6 +48,23 @@ class _Attend8(C.Structure):
                 ("slopes", _ptr), ("gate", _ptr), ("gate_row", _ll), ("gate_head", _ll), ("gate_dim", _ll), ("most_keys", _int), ("workspace", _ptr), ("workspace_bytes", _size)]
 
 
+class _Rotation(C.Structure):
+    _fields_ = [("turns", _ptr), ("dims", _int), ("neighbours", _int), ("gain", C.c_float)]
+
+
+class _Cache16(C.Structure):
+    _fields_ = [("k", _ptr), ("v", _ptr), ("type", _int), ("pages", _int), ("heads", _int), ("page", _int), ("dim", _int), ("table", _ptr), ("slots", _int), ("table_pages", _int)]
+
+
+class _Shared(C.Structure):
+    _fields_ = [("n", _int), ("first", _ptr), ("count", _ptr), ("positions", _ptr), ("group", _ptr), ("longest", _int), ("tokens", _int), ("most_own", _int)]
+
+
+class _Attend16(C.Structure):
+    _fields_ = [("q", _Rows), ("out", _Rows), ("heads", _int), ("scale", C.c_float), ("window", _int), ("softcap", C.c_float), ("sinks", _ptr), ("most_keys", _int), ("workspace", _ptr),
+                ("workspace_bytes", _size)]
+
+
 _lib = None
 
 
@@ -63,6 +81,12 @@ def _load() -> C.CDLL:
         L.calm_b200_seq_cache8_store.restype = _int
         L.calm_b200_seq_attend8_workspace.argtypes, L.calm_b200_seq_attend8_workspace.restype = [C.POINTER(_Cache8), C.POINTER(_Portions), C.POINTER(_Attend8)], _size
         L.calm_b200_seq_attend8.argtypes, L.calm_b200_seq_attend8.restype = [C.POINTER(_Cache8), C.POINTER(_Portions), C.POINTER(_Attend8), _ptr], _int
+        L.calm_b200_seq_rotate.argtypes, L.calm_b200_seq_rotate.restype = [C.POINTER(_Portions), C.POINTER(_Rotation), C.POINTER(_Rows), C.POINTER(_Rows), _int, _int, _ptr], _int
+        L.calm_b200_seq_cache16_store.argtypes = [C.POINTER(_Cache16), C.POINTER(_Portions), C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rotation), C.POINTER(_Rows), C.POINTER(_Rows), _int, _ptr]
+        L.calm_b200_seq_cache16_store.restype = _int
+        args = [C.POINTER(_Cache16), C.POINTER(_Portions), C.POINTER(_Shared), C.POINTER(_Attend16)]
+        L.calm_b200_seq_attend16_workspace.argtypes, L.calm_b200_seq_attend16_workspace.restype = args, _size
+        L.calm_b200_seq_attend16.argtypes, L.calm_b200_seq_attend16.restype = args + [_ptr], _int
         _lib = L
     return _lib
 
@@ -203,9 +227,13 @@ class UnitPool:
 
 class Batch:
     """The packed batch of a step: sequence i brings counts[i] new tokens, in order, at positions before[i] .. of slot slots[i].  The device arrays (`data`, int32 rows start,
-    count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest`."""
+    count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest`.
 
-    def __init__(self, slots: Sequence[int], counts: Sequence[int], before: Sequence[int], device=None):
+    shared: groups of neighbouring sequences that go on from one text, as (first sequence, sequences, positions): a cache holds the positions below that once, on the pages that the
+    table names for the group's first sequence, and Cache16.attend reads them once for all of the group.  The device array `groups` (int32 rows first, sequences, positions) may be written between replays
+    too (positions up to the largest that was given)."""
+
+    def __init__(self, slots: Sequence[int], counts: Sequence[int], before: Sequence[int], device=None, shared: Sequence[Tuple[int, int, int]] = ()):
         sl, cn, at = (np.array(_list(name, x), np.int32) for name, x in (("slots", slots), ("counts", counts), ("before", before)))
         if not len(sl) == len(cn) == len(at):
             raise ValueError("slots, counts and before must have one length")
@@ -216,12 +244,40 @@ class Batch:
         start = np.concatenate([[0], np.cumsum(cn, dtype=np.int64)])
         if start[-1] >= 2 ** 31 or (len(cn) and int((at.astype(np.int64) + cn).max()) >= 2 ** 31):
             raise ValueError("token numbers pass 31 bits")
+        groups, of = _grouped(shared, cn, at)
         self.tokens, self.longest = int(start[-1]), int(cn.max(initial=0))
         self.most_keys = int((at.astype(np.int64) + cn).max(initial=0))
         self.data = torch.from_numpy(np.stack([start[:-1].astype(np.int32), cn, sl, at])).to(torch.device("cuda") if device is None else device)
         self.index = _gpu("the batch", self.data)
         base, step = self.data.data_ptr(), self.data.stride(0) * 4
         self.c = _Portions(len(sl), base, base + step, base + 2 * step, base + 3 * step, self.longest)
+        self.groups = self.group_of = self.shared = None
+        if len(groups):
+            own = at.astype(np.int64) + cn - np.where(of >= 0, groups[of, 2], 0)
+            tokens = max(int(cn[f:f + n].sum()) for f, n, _ in groups.tolist())
+            both = torch.from_numpy(np.concatenate([groups.T.reshape(-1), of])).to(self.data.device)
+            self.groups, self.group_of = both[:groups.size].view(3, -1), both[groups.size:]
+            base, step = both.data_ptr(), 4 * len(groups)
+            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, int(groups[:, 2].max()), tokens, int(own.max()))
+
+
+def _grouped(shared, cn: np.ndarray, at: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
+    """Groups (first sequence, sequences, positions), in order, and the group that each sequence is in (-1: none)."""
+    try:
+        groups = [_list("a group", g) for g in shared]
+    except TypeError:
+        groups = [()]
+    if any(len(g) != 3 for g in groups):
+        raise ValueError("shared must be a list of groups (first sequence, sequences, positions)")
+    groups = np.array(sorted(list(g) for g in groups), np.int32).reshape(-1, 3)
+    of, end = np.full(len(cn), -1, np.int32), 0
+    for i, (first, n, positions) in enumerate(groups.tolist()):
+        if first < end or n < 1 or first + n > len(cn) or positions < 0:
+            raise ValueError(f"a group of {n} sequences from {first} on that share {positions} positions: groups lie apart among the {len(cn)} sequences")
+        if positions > int(at[first:first + n].min()):
+            raise ValueError(f"a group's sequences {first} .. {first + n - 1} do not all have {positions} positions before their new tokens")
+        of[first:first + n], end = i, first + n
+    return groups, of
 
 
 def _rows(name: str, t: torch.Tensor, index: int, heads: int, dim: int, least: int) -> _Rows:
@@ -313,4 +369,180 @@ class Cache8:
             work = torch.empty(need, dtype=torch.uint8, device=q.device)
             a.workspace, a.workspace_bytes = work.data_ptr(), need
         _run(index, L.calm_b200_seq_attend8, C.byref(c), C.byref(batch.c), C.byref(a))
+        return out
+
+
+class Rotation:
+    """How positions turn the channels of a head: the first `dims` of them, in pairs of "halves" (i, i + dims / 2) or "neighbours" (2i, 2i + 1), pair i by position * f_i with
+    f_i = base^(-2 i / dims).  `scaling` stretches f for contexts longer than a model was trained on:
+      {"kind": "linear", "factor"}                          f / factor
+      {"kind": "base", "factor"}                            the base times factor^(dims / (dims - 2))
+      {"kind": "wavelength", "factor", "length", "low", "high"}  w = length f / 2 pi: f / factor below `low`, f above `high`, a blend linear in w between
+      {"kind": "ramp", "factor", "length", "fast", "slow"}  the same by the pair's number, between the pairs that turn `fast` and `slow` times in `length` positions; cosines and sines
+                                                            times 0.1 ln(factor) + 1 (or "gain")
+    frequencies: f itself, float64 [dims / 2], in place of base and scaling."""
+
+    def __init__(self, dims: int, base: float = 10000.0, pairs: str = "halves", scaling: Optional[dict] = None, frequencies=None, device=None):
+        dims = _whole("dims", dims)
+        if dims < 2 or dims % 2:
+            raise ValueError(f"a rotation of {dims} channels: an even number from 2 on")
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError(f"pairs are \"halves\" or \"neighbours\", not {pairs!r}")
+        if frequencies is None:
+            self.frequencies, self.gain = rotation_frequencies(dims, base, scaling)
+        elif scaling is not None:
+            raise ValueError("frequencies that are given are not scaled")
+        else:
+            self.frequencies, self.gain = np.array(frequencies, np.float64), 1.0
+            if self.frequencies.shape != (dims // 2,) or not np.isfinite(self.frequencies).all():
+                raise ValueError(f"frequencies must be {dims // 2} finite numbers")
+        self.dims, self.pairs = dims, pairs
+        self.turns = torch.from_numpy(self.frequencies / (2.0 * math.pi)).to(torch.device("cuda") if device is None else device)
+        self.index = _gpu("the rotation", self.turns)
+        self.c = _Rotation(self.turns.data_ptr(), dims, int(pairs == "neighbours"), self.gain)
+
+
+def rotation_frequencies(dims: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[np.ndarray, float]:
+    """Step of every pair of a Rotation (float64 [dims / 2]) and the factor on cosines and sines."""
+    s = dict(scaling) if scaling else {"kind": "none"}
+    kind, gain, given = s.pop("kind", None), s.pop("gain", None), set(s)
+    wants = {"none": set(), "linear": {"factor"}, "base": {"factor"}, "wavelength": {"factor", "length", "low", "high"}, "ramp": {"factor", "length", "fast", "slow"}}
+    if kind not in wants or given != wants[kind]:
+        raise ValueError(f"scaling {scaling!r}: one of " + ", ".join(f"{k} ({', '.join(sorted(w))})" for k, w in wants.items() if w))
+    if not (base > 0 and math.isfinite(base)) or not all(v > 0 and math.isfinite(v) for v in s.values()):
+        raise ValueError(f"base {base}, scaling {scaling!r}: positive numbers")
+    if kind == "base":
+        if dims < 4:
+            raise ValueError("one pair of channels has no base to stretch")
+        base *= s["factor"] ** (dims / (dims - 2))
+    i = np.arange(dims // 2, dtype=np.float64)
+    f = base ** (-2.0 * i / dims)
+    if kind == "linear":
+        f = f / s["factor"]
+    elif kind == "wavelength":
+        if not s["low"] < s["high"]:
+            raise ValueError("low must be under high")
+        w = s["length"] * f / (2.0 * math.pi)
+        blend = np.clip((w - s["low"]) / (s["high"] - s["low"]), 0.0, 1.0)
+        f = (1.0 - blend) * f / s["factor"] + blend * f
+    elif kind == "ramp":
+        if base == 1.0:
+            raise ValueError("a base of 1 has no ramp")
+        at = [dims * math.log(s["length"] / (2.0 * math.pi * t)) / (2.0 * math.log(base)) for t in (s["fast"], s["slow"])]
+        lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
+        blend = np.clip((i - lo) / max(hi - lo, 0.001), 0.0, 1.0)
+        f = f / s["factor"] * blend + f * (1.0 - blend)
+        gain = 0.1 * math.log(s["factor"]) + 1.0 if gain is None else gain
+    return f, 1.0 if gain is None else float(gain)
+
+
+def _beside(rotation: Rotation, batch: Batch, index: int) -> None:
+    if not isinstance(rotation, Rotation):
+        raise ValueError("the rotation must be a seqops.Rotation")
+    for name, x in (("the rotation", rotation), ("the batch", batch)):
+        if x.index != index:
+            raise ValueError(f"{name} is on cuda:{x.index}, the call's other tensors on cuda:{index}")
+
+
+def _like(x: torch.Tensor, tokens: int) -> torch.Tensor:
+    """Where rows like x's go: what is behind the batch's tokens is zero."""
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if x.shape[0] == tokens else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+
+
+def rotate(x: torch.Tensor, batch: Batch, rotation: Rotation, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The batch's rows x [tokens, heads, dim] (float32, bfloat16 or float16; dim even) turned by their positions.  `out`: where they go, x itself or a tensor apart from it; rows behind the
+    batch's tokens stay as they are in it (zero without one)."""
+    index = _gpu("x", x)
+    if x.dim() != 3:
+        raise ValueError("x must be [tokens, heads, dim]")
+    _beside(rotation, batch, index)
+    heads, dim = x.shape[1:]
+    rx = _rows("x", x, index, heads, dim, batch.tokens)
+    if out is None:
+        out = _like(x, batch.tokens)
+    ro = _rows("out", out, index, heads, dim, rx.rows)
+    _run(index, _load().calm_b200_seq_rotate, C.byref(batch.c), C.byref(rotation.c), C.byref(rx), C.byref(ro), heads, dim)
+    return out
+
+
+class Cache16:
+    """A paged cache of keys and values in 16 bits: k and v [pages, heads, page, dim] in bfloat16 or float16.  `Cache16.empty` allocates one."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        self.index = _gpu("keys", k)
+        _gpu("values", v, self.index)
+        for t in (k, v):
+            if t.dim() != 4 or t.dtype not in (torch.bfloat16, torch.float16) or not t.is_contiguous() or t.shape != k.shape or t.dtype != k.dtype:
+                raise ValueError("keys and values must be contiguous [pages, heads, page, dim] in bfloat16 or float16, of one shape and type")
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self.pages, self.heads, self.page, self.dim = k.shape
+        self._pool = (k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.pages, self.heads, self.page, self.dim)
+        if self.dim % 16 or not 16 <= self.dim <= 256:
+            raise ValueError(f"rows of {self.dim} channels: a multiple of 16 up to 256 is served")
+
+    @staticmethod
+    def empty(pages: int, heads: int, page: int, dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda") -> "Cache16":
+        return Cache16(*(torch.zeros((pages, heads, page, dim), dtype=dtype, device=device) for _ in range(2)))
+
+    def buffers(self) -> List[torch.Tensor]:
+        """Both tensors as page buffers of a UnitPool: views [pages, 1, ...], since a page's first tokens are not its front (heads come first) and pages are copied whole."""
+        return [t.unsqueeze(1) for t in (self.k, self.v)]
+
+    def _with(self, table: torch.Tensor, batch: Batch) -> _Cache16:
+        _gpu("the page table", table, self.index)
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
+            raise ValueError("the page table must be contiguous int32 [slots, pages of a slot]")
+        if batch.index != self.index:
+            raise ValueError(f"the batch is on cuda:{batch.index}, the cache on cuda:{self.index}")
+        slots, table_pages = table.shape
+        return _Cache16(*self._pool, table.data_ptr(), slots, table_pages)
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, batch: Batch, rotation: Optional[Rotation] = None, q: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """The batch's key and value rows [tokens, heads, dim] into the pages that `table` (int32 [slots, pages of a slot]) names for their positions, the keys turned by their
+        positions where a rotation is given.  q: the step's queries [tokens, query heads, dim], turned in the same launch into q_out (q itself or a tensor apart from it; a new one without), which is returned."""
+        c, n, index = self._with(table, batch), batch.tokens, self.index
+        rk, rv = _rows("k", k, index, self.heads, self.dim, n), _rows("v", v, index, self.heads, self.dim, n)
+        turn, rq, ro, heads = None, None, None, 0
+        if rotation is not None:
+            _beside(rotation, batch, index)
+            turn = C.byref(rotation.c)
+        if q is not None:
+            if not isinstance(q, torch.Tensor) or q.dim() != 3:
+                raise ValueError("q must be [tokens, query heads, dim]")
+            heads = q.shape[1]
+            rq = _rows("q", q, index, heads, self.dim, n)
+            if q_out is None:
+                q_out = _like(q, n)
+            ro = _rows("q_out", q_out, index, heads, self.dim, rq.rows)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        _run(index, _load().calm_b200_seq_cache16_store, C.byref(c), C.byref(batch.c), C.byref(rk), C.byref(rv), turn, rq if rq is None else C.byref(rq), ro if ro is None else C.byref(ro), heads)
+        return q_out
+
+    def attend(self, q: torch.Tensor, table: torch.Tensor, batch: Batch, scale: float, window: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the batch's queries [tokens, query heads, dim] (of the cache's type) over the cache, which holds their own keys already (store comes first).  A token sees its
+        sequence's positions up to its own, the last `window` of them where that is not 0; positions that the batch's groups share are read once for the group.  sink: float32 [query heads], one more logit in the
+        softmax's denominator.  Rows of q behind the batch's tokens stay as they are in `out` (zero without one)."""
+        c, index = self._with(table, batch), self.index
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise ValueError("q must be [tokens, query heads, dim]")
+        heads = q.shape[1]
+        rq = _rows("q", q, index, heads, self.dim, batch.tokens)
+        if out is None:
+            out = _like(q, batch.tokens)
+        ro = _rows("out", out, index, heads, self.dim, rq.rows)
+        a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, None, 0)
+        if sink is not None:
+            _gpu("sink", sink, index)
+            if sink.shape != (heads,) or sink.dtype != torch.float32 or not sink.is_contiguous():
+                raise ValueError(f"sink must be contiguous float32 [{heads}]")
+            a.sinks = sink.data_ptr()
+        L, shared = _load(), None if batch.shared is None else C.byref(batch.shared)
+        need = L.calm_b200_seq_attend16_workspace(C.byref(c), C.byref(batch.c), shared, C.byref(a))
+        if need:
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), need
+        _run(index, L.calm_b200_seq_attend16, C.byref(c), C.byref(batch.c), shared, C.byref(a))
         return out

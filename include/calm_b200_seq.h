@@ -431,6 +431,64 @@ struct SeqAttend8 {
 size_t calm_b200_seq_attend8_workspace(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args);
 int calm_b200_seq_attend8(const struct SeqCache8* cache, const struct SeqPortions* batch, const struct SeqAttend8* args, void* stream);
 
+/* ---- rotary positions, a paged cache in 16 bits, attention over prefixes that sequences share ---- */
+
+/* How positions turn the channels of a head: of the first `dims` channels, pair i (channels 2i, 2i + 1 with `neighbours`, else i, i + dims / 2) at position p becomes
+ * gain (a cos w - b sin w), gain (b cos w + a sin w), w = 2 pi p turns[i]; the others stay.  The angle is taken in 64 bits and its whole turns off before anything becomes
+ * fp32, results are rounded to the rows' type once. */
+struct SeqRotation {
+	const double* turns; /* device [dims / 2]: turns a position */
+	int dims;            /* even, from 2 to the channels of a head */
+	int neighbours;
+	float gain;          /* on cosines and sines */
+};
+/* The batch's rows x [rows][heads][dim] (dim even, at most 1024) turned by their positions into out, which has their type and is x itself or apart from it. */
+int calm_b200_seq_rotate(const struct SeqPortions* batch, const struct SeqRotation* rotation, const struct SeqRows* x, const struct SeqRows* out, int heads, int dim, void* stream);
+
+/* Keys and values [pages][heads][page][dim] in bfloat16 or float16; sequence slot s finds its position p in page table[s][p / page], row p % page. */
+struct SeqCache16 {
+	void *k, *v;                 /* 16-byte aligned */
+	int type;                    /* SEQ_BF16 or SEQ_F16 */
+	int pages, heads, page, dim; /* dim a multiple of 16, at most 256 */
+	const int* table;            /* device [slots][table_pages] */
+	int slots, table_pages;
+};
+/* New rows of keys and values [rows][heads][dim] into the cache, rounded to its type (to nearest even) after the rotation of the keys, where there is one; in the same launch the step's queries
+ * [rows][q_heads][dim], turned alike, into q_out (their type; q itself or apart from it).  q NULL: no queries.  What a slot, position or page number outside the cache names is not written; queries are turned all
+ * the same. */
+int calm_b200_seq_cache16_store(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqRows* k, const struct SeqRows* v, const struct SeqRotation* rotation,
+                                const struct SeqRows* q, const struct SeqRows* q_out, int q_heads, void* stream);
+
+/* Groups of sequences of a batch that go on from the same text: group g is sequences first[g] .. first[g] + count[g] - 1, whose tokens lie back to back, and holds its positions below positions[g]
+ * once: they are found through the table's row of its first sequence's slot, whatever the others' rows say.  Groups do not overlap. */
+struct SeqShared {
+	int n;
+	const int *first, *count, *positions; /* device [n] */
+	const int* group;                     /* device [sequences]: the group that a sequence is in, -1: none */
+	int longest;                          /* at least the largest of positions */
+	int tokens;                           /* at least the new tokens of any group */
+	int most_own;                         /* at least the keys of any sequence behind what it shares (what the split of the work is planned for; more are still seen) */
+};
+/* Attention of the batch's tokens over the cache, which holds them already: the token at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p); query
+ * head h reads key head h / (heads / cache.heads).
+ *   s_j = softcap(scale q . k_j);  out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h]))
+ * A prefix that a group shares is read once for all of the group's tokens (or, where a sequence brings many, once for 128 or 256 of its rows).  Scores, softmax and sums are fp32; softmax weights enter the tensor cores in the cache's
+ * type.  Positions whose slot, table entry or page number is outside the cache are not seen; what they, positions behind a token or outside its window hold does not reach its result, unless a key that
+ * some other token of the same tile of at least 128 rows sees has a value that is not finite.  A token that sees nothing gets zeros.  Rows that belong to no sequence are left alone. */
+struct SeqAttend16 {
+	struct SeqRows q, out;   /* of the cache's type */
+	int heads;               /* query heads, a multiple of cache.heads */
+	float scale;
+	int window;
+	float softcap;           /* > 0: s = softcap tanh(s / softcap) after the scale */
+	const float* sinks;      /* [heads] or NULL */
+	int most_keys;           /* at least the keys that any token sees (what the split of the work is planned for; more are still seen) */
+	void* workspace;         /* calm_b200_seq_attend16_workspace bytes, 16-byte aligned; undefined between calls, not to be shared by calls that may overlap */
+	size_t workspace_bytes;
+};
+size_t calm_b200_seq_attend16_workspace(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args);
+int calm_b200_seq_attend16(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
