@@ -1,6 +1,7 @@
 // seqattend16.cu -- attention over a paged cache in 16 bits, where groups of sequences share a prefix (calm_b200_seq_attend16 in include/calm_b200_seq.h).
 
 #include "seqcache16.cuh"
+#include "tc05.cuh"
 
 namespace seqops {
 namespace {
@@ -117,23 +118,27 @@ __device__ __forceinline__ bool there(const C16& c, int rows, int b) {
 	const int n = c.count[b], p0 = c.pos0[b], start = c.start[b];
 	return n >= 1 && p0 >= 0 && p0 <= INT_MAX - n && start >= 0 && n <= rows - start;
 }
-// The rows of work unit z: tokens t0 .. t0 + tokens - 1 of the sequences first .. last; `prefix` positions are the group's.  false: nothing to do
+// The rows of a work unit: tokens t0 .. t0 + tokens - 1 of the sequences first .. last; `prefix` positions are the group's, found through sequence `lead`.  false: nothing to do
 struct Unit {
-	int first, last, t0, tokens, prefix;
+	int first, last, lead, t0, tokens, prefix;
 };
-__device__ __forceinline__ bool unit_of(const C16& c, const Attend& a, int z, Unit& u) {
-	if (a.families && z < c.groups) {
-		const int f = c.first[z], m = c.members[z];
-		if (f < 0 || m < 1 || f > c.n - m) return false;
-		const long long t0 = c.start[f], t1 = (long long)c.start[f + m - 1] + c.count[f + m - 1];
-		if (t0 < 0 || t1 <= t0 || t1 > a.rows) return false;
-		u.first = f, u.last = f + m - 1, u.t0 = (int)t0, u.tokens = (int)(t1 - t0), u.prefix = max(c.positions[z], 0);
-		return true;
+__device__ __forceinline__ bool group_unit(const C16& c, const Attend& a, int g, Unit& u) {
+	const int f = c.first[g], m = c.members[g];
+	if (f < 0 || m < 1 || f > c.n - m) return false;
+	const long long t0 = c.start[f], t1 = (long long)c.start[f + m - 1] + c.count[f + m - 1];
+	if (t0 < 0 || t1 <= t0 || t1 > a.rows) return false;
+	u.first = u.lead = f, u.last = f + m - 1, u.t0 = (int)t0, u.tokens = (int)(t1 - t0), u.prefix = max(c.positions[g], 0);
+	return true;
+}
+// a sequence; one that names a group is among that group's and has its rows among the group's
+__device__ __forceinline__ bool own_unit(const C16& c, const Attend& a, int b, Unit& u) {
+	const int g = c.groups ? c.group[b] : -1;
+	if (!there(c, a.rows, b)) return false;
+	u.prefix = 0, u.lead = -1;
+	if ((unsigned)g < (unsigned)c.groups) {
+		if (!group_unit(c, a, g, u) || b < u.first || b > u.last || c.start[b] < u.t0 || c.start[b] + c.count[b] > u.t0 + u.tokens) return false;
 	}
-	const int b = a.families ? z - c.groups : z, g = c.groups ? c.group[b] : -1;
-	const bool grouped = (unsigned)g < (unsigned)c.groups;
-	if ((a.families && grouped) || !there(c, a.rows, b)) return false;
-	u.first = u.last = b, u.t0 = c.start[b], u.tokens = c.count[b], u.prefix = grouped ? max(c.positions[g], 0) : 0;
+	u.first = u.last = b, u.t0 = c.start[b], u.tokens = c.count[b];
 	return true;
 }
 __device__ __forceinline__ int low_of(const Attend& a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
@@ -153,7 +158,10 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
 	Unit u;
 	if (a.before) pdl_launch_next();
-	if (!unit_of(c, a, blockIdx.z, u) || (long long)blockIdx.x * TILE >= (long long)u.tokens * a.group) {
+	const int z = blockIdx.z;
+	bool some_rows = a.families && z < c.groups ? group_unit(c, a, z, u) : own_unit(c, a, a.families ? z - c.groups : z, u);
+	if (a.families && z >= c.groups && some_rows && u.lead >= 0) some_rows = false; // (its group has it)
+	if (!some_rows || (long long)blockIdx.x * TILE >= (long long)u.tokens * a.group) {
 		if (a.before) pdl_wait_prev();
 		return;
 	}
@@ -183,8 +191,8 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		}
 		if (tail) seg_hi[seg] = min(pos + 1, c.reach(c.slot[seq]));
 		if (lane == 0) {
-			const int slot = c.slot[u.first];
-			const bool with = a.families && least != INT_MAX;
+			const bool with = a.families && u.prefix > 0 && least != INT_MAX;
+			const int slot = with ? c.slot[u.lead] : -1;
 			seg_slot[0] = slot, seg_lo[0] = with ? low_of(a, least) : 0, seg_hi[0] = with ? min(min(u.prefix, most + 1), c.reach(slot)) : 0;
 		}
 		__syncwarp();
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	// the warps' sums as one, eight rows at a time
 	float* const sums = reinterpret_cast<float*>(ring); // [warps][8][LD]
 	float* const own = sums + AR_WARPS * 8 * LD;        // [TILE][D + 2]: what this share of a cluster found
-	const int prefix_places = whole && c.groups && (unsigned)c.group[u.first] < (unsigned)c.groups ? a.before : 0;
+	const int prefix_places = whole && u.lead >= 0 ? a.before : 0;
 #pragma unroll
 	for (int q = 0; q < NQ; ++q) {
 		if (8 * q >= rows) break;
@@ -530,14 +538,370 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	cluster_sync(); // no CTA leaves while another reads what it found
 }
 
+// ---------------------------------------------------------------- many rows
+// Where many rows see the same keys, the products run on the fifth-generation tensor cores: a CTA takes one or two groups of 128 rows that read one key head - of a group of sequences over its prefix, or of one sequence
+// over its group's prefix and its own keys - and walks tiles of 128 keys.  One warp copies tiles with TMA, boxes of 64 channels and as many keys as lie side by side in a page (8 to 64), straight into the layout
+// that the products read: keys as rows, values as they lie with the channels as the product's columns.  One thread issues S = Q K^T of the next tile behind O += P V of this one; four warps a group, a row a thread, take S from tensor
+// memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run.  O stays in tensor memory; it is rescaled in the rare case that
+// a row's reference moves.
+constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
+constexpr int AW_SOFTMAX_REGS = 208, AW_OTHER_REGS = 80; // 256 x 208 + 128 x 80 = 63488 of the 384 x 168 = 64512 that the block is launched with
+
+template <int D>
+struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
+	static constexpr int PANELS = D / 64, SLOTS = D == 128 ? 5 : 9;
+	unsigned char q[2][PANELS][128 * 128];
+	unsigned char kv[SLOTS][PANELS][AW_KEYS * 128]; // keys and values in turn
+	uint64_t full[SLOTS], empty[SLOTS], mask_full[AW_MASKS], s_full[2], p_full[2], done[2], fix, idle;
+	uint32_t seen[AW_MASKS][4]; // keys that are there
+	int row_pos[256];
+	int span[4]; // the rows' least and largest position (of warps that found them)
+	uint32_t tmem;
+	int lost;
+};
+// a row of scores
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+#define AW_R8(b) "=f"(v[b]), "=f"(v[b + 1]), "=f"(v[b + 2]), "=f"(v[b + 3]), "=f"(v[b + 4]), "=f"(v[b + 5]), "=f"(v[b + 6]), "=f"(v[b + 7])
+#define AW_R32(b) AW_R8(b), AW_R8(b + 8), AW_R8(b + 16), AW_R8(b + 24)
+	asm volatile(
+	    "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+	    "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+	    "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+	    "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+	    "tcgen05.wait::ld.sync.aligned;"
+	    : AW_R32(0), AW_R32(32), AW_R32(64), AW_R32(96)
+	    : "r"(taddr)
+	    : "memory");
+#undef AW_R8
+#undef AW_R32
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+	asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+	             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+	             : "r"(taddr)
+	             : "memory");
+}
+// shared-memory descriptor of values [keys][64 channels], 128-byte swizzle, panels of 64 channels 16 KB apart: the product's columns are the channels, its depth the keys, eight keys 1024 bytes apart
+__device__ __forceinline__ uint64_t umma_desc_values(const void* tile) {
+	const uint64_t addr = (uint64_t)(smem_u32(tile) & 0x3FFFF) >> 4;
+	return addr | ((uint64_t)(AW_KEYS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+struct Wide {
+	int through;    // 1: every sequence's rows over its group's prefix and its own keys; 0: every group's rows over its prefix
+	int box;        // keys that a copy brings
+	int shares, each; // of a tile's keys, tiles of 128 of each
+	int tiles;      // of 256 rows, of the longest unit
+	int place;      // the first share's in stats and sums; -1: results go to out
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const C16 c, const Attend a, const Wide w) {
+	typedef AwShared<D> Shared;
+	constexpr int PANELS = Shared::PANELS, SLOTS = Shared::SLOTS, PIECES = D / 8;
+	constexpr uint32_t O_COL = 256;
+	extern __shared__ __align__(1024) unsigned char aw_raw[]; // (all of the kernel's shared memory: it starts where the swizzle's pattern does)
+	Shared& s = *reinterpret_cast<Shared*>(aw_raw);
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+	const int per = w.tiles * c.heads, share = blockIdx.x / per, kvh = blockIdx.x % per / w.tiles, tile = w.tiles - 1 - blockIdx.x % w.tiles; // (longest rows first)
+	pdl_launch_next();
+	Unit u;
+	if (w.through) {
+		if (!own_unit(c, a, blockIdx.z, u)) return;
+	} else if (!group_unit(c, a, blockIdx.z, u)) return;
+	if ((long long)tile * 256 >= (long long)u.tokens * a.group) return;
+	const int row0 = tile * 256, rows = (int)min(256LL, (long long)u.tokens * a.group - row0), groups = rows > 128 ? 2 : 1;
+
+	if (warp == 9) tmem_alloc(&s.tmem, 512);
+	if (tid == 0) {
+		for (int i = 0; i < SLOTS; ++i) mbar_init(s.full + i, 1), mbar_init(s.empty + i, 1);
+		for (int i = 0; i < AW_MASKS; ++i) mbar_init(s.mask_full + i, 1);
+		for (int g = 0; g < 2; ++g) mbar_init(s.s_full + g, 1), mbar_init(s.p_full + g, 4), mbar_init(s.done + g, 1);
+		mbar_init(&s.fix, 1), mbar_init(&s.idle, 1);
+		s.lost = 0, s.span[0] = INT_MAX, s.span[1] = -1;
+		mbar_init_fence();
+	}
+	if (tid < 256) s.row_pos[tid] = -1;
+	__syncthreads();
+	for (int b = u.first + tid; b <= u.last; b += AW_THREADS)
+		if (there(c, a.rows, b)) {
+			const long long r0 = (long long)(c.start[b] - u.t0) * a.group - row0, r1 = r0 + (long long)c.count[b] * a.group;
+			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) s.row_pos[r] = c.pos0[b] + (int)((r - r0) / a.group);
+		}
+	// queries, rows of 128 bytes a panel
+	{
+		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
+		for (int i = tid; i < groups * 128 * PIECES; i += AW_THREADS) {
+			const int r = i / PIECES, piece = i % PIECES, rr = row0 + min(r, rows - 1);
+			uint4 x = make_uint4(0, 0, 0, 0);
+			if (r < rows && piece * 8 < c.dim) {
+				const uint16_t* const q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + piece * 8;
+				if (vec) x = *reinterpret_cast<const uint4*>(q);
+				else
+					x = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+			}
+			*reinterpret_cast<uint4*>(s.q[r >> 7][piece >> 3] + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4)) = x;
+		}
+		fence_async_smem();
+	}
+	__syncthreads();
+	if (warp < 8) {
+		const int pos = s.row_pos[tid];
+		const int least = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos), most = __reduce_max_sync(0xffffffffu, pos);
+		if (lane == 0) atomicMin(&s.span[0], least), atomicMax(&s.span[1], most);
+	}
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem = s.tmem;
+	// the keys: positions lo .. hi - 1 of the prefix, then of the sequence's own, in tiles that begin where a copy may
+	const int least = s.span[0], most = s.span[1];
+	int lo[2] = {0, 0}, hi[2] = {0, 0}, base[2] = {0, 0}, count[2] = {0, 0}, slot[2] = {-1, -1};
+	if (most >= 0) {
+		slot[0] = u.lead >= 0 ? c.slot[u.lead] : -1, slot[1] = c.slot[u.first];
+		lo[0] = low_of(a, least), hi[0] = min(min(u.prefix, most + 1), c.reach(slot[0]));
+		if (w.through) lo[1] = max(u.prefix, low_of(a, least)), hi[1] = min(most + 1, c.reach(slot[1]));
+#pragma unroll
+		for (int k = 0; k < 2; ++k) base[k] = lo[k] & ~(w.box - 1), count[k] = hi[k] > lo[k] ? (hi[k] - base[k] + AW_KEYS - 1) / AW_KEYS : 0;
+	}
+	const int total = count[0] + count[1], begin = (int)min((long long)total, (long long)share * w.each), end = share == w.shares - 1 ? total : min(total, begin + w.each), tiles = end - begin;
+
+	if (warp < 8) {
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AW_SOFTMAX_REGS));
+		const int group = warp >> 2;
+		const int rpos = s.row_pos[tid], rlow = low_of(a, rpos), wide = low_of(a, most);
+		const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), scores_at = lanes + 128 * group, sums_at = lanes + O_COL + 128 * group;
+		const float qscale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * A16_LOG2E;
+		float m = -INFINITY, l = 0.f;
+		if (group < groups) {
+			for (int i = 0; i < tiles; ++i) {
+				const int at = begin + i, part = at >= count[0], pos0 = part ? base[1] + (at - count[0]) * AW_KEYS : base[0] + at * AW_KEYS;
+				if (!ap_wait_warp(s.mask_full + i % AW_MASKS, i / AW_MASKS & 1, &s.lost) || !ap_wait_warp(s.s_full + group, i & 1, &s.lost)) break;
+				tc_fence_after();
+				const uint4 seen = *reinterpret_cast<const uint4*>(s.seen[i % AW_MASKS]);
+				const bool all = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && pos0 >= wide && pos0 + AW_KEYS - 1 <= least;
+				const float ref = m == -INFINITY ? 0.f : m, most_z = m == -INFINITY ? -INFINITY : A16_MOST;
+				float z[128]; // log2 of the weights against the reference as it stands (against 0 before there is one)
+				tmem_ld128(scores_at, z);
+				if (a.softcap > 0.f) {
+					const float cap = a.softcap * A16_LOG2E;
+#pragma unroll
+					for (int k = 0; k < 128; ++k) z[k] = fmaf(cap, tanhf(z[k] * qscale), -ref);
+				} else {
+					const u64 by = pair_of(qscale, qscale), off = pair_of(-ref, -ref);
+#pragma unroll
+					for (int k = 0; k < 128; k += 2) {
+						const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), by, off));
+						z[k] = x.x, z[k + 1] = x.y;
+					}
+				}
+				if (!all) {
+					const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
+					const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
+#pragma unroll
+					for (int x = 0; x < 4; ++x) {
+						const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
+						const uint32_t below = t >= 32 ? 0xffffffffu : (1u << t) - 1, under = f >= 32 ? 0xffffffffu : (1u << f) - 1, see = words[x] & below & ~under;
+#pragma unroll
+						for (int k = 0; k < 32; ++k)
+							if (!(see >> k & 1)) z[32 * x + k] = -INFINITY;
+					}
+				}
+				float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+				for (int k = 0; k < 128; k += 2) tops[k / 2 % 4] = fmaxf(fmaxf(tops[k / 2 % 4], z[k]), z[k + 1]);
+				const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+				if (__any_sync(0xffffffffu, top > most_z)) { // references move
+					const float mn = top > most_z ? ref + top - A16_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = ref - (mn == -INFINITY ? 0.f : mn);
+#pragma unroll
+					for (int k = 0; k < 128; ++k) z[k] += by;
+					m = mn, l *= f;
+					if (i > 0) { // there are sums; the product that wrote them was issued before these scores'
+#pragma unroll 1
+						for (int col = 0; col < D; col += 8) tmem_scale8(sums_at + col, f);
+						tmem_st_wait();
+					}
+				}
+				u64 sum = 0;
+				uint32_t p[64];
+#pragma unroll
+				for (int k = 0; k < 128; k += 2) {
+					const float w0 = ex2(z[k]), w1 = ex2(z[k + 1]);
+					sum = add2(sum, pair_of(w0, w1));
+					p[k / 2] = pack2<T>(w0, w1);
+				}
+				tmem_st32(scores_at, *reinterpret_cast<uint32_t(*)[32]>(p)); // where the scores were
+				tmem_st32(scores_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
+				const float2 both = halves(sum);
+				l += both.x + both.y;
+				tmem_st_wait();
+				tc_fence_before();
+				__syncwarp();
+				if (lane == 0) mbar_arrive(s.p_full + group);
+			}
+			if (tiles > 0) ap_wait_warp(s.done + group, 0, &s.lost);
+			tc_fence_after();
+			const bool lost = *(volatile int*)&s.lost;
+			const int token = u.t0 + (row0 + min(tid, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(tid, rows - 1)) % a.group;
+			const bool writes = tid < rows && rpos >= 0;
+			const size_t place = ((size_t)token * a.heads + head) * a.places + w.place + share;
+			float norm = 1.f;
+			if (w.place < 0) {
+				const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY, mn = fmaxf(m, sk), down = m == -INFINITY ? 0.f : ex2(m - mn);
+				l *= down;
+				if (a.sinks) l += at_sink(sk, mn);
+				norm = l > 0.f ? down / l : l == 0.f ? 0.f : l; // (0: nothing was seen; a NaN stays one)
+			} else if (writes) a.stats[place] = make_float2(lost ? 0.f : m, lost ? NAN : l);
+			if (lost) norm = NAN;
+			const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
+#pragma unroll 1
+			for (int col = 0; col < c.dim; col += 16) {
+				float v[16];
+				__syncwarp(); // (rows behind the last one take part in the load)
+				if (tiles > 0) tmem_ld16(sums_at + col, v);
+				else {
+#pragma unroll
+					for (int k = 0; k < 16; ++k) v[k] = 0.f;
+				}
+				if (!writes) continue;
+				if (w.place >= 0) {
+					if (m == -INFINITY && !lost) continue; // (the fold leaves out what weighs nothing)
+					float4* const to = reinterpret_cast<float4*>(a.sums + place * c.dim + col);
+#pragma unroll
+					for (int k = 0; k < 4; ++k) to[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+				} else {
+					uint16_t* const to = a.out + token * a.o_row + head * a.o_head + col;
+					if (vec) {
+						uint32_t x[8];
+#pragma unroll
+						for (int k = 0; k < 8; ++k) x[k] = pack2<T>(v[2 * k] * norm, v[2 * k + 1] * norm);
+						reinterpret_cast<uint4*>(to)[0] = make_uint4(x[0], x[1], x[2], x[3]), reinterpret_cast<uint4*>(to)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+					} else {
+#pragma unroll
+						for (int k = 0; k < 16; ++k) to[k] = round16<T>(v[k] * norm);
+					}
+				}
+			}
+		}
+	} else {
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AW_OTHER_REGS));
+		if (warp == 8) {
+			// Copies: lane l brings panel l % PANELS of box l / PANELS of every tile, keys first.  Nothing waits for the table where it is asked.
+			const int boxes = AW_KEYS / w.box, box = lane / PANELS, panel = lane % PANELS, none = c.pages * c.heads * c.page; // (a row past the pool reads as zeros)
+			const bool mine = box < boxes;
+			int next = -1;
+			auto start = [&](int i, int& part) { // first position of tile i
+				const int at = begin + i;
+				part = at >= count[0];
+				return part ? base[1] + (at - count[0]) * AW_KEYS : base[0] + at * AW_KEYS;
+			};
+			auto look = [&](int i) { // the page of this lane's box
+				int part;
+				const int pos = start(i, part) + box * w.box, at = c.page_index(pos);
+				const bool some = mine && i < tiles && pos < (part ? hi[1] : hi[0]) && at < c.table_pages;
+				next = some ? __ldg(c.table + (size_t)(part ? slot[1] : slot[0]) * c.table_pages + at) : -1;
+			};
+			uint32_t fixes = 0;
+			int issued = 0; // slots asked for
+			if (tiles > 0) look(0);
+			for (int i = 0; i < tiles; ++i) {
+				int part;
+				const int pos0 = start(i, part), pos = pos0 + box * w.box, l0 = (part ? lo[1] : lo[0]) - pos0, h0 = (part ? hi[1] : hi[0]) - pos0;
+				const bool some = (unsigned)next < (unsigned)c.pages;
+				const int row = some ? (next * c.heads + kvh) * c.page + c.page_row(pos) : none;
+				const uint32_t have = __ballot_sync(0xffffffffu, some && panel == 0); // bit box * PANELS
+				look(i + 1);
+				uint32_t word = 0; // keys 32 lane .. of the tile that are there, for the first four lanes
+				if (lane < 4) {
+#pragma unroll 4
+					for (int k = 0; k < 32; k += 8)
+						if (have >> ((32 * lane + k) / w.box * PANELS) & 1) word |= 0xffu << k;
+					const int f = min(max(l0 - 32 * lane, 0), 32), t = min(max(h0 - 32 * lane, 0), 32);
+					word &= (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
+					s.seen[i % AW_MASKS][lane] = word;
+				}
+				const bool whole = __all_sync(0xffffffffu, lane >= 4 || word == 0xffffffffu);
+				__syncwarp();
+				if (lane == 0) mbar_arrive(s.mask_full + i % AW_MASKS);
+				// keys
+				int sl = issued % SLOTS;
+				if (!ap_wait_warp(s.empty + sl, (issued / SLOTS & 1) ^ 1, &s.lost)) break;
+				if (lane == 0) mbar_expect_tx(s.full + sl, PANELS * AW_KEYS * 128);
+				__syncwarp();
+				if (mine) tma_load_2d(s.kv[sl][panel] + box * w.box * 128, &tm_k, panel * 64, row, s.full + sl);
+				++issued;
+				// values; those of keys that are not there are zeros, whatever lies there
+				sl = issued % SLOTS;
+				if (!ap_wait_warp(s.empty + sl, (issued / SLOTS & 1) ^ 1, &s.lost)) break;
+				uint64_t* const bar = whole ? s.full + sl : &s.fix;
+				if (lane == 0) mbar_expect_tx(bar, PANELS * AW_KEYS * 128);
+				__syncwarp();
+				if (mine) tma_load_2d(s.kv[sl][panel] + box * w.box * 128, &tm_v, panel * 64, row, bar);
+				++issued;
+				if (!whole) {
+					if (!ap_wait_warp(&s.fix, fixes & 1, &s.lost)) break;
+					++fixes;
+					for (int k = 0; k < AW_KEYS; ++k)
+						if (!(__shfl_sync(0xffffffffu, word, k >> 5) >> (k & 31) & 1) && lane < 8 * PANELS) *reinterpret_cast<uint4*>(s.kv[sl][lane >> 3] + k * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+					fence_async_smem();
+					__syncwarp();
+					if (lane == 0) mbar_arrive(s.full + sl);
+				}
+			}
+			if (*(volatile int*)&s.lost) // given up: no copy is left in flight when the block's memory goes
+				for (int k = max(0, issued - SLOTS); k < issued; ++k) mbar_wait_warp(s.full + k % SLOTS, k / SLOTS & 1, 1u << 12);
+		} else if (warp == 9 && lane == 0) {
+			constexpr uint32_t type = std::is_same<T, bf16>::value ? (1u << 7) | (1u << 10) : 0;
+			constexpr uint32_t score = (1u << 4) | type | ((uint32_t)(AW_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows; values: columns side by side
+			auto scores = [&](int g, int sl) {
+#pragma unroll
+				for (int pn = 0; pn < PANELS; ++pn)
+#pragma unroll
+					for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * g, umma_desc_sw128(s.q[g][pn]) + 2 * k, umma_desc_sw128(s.kv[sl][pn]) + 2 * k, score, (pn | k) ? 1u : 0u);
+				umma_commit(s.s_full + g);
+			};
+			auto wait_slot = [&](int k) { return ap_wait(s.full + k % SLOTS, k / SLOTS & 1, &s.lost); };
+			bool good = tiles > 0 && wait_slot(0);
+			if (good) {
+				tc_fence_after();
+				for (int g = 0; g < groups; ++g) scores(g, 0);
+				umma_commit(s.empty);
+			}
+			for (int i = 0; i < tiles && good; ++i) {
+				const int v = (2 * i + 1) % SLOTS, k = (2 * i + 2) % SLOTS;
+				const bool more = i + 1 < tiles;
+				if (!(good = wait_slot(2 * i + 1) && (!more || wait_slot(2 * i + 2)))) break;
+				for (int g = 0; g < groups; ++g) {
+					if (!(good = ap_wait(s.p_full + g, i & 1, &s.lost))) break;
+					tc_fence_after();
+#pragma unroll
+					for (int x = 0; x < AW_KEYS / 16; ++x) umma_f16_ts(tmem + O_COL + 128 * g, tmem + 128 * g + 8 * x, umma_desc_values(s.kv[v]) + 128 * x, value, (i | x) ? 1u : 0u);
+					if (more) scores(g, k);
+					else umma_commit(s.done + g);
+				}
+				if (!good) break;
+				umma_commit(s.empty + v);
+				if (more) umma_commit(s.empty + k);
+			}
+			umma_commit(&s.idle); // nothing of this block's is left in the tensor core when its memory goes
+			mbar_wait_bounded(&s.idle, 0);
+		}
+	}
+	__syncwarp();
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
 // Folds the shares of one (token, head), in the order of their places: a warp for each.
 template <typename T>
 __global__ void __launch_bounds__(128) k_c16_fold(const C16 c, const Attend a) {
 	pdl_wait_prev();
 	const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-	if (!there(c, a.rows, b)) return;
-	const int n = c.count[b], start = c.start[b];
-	const int from = a.before && !(c.groups && (unsigned)c.group[b] < (unsigned)c.groups) ? a.before : 0; // (a sequence of no group has no shares of a prefix)
+	Unit u;
+	if (!own_unit(c, a, b, u)) return;
+	const int n = u.tokens, start = u.t0, from = u.lead < 0 ? a.before : 0; // (a sequence of no group has no shares of a prefix)
 	for (long long row = (long long)blockIdx.x * 4 + warp; row < (long long)n * a.group; row += gridDim.x * 4) {
 		const int token = start + (int)(row / a.group), head = kvh * a.group + (int)(row % a.group);
 		const size_t place = ((size_t)token * a.heads + head) * a.places;
@@ -571,36 +935,73 @@ __global__ void __launch_bounds__(128) k_c16_fold(const C16 c, const Attend a) {
 }
 
 // ---------------------------------------------------------------- the host's side
-// How the work is cut: rows of a CTA, shares of a tile's keys and the chunks of each, whether a cluster folds the shares.
+// How the work is cut.  Three ways: few rows of each group or sequence, prefix and own keys in one list (ROWS); the groups' prefixes as tiles of many rows, then every sequence's own keys (PREFIXES); every sequence as tiles of many
+// rows (TILES).
+enum A16Way { A16_ROWS, A16_PREFIXES, A16_TILES };
 struct A16Plan {
-	int tile, shares, each, cluster;
-	int units; // of the grid
-	long long most_rows; // of a unit
+	int way;
+	int tile, shares, each, cluster; // few rows: rows of a CTA, shares of a tile's keys and the chunks of each, whether a cluster folds the shares
+	int units;                       // of the grid
+	long long rows;                  // of a unit at most
+	Wide wide;                       // many rows
+	int wide_units;
+	int before, places;
 };
-constexpr int AR_ROOM = 148 * 3; // CTAs that run at a time
+constexpr int AR_ROOM = 148 * 3; // CTAs of few rows that run at a time
+constexpr int AW_ROOM = 148;     // and of many
+constexpr int AW_SHARES = 32;    // of a tile's keys at most (a lane for each where they are folded)
 
+int a16_box(int page) { // keys that lie side by side in every page, as a copy's box has them
+	int box = 1;
+	while (box < 64 && page % (2 * box) == 0) box *= 2;
+	return box;
+}
+void rows_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, int group, int units, long long rows, long long keys, bool clusters) {
+	r.rows = rows, r.tile = rows > 8 ? 16 : 8;
+	const int chunks = std::max(1, (int)std::min<long long>(cdiv(keys, AR_KEYS), INT_MAX / 2));
+	const long long n = std::max(1LL, (long long)units * cdiv(rows, r.tile) * c.heads), room = AR_ROOM;
+	long long shares = n >= room ? 1 : n > room / 2 ? cdiv(6 * room, n) : room / n;
+	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, n > room / 2 ? 2 * AR_WARPS : AR_WARPS), (long long)AR_SHARES}));
+	r.cluster = clusters && shares > 1 && n <= room / 2;
+	if (r.cluster) shares = shares >= 16 ? 16 : shares >= 8 ? 8 : shares >= 4 ? 4 : 2;
+	r.each = cdiv(chunks, shares), r.shares = r.cluster ? (int)shares : cdiv(chunks, r.each);
+}
+void wide_plan(A16Plan& r, const SeqCache16& c, int units, long long rows, long long keys) {
+	r.wide_units = units, r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256);
+	const long long n = std::max(1LL, (long long)units * r.wide.tiles * c.heads);
+	const int tiles = std::max(1, (int)std::min<long long>(cdiv(keys, AW_KEYS), INT_MAX / 2));
+	const long long shares = std::max(1LL, std::min({(long long)AW_ROOM / n, (long long)cdiv(tiles, 2), (long long)AW_SHARES}));
+	r.wide.each = cdiv(tiles, shares), r.wide.shares = cdiv(tiles, r.wide.each);
+}
 A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, const SeqAttend16& a) {
 	A16Plan r = {};
 	const int group = a.heads / c.heads, groups = s ? s->n : 0;
-	const long long tokens = std::max<long long>(p.longest, groups ? s->tokens : 0), rows = tokens * group;
-	r.units = p.n + groups, r.most_rows = rows;
-	const int units = groups ? std::max(groups, 1) : p.n; // (about: which sequences are in no group is the device's to know)
-	auto ctas = [&](int tile) { return (long long)units * cdiv(rows, tile) * c.heads; };
-	r.tile = rows > 8 ? 16 : 8;
-	const int own = groups ? std::max(s->most_own, 1) : std::max(a.most_keys, 1);
-	long long keys = (groups ? s->longest : 0) + (long long)own * (groups ? std::min<long long>(cdiv(r.tile, group), std::max(s->tokens, 1)) : 1);
-	if (a.window > 0) keys = std::min(keys, (long long)a.window + r.tile / group + own);
-	const int chunks = std::max(1, (int)std::min<long long>(cdiv(keys, AR_KEYS), INT_MAX / 2));
-	const long long n = std::max(1LL, ctas(r.tile)), room = AR_ROOM;
-	long long shares = n >= room ? 1 : n > room / 2 ? cdiv(6 * room, n) : room / n;
-	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, n > room / 2 ? 2 * AR_WARPS : AR_WARPS), (long long)AR_SHARES}));
-	r.cluster = shares > 1 && n <= room / 2;
-	if (r.cluster) shares = shares >= 16 ? 16 : shares >= 8 ? 8 : shares >= 4 ? 4 : 2;
-	r.each = cdiv(chunks, shares), r.shares = r.cluster ? (int)shares : cdiv(chunks, r.each);
+	const long long rows = (long long)p.longest * group, packed = groups ? (long long)s->tokens * group : 0;
+	const long long shared = groups ? s->longest : 0, own = std::max(1, groups ? s->most_own : a.most_keys);
+	auto seen = [&](long long keys, long long tokens) { return a.window > 0 ? std::min(keys, (long long)a.window + tokens) : keys; };
+	const bool wide = (c.dim == 64 || (c.dim > 64 && c.dim <= 128)) && c.page % 8 == 0 && c.pages > 0;
+	if (wide && rows >= 96) {
+		r.way = A16_TILES;
+		wide_plan(r, c, p.n, rows, seen(std::max(1, a.most_keys), 256 / group + 1));
+		r.wide.through = 1, r.places = r.wide.shares > 1 ? r.wide.shares : 0, r.wide.place = r.places ? 0 : -1;
+		return r;
+	}
+	if (wide && packed >= 48 && shared >= 512) {
+		r.way = A16_PREFIXES;
+		wide_plan(r, c, groups, packed, seen(shared, own));
+		r.before = r.wide.shares;
+		r.units = p.n;
+		rows_plan(r, c, p, group, p.n, rows, seen(own, 16), false);
+		r.places = r.before + (r.shares > 1 ? r.shares : 0);
+		return r;
+	}
+	r.way = A16_ROWS, r.units = p.n + groups;
+	const long long most = std::max(rows, packed), together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 1; // sequences of a CTA's rows at most
+	rows_plan(r, c, p, group, groups ? groups : p.n, most, seen(shared + own * together, 16 + own), true); // (about: which sequences are in no group is the device's to know)
+	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
-int a16_places(const A16Plan& p) { return p.shares > 1 && !p.cluster ? p.shares : 0; }
-size_t a16_bytes(const SeqCache16& c, const SeqAttend16& a, const A16Plan& p) { return (size_t)a.q.rows * a.heads * a16_places(p) * (c.dim * sizeof(float) + sizeof(float2)); }
+size_t a16_bytes(const SeqCache16& c, const SeqAttend16& a, const A16Plan& p) { return (size_t)a.q.rows * a.heads * p.places * (c.dim * sizeof(float) + sizeof(float2)); }
 
 int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s, const SeqAttend16* a) {
 	if (const int rc = check_cache16("attend16", c, p)) return rc;
@@ -636,6 +1037,36 @@ template <typename T, int D>
 cudaError_t rows_tile(int tile, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
 	return tile == 8 ? rows_launch<T, D, 1>(c, a, grid, after, st) : rows_launch<T, D, 2>(c, a, grid, after, st);
 }
+// a pool as rows of dim channels; boxes of 64 channels and `box` rows, swizzled by the row
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+cudaError_t pool_map(CUtensorMap& m, const SeqCache16& c, void* pool, int box) {
+	static const EncodeFn encode = [] {
+		cudaDriverEntryPointQueryResult found;
+		void* fn = nullptr;
+		return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess ? (EncodeFn)fn : nullptr;
+	}();
+	const cuuint64_t dims[2] = {(cuuint64_t)c.dim, (cuuint64_t)c.pages * c.heads * c.page}, strides[1] = {(cuuint64_t)c.dim * 2};
+	const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+	if (!encode || encode(&m, c.type == SEQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pool, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+	                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+		return cudaErrorInvalidValue;
+	return cudaSuccess;
+}
+template <typename T, int D>
+cudaError_t tiles_launch(const SeqCache16& cache, const C16& c, const Attend& a, const A16Plan& p, cudaStream_t st) {
+	static std::atomic<uint64_t> done{0};
+	CUtensorMap mk, mv;
+	cudaError_t e = pool_map(mk, cache, cache.k, p.wide.box);
+	if (e == cudaSuccess) e = pool_map(mv, cache, cache.v, p.wide.box);
+	if (e == cudaSuccess) e = allow(k_c16_tiles<T, D>, sizeof(AwShared<D>), done);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c16_tiles<T, D>, dim3(p.wide.tiles * c.heads * p.wide.shares, 1, p.wide_units), dim3(AW_THREADS), sizeof(AwShared<D>), mk, mv, c, a, p.wide);
+	return e;
+}
+template <typename T>
+cudaError_t tiles_wide(const SeqCache16& cache, const C16& c, const Attend& a, const A16Plan& p, cudaStream_t st) {
+	return c.dim == 64 ? tiles_launch<T, 64>(cache, c, a, p, st) : tiles_launch<T, 128>(cache, c, a, p, st);
+}
 template <typename T>
 cudaError_t rows_wide(int tile, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
 	return c.dim <= 64 ? rows_tile<T, 64>(tile, c, a, grid, after, st) : c.dim <= 128 ? rows_tile<T, 128>(tile, c, a, grid, after, st) : rows_tile<T, 256>(tile, c, a, grid, after, st);
@@ -663,14 +1094,17 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 	Attend a = {};
 	a.q = (const uint16_t*)q->q.p, a.q_row = q->q.row_stride, a.q_head = q->q.head_stride, a.out = (uint16_t*)q->out.p, a.o_row = q->out.row_stride, a.o_head = q->out.head_stride;
 	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap, a.window = q->window, a.sinks = q->sinks;
-	a.families = 1, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = 0, a.places = a16_places(plan);
+	a.families = plan.way == A16_ROWS, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = plan.before, a.places = plan.places;
 	a.sums = (float*)q->workspace, a.stats = (float2*)(a.sums + (size_t)a.rows * a.heads * a.places * c.dim);
-	const dim3 grid(cdiv(plan.most_rows, plan.tile), cache->heads * plan.shares, plan.units);
+	const dim3 grid(plan.way == A16_TILES ? 1 : cdiv(plan.rows, plan.tile), cache->heads * std::max(1, plan.shares), plan.units);
 	if (grid.y > 65535) return refuse("attend16: too many key heads");
+	if ((long long)plan.wide.tiles * cache->heads * plan.wide.shares > INT_MAX) return refuse("attend16: too many rows");
 	const cudaStream_t st = (cudaStream_t)stream;
 	const bool half = cache->type == SEQ_F16;
-	cudaError_t e = half ? rows_wide<__half>(plan.tile, c, a, grid, false, st) : rows_wide<bf16>(plan.tile, c, a, grid, false, st);
-	if (e == cudaSuccess && a.places) {
+	cudaError_t e = cudaSuccess;
+	if (plan.way != A16_ROWS) e = half ? tiles_wide<__half>(*cache, c, a, plan, st) : tiles_wide<bf16>(*cache, c, a, plan, st);
+	if (e == cudaSuccess && plan.way != A16_TILES) e = half ? rows_wide<__half>(plan.tile, c, a, grid, plan.before > 0, st) : rows_wide<bf16>(plan.tile, c, a, grid, plan.before > 0, st);
+	if (e == cudaSuccess && plan.places > plan.before) {
 		const dim3 fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 		e = launch(st, true, 1, half ? k_c16_fold<__half> : k_c16_fold<bf16>, fold, dim3(128), 0, c, a);
 	}
