@@ -9,17 +9,22 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 // A pair of channels (a, b) of a row at position p becomes (a cos - b sin, b cos + a sin) at the angle 2 pi p turns_i.  The angle is a product in 64 bits of which the whole turns are taken off
-// before it becomes fp32: 2^31 positions are as exact as one.  One launch for everything: queries, keys and values are one list of units (U neighbouring channels of a head, with the U
-// channels that they turn with where the pairs lie in two halves), a thread takes one unit of TURN_DEPTH tokens, asking for all of them before it uses the first; cosines and sines of the CTA's tokens
-// come from shared memory.
-constexpr int TURN_THREADS = 256, TURN_DEPTH = 4;
-constexpr int TURN_ANGLES = 4096; // cosines and sines of a CTA at most: 32 KB
+// before it becomes fp32: 2^31 positions are as exact as one.  A thread keeps one unit of channels (U neighbours of a head, with the U that they turn with where the pairs lie in two halves) of one token: it forms
+// the unit's cosines and sines once, in registers, and takes one head after another, asking for TURN_DEPTH of them before it uses the first.  Queries, keys and values are one launch.
+// Bound: memory.  11315 rows of 40 heads of 128 bf16 channels (232 MB) 44 us, 5.2 TB/s; 10383 rows of 32 query heads stored with 8 of keys and values (248 MB) 47 us, 5.3 TB/s; one token 2.4 and 2.9 us, a launch's latency.
+// (us of the two: blocks of 256 threads 50 and 54, of 64 45 and 46; TURN_DEPTH 4 44 and 51; TURN_HEADS 8 42 and 49, 20 47 and 49; angles through shared memory and a barrier 103 and 127.)
+constexpr int TURN_THREADS = 128, TURN_DEPTH = 2;
+constexpr int TURN_BLOCKS = 148 * 4; // blocks to keep every SM busy
+constexpr int TURN_HEADS = 16;       // heads of a thread at most
 
 struct TurnRows {
 	const void* p;
 	void* out; // queries: where they go
 	long long row, head, out_row, out_head;
 	int vec, out_vec; // a unit at a time
+};
+struct TurnPart { // how the threads of a block share a part's work: columns of units, heads
+	int columns, heads, side, each, blocks; // side: threads side by side on one column of a token, each: heads of a thread, blocks: of the grid for a token's heads
 };
 struct Turn {
 	TurnRows q, k, v;
@@ -32,28 +37,47 @@ struct Turn {
 	int q_heads, heads, dim;  // heads: of the cache, 0 without one
 	int pairs;                // pairs of channels
 	int page, page_shift, pages, slots, table_pages;
-	int turned, rest;         // units of a head that turn and that do not
-	int q_units, k_units, units; // units of a token's queries, its queries and keys, all of them
-	int q_rest;               // units of a query that are copied (0: in place)
-	int groups, step;         // of threads: each takes TURN_DEPTH tokens and every step'th unit
+	int turned;               // columns that turn
+	int in_place;             // 1: the columns of a query that do not turn are where they belong
+	int tokens;               // of a block
+	int spread;               // blocks that share a token's columns
+	TurnPart turn, copy;      // queries and keys; values
 };
 
+// a unit as it lies in memory, and as floats
 template <typename T, int U>
-__device__ __forceinline__ void load_unit(const T* p, bool vec, float (&x)[U]) {
-	constexpr int BYTES = U * sizeof(T);
-	if (!vec || BYTES < 4) {
+struct Raw {
+	static constexpr int BYTES = U * sizeof(T), WORDS = (BYTES + 3) / 4;
+	uint32_t w[WORDS];
+	__device__ __forceinline__ void load(const T* p, bool vec) {
+		if (BYTES < 4 || (!vec && sizeof(T) == 2)) {
+			const uint16_t* const h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-		for (int i = 0; i < U; ++i) x[i] = as_f32(p[i]);
-	} else if constexpr (BYTES == 32) {
-		const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-		x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-	} else {
-		typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2, uint32_t>::type>::type w = *reinterpret_cast<const decltype(w)*>(p);
-		const T* h = reinterpret_cast<const T*>(&w);
+			for (int i = 0; i < WORDS; ++i) w[i] = BYTES < 4 ? h[0] : h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+		} else if (!vec || BYTES == 4) {
 #pragma unroll
-		for (int i = 0; i < U; ++i) x[i] = as_f32(h[i]);
+			for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+		} else if constexpr (BYTES == 8) {
+			const uint2 x = *reinterpret_cast<const uint2*>(p);
+			w[0] = x.x, w[1] = x.y;
+		} else if constexpr (BYTES >= 16) {
+#pragma unroll
+			for (int i = 0; i < WORDS; i += 4) {
+				const uint4 x = reinterpret_cast<const uint4*>(p)[i / 4];
+				w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+			}
+		}
 	}
-}
+	__device__ __forceinline__ void floats(float (&x)[U]) const {
+#pragma unroll
+		for (int i = 0; i < U; ++i)
+			if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+			else {
+				const uint16_t h = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+				x[i] = as_f32(*reinterpret_cast<const T*>(&h));
+			}
+	}
+};
 template <typename T, int U>
 __device__ __forceinline__ void store_unit(T* p, bool vec, const float (&x)[U]) {
 	constexpr int BYTES = U * sizeof(T);
@@ -75,78 +99,86 @@ __device__ __forceinline__ void store_unit(T* p, bool vec, const float (&x)[U]) 
 // T: the rows' type, C: the cache's
 template <typename T, typename C, int U, bool NEIGHBOURS>
 __global__ void __launch_bounds__(TURN_THREADS) k_turn(const Turn a) {
-	extern __shared__ float2 angles[]; // [tokens][pairs]: cosine, sine
-	const int b = blockIdx.z, n = a.count[b], p0 = a.pos0[b], start = a.start[b], tokens = a.groups * TURN_DEPTH;
-	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start) return;
-	const long long first = (long long)blockIdx.x * tokens;
-	if (first >= n) return;
-	const int i0 = (int)first, here = min(tokens, n - i0);
-	__shared__ long long place[TURN_THREADS * TURN_DEPTH]; // of each token in a pool, in rows of its first head; -1: nowhere
-	for (int i = threadIdx.x; i < here * a.pairs; i += blockDim.x) {
-		const int t = i / a.pairs;
-		const double turn = (double)(p0 + i0 + t) * a.turns[i - t * a.pairs];
-		float s, c;
-		sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
-		angles[i] = make_float2(c * a.gain, s * a.gain);
-	}
-	if (a.heads)
-		for (int t = threadIdx.x; t < here; t += blockDim.x) {
-			const int pos = p0 + i0 + t, at = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page, slot = a.slot[b];
-			const int id = (unsigned)slot < (unsigned)a.slots && at < a.table_pages ? a.table[(size_t)slot * a.table_pages + at] : -1;
-			place[t] = (unsigned)id < (unsigned)a.pages ? (long long)id * a.heads * a.page + (pos - at * a.page) : -1;
-		}
-	__syncthreads();
-	const int group = threadIdx.x / a.step;
-	if (group >= a.groups) return;
-	const int t0 = group * TURN_DEPTH;
-	for (int u = blockIdx.y * a.step + threadIdx.x % a.step; u < a.units; u += gridDim.y * a.step) {
-		const bool is_q = u < a.q_units, is_v = u >= a.k_units;
-		const TurnRows& r = is_q ? a.q : is_v ? a.v : a.k;
-		const int v = is_q ? u : is_v ? u - a.k_units : u - a.q_units, turned = is_v ? 0 : a.turned, each = turned + (is_q ? a.q_rest : is_v ? a.dim / U : a.rest);
-		const int head = v / each, w = v - head * each;
-		const bool turns = w < turned;
-		// the unit's first channel; for pairs that lie in two halves the second half's is `pairs` further
-		const int d = (turns || NEIGHBOURS || is_v ? w : w + turned) * U;
-		const T* src = (const T*)r.p + (long long)(start + i0 + t0) * r.row + head * r.head + d;
-		float x[TURN_DEPTH][U], y[TURN_DEPTH][NEIGHBOURS ? 1 : U];
+	constexpr int ANGLES = NEIGHBOURS ? (U + 1) / 2 : U;
+	const bool is_v = blockIdx.y >= a.turn.blocks;
+	const TurnPart& part = is_v ? a.copy : a.turn;
+	const int width = min(part.columns, TURN_THREADS), at = threadIdx.x / width, column = threadIdx.x % width + blockIdx.x % a.spread * TURN_THREADS;
+	const int token = blockIdx.x / a.spread * a.tokens + at % a.tokens, side = at / a.tokens;
+	const int b = blockIdx.z, n = a.count[b], p0 = a.pos0[b], start = a.start[b];
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || token >= n || side >= part.side || column >= part.columns) return;
+	const bool turns = !is_v && column < a.turned;
+	double step[ANGLES];
+	if (turns)
 #pragma unroll
-		for (int t = 0; t < TURN_DEPTH; ++t)
-			if (t0 + t < here) {
-				load_unit<T, U>(src + t * r.row, r.vec, x[t]);
-				if constexpr (!NEIGHBOURS)
-					if (turns) load_unit<T, U>(src + t * r.row + a.pairs, r.vec, y[t]);
-			}
+		for (int i = 0; i < ANGLES; ++i) step[i] = a.turns[column * ANGLES + i];
+	// the unit's first channel; for pairs that lie in two halves the second half's is `pairs` further
+	const int d = (NEIGHBOURS || is_v || turns ? column : column + a.turned) * U, pos = p0 + token;
+	const int first = (is_v ? blockIdx.y - a.turn.blocks : blockIdx.y) * part.side * part.each + side, last = min(part.heads, first + part.side * part.each);
+	long long place = -1; // of the token in a pool, in rows of its first head; -1: nowhere
+	if (a.heads && (is_v || last > a.q_heads)) {
+		const int page = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page, slot = a.slot[b];
+		const int id = (unsigned)slot < (unsigned)a.slots && page < a.table_pages ? a.table[(size_t)slot * a.table_pages + page] : -1;
+		if ((unsigned)id < (unsigned)a.pages) place = (long long)id * a.heads * a.page + (pos - page * a.page);
+	}
+	float cosine[ANGLES], sine[ANGLES];
+	bool formed = false;
+	for (int h0 = first; h0 < last; h0 += part.side * TURN_DEPTH) {
+		Raw<T, U> x[TURN_DEPTH], y[NEIGHBOURS ? 1 : TURN_DEPTH];
 #pragma unroll
 		for (int t = 0; t < TURN_DEPTH; ++t) {
-			if (t0 + t >= here) break;
+			const int h = h0 + t * part.side;
+			if (h >= last) break;
+			const bool is_q = !is_v && h < a.q_heads;
+			if (is_q && a.in_place && !turns) continue;
+			const TurnRows& r = is_v ? a.v : is_q ? a.q : a.k;
+			const T* const src = (const T*)r.p + (long long)(start + token) * r.row + (is_v || is_q ? h : h - a.q_heads) * r.head + d;
+			x[t].load(src, r.vec);
+			if constexpr (!NEIGHBOURS)
+				if (turns) y[t].load(src + a.pairs, r.vec);
+		}
+		if (turns && !formed) { // (while the first heads are on their way)
+			formed = true;
+#pragma unroll
+			for (int i = 0; i < ANGLES; ++i) {
+				const double turn = (double)pos * step[i];
+				sincospif((float)(2.0 * (turn - rint(turn))), sine + i, cosine + i);
+				cosine[i] *= a.gain, sine[i] *= a.gain;
+			}
+		}
+#pragma unroll
+		for (int t = 0; t < TURN_DEPTH; ++t) {
+			const int h = h0 + t * part.side;
+			if (h >= last) break;
+			const bool is_q = !is_v && h < a.q_heads;
+			if (is_q && a.in_place && !turns) continue;
+			float u[U], v[NEIGHBOURS ? 1 : U];
+			x[t].floats(u);
 			if (turns) {
-				const float2* const cs = angles + (t0 + t) * a.pairs + (NEIGHBOURS ? d / 2 : d);
 				if constexpr (NEIGHBOURS) {
 #pragma unroll
 					for (int i = 0; i + 1 < U; i += 2) {
-						const float2 f = cs[i / 2];
-						const float p = x[t][i], q = x[t][i + 1];
-						x[t][i] = p * f.x - q * f.y, x[t][i + 1] = q * f.x + p * f.y;
+						const float p = u[i], q = u[i + 1];
+						u[i] = p * cosine[i / 2] - q * sine[i / 2], u[i + 1] = q * cosine[i / 2] + p * sine[i / 2];
 					}
 				} else {
+					y[t].floats(v);
 #pragma unroll
 					for (int i = 0; i < U; ++i) {
-						const float2 f = cs[i];
-						const float p = x[t][i], q = y[t][i];
-						x[t][i] = p * f.x - q * f.y, y[t][i] = q * f.x + p * f.y;
+						const float p = u[i], q = v[i];
+						u[i] = p * cosine[i] - q * sine[i], v[i] = q * cosine[i] + p * sine[i];
 					}
 				}
 			}
 			if (is_q) {
-				T* const to = (T*)r.out + (long long)(start + i0 + t0 + t) * r.out_row + head * r.out_head + d;
-				store_unit<T, U>(to, r.out_vec, x[t]);
+				T* const to = (T*)a.q.out + (long long)(start + token) * a.q.out_row + h * a.q.out_head + d;
+				store_unit<T, U>(to, a.q.out_vec, u);
 				if constexpr (!NEIGHBOURS)
-					if (turns) store_unit<T, U>(to + a.pairs, r.out_vec, y[t]);
-			} else if (place[t0 + t] >= 0) {
-				C* const to = (C*)(is_v ? a.vc : a.kc) + (place[t0 + t] + (long long)head * a.page) * a.dim + d;
-				store_unit<C, U>(to, true, x[t]); // (rows of a cache are 16-byte aligned)
+					if (turns) store_unit<T, U>(to + a.pairs, a.q.out_vec, v);
+			} else if (place >= 0) {
+				C* const to = (C*)(is_v ? a.vc : a.kc) + (place + (long long)(is_v ? h : h - a.q_heads) * a.page) * a.dim + d;
+				store_unit<C, U>(to, true, u); // (rows of a cache are 16-byte aligned)
 				if constexpr (!NEIGHBOURS)
-					if (turns) store_unit<C, U>(to + a.pairs, true, y[t]);
+					if (turns) store_unit<C, U>(to + a.pairs, true, v);
 			}
 		}
 	}
@@ -166,21 +198,21 @@ bool turn_vec(const void* p, long long row, long long head, int type, int u) {
 }
 
 template <typename T, typename C, int U>
-cudaError_t turn_of(bool neighbours, const Turn& a, dim3 grid, int threads, size_t smem, cudaStream_t st) {
-	return neighbours ? launch(st, false, 1, k_turn<T, C, U, true>, grid, dim3(threads), smem, a) : launch(st, false, 1, k_turn<T, C, U, false>, grid, dim3(threads), smem, a);
+cudaError_t turn_of(bool neighbours, const Turn& a, dim3 grid, int threads, cudaStream_t st) {
+	return neighbours ? launch(st, false, 1, k_turn<T, C, U, true>, grid, dim3(threads), 0, a) : launch(st, false, 1, k_turn<T, C, U, false>, grid, dim3(threads), 0, a);
 }
 template <typename T, typename C>
-cudaError_t turn_unit(int unit, bool neighbours, const Turn& a, dim3 grid, int threads, size_t smem, cudaStream_t st) {
+cudaError_t turn_unit(int unit, bool neighbours, const Turn& a, dim3 grid, int threads, cudaStream_t st) {
 	switch (unit) {
-	case 8: return turn_of<T, C, 8>(neighbours, a, grid, threads, smem, st);
-	case 4: return turn_of<T, C, 4>(neighbours, a, grid, threads, smem, st);
-	case 2: return turn_of<T, C, 2>(neighbours, a, grid, threads, smem, st);
-	default: return turn_of<T, C, 1>(false, a, grid, threads, smem, st);
+	case 8: return turn_of<T, C, 8>(neighbours, a, grid, threads, st);
+	case 4: return turn_of<T, C, 4>(neighbours, a, grid, threads, st);
+	case 2: return turn_of<T, C, 2>(neighbours, a, grid, threads, st);
+	default: return turn_of<T, C, 1>(false, a, grid, threads, st);
 	}
 }
 template <typename T>
-cudaError_t turn_type(int cache, int unit, bool neighbours, const Turn& a, dim3 grid, int threads, size_t smem, cudaStream_t st) {
-	return cache == SEQ_F16 ? turn_unit<T, __half>(unit, neighbours, a, grid, threads, smem, st) : turn_unit<T, bf16>(unit, neighbours, a, grid, threads, smem, st);
+cudaError_t turn_type(int cache, int unit, bool neighbours, const Turn& a, dim3 grid, int threads, cudaStream_t st) {
+	return cache == SEQ_F16 ? turn_unit<T, __half>(unit, neighbours, a, grid, threads, st) : turn_unit<T, bf16>(unit, neighbours, a, grid, threads, st);
 }
 
 TurnRows turn_rows(const SeqRows& r) {
@@ -209,27 +241,33 @@ int turn(const char* what, const SeqPortions& batch, const SeqRotation* rotation
 	a.dim = dim, a.pairs = dims / 2, a.start = batch.start, a.count = batch.count, a.slot = batch.slot, a.pos0 = batch.pos0;
 	if (rotation) a.turns = rotation->turns, a.gain = rotation->gain;
 	while (unit > 1 && ((neighbours ? dims : dims / 2) % unit || (dim - dims) % unit)) unit /= 2;
-	a.turned = (neighbours ? dims : dims / 2) / unit, a.rest = (dim - dims) / unit;
-	// Rest units begin behind the turned channels: with two halves these are twice as many as their units
-	a.q_rest = q && q->p == q_out->p && q->row_stride == q_out->row_stride && q->head_stride == q_out->head_stride ? 0 : a.rest;
-	const long long q_units = (long long)a.q_heads * (a.turned + a.q_rest), k_units = q_units + (long long)a.heads * (a.turned + a.rest), units = k_units + (long long)a.heads * (dim / unit);
-	if (units > INT_MAX / 2) return refuse("%s: %d heads of %d channels are too many", what, q_heads, dim);
-	if (!units || !batch.n || !batch.longest) return 0;
-	a.q_units = (int)q_units, a.k_units = (int)k_units, a.units = (int)units;
+	a.turned = (neighbours ? dims : dims / 2) / unit;
+	a.in_place = q && q->p == q_out->p && q->row_stride == q_out->row_stride && q->head_stride == q_out->head_stride;
+	if (!(a.q_heads + a.heads) || !batch.n || !batch.longest) return 0;
 	a.q.vec = q && turn_vec(a.q.p, a.q.row, a.q.head, type, unit), a.q.out_vec = q && turn_vec(a.q.out, a.q.out_row, a.q.out_head, type, unit);
 	a.k.vec = cache && turn_vec(a.k.p, a.k.row, a.k.head, type, unit), a.v.vec = cache && turn_vec(a.v.p, a.v.row, a.v.head, type, unit);
-	// a CTA's threads take all units of TURN_DEPTH tokens in as few rounds as they can, and more tokens where units are few; where tokens are few, several CTAs share a token's units
-	const int rounds = cdiv(units, TURN_THREADS);
-	a.step = (int)std::min<long long>(TURN_THREADS, cdiv(units, rounds));
-	a.groups = std::max(1, std::min({TURN_THREADS / a.step, cdiv(batch.longest, TURN_DEPTH), a.pairs ? TURN_ANGLES / (TURN_DEPTH * a.pairs) : TURN_ANGLES / 8}));
-	const int threads = cdiv(a.step * a.groups, 32) * 32, blocks = cdiv(batch.longest, a.groups * TURN_DEPTH);
-	const int split = (long long)blocks * batch.n < 2 * 148 ? std::min(rounds, 64) : 1;
-	const size_t smem = (size_t)a.groups * TURN_DEPTH * a.pairs * sizeof(float2);
-	const dim3 grid(blocks, split, batch.n);
+	// a block: as many tokens as its threads have room for, where tokens are few several heads at once; heads go to several blocks while these are few
+	a.turn.columns = a.turned + (dim - dims) / unit, a.copy.columns = dim / unit;
+	a.turn.heads = a.q_heads + a.heads, a.copy.heads = a.heads;
+	const int widest = cache ? a.copy.columns : a.turn.columns; // (of the two)
+	a.tokens = std::max(1, std::min(batch.longest, TURN_THREADS / widest));
+	a.spread = cdiv(widest, TURN_THREADS);
+	const int blocks = cdiv(batch.longest, a.tokens);
+	int threads = 32;
+	for (TurnPart* p : {&a.turn, &a.copy}) {
+		if (!p->heads) continue;
+		p->side = std::max(1, std::min(p->heads, TURN_THREADS / (p->columns * a.tokens)));
+		const int rounds = cdiv(p->heads, p->side), most = (int)std::max<long long>(1, TURN_BLOCKS / ((long long)blocks * batch.n));
+		p->each = cdiv(rounds, std::min(rounds, std::max(most, cdiv(rounds, TURN_HEADS))));
+		p->blocks = cdiv(rounds, p->each);
+		threads = std::max(threads, cdiv(std::min(p->columns, TURN_THREADS) * a.tokens * p->side, 32) * 32);
+	}
+	const dim3 grid((unsigned)((long long)blocks * a.spread), a.turn.blocks + a.copy.blocks, batch.n);
+	if (grid.y > 65535 || (long long)blocks * a.spread > INT_MAX) return refuse("%s: %d heads of %d channels are too many", what, a.turn.heads, dim);
 	const int ctype = cache ? cache->type : SEQ_BF16;
-	const cudaError_t e = type == SEQ_F32 ? turn_type<float>(ctype, unit, neighbours, a, grid, threads, smem, stream)
-	                      : type == SEQ_BF16 ? turn_type<bf16>(ctype, unit, neighbours, a, grid, threads, smem, stream)
-	                                         : turn_type<__half>(ctype, unit, neighbours, a, grid, threads, smem, stream);
+	const cudaError_t e = type == SEQ_F32 ? turn_type<float>(ctype, unit, neighbours, a, grid, threads, stream)
+	                      : type == SEQ_BF16 ? turn_type<bf16>(ctype, unit, neighbours, a, grid, threads, stream)
+	                                         : turn_type<__half>(ctype, unit, neighbours, a, grid, threads, stream);
 	return e == cudaSuccess ? 0 : failed(what, e);
 }
 } // namespace

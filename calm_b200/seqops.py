@@ -282,10 +282,10 @@ def _grouped(shared, cn: np.ndarray, at: np.ndarray) -> Tuple[np.ndarray, np.nda
 
 def _rows(name: str, t: torch.Tensor, index: int, heads: int, dim: int, least: int) -> _Rows:
     _gpu(name, t, index)
-    kind, stride = _TYPES.get(t.dtype), t.stride()
-    if kind is None or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (stride[2] != 1 and dim > 1):
+    kind, shape, stride = _TYPES.get(t.dtype), t.shape, t.stride()
+    if kind is None or len(shape) != 3 or shape[1] != heads or shape[2] != dim or (stride[2] != 1 and dim > 1):
         raise ValueError(f"{name} must be [tokens, {heads}, {dim}] in float32, bfloat16 or float16 with the channels contiguous, not {list(t.shape)} {t.dtype}")
-    n = t.shape[0]
+    n = shape[0]
     if n < least:
         raise ValueError(f"{name} has {n} rows for {least} tokens")
     return _Rows(t.data_ptr(), kind, stride[0], stride[1], min(n, 2 ** 31 - 1))
@@ -446,7 +446,7 @@ def _beside(rotation: Rotation, batch: Batch, index: int) -> None:
 
 def _like(x: torch.Tensor, tokens: int) -> torch.Tensor:
     """Where rows like x's go: what is behind the batch's tokens is zero."""
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if x.shape[0] == tokens else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty_like(x) if x.shape[0] == tokens else torch.zeros_like(x)
 
 
 def rotate(x: torch.Tensor, batch: Batch, rotation: Rotation, out: Optional[torch.Tensor] = None) -> torch.Tensor:

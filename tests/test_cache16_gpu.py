@@ -71,7 +71,7 @@ def as_was(x, n):
 @pytest.mark.parametrize("pairs", ["halves", "neighbours"])
 @pytest.mark.parametrize("heads,dim,dims,counts,before", [
     (32, 128, 128, [1], [4000]), (1, 2, 2, [1, 3], [0, 7]), (3, 64, 32, [5, 1, 2], [0, 100, 31]), (14, 80, 20, [130, 77], [3, 900000]), (2, 256, 256, [700], [0]), (7, 96, 12, [33], [5]),
-    (40, 128, 128, [513, 1, 0, 64], [0, 9, 5, 8191]), (1, 1024, 1024, [9], [2 ** 31 - 10]), (5, 6, 4, [300], [12]), (65, 192, 96, [3], [1])])
+    (40, 128, 128, [513, 1, 0, 64], [0, 9, 5, 8191]), (1, 1024, 1024, [9], [2 ** 31 - 10]), (5, 6, 4, [300], [12]), (65, 192, 96, [3], [1]), (3, 1022, 6, [2, 5], [8, 0]), (2, 770, 770, [3], [50])])
 def test_rotated_rows(heads, dim, dims, counts, before, pairs, dtype):
     x = torch.randn(sum(counts), heads, dim, generator=gen(dim + heads), device="cuda").to(DT[dtype])
     check_rotate(x, counts, before, seqops.Rotation(dims, 10000.0, pairs))
