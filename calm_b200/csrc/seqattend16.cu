@@ -28,6 +28,7 @@ struct Attend {
 	uint16_t* out;
 	long long o_row, o_head;
 	int rows, heads, group; // group: query heads a key head
+	int out_vec;            // four channels of a result at a time
 	float scale, softcap;
 	int window;
 	const float* sinks;
@@ -91,6 +92,15 @@ __device__ __forceinline__ uint16_t round16(float x) {
 	const T h = from_f32<T>(x);
 	return *reinterpret_cast<const uint16_t*>(&h);
 }
+// four neighbouring channels of a result
+template <typename T>
+__device__ __forceinline__ void put4(uint16_t* to, bool vec, const float4& v) {
+	const uint2 w = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+	if (vec) *reinterpret_cast<uint2*>(to) = w;
+	else to[0] = (uint16_t)w.x, to[1] = (uint16_t)(w.x >> 16), to[2] = (uint16_t)w.y, to[3] = (uint16_t)(w.y >> 16);
+}
+__device__ __forceinline__ void add4(float4& v, float f, const float4& x) { v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w); }
+__device__ __forceinline__ float4 times4(const float4& v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 // whether one of the two halves is infinite or no number
 template <typename T>
 __device__ __forceinline__ bool odd2(uint32_t x) {
@@ -140,6 +150,21 @@ __device__ __forceinline__ bool own_unit(const C16& c, const Attend& a, int b, U
 	}
 	u.first = u.last = b, u.t0 = c.start[b], u.tokens = c.count[b];
 	return true;
+}
+// v += what the shares at up to 32 places hold of four channels; lane k has the weight of place k.  All of them are asked for before one is used; where nothing weighs, nothing may have been written.
+__device__ __forceinline__ void add_places(float4& v, const float* p, int dim, int places, float weight) {
+#pragma unroll 1
+	for (int k0 = 0; k0 < places; k0 += 8) {
+		float4 x[8];
+#pragma unroll
+		for (int k = 0; k < 8; ++k)
+			if (k0 + k < places) x[k] = __ldg(reinterpret_cast<const float4*>(p + (size_t)(k0 + k) * dim));
+#pragma unroll
+		for (int k = 0; k < 8; ++k) {
+			const float f = __shfl_sync(0xffffffffu, weight, k0 + k);
+			if (k0 + k < places && f != 0.f) add4(v, f, x[k]);
+		}
+	}
 }
 __device__ __forceinline__ int low_of(const Attend& a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
 
@@ -473,30 +498,25 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 				den = den * down + warp_sum(pw * pl);
 				if (a.sinks) den += at_sink(sk, top);
 				const float norm = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
-				for (int d0 = 0; d0 < dim; d0 += 32) {
-					const int d = d0 + lane;
-					float v = 0.f;
-					if (d < dim) {
+				for (int d0 = 0; d0 < dim; d0 += 128) {
+					const int d = min(d0 + 4 * lane, dim - 4); // (every lane has a place's weight)
+					float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-						for (int w = 0; w < AR_WARPS; ++w) v = fmaf(wt[w], sums[(w * 8 + rr) * LD + d], v);
-						v *= down;
-					}
-					for (int k = 0; k < prefix_places; ++k) {
-						const float f = __shfl_sync(0xffffffffu, pw, k);
-						if (f != 0.f && d < dim) v = fmaf(f, a.sums[(place + k) * dim + d], v);
-					}
-					if (d < dim) a.out[token * a.o_row + head * a.o_head + d] = round16<T>(v * norm);
+					for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w] * down, *reinterpret_cast<const float4*>(sums + (w * 8 + rr) * LD + d));
+					add_places(v, a.sums + place * dim + d, dim, prefix_places, pw);
+					if (d0 + 4 * lane < dim) put4<T>(a.out + token * a.o_row + head * a.o_head + d, a.out_vec, times4(v, norm));
 				}
 			} else {
 				float2* const st = a.cluster ? reinterpret_cast<float2*>(own + r * (D + 2) + D) : a.stats + place + a.before + share;
 				float* const to = a.cluster ? own + r * (D + 2) : a.sums + (place + a.before + share) * dim;
 				if (lane == 0) *st = make_float2(mx, den);
 				if (mx != -INFINITY || a.cluster)
-					for (int d = lane; d < dim; d += 32) {
-						float v = 0.f;
+					for (int d = 4 * lane; d < dim; d += 128) {
+						float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-						for (int w = 0; w < AR_WARPS; ++w) v = fmaf(wt[w], sums[(w * 8 + rr) * LD + d], v);
-						to[d] = v;
+						for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w], *reinterpret_cast<const float4*>(sums + (w * 8 + rr) * LD + d));
+						if (a.cluster) to[d] = v.x, to[d + 1] = v.y, to[d + 2] = v.z, to[d + 3] = v.w; // (rows of the cluster's sums are 8-byte aligned)
+						else *reinterpret_cast<float4*>(to + d) = v;
 					}
 			}
 		}
@@ -553,7 +573,7 @@ struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	unsigned char q[2][PANELS][128 * 128];
 	unsigned char kv[SLOTS][PANELS][AW_KEYS * 128]; // keys and values in turn
 	uint64_t full[SLOTS], empty[SLOTS], mask_full[AW_MASKS], s_full[2], p_full[2], done[2], fix, idle;
-	uint32_t seen[AW_MASKS][4]; // keys that are there
+	alignas(16) uint32_t seen[AW_MASKS][4]; // keys that are there
 	int row_pos[256];
 	int span[4]; // the rows' least and largest position (of warps that found them)
 	uint32_t tmem;
@@ -575,13 +595,18 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
 #undef AW_R8
 #undef AW_R32
 }
+__device__ __forceinline__ float max_nan(float x, float y) { // NaN where one of them is
+	float r;
+	asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+	return r;
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 	asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
 	             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
 	             : "r"(taddr)
 	             : "memory");
 }
-// shared-memory descriptor of values [keys][64 channels], 128-byte swizzle, panels of 64 channels 16 KB apart: the product's columns are the channels, its depth the keys, eight keys 1024 bytes apart
+// shared-memory descriptor of values [keys][64 channels], 128-byte swizzle, panels of 64 channels one behind another: the product's columns are the channels, its depth the keys, eight keys 1024 bytes apart
 __device__ __forceinline__ uint64_t umma_desc_values(const void* tile) {
 	const uint64_t addr = (uint64_t)(smem_u32(tile) & 0x3FFFF) >> 4;
 	return addr | ((uint64_t)(AW_KEYS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -590,7 +615,7 @@ __device__ __forceinline__ uint64_t umma_desc_values(const void* tile) {
 struct Wide {
 	int through;    // 1: every sequence's rows over its group's prefix and its own keys; 0: every group's rows over its prefix
 	int box;        // keys that a copy brings
-	int shares, each; // of a tile's keys, tiles of 128 of each
+	int shares, each; // of a tile's keys, tiles of each
 	int tiles;      // of 256 rows, of the longest unit
 	int place;      // the first share's in stats and sums; -1: results go to out
 };
@@ -680,55 +705,72 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				tc_fence_after();
 				const uint4 seen = *reinterpret_cast<const uint4*>(s.seen[i % AW_MASKS]);
 				const bool all = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && pos0 >= wide && pos0 + AW_KEYS - 1 <= least;
-				const float ref = m == -INFINITY ? 0.f : m, most_z = m == -INFINITY ? -INFINITY : A16_MOST;
-				float z[128]; // log2 of the weights against the reference as it stands (against 0 before there is one)
+				const bool steady = __all_sync(0xffffffffu, all && m != -INFINITY) && !(a.softcap > 0.f) && a.scale > 0.f;
+				float z[128];
+				uint32_t p[64];
+				u64 sum = 0;
 				tmem_ld128(scores_at, z);
-				if (a.softcap > 0.f) {
-					const float cap = a.softcap * A16_LOG2E;
+				bool moves = true;
+				if (steady) { // the reference as it stands, unless a score passes it or is no number
+					float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-					for (int k = 0; k < 128; ++k) z[k] = fmaf(cap, tanhf(z[k] * qscale), -ref);
-				} else {
-					const u64 by = pair_of(qscale, qscale), off = pair_of(-ref, -ref);
+					for (int k = 0; k < 128; k += 2) tops[k / 2 % 4] = max_nan(max_nan(tops[k / 2 % 4], z[k]), z[k + 1]);
+					const float top = max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3]));
+					moves = __any_sync(0xffffffffu, !(fmaf(top, qscale, -m) <= A16_MOST));
+					if (!moves) {
+						const u64 by = pair_of(qscale, qscale), off = pair_of(-m, -m);
+#pragma unroll
+						for (int k = 0; k < 128; k += 2) {
+							const float2 y = halves(fma2(pair_of(z[k], z[k + 1]), by, off));
+							const float w0 = ex2(y.x), w1 = ex2(y.y);
+							sum = add2(sum, pair_of(w0, w1));
+							p[k / 2] = pack2<T>(w0, w1);
+						}
+					}
+				}
+				if (moves) {
+					const float ref = m == -INFINITY ? 0.f : m, most_z = m == -INFINITY ? -INFINITY : A16_MOST;
+					if (a.softcap > 0.f) {
+						const float cap = a.softcap * A16_LOG2E;
+#pragma unroll
+						for (int k = 0; k < 128; ++k) z[k] = fmaf(cap, tanhf(z[k] * qscale), -ref); // log2 of the weights against the reference (against 0 before there is one)
+					} else {
+#pragma unroll
+						for (int k = 0; k < 128; ++k) z[k] = fmaf(z[k], qscale, -ref);
+					}
+					if (!all) {
+						const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
+						const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
+#pragma unroll
+						for (int x = 0; x < 4; ++x) {
+							const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
+							const uint32_t see = words[x] & (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
+#pragma unroll
+							for (int k = 0; k < 32; ++k)
+								if (!(see >> k & 1)) z[32 * x + k] = -INFINITY;
+						}
+					}
+					float top = -INFINITY;
+#pragma unroll
+					for (int k = 0; k < 128; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
+					if (__any_sync(0xffffffffu, top > most_z)) { // references move
+						const float mn = top > most_z ? ref + top - A16_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), down = ref - (mn == -INFINITY ? 0.f : mn);
+#pragma unroll
+						for (int k = 0; k < 128; ++k) z[k] += down;
+						m = mn, l *= f;
+						if (i > 0) { // there are sums; the product that wrote them was issued before these scores'
+#pragma unroll 1
+							for (int col = 0; col < D; col += 8) tmem_scale8(sums_at + col, f);
+							tmem_st_wait();
+						}
+					}
+					sum = 0;
 #pragma unroll
 					for (int k = 0; k < 128; k += 2) {
-						const float2 x = halves(fma2(pair_of(z[k], z[k + 1]), by, off));
-						z[k] = x.x, z[k + 1] = x.y;
+						const float w0 = ex2(z[k]), w1 = ex2(z[k + 1]);
+						sum = add2(sum, pair_of(w0, w1));
+						p[k / 2] = pack2<T>(w0, w1);
 					}
-				}
-				if (!all) {
-					const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
-					const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
-#pragma unroll
-					for (int x = 0; x < 4; ++x) {
-						const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
-						const uint32_t below = t >= 32 ? 0xffffffffu : (1u << t) - 1, under = f >= 32 ? 0xffffffffu : (1u << f) - 1, see = words[x] & below & ~under;
-#pragma unroll
-						for (int k = 0; k < 32; ++k)
-							if (!(see >> k & 1)) z[32 * x + k] = -INFINITY;
-					}
-				}
-				float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-				for (int k = 0; k < 128; k += 2) tops[k / 2 % 4] = fmaxf(fmaxf(tops[k / 2 % 4], z[k]), z[k + 1]);
-				const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-				if (__any_sync(0xffffffffu, top > most_z)) { // references move
-					const float mn = top > most_z ? ref + top - A16_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), by = ref - (mn == -INFINITY ? 0.f : mn);
-#pragma unroll
-					for (int k = 0; k < 128; ++k) z[k] += by;
-					m = mn, l *= f;
-					if (i > 0) { // there are sums; the product that wrote them was issued before these scores'
-#pragma unroll 1
-						for (int col = 0; col < D; col += 8) tmem_scale8(sums_at + col, f);
-						tmem_st_wait();
-					}
-				}
-				u64 sum = 0;
-				uint32_t p[64];
-#pragma unroll
-				for (int k = 0; k < 128; k += 2) {
-					const float w0 = ex2(z[k]), w1 = ex2(z[k + 1]);
-					sum = add2(sum, pair_of(w0, w1));
-					p[k / 2] = pack2<T>(w0, w1);
 				}
 				tmem_st32(scores_at, *reinterpret_cast<uint32_t(*)[32]>(p)); // where the scores were
 				tmem_st32(scores_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
@@ -785,10 +827,11 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		}
 	} else {
 		asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AW_OTHER_REGS));
-		if (warp == 8) {
-			// Copies: lane l brings panel l % PANELS of box l / PANELS of every tile, keys first.  Nothing waits for the table where it is asked.
-			const int boxes = AW_KEYS / w.box, box = lane / PANELS, panel = lane % PANELS, none = c.pages * c.heads * c.page; // (a row past the pool reads as zeros)
-			const bool mine = box < boxes;
+		if (warp == 8 || warp == 11) {
+			// Copies: one warp the keys', one the values'.  Lane l looks up the page of box l of every tile, a tile ahead: nothing waits for the table where it is asked.
+			const bool values = warp == 11;
+			const CUtensorMap* const map = values ? &tm_v : &tm_k;
+			const int boxes = AW_KEYS / w.box, none = c.pages * c.heads * c.page; // (a row past the pool reads as zeros)
 			int next = -1;
 			auto start = [&](int i, int& part) { // first position of tile i
 				const int at = begin + i;
@@ -797,48 +840,46 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			};
 			auto look = [&](int i) { // the page of this lane's box
 				int part;
-				const int pos = start(i, part) + box * w.box, at = c.page_index(pos);
-				const bool some = mine && i < tiles && pos < (part ? hi[1] : hi[0]) && at < c.table_pages;
+				const int pos = start(i, part) + lane * w.box, at = c.page_index(pos);
+				const bool some = lane < boxes && i < tiles && pos < (part ? hi[1] : hi[0]) && at < c.table_pages;
 				next = some ? __ldg(c.table + (size_t)(part ? slot[1] : slot[0]) * c.table_pages + at) : -1;
 			};
 			uint32_t fixes = 0;
-			int issued = 0; // slots asked for
+			int issued = 0; // tiles asked for
 			if (tiles > 0) look(0);
 			for (int i = 0; i < tiles; ++i) {
 				int part;
-				const int pos0 = start(i, part), pos = pos0 + box * w.box, l0 = (part ? lo[1] : lo[0]) - pos0, h0 = (part ? hi[1] : hi[0]) - pos0;
+				const int pos0 = start(i, part), l0 = (part ? lo[1] : lo[0]) - pos0, h0 = (part ? hi[1] : hi[0]) - pos0;
 				const bool some = (unsigned)next < (unsigned)c.pages;
-				const int row = some ? (next * c.heads + kvh) * c.page + c.page_row(pos) : none;
-				const uint32_t have = __ballot_sync(0xffffffffu, some && panel == 0); // bit box * PANELS
+				const int row = some ? (next * c.heads + kvh) * c.page + c.page_row(pos0 + lane * w.box) : none;
+				const uint32_t have = __ballot_sync(0xffffffffu, some);
 				look(i + 1);
 				uint32_t word = 0; // keys 32 lane .. of the tile that are there, for the first four lanes
 				if (lane < 4) {
 #pragma unroll 4
 					for (int k = 0; k < 32; k += 8)
-						if (have >> ((32 * lane + k) / w.box * PANELS) & 1) word |= 0xffu << k;
+						if (have >> ((32 * lane + k) / w.box) & 1) word |= 0xffu << k;
 					const int f = min(max(l0 - 32 * lane, 0), 32), t = min(max(h0 - 32 * lane, 0), 32);
 					word &= (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
-					s.seen[i % AW_MASKS][lane] = word;
+					if (!values) s.seen[i % AW_MASKS][lane] = word;
 				}
-				const bool whole = __all_sync(0xffffffffu, lane >= 4 || word == 0xffffffffu);
+				const bool whole = !values || __all_sync(0xffffffffu, lane >= 4 || word == 0xffffffffu);
 				__syncwarp();
-				if (lane == 0) mbar_arrive(s.mask_full + i % AW_MASKS);
-				// keys
-				int sl = issued % SLOTS;
-				if (!ap_wait_warp(s.empty + sl, (issued / SLOTS & 1) ^ 1, &s.lost)) break;
-				if (lane == 0) mbar_expect_tx(s.full + sl, PANELS * AW_KEYS * 128);
-				__syncwarp();
-				if (mine) tma_load_2d(s.kv[sl][panel] + box * w.box * 128, &tm_k, panel * 64, row, s.full + sl);
-				++issued;
-				// values; those of keys that are not there are zeros, whatever lies there
-				sl = issued % SLOTS;
-				if (!ap_wait_warp(s.empty + sl, (issued / SLOTS & 1) ^ 1, &s.lost)) break;
+				if (!values && lane == 0) mbar_arrive(s.mask_full + i % AW_MASKS);
+				const int k = 2 * i + values, sl = k % SLOTS;
+				if (!ap_wait_warp(s.empty + sl, (k / SLOTS & 1) ^ 1, &s.lost)) break;
 				uint64_t* const bar = whole ? s.full + sl : &s.fix;
 				if (lane == 0) mbar_expect_tx(bar, PANELS * AW_KEYS * 128);
-				__syncwarp();
-				if (mine) tma_load_2d(s.kv[sl][panel] + box * w.box * 128, &tm_v, panel * 64, row, bar);
+				unsigned char* to = s.kv[sl][0];
+				for (int x = 0; x < boxes; ++x, to += w.box * 128) {
+					const int r = __shfl_sync(0xffffffffu, row, x);
+					if (lane == 0) {
+#pragma unroll
+						for (int pn = 0; pn < PANELS; ++pn) tma_load_2d(to + pn * AW_KEYS * 128, map, pn * 64, r, bar);
+					}
+				}
 				++issued;
-				if (!whole) {
+				if (!whole) { // values of keys that are not there are zeros, whatever lies there
 					if (!ap_wait_warp(&s.fix, fixes & 1, &s.lost)) break;
 					++fixes;
 					for (int k = 0; k < AW_KEYS; ++k)
@@ -849,8 +890,11 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				}
 			}
 			if (*(volatile int*)&s.lost) // given up: no copy is left in flight when the block's memory goes
-				for (int k = max(0, issued - SLOTS); k < issued; ++k) mbar_wait_warp(s.full + k % SLOTS, k / SLOTS & 1, 1u << 12);
-		} else if (warp == 9 && lane == 0) {
+				for (int i = max(0, issued - SLOTS); i < issued; ++i) {
+					const int k = 2 * i + values;
+					mbar_wait_warp(s.full + k % SLOTS, k / SLOTS & 1, 1u << 12);
+				}
+		} else if (warp == 9 && lane == 0) { // the products: the groups take turns
 			constexpr uint32_t type = std::is_same<T, bf16>::value ? (1u << 7) | (1u << 10) : 0;
 			constexpr uint32_t score = (1u << 4) | type | ((uint32_t)(AW_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows; values: columns side by side
 			auto scores = [&](int g, int sl) {
@@ -909,28 +953,23 @@ __global__ void __launch_bounds__(128) k_c16_fold(const C16 c, const Attend a) {
 		float mx = sk, den = 0.f;
 		for (int s = from + lane; s < a.places; s += 32) mx = fmaxf(mx, a.stats[place + s].x);
 		mx = warp_max(mx);
-		float v[8];
-#pragma unroll
-		for (int k = 0; k < 8; ++k) v[k] = 0.f;
+		float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 		for (int s0 = from; s0 < a.places; s0 += 32) {
 			const float2 st = s0 + lane < a.places ? a.stats[place + s0 + lane] : make_float2(-INFINITY, 0.f);
 			const float w = st.x == -INFINITY ? 0.f : ex2(st.x - mx);
 			den = fmaf(w, st.y, den);
-			for (int s = s0; s < min(a.places, s0 + 32); ++s) {
-				const float f = __shfl_sync(0xffffffffu, w, s - s0);
-				if (f == 0.f) continue; // (nothing may have been written there)
-				const float* const p = a.sums + (place + s) * c.dim;
 #pragma unroll
-				for (int k = 0; k < 8; ++k)
-					if (32 * k + lane < c.dim) v[k] = fmaf(f, p[32 * k + lane], v[k]);
+			for (int k = 0; k < 2; ++k) {
+				const int d = min(128 * k + 4 * lane, c.dim - 4);
+				if (128 * k < c.dim) add_places(v[k], a.sums + (place + s0) * c.dim + d, c.dim, min(a.places - s0, 32), w);
 			}
 		}
 		den = warp_sum(den);
 		if (a.sinks) den += at_sink(sk, mx);
 		const float norm = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
 #pragma unroll
-		for (int k = 0; k < 8; ++k)
-			if (32 * k + lane < c.dim) a.out[token * a.o_row + head * a.o_head + 32 * k + lane] = round16<T>(v[k] * norm);
+		for (int k = 0; k < 2; ++k)
+			if (128 * k + 4 * lane < c.dim) put4<T>(a.out + token * a.o_row + head * a.o_head + 128 * k + 4 * lane, a.out_vec, times4(v[k], norm));
 	}
 }
 
@@ -1094,6 +1133,7 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 	Attend a = {};
 	a.q = (const uint16_t*)q->q.p, a.q_row = q->q.row_stride, a.q_head = q->q.head_stride, a.out = (uint16_t*)q->out.p, a.o_row = q->out.row_stride, a.o_head = q->out.head_stride;
 	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap, a.window = q->window, a.sinks = q->sinks;
+	a.out_vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 8 == 0;
 	a.families = plan.way == A16_ROWS, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = plan.before, a.places = plan.places;
 	a.sums = (float*)q->workspace, a.stats = (float2*)(a.sums + (size_t)a.rows * a.heads * a.places * c.dim);
 	const dim3 grid(plan.way == A16_TILES ? 1 : cdiv(plan.rows, plan.tile), cache->heads * std::max(1, plan.shares), plan.units);
