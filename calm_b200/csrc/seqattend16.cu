@@ -69,11 +69,11 @@ constexpr size_t ar_smem() { return (size_t)8 * NQ * D * 2 + ar_ring<D>(); }
 template <typename T>
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
 	if constexpr (std::is_same<T, bf16>::value)
-		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+		asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 	else
-		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+		asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
@@ -101,11 +101,16 @@ __device__ __forceinline__ void put4(uint16_t* to, bool vec, const float4& v) {
 }
 __device__ __forceinline__ void add4(float4& v, float f, const float4& x) { v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w); }
 __device__ __forceinline__ float4 times4(const float4& v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
-// whether one of the two halves is infinite or no number
+// `sum` becomes no number where one of the two halves is infinite or no number
 template <typename T>
-__device__ __forceinline__ bool odd2(uint32_t x) {
-	constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00;
-	return (x & E) == E || (x >> 16 & E) == E;
+__device__ __forceinline__ void odd2(uint32_t x, uint32_t& sum) {
+	if constexpr (std::is_same<T, bf16>::value) {
+		const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __nv_bfloat162(__float2bfloat16_rn(0.f), __float2bfloat16_rn(0.f)), *reinterpret_cast<const __nv_bfloat162*>(&sum));
+		sum = *reinterpret_cast<const uint32_t*>(&r);
+	} else {
+		const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2(__float2half_rn(0.f), __float2half_rn(0.f)), *reinterpret_cast<const __half2*>(&sum));
+		sum = *reinterpret_cast<const uint32_t*>(&r);
+	}
 }
 // The halves that are finite, the others as zero; `inf`: +-1 for each infinity, `nan`: 1 for each that is no number (zero else)
 template <typename T>
@@ -166,6 +171,14 @@ __device__ __forceinline__ void add_places(float4& v, const float* p, int dim, i
 		}
 	}
 }
+// cap tanh(s) of x = -2 log2(e) s: (1 - t) / (1 + t) with t = 2^-|x|, two units of the special functions.  Off by 2^-21 cap at most: t by 2 steps (2^-22 of it), its difference from 1 by as much, the quotient's
+// reciprocal by 2^-23 and two roundings.
+__device__ __forceinline__ float capped(float x, float cap) {
+	const float t = ex2(-fabsf(x));
+	return copysignf(cap * __fdividef(1.f - t, 1.f + t), -x);
+}
+// chunks of the keys lo .. hi - 1, the first of which begins at a multiple of a chunk
+__device__ __forceinline__ int chunks_of(int lo, int hi) { return hi > lo ? (hi - lo / AR_KEYS * AR_KEYS + AR_KEYS - 1) / AR_KEYS : 0; }
 __device__ __forceinline__ int low_of(const Attend& a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
 
 template <typename T, int D, int NQ>
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	uint2* const qf = reinterpret_cast<uint2*>(ar_sm); // B fragments [KS][NQ][32]
 	ArStage<D>* const ring = reinterpret_cast<ArStage<D>*>(ar_sm + (size_t)TILE * D * 2);
 	__shared__ float fold_m[AR_WARPS][TILE], fold_l[AR_WARPS][TILE];
-	__shared__ int row_seq[TILE], row_pos[TILE], row_seg[TILE];
+	__shared__ int row_seq[TILE], row_pos[TILE], row_seg[TILE], row_slot[TILE];
 	__shared__ int seg_slot[TILE + 1], seg_lo[TILE + 1], seg_hi[TILE + 1], seg_base[TILE + 1]; // the prefix and the sequences of the tile's rows: keys lo .. hi - 1 of a slot, first chunk
 	__shared__ int list[4];                                                                     // segments, chunks, the rows' least and largest position
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -185,7 +198,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	if (a.before) pdl_launch_next();
 	const int z = blockIdx.z;
 	bool some_rows = a.families && z < c.groups ? group_unit(c, a, z, u) : own_unit(c, a, a.families ? z - c.groups : z, u);
-	if (a.families && z >= c.groups && some_rows && u.lead >= 0) some_rows = false; // (its group has it)
+	if (some_rows && ((a.families && z >= c.groups && u.lead >= 0) || (u.first == u.last && !there(c, a.rows, u.first)))) some_rows = false; // (a sequence that its group has; a group of one that makes no sense)
 	if (!some_rows || (long long)blockIdx.x * TILE >= (long long)u.tokens * a.group) {
 		if (a.before) pdl_wait_prev();
 		return;
@@ -193,44 +206,69 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	const int row0 = blockIdx.x * TILE, rows = (int)min((long long)TILE, (long long)u.tokens * a.group - row0);
 	const int H = c.heads, dim = c.dim;
 
-	// which sequence and position each row has
-	if (tid < TILE) row_seq[tid] = row_pos[tid] = -1;
-	__syncthreads();
-	for (int b = u.first + tid; b <= u.last; b += 32 * AR_WARPS)
-		if (there(c, a.rows, b)) {
-			const long long r0 = (long long)(c.start[b] - u.t0) * a.group - row0, r1 = r0 + (long long)c.count[b] * a.group;
-			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) row_seq[r] = b, row_pos[r] = c.pos0[b] + (int)((r - r0) / a.group);
-		}
-	__syncthreads();
-	if (warp == 0) {
-		const int seq = lane < TILE ? row_seq[lane] : -1, pos = lane < TILE ? row_pos[lane] : -1;
-		const int left = __shfl_up_sync(0xffffffffu, seq, 1), right = __shfl_down_sync(0xffffffffu, seq, 1);
-		const bool head = seq >= 0 && (lane == 0 || left != seq), tail = seq >= 0 && (lane == 31 || right != seq);
-		const uint32_t heads = __ballot_sync(0xffffffffu, head);
-		const int seg = __popc(heads & (0xffffffffu >> (31 - lane))); // (1: the first; 0: the prefix)
-		const int least = __reduce_min_sync(0xffffffffu, seq >= 0 ? pos : INT_MAX), most = __reduce_max_sync(0xffffffffu, pos);
-		if (lane < TILE) row_seg[lane] = seq >= 0 ? seg : -1;
-		if (head) {
-			const int slot = c.slot[seq];
-			seg_slot[seg] = slot, seg_lo[seg] = max(u.prefix, low_of(a, pos));
-		}
-		if (tail) seg_hi[seg] = min(pos + 1, c.reach(c.slot[seq]));
-		if (lane == 0) {
-			const bool with = a.families && u.prefix > 0 && least != INT_MAX;
-			const int slot = with ? c.slot[u.lead] : -1;
-			seg_slot[0] = slot, seg_lo[0] = with ? low_of(a, least) : 0, seg_hi[0] = with ? min(min(u.prefix, most + 1), c.reach(slot)) : 0;
-		}
-		__syncwarp();
-		const int segs = __popc(heads) + 1;
-		int chunks = lane < segs ? (max(seg_hi[lane] - seg_lo[lane], 0) + AR_KEYS - 1) / AR_KEYS : 0, sum = chunks;
+	// the queries are asked for first
+	constexpr int QF = KS * NQ * 32 / (32 * AR_WARPS) > 0 ? KS * NQ * 32 / (32 * AR_WARPS) : 1; // fragments of a thread
+	uint2 qx[QF];
 #pragma unroll
-		for (int o = 1; o < 32; o *= 2) {
-			const int x = __shfl_up_sync(0xffffffffu, sum, o);
-			if (lane >= o) sum += x;
-		}
-		if (lane < segs) seg_base[lane] = sum - chunks;
-		if (lane == segs - 1) list[0] = segs, list[1] = sum, list[2] = least, list[3] = most;
+	for (int f = 0; f < QF; ++f) {
+		const int i = tid + f * 32 * AR_WARPS, k = i / (NQ * 32), r = (i / 32 % NQ) * 8 + (i >> 2 & 7), d = k * 16 + (i & 3) * 2, rr = row0 + min(r, rows - 1);
+		const uint16_t* q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + d;
+		qx[f] = make_uint2(0, 0);
+		if (r < rows && d < dim) qx[f].x = q[0] | (uint32_t)q[1] << 16, qx[f].y = q[8] | (uint32_t)q[9] << 16; // (16 channels are there or not)
 	}
+	// which sequence and position each row has; the segments of the tile's list of keys: 0 the prefix, then every sequence of its rows
+	const bool alone = u.first == u.last;
+	if (alone) { // one sequence: nothing to look for
+		const int p0 = c.pos0[u.first] + (u.t0 - c.start[u.first]), low = p0 + row0 / a.group, high = p0 + (row0 + rows - 1) / a.group; // (a group of one has its sequence's rows)
+		if (tid < TILE) row_seq[tid] = tid < rows ? u.first : -1, row_pos[tid] = tid < rows ? p0 + (row0 + tid) / a.group : -1, row_seg[tid] = tid < rows ? 1 : -1;
+		if (tid == 0) {
+			const int slot = c.slot[u.first], reach = c.reach(slot);
+			const bool with = a.families && u.prefix > 0;
+			const int lo0 = with ? low_of(a, low) : 0, hi0 = with ? min(min(u.prefix, high + 1), reach) : 0, lo1 = max(u.prefix, low_of(a, low)), hi1 = min(high + 1, reach);
+			const int n0 = chunks_of(lo0, hi0), n1 = chunks_of(lo1, hi1);
+			seg_slot[0] = seg_slot[1] = slot, seg_lo[0] = lo0, seg_hi[0] = hi0, seg_lo[1] = lo1, seg_hi[1] = hi1, seg_base[0] = 0, seg_base[1] = n0;
+			list[0] = 2, list[1] = n0 + n1, list[2] = low, list[3] = high;
+		}
+	} else {
+		if (tid < TILE) row_seq[tid] = row_pos[tid] = -1;
+		const int lead_slot = c.slot[u.lead >= 0 ? u.lead : u.first];
+		__syncthreads();
+		for (int b = u.first + tid; b <= u.last; b += 32 * AR_WARPS) {
+			const int slot = c.slot[b], pos0 = c.pos0[b], start = c.start[b], count = c.count[b];
+			if (!there(c, a.rows, b)) continue;
+			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)count * a.group;
+			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) row_seq[r] = b, row_pos[r] = pos0 + (int)((unsigned)(r - r0) / (unsigned)a.group), row_slot[r] = slot;
+		}
+		__syncthreads();
+		if (warp == 0) {
+			const int seq = lane < TILE ? row_seq[lane] : -1, pos = lane < TILE ? row_pos[lane] : -1, slot = seq >= 0 ? row_slot[lane] : -1;
+			const int left = __shfl_up_sync(0xffffffffu, seq, 1), right = __shfl_down_sync(0xffffffffu, seq, 1);
+			const bool head = seq >= 0 && (lane == 0 || left != seq), tail = seq >= 0 && (lane == 31 || right != seq);
+			const uint32_t heads = __ballot_sync(0xffffffffu, head);
+			const int seg = __popc(heads & (0xffffffffu >> (31 - lane))); // (1: the first; 0: the prefix)
+			const int least = __reduce_min_sync(0xffffffffu, seq >= 0 ? pos : INT_MAX), most = __reduce_max_sync(0xffffffffu, pos);
+			if (lane < TILE) row_seg[lane] = seq >= 0 ? seg : -1;
+			if (head) seg_slot[seg] = slot, seg_lo[seg] = max(u.prefix, low_of(a, pos));
+			if (tail) seg_hi[seg] = min(pos + 1, c.reach(slot));
+			if (lane == 0) {
+				const bool with = u.prefix > 0 && least != INT_MAX;
+				seg_slot[0] = lead_slot, seg_lo[0] = with ? low_of(a, least) : 0, seg_hi[0] = with ? min(min(u.prefix, most + 1), c.reach(lead_slot)) : 0;
+			}
+			__syncwarp();
+			const int segs = __popc(heads) + 1;
+			int chunks = lane < segs ? chunks_of(seg_lo[lane], seg_hi[lane]) : 0, sum = chunks;
+#pragma unroll
+			for (int o = 1; o < 32; o *= 2) {
+				const int x = __shfl_up_sync(0xffffffffu, sum, o);
+				if (lane >= o) sum += x;
+			}
+			if (lane < segs) seg_base[lane] = sum - chunks;
+			if (lane == segs - 1) list[0] = segs, list[1] = sum, list[2] = least, list[3] = most;
+		}
+	}
+#pragma unroll
+	for (int f = 0; f < QF; ++f)
+		if (tid + f * 32 * AR_WARPS < KS * NQ * 32) qf[tid + f * 32 * AR_WARPS] = qx[f]; // B fragments
 	__syncthreads();
 	const int segs = list[0], total = list[1], least = list[2], most = list[3];
 	const int my_base = lane < segs ? seg_base[lane] : INT_MAX; // (at most 17 segments)
@@ -240,33 +278,35 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 
 	// the chunk to request: its segment, first position and end; the page of this lane's key, as the table has it: a load that nothing waits for where it is asked for
 	ArStage<D>& s = ring[warp];
-	int next = begin + warp, next_seg = 0, next_pos = 0, next_hi = 0, next_page = 0, next_row = 0;
+	int next = begin + warp, next_seg = 0, next_pos = 0, next_lo = 0, next_hi = 0, next_page = 0, next_row = 0;
 	uint32_t next_seen = 0;
 	bool page_ok = false;
 	auto look = [&]() {
 		const bool some = next < end;
-		next_seg = some ? __popc(__ballot_sync(0xffffffffu, my_base <= next)) - 1 : 0;
 		// (segments without keys start where the next one does: the last of those that start here has the chunk)
-		next_hi = seg_hi[next_seg], next_pos = seg_lo[next_seg] + (next - seg_base[next_seg]) * AR_KEYS;
+		next_seg = some ? __popc(__ballot_sync(0xffffffffu, my_base <= next)) - 1 : 0;
+		next_lo = seg_lo[next_seg], next_hi = seg_hi[next_seg], next_pos = (next_lo / AR_KEYS + next - seg_base[next_seg]) * AR_KEYS;
 		const int pos = next_pos + lane, at = c.page_index(max(pos, 0));
-		page_ok = some && pos < next_hi && at < c.table_pages;
+		page_ok = some && pos >= next_lo && pos < next_hi && at < c.table_pages;
 		next_page = page_ok ? __ldg(c.table + (size_t)seg_slot[next_seg] * c.table_pages + at) : -1;
 	};
 	look();
-	const int piece = lane % PIECES, prow = lane / PIECES; // which piece of which row of a group of 32 pieces this lane copies
+	constexpr int EACH = 32 / PIECES;                      // rows that a warp copies at a time
+	const int piece = lane % PIECES, prow = lane / PIECES; // which piece of which of them this lane copies
+	const bool eights = c.page % 8 == 0 && dim == D;       // eight keys from a multiple of eight on lie side by side
 	auto copy = [&](uint16_t* to, const uint16_t* from) { // the next chunk's keys or values
 		const uint32_t dst = smem_u32(to);
-		if (next_seen == 0xffffffffu && dim == D) {
+		if (next_seen == 0xffffffffu && eights) {
 #pragma unroll
-			for (int i = 0; i < PIECES; ++i) { // 32 rows of PIECES pieces, 32 pieces at a time
-				const int r = i * (32 / PIECES) + prow;
-				const long long o = (long long)__shfl_sync(0xffffffffu, next_row, r) * D;
-				cp16(dst + (r * PIECES + (piece ^ (r & 7))) * 16, from + o + piece * 8);
+			for (int g = 0; g < AR_KEYS / 8; ++g) {
+				const uint16_t* const src = from + (long long)__shfl_sync(0xffffffffu, next_row, g * 8) * D + prow * D + piece * 8;
+#pragma unroll
+				for (int i = 0; i < 8; i += EACH) cp16(dst + (g * 8 + i) * PIECES * 16 + prow * PIECES * 16 + (((piece ^ prow) ^ i) << 4), src + i * D);
 			}
 		} else {
-#pragma unroll
+#pragma unroll 4
 			for (int i = 0; i < PIECES; ++i) { // keys that are not there are zeros
-				const int r = i * (32 / PIECES) + prow;
+				const int r = i * EACH + prow;
 				const long long o = (long long)__shfl_sync(0xffffffffu, next_row, r) * dim;
 				const bool some = (next_seen >> r & 1) && piece * 8 < dim;
 				cp16(dst + (r * PIECES + (piece ^ (r & 7))) * 16, some ? from + o + piece * 8 : from, some);
@@ -295,23 +335,13 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	};
 	request_keys(), request_values();
 
-	// queries as B fragments
-	for (int i = tid; i < KS * NQ * 32; i += 32 * AR_WARPS) {
-		const int k = i / (NQ * 32), r = (i / 32 % NQ) * 8 + (i >> 2 & 7), d = k * 16 + (i & 3) * 2, rr = row0 + min(r, rows - 1);
-		const uint16_t* q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + d;
-		const bool some = r < rows && d < dim; // (16 channels are there or not)
-		uint2 x = make_uint2(0, 0);
-		if (some) x.x = q[0] | (uint32_t)q[1] << 16, x.y = q[8] | (uint32_t)q[9] << 16;
-		qf[i] = x;
-	}
-	__syncthreads();
 	uint2 qr[KEEP ? KS * NQ : 1];
 	if (KEEP) {
 #pragma unroll
 		for (int i = 0; i < KS * NQ; ++i) qr[i] = qf[i * 32 + lane];
 	}
 	auto qfrag = [&](int i) { return KEEP ? qr[i] : qf[i * 32 + lane]; };
-	const float qscale = a.softcap > 0.f ? a.scale : a.scale * A16_LOG2E;
+	const float qscale = a.scale * A16_LOG2E;
 
 	float acc[MT][NQ][4], m[NQ][2], l[NQ][2]; // queries 2t and 2t + 1 of each eight; m: the reference
 	int rpos[NQ][2], rseg[NQ][2];
@@ -336,30 +366,37 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		for (int i = 0; i < 2; ++i)
 #pragma unroll
 			for (int q = 0; q < NQ; ++q) z[i][q][0] = z[i][q][1] = z[i][q][2] = z[i][q][3] = 0.f;
+		// (fragments of two steps are asked for while the last two's are used)
+		constexpr int AHEAD = 2;
+		uint32_t A[2][AHEAD][2][4];
+		auto fetch = [&](int k0, uint32_t (&to)[AHEAD][2][4]) {
 #pragma unroll
-		for (int k = 0; k < KS; ++k) {
-			if (16 * k >= dim) break;
-			uint2 b[NQ];
+			for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
-			for (int q = 0; q < NQ; ++q) b[q] = qfrag(k * NQ + q);
+				for (int i = 0; i < 2; ++i) ldsm_x4(s.k + ((16 * i + (lane & 8) + lrow) * PIECES + ((2 * (k0 + k) + (lane >> 4)) ^ lrow)) * 8, to[k][i]);
+		};
+		fetch(0, A[0]);
 #pragma unroll
-			for (int i = 0; i < 2; ++i) {
-				uint32_t A[4];
-				ldsm_x4(s.k + ((16 * i + (lane & 8) + lrow) * PIECES + ((2 * k + (lane >> 4)) ^ lrow)) * 8, A);
+		for (int k0 = 0; k0 < KS; k0 += AHEAD) {
+			if (k0 + AHEAD < KS) fetch(k0 + AHEAD, A[(k0 / AHEAD + 1) & 1]);
 #pragma unroll
-				for (int q = 0; q < NQ; ++q) mma_16<T>(z[i][q], A, b[q]);
-			}
+			for (int k = 0; k < AHEAD; ++k)
+				if (16 * (k0 + k) < dim) // (channels that are not there: nothing was copied)
+#pragma unroll
+					for (int i = 0; i < 2; ++i)
+#pragma unroll
+						for (int q = 0; q < NQ; ++q) mma_16<T>(z[i][q], A[(k0 / AHEAD) & 1][k][i], qfrag((k0 + k) * NQ + q));
 		}
 		__syncwarp(); // every lane has its keys
 		request_keys();
 		if (a.softcap > 0.f) {
-			const float cap = a.softcap * A16_LOG2E, by = qscale / a.softcap;
+			const float cap = a.softcap * A16_LOG2E, by = -2.f * A16_LOG2E * a.scale / a.softcap;
 #pragma unroll
 			for (int i = 0; i < 2; ++i)
 #pragma unroll
 				for (int q = 0; q < NQ; ++q)
 #pragma unroll
-					for (int e = 0; e < 4; ++e) z[i][q][e] = cap * tanhf(z[i][q][e] * by);
+					for (int e = 0; e < 4; ++e) z[i][q][e] = capped(z[i][q][e] * by, cap);
 		} else {
 #pragma unroll
 			for (int i = 0; i < 2; ++i)
@@ -421,31 +458,56 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		asm volatile("cp.async.wait_group 1;" ::: "memory"); // the values; the next keys are the group behind them
 		__syncwarp();
 		// values: rows g and g + 8 of product i are channels 16 i + g, + 8
-#pragma unroll
-		for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-			for (int i = 0; i < MT; ++i) {
-				if (16 * i >= dim) break;
-				uint32_t A[4];
-				ldsm_x4_t(s.v + ((16 * kk + (lane >> 4) * 8 + lrow) * PIECES + ((2 * i + (lane >> 3 & 1)) ^ lrow)) * 8, A);
-				if (!all && __any_sync(0xffffffffu, odd2<T>(A[0]) || odd2<T>(A[1]) || odd2<T>(A[2]) || odd2<T>(A[3]))) { // a value that is not finite reaches the rows that see its key and no others
-					uint32_t inf[4], nan[4];
-#pragma unroll
-					for (int x = 0; x < 4; ++x) A[x] = split2<T>(A[x], inf[x], nan[x]);
-#pragma unroll
-					for (int q = 0; q < NQ; ++q) {
-						float s_inf[4] = {0.f, 0.f, 0.f, 0.f}, s_nan[4] = {0.f, 0.f, 0.f, 0.f};
-						mma_16<T>(s_inf, inf, p[kk][q]), mma_16<T>(s_nan, nan, p[kk][q]);
-#pragma unroll
-						for (int x = 0; x < 4; ++x) {
-							if (s_nan[x] != 0.f) acc[i][q][x] = NAN;
-							else if (s_inf[x] != 0.f) acc[i][q][x] += s_inf[x] * INFINITY;
-						}
-					}
+		bool odd = false; // where rows see different keys: a value that is not finite reaches the rows that see its key and no others
+		if (!all) {
+			uint32_t sum = 0;
+#pragma unroll 4
+			for (int i = 0; i < PIECES; ++i)
+				if (piece * 8 < dim) {
+					const int r = i * EACH + prow;
+					const uint4 w = *reinterpret_cast<const uint4*>(s.v + (r * PIECES + (piece ^ (r & 7))) * 8);
+					odd2<T>(w.x, sum), odd2<T>(w.y, sum), odd2<T>(w.z, sum), odd2<T>(w.w, sum);
 				}
+			odd = __any_sync(0xffffffffu, sum & 0x7fff7fff);
+		}
+		auto values = [&](int x, uint32_t (&to)[4]) { // step x: keys 16 (x / MT), channels 16 (x % MT)
+			ldsm_x4_t(s.v + ((16 * (x / MT) + (lane >> 4) * 8 + lrow) * PIECES + ((2 * (x % MT) + (lane >> 3 & 1)) ^ lrow)) * 8, to);
+		};
+		if (!odd) {
+			constexpr int DEPTH = 4;
+			uint32_t V[2][DEPTH][4];
 #pragma unroll
-				for (int q = 0; q < NQ; ++q) mma_16<T>(acc[i][q], A, p[kk][q]);
+			for (int x = 0; x < DEPTH; ++x) values(x, V[0][x]);
+#pragma unroll
+			for (int x0 = 0; x0 < 2 * MT; x0 += DEPTH) {
+				if (x0 + DEPTH < 2 * MT)
+#pragma unroll
+					for (int x = 0; x < DEPTH; ++x) values(x0 + DEPTH + x, V[(x0 / DEPTH + 1) & 1][x]);
+#pragma unroll
+				for (int x = 0; x < DEPTH; ++x)
+					if (16 * ((x0 + x) % MT) < dim)
+#pragma unroll
+						for (int q = 0; q < NQ; ++q) mma_16<T>(acc[(x0 + x) % MT][q], V[(x0 / DEPTH) & 1][x], p[(x0 + x) / MT][q]);
 			}
+		} else {
+#pragma unroll
+			for (int x = 0; x < 2 * MT; ++x) {
+				if (16 * (x % MT) >= dim) continue;
+				uint32_t V[4], inf[4], nan[4];
+				values(x, V);
+#pragma unroll
+				for (int e = 0; e < 4; ++e) V[e] = split2<T>(V[e], inf[e], nan[e]);
+#pragma unroll
+				for (int q = 0; q < NQ; ++q) {
+					float s_inf[4] = {0.f, 0.f, 0.f, 0.f}, s_nan[4] = {0.f, 0.f, 0.f, 0.f};
+					mma_16<T>(s_inf, inf, p[x / MT][q]), mma_16<T>(s_nan, nan, p[x / MT][q]), mma_16<T>(acc[x % MT][q], V, p[x / MT][q]);
+#pragma unroll
+					for (int e = 0; e < 4; ++e)
+						if (s_nan[e] != 0.f) acc[x % MT][q][e] = NAN;
+						else if (s_inf[e] != 0.f) acc[x % MT][q][e] += s_inf[e] * INFINITY;
+				}
+			}
+		}
 		__syncwarp(); // every lane has its values
 		request_values();
 	}
@@ -565,7 +627,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 // memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run.  O stays in tensor memory; it is rescaled in the rare case that
 // a row's reference moves.
 constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
-constexpr int AW_SOFTMAX_REGS = 208, AW_OTHER_REGS = 80; // 256 x 208 + 128 x 80 = 63488 of the 384 x 168 = 64512 that the block is launched with
+constexpr int AW_SOFTMAX_REGS = 200, AW_OTHER_REGS = 96; // 256 x 200 + 128 x 96 = 63488 of the 384 x 168 = 64512 that the block is launched with
 
 template <int D>
 struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
@@ -579,6 +641,10 @@ struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	uint32_t tmem;
 	int lost;
 };
+// shared -> global, 16-byte aligned, a multiple of 16 bytes
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+	asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
 // a row of scores
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
 #define AW_R8(b) "=f"(v[b]), "=f"(v[b + 1]), "=f"(v[b + 2]), "=f"(v[b + 3]), "=f"(v[b + 4]), "=f"(v[b + 5]), "=f"(v[b + 6]), "=f"(v[b + 7])
@@ -647,56 +713,79 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		mbar_init_fence();
 	}
 	if (tid < 256) s.row_pos[tid] = -1;
-	__syncthreads();
-	for (int b = u.first + tid; b <= u.last; b += AW_THREADS)
-		if (there(c, a.rows, b)) {
-			const long long r0 = (long long)(c.start[b] - u.t0) * a.group - row0, r1 = r0 + (long long)c.count[b] * a.group;
-			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) s.row_pos[r] = c.pos0[b] + (int)((r - r0) / a.group);
-		}
-	// queries, rows of 128 bytes a panel
-	{
-		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
-		for (int i = tid; i < groups * 128 * PIECES; i += AW_THREADS) {
-			const int r = i / PIECES, piece = i % PIECES, rr = row0 + min(r, rows - 1);
-			uint4 x = make_uint4(0, 0, 0, 0);
-			if (r < rows && piece * 8 < c.dim) {
-				const uint16_t* const q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + piece * 8;
-				if (vec) x = *reinterpret_cast<const uint4*>(q);
-				else
-					x = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
-			}
-			*reinterpret_cast<uint4*>(s.q[r >> 7][piece >> 3] + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4)) = x;
-		}
-		fence_async_smem();
-	}
-	__syncthreads();
-	if (warp < 8) {
-		const int pos = s.row_pos[tid];
-		const int least = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos), most = __reduce_max_sync(0xffffffffu, pos);
-		if (lane == 0) atomicMin(&s.span[0], least), atomicMax(&s.span[1], most);
-	}
-	tc_fence_before();
-	__syncthreads();
-	tc_fence_after();
-	const uint32_t tmem = s.tmem;
-	// the keys: positions lo .. hi - 1 of the prefix, then of the sequence's own, in tiles that begin where a copy may
-	const int least = s.span[0], most = s.span[1];
-	int lo[2] = {0, 0}, hi[2] = {0, 0}, base[2] = {0, 0}, count[2] = {0, 0}, slot[2] = {-1, -1};
-	if (most >= 0) {
-		slot[0] = u.lead >= 0 ? c.slot[u.lead] : -1, slot[1] = c.slot[u.first];
-		lo[0] = low_of(a, least), hi[0] = min(min(u.prefix, most + 1), c.reach(slot[0]));
-		if (w.through) lo[1] = max(u.prefix, low_of(a, least)), hi[1] = min(most + 1, c.reach(slot[1]));
+	const bool alone = u.first == u.last;
+	if (alone && !there(c, a.rows, u.first)) u.tokens = 0; // (a group of one that makes no sense: no keys, no rows)
+	const int lead_slot = u.lead >= 0 ? c.slot[u.lead] : -1, own_slot = c.slot[u.first], pos0 = c.pos0[u.first];
+	// The keys: positions lo .. hi - 1 of the prefix, then of the sequence's own, in tiles that begin where a copy may.  The copies need not wait for the rows' positions where these do not matter for the range.
+	const bool ranged = alone || a.window == 0;
+	int lo[2], hi[2], base[2], count[2], begin, tiles;
+	auto range = [&](int least, int most) {
+		lo[0] = low_of(a, least), hi[0] = min(u.prefix, c.reach(lead_slot)), lo[1] = hi[1] = 0;
+		if (alone || !ranged) hi[0] = min(hi[0], most + 1);
+		if (w.through) lo[1] = max(u.prefix, low_of(a, least)), hi[1] = min(most + 1, c.reach(own_slot));
 #pragma unroll
-		for (int k = 0; k < 2; ++k) base[k] = lo[k] & ~(w.box - 1), count[k] = hi[k] > lo[k] ? (hi[k] - base[k] + AW_KEYS - 1) / AW_KEYS : 0;
+		for (int k = 0; k < 2; ++k) base[k] = lo[k] & ~(w.box - 1), count[k] = u.tokens > 0 && hi[k] > lo[k] ? (hi[k] - base[k] + AW_KEYS - 1) / AW_KEYS : 0;
+		const int total = count[0] + count[1];
+		begin = (int)min((long long)total, (long long)share * w.each), tiles = (share == w.shares - 1 ? total : min(total, begin + w.each)) - begin;
+	};
+	const int low = pos0 + row0 / a.group, high = pos0 + (row0 + rows - 1) / a.group; // of one sequence's rows
+	__syncthreads();
+	if (warp == 8 || warp == 11) {
+		if (!ranged) asm volatile("bar.sync 2, %0;" ::"n"(AW_THREADS) : "memory");
+		range(ranged ? low : s.span[0], ranged ? high : s.span[1]);
+	} else {
+		for (int b = u.first + (warp < 8 ? tid : tid - 32); b <= u.last; b += AW_THREADS - 64) {
+			const int p0 = c.pos0[b], start = c.start[b], n = c.count[b];
+			if (!there(c, a.rows, b) || warp > 9) continue;
+			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)n * a.group;
+			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) s.row_pos[r] = p0 + (int)((unsigned)(r - r0) / (unsigned)a.group);
+		}
+		// queries, rows of 128 bytes a panel
+		const bool vec = ((uintptr_t)a.q | (uintptr_t)(a.q_row * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
+		if (warp < 8) {
+			constexpr int DEPTH = 8;
+#pragma unroll 1
+			for (int i0 = tid; i0 < groups * 128 * PIECES; i0 += 256 * DEPTH) {
+				uint4 x[DEPTH];
+#pragma unroll
+				for (int k = 0; k < DEPTH; ++k) {
+					const int i = i0 + 256 * k, r = i / PIECES, piece = i % PIECES, rr = row0 + min(r, rows - 1);
+					x[k] = make_uint4(0, 0, 0, 0);
+					if (r < rows && piece * 8 < c.dim) {
+						const uint16_t* const q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + piece * 8;
+						if (vec) x[k] = *reinterpret_cast<const uint4*>(q);
+						else x[k] = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+					}
+				}
+#pragma unroll
+				for (int k = 0; k < DEPTH; ++k) {
+					const int i = i0 + 256 * k, r = i / PIECES, piece = i % PIECES;
+					if (i < groups * 128 * PIECES) *reinterpret_cast<uint4*>(s.q[r >> 7][piece >> 3] + (r & 127) * 128 + (((piece & 7) ^ (r & 7)) << 4)) = x[k];
+				}
+			}
+			fence_async_smem();
+		}
+		asm volatile("bar.sync 1, %0;" ::"n"(AW_THREADS - 64) : "memory"); // everybody but the copying warps
+		if (warp < 8) {
+			const int pos = s.row_pos[tid];
+			const int least = __reduce_min_sync(0xffffffffu, pos < 0 ? INT_MAX : pos), most = __reduce_max_sync(0xffffffffu, pos);
+			if (lane == 0) atomicMin(&s.span[0], least), atomicMax(&s.span[1], most);
+		}
+		tc_fence_before();
+		asm volatile("bar.sync 1, %0;" ::"n"(AW_THREADS - 64) : "memory");
+		tc_fence_after();
+		if (!ranged) asm volatile("bar.sync 2, %0;" ::"n"(AW_THREADS) : "memory");
+		range(ranged ? low : s.span[0], ranged ? high : s.span[1]);
 	}
-	const int total = count[0] + count[1], begin = (int)min((long long)total, (long long)share * w.each), end = share == w.shares - 1 ? total : min(total, begin + w.each), tiles = end - begin;
+	const uint32_t tmem = s.tmem;
+	const int least = s.span[0], most = s.span[1];
 
 	if (warp < 8) {
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AW_SOFTMAX_REGS));
 		const int group = warp >> 2;
 		const int rpos = s.row_pos[tid], rlow = low_of(a, rpos), wide = low_of(a, most);
 		const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), scores_at = lanes + 128 * group, sums_at = lanes + O_COL + 128 * group;
-		const float qscale = a.softcap > 0.f ? a.scale / a.softcap : a.scale * A16_LOG2E;
+		const float qscale = a.softcap > 0.f ? -2.f * A16_LOG2E * a.scale / a.softcap : a.scale * A16_LOG2E;
 		float m = -INFINITY, l = 0.f;
 		if (group < groups) {
 			for (int i = 0; i < tiles; ++i) {
@@ -733,7 +822,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					if (a.softcap > 0.f) {
 						const float cap = a.softcap * A16_LOG2E;
 #pragma unroll
-						for (int k = 0; k < 128; ++k) z[k] = fmaf(cap, tanhf(z[k] * qscale), -ref); // log2 of the weights against the reference (against 0 before there is one)
+						for (int k = 0; k < 128; ++k) z[k] = capped(z[k] * qscale, cap) - ref; // log2 of the weights against the reference (against 0 before there is one)
 					} else {
 #pragma unroll
 						for (int k = 0; k < 128; ++k) z[k] = fmaf(z[k], qscale, -ref);
@@ -795,7 +884,11 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				norm = l > 0.f ? down / l : l == 0.f ? 0.f : l; // (0: nothing was seen; a NaN stays one)
 			} else if (writes) a.stats[place] = make_float2(lost ? 0.f : m, lost ? NAN : l);
 			if (lost) norm = NAN;
+			// A thread's row goes to shared memory (where keys and values were: the last product has ended, of the other group's too once both have) and from there as one copy.
 			const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
+			float* const row = reinterpret_cast<float*>(s.kv) + tid * (D + 4);
+			asm volatile("bar.sync 3, %0;" ::"r"(128 * groups) : "memory");
+			const bool nothing = w.place >= 0 && m == -INFINITY && !lost; // (the fold leaves out what weighs nothing)
 #pragma unroll 1
 			for (int col = 0; col < c.dim; col += 16) {
 				float v[16];
@@ -805,25 +898,29 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 #pragma unroll
 					for (int k = 0; k < 16; ++k) v[k] = 0.f;
 				}
-				if (!writes) continue;
 				if (w.place >= 0) {
-					if (m == -INFINITY && !lost) continue; // (the fold leaves out what weighs nothing)
-					float4* const to = reinterpret_cast<float4*>(a.sums + place * c.dim + col);
 #pragma unroll
-					for (int k = 0; k < 4; ++k) to[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+					for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(row + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
 				} else {
-					uint16_t* const to = a.out + token * a.o_row + head * a.o_head + col;
+					uint32_t x[8];
+#pragma unroll
+					for (int k = 0; k < 8; ++k) x[k] = pack2<T>(v[2 * k] * norm, v[2 * k + 1] * norm);
 					if (vec) {
-						uint32_t x[8];
+						uint4* const to = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(row) + col);
+						to[0] = make_uint4(x[0], x[1], x[2], x[3]), to[1] = make_uint4(x[4], x[5], x[6], x[7]);
+					} else if (writes) {
+						uint16_t* const to = a.out + token * a.o_row + head * a.o_head + col;
 #pragma unroll
-						for (int k = 0; k < 8; ++k) x[k] = pack2<T>(v[2 * k] * norm, v[2 * k + 1] * norm);
-						reinterpret_cast<uint4*>(to)[0] = make_uint4(x[0], x[1], x[2], x[3]), reinterpret_cast<uint4*>(to)[1] = make_uint4(x[4], x[5], x[6], x[7]);
-					} else {
-#pragma unroll
-						for (int k = 0; k < 16; ++k) to[k] = round16<T>(v[k] * norm);
+						for (int k = 0; k < 8; ++k) to[2 * k] = (uint16_t)x[k], to[2 * k + 1] = (uint16_t)(x[k] >> 16);
 					}
 				}
 			}
+			fence_async_smem();
+			if (writes && !nothing && (w.place >= 0 || vec)) {
+				if (w.place >= 0) bulk_store(a.sums + place * c.dim, row, c.dim * 4);
+				else bulk_store(a.out + token * a.o_row + head * a.o_head, row, c.dim * 2);
+			}
+			asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory"); // (written: what follows in the stream may read it)
 		}
 	} else {
 		asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AW_OTHER_REGS));
@@ -842,7 +939,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				int part;
 				const int pos = start(i, part) + lane * w.box, at = c.page_index(pos);
 				const bool some = lane < boxes && i < tiles && pos < (part ? hi[1] : hi[0]) && at < c.table_pages;
-				next = some ? __ldg(c.table + (size_t)(part ? slot[1] : slot[0]) * c.table_pages + at) : -1;
+				next = some ? __ldg(c.table + (size_t)(part ? own_slot : lead_slot) * c.table_pages + at) : -1;
 			};
 			uint32_t fixes = 0;
 			int issued = 0; // tiles asked for

@@ -140,7 +140,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) 
 // an 8 x 8 tile of fp16, a row's pair of neighbours a thread, with rows and columns exchanged
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 	uint32_t r;
-	asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+	asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
 	return r;
 }
 // false: given up, here or by another thread of the block; no thread goes on then, and the rows come out as NaN

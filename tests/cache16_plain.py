@@ -86,7 +86,7 @@ def attend(q, k, v, table, portions, groups, page, scale, window=0, softcap=0.0,
                 ds = ((D / 16 + 6) * mag + D / 16 * 17 * big) * 2.0 ** -23
                 if softcap:
                     s = softcap * np.tanh(s / softcap)
-                    ds = ds + 8 * F32 * np.abs(s)
+                    ds = ds + softcap * 2.0 ** -21 + 4 * F32 * np.abs(s)  # (1 - t) / (1 + t), t = e^(-2 |x|): t and its difference from 1 within 2^-22, the quotient's reciprocal within 2^-23
                 s = np.where(seen, s, -math.inf)
                 m = s.max(1, keepdims=True)
                 if sink is not None:
