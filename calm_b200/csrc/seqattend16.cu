@@ -60,7 +60,7 @@ struct ArStage { // a warp's chunk: the next one's keys come while its values ar
 };
 template <int D>
 __host__ __device__ constexpr size_t ar_ring() { // (the sums of the warps take its place)
-	const size_t a = (size_t)AR_WARPS * sizeof(ArStage<D>), b = ((size_t)AR_WARPS * 8 * (D + 4) + (size_t)AR_TILE * (D + 2)) * sizeof(float);
+	const size_t a = (size_t)AR_WARPS * sizeof(ArStage<D>), b = ((size_t)AR_WARPS * AR_TILE * (D + 4) + (size_t)AR_TILE * (D + 2)) * sizeof(float);
 	return a > b ? a : b;
 }
 template <int D, int NQ>
@@ -209,88 +209,31 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	// the queries are asked for first
 	constexpr int QF = KS * NQ * 32 / (32 * AR_WARPS) > 0 ? KS * NQ * 32 / (32 * AR_WARPS) : 1; // fragments of a thread
 	uint2 qx[QF];
+	{
+		static_assert(AR_WARPS % NQ == 0, "all fragments of a thread are of one row");
+		const int r = warp % NQ * 8 + g, rr = row0 + min(r, rows - 1), token = rr / a.group;
+		const uint16_t* const q = a.q + (long long)(u.t0 + token) * a.q_row + (long long)(kvh * a.group + rr - token * a.group) * a.q_head + 2 * t;
 #pragma unroll
-	for (int f = 0; f < QF; ++f) {
-		const int i = tid + f * 32 * AR_WARPS, k = i / (NQ * 32), r = (i / 32 % NQ) * 8 + (i >> 2 & 7), d = k * 16 + (i & 3) * 2, rr = row0 + min(r, rows - 1);
-		const uint16_t* q = a.q + (long long)(u.t0 + rr / a.group) * a.q_row + (long long)(kvh * a.group + rr % a.group) * a.q_head + d;
-		qx[f] = make_uint2(0, 0);
-		if (r < rows && d < dim) qx[f].x = q[0] | (uint32_t)q[1] << 16, qx[f].y = q[8] | (uint32_t)q[9] << 16; // (16 channels are there or not)
-	}
-	// which sequence and position each row has; the segments of the tile's list of keys: 0 the prefix, then every sequence of its rows
-	const bool alone = u.first == u.last;
-	if (alone) { // one sequence: nothing to look for
-		const int p0 = c.pos0[u.first] + (u.t0 - c.start[u.first]), low = p0 + row0 / a.group, high = p0 + (row0 + rows - 1) / a.group; // (a group of one has its sequence's rows)
-		if (tid < TILE) row_seq[tid] = tid < rows ? u.first : -1, row_pos[tid] = tid < rows ? p0 + (row0 + tid) / a.group : -1, row_seg[tid] = tid < rows ? 1 : -1;
-		if (tid == 0) {
-			const int slot = c.slot[u.first], reach = c.reach(slot);
-			const bool with = a.families && u.prefix > 0;
-			const int lo0 = with ? low_of(a, low) : 0, hi0 = with ? min(min(u.prefix, high + 1), reach) : 0, lo1 = max(u.prefix, low_of(a, low)), hi1 = min(high + 1, reach);
-			const int n0 = chunks_of(lo0, hi0), n1 = chunks_of(lo1, hi1);
-			seg_slot[0] = seg_slot[1] = slot, seg_lo[0] = lo0, seg_hi[0] = hi0, seg_lo[1] = lo1, seg_hi[1] = hi1, seg_base[0] = 0, seg_base[1] = n0;
-			list[0] = 2, list[1] = n0 + n1, list[2] = low, list[3] = high;
-		}
-	} else {
-		if (tid < TILE) row_seq[tid] = row_pos[tid] = -1;
-		const int lead_slot = c.slot[u.lead >= 0 ? u.lead : u.first];
-		__syncthreads();
-		for (int b = u.first + tid; b <= u.last; b += 32 * AR_WARPS) {
-			const int slot = c.slot[b], pos0 = c.pos0[b], start = c.start[b], count = c.count[b];
-			if (!there(c, a.rows, b)) continue;
-			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)count * a.group;
-			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) row_seq[r] = b, row_pos[r] = pos0 + (int)((unsigned)(r - r0) / (unsigned)a.group), row_slot[r] = slot;
-		}
-		__syncthreads();
-		if (warp == 0) {
-			const int seq = lane < TILE ? row_seq[lane] : -1, pos = lane < TILE ? row_pos[lane] : -1, slot = seq >= 0 ? row_slot[lane] : -1;
-			const int left = __shfl_up_sync(0xffffffffu, seq, 1), right = __shfl_down_sync(0xffffffffu, seq, 1);
-			const bool head = seq >= 0 && (lane == 0 || left != seq), tail = seq >= 0 && (lane == 31 || right != seq);
-			const uint32_t heads = __ballot_sync(0xffffffffu, head);
-			const int seg = __popc(heads & (0xffffffffu >> (31 - lane))); // (1: the first; 0: the prefix)
-			const int least = __reduce_min_sync(0xffffffffu, seq >= 0 ? pos : INT_MAX), most = __reduce_max_sync(0xffffffffu, pos);
-			if (lane < TILE) row_seg[lane] = seq >= 0 ? seg : -1;
-			if (head) seg_slot[seg] = slot, seg_lo[seg] = max(u.prefix, low_of(a, pos));
-			if (tail) seg_hi[seg] = min(pos + 1, c.reach(slot));
-			if (lane == 0) {
-				const bool with = u.prefix > 0 && least != INT_MAX;
-				seg_slot[0] = lead_slot, seg_lo[0] = with ? low_of(a, least) : 0, seg_hi[0] = with ? min(min(u.prefix, most + 1), c.reach(lead_slot)) : 0;
-			}
-			__syncwarp();
-			const int segs = __popc(heads) + 1;
-			int chunks = lane < segs ? chunks_of(seg_lo[lane], seg_hi[lane]) : 0, sum = chunks;
-#pragma unroll
-			for (int o = 1; o < 32; o *= 2) {
-				const int x = __shfl_up_sync(0xffffffffu, sum, o);
-				if (lane >= o) sum += x;
-			}
-			if (lane < segs) seg_base[lane] = sum - chunks;
-			if (lane == segs - 1) list[0] = segs, list[1] = sum, list[2] = least, list[3] = most;
+		for (int f = 0; f < QF; ++f) {
+			const int d = (warp + f * AR_WARPS) / NQ * 16;
+			qx[f] = make_uint2(0, 0);
+			if (r < rows && d < dim) qx[f].x = q[d] | (uint32_t)q[d + 1] << 16, qx[f].y = q[d + 8] | (uint32_t)q[d + 9] << 16; // (16 channels are there or not)
 		}
 	}
-#pragma unroll
-	for (int f = 0; f < QF; ++f)
-		if (tid + f * 32 * AR_WARPS < KS * NQ * 32) qf[tid + f * 32 * AR_WARPS] = qx[f]; // B fragments
-	__syncthreads();
-	const int segs = list[0], total = list[1], least = list[2], most = list[3];
-	const int my_base = lane < segs ? seg_base[lane] : INT_MAX; // (at most 17 segments)
-	const int begin = (int)min((long long)total, (long long)share * a.each), end = share == a.shares - 1 ? total : min(total, begin + a.each); // (more keys than were planned for: the last share's)
-	const bool whole = a.shares == 1 || (a.cluster && total <= a.each); // no other share has keys
-	if (whole && share > 0) return;                                     // (nor does any of the cluster wait)
-
-	// the chunk to request: its segment, first position and end; the page of this lane's key, as the table has it: a load that nothing waits for where it is asked for
+	// The first chunks of a prefix are asked for before the rest is known.  (Their keys are known without the rows where there is no window.)
 	ArStage<D>& s = ring[warp];
-	int next = begin + warp, next_seg = 0, next_pos = 0, next_lo = 0, next_hi = 0, next_page = 0, next_row = 0;
+	const int lead_slot = a.families && u.lead >= 0 ? c.slot[u.lead] : -1;
+	const int prefix = a.window == 0 ? min(a.families ? u.prefix : 0, c.reach(lead_slot)) : 0;
+	int next = (int)min((long long)INT_MAX / 2, (long long)share * a.each) + warp, next_seg = 0, next_pos = 0, next_lo = 0, next_hi = 0, next_page = 0, next_row = 0; // the chunk to request
 	uint32_t next_seen = 0;
 	bool page_ok = false;
-	auto look = [&]() {
-		const bool some = next < end;
-		// (segments without keys start where the next one does: the last of those that start here has the chunk)
-		next_seg = some ? __popc(__ballot_sync(0xffffffffu, my_base <= next)) - 1 : 0;
-		next_lo = seg_lo[next_seg], next_hi = seg_hi[next_seg], next_pos = (next_lo / AR_KEYS + next - seg_base[next_seg]) * AR_KEYS;
+	const bool early = next < chunks_of(0, prefix) && (share == a.shares - 1 || warp < a.each);
+	auto ask = [&](bool some, int slot) { // for the page of this lane's key, as the table has it: a load that nothing waits for where it is asked for
 		const int pos = next_pos + lane, at = c.page_index(max(pos, 0));
 		page_ok = some && pos >= next_lo && pos < next_hi && at < c.table_pages;
-		next_page = page_ok ? __ldg(c.table + (size_t)seg_slot[next_seg] * c.table_pages + at) : -1;
+		next_page = page_ok ? __ldg(c.table + (size_t)slot * c.table_pages + at) : -1;
 	};
-	look();
+	if (early) next_hi = prefix, next_pos = next * AR_KEYS, ask(true, lead_slot);
 	constexpr int EACH = 32 / PIECES;                      // rows that a warp copies at a time
 	const int piece = lane % PIECES, prow = lane / PIECES; // which piece of which of them this lane copies
 	const bool eights = c.page % 8 == 0 && dim == D;       // eight keys from a multiple of eight on lie side by side
@@ -313,17 +256,89 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 			}
 		}
 	};
-	auto request_keys = [&]() {
-		if (next < end) {
-			const bool some = page_ok && (unsigned)next_page < (unsigned)c.pages;
-			next_seen = __ballot_sync(0xffffffffu, some);
-			next_row = some ? (next_page * H + kvh) * c.page + c.page_row(next_pos + lane) : 0; // (rows of a pool: under 2^31)
-			copy(s.k, c.k);
-		}
-		asm volatile("cp.async.commit_group;" ::: "memory");
+	auto copy_keys = [&]() {
+		const bool some = page_ok && (unsigned)next_page < (unsigned)c.pages;
+		next_seen = __ballot_sync(0xffffffffu, some);
+		next_row = some ? (next_page * H + kvh) * c.page + c.page_row(next_pos + lane) : 0; // (rows of a pool: under 2^31)
+		copy(s.k, c.k);
 	};
-	int cur_seg = 0, cur_pos = 0;
-	uint32_t cur_seen = 0;
+	if (early) {
+		copy_keys();
+		asm volatile("cp.async.commit_group;" ::: "memory");
+		copy(s.v, c.v);
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	}
+	// which sequence and position each row has; the segments of the tile's list of keys: 0 the prefix, then every sequence of its rows
+	const bool alone = u.first == u.last;
+	if (alone) { // one sequence: nothing to look for
+		const int p0 = c.pos0[u.first] + (u.t0 - c.start[u.first]), low = p0 + row0 / a.group, high = p0 + (row0 + rows - 1) / a.group; // (a group of one has its sequence's rows)
+		if (tid < TILE) row_seq[tid] = tid < rows ? u.first : -1, row_pos[tid] = tid < rows ? p0 + (row0 + tid) / a.group : -1, row_seg[tid] = tid < rows ? 1 : -1;
+		if (tid == 0) {
+			const int slot = c.slot[u.first], reach = c.reach(slot);
+			const bool with = a.families && u.prefix > 0;
+			const int lo0 = with ? low_of(a, low) : 0, hi0 = with ? (a.window ? min(min(u.prefix, high + 1), reach) : prefix) : 0, lo1 = max(u.prefix, low_of(a, low)), hi1 = min(high + 1, reach);
+			const int n0 = chunks_of(lo0, hi0), n1 = chunks_of(lo1, hi1);
+			seg_slot[0] = seg_slot[1] = slot, seg_lo[0] = lo0, seg_hi[0] = hi0, seg_lo[1] = lo1, seg_hi[1] = hi1, seg_base[0] = 0, seg_base[1] = n0;
+			list[0] = 2, list[1] = n0 + n1, list[2] = low, list[3] = high;
+		}
+	} else {
+		if (tid < TILE) row_seq[tid] = row_pos[tid] = -1;
+		__syncthreads();
+		for (int b = u.first + tid; b <= u.last; b += 32 * AR_WARPS) {
+			const int slot = c.slot[b], pos0 = c.pos0[b], start = c.start[b], count = c.count[b];
+			if (!there(c, a.rows, b)) continue;
+			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)count * a.group;
+			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) row_seq[r] = b, row_pos[r] = pos0 + (int)((unsigned)(r - r0) / (unsigned)a.group), row_slot[r] = slot;
+		}
+		__syncthreads();
+		if (warp == 0) {
+			const int seq = lane < TILE ? row_seq[lane] : -1, pos = lane < TILE ? row_pos[lane] : -1, slot = seq >= 0 ? row_slot[lane] : -1;
+			const int left = __shfl_up_sync(0xffffffffu, seq, 1), right = __shfl_down_sync(0xffffffffu, seq, 1);
+			const bool head = seq >= 0 && (lane == 0 || left != seq), tail = seq >= 0 && (lane == 31 || right != seq);
+			const uint32_t heads = __ballot_sync(0xffffffffu, head);
+			const int seg = __popc(heads & (0xffffffffu >> (31 - lane))); // (1: the first; 0: the prefix)
+			const int least = __reduce_min_sync(0xffffffffu, seq >= 0 ? pos : INT_MAX), most = __reduce_max_sync(0xffffffffu, pos);
+			if (lane < TILE) row_seg[lane] = seq >= 0 ? seg : -1;
+			if (head) seg_slot[seg] = slot, seg_lo[seg] = max(u.prefix, low_of(a, pos));
+			if (tail) seg_hi[seg] = min(pos + 1, c.reach(slot));
+			if (lane == 0) {
+				const bool with = u.prefix > 0 && least != INT_MAX;
+				seg_slot[0] = lead_slot, seg_lo[0] = with ? low_of(a, least) : 0, seg_hi[0] = with ? (a.window ? min(min(u.prefix, most + 1), c.reach(lead_slot)) : prefix) : 0;
+			}
+			__syncwarp();
+			const int segs = __popc(heads) + 1;
+			int chunks = lane < segs ? chunks_of(seg_lo[lane], seg_hi[lane]) : 0, sum = chunks;
+#pragma unroll
+			for (int o = 1; o < 32; o *= 2) {
+				const int x = __shfl_up_sync(0xffffffffu, sum, o);
+				if (lane >= o) sum += x;
+			}
+			if (lane < segs) seg_base[lane] = sum - chunks;
+			if (lane == segs - 1) list[0] = segs, list[1] = sum, list[2] = least, list[3] = most;
+		}
+	}
+#pragma unroll
+	for (int f = 0; f < QF; ++f)
+		if (tid + f * 32 * AR_WARPS < KS * NQ * 32) qf[tid + f * 32 * AR_WARPS] = qx[f]; // B fragments
+	__syncthreads();
+	const int segs = list[0], total = list[1], least = list[2], most = list[3];
+	const int begin = (int)min((long long)total, (long long)share * a.each), end = share == a.shares - 1 ? total : min(total, begin + a.each); // (more keys than were planned for: the last share's)
+	const bool whole = a.shares == 1 || (a.cluster && total <= a.each); // no other share has keys
+
+	if (whole && share > 0) {
+		asm volatile("cp.async.wait_all;" ::: "memory");
+		return; // (nor does any of the cluster wait)
+	}
+	const int my_base = lane < segs ? seg_base[lane] : INT_MAX; // (at most 17 segments)
+	auto look = [&]() { // the chunk to request next: its segment, first position and end
+		const bool some = next < end;
+		// (segments without keys start where the next one does: the last of those that start here has the chunk)
+		next_seg = some ? __popc(__ballot_sync(0xffffffffu, my_base <= next)) - 1 : 0;
+		next_lo = seg_lo[next_seg], next_hi = seg_hi[next_seg], next_pos = (next_lo / AR_KEYS + next - seg_base[next_seg]) * AR_KEYS;
+		ask(some, seg_slot[next_seg]);
+	};
+	int cur_seg = 0, cur_pos = next_pos;
+	uint32_t cur_seen = next_seen;
 	auto request_values = [&]() { // of the chunk whose keys were requested last
 		cur_seg = next_seg, cur_pos = next_pos, cur_seen = next_seen;
 		if (next < end) {
@@ -333,7 +348,12 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		}
 		asm volatile("cp.async.commit_group;" ::: "memory");
 	};
-	request_keys(), request_values();
+	auto request_keys = [&]() {
+		if (next < end) copy_keys();
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	};
+	if (early) next += AR_WARPS, look(); // (both are on their way)
+	else look(), request_keys(), request_values();
 
 	uint2 qr[KEEP ? KS * NQ : 1];
 	if (KEEP) {
@@ -369,23 +389,27 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		// (fragments of two steps are asked for while the last two's are used)
 		constexpr int AHEAD = 2;
 		uint32_t A[2][AHEAD][2][4];
-		auto fetch = [&](int k0, uint32_t (&to)[AHEAD][2][4]) {
+		uint2 B[2][AHEAD][NQ];
+		auto fetch = [&](int k0, uint32_t (&to)[AHEAD][2][4], uint2 (&b)[AHEAD][NQ]) {
 #pragma unroll
-			for (int k = 0; k < AHEAD; ++k)
+			for (int k = 0; k < AHEAD; ++k) {
+#pragma unroll
+				for (int q = 0; q < NQ; ++q) b[k][q] = qfrag((k0 + k) * NQ + q);
 #pragma unroll
 				for (int i = 0; i < 2; ++i) ldsm_x4(s.k + ((16 * i + (lane & 8) + lrow) * PIECES + ((2 * (k0 + k) + (lane >> 4)) ^ lrow)) * 8, to[k][i]);
+			}
 		};
-		fetch(0, A[0]);
+		fetch(0, A[0], B[0]);
 #pragma unroll
 		for (int k0 = 0; k0 < KS; k0 += AHEAD) {
-			if (k0 + AHEAD < KS) fetch(k0 + AHEAD, A[(k0 / AHEAD + 1) & 1]);
+			if (k0 + AHEAD < KS) fetch(k0 + AHEAD, A[(k0 / AHEAD + 1) & 1], B[(k0 / AHEAD + 1) & 1]);
 #pragma unroll
 			for (int k = 0; k < AHEAD; ++k)
 				if (16 * (k0 + k) < dim) // (channels that are not there: nothing was copied)
 #pragma unroll
 					for (int i = 0; i < 2; ++i)
 #pragma unroll
-						for (int q = 0; q < NQ; ++q) mma_16<T>(z[i][q], A[(k0 / AHEAD) & 1][k][i], qfrag((k0 + k) * NQ + q));
+						for (int q = 0; q < NQ; ++q) mma_16<T>(z[i][q], A[(k0 / AHEAD) & 1][k][i], B[(k0 / AHEAD) & 1][k][q]);
 		}
 		__syncwarp(); // every lane has its keys
 		request_keys();
@@ -522,23 +546,23 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		}
 	if (a.before) pdl_wait_prev(); // the prefixes' shares
 
-	// the warps' sums as one, eight rows at a time
-	float* const sums = reinterpret_cast<float*>(ring); // [warps][8][LD]
-	float* const own = sums + AR_WARPS * 8 * LD;        // [TILE][D + 2]: what this share of a cluster found
+	// the warps' sums as one
+	float* const sums = reinterpret_cast<float*>(ring); // [warps][TILE][LD]
+	float* const own = sums + AR_WARPS * TILE * LD;     // [TILE][D + 2]: what this share of a cluster found
 	const int prefix_places = whole && u.lead >= 0 ? a.before : 0;
+	__syncthreads();
 #pragma unroll
-	for (int q = 0; q < NQ; ++q) {
-		if (8 * q >= rows) break;
-		__syncthreads();
+	for (int q = 0; q < NQ; ++q)
 #pragma unroll
 		for (int e = 0; e < 2; ++e) {
-			float* const to = sums + (warp * 8 + 2 * t + e) * LD + g;
+			float* const to = sums + (warp * TILE + 8 * q + 2 * t + e) * LD + g;
 #pragma unroll
 			for (int i = 0; i < MT; ++i) to[16 * i] = acc[i][q][e], to[16 * i + 8] = acc[i][q][2 + e];
 		}
-		__syncthreads();
-		for (int rr = warp; rr < min(8, rows - 8 * q); rr += AR_WARPS) {
-			const int r = 8 * q + rr;
+	__syncthreads();
+	{
+#pragma unroll 2
+		for (int r = warp; r < rows; r += AR_WARPS) {
 			if (row_seq[r] < 0) continue;
 			float mx = fold_m[0][r], den = 0.f, wt[AR_WARPS];
 #pragma unroll
@@ -564,7 +588,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 					const int d = min(d0 + 4 * lane, dim - 4); // (every lane has a place's weight)
 					float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-					for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w] * down, *reinterpret_cast<const float4*>(sums + (w * 8 + rr) * LD + d));
+					for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w] * down, *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
 					add_places(v, a.sums + place * dim + d, dim, prefix_places, pw);
 					if (d0 + 4 * lane < dim) put4<T>(a.out + token * a.o_row + head * a.o_head + d, a.out_vec, times4(v, norm));
 				}
@@ -576,7 +600,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 					for (int d = 4 * lane; d < dim; d += 128) {
 						float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-						for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w], *reinterpret_cast<const float4*>(sums + (w * 8 + rr) * LD + d));
+						for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w], *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
 						if (a.cluster) to[d] = v.x, to[d + 1] = v.y, to[d + 2] = v.z, to[d + 3] = v.w; // (rows of the cluster's sums are 8-byte aligned)
 						else *reinterpret_cast<float4*>(to + d) = v;
 					}
@@ -627,7 +651,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 // memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run.  O stays in tensor memory; it is rescaled in the rare case that
 // a row's reference moves.
 constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
-constexpr int AW_SOFTMAX_REGS = 200, AW_OTHER_REGS = 96; // 256 x 200 + 128 x 96 = 63488 of the 384 x 168 = 64512 that the block is launched with
+constexpr int AW_SOFTMAX_REGS = 176, AW_OTHER_REGS = 144; // 256 x 176 + 128 x 144 = 63488 of the 384 x 168 = 64512 that the block is launched with
 
 template <int D>
 struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
@@ -672,6 +696,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 	             : "r"(taddr)
 	             : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) { // (tcgen05.wait::st is the caller's)
+	asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+	             "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+	             : "memory");
+}
 // shared-memory descriptor of values [keys][64 channels], 128-byte swizzle, panels of 64 channels one behind another: the product's columns are the channels, its depth the keys, eight keys 1024 bytes apart
 __device__ __forceinline__ uint64_t umma_desc_values(const void* tile) {
 	const uint64_t addr = (uint64_t)(smem_u32(tile) & 0x3FFFF) >> 4;
@@ -702,6 +731,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	} else if (!group_unit(c, a, blockIdx.z, u)) return;
 	if ((long long)tile * 256 >= (long long)u.tokens * a.group) return;
 	const int row0 = tile * 256, rows = (int)min(256LL, (long long)u.tokens * a.group - row0), groups = rows > 128 ? 2 : 1;
+	const bool two = groups == 1; // the same rows twice: each of two groups of warps takes every other tile, and their sums are added at the end
 
 	if (warp == 9) tmem_alloc(&s.tmem, 512);
 	if (tid == 0) {
@@ -783,31 +813,32 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	if (warp < 8) {
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AW_SOFTMAX_REGS));
 		const int group = warp >> 2;
-		const int rpos = s.row_pos[tid], rlow = low_of(a, rpos), wide = low_of(a, most);
+		const int r = two ? tid & 127 : tid, rpos = s.row_pos[r], rlow = low_of(a, rpos), wide = low_of(a, most);
 		const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), scores_at = lanes + 128 * group, sums_at = lanes + O_COL + 128 * group;
 		const float qscale = a.softcap > 0.f ? -2.f * A16_LOG2E * a.scale / a.softcap : a.scale * A16_LOG2E;
 		float m = -INFINITY, l = 0.f;
-		if (group < groups) {
-			for (int i = 0; i < tiles; ++i) {
+		if (group < groups || two) {
+			int n = 0; // tiles of this group's
+			for (int i = two ? group : 0; i < tiles; i += two ? 2 : 1, ++n) {
 				const int at = begin + i, part = at >= count[0], pos0 = part ? base[1] + (at - count[0]) * AW_KEYS : base[0] + at * AW_KEYS;
-				if (!ap_wait_warp(s.mask_full + i % AW_MASKS, i / AW_MASKS & 1, &s.lost) || !ap_wait_warp(s.s_full + group, i & 1, &s.lost)) break;
+				if (!ap_wait_warp(s.mask_full + i % AW_MASKS, i / AW_MASKS & 1, &s.lost) || !ap_wait_warp(s.s_full + group, n & 1, &s.lost)) break;
 				tc_fence_after();
 				const uint4 seen = *reinterpret_cast<const uint4*>(s.seen[i % AW_MASKS]);
 				const bool all = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && pos0 >= wide && pos0 + AW_KEYS - 1 <= least;
-				const bool steady = __all_sync(0xffffffffu, all && m != -INFINITY) && !(a.softcap > 0.f) && a.scale > 0.f;
-				float z[128];
+				const bool steady = __all_sync(0xffffffffu, all && (m != -INFINITY || rpos < 0)) && !(a.softcap > 0.f) && a.scale > 0.f; // (a row that is not there has scores of zero)
+				const float ref = m == -INFINITY ? 0.f : m;
 				uint32_t p[64];
 				u64 sum = 0;
-				tmem_ld128(scores_at, z);
 				bool moves = true;
 				if (steady) { // the reference as it stands, unless a score passes it or is no number
-					float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+					float z[128], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+					tmem_ld128(scores_at, z);
 #pragma unroll
 					for (int k = 0; k < 128; k += 2) tops[k / 2 % 4] = max_nan(max_nan(tops[k / 2 % 4], z[k]), z[k + 1]);
 					const float top = max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3]));
-					moves = __any_sync(0xffffffffu, !(fmaf(top, qscale, -m) <= A16_MOST));
+					moves = __any_sync(0xffffffffu, !(fmaf(top, qscale, -ref) <= A16_MOST));
 					if (!moves) {
-						const u64 by = pair_of(qscale, qscale), off = pair_of(-m, -m);
+						const u64 by = pair_of(qscale, qscale), off = pair_of(-ref, -ref);
 #pragma unroll
 						for (int k = 0; k < 128; k += 2) {
 							const float2 y = halves(fma2(pair_of(z[k], z[k + 1]), by, off));
@@ -817,52 +848,58 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 						}
 					}
 				}
-				if (moves) {
-					const float ref = m == -INFINITY ? 0.f : m, most_z = m == -INFINITY ? -INFINITY : A16_MOST;
-					if (a.softcap > 0.f) {
-						const float cap = a.softcap * A16_LOG2E;
-#pragma unroll
-						for (int k = 0; k < 128; ++k) z[k] = capped(z[k] * qscale, cap) - ref; // log2 of the weights against the reference (against 0 before there is one)
-					} else {
-#pragma unroll
-						for (int k = 0; k < 128; ++k) z[k] = fmaf(z[k], qscale, -ref);
-					}
-					if (!all) {
-						const uint32_t words[4] = {seen.x, seen.y, seen.z, seen.w};
-						const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
-#pragma unroll
-						for (int x = 0; x < 4; ++x) {
-							const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
-							const uint32_t see = words[x] & (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
-#pragma unroll
-							for (int k = 0; k < 32; ++k)
-								if (!(see >> k & 1)) z[32 * x + k] = -INFINITY;
-						}
-					}
+				if (moves) { // 32 columns at a time, in few instructions: most often a block's first and last tiles
+					const float most_z = m == -INFINITY ? -INFINITY : A16_MOST, cap = a.softcap * A16_LOG2E;
+					const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
 					float top = -INFINITY;
+#pragma unroll 1
+					for (int x = 0; x < 4; ++x) { // log2 of the weights against the reference (against 0 before there is one), back to where the scores were
+						float y[32];
+						tmem_ld32(scores_at + 32 * x, y);
+						const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
+						const uint32_t see = s.seen[i % AW_MASKS][x] & (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
+						if (a.softcap > 0.f) {
 #pragma unroll
-					for (int k = 0; k < 128; k += 2) top = fmaxf(fmaxf(top, z[k]), z[k + 1]);
+							for (int k = 0; k < 32; ++k) y[k] = capped(y[k] * qscale, cap) - ref;
+						} else {
+#pragma unroll
+							for (int k = 0; k < 32; ++k) y[k] = fmaf(y[k], qscale, -ref);
+						}
+#pragma unroll
+						for (int k = 0; k < 32; ++k) {
+							if (!(see >> k & 1)) y[k] = -INFINITY;
+							top = fmaxf(top, y[k]);
+						}
+						tmem_st32(scores_at + 32 * x, reinterpret_cast<const uint32_t(&)[32]>(y));
+					}
+					float down = 0.f;
 					if (__any_sync(0xffffffffu, top > most_z)) { // references move
-						const float mn = top > most_z ? ref + top - A16_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn), down = ref - (mn == -INFINITY ? 0.f : mn);
-#pragma unroll
-						for (int k = 0; k < 128; ++k) z[k] += down;
+						const float mn = top > most_z ? ref + top - A16_SET : m, f = m == -INFINITY ? 0.f : ex2(m - mn);
+						down = ref - (mn == -INFINITY ? 0.f : mn);
 						m = mn, l *= f;
-						if (i > 0) { // there are sums; the product that wrote them was issued before these scores'
+						if (n > 0) { // there are sums; the product that wrote them was issued before these scores'
 #pragma unroll 1
 							for (int col = 0; col < D; col += 8) tmem_scale8(sums_at + col, f);
-							tmem_st_wait();
 						}
 					}
-					sum = 0;
+					tmem_st_wait();
+#pragma unroll 1
+					for (int x = 0; x < 4; ++x) {
+						float y[32];
+						uint32_t w[16];
+						tmem_ld32(scores_at + 32 * x, y);
 #pragma unroll
-					for (int k = 0; k < 128; k += 2) {
-						const float w0 = ex2(z[k]), w1 = ex2(z[k + 1]);
-						sum = add2(sum, pair_of(w0, w1));
-						p[k / 2] = pack2<T>(w0, w1);
+						for (int k = 0; k < 32; k += 2) {
+							const float w0 = ex2(y[k] + down), w1 = ex2(y[k + 1] + down);
+							sum = add2(sum, pair_of(w0, w1));
+							w[k / 2] = pack2<T>(w0, w1);
+						}
+						tmem_st16(scores_at + 16 * x, w); // (where scores were that have been read)
 					}
+				} else {
+					tmem_st32(scores_at, *reinterpret_cast<uint32_t(*)[32]>(p)); // where the scores were
+					tmem_st32(scores_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
 				}
-				tmem_st32(scores_at, *reinterpret_cast<uint32_t(*)[32]>(p)); // where the scores were
-				tmem_st32(scores_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
 				const float2 both = halves(sum);
 				l += both.x + both.y;
 				tmem_st_wait();
@@ -870,12 +907,34 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				__syncwarp();
 				if (lane == 0) mbar_arrive(s.p_full + group);
 			}
-			if (tiles > 0) ap_wait_warp(s.done + group, 0, &s.lost);
+			if (n > 0) ap_wait_warp(s.done + group, 0, &s.lost);
 			tc_fence_after();
 			const bool lost = *(volatile int*)&s.lost;
-			const int token = u.t0 + (row0 + min(tid, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(tid, rows - 1)) % a.group;
-			const bool writes = tid < rows && rpos >= 0;
+			const int token = u.t0 + (row0 + min(r, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(r, rows - 1)) % a.group;
+			const bool writes = r < rows && rpos >= 0 && !(two && group);
 			const size_t place = ((size_t)token * a.heads + head) * a.places + w.place + share;
+			float* const row = reinterpret_cast<float*>(s.kv) + tid * (D + 4);
+			asm volatile("bar.sync 3, 256;" ::: "memory"); // (both groups' products have ended)
+			float f0 = 1.f, f1 = 0.f; // of this group's sums and the other's
+			const float* const other = reinterpret_cast<const float*>(s.kv) + (tid ^ 128) * (D + 4);
+			if (two) {
+				if (group) {
+#pragma unroll 1
+					for (int col = 0; col < D && n > 0; col += 16) {
+						float v[16];
+						tmem_ld16(sums_at + col, v);
+#pragma unroll
+						for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(row + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+					}
+					row[D] = m, row[D + 1] = l;
+				}
+				asm volatile("bar.sync 3, 256;" ::: "memory");
+				if (!group && tiles > 1) {
+					const float m1 = other[D], top = fmaxf(m, m1);
+					f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
+					l = fmaf(l, f0, other[D + 1] * f1), m = top;
+				}
+			}
 			float norm = 1.f;
 			if (w.place < 0) {
 				const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY, mn = fmaxf(m, sk), down = m == -INFINITY ? 0.f : ex2(m - mn);
@@ -886,17 +945,19 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			if (lost) norm = NAN;
 			// A thread's row goes to shared memory (where keys and values were: the last product has ended, of the other group's too once both have) and from there as one copy.
 			const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
-			float* const row = reinterpret_cast<float*>(s.kv) + tid * (D + 4);
-			asm volatile("bar.sync 3, %0;" ::"r"(128 * groups) : "memory");
 			const bool nothing = w.place >= 0 && m == -INFINITY && !lost; // (the fold leaves out what weighs nothing)
 #pragma unroll 1
-			for (int col = 0; col < c.dim; col += 16) {
+			for (int col = 0; col < c.dim && !(two && group); col += 16) {
 				float v[16];
 				__syncwarp(); // (rows behind the last one take part in the load)
-				if (tiles > 0) tmem_ld16(sums_at + col, v);
+				if (n > 0) tmem_ld16(sums_at + col, v);
 				else {
 #pragma unroll
 					for (int k = 0; k < 16; ++k) v[k] = 0.f;
+				}
+				if (two && tiles > 1) {
+#pragma unroll
+					for (int k = 0; k < 16; ++k) v[k] = fmaf(v[k], f0, other[col + k] * f1);
 				}
 				if (w.place >= 0) {
 #pragma unroll
@@ -994,35 +1055,55 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		} else if (warp == 9 && lane == 0) { // the products: the groups take turns
 			constexpr uint32_t type = std::is_same<T, bf16>::value ? (1u << 7) | (1u << 10) : 0;
 			constexpr uint32_t score = (1u << 4) | type | ((uint32_t)(AW_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows; values: columns side by side
-			auto scores = [&](int g, int sl) {
+			auto wait_slot = [&](int k) { return ap_wait(s.full + k % SLOTS, k / SLOTS & 1, &s.lost); };
+			auto scores = [&](int g, int i) { // of tile i
 #pragma unroll
 				for (int pn = 0; pn < PANELS; ++pn)
 #pragma unroll
-					for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * g, umma_desc_sw128(s.q[g][pn]) + 2 * k, umma_desc_sw128(s.kv[sl][pn]) + 2 * k, score, (pn | k) ? 1u : 0u);
+					for (int k = 0; k < 4; ++k) umma_f16(tmem + 128 * g, umma_desc_sw128(s.q[two ? 0 : g][pn]) + 2 * k, umma_desc_sw128(s.kv[2 * i % SLOTS][pn]) + 2 * k, score, (pn | k) ? 1u : 0u);
 				umma_commit(s.s_full + g);
 			};
-			auto wait_slot = [&](int k) { return ap_wait(s.full + k % SLOTS, k / SLOTS & 1, &s.lost); };
-			bool good = tiles > 0 && wait_slot(0);
-			if (good) {
+			auto sums = [&](int g, int i, int n) { // the n-th of the group's
+				if (!ap_wait(s.p_full + g, n & 1, &s.lost)) return false;
 				tc_fence_after();
-				for (int g = 0; g < groups; ++g) scores(g, 0);
-				umma_commit(s.empty);
-			}
-			for (int i = 0; i < tiles && good; ++i) {
-				const int v = (2 * i + 1) % SLOTS, k = (2 * i + 2) % SLOTS;
-				const bool more = i + 1 < tiles;
-				if (!(good = wait_slot(2 * i + 1) && (!more || wait_slot(2 * i + 2)))) break;
-				for (int g = 0; g < groups; ++g) {
-					if (!(good = ap_wait(s.p_full + g, i & 1, &s.lost))) break;
-					tc_fence_after();
 #pragma unroll
-					for (int x = 0; x < AW_KEYS / 16; ++x) umma_f16_ts(tmem + O_COL + 128 * g, tmem + 128 * g + 8 * x, umma_desc_values(s.kv[v]) + 128 * x, value, (i | x) ? 1u : 0u);
-					if (more) scores(g, k);
-					else umma_commit(s.done + g);
+				for (int x = 0; x < AW_KEYS / 16; ++x) umma_f16_ts(tmem + O_COL + 128 * g, tmem + 128 * g + 8 * x, umma_desc_values(s.kv[(2 * i + 1) % SLOTS]) + 128 * x, value, (n | x) ? 1u : 0u);
+				return true;
+			};
+			// (slots are waited for before the weights and given back after both groups' products: nothing stands between a group's two)
+			bool good = true;
+			if (two) {
+				for (int i = 0; i < min(2, tiles) && good; ++i)
+					if ((good = wait_slot(2 * i))) {
+						tc_fence_after();
+						scores(i, i), umma_commit(s.empty + 2 * i % SLOTS);
+					}
+				for (int i = 0; i < tiles && good; ++i) {
+					const bool more = i + 2 < tiles;
+					if (!(good = wait_slot(2 * i + 1) && (!more || wait_slot(2 * i + 4)) && sums(i & 1, i, i >> 1))) break;
+					if (more) scores(i & 1, i + 2), umma_commit(s.empty + (2 * i + 4) % SLOTS);
+					else umma_commit(s.done + (i & 1));
+					umma_commit(s.empty + (2 * i + 1) % SLOTS);
 				}
-				if (!good) break;
-				umma_commit(s.empty + v);
-				if (more) umma_commit(s.empty + k);
+			} else {
+				good = tiles > 0 && wait_slot(0);
+				if (good) {
+					tc_fence_after();
+					for (int g = 0; g < groups; ++g) scores(g, 0);
+					umma_commit(s.empty);
+				}
+				for (int i = 0; i < tiles && good; ++i) {
+					const bool more = i + 1 < tiles;
+					if (!(good = wait_slot(2 * i + 1) && (!more || wait_slot(2 * i + 2)))) break;
+					for (int g = 0; g < groups && good; ++g) {
+						if (!(good = sums(g, i, i))) break;
+						if (more) scores(g, i + 1);
+						else umma_commit(s.done + g);
+					}
+					if (!good) break;
+					umma_commit(s.empty + (2 * i + 1) % SLOTS);
+					if (more) umma_commit(s.empty + (2 * i + 2) % SLOTS);
+				}
 			}
 			umma_commit(&s.idle); // nothing of this block's is left in the tensor core when its memory goes
 			mbar_wait_bounded(&s.idle, 0);
