@@ -50,21 +50,21 @@ constexpr float A16_MOST = 15.f, A16_SET = 10.f;
 // prefix, which all rows see, then those of each sequence of its rows, which only that sequence's rows see, in chunks of 32.  So a prefix is read once for 8 NQ rows, and a call of few rows needs one launch.
 // Each warp walks chunks of its own with references and sums of its own (no barrier between warps until the end), fed by a ring of asynchronous copies, into m16n8k16 products whose 16 rows are keys (scores: keys x queries) or
 // channels (values: channels x queries), so that eight rows of queries fill one.
-constexpr int AR_WARPS = 4, AR_KEYS = 32;
+constexpr int AR_KEYS = 32; // (of a warp's chunk)
 constexpr int AR_SHARES = 64;                // of a tile's keys at most
-constexpr int AR_TILE = 16, AR_CLUSTER = 16; // rows of a CTA at most; shares that a thread-block cluster folds at most
+constexpr int AR_TILE = 16, AR_CLUSTER = 8; // rows of a CTA at most; shares that a thread-block cluster folds
 
 template <int D>
 struct ArStage { // a warp's chunk: the next one's keys come while its values are used, the next one's values while their keys are
 	uint16_t k[AR_KEYS * D], v[AR_KEYS * D];
 };
-template <int D>
+template <int D, int W>
 __host__ __device__ constexpr size_t ar_ring() { // (the sums of the warps take its place)
-	const size_t a = (size_t)AR_WARPS * sizeof(ArStage<D>), b = ((size_t)AR_WARPS * AR_TILE * (D + 4) + (size_t)AR_TILE * (D + 2)) * sizeof(float);
+	const size_t a = (size_t)W * sizeof(ArStage<D>), b = ((size_t)W * AR_TILE * (D + 4) + (size_t)AR_TILE * (D + 2)) * sizeof(float);
 	return a > b ? a : b;
 }
-template <int D, int NQ>
-constexpr size_t ar_smem() { return (size_t)8 * NQ * D * 2 + ar_ring<D>(); }
+template <int D, int NQ, int W>
+constexpr size_t ar_smem() { return (size_t)8 * NQ * D * 2 + ar_ring<D, W>(); }
 
 template <typename T>
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
@@ -181,16 +181,17 @@ __device__ __forceinline__ float capped(float x, float cap) {
 __device__ __forceinline__ int chunks_of(int lo, int hi) { return hi > lo ? (hi - lo / AR_KEYS * AR_KEYS + AR_KEYS - 1) / AR_KEYS : 0; }
 __device__ __forceinline__ int low_of(const Attend& a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
 
-template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(const C16 c, const Attend a) {
+template <typename T, int D, int NQ, int W>
+__global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(const C16 c, const Attend a) {
 	constexpr bool KEEP = D * NQ <= 128; // the queries' fragments stay in registers
 	constexpr int KS = D / 16, MT = D / 16, PIECES = D / 8, TILE = 8 * NQ, LD = D + 4;
 	extern __shared__ __align__(128) unsigned char ar_sm[];
 	uint2* const qf = reinterpret_cast<uint2*>(ar_sm); // B fragments [KS][NQ][32]
 	ArStage<D>* const ring = reinterpret_cast<ArStage<D>*>(ar_sm + (size_t)TILE * D * 2);
-	__shared__ float fold_m[AR_WARPS][TILE], fold_l[AR_WARPS][TILE];
+	__shared__ float fold_m[W][TILE], fold_l[W][TILE];
 	__shared__ int row_seq[TILE], row_pos[TILE], row_seg[TILE], row_slot[TILE];
 	__shared__ int seg_slot[TILE + 1], seg_lo[TILE + 1], seg_hi[TILE + 1], seg_base[TILE + 1]; // the prefix and the sequences of the tile's rows: keys lo .. hi - 1 of a slot, first chunk
+	__shared__ long long row_place[TILE];                                                       // where a row's results go
 	__shared__ int list[4];                                                                     // segments, chunks, the rows' least and largest position
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 	const int kvh = blockIdx.y / a.shares, share = blockIdx.y - kvh * a.shares;
@@ -207,15 +208,15 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	const int H = c.heads, dim = c.dim;
 
 	// the queries are asked for first
-	constexpr int QF = KS * NQ * 32 / (32 * AR_WARPS) > 0 ? KS * NQ * 32 / (32 * AR_WARPS) : 1; // fragments of a thread
+	constexpr int QF = KS * NQ * 32 / (32 * W) > 0 ? KS * NQ * 32 / (32 * W) : 1; // fragments of a thread
 	uint2 qx[QF];
 	{
-		static_assert(AR_WARPS % NQ == 0, "all fragments of a thread are of one row");
+		static_assert(W % NQ == 0, "all fragments of a thread are of one row");
 		const int r = warp % NQ * 8 + g, rr = row0 + min(r, rows - 1), token = rr / a.group;
 		const uint16_t* const q = a.q + (long long)(u.t0 + token) * a.q_row + (long long)(kvh * a.group + rr - token * a.group) * a.q_head + 2 * t;
 #pragma unroll
 		for (int f = 0; f < QF; ++f) {
-			const int d = (warp + f * AR_WARPS) / NQ * 16;
+			const int d = (warp + f * W) / NQ * 16;
 			qx[f] = make_uint2(0, 0);
 			if (r < rows && d < dim) qx[f].x = q[d] | (uint32_t)q[d + 1] << 16, qx[f].y = q[d + 8] | (uint32_t)q[d + 9] << 16; // (16 channels are there or not)
 		}
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	} else {
 		if (tid < TILE) row_seq[tid] = row_pos[tid] = -1;
 		__syncthreads();
-		for (int b = u.first + tid; b <= u.last; b += 32 * AR_WARPS) {
+		for (int b = u.first + tid; b <= u.last; b += 32 * W) {
 			const int slot = c.slot[b], pos0 = c.pos0[b], start = c.start[b], count = c.count[b];
 			if (!there(c, a.rows, b)) continue;
 			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)count * a.group;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	}
 #pragma unroll
 	for (int f = 0; f < QF; ++f)
-		if (tid + f * 32 * AR_WARPS < KS * NQ * 32) qf[tid + f * 32 * AR_WARPS] = qx[f]; // B fragments
+		if (tid + f * 32 * W < KS * NQ * 32) qf[tid + f * 32 * W] = qx[f]; // B fragments
 	__syncthreads();
 	const int segs = list[0], total = list[1], least = list[2], most = list[3];
 	const int begin = (int)min((long long)total, (long long)share * a.each), end = share == a.shares - 1 ? total : min(total, begin + a.each); // (more keys than were planned for: the last share's)
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		cur_seg = next_seg, cur_pos = next_pos, cur_seen = next_seen;
 		if (next < end) {
 			copy(s.v, c.v);
-			next += AR_WARPS;
+			next += W;
 			look();
 		}
 		asm volatile("cp.async.commit_group;" ::: "memory");
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 		if (next < end) copy_keys();
 		asm volatile("cp.async.commit_group;" ::: "memory");
 	};
-	if (early) next += AR_WARPS, look(); // (both are on their way)
+	if (early) next += W, look(); // (both are on their way)
 	else look(), request_keys(), request_values();
 
 	uint2 qr[KEEP ? KS * NQ : 1];
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	const int wide = low_of(a, most); // from here on, and up to `least`, every row sees every key of a segment that is its own
 	const uint32_t lrow = lane & 7;
 
-	for (int chunk = begin + warp; chunk < end; chunk += AR_WARPS) {
+	for (int chunk = begin + warp; chunk < end; chunk += W) {
 		const int seg = cur_seg, pos = cur_pos;
 		const uint32_t seen = cur_seen;
 		asm volatile("cp.async.wait_group 1;" ::: "memory"); // the keys; the values are the group behind them
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 
 	// the warps' sums as one
 	float* const sums = reinterpret_cast<float*>(ring); // [warps][TILE][LD]
-	float* const own = sums + AR_WARPS * TILE * LD;     // [TILE][D + 2]: what this share of a cluster found
+	float* const own = sums + W * TILE * LD;     // [TILE][D + 2]: what this share of a cluster found
 	const int prefix_places = whole && u.lead >= 0 ? a.before : 0;
 	__syncthreads();
 #pragma unroll
@@ -560,51 +561,67 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 			for (int i = 0; i < MT; ++i) to[16 * i] = acc[i][q][e], to[16 * i + 8] = acc[i][q][2 + e];
 		}
 	__syncthreads();
-	{
-#pragma unroll 2
-		for (int r = warp; r < rows; r += AR_WARPS) {
+	if (prefix_places) { // with the prefix's shares: a warp a row
+#pragma unroll 1
+		for (int r = warp; r < rows; r += W) {
 			if (row_seq[r] < 0) continue;
-			float mx = fold_m[0][r], den = 0.f, wt[AR_WARPS];
-#pragma unroll
-			for (int w = 1; w < AR_WARPS; ++w) mx = fmaxf(mx, fold_m[w][r]);
-#pragma unroll
-			for (int w = 0; w < AR_WARPS; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - mx), den = fmaf(wt[w], fold_l[w][r], den);
 			const int token = u.t0 + (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
 			const size_t place = ((size_t)token * a.heads + head) * a.places;
-			if (whole) {
-				// with the prefix's shares, and a sink: one more term of the denominator
-				const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY;
-				float top = fmaxf(mx, sk), pm = -INFINITY, pl = 0.f;
-				if (lane < prefix_places) {
-					const float2 st = a.stats[place + lane];
-					pm = st.x, pl = st.y;
-				}
-				top = fmaxf(top, warp_max(pm));
-				const float pw = pm == -INFINITY ? 0.f : ex2(pm - top), down = mx == -INFINITY ? 0.f : ex2(mx - top);
-				den = den * down + warp_sum(pw * pl);
-				if (a.sinks) den += at_sink(sk, top);
-				const float norm = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
-				for (int d0 = 0; d0 < dim; d0 += 128) {
-					const int d = min(d0 + 4 * lane, dim - 4); // (every lane has a place's weight)
-					float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-					for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w] * down, *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
-					add_places(v, a.sums + place * dim + d, dim, prefix_places, pw);
-					if (d0 + 4 * lane < dim) put4<T>(a.out + token * a.o_row + head * a.o_head + d, a.out_vec, times4(v, norm));
-				}
-			} else {
-				float2* const st = a.cluster ? reinterpret_cast<float2*>(own + r * (D + 2) + D) : a.stats + place + a.before + share;
-				float* const to = a.cluster ? own + r * (D + 2) : a.sums + (place + a.before + share) * dim;
-				if (lane == 0) *st = make_float2(mx, den);
-				if (mx != -INFINITY || a.cluster)
-					for (int d = 4 * lane; d < dim; d += 128) {
-						float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-						for (int w = 0; w < AR_WARPS; ++w) add4(v, wt[w], *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
-						if (a.cluster) to[d] = v.x, to[d + 1] = v.y, to[d + 2] = v.z, to[d + 3] = v.w; // (rows of the cluster's sums are 8-byte aligned)
-						else *reinterpret_cast<float4*>(to + d) = v;
-					}
+			float pm = -INFINITY, pl = 0.f, mx = fold_m[0][r], den = 0.f, wt[W];
+			if (lane < prefix_places) {
+				const float2 st = a.stats[place + lane];
+				pm = st.x, pl = st.y;
 			}
+#pragma unroll
+			for (int w = 1; w < W; ++w) mx = fmaxf(mx, fold_m[w][r]);
+			const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY, top = fmaxf(fmaxf(mx, sk), warp_max(pm)), pw = pm == -INFINITY ? 0.f : ex2(pm - top);
+#pragma unroll
+			for (int w = 0; w < W; ++w) wt[w] = fold_m[w][r] == -INFINITY ? 0.f : ex2(fold_m[w][r] - top), den = fmaf(wt[w], fold_l[w][r], den);
+			den += warp_sum(pw * pl);
+			if (a.sinks) den += at_sink(sk, top); // one more term of the denominator
+			const float norm = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
+			for (int d0 = 0; d0 < dim; d0 += 128) {
+				const int d = min(d0 + 4 * lane, dim - 4); // (every lane has a place's weight)
+				float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+				for (int w = 0; w < W; ++w) add4(v, wt[w], *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
+				add_places(v, a.sums + place * dim + d, dim, prefix_places, pw);
+				if (d0 + 4 * lane < dim) put4<T>(a.out + token * a.o_row + head * a.o_head + d, a.out_vec, times4(v, norm));
+			}
+		}
+		return;
+	}
+	if (tid < rows) { // the warps' weights, with all that multiplies them
+		const int token = u.t0 + (row0 + tid) / a.group, head = kvh * a.group + (row0 + tid) % a.group;
+		const float sk = whole && a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY;
+		float mx = sk, den = 0.f, wt[W];
+#pragma unroll
+		for (int w = 0; w < W; ++w) mx = fmaxf(mx, fold_m[w][tid]);
+#pragma unroll
+		for (int w = 0; w < W; ++w) wt[w] = fold_m[w][tid] == -INFINITY ? 0.f : ex2(fold_m[w][tid] - mx), den = fmaf(wt[w], fold_l[w][tid], den);
+		float by = 1.f;
+		if (whole) {
+			if (a.sinks) den += at_sink(sk, mx); // one more term of the denominator
+			by = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
+		} else if (a.cluster) own[tid * (D + 2) + D] = mx, own[tid * (D + 2) + D + 1] = den;
+		else if (row_seq[tid] >= 0) a.stats[((size_t)token * a.heads + head) * a.places + a.before + share] = make_float2(mx, den);
+#pragma unroll
+		for (int w = 0; w < W; ++w) fold_m[w][tid] = wt[w] * by;
+		row_place[tid] = row_seq[tid] < 0 ? -1 : whole ? token * a.o_row + head * a.o_head : (long long)((((size_t)token * a.heads + head) * a.places + a.before + share) * dim);
+	}
+	__syncthreads();
+	const int quads = dim / 4;
+	for (int e = tid; e < rows * quads; e += 32 * W) {
+		const int r = e / quads, d = 4 * (e - r * quads);
+		float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+		for (int w = 0; w < W; ++w) add4(v, fold_m[w][r], *reinterpret_cast<const float4*>(sums + (w * TILE + r) * LD + d));
+		if (!whole && a.cluster) {
+			float* const to = own + r * (D + 2) + d; // (8-byte aligned)
+			*reinterpret_cast<float2*>(to) = make_float2(v.x, v.y), *reinterpret_cast<float2*>(to + 2) = make_float2(v.z, v.w);
+		} else if (row_place[r] >= 0) {
+			if (whole) put4<T>(a.out + row_place[r] + d, a.out_vec, v);
+			else *reinterpret_cast<float4*>(a.sums + row_place[r] + d) = v;
 		}
 	}
 	if (whole || !a.cluster) return;
@@ -634,7 +651,7 @@ __global__ void __launch_bounds__(32 * AR_WARPS, D <= 128 ? 3 : 1) k_c16_rows(co
 	}
 	__syncthreads();
 	const int all = rows * dim, from = (int)((long long)all * share / a.shares), to = (int)((long long)all * (share + 1) / a.shares);
-	for (int e = from + tid; e < to; e += 32 * AR_WARPS) {
+	for (int e = from + tid; e < to; e += 32 * W) {
 		const int r = e / dim, d = e - r * dim;
 		float v = 0.f;
 #pragma unroll 8
@@ -1158,6 +1175,7 @@ enum A16Way { A16_ROWS, A16_PREFIXES, A16_TILES };
 struct A16Plan {
 	int way;
 	int tile, shares, each, cluster; // few rows: rows of a CTA, shares of a tile's keys and the chunks of each, whether a cluster folds the shares
+	int warps;                       // of a CTA
 	int units;                       // of the grid
 	long long rows;                  // of a unit at most
 	Wide wide;                       // many rows
@@ -1173,15 +1191,22 @@ int a16_box(int page) { // keys that lie side by side in every page, as a copy's
 	while (box < 64 && page % (2 * box) == 0) box *= 2;
 	return box;
 }
-void rows_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, int group, int units, long long rows, long long keys, bool clusters) {
-	r.rows = rows, r.tile = rows > 8 ? 16 : 8;
-	const int chunks = std::max(1, (int)std::min<long long>(cdiv(keys, AR_KEYS), INT_MAX / 2));
+// Shares of a tile's keys: folded inside clusters of eight CTAs of eight warps where tiles and keys are few, through memory else.  us, clusters / memory, one sequence of 32 heads over 8 key heads of 128 channels: 1000 keys
+// 9.3 / 9.5, 4000 11.2 / 11.7, 16000 19.3 / 16.9, 60000 53 / 48 (over 2 key heads 9.5 / 9.5, 11.4 / 10.9, 19 / 15, 48 / 22); four beams behind 1000 positions 13.1 / 13.5, 4000 14.3 / 16.1, 16000 25 / 23; twice that, which
+// clusters of eight do not fit side by side, 21.4 / 19.1.  Clusters of 16 (of four warps) 18.1 and 26.5 for the four beams.
+void rows_plan(A16Plan& r, const SeqCache16& c, int group, int units, long long rows, long long keys, bool clusters) {
+	r.rows = rows, r.tile = rows > 8 ? 16 : 8, r.warps = 4;
+	const int chunks = std::max(1, (int)std::min<long long>(cdiv(keys, AR_KEYS) + 1, INT_MAX / 2));
 	const long long n = std::max(1LL, (long long)units * cdiv(rows, r.tile) * c.heads), room = AR_ROOM;
+	r.cluster = clusters && c.dim <= 128 && n <= 12 && chunks > 4 && chunks <= 192;
+	if (r.cluster) {
+		r.warps = 8, r.shares = AR_CLUSTER, r.each = cdiv(chunks, r.shares);
+		return;
+	}
+	// many CTAs: several rounds, so that the last one is short
 	long long shares = n >= room ? 1 : n > room / 2 ? cdiv(6 * room, n) : room / n;
-	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, n > room / 2 ? 2 * AR_WARPS : AR_WARPS), (long long)AR_SHARES}));
-	r.cluster = clusters && shares > 1 && n <= room / 2;
-	if (r.cluster) shares = shares >= 16 ? 16 : shares >= 8 ? 8 : shares >= 4 ? 4 : 2;
-	r.each = cdiv(chunks, shares), r.shares = r.cluster ? (int)shares : cdiv(chunks, r.each);
+	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, n > room / 2 ? 8 : 4), (long long)AR_SHARES}));
+	r.each = cdiv(chunks, shares), r.shares = cdiv(chunks, r.each);
 }
 void wide_plan(A16Plan& r, const SeqCache16& c, int units, long long rows, long long keys) {
 	r.wide_units = units, r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256);
@@ -1208,13 +1233,13 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 		wide_plan(r, c, groups, packed, seen(shared, own));
 		r.before = r.wide.shares;
 		r.units = p.n;
-		rows_plan(r, c, p, group, p.n, rows, seen(own, 16), false);
+		rows_plan(r, c, group, p.n, rows, seen(own, 16), false);
 		r.places = r.before + (r.shares > 1 ? r.shares : 0);
 		return r;
 	}
 	r.way = A16_ROWS, r.units = p.n + groups;
 	const long long most = std::max(rows, packed), together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 1; // sequences of a CTA's rows at most
-	rows_plan(r, c, p, group, groups ? groups : p.n, most, seen(shared + own * together, 16 + own), true); // (about: which sequences are in no group is the device's to know)
+	rows_plan(r, c, group, groups ? groups : p.n, most, seen(shared + own * together, 16 + own), true); // (about: which sequences are in no group is the device's to know)
 	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
@@ -1242,17 +1267,19 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	return 0;
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int W>
 cudaError_t rows_launch(const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
-	constexpr size_t smem = ar_smem<D, NQ>();
+	constexpr size_t smem = ar_smem<D, NQ, W>();
 	static std::atomic<uint64_t> done{0};
-	cudaError_t e = allow(k_c16_rows<T, D, NQ>, smem, done, true);
-	if (e == cudaSuccess) e = launch(st, after, a.cluster ? a.shares : 1, k_c16_rows<T, D, NQ>, grid, dim3(32 * AR_WARPS), smem, c, a);
+	cudaError_t e = allow(k_c16_rows<T, D, NQ, W>, smem, done, true);
+	if (e == cudaSuccess) e = launch(st, after, a.cluster ? a.shares : 1, k_c16_rows<T, D, NQ, W>, grid, dim3(32 * W), smem, c, a);
 	return e;
 }
 template <typename T, int D>
-cudaError_t rows_tile(int tile, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
-	return tile == 8 ? rows_launch<T, D, 1>(c, a, grid, after, st) : rows_launch<T, D, 2>(c, a, grid, after, st);
+cudaError_t rows_tile(const A16Plan& p, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
+	if constexpr (D <= 128)
+		if (p.warps == 8) return p.tile == 8 ? rows_launch<T, D, 1, 8>(c, a, grid, after, st) : rows_launch<T, D, 2, 8>(c, a, grid, after, st);
+	return p.tile == 8 ? rows_launch<T, D, 1, 4>(c, a, grid, after, st) : rows_launch<T, D, 2, 4>(c, a, grid, after, st);
 }
 // a pool as rows of dim channels; boxes of 64 channels and `box` rows, swizzled by the row
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
@@ -1285,8 +1312,8 @@ cudaError_t tiles_wide(const SeqCache16& cache, const C16& c, const Attend& a, c
 	return c.dim == 64 ? tiles_launch<T, 64>(cache, c, a, p, st) : tiles_launch<T, 128>(cache, c, a, p, st);
 }
 template <typename T>
-cudaError_t rows_wide(int tile, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
-	return c.dim <= 64 ? rows_tile<T, 64>(tile, c, a, grid, after, st) : c.dim <= 128 ? rows_tile<T, 128>(tile, c, a, grid, after, st) : rows_tile<T, 256>(tile, c, a, grid, after, st);
+cudaError_t rows_wide(const A16Plan& p, const C16& c, const Attend& a, dim3 grid, bool after, cudaStream_t st) {
+	return c.dim <= 64 ? rows_tile<T, 64>(p, c, a, grid, after, st) : c.dim <= 128 ? rows_tile<T, 128>(p, c, a, grid, after, st) : rows_tile<T, 256>(p, c, a, grid, after, st);
 }
 } // namespace
 } // namespace seqops
@@ -1321,7 +1348,7 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 	const bool half = cache->type == SEQ_F16;
 	cudaError_t e = cudaSuccess;
 	if (plan.way != A16_ROWS) e = half ? tiles_wide<__half>(*cache, c, a, plan, st) : tiles_wide<bf16>(*cache, c, a, plan, st);
-	if (e == cudaSuccess && plan.way != A16_TILES) e = half ? rows_wide<__half>(plan.tile, c, a, grid, plan.before > 0, st) : rows_wide<bf16>(plan.tile, c, a, grid, plan.before > 0, st);
+	if (e == cudaSuccess && plan.way != A16_TILES) e = half ? rows_wide<__half>(plan, c, a, grid, plan.before > 0, st) : rows_wide<bf16>(plan, c, a, grid, plan.before > 0, st);
 	if (e == cudaSuccess && plan.places > plan.before) {
 		const dim3 fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 		e = launch(st, true, 1, half ? k_c16_fold<__half> : k_c16_fold<bf16>, fold, dim3(128), 0, c, a);

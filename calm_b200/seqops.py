@@ -100,16 +100,19 @@ def _check(rc: int) -> None:
 
 def _run(index: int, function, *args) -> None:
     """One call of the library on torch's current stream of device `index`, with that as the current device (most often it is already)."""
-    if torch.cuda.current_device() == index:
-        _check(function(*args, _stream(index)))
+    if _device() == index:
+        rc = function(*args, _stream(index))
+        if rc:
+            _check(rc)
     else:
         with torch.cuda.device(index):
             _check(function(*args, _stream(index)))
 
 
-try:  # the handle itself; the stream object that carries it costs as much as a launch
-    from torch._C import _cuda_getCurrentRawStream as _stream
+try:  # the handle and the number themselves; the objects and checks around them cost as much as a launch (a device is in use: the call's tensors are on it)
+    from torch._C import _cuda_getCurrentRawStream as _stream, _cuda_getDevice as _device
 except ImportError:
+    _device = torch.cuda.current_device
 
     def _stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
@@ -439,28 +442,30 @@ def rotation_frequencies(dims: int, base: float = 10000.0, scaling: Optional[dic
 def _beside(rotation: Rotation, batch: Batch, index: int) -> None:
     if not isinstance(rotation, Rotation):
         raise ValueError("the rotation must be a seqops.Rotation")
-    for name, x in (("the rotation", rotation), ("the batch", batch)):
-        if x.index != index:
-            raise ValueError(f"{name} is on cuda:{x.index}, the call's other tensors on cuda:{index}")
+    if rotation.index != index or batch.index != index:
+        raise ValueError(f"the rotation is on cuda:{rotation.index}, the batch on cuda:{batch.index}, the call's other tensors on cuda:{index}")
 
 
-def _like(x: torch.Tensor, tokens: int) -> torch.Tensor:
-    """Where rows like x's go: what is behind the batch's tokens is zero."""
-    return torch.empty_like(x) if x.shape[0] == tokens else torch.zeros_like(x)
+def _like(x: torch.Tensor, rows: _Rows, tokens: int) -> Tuple[torch.Tensor, _Rows]:
+    """Where rows like x's go, which are described: what is behind the batch's tokens is zero."""
+    out = torch.empty_like(x) if rows.rows == tokens else torch.zeros_like(x)
+    stride = out.stride()
+    return out, _Rows(out.data_ptr(), rows.type, stride[0], stride[1], rows.rows)
 
 
 def rotate(x: torch.Tensor, batch: Batch, rotation: Rotation, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The batch's rows x [tokens, heads, dim] (float32, bfloat16 or float16; dim even) turned by their positions.  `out`: where they go, x itself or a tensor apart from it; rows behind the
     batch's tokens stay as they are in it (zero without one)."""
-    index = _gpu("x", x)
-    if x.dim() != 3:
+    index, shape = _gpu("x", x), x.shape
+    if len(shape) != 3:
         raise ValueError("x must be [tokens, heads, dim]")
     _beside(rotation, batch, index)
-    heads, dim = x.shape[1:]
+    heads, dim = shape[1], shape[2]
     rx = _rows("x", x, index, heads, dim, batch.tokens)
     if out is None:
-        out = _like(x, batch.tokens)
-    ro = _rows("out", out, index, heads, dim, rx.rows)
+        out, ro = _like(x, rx, batch.tokens)
+    else:
+        ro = _rows("out", out, index, heads, dim, rx.rows)
     _run(index, _load().calm_b200_seq_rotate, C.byref(batch.c), C.byref(rotation.c), C.byref(rx), C.byref(ro), heads, dim)
     return out
 
@@ -513,8 +518,9 @@ class Cache16:
             heads = q.shape[1]
             rq = _rows("q", q, index, heads, self.dim, n)
             if q_out is None:
-                q_out = _like(q, n)
-            ro = _rows("q_out", q_out, index, heads, self.dim, rq.rows)
+                q_out, ro = _like(q, rq, n)
+            else:
+                ro = _rows("q_out", q_out, index, heads, self.dim, rq.rows)
         elif q_out is not None:
             raise ValueError("q_out without q")
         _run(index, _load().calm_b200_seq_cache16_store, C.byref(c), C.byref(batch.c), C.byref(rk), C.byref(rv), turn, rq if rq is None else C.byref(rq), ro if ro is None else C.byref(ro), heads)
@@ -531,8 +537,9 @@ class Cache16:
         heads = q.shape[1]
         rq = _rows("q", q, index, heads, self.dim, batch.tokens)
         if out is None:
-            out = _like(q, batch.tokens)
-        ro = _rows("out", out, index, heads, self.dim, rq.rows)
+            out, ro = _like(q, rq, batch.tokens)
+        else:
+            ro = _rows("out", out, index, heads, self.dim, rq.rows)
         a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, None, 0)
         if sink is not None:
             _gpu("sink", sink, index)
