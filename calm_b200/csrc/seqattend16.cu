@@ -16,8 +16,8 @@ struct C16 {
 	int page_shift; // log2 of page, -1: no power of two
 	const int *start, *count, *slot, *pos0;
 	int n;
-	int groups;
-	const int *first, *members, *positions, *group;
+	int groups, alone; // groups; sequences of none
+	const int *first, *members, *positions, *group, *lonely;
 	__device__ __forceinline__ int reach(int slot) const { return (unsigned)slot < (unsigned)slots && pages > 0 ? (int)min((long long)table_pages * page, INT_MAX - 256LL) : 0; } // positions that the table has
 	__device__ __forceinline__ int page_index(int pos) const { return page_shift >= 0 ? pos >> page_shift : pos / page; }
 	__device__ __forceinline__ int page_row(int pos) const { return page_shift >= 0 ? pos & (page - 1) : pos % page; }
@@ -157,13 +157,13 @@ __device__ __forceinline__ bool own_unit(const C16& c, const Attend& a, int b, U
 	return true;
 }
 // v += what the shares at up to 32 places hold of four channels; lane k has the weight of place k.  All of them are asked for before one is used; where nothing weighs, nothing may have been written.
-__device__ __forceinline__ void add_places(float4& v, const float* p, int dim, int places, float weight) {
+__device__ __forceinline__ void add_places(float4& v, const float* p, size_t stride, int places, float weight) {
 #pragma unroll 1
 	for (int k0 = 0; k0 < places; k0 += 8) {
 		float4 x[8];
 #pragma unroll
 		for (int k = 0; k < 8; ++k)
-			if (k0 + k < places) x[k] = __ldg(reinterpret_cast<const float4*>(p + (size_t)(k0 + k) * dim));
+			if (k0 + k < places) x[k] = *reinterpret_cast<const float4*>(p + (k0 + k) * stride);
 #pragma unroll
 		for (int k = 0; k < 8; ++k) {
 			const float f = __shfl_sync(0xffffffffu, weight, k0 + k);
@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 	Unit u;
 	if (a.before) pdl_launch_next();
 	const int z = blockIdx.z;
-	bool some_rows = a.families && z < c.groups ? group_unit(c, a, z, u) : own_unit(c, a, a.families ? z - c.groups : z, u);
+	const int b = a.families && c.groups ? (z < c.groups ? 0 : c.lonely[z - c.groups]) : z;
+	bool some_rows = a.families && z < c.groups ? group_unit(c, a, z, u) : (unsigned)b < (unsigned)c.n && own_unit(c, a, b, u);
 	if (some_rows && ((a.families && z >= c.groups && u.lead >= 0) || (u.first == u.last && !there(c, a.rows, u.first)))) some_rows = false; // (a sequence that its group has; a group of one that makes no sense)
 	if (!some_rows || (long long)blockIdx.x * TILE >= (long long)u.tokens * a.group) {
 		if (a.before) pdl_wait_prev();
@@ -678,7 +679,8 @@ struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	uint64_t full[SLOTS], empty[SLOTS], mask_full[AW_MASKS], s_full[2], p_full[2], done[2], fix, idle;
 	alignas(16) uint32_t seen[AW_MASKS][4]; // keys that are there
 	int row_pos[256];
-	int span[4]; // the rows' least and largest position (of warps that found them)
+	int span[2]; // the rows' least and largest position
+	int found[3], sums[AW_THREADS / 32]; // the task
 	uint32_t tmem;
 	int lost;
 };
@@ -724,13 +726,52 @@ __device__ __forceinline__ uint64_t umma_desc_values(const void* tile) {
 	return addr | ((uint64_t)(AW_KEYS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// The work of k_c16_tiles: a CTA takes a share of the keys of 256 rows that read one key head.
+//   groups (through 0): row tiles and key heads of every group, `shares` of its prefix's keys, `each` tiles of 128 of them; results in the shares' places
+//   sequences (through 1): tasks - row tiles and key heads of all sequences, one after another - of which the first `cut` are whole, those from there to `planned` are split into `shares`, so that the last round of
+//   CTAs is as long as it has to be, and those behind (where sequences have grown since the plan was made) are whole again.  Whole ones go to out, split ones to places that k_c16_join folds.
 struct Wide {
-	int through;    // 1: every sequence's rows over its group's prefix and its own keys; 0: every group's rows over its prefix
-	int box;        // keys that a copy brings
-	int shares, each; // of a tile's keys, tiles of each
-	int tiles;      // of 256 rows, of the longest unit
-	int place;      // the first share's in stats and sums; -1: results go to out
+	int through;
+	int box;          // keys that a copy brings
+	int shares, each;
+	int tiles;        // of 256 rows, of the longest unit
+	int cut, planned;
 };
+struct Task {
+	int z, kvh, tile;
+};
+// task t: sequences in order, their key heads, their row tiles from the last (which sees most keys) on.  All of a block's N threads; false: there is none
+template <int N>
+__device__ __forceinline__ bool task_of(const C16& c, const Attend& a, int t, int (&found)[3], int (&sums)[N / 32], Task& r) { // (both: of shared memory)
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+	int before = 0;
+	if (tid == 0) found[0] = -1;
+	for (int b0 = 0; b0 < c.n; b0 += N) {
+		const int b = b0 + tid;
+		const int tiles = b < c.n && there(c, a.rows, b) ? (int)(((long long)c.count[b] * a.group + 255) / 256) : 0;
+		int sum = tiles;
+#pragma unroll
+		for (int o = 1; o < 32; o *= 2) {
+			const int x = __shfl_up_sync(0xffffffffu, sum, o);
+			if (lane >= o) sum += x;
+		}
+		__syncthreads();
+		if (lane == 31) sums[warp] = sum;
+		__syncthreads();
+		int all = 0;
+		for (int w = 0; w < N / 32; ++w) {
+			if (w < warp) sum += sums[w];
+			all += sums[w];
+		}
+		const long long from = (long long)(before + sum - tiles) * c.heads, to = (long long)(before + sum) * c.heads;
+		if (t >= from && t < to) found[0] = b, found[1] = (int)((t - from) / tiles), found[2] = tiles - 1 - (int)((t - from) % tiles);
+		before += all;
+		if ((long long)before * c.heads > t) break;
+	}
+	__syncthreads();
+	r.z = found[0], r.kvh = found[1], r.tile = found[2];
+	return r.z >= 0;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const C16 c, const Attend a, const Wide w) {
@@ -740,12 +781,21 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	extern __shared__ __align__(1024) unsigned char aw_raw[]; // (all of the kernel's shared memory: it starts where the swizzle's pattern does)
 	Shared& s = *reinterpret_cast<Shared*>(aw_raw);
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-	const int per = w.tiles * c.heads, share = blockIdx.x / per, kvh = blockIdx.x % per / w.tiles, tile = w.tiles - 1 - blockIdx.x % w.tiles; // (longest rows first)
 	pdl_launch_next();
 	Unit u;
+	Task task;
+	int share = 0, shares = 1, place0 = -1; // the places of a split task's rows
 	if (w.through) {
-		if (!own_unit(c, a, blockIdx.z, u)) return;
-	} else if (!group_unit(c, a, blockIdx.z, u)) return;
+		const int split = (w.planned - w.cut) * w.shares, x = (int)blockIdx.x - w.cut;
+		if (x >= 0 && x < split) share = x % w.shares, shares = w.shares, place0 = x * 256;
+		if (!task_of<AW_THREADS>(c, a, x < 0 ? (int)blockIdx.x : x < split ? w.cut + x / w.shares : w.planned + x - split, s.found, s.sums, task) || !own_unit(c, a, task.z, u)) return;
+	} else {
+		const int per = w.tiles * c.heads;
+		share = blockIdx.x / per, shares = w.shares, task.kvh = blockIdx.x % per / w.tiles, task.tile = blockIdx.x % w.tiles;
+		if (!group_unit(c, a, blockIdx.z, u)) return;
+	}
+	const int kvh = task.kvh, tile = task.tile;
+	const bool partial = !w.through || shares > 1;
 	if ((long long)tile * 256 >= (long long)u.tokens * a.group) return;
 	const int row0 = tile * 256, rows = (int)min(256LL, (long long)u.tokens * a.group - row0), groups = rows > 128 ? 2 : 1;
 	const bool two = groups == 1; // the same rows twice: each of two groups of warps takes every other tile, and their sums are added at the end
@@ -773,7 +823,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 #pragma unroll
 		for (int k = 0; k < 2; ++k) base[k] = lo[k] & ~(w.box - 1), count[k] = u.tokens > 0 && hi[k] > lo[k] ? (hi[k] - base[k] + AW_KEYS - 1) / AW_KEYS : 0;
 		const int total = count[0] + count[1];
-		begin = (int)min((long long)total, (long long)share * w.each), tiles = (share == w.shares - 1 ? total : min(total, begin + w.each)) - begin;
+		const int each = w.through ? (total + shares - 1) / shares : w.each;
+		begin = (int)min((long long)total, (long long)share * each), tiles = (share == shares - 1 ? total : min(total, begin + each)) - begin;
 	};
 	const int low = pos0 + row0 / a.group, high = pos0 + (row0 + rows - 1) / a.group; // of one sequence's rows
 	__syncthreads();
@@ -929,7 +980,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			const bool lost = *(volatile int*)&s.lost;
 			const int token = u.t0 + (row0 + min(r, rows - 1)) / a.group, head = kvh * a.group + (row0 + min(r, rows - 1)) % a.group;
 			const bool writes = r < rows && rpos >= 0 && !(two && group);
-			const size_t place = ((size_t)token * a.heads + head) * a.places + w.place + share;
+			const size_t place = w.through ? (size_t)max(place0, 0) + r : ((size_t)token * a.heads + head) * a.places + share;
 			float* const row = reinterpret_cast<float*>(s.kv) + tid * (D + 4);
 			asm volatile("bar.sync 3, 256;" ::: "memory"); // (both groups' products have ended)
 			float f0 = 1.f, f1 = 0.f; // of this group's sums and the other's
@@ -953,7 +1004,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				}
 			}
 			float norm = 1.f;
-			if (w.place < 0) {
+			if (!partial) {
 				const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY, mn = fmaxf(m, sk), down = m == -INFINITY ? 0.f : ex2(m - mn);
 				l *= down;
 				if (a.sinks) l += at_sink(sk, mn);
@@ -962,7 +1013,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			if (lost) norm = NAN;
 			// A thread's row goes to shared memory (where keys and values were: the last product has ended, of the other group's too once both have) and from there as one copy.
 			const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 16 == 0;
-			const bool nothing = w.place >= 0 && m == -INFINITY && !lost; // (the fold leaves out what weighs nothing)
+			const bool nothing = partial && m == -INFINITY && !lost; // (the fold leaves out what weighs nothing)
 #pragma unroll 1
 			for (int col = 0; col < c.dim && !(two && group); col += 16) {
 				float v[16];
@@ -976,7 +1027,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 #pragma unroll
 					for (int k = 0; k < 16; ++k) v[k] = fmaf(v[k], f0, other[col + k] * f1);
 				}
-				if (w.place >= 0) {
+				if (partial) {
 #pragma unroll
 					for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(row + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
 				} else {
@@ -994,8 +1045,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				}
 			}
 			fence_async_smem();
-			if (writes && !nothing && (w.place >= 0 || vec)) {
-				if (w.place >= 0) bulk_store(a.sums + place * c.dim, row, c.dim * 4);
+			if (writes && !nothing && (partial || vec)) {
+				if (partial) bulk_store(a.sums + place * c.dim, row, c.dim * 4);
 				else bulk_store(a.out + token * a.o_row + head * a.o_head, row, c.dim * 2);
 			}
 			asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory"); // (written: what follows in the stream may read it)
@@ -1133,6 +1184,33 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
+// Folds the shares of a split task (Wide), 32 rows a block, a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(128) k_c16_join(const C16 c, const Attend a, const Wide w) {
+	pdl_wait_prev();
+	Task task;
+	Unit u;
+	__shared__ int found[3], sums[4];
+	if (!task_of<128>(c, a, w.cut + blockIdx.x, found, sums, task) || !own_unit(c, a, task.z, u)) return;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = task.tile * 256, rows = (int)min(256LL, (long long)u.tokens * a.group - row0);
+	for (int r = blockIdx.y * 32 + warp; r < min(rows, (int)blockIdx.y * 32 + 32); r += 4) {
+		const int token = u.t0 + (row0 + r) / a.group, head = task.kvh * a.group + (row0 + r) % a.group;
+		const size_t place = (size_t)blockIdx.x * w.shares * 256 + r;
+		const float sk = a.sinks ? a.sinks[head] * A16_LOG2E : -INFINITY;
+		const float2 st = lane < w.shares ? a.stats[place + lane * 256] : make_float2(-INFINITY, 0.f);
+		const float top = fmaxf(sk, warp_max(st.x)), weight = st.x == -INFINITY ? 0.f : ex2(st.x - top);
+		float den = warp_sum(weight * st.y);
+		if (a.sinks) den += at_sink(sk, top);
+		const float norm = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den; // (0: nothing was seen; a NaN stays one)
+		for (int d0 = 0; d0 < c.dim; d0 += 128) {
+			const int d = min(d0 + 4 * lane, c.dim - 4);
+			float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+			add_places(v, a.sums + place * c.dim + d, (size_t)256 * c.dim, w.shares, weight);
+			if (d0 + 4 * lane < c.dim) put4<T>(a.out + token * a.o_row + head * a.o_head + d, a.out_vec, times4(v, norm));
+		}
+	}
+}
+
 // Folds the shares of one (token, head), in the order of their places: a warp for each.
 template <typename T>
 __global__ void __launch_bounds__(128) k_c16_fold(const C16 c, const Attend a) {
@@ -1181,6 +1259,7 @@ struct A16Plan {
 	Wide wide;                       // many rows
 	int wide_units;
 	int before, places;
+	long long tasks, split_places;   // many rows of sequences: CTAs, places of the split ones' rows
 };
 constexpr int AR_ROOM = 148 * 3; // CTAs of few rows that run at a time
 constexpr int AW_ROOM = 148;     // and of many
@@ -1208,12 +1287,29 @@ void rows_plan(A16Plan& r, const SeqCache16& c, int group, int units, long long 
 	shares = std::max(1LL, std::min({shares, (long long)cdiv(chunks, n > room / 2 ? 8 : 4), (long long)AR_SHARES}));
 	r.each = cdiv(chunks, shares), r.shares = cdiv(chunks, r.each);
 }
-void wide_plan(A16Plan& r, const SeqCache16& c, int units, long long rows, long long keys) {
-	r.wide_units = units, r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256);
-	const long long n = std::max(1LL, (long long)units * r.wide.tiles * c.heads);
-	const int tiles = std::max(1, (int)std::min<long long>(cdiv(keys, AW_KEYS), INT_MAX / 2));
-	const long long shares = std::max(1LL, std::min({(long long)AW_ROOM / n, (long long)cdiv(tiles, 2), (long long)AW_SHARES}));
-	r.wide.each = cdiv(tiles, shares), r.wide.shares = cdiv(tiles, r.wide.each);
+// Groups: as many shares of their prefixes as CTAs run at a time, of one length for all groups (`lengths`: what each of them shared when the batch was described).
+void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long rows, long long most) {
+	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide_units = s.n;
+	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
+	const long long per = (long long)r.wide.tiles * c.heads;
+	auto ctas = [&](int each) { // that have keys
+		long long n = 0;
+		for (int g = 0; g < s.n; ++g) n += std::max(1, cdiv(s.lengths ? std::min<long long>(s.lengths[g], most) : most, (long long)each * AW_KEYS));
+		return n * per;
+	};
+	int each = std::max(cdiv(longest, AW_SHARES), std::min(4, longest)); // (two for each group of warps)
+	while (each < longest && ctas(each) > AW_ROOM) each += std::max(1, each / 16);
+	r.wide.each = std::min(each, longest), r.wide.shares = cdiv(longest, r.wide.each);
+}
+// Sequences: whole tasks, but for those that a last round of fewer CTAs than run at a time would have.
+void tasks_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, const SeqAttend16& a, long long rows, long long most) {
+	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide.through = 1, r.wide_units = 1;
+	const long long all = (long long)p.n * r.wide.tiles * c.heads, live = a.row_tiles > 0 ? std::min(all, a.row_tiles * c.heads) : all, rest = live % AW_ROOM;
+	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
+	const long long shares = rest ? std::min<long long>({AW_ROOM / rest, cdiv(longest, 4), AW_SHARES}) : 1;
+	r.wide.shares = (int)std::max(1LL, shares), r.wide.planned = (int)std::min<long long>(live, INT_MAX), r.wide.cut = shares > 1 ? (int)(live - rest) : r.wide.planned;
+	r.tasks = all + (long long)(r.wide.planned - r.wide.cut) * (r.wide.shares - 1);
+	r.split_places = (long long)(r.wide.planned - r.wide.cut) * r.wide.shares * 256;
 }
 A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, const SeqAttend16& a) {
 	A16Plan r = {};
@@ -1224,26 +1320,26 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	const bool wide = (c.dim == 64 || (c.dim > 64 && c.dim <= 128)) && c.page % 8 == 0 && c.pages > 0;
 	if (wide && rows >= 96) {
 		r.way = A16_TILES;
-		wide_plan(r, c, p.n, rows, seen(std::max(1, a.most_keys), 256 / group + 1));
-		r.wide.through = 1, r.places = r.wide.shares > 1 ? r.wide.shares : 0, r.wide.place = r.places ? 0 : -1;
+		tasks_plan(r, c, p, a, rows, seen(std::max(1, a.most_keys), 256 / group + 1));
 		return r;
 	}
 	if (wide && packed >= 48 && shared >= 512) {
 		r.way = A16_PREFIXES;
-		wide_plan(r, c, groups, packed, seen(shared, own));
+		groups_plan(r, c, *s, packed, seen(shared, own));
 		r.before = r.wide.shares;
 		r.units = p.n;
 		rows_plan(r, c, group, p.n, rows, seen(own, 16), false);
 		r.places = r.before + (r.shares > 1 ? r.shares : 0);
 		return r;
 	}
-	r.way = A16_ROWS, r.units = p.n + groups;
+	r.way = A16_ROWS, r.units = groups ? groups + s->n_alone : p.n;
 	const long long most = std::max(rows, packed), together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 1; // sequences of a CTA's rows at most
-	rows_plan(r, c, group, groups ? groups : p.n, most, seen(shared + own * together, 16 + own), true); // (about: which sequences are in no group is the device's to know)
+	rows_plan(r, c, group, r.units, most, seen(shared + own * together, 16 + own), true);
 	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
-size_t a16_bytes(const SeqCache16& c, const SeqAttend16& a, const A16Plan& p) { return (size_t)a.q.rows * a.heads * p.places * (c.dim * sizeof(float) + sizeof(float2)); }
+size_t a16_rows(const SeqAttend16& a, const A16Plan& p) { return p.way == A16_TILES ? p.split_places : (size_t)a.q.rows * a.heads * p.places; }
+size_t a16_bytes(const SeqCache16& c, const SeqAttend16& a, const A16Plan& p) { return a16_rows(a, p) * (c.dim * sizeof(float) + sizeof(float2)); }
 
 int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s, const SeqAttend16* a) {
 	if (const int rc = check_cache16("attend16", c, p)) return rc;
@@ -1258,7 +1354,8 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	if (s) {
 		if (s->n < 0 || s->n > p->n || s->longest < 0 || s->tokens < 0 || s->most_own < 0) return refuse("attend16: %d groups of %d sequences, longest %d, tokens %d", s->n, p->n, s->longest, s->tokens);
 		if (s->n && (!s->first || !s->count || !s->positions || !s->group)) return refuse("attend16: the groups' description is missing");
-		if (((uintptr_t)s->first | (uintptr_t)s->count | (uintptr_t)s->positions | (uintptr_t)s->group) % 4) return refuse("attend16: the groups' description is not aligned to 4 bytes");
+		if (s->n_alone < 0 || s->n_alone > p->n || (s->n && s->n_alone && !s->alone)) return refuse("attend16: %d sequences of %d in no group of the groups' description", s->n_alone, p->n);
+		if (((uintptr_t)s->first | (uintptr_t)s->count | (uintptr_t)s->positions | (uintptr_t)s->group | (uintptr_t)s->alone) % 4) return refuse("attend16: the groups' description is not aligned to 4 bytes");
 		if (p->n + s->n > 65535) return refuse("attend16: %d sequences and %d groups: at most 65535", p->n, s->n);
 	}
 	if (std::max(p->longest, s && s->n ? s->tokens : 0) * group > INT_MAX - 256) return refuse("attend16: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence or group", std::max(p->longest, s ? s->tokens : 0), (int)group);
@@ -1304,7 +1401,7 @@ cudaError_t tiles_launch(const SeqCache16& cache, const C16& c, const Attend& a,
 	cudaError_t e = pool_map(mk, cache, cache.k, p.wide.box);
 	if (e == cudaSuccess) e = pool_map(mv, cache, cache.v, p.wide.box);
 	if (e == cudaSuccess) e = allow(k_c16_tiles<T, D>, sizeof(AwShared<D>), done);
-	if (e == cudaSuccess) e = launch(st, false, 1, k_c16_tiles<T, D>, dim3(p.wide.tiles * c.heads * p.wide.shares, 1, p.wide_units), dim3(AW_THREADS), sizeof(AwShared<D>), mk, mv, c, a, p.wide);
+	if (e == cudaSuccess) e = launch(st, false, 1, k_c16_tiles<T, D>, dim3((unsigned)(p.way == A16_TILES ? p.tasks : (long long)p.wide.tiles * c.heads * p.wide.shares), 1, p.wide_units), dim3(AW_THREADS), sizeof(AwShared<D>), mk, mv, c, a, p.wide);
 	return e;
 }
 template <typename T>
@@ -1334,21 +1431,23 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 	C16 c = {};
 	c.k = (const uint16_t*)cache->k, c.v = (const uint16_t*)cache->v, c.table = cache->table, c.pages = cache->pages, c.heads = cache->heads, c.page = cache->page, c.dim = cache->dim;
 	c.slots = cache->slots, c.table_pages = cache->table_pages, c.page_shift = log2_of(cache->page), c.start = batch->start, c.count = batch->count, c.slot = batch->slot, c.pos0 = batch->pos0, c.n = batch->n;
-	if (shared && shared->n) c.groups = shared->n, c.first = shared->first, c.members = shared->count, c.positions = shared->positions, c.group = shared->group;
+	if (shared && shared->n) c.groups = shared->n, c.first = shared->first, c.members = shared->count, c.positions = shared->positions, c.group = shared->group, c.alone = shared->n_alone, c.lonely = shared->alone;
 	Attend a = {};
 	a.q = (const uint16_t*)q->q.p, a.q_row = q->q.row_stride, a.q_head = q->q.head_stride, a.out = (uint16_t*)q->out.p, a.o_row = q->out.row_stride, a.o_head = q->out.head_stride;
 	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap, a.window = q->window, a.sinks = q->sinks;
 	a.out_vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 8 == 0;
 	a.families = plan.way == A16_ROWS, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = plan.before, a.places = plan.places;
-	a.sums = (float*)q->workspace, a.stats = (float2*)(a.sums + (size_t)a.rows * a.heads * a.places * c.dim);
+	a.sums = (float*)q->workspace, a.stats = (float2*)(a.sums + a16_rows(*q, plan) * c.dim);
 	const dim3 grid(plan.way == A16_TILES ? 1 : cdiv(plan.rows, plan.tile), cache->heads * std::max(1, plan.shares), plan.units);
 	if (grid.y > 65535) return refuse("attend16: too many key heads");
-	if ((long long)plan.wide.tiles * cache->heads * plan.wide.shares > INT_MAX) return refuse("attend16: too many rows");
+	if ((long long)plan.wide.tiles * cache->heads * plan.wide.shares > INT_MAX || plan.tasks > INT_MAX || plan.split_places > INT_MAX) return refuse("attend16: too many rows");
 	const cudaStream_t st = (cudaStream_t)stream;
 	const bool half = cache->type == SEQ_F16;
 	cudaError_t e = cudaSuccess;
 	if (plan.way != A16_ROWS) e = half ? tiles_wide<__half>(*cache, c, a, plan, st) : tiles_wide<bf16>(*cache, c, a, plan, st);
 	if (e == cudaSuccess && plan.way != A16_TILES) e = half ? rows_wide<__half>(plan, c, a, grid, plan.before > 0, st) : rows_wide<bf16>(plan, c, a, grid, plan.before > 0, st);
+	if (e == cudaSuccess && plan.split_places)
+		e = launch(st, true, 1, half ? k_c16_join<__half> : k_c16_join<bf16>, dim3(plan.wide.planned - plan.wide.cut, 8), dim3(128), 0, c, a, plan.wide);
 	if (e == cudaSuccess && plan.places > plan.before) {
 		const dim3 fold(std::min(cdiv((long long)batch->longest * a.group, 4), 65535), cache->heads, batch->n);
 		e = launch(st, true, 1, half ? k_c16_fold<__half> : k_c16_fold<bf16>, fold, dim3(128), 0, c, a);

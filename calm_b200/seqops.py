@@ -57,12 +57,13 @@ class _Cache16(C.Structure):
 
 
 class _Shared(C.Structure):
-    _fields_ = [("n", _int), ("first", _ptr), ("count", _ptr), ("positions", _ptr), ("group", _ptr), ("longest", _int), ("tokens", _int), ("most_own", _int)]
+    _fields_ = [("n", _int), ("first", _ptr), ("count", _ptr), ("positions", _ptr), ("group", _ptr), ("n_alone", _int), ("alone", _ptr), ("longest", _int), ("tokens", _int), ("most_own", _int),
+                ("lengths", _ptr)]
 
 
 class _Attend16(C.Structure):
-    _fields_ = [("q", _Rows), ("out", _Rows), ("heads", _int), ("scale", C.c_float), ("window", _int), ("softcap", C.c_float), ("sinks", _ptr), ("most_keys", _int), ("workspace", _ptr),
-                ("workspace_bytes", _size)]
+    _fields_ = [("q", _Rows), ("out", _Rows), ("heads", _int), ("scale", C.c_float), ("window", _int), ("softcap", C.c_float), ("sinks", _ptr), ("most_keys", _int), ("row_tiles", _ll),
+                ("workspace", _ptr), ("workspace_bytes", _size)]
 
 
 _lib = None
@@ -255,13 +256,23 @@ class Batch:
         base, step = self.data.data_ptr(), self.data.stride(0) * 4
         self.c = _Portions(len(sl), base, base + step, base + 2 * step, base + 3 * step, self.longest)
         self.groups = self.group_of = self.shared = None
+        self._counts, self._tiles = cn, {}
         if len(groups):
             own = at.astype(np.int64) + cn - np.where(of >= 0, groups[of, 2], 0)
             tokens = max(int(cn[f:f + n].sum()) for f, n, _ in groups.tolist())
-            both = torch.from_numpy(np.concatenate([groups.T.reshape(-1), of])).to(self.data.device)
-            self.groups, self.group_of = both[:groups.size].view(3, -1), both[groups.size:]
+            alone, self._lengths = np.flatnonzero(of < 0).astype(np.int32), np.ascontiguousarray(groups[:, 2])
+            both = torch.from_numpy(np.concatenate([groups.T.reshape(-1), of, alone])).to(self.data.device)
+            self.groups, self.group_of = both[:groups.size].view(3, -1), both[groups.size:groups.size + len(of)]
             base, step = both.data_ptr(), 4 * len(groups)
-            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, int(groups[:, 2].max()), tokens, int(own.max()))
+            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, len(alone), base + 3 * step + 4 * len(of), int(groups[:, 2].max()), tokens, int(own.max()),
+                                  self._lengths.ctypes.data)
+
+    def _row_tiles(self, group: int) -> int:
+        """Tiles of 256 pairs of token and head, `group` heads a token, over all sequences."""
+        n = self._tiles.get(group)
+        if n is None:
+            n = self._tiles[group] = int(-(-(self._counts.astype(np.int64) * group) // 256).sum()) if len(self._counts) else 0
+        return n
 
 
 def _grouped(shared, cn: np.ndarray, at: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
@@ -540,7 +551,7 @@ class Cache16:
             out, ro = _like(q, rq, batch.tokens)
         else:
             ro = _rows("out", out, index, heads, self.dim, rq.rows)
-        a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, None, 0)
+        a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, batch._row_tiles(heads // self.heads), None, 0)
         if sink is not None:
             _gpu("sink", sink, index)
             if sink.shape != (heads,) or sink.dtype != torch.float32 or not sink.is_contiguous():

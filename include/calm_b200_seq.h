@@ -465,9 +465,12 @@ struct SeqShared {
 	int n;
 	const int *first, *count, *positions; /* device [n] */
 	const int* group;                     /* device [sequences]: the group that a sequence is in, -1: none */
+	int n_alone;
+	const int* alone;                     /* device [n_alone]: the sequences that are in none */
 	int longest;                          /* at least the largest of positions */
 	int tokens;                           /* at least the new tokens of any group */
 	int most_own;                         /* at least the keys of any sequence behind what it shares (what the split of the work is planned for; more are still seen) */
+	const int* lengths;                   /* HOST [n] or NULL: about what each group shares (what the split of the work is planned for) */
 };
 /* Attention of the batch's tokens over the cache, which holds them already: the token at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p); query
  * head h reads key head h / (heads / cache.heads).
@@ -483,6 +486,7 @@ struct SeqAttend16 {
 	float softcap;           /* > 0: s = softcap tanh(s / softcap) after the scale */
 	const float* sinks;      /* [heads] or NULL */
 	int most_keys;           /* at least the keys that any token sees (what the split of the work is planned for; more are still seen) */
+	long long row_tiles;     /* about the sum over the sequences of ceil(tokens * (heads / cache.heads) / 256) (what the split of the work is planned for); 0: as many as there can be */
 	void* workspace;         /* calm_b200_seq_attend16_workspace bytes, 16-byte aligned; undefined between calls, not to be shared by calls that may overlap */
 	size_t workspace_bytes;
 };

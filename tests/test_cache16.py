@@ -44,7 +44,7 @@ def rotation(**over):
 
 
 def shared(**over):
-    return made(seqops._Shared, dict(n=1, first=4096, count=4096, positions=4096, group=4096, longest=100, tokens=10, most_own=20), over)
+    return made(seqops._Shared, dict(n=1, first=4096, count=4096, positions=4096, group=4096, n_alone=0, alone=None, longest=100, tokens=10, most_own=20, lengths=None), over)
 
 
 def ref(x):
@@ -52,7 +52,7 @@ def ref(x):
 
 
 def attend(c=None, p=None, s=None, stream=False, **over):
-    a = made(seqops._Attend16, dict(q=rows(), out=rows(), heads=4, scale=1.0, window=0, softcap=0.0, sinks=None, most_keys=100, workspace=None, workspace_bytes=0), over)
+    a = made(seqops._Attend16, dict(q=rows(), out=rows(), heads=4, scale=1.0, window=0, softcap=0.0, sinks=None, most_keys=100, row_tiles=0, workspace=None, workspace_bytes=0), over)
     return ref(c or cache()), ref(p or portions()), ref(s), ref(a)
 
 
@@ -106,7 +106,7 @@ def test_attend_refusals_and_workspace():
         says(L.calm_b200_seq_attend16(*attend(c=cache(**over)), None), "attend16", word)
     for over, word in BAD_BATCHES:
         says(L.calm_b200_seq_attend16(*attend(p=portions(**over)), None), "attend16", word)
-    for over, word in ((dict(n=-1), "groups"), (dict(n=3), "groups"), (dict(longest=-1), "groups"), (dict(tokens=-1), "groups"), (dict(most_own=-1), "groups"), (dict(first=None), "groups"), (dict(group=None), "groups"),
+    for over, word in ((dict(n=-1), "groups"), (dict(n=3), "groups"), (dict(longest=-1), "groups"), (dict(tokens=-1), "groups"), (dict(most_own=-1), "groups"), (dict(first=None), "groups"), (dict(group=None), "groups"), (dict(n_alone=-1), "no group"), (dict(n_alone=3), "no group"), (dict(n_alone=1), "no group"), (dict(n_alone=1, alone=4098), "aligned"),
                        (dict(positions=4098), "aligned")):
         says(L.calm_b200_seq_attend16(*attend(s=shared(**over)), None), "attend16", word)
     for over, word in ((dict(heads=3), "query heads"), (dict(heads=0), "query heads"), (dict(q=rows(type=4)), "type"), (dict(out=rows(type=2)), "type"), (dict(q=rows(type=0), out=rows(type=0)), "type"),
