@@ -688,6 +688,7 @@ struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
 	asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
 }
+static_assert(sizeof(AwShared<128>) <= 227 * 1024 && sizeof(AwShared<64>) <= 227 * 1024, "shared memory of a CTA");
 // a row of scores
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
 #define AW_R8(b) "=f"(v[b]), "=f"(v[b + 1]), "=f"(v[b + 2]), "=f"(v[b + 3]), "=f"(v[b + 4]), "=f"(v[b + 5]), "=f"(v[b + 6]), "=f"(v[b + 7])
@@ -1275,7 +1276,7 @@ int a16_box(int page) { // keys that lie side by side in every page, as a copy's
 // clusters of eight do not fit side by side, 21.4 / 19.1.  Clusters of 16 (of four warps) 18.1 and 26.5 for the four beams.
 void rows_plan(A16Plan& r, const SeqCache16& c, int group, int units, long long rows, long long keys, bool clusters) {
 	r.rows = rows, r.tile = rows > 8 ? 16 : 8, r.warps = 4;
-	const int chunks = std::max(1, (int)std::min<long long>(cdiv(keys, AR_KEYS) + 1, INT_MAX / 2));
+	const int chunks = (int)std::min<long long>(std::max(keys, 0LL) / AR_KEYS + 2, INT_MAX / 2); // (they begin anywhere)
 	const long long n = std::max(1LL, (long long)units * cdiv(rows, r.tile) * c.heads), room = AR_ROOM;
 	r.cluster = clusters && c.dim <= 128 && n <= 12 && chunks > 4 && chunks <= 192;
 	if (r.cluster) {
@@ -1298,6 +1299,7 @@ void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long 
 		return n * per;
 	};
 	int each = std::max(cdiv(longest, AW_SHARES), std::min(4, longest)); // (two for each group of warps)
+	if (s.n * per >= AW_ROOM) each = longest;
 	while (each < longest && ctas(each) > AW_ROOM) each += std::max(1, each / 16);
 	r.wide.each = std::min(each, longest), r.wide.shares = cdiv(longest, r.wide.each);
 }
@@ -1315,26 +1317,41 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	A16Plan r = {};
 	const int group = a.heads / c.heads, groups = s ? s->n : 0;
 	const long long rows = (long long)p.longest * group, packed = groups ? (long long)s->tokens * group : 0;
-	const long long shared = groups ? s->longest : 0, own = std::max(1, groups ? s->most_own : a.most_keys);
-	auto seen = [&](long long keys, long long tokens) { return a.window > 0 ? std::min(keys, (long long)a.window + tokens) : keys; };
-	const bool wide = (c.dim == 64 || (c.dim > 64 && c.dim <= 128)) && c.page % 8 == 0 && c.pages > 0;
-	if (wide && rows >= 96) {
+	// keys that a row sees at most: of a prefix, behind one, of a sequence of no group
+	auto seen = [&](long long keys) { return a.window > 0 ? std::min(keys, (long long)a.window + p.longest) : keys; };
+	const long long shared = groups ? seen(s->longest) : 0, own = groups ? seen(s->most_own) : 0, lone = groups ? (s->n_alone ? seen(s->most_alone) : 0) : seen(std::max(a.most_keys, 1));
+	const bool wide = (c.dim == 64 || (c.dim > 64 && c.dim <= 128)) && c.page % 8 == 0 && c.pages > 0 && std::max(rows, packed) <= 65535 * 256LL;
+	// Each way's time, estimated in us from the work that it does; the least.  Of 135 shapes that were measured in all their ways (1 to 8 groups of 3 to 64 sequences of 1 to 100 tokens behind 600 to 12000 positions, 1 to 8 key
+	// heads of 64 and 128 channels) the rule takes one that is 1.4 % slower than the best in the mean.  us, few rows / prefixes / tiles: 8 groups of 8 sequences of 4 heads a key head behind up to 3000 positions 33 / 50, 4 groups of 16
+	// behind up to 12000 104 / 79, one of 64 behind 600 25 / 33, behind 3000 37 / 35; 16 sequences of up to 20 tokens behind 600 56 / 43 / 25, behind 12000 253 / 88 / 185; 3 of 60 behind 4000 97 / 47 / 51.
+	double prefix = (double)shared; // what the groups share in the mean
+	if (groups && s->lengths) {
+		prefix = 0.;
+		for (int g = 0; g < groups; ++g) prefix += std::min<double>(s->lengths[g], (double)shared) / groups;
+	}
+	const int alone = groups ? s->n_alone : p.n;
+	const long long together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 0; // sequences of a CTA's rows at most
+	const long long most = std::max(shared + own * together, lone), units = groups + alone, tiles_g = (long long)groups * cdiv(packed, 16) * c.heads, tiles_a = (long long)alone * cdiv(rows, 16) * c.heads;
+	const double us_rows = 10. + (tiles_g * (prefix + own * together) + tiles_a * lone) / 20000. + 2. * most / (128. * std::max<double>(1., std::min<double>(AR_SHARES, (double)AR_ROOM / std::max(tiles_g + tiles_a, 1LL))));
+	const double us_tile = 2. / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs
+	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(packed, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
+	const double us_tiles = 24. + us_tile * c.heads * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256)) * (groups ? prefix + own : lone);
+	if (wide && rows >= 32 && us_tiles < us_rows && (!groups || us_tiles <= us_prefixes)) {
 		r.way = A16_TILES;
-		tasks_plan(r, c, p, a, rows, seen(std::max(1, a.most_keys), 256 / group + 1));
+		tasks_plan(r, c, p, a, rows, std::max(shared + own, lone));
 		return r;
 	}
-	if (wide && packed >= 48 && shared >= 512) {
+	if (wide && packed > 0 && us_prefixes < us_rows) {
 		r.way = A16_PREFIXES;
-		groups_plan(r, c, *s, packed, seen(shared, own));
+		groups_plan(r, c, *s, packed, shared);
 		r.before = r.wide.shares;
 		r.units = p.n;
-		rows_plan(r, c, group, p.n, rows, seen(own, 16), false);
+		rows_plan(r, c, group, p.n, rows, std::max(own, lone), false);
 		r.places = r.before + (r.shares > 1 ? r.shares : 0);
 		return r;
 	}
-	r.way = A16_ROWS, r.units = groups ? groups + s->n_alone : p.n;
-	const long long most = std::max(rows, packed), together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 1; // sequences of a CTA's rows at most
-	rows_plan(r, c, group, r.units, most, seen(shared + own * together, 16 + own), true);
+	r.way = A16_ROWS, r.units = (int)units;
+	rows_plan(r, c, group, r.units, std::max(rows, packed), most, true);
 	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
@@ -1352,7 +1369,7 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	if (a->heads > 65535) return refuse("attend16: at most 65535 query heads");
 	const long long group = a->heads / c->heads;
 	if (s) {
-		if (s->n < 0 || s->n > p->n || s->longest < 0 || s->tokens < 0 || s->most_own < 0) return refuse("attend16: %d groups of %d sequences, longest %d, tokens %d", s->n, p->n, s->longest, s->tokens);
+		if (s->n < 0 || s->n > p->n || s->longest < 0 || s->tokens < 0 || s->most_own < 0 || s->most_alone < 0) return refuse("attend16: %d groups of %d sequences, longest %d, tokens %d", s->n, p->n, s->longest, s->tokens);
 		if (s->n && (!s->first || !s->count || !s->positions || !s->group)) return refuse("attend16: the groups' description is missing");
 		if (s->n_alone < 0 || s->n_alone > p->n || (s->n && s->n_alone && !s->alone)) return refuse("attend16: %d sequences of %d in no group of the groups' description", s->n_alone, p->n);
 		if (((uintptr_t)s->first | (uintptr_t)s->count | (uintptr_t)s->positions | (uintptr_t)s->group | (uintptr_t)s->alone) % 4) return refuse("attend16: the groups' description is not aligned to 4 bytes");
@@ -1360,7 +1377,8 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	}
 	if (std::max(p->longest, s && s->n ? s->tokens : 0) * group > INT_MAX - 256) return refuse("attend16: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence or group", std::max(p->longest, s ? s->tokens : 0), (int)group);
 	if ((uintptr_t)a->sinks % 4) return refuse("attend16: sinks are not aligned to 4 bytes");
-	if (!(a->scale == a->scale) || a->window < 0 || !(a->softcap >= 0.f)) return refuse("attend16: scale, window or softcap out of range");
+	if (!(a->scale == a->scale) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY)) return refuse("attend16: scale, window or softcap out of range");
+	if (a->row_tiles < 0) return refuse("attend16: %lld row tiles", a->row_tiles);
 	return 0;
 }
 
@@ -1453,4 +1471,11 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 		e = launch(st, true, 1, half ? k_c16_fold<__half> : k_c16_fold<bf16>, fold, dim3(128), 0, c, a);
 	}
 	return e == cudaSuccess ? 0 : failed("attend16", e);
+}
+
+extern "C" int calm_b200_seq_attend16_way(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared, const struct SeqAttend16* args) {
+	using namespace seqops;
+	if (const int rc = check_attend16(cache, batch, shared, args)) return rc;
+	const A16Plan p = a16_plan(*cache, *batch, shared, *args);
+	return p.way | (p.way == A16_ROWS && p.cluster ? 4 : 0) | (p.places > p.before || p.split_places ? 8 : 0);
 }

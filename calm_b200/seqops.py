@@ -58,7 +58,7 @@ class _Cache16(C.Structure):
 
 class _Shared(C.Structure):
     _fields_ = [("n", _int), ("first", _ptr), ("count", _ptr), ("positions", _ptr), ("group", _ptr), ("n_alone", _int), ("alone", _ptr), ("longest", _int), ("tokens", _int), ("most_own", _int),
-                ("lengths", _ptr)]
+                ("most_alone", _int), ("lengths", _ptr)]
 
 
 class _Attend16(C.Structure):
@@ -88,6 +88,7 @@ def _load() -> C.CDLL:
         args = [C.POINTER(_Cache16), C.POINTER(_Portions), C.POINTER(_Shared), C.POINTER(_Attend16)]
         L.calm_b200_seq_attend16_workspace.argtypes, L.calm_b200_seq_attend16_workspace.restype = args, _size
         L.calm_b200_seq_attend16.argtypes, L.calm_b200_seq_attend16.restype = args + [_ptr], _int
+        L.calm_b200_seq_attend16_way.argtypes, L.calm_b200_seq_attend16_way.restype = args, _int
         _lib = L
     return _lib
 
@@ -264,8 +265,8 @@ class Batch:
             both = torch.from_numpy(np.concatenate([groups.T.reshape(-1), of, alone])).to(self.data.device)
             self.groups, self.group_of = both[:groups.size].view(3, -1), both[groups.size:groups.size + len(of)]
             base, step = both.data_ptr(), 4 * len(groups)
-            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, len(alone), base + 3 * step + 4 * len(of), int(groups[:, 2].max()), tokens, int(own.max()),
-                                  self._lengths.ctypes.data)
+            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, len(alone), base + 3 * step + 4 * len(of), int(groups[:, 2].max()), tokens,
+                                  int(own[of >= 0].max()), int(own[of < 0].max(initial=0)), self._lengths.ctypes.data)
 
     def _row_tiles(self, group: int) -> int:
         """Tiles of 256 pairs of token and head, `group` heads a token, over all sequences."""

@@ -469,7 +469,7 @@ struct SeqShared {
 	const int* alone;                     /* device [n_alone]: the sequences that are in none */
 	int longest;                          /* at least the largest of positions */
 	int tokens;                           /* at least the new tokens of any group */
-	int most_own;                         /* at least the keys of any sequence behind what it shares (what the split of the work is planned for; more are still seen) */
+	int most_own, most_alone;             /* about the most keys of a group's sequence behind what it shares, of a sequence of no group (what the split of the work is planned for; more are still seen) */
 	const int* lengths;                   /* HOST [n] or NULL: about what each group shares (what the split of the work is planned for) */
 };
 /* Attention of the batch's tokens over the cache, which holds them already: the token at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p); query
@@ -492,6 +492,9 @@ struct SeqAttend16 {
 };
 size_t calm_b200_seq_attend16_workspace(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args);
 int calm_b200_seq_attend16(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args, void* stream);
+/* how a call would go, for tests: 0 few rows (prefix and own keys in one list), 1 prefixes as tiles of many rows first, 2 every sequence as tiles of many rows; + 4: clusters fold the shares of keys, + 8: another
+ * kernel folds them; or -3 */
+int calm_b200_seq_attend16_way(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args);
 
 #ifdef __cplusplus
 }

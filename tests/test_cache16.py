@@ -44,7 +44,7 @@ def rotation(**over):
 
 
 def shared(**over):
-    return made(seqops._Shared, dict(n=1, first=4096, count=4096, positions=4096, group=4096, n_alone=0, alone=None, longest=100, tokens=10, most_own=20, lengths=None), over)
+    return made(seqops._Shared, dict(n=1, first=4096, count=4096, positions=4096, group=4096, n_alone=0, alone=None, longest=100, tokens=10, most_own=20, most_alone=0, lengths=None), over)
 
 
 def ref(x):
@@ -106,12 +106,12 @@ def test_attend_refusals_and_workspace():
         says(L.calm_b200_seq_attend16(*attend(c=cache(**over)), None), "attend16", word)
     for over, word in BAD_BATCHES:
         says(L.calm_b200_seq_attend16(*attend(p=portions(**over)), None), "attend16", word)
-    for over, word in ((dict(n=-1), "groups"), (dict(n=3), "groups"), (dict(longest=-1), "groups"), (dict(tokens=-1), "groups"), (dict(most_own=-1), "groups"), (dict(first=None), "groups"), (dict(group=None), "groups"), (dict(n_alone=-1), "no group"), (dict(n_alone=3), "no group"), (dict(n_alone=1), "no group"), (dict(n_alone=1, alone=4098), "aligned"),
+    for over, word in ((dict(n=-1), "groups"), (dict(n=3), "groups"), (dict(longest=-1), "groups"), (dict(tokens=-1), "groups"), (dict(most_own=-1), "groups"), (dict(most_alone=-1), "groups"), (dict(first=None), "groups"), (dict(group=None), "groups"), (dict(n_alone=-1), "no group"), (dict(n_alone=3), "no group"), (dict(n_alone=1), "no group"), (dict(n_alone=1, alone=4098), "aligned"),
                        (dict(positions=4098), "aligned")):
         says(L.calm_b200_seq_attend16(*attend(s=shared(**over)), None), "attend16", word)
     for over, word in ((dict(heads=3), "query heads"), (dict(heads=0), "query heads"), (dict(q=rows(type=4)), "type"), (dict(out=rows(type=2)), "type"), (dict(q=rows(type=0), out=rows(type=0)), "type"),
-                       (dict(out=rows(rows=9)), "rows"), (dict(window=-1), "range"), (dict(softcap=-1.0), "range"), (dict(softcap=float("nan")), "range"), (dict(scale=float("nan")), "range"),
-                       (dict(q=rows(p=None)), "missing"), (dict(sinks=4098), "aligned")):
+                       (dict(out=rows(rows=9)), "rows"), (dict(window=-1), "range"), (dict(softcap=-1.0), "range"), (dict(softcap=float("nan")), "range"), (dict(softcap=math.inf), "range"), (dict(scale=float("nan")), "range"),
+                       (dict(q=rows(p=None)), "missing"), (dict(sinks=4098), "aligned"), (dict(row_tiles=-1), "row tiles")):
         says(L.calm_b200_seq_attend16(*attend(**over), None), "attend16", word)
     for longest, heads in ((1 << 30, 72), (2 ** 31 - 1, 4)):
         says(L.calm_b200_seq_attend16(*attend(p=portions(longest=longest), heads=heads), None), "attend16", "pairs")
@@ -124,6 +124,24 @@ def test_attend_refusals_and_workspace():
     says(L.calm_b200_seq_attend16(*attend(**a), None), "workspace")
     says(L.calm_b200_seq_attend16(*attend(**a, workspace=4096, workspace_bytes=need - 1), None), "workspace")
     says(L.calm_b200_seq_attend16(*attend(**a, workspace=4100, workspace_bytes=need), None), "workspace")
+
+
+def test_the_way_follows_sizes_types_and_pages():
+    """Shapes that were measured in all their ways (the rule stands at a16_plan), and what the tensor-memory kernel does not serve."""
+    def way(n, longest, heads, kv, dim, page, groups=0, positions=0, own=50, keys=4000, **over):
+        s = shared(n=groups, longest=positions, tokens=n * longest // max(groups, 1), most_own=own) if groups else None
+        big = rows(rows=n * longest, row_stride=heads * dim, head_stride=dim)
+        return L.calm_b200_seq_attend16_way(*attend(c=cache(heads=kv, dim=dim, page=page, pages=5000), p=portions(n=n, longest=longest), s=s, heads=heads, q=big, out=big, most_keys=keys, **over))
+
+    assert way(1, 1, 32, 8, 128, 16) == 4 and way(4, 1, 32, 8, 128, 16, 1, 3000) == 4            # a user's tokens, four beams: clusters
+    assert way(1, 1, 32, 8, 128, 16, keys=16000) == 8 and way(150, 1, 32, 8, 128, 16, keys=900) == 0  # shares through memory; none
+    assert way(64, 1, 32, 8, 128, 16, 1, 16000, 1000) == 1 and way(64, 1, 32, 8, 128, 16, 1, 600) & 3 == 0
+    assert way(16, 300, 32, 8, 128, 16, 1, 12000, 300, keys=12300) & 3 in (1, 2) and way(2, 900, 32, 8, 128, 16, keys=900) & 3 == 2
+    for dim, page in ((128, 12), (256, 16), (48, 16)):
+        assert way(64, 1, 32, 8, dim, page, 1, 16000, 1000) & 3 == 0 and way(2, 900, 32, 8, dim, page, keys=900) & 3 == 0
+    for dim in (64, 80, 96, 112, 128):
+        assert way(2, 900, 32, 8, dim, 24, keys=900) & 3 == 2
+    assert way(3, 1, 3, 2, 64, 16) == -3
 
 
 def test_batches_of_groups():

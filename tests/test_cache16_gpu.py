@@ -304,6 +304,43 @@ def test_attention_of_many_rows(page, dim, kv_heads, group, counts, before, grou
     attention(counts, before, groups, kv_heads, group, dim, page, dtype)
 
 
+def way_of(cache, table, q, batch):
+    """The way that Cache16.attend's call takes."""
+    import ctypes as C
+
+    c = cache._with(torch.tensor(table, device="cuda"), batch)
+    r = seqops._rows("q", q, 0, q.shape[1], cache.dim, batch.tokens)
+    a = seqops._Attend16(r, r, q.shape[1], 1.0, 0, 0.0, None, batch.most_keys, batch._row_tiles(q.shape[1] // cache.heads), None, 0)
+    return seqops._load().calm_b200_seq_attend16_way(C.byref(c), C.byref(batch.c), None if batch.shared is None else C.byref(batch.shared), C.byref(a))
+
+
+@pytest.mark.parametrize("way,page,dim,kv_heads,group,counts,before,groups", [
+    (0, 16, 128, 8, 4, [1] * 70, [200] * 70, []), (4, 16, 128, 2, 4, [1, 1], [1200, 1210], [(0, 2, 1200)]), (8, 16, 64, 4, 4, [1] * 9, [1000 * (i % 3) for i in range(9)], []),
+    (1, 16, 128, 8, 4, [1] * 48, [6000 + i for i in range(48)], [(0, 48, 6000)]), (9, 8, 64, 2, 8, [1] * 50, [12000 + 40 * (i % 9) for i in range(48)] + [5000, 13], [(0, 24, 12000), (24, 24, 9001)]),
+    (2, 16, 128, 37, 1, [256, 100, 3, 200], [0, 100, 600, 40], []), (10, 16, 128, 2, 4, [300, 1, 170, 90], [1500, 1500, 1500, 1600], [(0, 4, 1500)]), (10, 24, 80, 1, 4, [900], [0], [])])
+def test_every_way(way, page, dim, kv_heads, group, counts, before, groups):
+    made = make(counts, before, groups, kv_heads, group, dim, page, torch.bfloat16, 3)
+    assert way_of(*made[:4]) == way
+    check_attend(*made, counts, before, groups, sink=torch.randn(kv_heads * group, generator=gen(5), device="cuda"))
+
+
+def test_groups_and_sequences_without_tokens():
+    attention([0, 0, 1, 0, 40], [700, 700, 30, 9, 5], [(0, 2, 640), (3, 1, 9)], 2, 4, 128, 16, "bf16")
+    attention([0, 0, 300], [700, 700, 30], [(0, 2, 640)], 2, 4, 128, 16, "bf16")
+    made = make([0, 0], [700, 700], [(0, 2, 640)], 2, 4, 128, 16, torch.bfloat16)
+    assert made[0].attend(made[2], torch.tensor(made[1], device="cuda"), made[3], scale=1.0).shape == (0, 8, 128)
+
+
+def test_sequences_that_have_grown_since_the_call_was_captured():
+    """Positions and counts past what the split of the work was planned for."""
+    for counts, before, groups, more in (([1] * 6, [100] * 6, [(0, 4, 64)], 1800), ([1], [50], [], 3000), ([200, 100], [100, 64], [(0, 2, 64)], 700), ([1] * 40, [64] * 40, [(0, 40, 48)], 900)):
+        now = [b + more for b in before]
+        cache, table, q, batch, slots = make(counts, now, groups, 2, 4, 128, 16, torch.bfloat16, 5)
+        small = seqops.Batch([int(s) for s in slots], counts, before, shared=groups)
+        small.data[3] += more
+        check_attend(cache, table, q, small, slots, counts, now, groups, got=cache.attend(q, torch.tensor(table, device="cuda"), small, scale=128 ** -0.5))
+
+
 def test_attention_of_few_tokens_over_many_keys():
     attention([1], [40000], [], 2, 4, 128, 16, "bf16")
     attention([1, 1], [30000, 30010], [(0, 2, 30000)], 1, 8, 64, 16, "fp16")
