@@ -1274,10 +1274,10 @@ int a16_box(int page) { // keys that lie side by side in every page, as a copy's
 // Shares of a tile's keys: folded inside clusters of eight CTAs of eight warps where tiles and keys are few, through memory else.  us, clusters / memory, one sequence of 32 heads over 8 key heads of 128 channels: 1000 keys
 // 9.3 / 9.5, 4000 11.2 / 11.7, 16000 19.3 / 16.9, 60000 53 / 48 (over 2 key heads 9.5 / 9.5, 11.4 / 10.9, 19 / 15, 48 / 22); four beams behind 1000 positions 13.1 / 13.5, 4000 14.3 / 16.1, 16000 25 / 23; twice that, which
 // clusters of eight do not fit side by side, 21.4 / 19.1.  Clusters of 16 (of four warps) 18.1 and 26.5 for the four beams.
-void rows_plan(A16Plan& r, const SeqCache16& c, int group, int units, long long rows, long long keys, bool clusters) {
-	r.rows = rows, r.tile = rows > 8 ? 16 : 8, r.warps = 4;
+void rows_plan(A16Plan& r, const SeqCache16& c, long long n, long long rows, long long keys, bool clusters) { // n: tiles that have rows
+	n = std::max(1LL, n), r.rows = rows, r.tile = rows > 8 ? 16 : 8, r.warps = 4;
 	const int chunks = (int)std::min<long long>(std::max(keys, 0LL) / AR_KEYS + 2, INT_MAX / 2); // (they begin anywhere)
-	const long long n = std::max(1LL, (long long)units * cdiv(rows, r.tile) * c.heads), room = AR_ROOM;
+	const long long room = AR_ROOM;
 	r.cluster = clusters && c.dim <= 128 && n <= 12 && chunks > 4 && chunks <= 192;
 	if (r.cluster) {
 		r.warps = 8, r.shares = AR_CLUSTER, r.each = cdiv(chunks, r.shares);
@@ -1333,7 +1333,7 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	const long long together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 0; // sequences of a CTA's rows at most
 	const long long most = std::max(shared + own * together, lone), units = groups + alone, tiles_g = (long long)groups * cdiv(packed, 16) * c.heads, tiles_a = (long long)alone * cdiv(rows, 16) * c.heads;
 	const double us_rows = 10. + (tiles_g * (prefix + own * together) + tiles_a * lone) / 20000. + 2. * most / (128. * std::max<double>(1., std::min<double>(AR_SHARES, (double)AR_ROOM / std::max(tiles_g + tiles_a, 1LL))));
-	const double us_tile = 2. / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs
+	const double us_tile = (a.softcap > 0.f ? 6. : 2.) / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs (a soft cap: two more special functions a score)
 	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(packed, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
 	const double us_tiles = 24. + us_tile * c.heads * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256)) * (groups ? prefix + own : lone);
 	if (wide && rows >= 32 && us_tiles < us_rows && (!groups || us_tiles <= us_prefixes)) {
@@ -1346,12 +1346,12 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 		groups_plan(r, c, *s, packed, shared);
 		r.before = r.wide.shares;
 		r.units = p.n;
-		rows_plan(r, c, group, p.n, rows, std::max(own, lone), false);
+		rows_plan(r, c, (long long)p.n * cdiv(rows, 16) * c.heads, rows, std::max(own, lone), false);
 		r.places = r.before + (r.shares > 1 ? r.shares : 0);
 		return r;
 	}
 	r.way = A16_ROWS, r.units = (int)units;
-	rows_plan(r, c, group, r.units, std::max(rows, packed), most, true);
+	rows_plan(r, c, tiles_g + tiles_a, std::max(rows, packed), most, true);
 	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
