@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	} else {
 		for (int b = u.first + (warp < 8 ? tid : tid - 32); b <= u.last; b += AW_THREADS - 64) {
 			const int p0 = c.pos0[b], start = c.start[b], n = c.count[b];
-			if (!there(c, a.rows, b) || warp > 9) continue;
+			if (!there(c, a.rows, b)) continue;
 			const long long r0 = (long long)(start - u.t0) * a.group - row0, r1 = r0 + (long long)n * a.group;
 			for (long long r = max(r0, 0LL); r < min(r1, (long long)rows); ++r) s.row_pos[r] = p0 + (int)((unsigned)(r - r0) / (unsigned)a.group);
 		}

@@ -324,6 +324,13 @@ def test_every_way(way, page, dim, kv_heads, group, counts, before, groups):
     check_attend(*made, counts, before, groups, sink=torch.randn(kv_heads * group, generator=gen(5), device="cuda"))
 
 
+@pytest.mark.parametrize("way,group,counts,before,groups", [(1, 4, [1] * 700, [1200 + i % 40 for i in range(700)], [(0, 330, 1200), (330, 370, 1190)]), (0, 1, [1] * 400, [20 + i % 7 for i in range(400)], [(0, 400, 16)])])
+def test_groups_of_more_sequences_than_a_block_has_threads(way, group, counts, before, groups):
+    made = make(counts, before, groups, 2, group, 64, 16, torch.bfloat16, 21)
+    check_attend(*made, counts, before, groups)
+    assert way_of(*made[:4]) & 3 == way
+
+
 def test_groups_and_sequences_without_tokens():
     attention([0, 0, 1, 0, 40], [700, 700, 30, 9, 5], [(0, 2, 640), (3, 1, 9)], 2, 4, 128, 16, "bf16")
     attention([0, 0, 300], [700, 700, 30], [(0, 2, 640)], 2, 4, 128, 16, "bf16")
