@@ -1306,7 +1306,9 @@ void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long 
 // Sequences: whole tasks, but for those that a last round of fewer CTAs than run at a time would have.
 void tasks_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, const SeqAttend16& a, long long rows, long long most) {
 	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide.through = 1, r.wide_units = 1;
-	const long long all = (long long)p.n * r.wide.tiles * c.heads, live = a.row_tiles > 0 ? std::min(all, a.row_tiles * c.heads) : all, rest = live % AW_ROOM;
+	// As many tasks as there can be, whatever the counts become: no more tiles than the rows fill and one begun for every sequence.  (A prompt of 8192 tokens among 255 single ones behind 2000 positions 1234 us; with as many
+	// blocks for each as the prompt has tiles 3318.)
+	const long long all = std::min((long long)p.n * r.wide.tiles, (long long)a.q.rows * (a.heads / c.heads) / 256 + p.n) * c.heads, live = a.row_tiles > 0 ? std::min(all, a.row_tiles * c.heads) : all, rest = live % AW_ROOM;
 	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
 	const long long shares = rest ? std::min<long long>({AW_ROOM / rest, cdiv(longest, 4), AW_SHARES}) : 1;
 	r.wide.shares = (int)std::max(1LL, shares), r.wide.planned = (int)std::min<long long>(live, INT_MAX), r.wide.cut = shares > 1 ? (int)(live - rest) : r.wide.planned;
@@ -1377,7 +1379,7 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	}
 	if (std::max(p->longest, s && s->n ? s->tokens : 0) * group > INT_MAX - 256) return refuse("attend16: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence or group", std::max(p->longest, s ? s->tokens : 0), (int)group);
 	if ((uintptr_t)a->sinks % 4) return refuse("attend16: sinks are not aligned to 4 bytes");
-	if (!(a->scale == a->scale) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY)) return refuse("attend16: scale, window or softcap out of range");
+	if (!(std::fabs(a->scale) < INFINITY) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY) || (a->softcap > 0.f && !(2.f * A16_LOG2E * std::fabs(a->scale) / a->softcap < INFINITY))) return refuse("attend16: scale, window or softcap out of range");
 	if (a->row_tiles < 0) return refuse("attend16: %lld row tiles", a->row_tiles);
 	return 0;
 }

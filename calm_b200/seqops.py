@@ -235,8 +235,8 @@ class Batch:
     count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest`.
 
     shared: groups of neighbouring sequences that go on from one text, as (first sequence, sequences, positions): a cache holds the positions below that once, on the pages that the
-    table names for the group's first sequence, and Cache16.attend reads them once for all of the group.  The device array `groups` (int32 rows first, sequences, positions) may be written between replays
-    too (positions up to the largest that was given)."""
+    table names for the group's first sequence, and Cache16.attend reads them once for all of the group.  Of the device array `groups` (int32 rows first, sequences, positions) the positions may be written
+    between replays too, up to the largest that was given; which sequences a group has stays."""
 
     def __init__(self, slots: Sequence[int], counts: Sequence[int], before: Sequence[int], device=None, shared: Sequence[Tuple[int, int, int]] = ()):
         sl, cn, at = (np.array(_list(name, x), np.int32) for name, x in (("slots", slots), ("counts", counts), ("before", before)))

@@ -126,6 +126,11 @@ def test_attend_refusals_and_workspace():
     says(L.calm_b200_seq_attend16(*attend(**a, workspace=4100, workspace_bytes=need), None), "workspace")
 
 
+@pytest.mark.parametrize("over", [dict(scale=math.inf), dict(scale=-math.inf), dict(scale=1.0, softcap=1e-44)])
+def test_attend_refuses_scores_that_no_number_holds(over):
+    says(L.calm_b200_seq_attend16(*attend(**over), None), "attend16", "range")
+
+
 def test_the_way_follows_sizes_types_and_pages():
     """Shapes that were measured in all their ways (the rule stands at a16_plan), and what the tensor-memory kernel does not serve."""
     def way(n, longest, heads, kv, dim, page, groups=0, positions=0, own=50, keys=4000, **over):

@@ -331,6 +331,19 @@ def test_groups_of_more_sequences_than_a_block_has_threads(way, group, counts, b
     assert way_of(*made[:4]) & 3 == way
 
 
+def test_one_prompt_among_single_tokens():
+    """As many blocks as the rows have tiles, not as many as if every sequence were as long as the longest."""
+    for groups in ([], [(0, 30, 64)]):
+        attention([1] * 40 + [1100] + [0] * 3 + [1] * 20, [64 + 9 * i for i in range(64)], groups, 2, 4, 64, 16, "bf16", seed=23)
+        attention([1300, 0, 2], [0, 5, 100], [], 3, 2, 128, 8, "fp16", seed=24)
+
+
+@pytest.mark.parametrize("counts,before,groups", [([1, 1, 2], [300, 310, 305], [(0, 2, 300)]), ([90] * 5, [300] * 5, [(0, 4, 288)]), ([400], [0], [])])
+def test_scales_below_zero(counts, before, groups):
+    attention(counts, before, groups, 2, 4, 128, 16, "bf16", seed=25, scale=-0.11)
+    attention(counts, before, groups, 2, 4, 64, 16, "fp16", seed=26, scale=-0.11, softcap=3.0)
+
+
 def test_groups_and_sequences_without_tokens():
     attention([0, 0, 1, 0, 40], [700, 700, 30, 9, 5], [(0, 2, 640), (3, 1, 9)], 2, 4, 128, 16, "bf16")
     attention([0, 0, 300], [700, 700, 30], [(0, 2, 640)], 2, 4, 128, 16, "bf16")
