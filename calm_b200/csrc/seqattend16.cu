@@ -32,7 +32,8 @@ struct Attend {
 	float scale, softcap;
 	int window;
 	const float* sinks;
-	int families;     // 1: groups with their prefixes and own keys, and the sequences of no group; 0: every sequence behind what it shares
+	int families;     // 1: groups with their prefixes and own keys, and the sequences of no group; 0: every sequence behind what it shares;
+	                  // -t: k_c16_rows has the sequences of at most t tokens with their prefixes, k_c16_tiles the others, both at once
 	int shares, each; // shares of a tile's keys, chunks of each
 	int cluster;      // 1: the shares of a tile are a cluster
 	int before;       // places of `stats` and `sums` that the prefixes' shares have
@@ -50,6 +51,8 @@ constexpr float A16_MOST = 15.f, A16_SET = 10.f;
 // prefix, which all rows see, then those of each sequence of its rows, which only that sequence's rows see, in chunks of 32.  So a prefix is read once for 8 NQ rows, and a call of few rows needs one launch.
 // Each warp walks chunks of its own with references and sums of its own (no barrier between warps until the end), fed by a ring of asynchronous copies, into m16n8k16 products whose 16 rows are keys (scores: keys x queries) or
 // channels (values: channels x queries), so that eight rows of queries fill one.
+// Bound: memory where keys are many - 32 sequences of up to 6000 keys, 8 key heads of 128 channels (500 MB) 87 us, 5.8 TB/s with the fold - and the way of a chunk (copy, products, softmax, products) where they are few: 4 sequences
+// behind 4000 shared ones 13.7 us, 64 CTAs. Masked or capped scores cost instructions: 18 sequences of 5 tokens, window 2048, cap and sinks 36 us at 0.4 of the issue slots.
 constexpr int AR_KEYS = 32; // (of a warp's chunk)
 constexpr int AR_SHARES = 64;                // of a tile's keys at most
 constexpr int AR_TILE = 16, AR_CLUSTER = 8; // rows of a CTA at most; shares that a thread-block cluster folds
@@ -198,11 +201,17 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 	Unit u;
 	if (a.before) pdl_launch_next();
 	const int z = blockIdx.z;
-	const int b = a.families && c.groups ? (z < c.groups ? 0 : c.lonely[z - c.groups]) : z;
-	bool some_rows = a.families && z < c.groups ? group_unit(c, a, z, u) : (unsigned)b < (unsigned)c.n && own_unit(c, a, b, u);
-	if (some_rows && ((a.families && z >= c.groups && u.lead >= 0) || (u.first == u.last && !there(c, a.rows, u.first)))) some_rows = false; // (a sequence that its group has; a group of one that makes no sense)
+	const bool grouped = a.families == 1 && c.groups;
+	const int b = grouped ? (z < c.groups ? 0 : c.lonely[z - c.groups]) : z;
+	bool some_rows = grouped && z < c.groups ? group_unit(c, a, z, u) : (unsigned)b < (unsigned)c.n && own_unit(c, a, b, u);
+	if (some_rows && ((grouped && z >= c.groups && u.lead >= 0) || (u.first == u.last && !there(c, a.rows, u.first)))) some_rows = false; // (a sequence that its group has; a group of one that makes no sense)
+	if (D <= 128 && some_rows && a.families < 0 && u.tokens > -a.families) some_rows = false;
+	// The kernel before this one has ended when this one has: all blocks wait for what they read of it, or where they read nothing one does.
+	auto wait = [&]() {
+		if (a.before || (D <= 128 && a.families < 0 && !(blockIdx.x | blockIdx.y | blockIdx.z))) pdl_wait_prev();
+	};
 	if (!some_rows || (long long)blockIdx.x * TILE >= (long long)u.tokens * a.group) {
-		if (a.before) pdl_wait_prev();
+		wait();
 		return;
 	}
 	const int row0 = blockIdx.x * TILE, rows = (int)min((long long)TILE, (long long)u.tokens * a.group - row0);
@@ -278,9 +287,9 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 		if (tid == 0) {
 			const int slot = c.slot[u.first], reach = c.reach(slot);
 			const bool with = a.families && u.prefix > 0;
-			const int lo0 = with ? low_of(a, low) : 0, hi0 = with ? (a.window ? min(min(u.prefix, high + 1), reach) : prefix) : 0, lo1 = max(u.prefix, low_of(a, low)), hi1 = min(high + 1, reach);
+			const int lo0 = with ? low_of(a, low) : 0, hi0 = with ? (a.window ? min(min(u.prefix, high + 1), c.reach(lead_slot)) : prefix) : 0, lo1 = max(u.prefix, low_of(a, low)), hi1 = min(high + 1, reach);
 			const int n0 = chunks_of(lo0, hi0), n1 = chunks_of(lo1, hi1);
-			seg_slot[0] = seg_slot[1] = slot, seg_lo[0] = lo0, seg_hi[0] = hi0, seg_lo[1] = lo1, seg_hi[1] = hi1, seg_base[0] = 0, seg_base[1] = n0;
+			seg_slot[0] = lead_slot, seg_slot[1] = slot, seg_lo[0] = lo0, seg_hi[0] = hi0, seg_lo[1] = lo1, seg_hi[1] = hi1, seg_base[0] = 0, seg_base[1] = n0;
 			list[0] = 2, list[1] = n0 + n1, list[2] = low, list[3] = high;
 		}
 	} else {
@@ -546,7 +555,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 			for (int o = 4; o < 32; o *= 2) l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], o);
 			if (g == 0) fold_m[warp][8 * q + 2 * t + e] = m[q][e], fold_l[warp][8 * q + 2 * t + e] = l[q][e];
 		}
-	if (a.before) pdl_wait_prev(); // the prefixes' shares
+	wait(); // the prefixes' shares
 
 	// the warps' sums as one
 	float* const sums = reinterpret_cast<float*>(ring); // [warps][TILE][LD]
@@ -663,11 +672,16 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 }
 
 // ---------------------------------------------------------------- many rows
-// Where many rows see the same keys, the products run on the fifth-generation tensor cores: a CTA takes one or two groups of 128 rows that read one key head - of a group of sequences over its prefix, or of one sequence
-// over its group's prefix and its own keys - and walks tiles of 128 keys.  One warp copies tiles with TMA, boxes of 64 channels and as many keys as lie side by side in a page (8 to 64), straight into the layout
-// that the products read: keys as rows, values as they lie with the channels as the product's columns.  One thread issues S = Q K^T of the next tile behind O += P V of this one; four warps a group, a row a thread, take S from tensor
-// memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run.  O stays in tensor memory; it is rescaled in the rare case that
-// a row's reference moves.
+// Where many rows see the same keys, the products run on the fifth-generation tensor cores: a CTA takes up to 256 rows that read one key head - of a group of sequences over its prefix, or of one sequence over its group's prefix
+// and its own keys - and walks tiles of 128 keys.  Two warps, one for keys and one for values, copy tiles with TMA, boxes of 64 channels and as many keys as lie side by side in a page (8 to 64), straight into the layout that the
+// products read: keys as rows, values as they lie with the channels as the product's columns.  One thread issues S = Q K^T of the next tile behind O += P V of this one; four warps for each 128 rows, a row a thread, take S from
+// tensor memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run; up to 128 rows are taken by both groups, every other tile
+// each, and their sums are added at the end.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.  Tiles that some row sees in part go through a slower way of 32 columns at a time in few
+// instructions.  Results leave through shared memory, a row a copy.
+// Bound: a tile's way through its roles.  256 rows and 128 keys of 128 channels take about 3700 cycles: the products 2048 by the tensor cores' rate (about 2560 as they are, 80 cycles for 64), softmax 1680 to 1800 for a group and
+// 110 of hand-over.  16 sequences of up to 300 tokens behind 12000 positions, 32 heads over 8: 722 us where the products alone would be 378 (0.44 of the tensor pipes, 0.47 of the special functions'); its loads alone took 570 us
+// from pages of 16 keys, 459 of 32, 416 of 64, 795 of 8.  Tried: tiles of 64 keys with scores ahead 1330 us (N = 64 costs what N = 128 does), weights handed over in halves 905 to 1134, a polynomial for part of the exponentials
+// 1085 against 973, a product thread a group 977 to 1017.
 constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
 constexpr int AW_SOFTMAX_REGS = 176, AW_OTHER_REGS = 144; // 256 x 176 + 128 x 144 = 63488 of the 384 x 168 = 64512 that the block is launched with
 
@@ -749,7 +763,7 @@ __device__ __forceinline__ bool task_of(const C16& c, const Attend& a, int t, in
 	if (tid == 0) found[0] = -1;
 	for (int b0 = 0; b0 < c.n; b0 += N) {
 		const int b = b0 + tid;
-		const int tiles = b < c.n && there(c, a.rows, b) ? (int)(((long long)c.count[b] * a.group + 255) / 256) : 0;
+		const int tiles = b < c.n && there(c, a.rows, b) && c.count[b] > -a.families ? (int)(((long long)c.count[b] * a.group + 255) / 256) : 0;
 		int sum = tiles;
 #pragma unroll
 		for (int o = 1; o < 32; o *= 2) {
@@ -1185,7 +1199,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// Folds the shares of a split task (Wide), 32 rows a block, a warp a row.
+// Folds the shares of a split task (Wide), 32 rows a block, a warp a row.  Bound: latency; 20 tasks of 7 shares (17 MB) 20 us with caches cold, behind a kernel that the split makes 110 us shorter.
 template <typename T>
 __global__ void __launch_bounds__(128) k_c16_join(const C16 c, const Attend a, const Wide w) {
 	pdl_wait_prev();
@@ -1212,7 +1226,7 @@ __global__ void __launch_bounds__(128) k_c16_join(const C16 c, const Attend a, c
 	}
 }
 
-// Folds the shares of one (token, head), in the order of their places: a warp for each.
+// Folds the shares of one (token, head), in the order of their places: a warp for each.  Bound: latency; 18 sequences of 5 tokens with 24 heads 7.8 us, 32 of one token with 32 heads and 11 shares 8.5 us (caches cold, launch included).
 template <typename T>
 __global__ void __launch_bounds__(128) k_c16_fold(const C16 c, const Attend a) {
 	pdl_wait_prev();
@@ -1261,6 +1275,7 @@ struct A16Plan {
 	int wide_units;
 	int before, places;
 	long long tasks, split_places;   // many rows of sequences: CTAs, places of the split ones' rows
+	int apart;                       // the rows of those that go apart, at most
 };
 constexpr int AR_ROOM = 148 * 3; // CTAs of few rows that run at a time
 constexpr int AW_ROOM = 148;     // and of many
@@ -1308,7 +1323,7 @@ void tasks_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, const Seq
 	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide.through = 1, r.wide_units = 1;
 	// As many tasks as there can be, whatever the counts become: no more tiles than the rows fill and one begun for every sequence.  (A prompt of 8192 tokens among 255 single ones behind 2000 positions 1234 us; with as many
 	// blocks for each as the prompt has tiles 3318.)
-	const long long all = std::min((long long)p.n * r.wide.tiles, (long long)a.q.rows * (a.heads / c.heads) / 256 + p.n) * c.heads, live = a.row_tiles > 0 ? std::min(all, a.row_tiles * c.heads) : all, rest = live % AW_ROOM;
+	const long long all = std::min((long long)p.n * r.wide.tiles, (long long)a.q.rows * (a.heads / c.heads) / 256 + p.n) * c.heads, live = a.row_tiles > 0 ? std::min(all, std::max(0LL, a.row_tiles - (r.apart ? a.few : 0)) * c.heads) : all, rest = live % AW_ROOM;
 	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
 	const long long shares = rest ? std::min<long long>({AW_ROOM / rest, cdiv(longest, 4), AW_SHARES}) : 1;
 	r.wide.shares = (int)std::max(1LL, shares), r.wide.planned = (int)std::min<long long>(live, INT_MAX), r.wide.cut = shares > 1 ? (int)(live - rest) : r.wide.planned;
@@ -1323,7 +1338,7 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	auto seen = [&](long long keys) { return a.window > 0 ? std::min(keys, (long long)a.window + p.longest) : keys; };
 	const long long shared = groups ? seen(s->longest) : 0, own = groups ? seen(s->most_own) : 0, lone = groups ? (s->n_alone ? seen(s->most_alone) : 0) : seen(std::max(a.most_keys, 1));
 	const bool wide = (c.dim == 64 || (c.dim > 64 && c.dim <= 128)) && c.page % 8 == 0 && c.pages > 0 && std::max(rows, packed) <= 65535 * 256LL;
-	// Each way's time, estimated in us from the work that it does; the least.  Of 135 shapes that were measured in all their ways (1 to 8 groups of 3 to 64 sequences of 1 to 100 tokens behind 600 to 12000 positions, 1 to 8 key
+	// Each way's time, estimated in us from the work that it does; the least.  Of 129 shapes that were measured in all their ways (1 to 8 groups of 3 to 64 sequences of 1 to 100 tokens behind 600 to 12000 positions, 1 to 8 key
 	// heads of 64 and 128 channels) the rule takes one that is 1.4 % slower than the best in the mean.  us, few rows / prefixes / tiles: 8 groups of 8 sequences of 4 heads a key head behind up to 3000 positions 33 / 50, 4 groups of 16
 	// behind up to 12000 104 / 79, one of 64 behind 600 25 / 33, behind 3000 37 / 35; 16 sequences of up to 20 tokens behind 600 56 / 43 / 25, behind 12000 253 / 88 / 185; 3 of 60 behind 4000 97 / 47 / 51.
 	double prefix = (double)shared; // what the groups share in the mean
@@ -1337,9 +1352,19 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	const double us_rows = 10. + (tiles_g * (prefix + own * together) + tiles_a * lone) / 20000. + 2. * most / (128. * std::max<double>(1., std::min<double>(AR_SHARES, (double)AR_ROOM / std::max(tiles_g + tiles_a, 1LL))));
 	const double us_tile = (a.softcap > 0.f ? 6. : 2.) / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs (a soft cap: two more special functions a score)
 	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(packed, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
-	const double us_tiles = 24. + us_tile * c.heads * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256)) * (groups ? prefix + own : lone);
+	const double us_row = us_tile * c.heads * (groups ? prefix + own : lone), us_all = 24. + us_row * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256));
+	// Single tokens among prompts are a tile each, of which their rows are a small part: they go apart, in CTAs of few rows beside the tiles' last ones.  us, together / apart, 32 heads over 8 of
+	// 128 channels: a prompt of 8192 among 255 tokens behind 2000 positions 1239 / 924 (602 and 293 by themselves), of 2048 among 63 264 / 158, of 512 among 31 132 / 85, 8 of 600 among 120 480 / 389, 2 of 900 with 20 that share 1500
+	// 157 / 125, one of 500 among 16 behind 20000 391 / 303, one of 300 among 5 42 / 42 (taken together).
+	const double us_apart = us_all - us_row * a.few + cdiv((long long)a.few * c.heads, AR_ROOM) * (4. + std::max(shared + own, lone) / 130.);
+	const bool apart = a.few > 0 && a.row_tiles > a.few && us_apart < us_all;
+	const double us_tiles = apart ? us_apart : us_all;
 	if (wide && rows >= 32 && us_tiles < us_rows && (!groups || us_tiles <= us_prefixes)) {
 		r.way = A16_TILES;
+		if (apart) {
+			r.apart = std::max(8, group), r.rows = r.apart, r.tile = r.apart > 8 ? 16 : 8, r.warps = 4, r.shares = 1, r.units = p.n;
+			r.each = (int)std::min<long long>(std::max(shared + own, lone) / AR_KEYS + 3, INT_MAX / 2);
+		}
 		tasks_plan(r, c, p, a, rows, std::max(shared + own, lone));
 		return r;
 	}
@@ -1380,7 +1405,7 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	if (std::max(p->longest, s && s->n ? s->tokens : 0) * group > INT_MAX - 256) return refuse("attend16: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence or group", std::max(p->longest, s ? s->tokens : 0), (int)group);
 	if ((uintptr_t)a->sinks % 4) return refuse("attend16: sinks are not aligned to 4 bytes");
 	if (!(std::fabs(a->scale) < INFINITY) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY) || (a->softcap > 0.f && !(2.f * A16_LOG2E * std::fabs(a->scale) / a->softcap < INFINITY))) return refuse("attend16: scale, window or softcap out of range");
-	if (a->row_tiles < 0) return refuse("attend16: %lld row tiles", a->row_tiles);
+	if (a->row_tiles < 0 || a->few < 0) return refuse("attend16: %lld row tiles, %d sequences of few rows", a->row_tiles, a->few);
 	return 0;
 }
 
@@ -1456,16 +1481,17 @@ extern "C" int calm_b200_seq_attend16(const struct SeqCache16* cache, const stru
 	a.q = (const uint16_t*)q->q.p, a.q_row = q->q.row_stride, a.q_head = q->q.head_stride, a.out = (uint16_t*)q->out.p, a.o_row = q->out.row_stride, a.o_head = q->out.head_stride;
 	a.rows = q->q.rows, a.heads = q->heads, a.group = q->heads / cache->heads, a.scale = q->scale, a.softcap = q->softcap, a.window = q->window, a.sinks = q->sinks;
 	a.out_vec = ((uintptr_t)a.out | (uintptr_t)(a.o_row * 2) | (uintptr_t)(a.o_head * 2)) % 8 == 0;
-	a.families = plan.way == A16_ROWS, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = plan.before, a.places = plan.places;
+	a.families = plan.way == A16_ROWS ? 1 : -plan.apart / a.group, a.shares = plan.shares, a.each = plan.each, a.cluster = plan.cluster, a.before = plan.before, a.places = plan.places;
 	a.sums = (float*)q->workspace, a.stats = (float2*)(a.sums + a16_rows(*q, plan) * c.dim);
-	const dim3 grid(plan.way == A16_TILES ? 1 : cdiv(plan.rows, plan.tile), cache->heads * std::max(1, plan.shares), plan.units);
+	const dim3 grid(plan.way == A16_TILES && !plan.apart ? 1 : cdiv(plan.rows, plan.tile), cache->heads * std::max(1, plan.shares), plan.units);
 	if (grid.y > 65535) return refuse("attend16: too many key heads");
 	if ((long long)plan.wide.tiles * cache->heads * plan.wide.shares > INT_MAX || plan.tasks > INT_MAX || plan.split_places > INT_MAX) return refuse("attend16: too many rows");
 	const cudaStream_t st = (cudaStream_t)stream;
 	const bool half = cache->type == SEQ_F16;
 	cudaError_t e = cudaSuccess;
 	if (plan.way != A16_ROWS) e = half ? tiles_wide<__half>(*cache, c, a, plan, st) : tiles_wide<bf16>(*cache, c, a, plan, st);
-	if (e == cudaSuccess && plan.way != A16_TILES) e = half ? rows_wide<__half>(plan, c, a, grid, plan.before > 0, st) : rows_wide<bf16>(plan, c, a, grid, plan.before > 0, st);
+	const bool after = plan.before > 0 || plan.apart > 0;
+	if (e == cudaSuccess && (plan.way != A16_TILES || plan.apart)) e = half ? rows_wide<__half>(plan, c, a, grid, after, st) : rows_wide<bf16>(plan, c, a, grid, after, st);
 	if (e == cudaSuccess && plan.split_places)
 		e = launch(st, true, 1, half ? k_c16_join<__half> : k_c16_join<bf16>, dim3(plan.wide.planned - plan.wide.cut, 8), dim3(128), 0, c, a, plan.wide);
 	if (e == cudaSuccess && plan.places > plan.before) {
@@ -1479,5 +1505,5 @@ extern "C" int calm_b200_seq_attend16_way(const struct SeqCache16* cache, const 
 	using namespace seqops;
 	if (const int rc = check_attend16(cache, batch, shared, args)) return rc;
 	const A16Plan p = a16_plan(*cache, *batch, shared, *args);
-	return p.way | (p.way == A16_ROWS && p.cluster ? 4 : 0) | (p.places > p.before || p.split_places ? 8 : 0);
+	return p.way | (p.way == A16_ROWS && p.cluster ? 4 : 0) | (p.places > p.before || p.split_places ? 8 : 0) | (p.apart ? 16 : 0);
 }

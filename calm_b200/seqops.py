@@ -63,7 +63,7 @@ class _Shared(C.Structure):
 
 class _Attend16(C.Structure):
     _fields_ = [("q", _Rows), ("out", _Rows), ("heads", _int), ("scale", C.c_float), ("window", _int), ("softcap", C.c_float), ("sinks", _ptr), ("most_keys", _int), ("row_tiles", _ll),
-                ("workspace", _ptr), ("workspace_bytes", _size)]
+                ("workspace", _ptr), ("workspace_bytes", _size), ("few", _int)]
 
 
 _lib = None
@@ -270,10 +270,15 @@ class Batch:
 
     def _row_tiles(self, group: int) -> int:
         """Tiles of 256 pairs of token and head, `group` heads a token, over all sequences."""
-        n = self._tiles.get(group)
-        if n is None:
-            n = self._tiles[group] = int(-(-(self._counts.astype(np.int64) * group) // 256).sum()) if len(self._counts) else 0
-        return n
+        return self._split(group)[0]
+
+    def _split(self, group: int) -> Tuple[int, int]:
+        """Those tiles, and the sequences with few such pairs."""
+        found = self._tiles.get(group)
+        if found is None:
+            pairs = self._counts.astype(np.int64) * group
+            found = self._tiles[group] = int((-(-pairs // 256)).sum()), int(((pairs > 0) & (pairs <= max(8, group))).sum())
+        return found
 
 
 def _grouped(shared, cn: np.ndarray, at: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
@@ -552,7 +557,8 @@ class Cache16:
             out, ro = _like(q, rq, batch.tokens)
         else:
             ro = _rows("out", out, index, heads, self.dim, rq.rows)
-        a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, batch._row_tiles(heads // self.heads), None, 0)
+        a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, 0, None, 0)
+        a.row_tiles, a.few = batch._split(heads // self.heads)
         if sink is not None:
             _gpu("sink", sink, index)
             if sink.shape != (heads,) or sink.dtype != torch.float32 or not sink.is_contiguous():

@@ -489,11 +489,12 @@ struct SeqAttend16 {
 	long long row_tiles;     /* about the sum over the sequences of ceil(tokens * (heads / cache.heads) / 256) (what the split of the work is planned for); 0: as many as there can be */
 	void* workspace;         /* calm_b200_seq_attend16_workspace bytes, 16-byte aligned; undefined between calls, not to be shared by calls that may overlap */
 	size_t workspace_bytes;
+	int few;                 /* with row_tiles: about the sequences of a token or more with tokens * (heads / cache.heads) <= max(8, heads / cache.heads) (what the split of the work is planned for) */
 };
 size_t calm_b200_seq_attend16_workspace(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args);
 int calm_b200_seq_attend16(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args, void* stream);
 /* how a call would go, for tests: 0 few rows (prefix and own keys in one list), 1 prefixes as tiles of many rows first, 2 every sequence as tiles of many rows; + 4: clusters fold the shares of keys, + 8: another
- * kernel folds them; or -3 */
+ * kernel folds them; 2 + 16: sequences of few rows apart; or -3 */
 int calm_b200_seq_attend16_way(const struct SeqCache16* cache, const struct SeqPortions* batch, const struct SeqShared* shared /* or NULL */, const struct SeqAttend16* args);
 
 #ifdef __cplusplus

@@ -52,7 +52,7 @@ def ref(x):
 
 
 def attend(c=None, p=None, s=None, stream=False, **over):
-    a = made(seqops._Attend16, dict(q=rows(), out=rows(), heads=4, scale=1.0, window=0, softcap=0.0, sinks=None, most_keys=100, row_tiles=0, workspace=None, workspace_bytes=0), over)
+    a = made(seqops._Attend16, dict(q=rows(), out=rows(), heads=4, scale=1.0, window=0, softcap=0.0, sinks=None, most_keys=100, row_tiles=0, workspace=None, workspace_bytes=0, few=0), over)
     return ref(c or cache()), ref(p or portions()), ref(s), ref(a)
 
 
@@ -111,7 +111,7 @@ def test_attend_refusals_and_workspace():
         says(L.calm_b200_seq_attend16(*attend(s=shared(**over)), None), "attend16", word)
     for over, word in ((dict(heads=3), "query heads"), (dict(heads=0), "query heads"), (dict(q=rows(type=4)), "type"), (dict(out=rows(type=2)), "type"), (dict(q=rows(type=0), out=rows(type=0)), "type"),
                        (dict(out=rows(rows=9)), "rows"), (dict(window=-1), "range"), (dict(softcap=-1.0), "range"), (dict(softcap=float("nan")), "range"), (dict(softcap=math.inf), "range"), (dict(scale=float("nan")), "range"),
-                       (dict(q=rows(p=None)), "missing"), (dict(sinks=4098), "aligned"), (dict(row_tiles=-1), "row tiles")):
+                       (dict(q=rows(p=None)), "missing"), (dict(sinks=4098), "aligned"), (dict(row_tiles=-1), "row tiles"), (dict(few=-1), "few rows")):
         says(L.calm_b200_seq_attend16(*attend(**over), None), "attend16", word)
     for longest, heads in ((1 << 30, 72), (2 ** 31 - 1, 4)):
         says(L.calm_b200_seq_attend16(*attend(p=portions(longest=longest), heads=heads), None), "attend16", "pairs")

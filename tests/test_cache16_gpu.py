@@ -338,6 +338,40 @@ def test_one_prompt_among_single_tokens():
         attention([1300, 0, 2], [0, 5, 100], [], 3, 2, 128, 8, "fp16", seed=24)
 
 
+@pytest.mark.parametrize("opt", [dict(), dict(window=150), dict(window=40, softcap=4.0, sinks=True)], ids=lambda o: "-".join(o))
+@pytest.mark.parametrize("dim,kv_heads,group,page,dtype", [(128, 8, 4, 16, "bf16"), (64, 4, 1, 8, "fp16"), (80, 3, 12, 24, "bf16"), (128, 2, 33, 16, "bf16")])
+def test_single_tokens_go_apart_from_prompts(dim, kv_heads, group, page, dtype, opt):
+    """Both kernels at once, with prefixes that single tokens, prompts and both share, and the same after counts have changed between the two kinds."""
+    counts, before = [1] * 30 + [300] + [2] * 3 + [0, 1, 171] + [1] * 5, [300 + 7 * i for i in range(42)]
+    for groups in ([], [(0, 20, 290), (28, 4, 490), (38, 3, 0)]):
+        made = make(counts, before, groups, kv_heads, group, dim, page, DT[dtype], 31)
+        sink = dict(sink=torch.randn(kv_heads * group, generator=gen(5), device="cuda")) if "sinks" in opt else {}
+        more = dict({k: x for k, x in opt.items() if k != "sinks"}, **sink)
+        check_attend(*made, counts, before, groups, **more)
+        cache, table, q, batch, slots = made
+        now = [300, 1] + counts[2:30] + [1] + counts[31:36] + [1] + counts[37:]  # (not more rows than there were)
+        start = np.concatenate([[0], np.cumsum(now)])[:-1]
+        if groups:
+            continue  # (their sequences' pages are not long enough)
+        room = seqops.Batch(slots.tolist(), counts, before)
+        room.data[1].copy_(torch.tensor(now, dtype=torch.int32)), room.data[0].copy_(torch.tensor(start, dtype=torch.int32))
+        check_attend(cache, table, q, room, slots, now, before, groups, got=cache.attend(q, torch.tensor(table, device="cuda"), room, scale=dim ** -0.5, **more), **more)
+
+
+def test_apart_when_the_rule_says_so():
+    import ctypes as C
+
+    for counts, before, groups, apart in (([1] * 63 + [2048], [2000] * 63 + [0], [], True), ([300] * 16, [500] * 16, [], False), ([1] * 20 + [900] * 2, [1500] * 22, [(0, 22, 1500)], True)):
+        batch = seqops.Batch(list(range(len(counts))), counts, before, shared=groups)
+        cache = seqops.Cache16.empty(2, 8, 16, 128)
+        q = torch.empty(batch.tokens, 32, 128, dtype=torch.bfloat16, device="cuda")
+        c, r = cache._with(torch.zeros(len(counts), 300, dtype=torch.int32, device="cuda"), batch), seqops._rows("q", q, 0, 32, 128, batch.tokens)
+        a = seqops._Attend16(r, r, 32, 1.0, 0, 0.0, None, batch.most_keys, 0, None, 0)
+        a.row_tiles, a.few = batch._split(4)
+        way = seqops._load().calm_b200_seq_attend16_way(C.byref(c), C.byref(batch.c), None if batch.shared is None else C.byref(batch.shared), C.byref(a))
+        assert way & 3 == 2 and bool(way & 16) == apart
+
+
 @pytest.mark.parametrize("counts,before,groups", [([1, 1, 2], [300, 310, 305], [(0, 2, 300)]), ([90] * 5, [300] * 5, [(0, 4, 288)]), ([400], [0], [])])
 def test_scales_below_zero(counts, before, groups):
     attention(counts, before, groups, 2, 4, 128, 16, "bf16", seed=25, scale=-0.11)
