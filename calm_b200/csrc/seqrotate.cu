@@ -103,9 +103,11 @@ __global__ void __launch_bounds__(TURN_THREADS) k_turn(const Turn a) {
 	const bool is_v = blockIdx.y >= a.turn.blocks;
 	const TurnPart& part = is_v ? a.copy : a.turn;
 	const int width = min(part.columns, TURN_THREADS), at = threadIdx.x / width, column = threadIdx.x % width + blockIdx.x % a.spread * TURN_THREADS;
-	const int token = blockIdx.x / a.spread * a.tokens + at % a.tokens, side = at / a.tokens;
+	const unsigned index = blockIdx.x / a.spread * a.tokens + at % a.tokens; // (the last block's threads may pass 2^31)
+	const int side = at / a.tokens;
 	const int b = blockIdx.z, n = a.count[b], p0 = a.pos0[b], start = a.start[b];
-	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || token >= n || side >= part.side || column >= part.columns) return;
+	if (n < 1 || p0 < 0 || p0 > INT_MAX - n || start < 0 || n > a.rows - start || index >= (unsigned)n || side >= part.side || column >= part.columns) return;
+	const int token = (int)index;
 	const bool turns = !is_v && column < a.turned;
 	double step[ANGLES];
 	if (turns)
