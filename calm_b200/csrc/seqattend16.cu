@@ -1289,8 +1289,8 @@ int a16_box(int page) { // keys that lie side by side in every page, as a copy's
 // Shares of a tile's keys: folded inside clusters of eight CTAs of eight warps where tiles and keys are few, through memory else.  us, clusters / memory, one sequence of 32 heads over 8 key heads of 128 channels: 1000 keys
 // 9.3 / 9.5, 4000 11.2 / 11.7, 16000 19.3 / 16.9, 60000 53 / 48 (over 2 key heads 9.5 / 9.5, 11.4 / 10.9, 19 / 15, 48 / 22); four beams behind 1000 positions 13.1 / 13.5, 4000 14.3 / 16.1, 16000 25 / 23; twice that, which
 // clusters of eight do not fit side by side, 21.4 / 19.1.  Clusters of 16 (of four warps) 18.1 and 26.5 for the four beams.
-void rows_plan(A16Plan& r, const SeqCache16& c, long long n, long long rows, long long keys, bool clusters) { // n: tiles that have rows
-	n = std::max(1LL, n), r.rows = rows, r.tile = rows > 8 ? 16 : 8, r.warps = 4;
+void rows_plan(A16Plan& r, const SeqCache16& c, long long n, long long rows, long long likely, long long keys, bool clusters) { // n: tiles that have rows; rows: of a unit at most, likely: about
+	n = std::max(1LL, n), r.rows = rows, r.tile = likely > 8 ? 16 : 8, r.warps = 4;
 	const int chunks = (int)std::min<long long>(std::max(keys, 0LL) / AR_KEYS + 2, INT_MAX / 2); // (they begin anywhere)
 	const long long room = AR_ROOM;
 	r.cluster = clusters && c.dim <= 128 && n <= 12 && chunks > 4 && chunks <= 192;
@@ -1304,10 +1304,10 @@ void rows_plan(A16Plan& r, const SeqCache16& c, long long n, long long rows, lon
 	r.each = cdiv(chunks, shares), r.shares = cdiv(chunks, r.each);
 }
 // Groups: as many shares of their prefixes as CTAs run at a time, of one length for all groups (`lengths`: what each of them shared when the batch was described).
-void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long rows, long long most) {
+void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long rows, long long likely, long long most) {
 	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide_units = s.n;
 	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
-	const long long per = (long long)r.wide.tiles * c.heads;
+	const long long per = (long long)cdiv(likely, 256) * c.heads;
 	auto ctas = [&](int each) { // that have keys
 		long long n = 0;
 		for (int g = 0; g < s.n; ++g) n += std::max(1, cdiv(s.lengths ? std::min<long long>(s.lengths[g], most) : most, (long long)each * AW_KEYS));
@@ -1333,7 +1333,8 @@ void tasks_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, const Seq
 A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, const SeqAttend16& a) {
 	A16Plan r = {};
 	const int group = a.heads / c.heads, groups = s ? s->n : 0;
-	const long long rows = (long long)p.longest * group, packed = groups ? (long long)s->tokens * group : 0;
+	// `packed`: rows of a group at most, which the grids have room for; `likely`: about, which times and shares are reckoned from
+	const long long rows = (long long)p.longest * group, packed = groups ? (long long)std::min(s->tokens, a.q.rows) * group : 0, likely = groups && s->likely > 0 ? std::min(packed, (long long)s->likely * group) : packed;
 	// keys that a row sees at most: of a prefix, behind one, of a sequence of no group
 	auto seen = [&](long long keys) { return a.window > 0 ? std::min(keys, (long long)a.window + p.longest) : keys; };
 	const long long shared = groups ? seen(s->longest) : 0, own = groups ? seen(s->most_own) : 0, lone = groups ? (s->n_alone ? seen(s->most_alone) : 0) : seen(std::max(a.most_keys, 1));
@@ -1347,11 +1348,11 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 		for (int g = 0; g < groups; ++g) prefix += std::min<double>(s->lengths[g], (double)shared) / groups;
 	}
 	const int alone = groups ? s->n_alone : p.n;
-	const long long together = groups ? std::min<long long>(cdiv(16, group), std::max(s->tokens, 1)) : 0; // sequences of a CTA's rows at most
-	const long long most = std::max(shared + own * together, lone), units = groups + alone, tiles_g = (long long)groups * cdiv(packed, 16) * c.heads, tiles_a = (long long)alone * cdiv(rows, 16) * c.heads;
+	const long long together = groups ? std::min<long long>(cdiv(16, group), std::max(likely / group, 1LL)) : 0; // sequences of a CTA's rows at most
+	const long long most = std::max(shared + own * together, lone), units = groups + alone, tiles_g = (long long)groups * cdiv(likely, 16) * c.heads, tiles_a = (long long)alone * cdiv(rows, 16) * c.heads;
 	const double us_rows = 10. + (tiles_g * (prefix + own * together) + tiles_a * lone) / 20000. + 2. * most / (128. * std::max<double>(1., std::min<double>(AR_SHARES, (double)AR_ROOM / std::max(tiles_g + tiles_a, 1LL))));
 	const double us_tile = (a.softcap > 0.f ? 6. : 2.) / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs (a soft cap: two more special functions a score)
-	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(packed, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
+	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(likely, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
 	const double us_row = us_tile * c.heads * (groups ? prefix + own : lone), us_all = 24. + us_row * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256));
 	// Single tokens among prompts are a tile each, of which their rows are a small part: they go apart, in CTAs of few rows beside the tiles' last ones.  us, together / apart, 32 heads over 8 of
 	// 128 channels: a prompt of 8192 among 255 tokens behind 2000 positions 1239 / 924 (602 and 293 by themselves), of 2048 among 63 264 / 158, of 512 among 31 132 / 85, 8 of 600 among 120 480 / 389, 2 of 900 with 20 that share 1500
@@ -1370,15 +1371,15 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	}
 	if (wide && packed > 0 && us_prefixes < us_rows) {
 		r.way = A16_PREFIXES;
-		groups_plan(r, c, *s, packed, shared);
+		groups_plan(r, c, *s, packed, likely, shared);
 		r.before = r.wide.shares;
 		r.units = p.n;
-		rows_plan(r, c, (long long)p.n * cdiv(rows, 16) * c.heads, rows, std::max(own, lone), false);
+		rows_plan(r, c, (long long)p.n * cdiv(rows, 16) * c.heads, rows, rows, std::max(own, lone), false);
 		r.places = r.before + (r.shares > 1 ? r.shares : 0);
 		return r;
 	}
 	r.way = A16_ROWS, r.units = (int)units;
-	rows_plan(r, c, tiles_g + tiles_a, std::max(rows, packed), most, true);
+	rows_plan(r, c, tiles_g + tiles_a, std::max(rows, packed), std::max(rows, likely), most, true);
 	r.places = r.shares > 1 && !r.cluster ? r.shares : 0;
 	return r;
 }
@@ -1396,7 +1397,7 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	if (a->heads > 65535) return refuse("attend16: at most 65535 query heads");
 	const long long group = a->heads / c->heads;
 	if (s) {
-		if (s->n < 0 || s->n > p->n || s->longest < 0 || s->tokens < 0 || s->most_own < 0 || s->most_alone < 0) return refuse("attend16: %d groups of %d sequences, longest %d, tokens %d", s->n, p->n, s->longest, s->tokens);
+		if (s->n < 0 || s->n > p->n || s->longest < 0 || s->tokens < 0 || s->likely < 0 || s->most_own < 0 || s->most_alone < 0) return refuse("attend16: %d groups of %d sequences, longest %d, tokens %d", s->n, p->n, s->longest, s->tokens);
 		if (s->n && (!s->first || !s->count || !s->positions || !s->group)) return refuse("attend16: the groups' description is missing");
 		if (s->n_alone < 0 || s->n_alone > p->n || (s->n && s->n_alone && !s->alone)) return refuse("attend16: %d sequences of %d in no group of the groups' description", s->n_alone, p->n);
 		if (((uintptr_t)s->first | (uintptr_t)s->count | (uintptr_t)s->positions | (uintptr_t)s->group | (uintptr_t)s->alone) % 4) return refuse("attend16: the groups' description is not aligned to 4 bytes");

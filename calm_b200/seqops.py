@@ -61,6 +61,11 @@ class _Shared(C.Structure):
                 ("most_alone", _int), ("lengths", _ptr)]
 
 
+class _Groups(C.Structure):
+    """struct SeqShared whole: `likely` lies where _Shared has padding, which is zero."""
+    _fields_ = _Shared._fields_[:6] + [("likely", _int)] + _Shared._fields_[6:]
+
+
 class _Attend16(C.Structure):
     _fields_ = [("q", _Rows), ("out", _Rows), ("heads", _int), ("scale", C.c_float), ("window", _int), ("softcap", C.c_float), ("sinks", _ptr), ("most_keys", _int), ("row_tiles", _ll),
                 ("workspace", _ptr), ("workspace_bytes", _size), ("few", _int)]
@@ -85,7 +90,7 @@ def _load() -> C.CDLL:
         L.calm_b200_seq_rotate.argtypes, L.calm_b200_seq_rotate.restype = [C.POINTER(_Portions), C.POINTER(_Rotation), C.POINTER(_Rows), C.POINTER(_Rows), _int, _int, _ptr], _int
         L.calm_b200_seq_cache16_store.argtypes = [C.POINTER(_Cache16), C.POINTER(_Portions), C.POINTER(_Rows), C.POINTER(_Rows), C.POINTER(_Rotation), C.POINTER(_Rows), C.POINTER(_Rows), _int, _ptr]
         L.calm_b200_seq_cache16_store.restype = _int
-        args = [C.POINTER(_Cache16), C.POINTER(_Portions), C.POINTER(_Shared), C.POINTER(_Attend16)]
+        args = [C.POINTER(_Cache16), C.POINTER(_Portions), _ptr, C.POINTER(_Attend16)]
         L.calm_b200_seq_attend16_workspace.argtypes, L.calm_b200_seq_attend16_workspace.restype = args, _size
         L.calm_b200_seq_attend16.argtypes, L.calm_b200_seq_attend16.restype = args + [_ptr], _int
         L.calm_b200_seq_attend16_way.argtypes, L.calm_b200_seq_attend16_way.restype = args, _int
@@ -232,7 +237,7 @@ class UnitPool:
 
 class Batch:
     """The packed batch of a step: sequence i brings counts[i] new tokens, in order, at positions before[i] .. of slot slots[i].  The device arrays (`data`, int32 rows start,
-    count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest`.
+    count, slot, position) may be written between replays of a captured call, as long as counts stay within `longest` and all rows within those of the call's tensors.
 
     shared: groups of neighbouring sequences that go on from one text, as (first sequence, sequences, positions): a cache holds the positions below that once, on the pages that the
     table names for the group's first sequence, and Cache16.attend reads them once for all of the group.  Of the device array `groups` (int32 rows first, sequences, positions) the positions may be written
@@ -260,13 +265,22 @@ class Batch:
         self._counts, self._tiles = cn, {}
         if len(groups):
             own = at.astype(np.int64) + cn - np.where(of >= 0, groups[of, 2], 0)
-            tokens = max(int(cn[f:f + n].sum()) for f, n, _ in groups.tolist())
+            likely = max(1, max(int(cn[f:f + n].sum()) for f, n, _ in groups.tolist()))
+            self._most_tokens = int(groups[:, 1].max()) * self.longest  # of a group, whatever counts up to `longest` are written
             alone, self._lengths = np.flatnonzero(of < 0).astype(np.int32), np.ascontiguousarray(groups[:, 2])
             both = torch.from_numpy(np.concatenate([groups.T.reshape(-1), of, alone])).to(self.data.device)
             self.groups, self.group_of = both[:groups.size].view(3, -1), both[groups.size:groups.size + len(of)]
             base, step = both.data_ptr(), 4 * len(groups)
-            self.shared = _Shared(len(groups), base, base + step, base + 2 * step, base + 3 * step, len(alone), base + 3 * step + 4 * len(of), int(groups[:, 2].max()), tokens,
-                                  int(own[of >= 0].max()), int(own[of < 0].max(initial=0)), self._lengths.ctypes.data)
+            self.shared = _Groups(len(groups), base, base + step, base + 2 * step, base + 3 * step, len(alone), likely, base + 3 * step + 4 * len(of), int(groups[:, 2].max()),
+                                  min(self._most_tokens, self.tokens), int(own[of >= 0].max()), int(own[of < 0].max(initial=0)), self._lengths.ctypes.data)
+
+    def _shared_by(self, rows: int) -> Optional[_Groups]:
+        """The groups' description for `rows` rows of queries: a group's counts may grow as far as `longest` and the rows allow."""
+        if self.shared is None or min(self._most_tokens, rows) == self.shared.tokens:
+            return self.shared
+        more = _Groups.from_buffer_copy(self.shared)
+        more.tokens = min(self._most_tokens, rows)
+        return more
 
     def _row_tiles(self, group: int) -> int:
         """Tiles of 256 pairs of token and head, `group` heads a token, over all sequences."""
@@ -564,7 +578,9 @@ class Cache16:
             if sink.shape != (heads,) or sink.dtype != torch.float32 or not sink.is_contiguous():
                 raise ValueError(f"sink must be contiguous float32 [{heads}]")
             a.sinks = sink.data_ptr()
-        L, shared = _load(), None if batch.shared is None else C.byref(batch.shared)
+        L, shared = _load(), batch._shared_by(rq.rows)
+        if shared is not None:
+            shared = C.byref(shared)
         need = L.calm_b200_seq_attend16_workspace(C.byref(c), C.byref(batch.c), shared, C.byref(a))
         if need:
             work = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -466,9 +466,10 @@ struct SeqShared {
 	const int *first, *count, *positions; /* device [n] */
 	const int* group;                     /* device [sequences]: the group that a sequence is in, -1: none */
 	int n_alone;
+	int likely;                           /* about the new tokens of the largest group (what the split of the work is planned for); 0: tokens */
 	const int* alone;                     /* device [n_alone]: the sequences that are in none */
 	int longest;                          /* at least the largest of positions */
-	int tokens;                           /* at least the new tokens of any group */
+	int tokens;                           /* at least the new tokens of any group, whatever counts are written before a replay */
 	int most_own, most_alone;             /* about the most keys of a group's sequence behind what it shares, of a sequence of no group (what the split of the work is planned for; more are still seen) */
 	const int* lengths;                   /* HOST [n] or NULL: about what each group shares (what the split of the work is planned for) */
 };

@@ -1,5 +1,6 @@
 """Rotary positions, the paged cache in 16 bits and attention over shared prefixes at the edges of what their calls allow: the longest sequences, batches that change between replays, values and
 scores at the ends of their types' ranges."""
+import ctypes as C
 import math
 import os
 import sys
@@ -10,7 +11,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import cache16_plain as plain  # noqa: E402
-from test_cache16_gpu import as64, gen, near  # noqa: E402
+from test_cache16_gpu import as64, check_attend, gen, make, near  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +28,40 @@ def test_a_sequence_of_as_many_tokens_as_an_int_holds():
     want, tol = plain.rotate(np.broadcast_to(as64(k), (32, 1, 48)), pos, rot.frequencies, rot.gain, rot.pairs)
     near(torch.cat([cache.k[2, 0], cache.k[0, 0]])[:, None], want, tol, torch.float16)
     assert torch.equal(cache.v[[2, 0], 0], v.expand(2, 16, 48)) and (cache.k[[1, 3]] == 0).all() and (cache.v[[1, 3]] == 0).all()
+
+
+# ---------------------------------------------------------------- attention
+
+def way_of(cache, table, q, batch, **opt):
+    """The way that Cache16.attend's call takes, as it describes the call (calm_b200_seq_attend16_way)."""
+    c, rows = cache._with(torch.tensor(table, device="cuda"), batch), seqops._rows("q", q, 0, q.shape[1], cache.dim, batch.tokens)
+    a = seqops._Attend16(rows, rows, q.shape[1], opt.get("scale", cache.dim ** -0.5), opt.get("window", 0), opt.get("softcap", 0.0), None, batch.most_keys, 0, None, 0)
+    a.row_tiles, a.few = batch._split(q.shape[1] // cache.heads)
+    shared = batch._shared_by(rows.rows)
+    return seqops._load().calm_b200_seq_attend16_way(C.byref(c), C.byref(batch.c), None if shared is None else C.byref(shared), C.byref(a))
+
+
+@pytest.mark.parametrize("way,kv_heads,page,counts,now,before,groups", [
+    (4, 2, 16, [5, 1, 1, 1, 5], [5, 5, 1, 1, 1], [600, 610, 620, 605, 30], [(0, 2, 600), (2, 2, 590)]),                     # shares folded by clusters; as many rows as there were
+    (4, 2, 16, [4, 1, 1], [4, 4, 4], [900, 903, 901], [(0, 3, 900)]),                                                      # more rows, which q has
+    (8, 8, 16, [5, 1, 1, 1] * 4, [5, 5, 5, 1] * 4, [2600 + 7 * i for i in range(16)], [(4 * i, 4, 2600) for i in range(4)]),  # folded through memory
+    (0, 16, 12, [6, 1, 1, 1] * 12, [6] * 48, [100 + 7 * i for i in range(48)], [(4 * i, 4, 96) for i in range(12)]),         # not split
+    (1, 8, 16, [6] + [1] * 31 + [2], [6] * 32 + [1], [5000 + i for i in range(32)] + [900], [(0, 32, 5000)]),                 # the prefix as tiles of all of a group's rows: more tiles
+    (9, 4, 16, [6] + [1] * 31 + [2], [6] * 32 + [1], [5000 + 40 * i for i in range(32)] + [900], [(0, 32, 5000)]),            # own keys folded
+])
+def test_groups_whose_counts_grow_between_replays(way, kv_heads, page, counts, now, before, groups):
+    """Counts up to the longest one that was described, written after the call was captured: no row of a group is lost."""
+    cache, table, q, _, slots = make(now, before, groups, kv_heads, 4, 64, page, torch.bfloat16, 41)
+    batch, dev, out = seqops.Batch(slots.tolist(), counts, before, shared=groups), torch.tensor(table, device="cuda"), torch.empty_like(q)
+    assert way_of(cache, table, q, batch) == way
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cache.attend(q, dev, batch, scale=0.125, out=out)
+    for c in (now, counts):
+        batch.data[0].copy_(torch.tensor(np.concatenate([[0], np.cumsum(c)])[:-1], dtype=torch.int32))
+        batch.data[1].copy_(torch.tensor(c, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        check_attend(cache, table, q, batch, slots, c, before, groups, got=out, scale=0.125)
+        assert (out[sum(c):] == 7.0).all()
