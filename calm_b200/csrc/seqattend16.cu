@@ -115,18 +115,20 @@ __device__ __forceinline__ void odd2(uint32_t x, uint32_t& sum) {
 		sum = *reinterpret_cast<const uint32_t*>(&r);
 	}
 }
-// The halves that are finite, the others as zero; `inf`: +-1 for each infinity, `nan`: 1 for each that is no number (zero else)
+// The halves that are finite, the others as zero; `up`: 1 for each +infinity, `down`: 1 for each -infinity, both for each that is no number (zero else)
 template <typename T>
-__device__ __forceinline__ uint32_t split2(uint32_t x, uint32_t& inf, uint32_t& nan) {
+__device__ __forceinline__ uint32_t split2(uint32_t x, uint32_t& up, uint32_t& down) {
 	constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00, M = 0x7fff ^ E, ONE = std::is_same<T, bf16>::value ? 0x3f80 : 0x3c00;
 	uint32_t y = 0;
-	inf = nan = 0;
+	up = down = 0;
 #pragma unroll
 	for (int s = 0; s < 32; s += 16) {
 		const uint32_t h = x >> s & 0xffff;
 		if ((h & E) != E) y |= h << s;
-		else if (h & M) nan |= ONE << s;
-		else inf |= (ONE | (h & 0x8000)) << s;
+		else {
+			if (h & M || !(h & 0x8000)) up |= ONE << s;
+			if (h & M || h & 0x8000) down |= ONE << s;
+		}
 	}
 	return y;
 }
@@ -528,18 +530,17 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 #pragma unroll
 			for (int x = 0; x < 2 * MT; ++x) {
 				if (16 * (x % MT) >= dim) continue;
-				uint32_t V[4], inf[4], nan[4];
+				uint32_t V[4], up[4], down[4];
 				values(x, V);
 #pragma unroll
-				for (int e = 0; e < 4; ++e) V[e] = split2<T>(V[e], inf[e], nan[e]);
+				for (int e = 0; e < 4; ++e) V[e] = split2<T>(V[e], up[e], down[e]);
 #pragma unroll
 				for (int q = 0; q < NQ; ++q) {
-					float s_inf[4] = {0.f, 0.f, 0.f, 0.f}, s_nan[4] = {0.f, 0.f, 0.f, 0.f};
-					mma_16<T>(s_inf, inf, p[x / MT][q]), mma_16<T>(s_nan, nan, p[x / MT][q]), mma_16<T>(acc[x % MT][q], V, p[x / MT][q]);
+					float s_up[4] = {0.f, 0.f, 0.f, 0.f}, s_down[4] = {0.f, 0.f, 0.f, 0.f};
+					mma_16<T>(s_up, up, p[x / MT][q]), mma_16<T>(s_down, down, p[x / MT][q]), mma_16<T>(acc[x % MT][q], V, p[x / MT][q]);
 #pragma unroll
-					for (int e = 0; e < 4; ++e)
-						if (s_nan[e] != 0.f) acc[x % MT][q][e] = NAN;
-						else if (s_inf[e] != 0.f) acc[x % MT][q][e] += s_inf[e] * INFINITY;
+					for (int e = 0; e < 4; ++e) // (both: infinity less infinity)
+						if (s_up[e] > 0.f || s_down[e] > 0.f) acc[x % MT][q][e] += s_up[e] > 0.f ? s_down[e] > 0.f ? NAN : INFINITY : -INFINITY;
 				}
 			}
 		}

@@ -65,3 +65,25 @@ def test_groups_whose_counts_grow_between_replays(way, kv_heads, page, counts, n
         graph.replay()
         check_attend(cache, table, q, batch, slots, c, before, groups, got=out, scale=0.125)
         assert (out[sum(c):] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 4), (128, 9), (256, 2)])
+def test_opposite_infinities_are_no_number(dim, group, dtype):
+    """Infinities of both signs in one channel of keys that some row sees only in part: NaN for the rows that see both, an infinity for those that see one, wherever the others' masks fall."""
+    counts, before, groups = [1, 3, 1], [100, 100, 20], [(0, 2, 96)]
+    cache, table, q, batch, slots = make(counts, before, groups, 1, group, dim, 16, dtype, 51)
+
+    def at(seq, pos):
+        s = slots[0] if seq < 2 and pos < 96 else slots[seq]
+        return int(table[s, pos // 16]), 0, pos % 16
+
+    cache.k[at(1, 100)] = cache.k[at(1, 99)]  # one key twice: one weight
+    cache.v[at(1, 99)][3], cache.v[at(1, 100)][3] = math.inf, -math.inf
+    cache.v[at(1, 98)][5], cache.v[at(1, 102)][5] = -math.inf, math.inf  # the last token sees both
+    cache.v[at(2, 18)][7], cache.v[at(2, 19)][7], cache.v[at(2, 17)][8] = math.inf, -math.inf, -math.inf
+    cache.v[at(2, 3)][9], cache.v[at(2, 4)][9] = math.nan, math.inf
+    assert way_of(cache, table, q, batch) & 3 == 0
+    got = check_attend(cache, table, q, batch, slots, counts, before, groups)
+    assert got[1:4, :, 3].isnan().all() and (got[1:3, :, 5] == -math.inf).all() and got[3, :, 5].isnan().all()
+    assert got[4, :, 7].isnan().all() and (got[4, :, 8] == -math.inf).all() and got[4, :, 9].isnan().all() and got[0].isfinite().all()
