@@ -176,11 +176,43 @@ __device__ __forceinline__ void add_places(float4& v, const float* p, size_t str
 		}
 	}
 }
-// cap tanh(s) of x = -2 log2(e) s: (1 - t) / (1 + t) with t = 2^-|x|, two units of the special functions.  Off by 2^-21 cap at most: t by 2 steps (2^-22 of it), its difference from 1 by as much, the quotient's
-// reciprocal by 2^-23 and two roundings.
-__device__ __forceinline__ float capped(float x, float cap) {
-	const float t = ex2(-fabsf(x));
-	return copysignf(cap * __fdividef(1.f - t, 1.f + t), -x);
+// Soft caps: cap tanh(s / cap), off by 10 2^-24 of the score at most, whatever the cap.  For |u| = |s / cap| <= 1 it is s times the fifth convergent of tanh(u) / u = 1 / (1 + u^2 / (3 + u^2 / (5 + ...))), Lambert's
+// continued fraction, (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4): off by 2^-24, with the roundings of two quotients' parts, a reciprocal and three products.  Else cap (1 - t) / (1 + t) with t = e^(-2 |u|), where 1 - t
+// is 0.86 or more.  (That form alone is off by 2^-21 of the cap: at a cap of 10^6 no score is left.)
+struct Cap {
+	float by, most; // u of a product of query and key; the cap for exponents of 2
+};
+__device__ __forceinline__ Cap cap_of(const Attend& a) { // (u is 0 where scores are, and an infinity where they are)
+	return {a.scale == 0.f ? 0.f : copysignf(fmaxf(fabsf(a.scale / a.softcap), 1.4e-45f), a.scale), fminf(a.softcap * A16_LOG2E, 3.40282347e38f)};
+}
+__device__ __forceinline__ float over(float x, float y) { // x / y for 1 <= y <= 2
+	float r;
+	asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+	return x * r;
+}
+// N products of query and key as capped exponents of 2; a warp reckons both forms where one of its scores is past the cap (a prompt of 8192 tokens, 32 heads over 8 of 128 channels: 1256 us, 1528 where all warps do, 608
+// without a cap; a division in each form 1320 and 3407).
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&z)[N], const Cap& cap, float qscale) {
+	float top = 0.f;
+#pragma unroll
+	for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(z[i]));
+	auto form = [&](float x, bool far) {
+		const float u = x * cap.by, w = u * u;
+		float num = x * qscale * fmaf(w, fmaf(w, 1.f / 945.f, 1.f / 9.f), 1.f), den = fmaf(w, fmaf(w, 1.f / 63.f, 4.f / 9.f), 1.f);
+		if (far) {
+			const float t = ex2(-2.f * A16_LOG2E * fabsf(u));
+			num = fabsf(u) > 1.f ? copysignf(fmaf(-cap.most, t, cap.most), u) : num, den = fabsf(u) > 1.f ? 1.f + t : den;
+		}
+		return over(num, den);
+	};
+	if (__any_sync(0xffffffffu, top * fabsf(cap.by) > 1.f)) {
+#pragma unroll
+		for (int i = 0; i < N; ++i) z[i] = form(z[i], true);
+	} else {
+#pragma unroll
+		for (int i = 0; i < N; ++i) z[i] = form(z[i], false);
+	}
 }
 // chunks of the keys lo .. hi - 1, the first of which begins at a multiple of a chunk
 __device__ __forceinline__ int chunks_of(int lo, int hi) { return hi > lo ? (hi - lo / AR_KEYS * AR_KEYS + AR_KEYS - 1) / AR_KEYS : 0; }
@@ -427,13 +459,7 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 		__syncwarp(); // every lane has its keys
 		request_keys();
 		if (a.softcap > 0.f) {
-			const float cap = a.softcap * A16_LOG2E, by = -2.f * A16_LOG2E * a.scale / a.softcap;
-#pragma unroll
-			for (int i = 0; i < 2; ++i)
-#pragma unroll
-				for (int q = 0; q < NQ; ++q)
-#pragma unroll
-					for (int e = 0; e < 4; ++e) z[i][q][e] = capped(z[i][q][e] * by, cap);
+			cap_scores(reinterpret_cast<float(&)[8 * NQ]>(z), cap_of(a), qscale);
 		} else {
 #pragma unroll
 			for (int i = 0; i < 2; ++i)
@@ -899,7 +925,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		const int group = warp >> 2;
 		const int r = two ? tid & 127 : tid, rpos = s.row_pos[r], rlow = low_of(a, rpos), wide = low_of(a, most);
 		const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), scores_at = lanes + 128 * group, sums_at = lanes + O_COL + 128 * group;
-		const float qscale = a.softcap > 0.f ? -2.f * A16_LOG2E * a.scale / a.softcap : a.scale * A16_LOG2E;
+		const float qscale = a.scale * A16_LOG2E;
 		float m = -INFINITY, l = 0.f;
 		if (group < groups || two) {
 			int n = 0; // tiles of this group's
@@ -933,7 +959,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					}
 				}
 				if (moves) { // 32 columns at a time, in few instructions: most often a block's first and last tiles
-					const float most_z = m == -INFINITY ? -INFINITY : A16_MOST, cap = a.softcap * A16_LOG2E;
+					const float most_z = m == -INFINITY ? -INFINITY : A16_MOST;
 					const int from = min(max(rlow - pos0, 0), 128), to = min(max(rpos + 1 - pos0, 0), 128); // of this row: keys from .. to - 1
 					float top = -INFINITY;
 #pragma unroll 1
@@ -943,8 +969,9 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 						const int f = min(max(from - 32 * x, 0), 32), t = min(max(to - 32 * x, 0), 32);
 						const uint32_t see = s.seen[i % AW_MASKS][x] & (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
 						if (a.softcap > 0.f) {
+							cap_scores(y, cap_of(a), qscale);
 #pragma unroll
-							for (int k = 0; k < 32; ++k) y[k] = capped(y[k] * qscale, cap) - ref;
+							for (int k = 0; k < 32; ++k) y[k] -= ref;
 						} else {
 #pragma unroll
 							for (int k = 0; k < 32; ++k) y[k] = fmaf(y[k], qscale, -ref);
@@ -1352,7 +1379,7 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	const long long together = groups ? std::min<long long>(cdiv(16, group), std::max(likely / group, 1LL)) : 0; // sequences of a CTA's rows at most
 	const long long most = std::max(shared + own * together, lone), units = groups + alone, tiles_g = (long long)groups * cdiv(likely, 16) * c.heads, tiles_a = (long long)alone * cdiv(rows, 16) * c.heads;
 	const double us_rows = 10. + (tiles_g * (prefix + own * together) + tiles_a * lone) / 20000. + 2. * most / (128. * std::max<double>(1., std::min<double>(AR_SHARES, (double)AR_ROOM / std::max(tiles_g + tiles_a, 1LL))));
-	const double us_tile = (a.softcap > 0.f ? 6. : 2.) / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs (a soft cap: two more special functions a score)
+	const double us_tile = (a.softcap > 0.f ? 6. : 2.) / AW_ROOM / AW_KEYS; // a key of 256 rows, on one of the SMs (a soft cap: a reciprocal and eight products and sums more a score, and every tile takes the slower way)
 	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(likely, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
 	const double us_row = us_tile * c.heads * (groups ? prefix + own : lone), us_all = 24. + us_row * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256));
 	// Single tokens among prompts are a tile each, of which their rows are a small part: they go apart, in CTAs of few rows beside the tiles' last ones.  us, together / apart, 32 heads over 8 of

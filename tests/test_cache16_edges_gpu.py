@@ -87,3 +87,49 @@ def test_opposite_infinities_are_no_number(dim, group, dtype):
     got = check_attend(cache, table, q, batch, slots, counts, before, groups)
     assert got[1:4, :, 3].isnan().all() and (got[1:3, :, 5] == -math.inf).all() and got[3, :, 5].isnan().all()
     assert got[4, :, 7].isnan().all() and (got[4, :, 8] == -math.inf).all() and got[4, :, 9].isnan().all() and got[0].isfinite().all()
+
+
+def capped_attention(q, k, v, p0, scale, softcap, half):
+    """One sequence's rows q [n][heads][dim] at positions p0 .. over k, v [positions][kv heads][dim] in 64 bits, and what the kernels' arithmetic may be off by before the last rounding.
+
+    Bound: as plain.attend's, but for the cap, which may change a score s by 12 2^-24 of |s|: a rational form of u = s / cap within 2^-24, its numerator and denominator within 1.5 2^-24 each, a
+    reciprocal within 2 2^-24, three products within 2^-24 each, u itself within 3 2^-24, of which no more than as much reaches the score."""
+    n, heads, dim = q.shape
+    group, keys = heads // k.shape[1], p0 + n
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    seen = np.arange(keys)[None] <= p0 + np.arange(n)[:, None]
+    for h in range(heads):
+        x, kk, vv = q[:, h], k[:keys, h // group], v[:keys, h // group]
+        s = x @ kk.T * scale
+        mag, big = np.abs(x) @ np.abs(kk).T * abs(scale), np.abs(kk).max(1)[None] * np.abs(x).max(1)[:, None] * abs(scale)
+        ds = ((dim / 16 + 6) * mag + dim / 16 * 17 * big) * 2.0 ** -23
+        s = softcap * np.tanh(s / softcap)
+        s = np.where(seen, s, -math.inf)
+        m = s.max(1, keepdims=True)
+        ds = np.where(seen, ds + 12 * plain.F32 * np.abs(s) + 6 * plain.F32 * (np.abs(s - m) + np.abs(s)) + 2.0 ** -21, 0.0)
+        p = np.where(seen, np.exp(s - m), 0.0)
+        p /= p.sum(1, keepdims=True)
+        o, adds = p @ vv, (keys / 16 + 200) * 2.0 ** -23
+        ds = np.where(seen, ds, 0.0)
+        cut = keys / 16 * 17 * 2.0 ** -23 * p.max(1)[:, None] * np.abs(vv).max(0)
+        out[:, h] = o
+        tol[:, h] = (p * ds) @ np.abs(vv) + (p * ds).sum(1)[:, None] * np.abs(o) + (half + adds) * (p @ np.abs(vv)) + adds * np.abs(o) + cut + 2.0 ** -35 * seen @ np.abs(vv)
+    return out, tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("softcap", [0.5, 30.0, 1e4, 1e6, 1e8, 1e20, 3e38])
+@pytest.mark.parametrize("way,dim,kv,group,counts,before", [(4, 128, 2, 3, [2], [700]), (0, 64, 8, 3, [1, 4, 1], [400, 333, 90]), (2, 128, 8, 4, [300], [200]), (2, 64, 8, 4, [500, 530], [0, 70])])
+def test_soft_caps_of_any_size(way, dim, kv, group, counts, before, softcap, dtype):
+    """Scores of a deviation of 3, some far past a small cap: a large cap leaves them as they are."""
+    cache, table, q, batch, slots = make(counts, before, [], kv, group, dim, 16, dtype, 61)
+    q *= 3.0 / 1.3
+    assert way_of(cache, table, q, batch, softcap=softcap) & ~8 == way
+    got = cache.attend(q, torch.tensor(table, device="cuda"), batch, scale=dim ** -0.5, softcap=softcap)
+    at = 0
+    for i, (n, b) in enumerate(zip(counts, before)):
+        ids = table[slots[i], :-(-(n + b) // 16)]
+        k, v = (as64(x)[ids].transpose(0, 2, 1, 3).reshape(-1, kv, dim) for x in (cache.k, cache.v))
+        want, tol = capped_attention(as64(q)[at:at + n], k, v, b, dim ** -0.5, softcap, torch.finfo(dtype).eps / 2)
+        near(got[at:at + n], want, tol, dtype)
+        at += n
