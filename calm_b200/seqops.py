@@ -413,7 +413,7 @@ class Rotation:
       {"kind": "base", "factor"}                            the base times factor^(dims / (dims - 2))
       {"kind": "wavelength", "factor", "length", "low", "high"}  w = length f / 2 pi: f / factor below `low`, f above `high`, a blend linear in w between
       {"kind": "ramp", "factor", "length", "fast", "slow"}  the same by the pair's number, between the pairs that turn `fast` and `slow` times in `length` positions; cosines and sines
-                                                            times 0.1 ln(factor) + 1 (or "gain")
+                                                            times 0.1 ln(factor) + 1, 1 for factors below 1 (or "gain")
     frequencies: f itself, float64 [dims / 2], in place of base and scaling."""
 
     def __init__(self, dims: int, base: float = 10000.0, pairs: str = "halves", scaling: Optional[dict] = None, frequencies=None, device=None):
@@ -466,7 +466,7 @@ def rotation_frequencies(dims: int, base: float = 10000.0, scaling: Optional[dic
         lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
         blend = np.clip((i - lo) / max(hi - lo, 0.001), 0.0, 1.0)
         f = f / s["factor"] * blend + f * (1.0 - blend)
-        gain = 0.1 * math.log(s["factor"]) + 1.0 if gain is None else gain
+        gain = 0.1 * math.log(max(s["factor"], 1.0)) + 1.0 if gain is None else gain
     return f, 1.0 if gain is None else float(gain)
 
 
