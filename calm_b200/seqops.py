@@ -427,24 +427,55 @@ class Rotation:
         elif scaling is not None:
             raise ValueError("frequencies that are given are not scaled")
         else:
-            self.frequencies, self.gain = np.array(frequencies, np.float64), 1.0
+            try:
+                self.frequencies, self.gain = np.array(frequencies, np.float64), 1.0
+            except (TypeError, ValueError, OverflowError):
+                raise ValueError(f"frequencies must be {dims // 2} finite numbers") from None
             if self.frequencies.shape != (dims // 2,) or not np.isfinite(self.frequencies).all():
                 raise ValueError(f"frequencies must be {dims // 2} finite numbers")
+        if abs(self.gain) > np.finfo(np.float32).max:
+            raise ValueError(f"gain = {self.gain} passes float32")
         self.dims, self.pairs = dims, pairs
         self.turns = torch.from_numpy(self.frequencies / (2.0 * math.pi)).to(torch.device("cuda") if device is None else device)
         self.index = _gpu("the rotation", self.turns)
         self.c = _Rotation(self.turns.data_ptr(), dims, int(pairs == "neighbours"), self.gain)
 
 
+def _real(name: str, value) -> float:
+    """A finite number as a float."""
+    try:
+        v = math.nan if isinstance(value, (str, bytes)) else float(value)
+    except (TypeError, ValueError, OverflowError):
+        v = math.nan
+    if not math.isfinite(v):
+        raise ValueError(f"{name} must be a finite number, not {value!r}")
+    return v
+
+
 def rotation_frequencies(dims: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[np.ndarray, float]:
     """Step of every pair of a Rotation (float64 [dims / 2]) and the factor on cosines and sines."""
+    wants = {"none": set(), "linear": {"factor"}, "base": {"factor"}, "wavelength": {"factor", "length", "low", "high"}, "ramp": {"factor", "length", "fast", "slow"}}
+    if scaling is not None and not isinstance(scaling, dict):
+        raise ValueError(f"scaling must be a dict, not {scaling!r}")
     s = dict(scaling) if scaling else {"kind": "none"}
     kind, gain, given = s.pop("kind", None), s.pop("gain", None), set(s)
-    wants = {"none": set(), "linear": {"factor"}, "base": {"factor"}, "wavelength": {"factor", "length", "low", "high"}, "ramp": {"factor", "length", "fast", "slow"}}
-    if kind not in wants or given != wants[kind]:
+    if not isinstance(kind, str) or kind not in wants or given != wants[kind]:
         raise ValueError(f"scaling {scaling!r}: one of " + ", ".join(f"{k} ({', '.join(sorted(w))})" for k, w in wants.items() if w))
-    if not (base > 0 and math.isfinite(base)) or not all(v > 0 and math.isfinite(v) for v in s.values()):
+    base, s = _real("base", base), {k: _real(k, v) for k, v in s.items()}
+    gain = None if gain is None else _real("gain", gain)
+    if not (base > 0 and all(v > 0 for v in s.values())):
         raise ValueError(f"base {base}, scaling {scaling!r}: positive numbers")
+    try:
+        with np.errstate(over="ignore", invalid="ignore", divide="ignore"):
+            f, gain = _stretched(dims, base, kind, s, gain)
+    except (OverflowError, ZeroDivisionError):
+        f = np.full(1, math.inf)
+    if not np.isfinite(f).all():
+        raise ValueError(f"base {base}, scaling {scaling!r}: frequencies that no number holds")
+    return f, 1.0 if gain is None else gain
+
+
+def _stretched(dims: int, base: float, kind: str, s: dict, gain: Optional[float]) -> Tuple[np.ndarray, Optional[float]]:
     if kind == "base":
         if dims < 4:
             raise ValueError("one pair of channels has no base to stretch")
@@ -462,12 +493,14 @@ def rotation_frequencies(dims: int, base: float = 10000.0, scaling: Optional[dic
     elif kind == "ramp":
         if base == 1.0:
             raise ValueError("a base of 1 has no ramp")
+        if s["fast"] < s["slow"]:
+            raise ValueError("fast must not be under slow")
         at = [dims * math.log(s["length"] / (2.0 * math.pi * t)) / (2.0 * math.log(base)) for t in (s["fast"], s["slow"])]
         lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
         blend = np.clip((i - lo) / max(hi - lo, 0.001), 0.0, 1.0)
         f = f / s["factor"] * blend + f * (1.0 - blend)
         gain = 0.1 * math.log(max(s["factor"], 1.0)) + 1.0 if gain is None else gain
-    return f, 1.0 if gain is None else float(gain)
+    return f, gain
 
 
 def _beside(rotation: Rotation, batch: Batch, index: int) -> None:
