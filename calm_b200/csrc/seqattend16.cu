@@ -1433,7 +1433,7 @@ int check_attend16(const SeqCache16* c, const SeqPortions* p, const SeqShared* s
 	}
 	if (std::max(p->longest, s && s->n ? s->tokens : 0) * group > INT_MAX - 256) return refuse("attend16: %d tokens of %d query heads a key head: at most 2^31 pairs a sequence or group", std::max(p->longest, s ? s->tokens : 0), (int)group);
 	if ((uintptr_t)a->sinks % 4) return refuse("attend16: sinks are not aligned to 4 bytes");
-	if (!(std::fabs(a->scale) < INFINITY) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY) || (a->softcap > 0.f && !(2.f * A16_LOG2E * std::fabs(a->scale) / a->softcap < INFINITY))) return refuse("attend16: scale, window or softcap out of range");
+	if (!(A16_LOG2E * std::fabs(a->scale) < INFINITY) || a->window < 0 || !(a->softcap >= 0.f && a->softcap < INFINITY) || (a->softcap > 0.f && !(2.f * A16_LOG2E * std::fabs(a->scale) / a->softcap < INFINITY))) return refuse("attend16: scale, window or softcap out of range");
 	if (a->row_tiles < 0 || a->few < 0) return refuse("attend16: %lld row tiles, %d sequences of few rows", a->row_tiles, a->few);
 	return 0;
 }

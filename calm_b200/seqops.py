@@ -433,7 +433,7 @@ class Rotation:
                 raise ValueError(f"frequencies must be {dims // 2} finite numbers") from None
             if self.frequencies.shape != (dims // 2,) or not np.isfinite(self.frequencies).all():
                 raise ValueError(f"frequencies must be {dims // 2} finite numbers")
-        if abs(self.gain) > np.finfo(np.float32).max:
+        if abs(self.gain) > float(np.finfo(np.float32).max):
             raise ValueError(f"gain = {self.gain} passes float32")
         self.dims, self.pairs = dims, pairs
         self.turns = torch.from_numpy(self.frequencies / (2.0 * math.pi)).to(torch.device("cuda") if device is None else device)
@@ -546,6 +546,8 @@ class Cache16:
         self.k, self.v, self.dtype = k, v, k.dtype
         self.pages, self.heads, self.page, self.dim = k.shape
         self._pool = (k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], self.pages, self.heads, self.page, self.dim)
+        if not self.heads or not self.page:
+            raise ValueError(f"a cache of {self.heads} heads, {self.page} tokens a page")
         if self.dim % 16 or not 16 <= self.dim <= 256:
             raise ValueError(f"rows of {self.dim} channels: a multiple of 16 up to 256 is served")
 
@@ -604,7 +606,10 @@ class Cache16:
             out, ro = _like(q, rq, batch.tokens)
         else:
             ro = _rows("out", out, index, heads, self.dim, rq.rows)
+        scale, softcap = _real("scale", scale), _real("softcap", softcap)
         a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, 0, None, 0)
+        if softcap and not a.softcap:
+            raise ValueError(f"softcap = {softcap} is out of float32's range")
         a.row_tiles, a.few = batch._split(heads // self.heads)
         if sink is not None:
             _gpu("sink", sink, index)

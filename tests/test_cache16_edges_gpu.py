@@ -133,3 +133,15 @@ def test_soft_caps_of_any_size(way, dim, kv, group, counts, before, softcap, dty
         want, tol = capped_attention(as64(q)[at:at + n], k, v, b, dim ** -0.5, softcap, torch.finfo(dtype).eps / 2)
         near(got[at:at + n], want, tol, dtype)
         at += n
+
+
+def test_numbers_and_caches_that_mean_nothing_are_refused():
+    cache, table, q, batch, _ = make([1, 1], [50, 50], [(0, 2, 48)], 2, 2, 64, 16, torch.float16, 4)
+    dev = torch.tensor(table, device="cuda")
+    for kw in (dict(scale="1"), dict(scale=None), dict(scale=math.nan), dict(scale=-math.inf), dict(scale=10 ** 400), dict(scale=3e38), dict(scale=1.0, softcap=1e-50), dict(scale=1.0, softcap="2"), dict(scale=1.0, softcap=1e39)):
+        with pytest.raises(ValueError, match="scale|softcap|range"):
+            cache.attend(q, dev, batch, **kw)
+    assert torch.equal(cache.attend(q, dev, batch, scale=np.float32(0.125), softcap=np.float64(2.0)), cache.attend(q, dev, batch, scale=0.125, softcap=2))
+    for shape in ((2, 0, 16, 64), (2, 2, 0, 64)):
+        with pytest.raises(ValueError, match="a cache of"):
+            seqops.Cache16.empty(*shape)
