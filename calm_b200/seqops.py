@@ -514,6 +514,9 @@ def _like(x: torch.Tensor, rows: _Rows, tokens: int) -> Tuple[torch.Tensor, _Row
     """Where rows like x's go, which are described: what is behind the batch's tokens is zero."""
     out = torch.empty_like(x) if rows.rows == tokens else torch.zeros_like(x)
     stride = out.stride()
+    if stride[2] != 1:  # (like rows that overlap)
+        out = out.contiguous()
+        stride = out.stride()
     return out, _Rows(out.data_ptr(), rows.type, stride[0], stride[1], rows.rows)
 
 

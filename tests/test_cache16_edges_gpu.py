@@ -145,3 +145,18 @@ def test_numbers_and_caches_that_mean_nothing_are_refused():
     for shape in ((2, 0, 16, 64), (2, 2, 0, 64)):
         with pytest.raises(ValueError, match="a cache of"):
             seqops.Cache16.empty(*shape)
+
+
+@pytest.mark.parametrize("strides", [(2, 1, 1), (1, 1, 1), (0, 1, 1), (0, 64, 1), (64, 0, 1)])
+@pytest.mark.parametrize("rows", [3, 5])
+def test_rows_that_overlap(strides, rows):
+    """Windows on one line of numbers, rows that stand for many: results are tensors of their own."""
+    line = torch.randn(2000, generator=gen(71), device="cuda").half()
+    x, batch, rot = line.as_strided((rows, 2, 64), strides), seqops.Batch([0], [3], [5]), seqops.Rotation(64)
+    apart = x.clone(memory_format=torch.contiguous_format)
+    assert torch.equal(seqops.rotate(x, batch, rot), seqops.rotate(apart, batch, rot))
+    caches = [seqops.Cache16(*(torch.randn(2, 1, 16, 64, generator=gen(i), device="cuda").half() for i in (1, 2))) for _ in range(2)]
+    table = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    turned = [c.store(y[:, :1], y[:, 1:], table, batch, rotation=rot, q=y) for c, y in zip(caches, (x, apart))]
+    assert torch.equal(*turned) and torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+    assert torch.equal(*(c.attend(y, table, batch, scale=0.125) for c, y in zip(caches, (x, apart))))
