@@ -520,6 +520,15 @@ def _like(x: torch.Tensor, rows: _Rows, tokens: int) -> Tuple[torch.Tensor, _Row
     return out, _Rows(out.data_ptr(), rows.type, stride[0], stride[1], rows.rows)
 
 
+def _into(name: str, t: torch.Tensor, index: int, heads: int, dim: int, least: int) -> _Rows:
+    """Rows that are written: none lies on another."""
+    r = _rows(name, t, index, heads, dim, least)
+    steps = [s for s, n in ((r.row_stride, r.rows), (r.head_stride, heads)) if n > 1]
+    if (steps and min(steps) < dim) or (len(steps) == 2 and steps[0] == steps[1]):
+        raise ValueError(f"{name} has rows that overlap (strides {list(t.stride())})")
+    return r
+
+
 def rotate(x: torch.Tensor, batch: Batch, rotation: Rotation, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The batch's rows x [tokens, heads, dim] (float32, bfloat16 or float16; dim even) turned by their positions.  `out`: where they go, x itself or a tensor apart from it; rows behind the
     batch's tokens stay as they are in it (zero without one)."""
@@ -532,7 +541,7 @@ def rotate(x: torch.Tensor, batch: Batch, rotation: Rotation, out: Optional[torc
     if out is None:
         out, ro = _like(x, rx, batch.tokens)
     else:
-        ro = _rows("out", out, index, heads, dim, rx.rows)
+        ro = _into("out", out, index, heads, dim, rx.rows)
     _run(index, _load().calm_b200_seq_rotate, C.byref(batch.c), C.byref(rotation.c), C.byref(rx), C.byref(ro), heads, dim)
     return out
 
@@ -589,7 +598,7 @@ class Cache16:
             if q_out is None:
                 q_out, ro = _like(q, rq, n)
             else:
-                ro = _rows("q_out", q_out, index, heads, self.dim, rq.rows)
+                ro = _into("q_out", q_out, index, heads, self.dim, rq.rows)
         elif q_out is not None:
             raise ValueError("q_out without q")
         _run(index, _load().calm_b200_seq_cache16_store, C.byref(c), C.byref(batch.c), C.byref(rk), C.byref(rv), turn, rq if rq is None else C.byref(rq), ro if ro is None else C.byref(ro), heads)
@@ -608,7 +617,7 @@ class Cache16:
         if out is None:
             out, ro = _like(q, rq, batch.tokens)
         else:
-            ro = _rows("out", out, index, heads, self.dim, rq.rows)
+            ro = _into("out", out, index, heads, self.dim, rq.rows)
         scale, softcap = _real("scale", scale), _real("softcap", softcap)
         a = _Attend16(rq, ro, heads, scale, _whole("window", window), softcap, None, batch.most_keys, 0, None, 0)
         if softcap and not a.softcap:

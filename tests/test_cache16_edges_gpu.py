@@ -160,3 +160,20 @@ def test_rows_that_overlap(strides, rows):
     turned = [c.store(y[:, :1], y[:, 1:], table, batch, rotation=rot, q=y) for c, y in zip(caches, (x, apart))]
     assert torch.equal(*turned) and torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
     assert torch.equal(*(c.attend(y, table, batch, scale=0.125) for c, y in zip(caches, (x, apart))))
+
+
+def test_results_whose_rows_overlap_are_refused():
+    line, batch, rot = torch.zeros(4000, device="cuda").half(), seqops.Batch([0], [3], [5]), seqops.Rotation(64)
+    cache, table = seqops.Cache16.empty(2, 1, 16, 64, torch.float16), torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 2, 64, generator=gen(5), device="cuda").half()
+    for strides in ((2, 1, 1), (0, 64, 1), (64, 0, 1), (64, 64, 1), (63, 256, 1), (256, 63, 1)):
+        out = line.as_strided((3, 2, 64), strides)
+        for call in (lambda: seqops.rotate(q, batch, rot, out=out), lambda: cache.store(q[:, :1], q[:, 1:], table, batch, rotation=rot, q=q, q_out=out), lambda: cache.attend(q, table, batch, scale=1.0, out=out)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    assert (line == 0).all()
+    for strides in ((128, 64, 1), (64, 192, 1), (70, 500, 1), (700, 64, 1)):
+        out = line.as_strided((3, 2, 64), strides)
+        assert torch.equal(seqops.rotate(q, batch, rot, out=out), seqops.rotate(q, batch, rot))
+    one, single = line.as_strided((1, 1, 64), (0, 0, 1)), seqops.Batch([0], [1], [5])
+    assert torch.equal(seqops.rotate(q[:1, :1], single, rot, out=one), seqops.rotate(q[:1, :1], single, rot))
