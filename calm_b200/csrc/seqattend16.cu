@@ -469,17 +469,18 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 					for (int e = 0; e < 4; ++e) z[i][q][e] *= qscale;
 		}
 		const bool all = seen == 0xffffffffu && (seg == 0 || segs == 2) && pos >= wide && pos + AR_KEYS - 1 <= least;
-		if (!all) { // some row does not see some key; this thread's keys are 8 j + g
+		auto sees_key = [&](int j, int q, int e) { // this thread's keys are 8 j + g
+			const int kp = pos + 8 * j + g;
+			return (seen >> (8 * j + g) & 1) && kp <= rpos[q][e] && kp >= low_of(a, rpos[q][e]) && (seg == 0 || seg == rseg[q][e]);
+		};
+		if (!all) { // some row does not see some key
 #pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				const int kp = pos + 8 * j + g;
-				const bool some = seen >> (8 * j + g) & 1;
+			for (int j = 0; j < 4; ++j)
 #pragma unroll
 				for (int q = 0; q < NQ; ++q)
 #pragma unroll
 					for (int e = 0; e < 2; ++e)
-						if (!(some && kp <= rpos[q][e] && kp >= low_of(a, rpos[q][e]) && (seg == 0 || seg == rseg[q][e]))) z[j >> 1][q][(j & 1) * 2 + e] = -INFINITY;
-			}
+						if (!sees_key(j, q, e)) z[j >> 1][q][(j & 1) * 2 + e] = -INFINITY;
 		}
 		bool move = false;
 #pragma unroll
@@ -554,19 +555,28 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 			}
 		} else {
 #pragma unroll
-			for (int x = 0; x < 2 * MT; ++x) {
-				if (16 * (x % MT) >= dim) continue;
-				uint32_t V[4], up[4], down[4];
-				values(x, V);
-#pragma unroll
-				for (int e = 0; e < 4; ++e) V[e] = split2<T>(V[e], up[e], down[e]);
+			for (int i = 0; i < 2; ++i) {
+				uint2 sees[NQ]; // 1 for each key that a row sees, even if its weight rounds to nothing
 #pragma unroll
 				for (int q = 0; q < NQ; ++q) {
-					float s_up[4] = {0.f, 0.f, 0.f, 0.f}, s_down[4] = {0.f, 0.f, 0.f, 0.f};
-					mma_16<T>(s_up, up, p[x / MT][q]), mma_16<T>(s_down, down, p[x / MT][q]), mma_16<T>(acc[x % MT][q], V, p[x / MT][q]);
+					auto two = [&](int j) { return transposed(pack2<T>(sees_key(j, q, 0) ? 1.f : 0.f, sees_key(j, q, 1) ? 1.f : 0.f)); };
+					sees[q] = make_uint2(two(2 * i), two(2 * i + 1));
+				}
 #pragma unroll
-					for (int e = 0; e < 4; ++e) // (both: infinity less infinity)
-						if (s_up[e] > 0.f || s_down[e] > 0.f) acc[x % MT][q][e] += s_up[e] > 0.f ? s_down[e] > 0.f ? NAN : INFINITY : -INFINITY;
+				for (int x = 0; x < MT; ++x) {
+					if (16 * x >= dim) continue;
+					uint32_t V[4], up[4], down[4];
+					values(i * MT + x, V);
+#pragma unroll
+					for (int e = 0; e < 4; ++e) V[e] = split2<T>(V[e], up[e], down[e]);
+#pragma unroll
+					for (int q = 0; q < NQ; ++q) {
+						float s_up[4] = {0.f, 0.f, 0.f, 0.f}, s_down[4] = {0.f, 0.f, 0.f, 0.f};
+						mma_16<T>(s_up, up, sees[q]), mma_16<T>(s_down, down, sees[q]), mma_16<T>(acc[x][q], V, p[i][q]);
+#pragma unroll
+						for (int e = 0; e < 4; ++e) // (both: infinity less infinity)
+							if (s_up[e] > 0.f || s_down[e] > 0.f) acc[x][q][e] += s_up[e] > 0.f ? s_down[e] > 0.f ? NAN : INFINITY : -INFINITY;
+					}
 				}
 			}
 		}

@@ -177,3 +177,17 @@ def test_results_whose_rows_overlap_are_refused():
         assert torch.equal(seqops.rotate(q, batch, rot, out=out), seqops.rotate(q, batch, rot))
     one, single = line.as_strided((1, 1, 64), (0, 0, 1)), seqops.Batch([0], [1], [5])
     assert torch.equal(seqops.rotate(q[:1, :1], single, rot, out=one), seqops.rotate(q[:1, :1], single, rot))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 12), (256, 2)])
+def test_infinities_of_little_weight_are_infinities(dim, group, dtype):
+    """Keys whose softmax weight is far under what 16 bits hold, in a chunk that not every row sees whole."""
+    counts, before = [1, 2], [90, 75]
+    cache, table, q, batch, slots = make(counts, before, [], 1, group, dim, 16, dtype, 81)
+    q[:] = q[:, :1].abs()  # rows alike
+    at = int(table[slots[1], 70 // 16]), 0, 70 % 16
+    cache.k[at] = -60.0 * dim ** 0.5 / dim  # scores of about -60
+    cache.v[at][2], cache.v[at][4] = math.inf, -math.inf
+    got = check_attend(cache, table, q, batch, slots, counts, before, [])
+    assert (got[1:, :, 2] == math.inf).all() and (got[1:, :, 4] == -math.inf).all() and got[0].isfinite().all() and got[1:, :, 5:].isfinite().all()
