@@ -716,6 +716,9 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 // tensor memory, form the weights and write them back where the scores stood, the next product's operand.  While one group's weights are formed the other's products run; up to 128 rows are taken by both groups, every other tile
 // each, and their sums are added at the end.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.  Tiles that some row sees in part go through a slower way of 32 columns at a time in few
 // instructions.  Results leave through shared memory, a row a copy.
+// Where some row does not see some key of a tile its weight is 0, and 0 times a value that is not finite would be no number: the warp that copies values looks at such tiles and takes those values out, and the rows that see their
+// keys add them to their results at the end (add_odd; reached by values that are not finite alone).  Looking costs 1 % where every other tile is one (a prompt of 2048 of 64 channels 81.3 -> 81.9 us, with 128 none: it is done
+// two tiles ahead).
 // Bound: a tile's way through its roles.  256 rows and 128 keys of 128 channels take about 3700 cycles: the products 2048 by the tensor cores' rate (about 2560 as they are, 80 cycles for 64), softmax 1680 to 1800 for a group and
 // 110 of hand-over.  16 sequences of up to 300 tokens behind 12000 positions, 32 heads over 8: 722 us where the products alone would be 378 (0.44 of the tensor pipes, 0.47 of the special functions'); its loads alone took 570 us
 // from pages of 16 keys, 459 of 32, 416 of 64, 795 of 8.  Tried: tiles of 64 keys with scores ahead 1330 us (N = 64 costs what N = 128 does), weights handed over in halves 905 to 1134, a polynomial for part of the exponentials
@@ -723,6 +726,12 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
 constexpr int AW_SOFTMAX_REGS = 176, AW_OTHER_REGS = 144; // 256 x 176 + 128 x 144 = 63488 of the 384 x 168 = 64512 that the block is launched with
 
+struct AwOdd { // where values that are not finite were taken out: the block's tiles of keys, for the rows that see such values
+	int found;
+	C16 c;
+	int kvh, box, lo[2], hi[2], base[2], slot[2], first, begin, tiles; // first: tiles of the prefix
+	int wide, least; // every row sees the keys wide .. least
+};
 template <int D>
 struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the row
 	static constexpr int PANELS = D / 64, SLOTS = D == 128 ? 5 : 9;
@@ -735,6 +744,7 @@ struct AwShared { // tiles of rows of 128 bytes, 16-byte pieces swizzled by the 
 	int found[3], sums[AW_THREADS / 32]; // the task
 	uint32_t tmem;
 	int lost;
+	AwOdd odd;
 };
 // shared -> global, 16-byte aligned, a multiple of 16 bytes
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
@@ -826,6 +836,63 @@ __device__ __forceinline__ bool task_of(const C16& c, const Attend& a, int t, in
 	return r.z >= 0;
 }
 
+// A tile of values: zeros for those of keys that are not there (`word`: keys 32 lane .. that are, for the first four lanes) and for what is not finite.  True: there was some of that.  A warp.
+template <typename T, int PANELS>
+__device__ __forceinline__ bool clear_values(unsigned char* tile, bool there, uint32_t word) {
+	const int lane = threadIdx.x & 31;
+	if (!there) {
+		for (int k = 0; k < AW_KEYS; ++k)
+			if (!(__shfl_sync(0xffffffffu, word, k >> 5) >> (k & 31) & 1) && lane < 8 * PANELS) *reinterpret_cast<uint4*>(tile + (lane >> 3) * AW_KEYS * 128 + k * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+		__syncwarp();
+	}
+	uint4* const all = reinterpret_cast<uint4*>(tile) + lane;
+	uint32_t sum = 0;
+#pragma unroll 8
+	for (int e = 0; e < AW_KEYS * 8 * PANELS; e += 32) {
+		const uint4 x = all[e];
+		odd2<T>(x.x, sum), odd2<T>(x.y, sum), odd2<T>(x.z, sum), odd2<T>(x.w, sum);
+	}
+	const bool found = __any_sync(0xffffffffu, sum & 0x7fff7fff);
+	if (found)
+		for (int e = 0; e < AW_KEYS * 8 * PANELS; e += 32) {
+			uint32_t up, down;
+			const uint4 x = all[e];
+			all[e] = make_uint4(split2<T>(x.x, up, down), split2<T>(x.y, up, down), split2<T>(x.z, up, down), split2<T>(x.w, up, down));
+		}
+	return found;
+}
+// What the keys from .. to hold that is not finite, in the tiles whose values were looked at, added to a row of results (32-bit sums or the cache's type).
+template <typename T>
+__device__ __noinline__ void add_odd(const AwOdd& o, int from, int to, int dim, void* row, bool sums) {
+	auto page_of = [&](int part, int pos) {
+		const int at = o.c.page_index(pos);
+		return pos >= o.lo[part] && pos < o.hi[part] && at < o.c.table_pages ? __ldg(o.c.table + (size_t)o.slot[part] * o.c.table_pages + at) : -1;
+	};
+	for (int i = 0; i < o.tiles; ++i) {
+		const int at = o.begin + i, part = at >= o.first, pos0 = o.base[part] + (at - (part ? o.first : 0)) * AW_KEYS;
+		bool looked = pos0 < o.wide || pos0 + AW_KEYS - 1 > o.least || pos0 < o.lo[part] || pos0 + AW_KEYS > o.hi[part];
+		for (int k = 0; k < AW_KEYS && !looked; k += o.box) looked = (unsigned)page_of(part, pos0 + k) >= (unsigned)o.c.pages;
+		if (!looked) continue;
+		for (int pos = max(pos0, from); pos <= min(pos0 + AW_KEYS - 1, to); ++pos) {
+			const int id = page_of(part, pos);
+			if ((unsigned)id >= (unsigned)o.c.pages) continue;
+			const T* const v = reinterpret_cast<const T*>(o.c.v) + (((long long)id * o.c.heads + o.kvh) * o.c.page + o.c.page_row(pos)) * dim;
+			for (int d = 0; d < dim; d += 8) {
+				const uint4 w = *reinterpret_cast<const uint4*>(v + d);
+				uint32_t odd = 0;
+				odd2<T>(w.x, odd), odd2<T>(w.y, odd), odd2<T>(w.z, odd), odd2<T>(w.w, odd);
+				if (!(odd & 0x7fff7fff)) continue;
+				for (int k = d; k < d + 8; ++k) {
+					const float x = as_f32(v[k]);
+					if (fabsf(x) < INFINITY) continue;
+					if (sums) static_cast<float*>(row)[k] += x;
+					else static_cast<T*>(row)[k] = from_f32<T>(as_f32(static_cast<T*>(row)[k]) + x);
+				}
+			}
+		}
+	}
+}
+
 // CAP: soft caps, which all tiles take the slower way for.  (One kernel for both: 731 us for 719 without a cap, 16 sequences of up to 300 tokens behind 12000.)
 template <typename T, int D, bool CAP>
 __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const C16 c, const Attend a, const Wide w) {
@@ -860,7 +927,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		for (int i = 0; i < AW_MASKS; ++i) mbar_init(s.mask_full + i, 1);
 		for (int g = 0; g < 2; ++g) mbar_init(s.s_full + g, 1), mbar_init(s.p_full + g, 4), mbar_init(s.done + g, 1);
 		mbar_init(&s.fix, 1), mbar_init(&s.idle, 1);
-		s.lost = 0, s.span[0] = INT_MAX, s.span[1] = -1;
+		s.lost = 0, s.odd.found = 0, s.span[0] = INT_MAX, s.span[1] = -1;
 		mbar_init_fence();
 	}
 	if (tid < 256) s.row_pos[tid] = -1;
@@ -882,8 +949,10 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	};
 	const int low = pos0 + row0 / a.group, high = pos0 + (row0 + rows - 1) / a.group; // of one sequence's rows
 	__syncthreads();
+	// (the values' copies look at what some row does not see)
+	const int waiting = alone ? 0 : ranged ? AW_THREADS - 32 : AW_THREADS;
 	if (warp == 8 || warp == 11) {
-		if (!ranged) asm volatile("bar.sync 2, %0;" ::"n"(AW_THREADS) : "memory");
+		if (waiting && (warp == 11 || !ranged)) asm volatile("bar.sync 2, %0;" ::"r"(waiting) : "memory");
 		range(ranged ? low : s.span[0], ranged ? high : s.span[1]);
 	} else {
 		for (int b = u.first + (warp < 8 ? tid : tid - 32); b <= u.last; b += AW_THREADS - 64) {
@@ -926,7 +995,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 		tc_fence_before();
 		asm volatile("bar.sync 1, %0;" ::"n"(AW_THREADS - 64) : "memory");
 		tc_fence_after();
-		if (!ranged) asm volatile("bar.sync 2, %0;" ::"n"(AW_THREADS) : "memory");
+		if (waiting) asm volatile("bar.sync 2, %0;" ::"r"(waiting) : "memory");
 		range(ranged ? low : s.span[0], ranged ? high : s.span[1]);
 	}
 	const uint32_t tmem = s.tmem;
@@ -1032,7 +1101,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			const bool writes = r < rows && rpos >= 0 && !(two && group);
 			const size_t place = w.through ? (size_t)max(place0, 0) + r : ((size_t)token * a.heads + head) * a.places + share;
 			float* const row = reinterpret_cast<float*>(s.kv) + tid * (D + 4);
-			asm volatile("bar.sync 3, 256;" ::: "memory"); // (both groups' products have ended)
+			asm volatile("bar.sync 4, 288;" ::: "memory"); // (both groups' products have ended, and what the values' copies found is there)
 			float f0 = 1.f, f1 = 0.f; // of this group's sums and the other's
 			const float* const other = reinterpret_cast<const float*>(s.kv) + (tid ^ 128) * (D + 4);
 			if (two) {
@@ -1094,6 +1163,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					}
 				}
 			}
+			if (s.odd.found && writes && !nothing)
+				add_odd<T>(s.odd, low_of(a, rpos), rpos, c.dim, partial || vec ? static_cast<void*>(row) : a.out + token * a.o_row + head * a.o_head, partial);
 			fence_async_smem();
 			if (writes && !nothing && (partial || vec)) {
 				if (partial) bulk_store(a.sums + place * c.dim, row, c.dim * 4);
@@ -1122,6 +1193,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			};
 			uint32_t fixes = 0;
 			int issued = 0; // tiles asked for
+			const int seen_by_all = alone ? low : s.span[0], wide = low_of(a, alone ? high : s.span[1]); // (of the values' warp)
 			if (tiles > 0) look(0);
 			for (int i = 0; i < tiles; ++i) {
 				int part;
@@ -1139,7 +1211,8 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					word &= (t >= 32 ? 0xffffffffu : (1u << t) - 1) & ~(f >= 32 ? 0xffffffffu : (1u << f) - 1);
 					if (!values) s.seen[i % AW_MASKS][lane] = word;
 				}
-				const bool whole = !values || __all_sync(0xffffffffu, lane >= 4 || word == 0xffffffffu);
+				// Values go through this warp where a key is not there or some row does not see some key: 0 times what is not finite would be no number.
+				const bool there = __all_sync(0xffffffffu, lane >= 4 || word == 0xffffffffu), whole = !values || (there && pos0 >= wide && pos0 + AW_KEYS - 1 <= seen_by_all);
 				__syncwarp();
 				if (!values && lane == 0) mbar_arrive(s.mask_full + i % AW_MASKS);
 				const int k = 2 * i + values, sl = k % SLOTS;
@@ -1155,11 +1228,16 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					}
 				}
 				++issued;
-				if (!whole) { // values of keys that are not there are zeros, whatever lies there
+				if (!whole) { // values of keys that are not there are zeros, whatever lies there, and so are values that are not finite: rows that see them get them at the end
 					if (!ap_wait_warp(&s.fix, fixes & 1, &s.lost)) break;
 					++fixes;
-					for (int k = 0; k < AW_KEYS; ++k)
-						if (!(__shfl_sync(0xffffffffu, word, k >> 5) >> (k & 31) & 1) && lane < 8 * PANELS) *reinterpret_cast<uint4*>(s.kv[sl][lane >> 3] + k * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+					if (clear_values<T, PANELS>(s.kv[sl][0], there, word)) {
+						if (lane == 0) {
+							AwOdd& o = s.odd;
+							o.found = 1, o.c = c, o.kvh = kvh, o.box = w.box, o.slot[0] = lead_slot, o.slot[1] = own_slot, o.first = count[0], o.begin = begin, o.tiles = tiles, o.wide = wide, o.least = seen_by_all;
+							o.lo[0] = lo[0], o.lo[1] = lo[1], o.hi[0] = hi[0], o.hi[1] = hi[1], o.base[0] = base[0], o.base[1] = base[1];
+						}
+					}
 					fence_async_smem();
 					__syncwarp();
 					if (lane == 0) mbar_arrive(s.full + sl);
@@ -1170,6 +1248,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					const int k = 2 * i + values;
 					mbar_wait_warp(s.full + k % SLOTS, k / SLOTS & 1, 1u << 12);
 				}
+			if (values) asm volatile("bar.arrive 4, 288;" ::: "memory");
 		} else if (warp == 9 && lane == 0) { // the products: the groups take turns
 			constexpr uint32_t type = std::is_same<T, bf16>::value ? (1u << 7) | (1u << 10) : 0;
 			constexpr uint32_t score = (1u << 4) | type | ((uint32_t)(AW_KEYS >> 3) << 17) | (8u << 24), value = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24); // 128 rows; values: columns side by side

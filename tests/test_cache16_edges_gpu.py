@@ -191,3 +191,49 @@ def test_infinities_of_little_weight_are_infinities(dim, group, dtype):
     cache.v[at][2], cache.v[at][4] = math.inf, -math.inf
     got = check_attend(cache, table, q, batch, slots, counts, before, [])
     assert (got[1:, :, 2] == math.inf).all() and (got[1:, :, 4] == -math.inf).all() and got[0].isfinite().all() and got[1:, :, 5:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("way,counts,before,groups,kv_heads,group,dim,page,opt", [
+    (2, [600], [0], [], 8, 4, 128, 16, {}),                                                             # a prompt
+    (10, [700, 100], [40, 300], [], 4, 4, 64, 16, {}),                                                  # tasks cut by their keys
+    (10, [900], [700], [], 2, 4, 80, 24, dict(window=150)),
+    (2, [300], [200], [], 8, 4, 128, 16, dict(window=90)),
+    (2, [30] * 40, [100] * 40, [], 8, 4, 128, 8, {}),                                                   # up to 128 rows: two groups of warps on every other tile
+    (18, [1] * 63 + [600], [500] * 63 + [0], [], 8, 4, 128, 16, dict(softcap=30.0)),                    # single tokens apart
+    (10, [300, 1, 170, 90], [1500] * 4, [(0, 4, 1500)], 2, 4, 128, 16, dict(window=1000)),              # tasks over a shared prefix
+    (9, [1] * 48, [6000 + 5 * i for i in range(48)], [(0, 48, 6000)], 8, 4, 128, 16, dict(window=5000)),  # the prefix as tiles of a group's rows, which see different parts of it
+    (9, [3] * 24, [6000 + 9 * i for i in range(24)], [(0, 24, 6000)], 8, 2, 64, 16, dict(window=5500)),
+])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(way, counts, before, groups, kv_heads, group, dim, page, opt, dtype):
+    """Of tokens and sequences whose rows share a tile of 128 rows or more, those that do not see a key have nothing of its value."""
+    made = make(counts, before, groups, kv_heads, group, dim, page, dtype, 91)
+    cache, table, q, batch, slots = made
+    assert way_of(cache, table, q, batch, **opt) == way
+    rng, shared = np.random.default_rng(5), {f: p for f, _, p in groups}
+    for i, (n, b) in enumerate(zip(counts, before)):  # the first rows' windows' edges, the new tokens themselves
+        own = b + rng.integers(0, n, 3)
+        edge = b - opt["window"] + rng.integers(2, 40, 3) if "window" in opt else own
+        for j, pos in enumerate((own[0], own[1], edge[0], edge[1])):
+            if pos < 0 or (i % 5 and n < 20):
+                continue
+            at = int(table[slots[i], pos // page]), j % kv_heads, int(pos % page)
+            cache.v[at][(3 * j + i) % dim] = (math.nan, math.inf, -math.inf, math.nan)[(i + j) % 4]
+    if "window" in opt:  # a prefix's values, which some rows' windows have left behind
+        for f, p in shared.items():
+            for j, pos in enumerate(before[f] - opt["window"] + np.array([3, 9, 30, 61, 62])):
+                cache.v[int(table[slots[f], pos // page]), j % kv_heads, int(pos % page)][5 * j] = (math.inf, math.nan, -math.inf)[j % 3]
+    got = check_attend(*made, counts, before, groups, **opt)
+    assert 0 < (~got.isfinite()).sum() < got.numel() // 8
+
+
+def test_values_that_are_not_finite_beside_pages_that_are_not_there():
+    counts, before = [500, 300], [100, 0]
+    made = make(counts, before, [], 8, 4, 64, 8, torch.bfloat16, 92)
+    cache, table, q, batch, slots = made
+    table[slots[0], 3], table[slots[0], 40], table[slots[1], 0] = -1, 10 ** 6, -1
+    for pos, x in ((9, math.nan), (17, math.inf), (333, -math.inf), (560, math.nan)):
+        cache.v[int(table[slots[0], pos // 8]), 2, pos % 8, pos % 64] = x
+    assert way_of(cache, table, q, batch) & 3 == 2
+    got = check_attend(*made, counts, before, [])
+    assert got[:, 4:8].isfinite().all() and got[500:].isfinite().all() and (got[500:508] == 0).all()
