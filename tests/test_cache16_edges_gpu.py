@@ -237,3 +237,29 @@ def test_values_that_are_not_finite_beside_pages_that_are_not_there():
     assert way_of(cache, table, q, batch) & 3 == 2
     got = check_attend(*made, counts, before, [])
     assert got[:, 4:8].isfinite().all() and got[500:].isfinite().all() and (got[500:508] == 0).all()
+
+
+@pytest.mark.parametrize("opt", [dict(), dict(window=150), dict(window=40, softcap=4.0)], ids=lambda o: "-".join(o))
+@pytest.mark.parametrize("dim,kv_heads,group,page", [(128, 4, 4, 16), (64, 4, 1, 8), (80, 2, 12, 24), (128, 2, 33, 16)])
+def test_single_tokens_beside_prompts(dim, kv_heads, group, page, opt):
+    """Every layout really goes apart (units of one CTA and of several), and still does what it should after counts and positions have changed, between the two kinds too."""
+    counts = [1] * 100 + [130] + [2] * 3 + [0, 1, 90] + [1] * 5
+    before = [100 + 7 * (i % 30) for i in range(len(counts))]
+    now = counts[:10] + [130, 2, 0] + counts[13:100] + [1] + counts[101:106] + [2] + counts[107:]  # (not more rows than there were)
+    assert sum(now) <= sum(counts)
+    later = [b + 45 for b in before]
+    for groups in ([], [(0, 90, 90), (98, 4, 100)]):
+        most = [max(a, b) for a, b in zip(counts, now)]
+        cache, table, full, _, slots = make(most, later, groups, kv_heads, group, dim, page, torch.bfloat16, 31)
+        q = full[:sum(counts)]
+        batch, dev = seqops.Batch(slots.tolist(), counts, before, shared=groups), torch.tensor(table, device="cuda")
+        assert way_of(cache, table, q, batch, **opt) & 19 == 18
+        out = torch.empty_like(q)
+        for c, at in ((counts, before), (now, later)):
+            batch.data[0].copy_(torch.tensor(np.concatenate([[0], np.cumsum(c)])[:-1], dtype=torch.int32))
+            batch.data[1].copy_(torch.tensor(c, dtype=torch.int32))
+            batch.data[3].copy_(torch.tensor(at, dtype=torch.int32))
+            out.fill_(7.0)
+            cache.attend(q, dev, batch, scale=dim ** -0.5, out=out, **opt)
+            check_attend(cache, table, q, batch, slots, c, at, groups, got=out, **opt)
+            assert (out[sum(c):] == 7.0).all()
