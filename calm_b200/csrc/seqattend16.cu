@@ -51,8 +51,8 @@ constexpr float A16_MOST = 15.f, A16_SET = 10.f;
 // prefix, which all rows see, then those of each sequence of its rows, which only that sequence's rows see, in chunks of 32.  So a prefix is read once for 8 NQ rows, and a call of few rows needs one launch.
 // Each warp walks chunks of its own with references and sums of its own (no barrier between warps until the end), fed by a ring of asynchronous copies, into m16n8k16 products whose 16 rows are keys (scores: keys x queries) or
 // channels (values: channels x queries), so that eight rows of queries fill one.
-// Bound: memory where keys are many - 32 sequences of up to 6000 keys, 8 key heads of 128 channels (500 MB) 87 us, 5.8 TB/s with the fold - and the way of a chunk (copy, products, softmax, products) where they are few: 4 sequences
-// behind 4000 shared ones 13.7 us, 64 CTAs. Masked or capped scores cost instructions: 18 sequences of 5 tokens, window 2048, cap and sinks 36 us at 0.4 of the issue slots.
+// Bound: memory where keys are many - 32 sequences of up to 6000 keys, 8 key heads of 128 channels (500 MB) 86 us, 5.8 TB/s with the fold - and the way of a chunk (copy, products, softmax, products) where they are few: 4 sequences
+// behind 4000 shared ones 13.2 us, 64 CTAs. Masked or capped scores cost instructions: 18 sequences of 5 tokens, window 2048, cap and sinks 37 us at 0.4 of the issue slots.
 constexpr int AR_KEYS = 32; // (of a warp's chunk)
 constexpr int AR_SHARES = 64;                // of a tile's keys at most
 constexpr int AR_TILE = 16, AR_CLUSTER = 8; // rows of a CTA at most; shares that a thread-block cluster folds
@@ -190,7 +190,7 @@ __device__ __forceinline__ float over(float x, float y) { // x / y for 1 <= y <=
 	asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
 	return x * r;
 }
-// N products of query and key as capped exponents of 2; a warp reckons both forms where one of its scores is past the cap (a prompt of 8192 tokens, 32 heads over 8 of 128 channels: 1256 us, 1528 where all warps do, 608
+// N products of query and key as capped exponents of 2; a warp reckons both forms where one of its scores is past the cap (a prompt of 8192 tokens, 32 heads over 8 of 128 channels: 1181 us, 1461 where all warps do, 597
 // without a cap; a division in each form 1320 and 3407).
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&z)[N], const Cap& cap, float qscale) {
@@ -717,12 +717,12 @@ __global__ void __launch_bounds__(32 * W, W > 4 || D > 128 ? 1 : 3) k_c16_rows(c
 // each, and their sums are added at the end.  O stays in tensor memory; it is rescaled in the rare case that a row's reference moves.  Tiles that some row sees in part go through a slower way of 32 columns at a time in few
 // instructions.  Results leave through shared memory, a row a copy.
 // Where some row does not see some key of a tile its weight is 0, and 0 times a value that is not finite would be no number: the warp that copies values looks at such tiles and takes those values out, and the rows that see their
-// keys add them to their results at the end (add_odd; reached by values that are not finite alone).  Looking costs 1 % where every other tile is one (a prompt of 2048 of 64 channels 81.3 -> 81.9 us, with 128 none: it is done
-// two tiles ahead).
+// keys add them to their results at the end (add_odd; reached by values that are not finite alone).  Looking takes 0.4 us a tile, which nothing waits for unless most of a block's tiles are of that kind (27 rows over windows' edges, four
+// tiles a block, 21.4 -> 24.1 us).  Both functions stay out of line, and the copies' loop rolled: inline 91 us for 82 where up to 128 rows are taken by both groups, unrolled 715 for 710 in the case below.
 // Bound: a tile's way through its roles.  256 rows and 128 keys of 128 channels take about 3700 cycles: the products 2048 by the tensor cores' rate (about 2560 as they are, 80 cycles for 64), softmax 1680 to 1800 for a group and
-// 110 of hand-over.  16 sequences of up to 300 tokens behind 12000 positions, 32 heads over 8: 722 us where the products alone would be 378 (0.44 of the tensor pipes, 0.47 of the special functions'); its loads alone took 570 us
+// 110 of hand-over.  16 sequences of up to 300 tokens behind 12000 positions, 32 heads over 8: 711 us where the products alone would be 378 (0.45 of the tensor pipes, 0.47 of the special functions'); its loads alone took 570 us
 // from pages of 16 keys, 459 of 32, 416 of 64, 795 of 8.  Tried: tiles of 64 keys with scores ahead 1330 us (N = 64 costs what N = 128 does), weights handed over in halves 905 to 1134, a polynomial for part of the exponentials
-// 1085 against 973, a product thread a group 977 to 1017.
+// 1085 against 973, a product thread a group 977 to 1017, copying warps with code of their own 820.
 constexpr int AW_KEYS = 128, AW_THREADS = 384, AW_MASKS = 8;
 constexpr int AW_SOFTMAX_REGS = 176, AW_OTHER_REGS = 144; // 256 x 176 + 128 x 144 = 63488 of the 384 x 168 = 64512 that the block is launched with
 
@@ -838,7 +838,7 @@ __device__ __forceinline__ bool task_of(const C16& c, const Attend& a, int t, in
 
 // A tile of values: zeros for those of keys that are not there (`word`: keys 32 lane .. that are, for the first four lanes) and for what is not finite.  True: there was some of that.  A warp.
 template <typename T, int PANELS>
-__device__ __forceinline__ bool clear_values(unsigned char* tile, bool there, uint32_t word) {
+__device__ __noinline__ bool clear_values(unsigned char* tile, bool there, uint32_t word) {
 	const int lane = threadIdx.x & 31;
 	if (!there) {
 		for (int k = 0; k < AW_KEYS; ++k)
@@ -846,13 +846,13 @@ __device__ __forceinline__ bool clear_values(unsigned char* tile, bool there, ui
 		__syncwarp();
 	}
 	uint4* const all = reinterpret_cast<uint4*>(tile) + lane;
-	uint32_t sum = 0;
+	uint32_t sums[4] = {0, 0, 0, 0};
 #pragma unroll 8
 	for (int e = 0; e < AW_KEYS * 8 * PANELS; e += 32) {
 		const uint4 x = all[e];
-		odd2<T>(x.x, sum), odd2<T>(x.y, sum), odd2<T>(x.z, sum), odd2<T>(x.w, sum);
+		odd2<T>(x.x, sums[0]), odd2<T>(x.y, sums[1]), odd2<T>(x.z, sums[2]), odd2<T>(x.w, sums[3]);
 	}
-	const bool found = __any_sync(0xffffffffu, sum & 0x7fff7fff);
+	const bool found = __any_sync(0xffffffffu, (sums[0] | sums[1] | sums[2] | sums[3]) & 0x7fff7fff);
 	if (found)
 		for (int e = 0; e < AW_KEYS * 8 * PANELS; e += 32) {
 			uint32_t up, down;
@@ -893,7 +893,7 @@ __device__ __noinline__ void add_odd(const AwOdd& o, int from, int to, int dim, 
 	}
 }
 
-// CAP: soft caps, which all tiles take the slower way for.  (One kernel for both: 731 us for 719 without a cap, 16 sequences of up to 300 tokens behind 12000.)
+// CAP: soft caps, which all tiles take the slower way for.  (One kernel for both: 731 us for 713 without a cap, 16 sequences of up to 300 tokens behind 12000.)
 template <typename T, int D, bool CAP>
 __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const C16 c, const Attend a, const Wide w) {
 	typedef AwShared<D> Shared;
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 	// (the values' copies look at what some row does not see)
 	const int waiting = alone ? 0 : ranged ? AW_THREADS - 32 : AW_THREADS;
 	if (warp == 8 || warp == 11) {
-		if (waiting && (warp == 11 || !ranged)) asm volatile("bar.sync 2, %0;" ::"r"(waiting) : "memory");
+		if (!ranged) asm volatile("bar.sync 2, %0;" ::"r"(waiting) : "memory");
 		range(ranged ? low : s.span[0], ranged ? high : s.span[1]);
 	} else {
 		for (int b = u.first + (warp < 8 ? tid : tid - 32); b <= u.last; b += AW_THREADS - 64) {
@@ -1193,8 +1193,14 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 			};
 			uint32_t fixes = 0;
 			int issued = 0; // tiles asked for
-			const int seen_by_all = alone ? low : s.span[0], wide = low_of(a, alone ? high : s.span[1]); // (of the values' warp)
 			if (tiles > 0) look(0);
+			if (values && ranged && waiting) asm volatile("bar.sync 2, %0;" ::"r"(waiting) : "memory");
+			const int seen_by_all = alone ? low : s.span[0], wide = low_of(a, alone ? high : s.span[1]); // (of the values' warp)
+			if (values && lane == 0) { // for the rows that see values which are taken out
+				AwOdd& o = s.odd;
+				o.c = c, o.kvh = kvh, o.box = w.box, o.slot[0] = lead_slot, o.slot[1] = own_slot, o.first = count[0], o.begin = begin, o.tiles = tiles, o.wide = wide, o.least = seen_by_all;
+				o.lo[0] = lo[0], o.lo[1] = lo[1], o.hi[0] = hi[0], o.hi[1] = hi[1], o.base[0] = base[0], o.base[1] = base[1];
+			}
 			for (int i = 0; i < tiles; ++i) {
 				int part;
 				const int pos0 = start(i, part), l0 = (part ? lo[1] : lo[0]) - pos0, h0 = (part ? hi[1] : hi[0]) - pos0;
@@ -1220,6 +1226,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 				uint64_t* const bar = whole ? s.full + sl : &s.fix;
 				if (lane == 0) mbar_expect_tx(bar, PANELS * AW_KEYS * 128);
 				unsigned char* to = s.kv[sl][0];
+#pragma unroll 1
 				for (int x = 0; x < boxes; ++x, to += w.box * 128) {
 					const int r = __shfl_sync(0xffffffffu, row, x);
 					if (lane == 0) {
@@ -1232,11 +1239,7 @@ __global__ void __launch_bounds__(AW_THREADS, 1) k_c16_tiles(const __grid_consta
 					if (!ap_wait_warp(&s.fix, fixes & 1, &s.lost)) break;
 					++fixes;
 					if (clear_values<T, PANELS>(s.kv[sl][0], there, word)) {
-						if (lane == 0) {
-							AwOdd& o = s.odd;
-							o.found = 1, o.c = c, o.kvh = kvh, o.box = w.box, o.slot[0] = lead_slot, o.slot[1] = own_slot, o.first = count[0], o.begin = begin, o.tiles = tiles, o.wide = wide, o.least = seen_by_all;
-							o.lo[0] = lo[0], o.lo[1] = lo[1], o.hi[0] = hi[0], o.hi[1] = hi[1], o.base[0] = base[0], o.base[1] = base[1];
-						}
+						if (lane == 0) s.odd.found = 1;
 					}
 					fence_async_smem();
 					__syncwarp();
