@@ -176,7 +176,7 @@ __device__ __forceinline__ void add_places(float4& v, const float* p, size_t str
 		}
 	}
 }
-// Soft caps: cap tanh(s / cap), off by 10 2^-24 of the score at most, whatever the cap.  For |u| = |s / cap| <= 1 it is s times the fifth convergent of tanh(u) / u = 1 / (1 + u^2 / (3 + u^2 / (5 + ...))), Lambert's
+// Soft caps: cap tanh(s / cap), off by 12 2^-24 of the score at most, whatever the cap.  For |u| = |s / cap| <= 1 it is s times the fifth convergent of tanh(u) / u = 1 / (1 + u^2 / (3 + u^2 / (5 + ...))), Lambert's
 // continued fraction, (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4): off by 2^-24, with the roundings of two quotients' parts, a reciprocal and three products.  Else cap (1 - t) / (1 + t) with t = e^(-2 |u|), where 1 - t
 // is 0.86 or more.  (That form alone is off by 2^-21 of the cap: at a cap of 10^6 no score is left.)
 struct Cap {
@@ -1438,7 +1438,7 @@ void groups_plan(A16Plan& r, const SeqCache16& c, const SeqShared& s, long long 
 // Sequences: whole tasks, but for those that a last round of fewer CTAs than run at a time would have.
 void tasks_plan(A16Plan& r, const SeqCache16& c, const SeqPortions& p, const SeqAttend16& a, long long rows, long long most) {
 	r.wide.box = a16_box(c.page), r.wide.tiles = cdiv(rows, 256), r.wide.through = 1, r.wide_units = 1;
-	// As many tasks as there can be, whatever the counts become: no more tiles than the rows fill and one begun for every sequence.  (A prompt of 8192 tokens among 255 single ones behind 2000 positions 1234 us; with as many
+	// As many tasks as there can be, whatever the counts become: no more tiles than the rows fill and one begun for every sequence.  (A prompt of 8192 tokens among 255 single ones behind 2000 positions 1243 us; with as many
 	// blocks for each as the prompt has tiles 3318.)
 	const long long all = std::min((long long)p.n * r.wide.tiles, (long long)a.q.rows * (a.heads / c.heads) / 256 + p.n) * c.heads, live = a.row_tiles > 0 ? std::min(all, std::max(0LL, a.row_tiles - (r.apart ? a.few : 0)) * c.heads) : all, rest = live % AW_ROOM;
 	const int longest = std::max(1, (int)std::min<long long>(cdiv(most, AW_KEYS), INT_MAX / 2));
@@ -1472,8 +1472,8 @@ A16Plan a16_plan(const SeqCache16& c, const SeqPortions& p, const SeqShared* s, 
 	const double us_prefixes = 20. + us_tile * groups * c.heads * cdiv(likely, 256) * prefix + cdiv((long long)p.n * c.heads * cdiv(rows, 16), AR_ROOM) * (4. + std::max(own, lone) / 130.);
 	const double us_row = us_tile * c.heads * (groups ? prefix + own : lone), us_all = 24. + us_row * (double)(a.row_tiles > 0 ? a.row_tiles : (long long)p.n * cdiv(rows, 256));
 	// Single tokens among prompts are a tile each, of which their rows are a small part: they go apart, in CTAs of few rows beside the tiles' last ones.  us, together / apart, 32 heads over 8 of
-	// 128 channels: a prompt of 8192 among 255 tokens behind 2000 positions 1239 / 924 (602 and 293 by themselves), of 2048 among 63 264 / 158, of 512 among 31 132 / 85, 8 of 600 among 120 480 / 389, 2 of 900 with 20 that share 1500
-	// 157 / 125, one of 500 among 16 behind 20000 391 / 303, one of 300 among 5 42 / 42 (taken together).
+	// 128 channels: a prompt of 8192 among 255 tokens behind 2000 positions 1243 / 917 (594 and 293 by themselves), of 2048 among 63 262 / 158, of 512 among 31 133 / 86, 8 of 600 among 120 479 / 388, 2 of 900 with 20 that share 1500
+	// 154 / 123, one of 500 among 16 behind 20000 395 / 306, one of 300 among 5 42 / 42 (taken together).
 	const double us_apart = us_all - us_row * a.few + cdiv((long long)a.few * c.heads, AR_ROOM) * (4. + std::max(shared + own, lone) / 130.);
 	const bool apart = a.few > 0 && a.row_tiles > a.few && us_apart < us_all;
 	const double us_tiles = apart ? us_apart : us_all;

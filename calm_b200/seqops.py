@@ -1,9 +1,9 @@
 """Operators of the layer-list library on the caller's own GPU tensors (include/calm_b200_seq.h, second half): the n best continuations of beams, copies of
 cache pages and state slots, caches of keys and values in 8 and in 16 bits and attention over them, prefixes that sequences share, rotary positions.  The serving runtime (seqlib.SeqDeviceModel, serving.Scheduler) runs
-on the same kernels.
+on the kernels of the beams, the copies and the 8-bit cache; rotary positions, the 16-bit cache and shared prefixes are for callers with a loop of their own.
 
 Calls run on torch's current stream of the tensors' device, return before the work is done and can be captured into CUDA graphs.  What a call refuses raises
-ValueError before anything is launched.  Like everywhere in this package there is no CPU path."""
+ValueError before anything is launched.  None has a gradient: results require none, whatever the inputs do.  Like everywhere in this package there is no CPU path."""
 from __future__ import annotations
 
 import ctypes as C
@@ -408,7 +408,7 @@ class Cache8:
 
 class Rotation:
     """How positions turn the channels of a head: the first `dims` of them, in pairs of "halves" (i, i + dims / 2) or "neighbours" (2i, 2i + 1), pair i by position * f_i with
-    f_i = base^(-2 i / dims).  `scaling` stretches f for contexts longer than a model was trained on:
+    f_i = base^(-2 i / dims).  Angles are exact to 3 2^-53 of themselves and 2^-23 of a radian.  `scaling` stretches f for contexts longer than a model was trained on:
       {"kind": "linear", "factor"}                          f / factor
       {"kind": "base", "factor"}                            the base times factor^(dims / (dims - 2))
       {"kind": "wavelength", "factor", "length", "low", "high"}  w = length f / 2 pi: f / factor below `low`, f above `high`, a blend linear in w between

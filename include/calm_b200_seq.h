@@ -332,7 +332,8 @@ void calm_b200_seq_set_perf(void* handle, int on);
 int calm_b200_seq_perf_stats(void* handle, int kind, char* name, int name_cap, double* ms_total, double* bytes_total, double* flops_total, long* launches);
 
 /* ---- operators on the caller's device memory -----------------------------------------------------------------------------------
- * What continuing one text in several sequences needs, for callers with buffers of their own; the runtime above runs on the same kernels.
+ * What continuing one text in several sequences needs, for callers with buffers of their own; the runtime above runs on the kernels of the
+ * beams, the copies and the 8-bit cache.
  * Every call launches on `stream` (a cudaStream_t of the current device, NULL: the default one), returns before the work is done, allocates nothing and can
  * be captured into a CUDA graph.  Returns 0; -3 when an argument is refused, -4 when CUDA reports an error (nothing has been launched then that the call's
  * own kernels have not finished with): calm_b200_seq_error() says why, per host thread.  Calls from several host threads do not disturb each other as long as
@@ -485,7 +486,7 @@ struct SeqAttend16 {
 	int heads;               /* query heads, a multiple of cache.heads */
 	float scale;
 	int window;
-	float softcap;           /* > 0: s = softcap tanh(s / softcap) after the scale */
+	float softcap;           /* > 0: s = softcap tanh(s / softcap) after the scale, to 12 2^-24 of s whatever the cap */
 	const float* sinks;      /* [heads] or NULL */
 	int most_keys;           /* at least the keys that any token sees (what the split of the work is planned for; more are still seen) */
 	long long row_tiles;     /* about the sum over the sequences of ceil(tokens * (heads / cache.heads) / 256) (what the split of the work is planned for); 0: as many as there can be */
