@@ -479,7 +479,7 @@ struct SeqShared {
  *   s_j = softcap(scale q . k_j);  out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h]))
  * A prefix that a group shares is read once for all of the group's tokens (or, where a sequence brings many, once for 128 or 256 of its rows).  Scores, softmax and sums are fp32; softmax weights enter the tensor cores in the cache's
  * type.  Positions whose slot, table entry or page number is outside the cache are not seen; what they, positions behind a token or outside its window hold does not reach its result.  A value that is not finite
- * reaches the tokens that see it, whatever its weight (as no number where a weight that rounds to nothing is multiplied with it).  A token that sees nothing gets zeros.  Rows that belong to no sequence are left alone.
+ * reaches the tokens that see it and no others; where its weight rounds to nothing an infinity may become no number, and under 2^-126 of the others' weights it may be left out.  A token that sees nothing gets zeros.  Rows that belong to no sequence are left alone.
  * Weights of up to 2^15 are summed before the sums are divided: bfloat16 values past 2^112 over the number of keys may become infinities. */
 struct SeqAttend16 {
 	struct SeqRows q, out;   /* of the cache's type */
